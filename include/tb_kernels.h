@@ -252,6 +252,114 @@ int tb_obs_sparsegpt(float* W, int r, int d, const float* H, float damp_frac, in
  * its last in-block step, [3] all three.  Writes min(n, 4) values. */
 int tb_obs_sparsegpt_phase_times(float* ms_out, int n);
 
+/* ---- calibration from 8-bit activation checkpoints ------------------------ */
+/* The two inputs of pruning, gradient samples (Fisher) and X^T X (exact OBS),
+ * from activations that a calibration pass kept in 8 bits.  No reference
+ * counterpart: the reference takes gradients from its caller
+ * (ehap.hpp:148-201) and has no activation Hessian (docs/EHAP.md:248-250).
+ *
+ * A checkpoint of X [n][d] is one int8 code q per value and one exponent byte
+ * E per feature and block of TB_ACT8_BLOCK consecutive tokens.  It stands for
+ *     xhat = q * 2^(E - 127)
+ * where E is the smallest value >= 1 for which every code of the block rounds
+ * into [-127, 127] (q = x * 2^(127-E), ties to even).  The scale belongs to a
+ * feature because calibration activations have heavy columns.  xhat has 7
+ * significant bits, so it is exact in BF16, and every product formed from a
+ * checkpoint below is the exact product of xhat.  A NaN or an infinity in a
+ * block's kept tokens sets E = 255: the whole block of that feature reads
+ * back as NaN. */
+#define TB_ACT8_BLOCK 128
+typedef struct tb_act8 {
+    uint32_t struct_size;  /* sizeof(tb_act8)                                          */
+    int32_t  d;            /* features                                                 */
+    int64_t  n;            /* tokens, below 2^31 - 64                                  */
+    int8_t*  codes;        /* [n][ldq], device, 16-byte aligned                        */
+    int64_t  ldq;          /* >= d, a multiple of 16                                   */
+    uint8_t* exps;         /* [ceil(n / TB_ACT8_BLOCK)][lde], device, 16-byte aligned  */
+    int64_t  lde;          /* >= d, a multiple of 16                                   */
+} tb_act8;
+/* Packs X [n][ldx] (dtype TB_F32 / TB_F16 / TB_BF16; F16 as IEEE, subnormals
+ * included) into ck.  keep: n bytes or NULL; a token whose byte is 0 (padding)
+ * is stored as zeros and does not enter the scales, whatever its values.
+ * Columns d..ldq-1 and d..lde-1 are left as they were.  n = 0 does nothing. */
+int tb_act8_pack(const tb_act8* ck, const void* x, int dtype, int64_t ldx, const uint8_t* keep, void* stream);
+/* xhat as [n][ldo] of dtype (exact in TB_F32 and TB_BF16, rounded in TB_F16). */
+int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* stream);
+/* Weight gradients of y = W x from the checkpoint of x: for each sample s
+ *     G_s [r][d] = sum over its tokens t of dy_t xhat_t^T
+ * written as g_dtype (TB_F32 or TB_BF16) at grads + s * g_stride (elements; 0
+ * means r * d): the gradient samples that tb_score_mask_pack and
+ * tb_fisher_ema_step read.  TB_F16 is TB_ERR_UNSUPPORTED: the passes that read
+ * F16 gradients decode subnormals as the reference does, not as IEEE values.
+ * dy [n][lddy] is of dy_dtype.  samples: device array of S (begin, end) token
+ * pairs, clamped to [0, n], in any order, overlapping or not; NULL means one
+ * sample of all tokens (S = 1).  An empty sample's gradient is zero; tokens of
+ * no sample are not read into any.  Sums are in FP32 and every product is
+ * exact: FP32 (F16) dy is split into three (two) BF16 parts, in scratch of
+ * 6 (4) bytes per value from the library's per-device pool; rows of a BF16 dy
+ * that are not 16-byte aligned are first copied to such scratch. */
+int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
+                        const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride, void* stream);
+/* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
+ * 148-201) per sample, in their order, without the gradients in memory: with
+ * G_s as above in FP32, the first step (first_step != 0, F not read) gives
+ * F = (alpha g) g, the others F = beta F + ((alpha (1 - beta)) g) g.  fisher
+ * is [r][d].  A sample without tokens is a step with g = 0. */
+int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r, const int64_t* samples,
+                   int S, float alpha, float beta, int first_step, float* fisher, void* stream);
+/* H = scale * Xhat^T Xhat (accumulate != 0: added to H): tb_obs_hessian_scaled
+ * from a checkpoint, for any d and n.  H is [d][d]; only the 128x128 tiles on
+ * or below the diagonal are written.  n = 0 gives zeros (accumulate: H stays). */
+int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, void* stream);
+
+/* ---- low-rank adapters beside a shared projection ------------------------- */
+/* A projection W shared by many requests, each with a low-rank adapter or
+ * none: token t of adapter a = token_adapter[t] sees W + scale[a] B_a A_a.
+ * The calibration of such a projection runs its forward with the adapters in
+ * place and its backward from the 8-bit checkpoint of x.  No reference
+ * counterpart.  BF16 operands, FP32 sums; A x and B^T dy stay in FP32 and
+ * enter the second product as two BF16 parts (a relative 2^-17). */
+typedef struct tb_adapter_args {
+    uint32_t struct_size;  /* sizeof(tb_adapter_args)                                    */
+    int32_t  dtype;        /* of w, a, b, x, y, dy, dx, da, db: TB_BF16                  */
+    int64_t  n;            /* tokens, below 2^31 - 256                                   */
+    int32_t  d, r;         /* in and out features                                        */
+    int32_t  rank;         /* 1..128                                                     */
+    int32_t  n_adapters;   /* 0: the projection alone                                    */
+    const void* w;         /* [r][ldw]                                                   */
+    int64_t  ldw;
+    const void* a;         /* [n_adapters * rank][lda]                                   */
+    int64_t  lda;
+    const void* b;         /* [n_adapters * r][ldb]                                      */
+    int64_t  ldb;
+    const float*   scale;          /* [n_adapters], device                               */
+    const int32_t* token_adapter;  /* [n], device; outside [0, n_adapters) = no adapter  */
+    /* forward */
+    const void* x;         /* [n][ldx]                                                   */
+    int64_t  ldx;
+    void*    y;            /* [n][ldy]                                                   */
+    int64_t  ldy;
+    /* backward */
+    const void* dy;        /* [n][lddy]                                                  */
+    int64_t  lddy;
+    const tb_act8* x8;     /* checkpoint of x (host struct)                              */
+    void*    dx;           /* [n][lddx], or NULL                                         */
+    int64_t  lddx;
+    void*    da;           /* laid out as a, or NULL (da and db are given together)      */
+    void*    db;           /* laid out as b, or NULL                                     */
+} tb_adapter_args;
+/* y_t = W x_t + scale[a] B_a (A_a x_t).  All inputs 16-byte aligned with row
+ * strides that are multiples of 8; outputs may have any stride.  Columns
+ * behind the last one (d..lda-1 and so on) are neither used nor written.
+ * Scratch: 4 bytes per token and rank, from the library's per-device pool. */
+int tb_adapter_forward(const tb_adapter_args* args, void* stream);
+/* With v_t = scale[a] B_a^T dy_t and u_t = scale[a] A_a xhat_t:
+ *     dx_t = W^T dy_t + A_a^T v_t,   da_a = sum v_t xhat_t^T,   db_a = sum dy_t u_t^T
+ * over the tokens of adapter a (zero where it has none).  da and db do not
+ * depend on the order in which blocks run: their sums have a fixed order.
+ * With dx NULL, w may be NULL; with da and db NULL, x8 may be NULL. */
+int tb_adapter_backward(const tb_adapter_args* args, void* stream);
+
 /* ---- fused score -> mask -> pack pass ------------------------------------ */
 /* One pass over a tensor: Fisher EMA over S gradient samples, importance,
  * CORING N:M mask, apply, redistribution, and emission of the .tb weight and

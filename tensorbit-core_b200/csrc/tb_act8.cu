@@ -1,0 +1,336 @@
+// 8-bit activation checkpoints and what a calibration pass makes of them:
+// packing, reading back, weight gradients per sample, the Fisher EMA of those
+// gradients, and X^T X for exact OBS (contract in include/tb_kernels.h).
+#include <algorithm>
+
+#include "tb_act8.cuh"
+#include "tb_device.cuh"
+#include "tb_runtime.h"
+#include "tb_simple_gemm.cuh"
+
+namespace tb {
+namespace act8 {
+
+int check(const tb_act8* ck, const char* who, View* v) {
+    if (!ck || ck->struct_size != sizeof(tb_act8)) return fail(TB_ERR_ARG, "%s: null checkpoint or bad struct_size", who);
+    if (ck->d <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: a checkpoint has at least one feature", who);
+    if (ck->n < 0 || ck->n > 0x7FFFFFFFll - 64) return fail(TB_ERR_SHAPE, "%s: %lld tokens", who, static_cast<long long>(ck->n));
+    if (ck->ldq < ck->d || ck->ldq % 16 || ck->lde < ck->d || ck->lde % 16)
+        return fail(TB_ERR_ARG, "%s: ldq and lde must be multiples of 16 and at least d", who);
+    if (ck->n > 0 && (!ck->codes || !ck->exps || reinterpret_cast<uintptr_t>(ck->codes) % 16 ||
+                      reinterpret_cast<uintptr_t>(ck->exps) % 16))
+        return fail(TB_ERR_ARG, "%s: codes and exps must be non-null and 16-byte aligned", who);
+    *v = {ck->codes, ck->exps, ck->ldq, ck->lde, ck->n, ck->d};
+    return TB_OK;
+}
+
+namespace {
+
+// One block of 256 threads holds 128 tokens x 128 features in registers, so X
+// is read once: thread (row, col) has 8 consecutive features of 8 tokens.
+constexpr int kFeat = 128, kRowsPass = 16, kPasses = kBlock / kRowsPass;
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* x, long long at, int valid, float (&v)[8]) {
+    using E = Elem<DT>;
+    if (VEC && valid >= 8) {
+        if constexpr (DT == TB_F32) {
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+            const float4 lo = p[0], hi = p[1];
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+        } else {
+            const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DT == TB_BF16) {
+                    v[2 * i] = __uint_as_float(w[i] << 16);
+                    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                } else {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    v[2 * i] = f.x;
+                    v[2 * i + 1] = f.y;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? E::load(x, at + i) : 0.0f;
+    }
+}
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const View ck, const void* __restrict__ x, const long long ldx,
+                                                   const uint8_t* __restrict__ keep) {
+    __shared__ uint32_t smax[kRowsPass][kFeat];
+    const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+    const int f0 = blockIdx.x * kFeat + col * 8;
+    const int valid = ck.d - f0;  // features of this thread (may be <= 0 or > 8)
+    const long long t0 = static_cast<long long>(blockIdx.y) * kBlock;
+    float v[kPasses][8];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const long long t = t0 + p * kRowsPass + row;
+        if (t < ck.n && valid > 0 && (!keep || keep[t])) load8<DT, VEC>(x, t * ldx + f0, valid, v[p]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) m = max(m, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
+        smax[row][col * 8 + i] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x < kFeat) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int r = 0; r < kRowsPass; ++r) m = max(m, smax[r][threadIdx.x]);
+        const uint32_t e = exponent_of(m);
+        smax[0][threadIdx.x] = e;
+        const int f = blockIdx.x * kFeat + threadIdx.x;
+        if (f < ck.d) ck.exps[blockIdx.y * ck.lde + f] = static_cast<uint8_t>(e);
+    }
+    __syncthreads();
+    if (valid <= 0) return;
+    uint32_t e[8];
+    float inv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        e[i] = smax[0][col * 8 + i];
+        inv[i] = e[i] == 255u ? 0.0f : inverse_scale(e[i]);
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const long long t = t0 + p * kRowsPass + row;
+        if (t >= ck.n) break;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int q = e[i] == 255u ? 0 : __float2int_rn(v[p][i] * inv[i]);
+            w[i >> 2] |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * (i & 3));
+        }
+        int8_t* out = ck.codes + t * ck.ldq + f0;
+        if (valid >= 8) {
+            *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+        } else {
+            for (int i = 0; i < valid; ++i) out[i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
+        }
+    }
+}
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) unpack_kernel(const View ck, void* __restrict__ out, const long long ldo) {
+    using T = typename Elem<DT>::T;
+    const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+    const int f0 = blockIdx.x * kFeat + col * 8;
+    const int valid = ck.d - f0;
+    if (valid <= 0) return;
+    const long long t0 = static_cast<long long>(blockIdx.y) * kBlock;
+    const uint2 ew = *reinterpret_cast<const uint2*>(ck.exps + blockIdx.y * ck.lde + f0);
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = scale_f32(((i < 4 ? ew.x : ew.y) >> (8 * (i & 3))) & 0xFFu);
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const long long t = t0 + p * kRowsPass + row;
+        if (t >= ck.n) break;
+        const uint2 w = *reinterpret_cast<const uint2*>(ck.codes + t * ck.ldq + f0);
+        T o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int q = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+            o[i] = Elem<DT>::to(static_cast<float>(q) * s[i]);
+        }
+        T* dst = static_cast<T*>(out) + t * ldo + f0;
+        if (VEC && valid >= 8) {
+            const uint4* src = reinterpret_cast<const uint4*>(o);
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = src[i];
+        } else {
+            for (int i = 0; i < 8 && i < valid; ++i) dst[i] = o[i];
+        }
+    }
+}
+
+__device__ __forceinline__ float xhat(const View& ck, long long t, long long f) {
+    return static_cast<float>(ck.codes[t * ck.ldq + f]) * scale_f32(ck.exps[(t / kBlock) * ck.lde + f]);
+}
+__device__ __forceinline__ float value(const void* p, int dt, long long i) {
+    return dt == TB_F32 ? Elem<TB_F32>::load(p, i) : dt == TB_F16 ? Elem<TB_F16>::load(p, i) : Elem<TB_BF16>::load(p, i);
+}
+
+struct GradOp {
+    static constexpr bool kRowA = false, kRowB = true;
+    View ck;
+    const void* dy;
+    int dy_dtype;
+    long long lddy, M, N;
+    const int64_t* samples;
+    int S;
+    void* grads;
+    int g_dtype;
+    long long g_stride;
+    float* fisher;  // EMA over the samples instead of gradients
+    float alpha, beta;
+    int first_step;
+    __device__ bool wanted(long long, long long) const { return true; }
+    __device__ int first_unit(int z) const { return fisher ? 0 : z; }
+    __device__ int last_unit(int z) const { return fisher ? S : z + 1; }
+    __device__ long long k_begin(int s) const { return samples ? max(0ll, static_cast<long long>(samples[2 * s])) : 0; }
+    __device__ long long k_end(int s) const { return samples ? min(ck.n, static_cast<long long>(samples[2 * s + 1])) : ck.n; }
+    __device__ float a(long long m, long long t) const { return value(dy, dy_dtype, t * lddy + m); }
+    __device__ float b(long long t, long long n) const { return xhat(ck, t, n); }
+    __device__ void store(int s, long long m, long long n, float g) const {
+        if (fisher) {
+            float* F = fisher + m * N + n;
+            *F = (s == 0 && first_step) ? ema_first(alpha, g) : ema_next(*F, beta, alpha * (1.0f - beta), g);
+        } else if (g_dtype == TB_F32) {
+            static_cast<float*>(grads)[s * g_stride + m * N + n] = g;
+        } else {
+            static_cast<__nv_bfloat16*>(grads)[s * g_stride + m * N + n] = __float2bfloat16_rn(g);
+        }
+    }
+};
+
+struct HessianOp {
+    static constexpr bool kRowA = false, kRowB = true;
+    View ck;
+    long long M, N;
+    float scale;
+    int accumulate;
+    float* H;
+    __device__ bool wanted(long long m0, long long n0) const { return m0 / 128 >= n0 / 128; }
+    __device__ int first_unit(int) const { return 0; }
+    __device__ int last_unit(int) const { return 1; }
+    __device__ long long k_begin(int) const { return 0; }
+    __device__ long long k_end(int) const { return ck.n; }
+    __device__ float a(long long m, long long t) const { return xhat(ck, t, m); }
+    __device__ float b(long long t, long long n) const { return xhat(ck, t, n); }
+    __device__ void store(int, long long m, long long n, float g) const {
+        float* h = H + m * N + n;
+        *h = accumulate ? *h + scale * g : scale * g;
+    }
+};
+
+bool vectors(const void* p, long long ld, int esize) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * esize) % 16 == 0;
+}
+
+int check_dy(const char* who, const void* dy, int dtype, int64_t lddy, int r, int64_t n, const int64_t* samples, int S) {
+    if (dtype < TB_F32 || dtype > TB_BF16) return fail(TB_ERR_ARG, "%s: bad dy dtype %d", who, dtype);
+    if (r <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: r must be positive", who);
+    if (S < 0 || S > 65535 || (!samples && S != 1))
+        return fail(TB_ERR_ARG, "%s: S must be in 0..65535, and 1 where samples is NULL", who);
+    if (n > 0 && S > 0 && (!dy || lddy < r)) return fail(TB_ERR_ARG, "%s: dy is null or lddy < r", who);
+    return TB_OK;
+}
+
+}  // namespace
+}  // namespace act8
+}  // namespace tb
+
+using namespace tb;
+using namespace tb::act8;
+
+extern "C" int tb_act8_pack(const tb_act8* ckp, const void* x, int dtype, int64_t ldx, const uint8_t* keep,
+                            void* stream) {
+    View ck;
+    int rc = act8::check(ckp, "tb_act8_pack", &ck);
+    if (rc) return rc;
+    if (dtype < TB_F32 || dtype > TB_BF16) return fail(TB_ERR_ARG, "tb_act8_pack: bad dtype %d", dtype);
+    if (ck.n == 0) return TB_OK;
+    if (!x || ldx < ck.d) return fail(TB_ERR_ARG, "tb_act8_pack: x is null or ldx < d");
+    if ((rc = require_device(nullptr))) return rc;
+    const long long blocks = (ck.n + kBlock - 1) / kBlock;
+    auto st = static_cast<cudaStream_t>(stream);
+    // The grid's y extent ends at 65535 blocks of tokens: longer checkpoints take several launches.
+    for (long long b0 = 0; b0 < blocks; b0 += 65535) {
+        const long long nb = std::min(blocks - b0, 65535ll), t0 = b0 * kBlock;
+        const View v{ck.codes + t0 * ck.ldq, ck.exps + b0 * ck.lde, ck.ldq, ck.lde, ck.n - t0, ck.d};
+        const dim3 grid((ck.d + kFeat - 1) / kFeat, static_cast<unsigned>(nb));
+        const void* xp = static_cast<const char*>(x) + t0 * ldx * (dtype == TB_F32 ? 4 : 2);
+        const uint8_t* kp = keep ? keep + t0 : nullptr;
+        const bool vec = vectors(x, ldx, dtype == TB_F32 ? 4 : 2);
+        switch (dtype) {
+        case TB_F32: vec ? pack_kernel<TB_F32, true><<<grid, 256, 0, st>>>(v, xp, ldx, kp) : pack_kernel<TB_F32, false><<<grid, 256, 0, st>>>(v, xp, ldx, kp); break;
+        case TB_F16: vec ? pack_kernel<TB_F16, true><<<grid, 256, 0, st>>>(v, xp, ldx, kp) : pack_kernel<TB_F16, false><<<grid, 256, 0, st>>>(v, xp, ldx, kp); break;
+        default: vec ? pack_kernel<TB_BF16, true><<<grid, 256, 0, st>>>(v, xp, ldx, kp) : pack_kernel<TB_BF16, false><<<grid, 256, 0, st>>>(v, xp, ldx, kp); break;
+        }
+    }
+    return check_launch("pack_kernel");
+}
+
+extern "C" int tb_act8_unpack(const tb_act8* ckp, void* out, int dtype, int64_t ldo, void* stream) {
+    View ck;
+    int rc = act8::check(ckp, "tb_act8_unpack", &ck);
+    if (rc) return rc;
+    if (dtype < TB_F32 || dtype > TB_BF16) return fail(TB_ERR_ARG, "tb_act8_unpack: bad dtype %d", dtype);
+    if (ck.n == 0) return TB_OK;
+    if (!out || ldo < ck.d) return fail(TB_ERR_ARG, "tb_act8_unpack: out is null or ldo < d");
+    if ((rc = require_device(nullptr))) return rc;
+    const long long blocks = (ck.n + kBlock - 1) / kBlock;
+    auto st = static_cast<cudaStream_t>(stream);
+    for (long long b0 = 0; b0 < blocks; b0 += 65535) {
+        const long long nb = std::min(blocks - b0, 65535ll), t0 = b0 * kBlock;
+        const View v{ck.codes + t0 * ck.ldq, ck.exps + b0 * ck.lde, ck.ldq, ck.lde, ck.n - t0, ck.d};
+        const dim3 grid((ck.d + kFeat - 1) / kFeat, static_cast<unsigned>(nb));
+        void* op = static_cast<char*>(out) + t0 * ldo * (dtype == TB_F32 ? 4 : 2);
+        const bool vec = vectors(out, ldo, dtype == TB_F32 ? 4 : 2);
+        switch (dtype) {
+        case TB_F32: vec ? unpack_kernel<TB_F32, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F32, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        case TB_F16: vec ? unpack_kernel<TB_F16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        default: vec ? unpack_kernel<TB_BF16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_BF16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        }
+    }
+    return check_launch("unpack_kernel");
+}
+
+extern "C" int tb_act8_weight_grad(const tb_act8* ckp, const void* dy, int dy_dtype, int64_t lddy, int r,
+                                   const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride,
+                                   void* stream) {
+    View ck;
+    int rc = act8::check(ckp, "tb_act8_weight_grad", &ck);
+    if (!rc) rc = check_dy("tb_act8_weight_grad", dy, dy_dtype, lddy, r, ck.n, samples, S);
+    if (rc) return rc;
+    const long long rd = static_cast<long long>(r) * ck.d;
+    if (g_dtype == TB_F16) return fail(TB_ERR_UNSUPPORTED, "tb_act8_weight_grad: gradients are TB_F32 or TB_BF16");
+    if (g_dtype != TB_F32 && g_dtype != TB_BF16) return fail(TB_ERR_ARG, "tb_act8_weight_grad: bad gradient dtype %d", g_dtype);
+    if (g_stride == 0) g_stride = rd;
+    if (g_stride < rd) return fail(TB_ERR_SHAPE, "tb_act8_weight_grad: g_stride below r * d");
+    if (S == 0) return TB_OK;
+    if (!grads) return fail(TB_ERR_ARG, "tb_act8_weight_grad: null gradients");
+    if ((rc = require_device(nullptr))) return rc;
+    GradOp op{ck, dy, dy_dtype, lddy, r, ck.d, samples, S, grads, g_dtype, g_stride, nullptr, 0.0f, 0.0f, 0};
+    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (r + 63) / 64, S), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
+    return check_launch("act8 weight gradient");
+}
+
+extern "C" int tb_act8_fisher(const tb_act8* ckp, const void* dy, int dy_dtype, int64_t lddy, int r,
+                              const int64_t* samples, int S, float alpha, float beta, int first_step, float* fisher,
+                              void* stream) {
+    View ck;
+    int rc = act8::check(ckp, "tb_act8_fisher", &ck);
+    if (!rc) rc = check_dy("tb_act8_fisher", dy, dy_dtype, lddy, r, ck.n, samples, S);
+    if (rc) return rc;
+    if (S == 0) return TB_OK;
+    if (!fisher) return fail(TB_ERR_ARG, "tb_act8_fisher: null Fisher state");
+    if ((rc = require_device(nullptr))) return rc;
+    GradOp op{ck, dy, dy_dtype, lddy, r, ck.d, samples, S, nullptr, TB_F32, 0, fisher, alpha, beta, first_step};
+    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (r + 63) / 64, 1), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
+    return check_launch("act8 Fisher");
+}
+
+extern "C" int tb_act8_hessian(const tb_act8* ckp, float scale, int accumulate, float* H, void* stream) {
+    View ck;
+    int rc = act8::check(ckp, "tb_act8_hessian", &ck);
+    if (rc) return rc;
+    if (!H) return fail(TB_ERR_ARG, "tb_act8_hessian: null H");
+    if ((rc = require_device(nullptr))) return rc;
+    HessianOp op{ck, ck.d, ck.d, scale, accumulate, H};
+    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (ck.d + 63) / 64, 1), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
+    return check_launch("act8 Hessian");
+}

@@ -66,6 +66,49 @@ class PruneArgs(C.Structure):
     ]
 
 
+class Act8(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("d", C.c_int32),
+        ("n", C.c_int64),
+        ("codes", C.c_void_p),
+        ("ldq", C.c_int64),
+        ("exps", C.c_void_p),
+        ("lde", C.c_int64),
+    ]
+
+
+class AdapterArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("n", C.c_int64),
+        ("d", C.c_int32),
+        ("r", C.c_int32),
+        ("rank", C.c_int32),
+        ("n_adapters", C.c_int32),
+        ("w", C.c_void_p),
+        ("ldw", C.c_int64),
+        ("a", C.c_void_p),
+        ("lda", C.c_int64),
+        ("b", C.c_void_p),
+        ("ldb", C.c_int64),
+        ("scale", C.c_void_p),
+        ("token_adapter", C.c_void_p),
+        ("x", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("y", C.c_void_p),
+        ("ldy", C.c_int64),
+        ("dy", C.c_void_p),
+        ("lddy", C.c_int64),
+        ("x8", C.POINTER(Act8)),
+        ("dx", C.c_void_p),
+        ("lddx", C.c_int64),
+        ("da", C.c_void_p),
+        ("db", C.c_void_p),
+    ]
+
+
 def header_symbols() -> list[str]:
     """Names of every function declared in include/tb_kernels.h."""
     txt = open(HEADER).read()
@@ -83,7 +126,7 @@ def lib() -> C.CDLL:
             raise FileNotFoundError(
                 f"{LIB_PATH} is not built; run `python tensorbit-core_b200/build.py` (needs nvcc)")
         L = C.CDLL(LIB_PATH)
-        vp, sz, i32, f32 = C.c_void_p, C.c_size_t, C.c_int, C.c_float
+        vp, sz, i32, i64, f32 = C.c_void_p, C.c_size_t, C.c_int, C.c_int64, C.c_float
         sig = {
             "tb_abi_version": ([], i32),
             "tb_last_error": ([], C.c_char_p),
@@ -132,6 +175,13 @@ def lib() -> C.CDLL:
             "tb_obs_hessian_scaled": ([vp, i32, i32, f32, vp, vp], i32),
             "tb_obs_sparsegpt": ([vp, i32, i32, vp, f32, i32, i32, vp, vp, vp], i32),
             "tb_obs_sparsegpt_phase_times": ([C.POINTER(C.c_float), i32], i32),
+            "tb_act8_pack": ([C.POINTER(Act8), vp, i32, i64, vp, vp], i32),
+            "tb_act8_unpack": ([C.POINTER(Act8), vp, i32, i64, vp], i32),
+            "tb_act8_weight_grad": ([C.POINTER(Act8), vp, i32, i64, i32, vp, i32, vp, i32, i64, vp], i32),
+            "tb_act8_fisher": ([C.POINTER(Act8), vp, i32, i64, i32, vp, i32, f32, f32, i32, vp, vp], i32),
+            "tb_act8_hessian": ([C.POINTER(Act8), f32, i32, vp, vp], i32),
+            "tb_adapter_forward": ([C.POINTER(AdapterArgs), vp], i32),
+            "tb_adapter_backward": ([C.POINTER(AdapterArgs), vp], i32),
             "tb_score_mask_pack": ([C.POINTER(PruneArgs), vp], i32),
             "tb_fisher_partial_scatter": ([vp, i32, sz, sz, sz, vp, i32, C.POINTER(C.c_uint64), C.POINTER(vp), i32,
                                            vp], i32),
@@ -190,3 +240,53 @@ def score_mask_pack(args: PruneArgs, stream=None) -> int:
 
 def score_mask_pack_host(args: PruneArgs) -> int:
     return lib().tb_score_mask_pack_host(C.byref(args))
+
+
+def act8(*, n, d, codes, exps, ldq, lde) -> Act8:
+    """A checkpoint of n tokens with d features: codes [n][ldq], exponent bytes [ceil(n / 128)][lde]."""
+    return Act8(C.sizeof(Act8), d, n, codes, ldq, exps, lde)
+
+
+def act8_pack(ck: Act8, x, dtype, ldx, *, keep=None, stream=None) -> int:
+    return lib().tb_act8_pack(C.byref(ck), x, dtype, ldx, keep, stream)
+
+
+def act8_unpack(ck: Act8, out, dtype, ldo, *, stream=None) -> int:
+    return lib().tb_act8_unpack(C.byref(ck), out, dtype, ldo, stream)
+
+
+def act8_weight_grad(ck: Act8, dy, dy_dtype, lddy, r, samples, S, grads, g_dtype, *, g_stride=0, stream=None) -> int:
+    return lib().tb_act8_weight_grad(C.byref(ck), dy, dy_dtype, lddy, r, samples, S, grads, g_dtype, g_stride, stream)
+
+
+def act8_fisher(ck: Act8, dy, dy_dtype, lddy, r, samples, S, fisher, *, alpha=0.01, beta=0.99, first_step=True,
+                stream=None) -> int:
+    return lib().tb_act8_fisher(C.byref(ck), dy, dy_dtype, lddy, r, samples, S, alpha, beta, int(first_step), fisher,
+                                stream)
+
+
+def act8_hessian(ck: Act8, scale, H, *, accumulate=False, stream=None) -> int:
+    return lib().tb_act8_hessian(C.byref(ck), scale, int(accumulate), H, stream)
+
+
+def adapter_args(*, n, d, r, rank, n_adapters, a=None, lda=0, b=None, ldb=0, scale=None, token_adapter=None, w=None,
+                 ldw=0, x=None, ldx=0, y=None, ldy=0, dy=None, lddy=0, x8=None, dx=None, lddx=0, da=None,
+                 db=None, dtype=BF16) -> AdapterArgs:
+    p = AdapterArgs()
+    p.struct_size = C.sizeof(AdapterArgs)
+    p.dtype, p.n, p.d, p.r, p.rank, p.n_adapters = dtype, n, d, r, rank, n_adapters
+    p.w, p.ldw, p.a, p.lda, p.b, p.ldb = w, ldw, a, lda, b, ldb
+    p.scale, p.token_adapter = scale, token_adapter
+    p.x, p.ldx, p.y, p.ldy, p.dy, p.lddy = x, ldx, y, ldy, dy, lddy
+    if x8 is not None:
+        p.x8 = C.pointer(x8)
+    p.dx, p.lddx, p.da, p.db = dx, lddx, da, db
+    return p
+
+
+def adapter_forward(args: AdapterArgs, stream=None) -> int:
+    return lib().tb_adapter_forward(C.byref(args), stream)
+
+
+def adapter_backward(args: AdapterArgs, stream=None) -> int:
+    return lib().tb_adapter_backward(C.byref(args), stream)

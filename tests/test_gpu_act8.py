@@ -1,0 +1,355 @@
+"""GPU: 8-bit activation checkpoints and what is computed from them, against the
+float64 restatement in act8_ref.py.
+
+Bars.  Codes, exponents and values read back are exact.  A sum of n products is
+held to n * 2^-23 of the sum of its terms' magnitudes: every product is exact,
+an FP32 addition (or the alignment of a product in a tensor-core step, which
+truncates) loses at most 2^-23 of the largest partial sum, and no partial sum
+exceeds that sum of magnitudes; FP32 and F16 dy have three and two parts, hence
+three and two times the additions.  A BF16 result adds half a step, 2^-8 of the
+value.  Beside that bound, which grows with n, the 2-norm error of FP32 results
+stays below 2e-6: rounding errors of n terms add like sqrt(n), and both sides
+of the ratio do, so it is a few times 2^-24 times the depth of one partial sum
+(16 tensor-core steps) whatever n."""
+import math
+
+import pytest
+
+import act8_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(torch, n, d, dtype, seed, ld=None, scale=1.0, heavy=20.0):
+    """[n][d] normal values with 1 % heavy columns, as a view of rows of stride ld."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, d, device="cuda", generator=g) * scale
+    if heavy:
+        x[:, torch.randperm(d, device="cuda", generator=g)[: max(1, d // 100)]] *= heavy
+    buf = torch.full((max(1, n), ld or d), 7.0, device="cuda", dtype=dtype)
+    buf[:n, :d] = x.to(dtype)
+    return buf[:n, :d]
+
+
+def code(tb, torch, dtype):
+    return {torch.float32: tb.F32, torch.float16: tb.F16, torch.bfloat16: tb.BF16}[dtype]
+
+
+class Checkpoint:
+    def __init__(self, torch, tb, n, d, ldq=None, lde=None):
+        self.n, self.d = n, d
+        self.codes = torch.full((max(1, n), ldq or ref.up(d, 16)), 85, device="cuda", dtype=torch.int8)
+        self.exps = torch.full((max(1, -(-n // 128)), lde or ref.up(d, 16)), 85, device="cuda", dtype=torch.uint8)
+        self.s = tb.act8(n=n, d=d, codes=self.codes.data_ptr(), ldq=self.codes.stride(0), exps=self.exps.data_ptr(),
+                         lde=self.exps.stride(0))
+
+    def values(self, torch):
+        return ref.values(torch, self.codes[: self.n, : self.d], self.exps[:, : self.d])
+
+
+def packed(torch, tb, x, keep=None, **kw):
+    n, d = x.shape
+    c = Checkpoint(torch, tb, n, d, **kw)
+    tb.check(tb.act8_pack(c.s, x.data_ptr(), code(tb, torch, x.dtype), x.stride(0),
+                          keep=None if keep is None else keep.data_ptr()))
+    return c
+
+
+@pytest.mark.parametrize("n,d,dtype,ld", [
+    (1, 1, "float32", None), (1, 4096, "bfloat16", None), (127, 129, "float16", 131), (128, 128, "float32", None),
+    (129, 200, "bfloat16", 208), (300, 77, "bfloat16", 77), (1000, 515, "float32", 516), (257, 1024, "float16", 1024)])
+def test_pack_and_unpack_are_exact(cuda, tblib, n, d, dtype, ld):
+    torch, tb = cuda, tblib
+    x = rows(torch, n, d, getattr(torch, dtype), n + d, ld)
+    if n > 2:
+        x[1].zero_()
+        x[:, 0] = 0.0
+        x[0, d // 2] = 1e-4 if dtype == "float16" else 1e-42  # subnormal in FP32
+    c = packed(torch, tb, x, ldq=ref.up(d, 16) + 16, lde=ref.up(d, 16) + 32)
+    q, e = ref.pack(torch, x)
+    assert torch.equal(c.codes[:n, :d], q) and torch.equal(c.exps[:, :d], e)
+    assert bool((c.codes[:, d:] == 85).all()) and bool((c.exps[:, d:] == 85).all())
+    want = ref.values(torch, q, e)
+    for out_t in (torch.float32, torch.bfloat16, torch.float16):
+        out = torch.full((n + 1, d + 3), 9.0, device="cuda", dtype=out_t)
+        tb.check(tb.act8_unpack(c.s, out.data_ptr(), code(tb, torch, out_t), d + 3))
+        assert torch.equal(out[:n, :d], want.to(out_t))
+        assert bool((out[n:] == 9).all()) and bool((out[:, d:] == 9).all())
+    # half a step of a block's scale, and scales no larger than needed
+    amax = x.double().abs().amax(0)
+    assert bool(((want - x.double()).abs() <= amax / 126.9).all())
+
+
+def test_pack_borders(cuda, tblib):
+    """Largest values around the border where the exponent steps (127.5 codes), powers of two, the ends of FP32."""
+    torch, tb = cuda, tblib
+    vals = [127.0, 127.49, 127.5, 127.50001, 128.0, 1.0, 0.99609375, 0.9960937, 1.9921875, 1.9921874, 3.4028235e38,
+            1.1754944e-38, 1e-45, 0.0, 2.0 ** -120, 2.0 ** -119]
+    x = torch.zeros(3, len(vals), device="cuda")
+    x[1] = torch.tensor(vals, device="cuda")
+    x[2] = -x[1] / 3
+    c = packed(torch, tb, x)
+    q, e = ref.pack(torch, x)
+    assert torch.equal(c.codes[:3, : len(vals)], q) and torch.equal(c.exps[:, : len(vals)], e)
+
+
+def test_padding_and_values_that_are_no_numbers(cuda, tblib):
+    torch, tb = cuda, tblib
+    n, d = 300, 40
+    x = rows(torch, n, d, torch.float32, 5)
+    keep = (torch.arange(n, device="cuda") % 100 < 70).to(torch.uint8)
+    x[keep == 0] = math.nan
+    x[99] = math.inf
+    x[130, 3], x[140, 4], x[150, 5] = math.nan, math.inf, -math.inf
+    keep[[130, 140, 150]] = 1
+    c = packed(torch, tb, x, keep)
+    q, e = ref.pack(torch, x, keep)
+    assert torch.equal(c.codes[:n, :d], q) and torch.equal(c.exps[:, :d], e)
+    out = torch.empty(n, d, device="cuda")
+    tb.check(tb.act8_unpack(c.s, out.data_ptr(), tb.F32, d))
+    assert bool((out[:128][keep[:128] == 0] == 0).all()) and bool(torch.isfinite(out[:128]).all())
+    assert bool(torch.isnan(out[128:256, 3:6]).all()) and int(torch.isnan(out).sum()) == 3 * 128
+    # every token padding: all codes zero
+    c = packed(torch, tb, x, torch.zeros(n, device="cuda", dtype=torch.uint8))
+    assert not bool(c.codes[:n, :d].any()) and bool((c.exps[:, :d] == 1).all())
+
+
+PARTS = {"bfloat16": 1, "float16": 2, "float32": 3}
+
+
+def pairs(torch, samples):
+    return torch.tensor(samples, device="cuda", dtype=torch.int64).reshape(-1, 2)
+
+
+def check_sums(torch, got, want, mag, terms, bf16=False):
+    bar = terms * 2.0 ** -23 * mag + 1e-300
+    if bf16:
+        bar = bar * 1.01 + 2.0 ** -8 * want.abs() + 1e-40
+    over = ((got.double() - want).abs() - bar).max().item()
+    assert over <= 0, over
+    if not bf16 and float(want.norm()) > 0:
+        assert float((got.double() - want).norm() / want.norm()) <= 2e-6
+
+
+@pytest.mark.parametrize("n,r,d,dy_t,g_t,samples", [
+    (1, 1, 1, "float32", "float32", None), (5, 3, 7, "bfloat16", "float32", [(0, 5)]),
+    (64, 128, 256, "bfloat16", "bfloat16", None), (130, 64, 130, "bfloat16", "float32", [(0, 64), (64, 130)]),
+    (333, 257, 511, "bfloat16", "bfloat16", [(0, 1), (1, 64), (64, 64), (64, 333)]),
+    (700, 129, 384, "float32", "float32", [(0, 127), (127, 500), (500, 700)]),
+    (515, 200, 272, "float16", "float32", [(3, 130), (400, 512)]),
+    (2000, 384, 640, "bfloat16", "bfloat16", [(0, 700), (650, 1400), (1400, 2000), (0, 2000), (0, 700)]),
+    (4100, 256, 256, "bfloat16", "float32", None), (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)])])
+def test_weight_grad(cuda, tblib, n, r, d, dy_t, g_t, samples):
+    torch, tb = cuda, tblib
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, n))
+    # a BF16 dy of odd stride goes through scratch, one of aligned rows does not
+    dy = rows(torch, n, r, getattr(torch, dy_t), n + 1, ref.up(r, 8) + (1 if n in (5, 130) else 8), 1e-2, 0)
+    S = len(samples) if samples else 1
+    stride = r * d + 5
+    out = torch.full((S, stride), 3.0, device="cuda", dtype=getattr(torch, g_t))
+    sp = pairs(torch, samples) if samples else None
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r,
+                                 sp.data_ptr() if samples else None, S, out.data_ptr(), code(tb, torch, out.dtype),
+                                 g_stride=stride))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    assert bool((out[:, r * d:] == 3).all())
+    for s, (G, A) in enumerate(ref.gradients(torch, dy, c.values(torch), samples or [(0, n)])):
+        check_sums(torch, out[s, : r * d].view(r, d), G, A, n * PARTS[dy_t], g_t == "bfloat16")
+
+
+def test_weight_grad_leaves_other_tokens_out(cuda, tblib):
+    """NaN and infinities in tokens of no sample reach no gradient; those of one sample stay in it."""
+    torch, tb = cuda, tblib
+    n, r, d = 400, 136, 200
+    x = rows(torch, n, d, torch.float32, 1)
+    x[384:] = math.nan
+    c = packed(torch, tb, x)
+    for dt in (torch.bfloat16, torch.float32):
+        dy = rows(torch, n, r, dt, 2, 136, 1e-2, 0)
+        dy[100:110] = math.inf
+        dy[200, 5] = math.nan
+        dy[300:310] = -math.inf
+        samples = [(10, 100), (110, 201), (201, 300), (310, 384), (310, 390)]
+        out = torch.empty(5, r, d, device="cuda")
+        tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), code(tb, torch, dt), dy.stride(0), r,
+                                     pairs(torch, samples).data_ptr(), 5, out.data_ptr(), tb.F32))
+        fine = torch.isfinite(out)
+        assert bool(fine[[0, 2, 3]].all()) and not bool(fine[4].any())
+        assert not bool(fine[1, 5].any()) and bool(fine[1, :5].all()) and bool(fine[1, 6:].all())
+
+
+@pytest.mark.parametrize("n,r,d,dy_t,S,first", [
+    (60, 128, 128, "float32", 8, True), (600, 130, 70, "bfloat16", 3, False), (1, 5, 9, "bfloat16", 1, True),
+    (900, 256, 640, "bfloat16", 7, True), (513, 384, 257, "float16", 4, False), (3000, 136, 264, "bfloat16", 2, True)])
+def test_fisher(cuda, tblib, n, r, d, dy_t, S, first):
+    """The EMA of the float64 gradients: each g is within its sum's bar, a square doubles that, and each step rounds four times."""
+    torch, tb = cuda, tblib
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, n, heavy=0))
+    dy = rows(torch, n, r, getattr(torch, dy_t), n + 1, ref.up(r, 8), 1e-2, 0)
+    cuts = sorted(torch.randint(0, n + 1, (S - 1,), generator=torch.Generator().manual_seed(n)).tolist())
+    samples = list(zip([0] + cuts, cuts + [n]))
+    F0 = torch.rand(r, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    F = F0.clone() if not first else torch.full((r, d), math.nan, device="cuda")
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, pairs(torch, samples).data_ptr(),
+                            S, F.data_ptr(), alpha=0.01, beta=0.99, first_step=first))
+    torch.cuda.synchronize()
+    ga = ref.gradients(torch, dy, c.values(torch), samples)
+    f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))  # the FP32 constants that the recurrence uses
+    alpha, beta = f32(0.01), f32(0.99)
+    want = ref.fisher(torch, [G for G, _ in ga], alpha, beta, None if first else F0.double())
+    slack = n * PARTS[dy_t] * 2.0 ** -23
+    worst = ref.fisher(torch, [G.abs() + slack * A for G, A in ga], alpha, beta, None if first else F0.double())
+    bar = (worst - want) + 5 * S * 2.0 ** -24 * worst + 1e-40
+    assert float(((F.double() - want).abs() - bar).max()) <= 0
+    assert float((F.double() - want).norm() / want.norm()) <= 4e-6
+
+
+def test_fisher_equals_its_steps(cuda, tblib):
+    """One fused call and tb_fisher_ema_step over the FP32 gradients of the same call's family agree to rounding of g."""
+    torch, tb = cuda, tblib
+    n, r, d, S = 500, 256, 384, 5
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 4))
+    dy = rows(torch, n, r, torch.bfloat16, 5, 256, 1e-2, 0)
+    sp = pairs(torch, [(i * 100, i * 100 + 100) for i in range(S)])
+    G = torch.empty(S, r, d, device="cuda")
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, 256, r, sp.data_ptr(), S, G.data_ptr(), tb.F32))
+    F, F2 = torch.empty(r, d, device="cuda"), torch.zeros(r, d, device="cuda")
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, 256, r, sp.data_ptr(), S, F.data_ptr()))
+    for s in range(S):
+        tb.check(tb.lib().tb_fisher_ema_step(F2.data_ptr(), G[s].data_ptr(), tb.F32, r * d, 0.01, 0.99, int(s == 0), None))
+    assert float((F - F2).norm() / F2.norm()) <= 1e-6
+
+
+@pytest.mark.parametrize("n,d,acc", [(1, 1, False), (64, 128, False), (130, 200, True), (1000, 640, False),
+                                     (777, 515, True), (0, 96, False), (0, 96, True), (4096, 256, False), (300, 1100, True)])
+def test_hessian(cuda, tblib, n, d, acc):
+    torch, tb = cuda, tblib
+    x = rows(torch, n, d, torch.float32, n + d)
+    c = packed(torch, tb, x) if n else Checkpoint(torch, tb, 0, d)
+    H = rows(torch, d, d, torch.float32, 9, heavy=0).contiguous()
+    H0 = H.clone()
+    scale = 1.0 / max(1, n)
+    tb.check(tb.act8_hessian(c.s, scale, H.data_ptr(), accumulate=acc))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    t = torch.arange(d, device="cuda") // 128
+    lower = t[:, None] >= t[None]
+    assert torch.equal(H[~lower], H0[~lower])
+    xh = c.values(torch) if n else torch.zeros(0, d, device="cuda", dtype=torch.float64)
+    s32 = float(torch.tensor(scale, dtype=torch.float32))
+    want = s32 * (xh.t() @ xh) + (H0.double() if acc else 0)
+    mag = s32 * (xh.abs().t() @ xh.abs()) + (H0.double().abs() if acc else 0)
+    err = (H.double() - want).abs() - (n + 3) * 2.0 ** -23 * mag
+    assert float(err[lower].max()) <= 0
+    if not acc and n:
+        assert float((H.double() - want)[lower].norm() / want[lower].norm()) <= 1e-6
+
+
+def test_hessian_of_a_block_without_numbers(cuda, tblib):
+    torch, tb = cuda, tblib
+    x = rows(torch, 200, 150, torch.float32, 3)
+    x[150, 7] = math.inf
+    c = packed(torch, tb, x)
+    H = torch.zeros(150, 150, device="cuda")
+    tb.check(tb.act8_hessian(c.s, 1.0, H.data_ptr()))
+    t = torch.arange(150, device="cuda")
+    hit = ((t[:, None] == 7) | (t[None] == 7)) & (t[:, None] // 128 >= t[None] // 128)
+    assert bool(torch.isnan(H[hit]).all()) and bool(torch.isfinite(H[~hit]).all())
+
+
+def test_hessian_matches_the_bf16_entry(cuda, tblib):
+    """xhat is exact in BF16: tb_obs_hessian of the values read back gives the same matrix to FP32 rounding."""
+    torch, tb = cuda, tblib
+    n, d = 640, 512
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 12))
+    H, H2 = torch.zeros(d, d, device="cuda"), torch.zeros(d, d, device="cuda")
+    xt = c.values(torch).t().contiguous().bfloat16()
+    tb.check(tb.lib().tb_obs_hessian(xt.data_ptr(), d, n, H2.data_ptr(), None))
+    tb.check(tb.act8_hessian(c.s, 1.0 / n, H.data_ptr()))
+    torch.cuda.synchronize()
+    assert float((H - H2).norm() / H2.norm()) <= 1e-6
+
+
+def test_two_streams_and_two_graphs(cuda, tblib):
+    """Calls on two streams at once, and two captured graphs replayed in turn with changed inputs, give what single calls give."""
+    torch, tb = cuda, tblib
+    n, r, d = 700, 264, 520
+    sets = []
+    for i in range(2):
+        c = packed(torch, tb, rows(torch, n, d, torch.float32, 20 + i))
+        dy = rows(torch, n, r, torch.float32, 30 + i, 264, 1e-2, 0)  # FP32: takes scratch
+        sp = pairs(torch, [(0, 300 + i), (300 + i, n)])
+        out = [torch.empty(2, r, d, device="cuda"), torch.empty(r, d, device="cuda"), torch.zeros(d, d, device="cuda")]
+        sets.append((c, dy, sp, out))
+
+    def go(k, stream):
+        c, dy, sp, (G, F, H) = sets[k]
+        tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.F32, 264, r, sp.data_ptr(), 2, G.data_ptr(), tb.F32, stream=stream))
+        tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.F32, 264, r, sp.data_ptr(), 2, F.data_ptr(), stream=stream))
+        tb.check(tb.act8_hessian(c.s, 1.0, H.data_ptr(), stream=stream))
+
+    def single(k):
+        go(k, None)
+        torch.cuda.synchronize()
+        return [t.clone() for t in sets[k][3]]
+
+    want = [single(0), single(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for t in sets[0][3] + sets[1][3]:
+            t.fill_(-1.0)
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            go(k, streams[k].cuda_stream)
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            low = [torch.tril(a) for a in sets[k][3][2:]], [torch.tril(a) for a in want[k][2:]]
+            assert all(torch.equal(a, b) for a, b in zip(sets[k][3][:2] + low[0], want[k][:2] + low[1]))
+    graphs = []
+    for k in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            go(k, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for t in sets[0][3] + sets[1][3]:
+        t.fill_(-1.0)
+    for k in (0, 1, 0, 1):
+        graphs[k].replay()
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(sets[k][3][:2], want[k][:2]))
+    sets[0][2].copy_(pairs(torch, [(0, 1), (1, 1)]))  # new sample bounds under the captured graph
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert not bool(sets[0][3][0][1].any()) and not torch.equal(sets[0][3][0][0], want[0][0][0])
+
+
+def test_calibration_end_to_end(cuda, tblib):
+    """A layer's calibration from one checkpoint: the Fisher state scored and masked by the fused pass equals the pass
+    over the materialised gradients' own EMA, and the Hessian prunes the layer."""
+    import ctypes as C
+    torch, tb = cuda, tblib
+    n, r, d, S = 512, 256, 512, 4
+    c = packed(torch, tb, rows(torch, n, d, torch.bfloat16, 40))
+    dy = rows(torch, n, r, torch.bfloat16, 41, 256, 1e-2, 0)
+    sp = pairs(torch, [(i * 128, i * 128 + 128) for i in range(S)])
+    W = rows(torch, r, d, torch.float32, 42, scale=0.02, heavy=0).contiguous()
+    F = torch.empty(r, d, device="cuda")
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, 256, r, sp.data_ptr(), S, F.data_ptr()))
+    G = torch.empty(S, r, d, device="cuda")
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, 256, r, sp.data_ptr(), S, G.data_ptr(), tb.F32))
+    outs = []
+    for kw in (dict(grads=None, S=0, fisher_in=F.data_ptr(), fisher_steps_in=S), dict(grads=G.data_ptr(), S=S)):
+        w, m = torch.empty(r, d, device="cuda"), torch.empty(r * d // 4, device="cuda", dtype=torch.uint8)
+        a = tb.prune_args(weights=W.data_ptr(), w_dtype=tb.F32, g_dtype=tb.F32, N=r * d, w_out=w.data_ptr(),
+                          mask_out=m.data_ptr(), **kw)
+        tb.check(tb.score_mask_pack(a))
+        outs.append((w, m))
+    torch.cuda.synchronize()
+    assert float((outs[0][1] != outs[1][1]).float().mean()) <= 1e-3  # near ties only: F differs by rounding
+    H = torch.zeros(d, d, device="cuda")
+    tb.check(tb.act8_hessian(c.s, 1.0 / n, H.data_ptr()))
+    mask = torch.empty(r * d // 4, device="cuda", dtype=torch.uint8)
+    tb.check(tb.lib().tb_obs_sparsegpt(W.data_ptr(), r, d, H.data_ptr(), 0.01, 2, 4, mask.data_ptr(), None, None))
+    assert float((W == 0).float().mean()) == 0.5

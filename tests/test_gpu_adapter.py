@@ -1,0 +1,235 @@
+"""GPU: low-rank adapters beside a shared projection, against float64.
+
+Bars.  A BF16 result is off by half a step, 2^-8 of its value, and by its sum:
+every product of two BF16 values is exact and each of the K additions loses at
+most 2^-23 of the sum of magnitudes; u and v, FP32 sums themselves, enter their
+second product as two BF16 parts, 2^-16 of their magnitude (2^-9 of 2^-9, with
+room for the parts' sum).  So |error| <= 2^-8 |y| + (K 2^-23 + 2^-16) * mag."""
+import math
+
+import pytest
+
+import act8_ref as ref
+from test_gpu_act8 import packed, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def bf(torch, n, d, seed, scale=1.0):
+    return rows(torch, n, d, torch.bfloat16, seed, ref.up(d, 8), scale, 0)
+
+
+class Case:
+    def __init__(self, torch, n, d, r, rank, na, who, seed=0):
+        self.torch, self.n, self.d, self.r, self.rank, self.na = torch, n, d, r, rank, na
+        self.w = bf(torch, r, d, seed + 1, 0.05)
+        self.a = bf(torch, max(1, na) * rank, d, seed + 2, 1 / math.sqrt(d))
+        self.b = bf(torch, max(1, na) * r, rank, seed + 3, 0.3)
+        self.x, self.dy = bf(torch, n, d, seed + 4), bf(torch, n, r, seed + 5, 0.1)
+        self.scale = torch.rand(max(1, na), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)) + 0.5
+        self.who = who.to(torch.int32).cuda().contiguous()
+        self.y = torch.full((n + 1, r + 5), 3.0, device="cuda", dtype=torch.bfloat16)
+        self.dx = torch.full((n + 1, d + 3), 3.0, device="cuda", dtype=torch.bfloat16)
+        self.da = torch.full((max(1, na) * rank, self.a.stride(0)), 3.0, device="cuda", dtype=torch.bfloat16)
+        self.db = torch.full((max(1, na) * r, self.b.stride(0)), 3.0, device="cuda", dtype=torch.bfloat16)
+        self.ref = ref.Adapters(torch, self.w, self.a.reshape(-1, rank, d)[:na], self.b.reshape(-1, r, rank)[:na],
+                                self.scale, self.who)
+
+    def args(self, tb, **kw):
+        a = dict(n=self.n, d=self.d, r=self.r, rank=self.rank, n_adapters=self.na, w=self.w.data_ptr(), ldw=self.w.stride(0),
+                 a=self.a.data_ptr(), lda=self.a.stride(0), b=self.b.data_ptr(), ldb=self.b.stride(0),
+                 scale=self.scale.data_ptr(), token_adapter=self.who.data_ptr(), x=self.x.data_ptr(), ldx=self.x.stride(0),
+                 y=self.y.data_ptr(), ldy=self.y.stride(0), dy=self.dy.data_ptr(), lddy=self.dy.stride(0),
+                 dx=self.dx.data_ptr(), lddx=self.dx.stride(0), da=self.da.data_ptr(), db=self.db.data_ptr())
+        a.update(kw)
+        return tb.adapter_args(**a)
+
+
+def check(torch, got, want, mag, K):
+    err = (got.double() - want).abs() - (2.0 ** -8 * want.abs() + (K * 2.0 ** -23 + 2.0 ** -16) * 1.01 * mag + 1e-40)
+    assert float(err.max()) <= 0, float(err.max())
+
+
+def who_of(torch, n, na, kind, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "mixed":
+        return torch.randint(-1, max(1, na), (n,), generator=g)
+    if kind == "none":
+        return torch.full((n,), -1)
+    if kind == "one":
+        return torch.zeros(n, dtype=torch.int64)
+    if kind == "wild":  # indexes that name no adapter
+        return torch.tensor([-7, na, na + 5, 0, 2 ** 31 - 1, -2 ** 31])[torch.arange(n) % 6]
+    return torch.div(torch.arange(n) * max(1, na), max(1, n), rounding_mode="floor")
+
+
+SHAPES = [
+    (1, 64, 64, 8, 1, "one"), (1, 4096, 1024, 16, 4, "mixed"), (3, 40, 24, 1, 2, "runs"), (8, 520, 136, 16, 8, "runs"),
+    (17, 256, 264, 5, 3, "mixed"), (33, 136, 1000, 64, 2, "runs"), (64, 512, 256, 128, 3, "mixed"),
+    (130, 384, 520, 33, 4, "runs"), (300, 264, 136, 16, 40, "mixed"), (257, 128, 256, 24, 2, "wild"),
+    (520, 1024, 384, 32, 5, "runs"), (100, 77, 51, 8, 2, "none"), (90, 200, 72, 12, 0, "none"),
+    (1100, 256, 640, 100, 3, "runs")]
+
+
+@pytest.mark.parametrize("n,d,r,rank,na,kind", SHAPES)
+def test_forward(cuda, tblib, n, d, r, rank, na, kind):
+    torch, tb = cuda, tblib
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, kind))
+    tb.check(tb.adapter_forward(c.args(tb)))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    check(torch, c.y[:n, :r], c.ref.forward(c.x), c.ref.forward(c.x, True), d + rank)
+    assert bool((c.y[n:] == 3).all()) and bool((c.y[:, r:] == 3).all())
+
+
+@pytest.mark.parametrize("n,d,r,rank,na,kind", SHAPES)
+def test_backward(cuda, tblib, n, d, r, rank, na, kind):
+    torch, tb = cuda, tblib
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, kind), 10)
+    ck = packed(torch, tb, c.x)
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    xh = ck.values(torch)
+    dx, da, db = c.ref.backward(c.dy, xh)
+    mx, ma, mb = c.ref.backward(c.dy, xh, True)
+    check(torch, c.dx[:n, :d], dx, mx, r + rank)
+    assert bool((c.dx[n:] == 3).all()) and bool((c.dx[:, d:] == 3).all())
+    if na:
+        check(torch, c.da[:, :d].reshape(na, rank, d), da, ma, n + r)
+        check(torch, c.db[:, :rank].reshape(na, r, rank), db, mb, n + d)
+        assert bool((c.da[:, d:] == 3).all()) and bool((c.db[:, rank:] == 3).all())
+
+
+def test_gradients_against_differences(cuda, tblib):
+    """The loss sum(dy * y(xhat)) in float64, differenced along random directions of x, A and B, against the kernels'
+    gradients: y is linear in each of them alone, so a central difference is exact to float64 rounding, and the
+    gradients' own errors are their entries' half steps, which add to at most 2^-8 sum |g||direction|, and their sums'."""
+    torch, tb = cuda, tblib
+    c = Case(torch, 70, 96, 80, 8, 3, who_of(torch, 70, 3, "mixed"), 20)
+    ck = packed(torch, tb, c.x)
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    torch.cuda.synchronize()
+    xh = ck.values(torch)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    R = c.ref
+    mags = R.backward(c.dy, xh, True)
+    for name, grad, mag in (("x", c.dx[:70, :96], mags[0]), ("a", c.da[:, :96].reshape(3, 8, 96), mags[1]),
+                            ("b", c.db[:, :8].reshape(3, 80, 8), mags[2])):
+        v = torch.randn(grad.shape, device="cuda", generator=g, dtype=torch.float64)
+        loss = []
+        for h in (0.5, -0.5):
+            m = ref.Adapters(torch, R.w, R.a + (h * v if name == "a" else 0), R.b + (h * v if name == "b" else 0), R.scale, R.who)
+            loss.append(float((c.dy.double() * m.forward(xh + (h * v if name == "x" else 0))).sum()))
+        want, got = loss[0] - loss[1], float((grad.double() * v).sum())
+        bar = float((v.abs() * (2.0 ** -8 * grad.double().abs() + 2.0 ** -15 * mag)).sum())
+        assert abs(want - got) <= bar
+
+
+def test_values_of_other_tokens_stay_out(cuda, tblib):
+    """NaN and infinities in one adapter, one token or an adapter's unused rows reach only what uses them."""
+    torch, tb = cuda, tblib
+    n, d, r, rank, na = 150, 200, 136, 16, 4
+    who = who_of(torch, n, 3, "runs")  # adapter 3 is used by nobody
+    c = Case(torch, n, d, r, rank, na, who, 30)
+    c.a[3 * rank:] = math.nan
+    c.b[3 * r:] = math.inf
+    c.a[rank] = math.nan  # one row of adapter 1
+    c.x[140] = math.inf   # a token of adapter 2
+    tb.check(tb.adapter_forward(c.args(tb)))
+    y = c.y[:n, :r]
+    bad = (c.who == 1) | (torch.arange(n, device="cuda") == 140)
+    assert bool(torch.isfinite(y[~bad]).all()) and not bool(torch.isfinite(y[bad]).any())
+    c = Case(torch, n, d, r, rank, na, who, 30)
+    ck = packed(torch, tb, c.x)
+    c.dy[5] = math.nan    # a token of adapter 0
+    c.b[3 * r:] = math.nan
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    dx, da, db = c.dx[:n, :d], c.da[:, :d].reshape(na, rank, d), c.db[:, :rank].reshape(na, r, rank)
+    assert bool(torch.isnan(dx[5]).all()) and int(torch.isnan(dx).sum()) == d
+    assert bool(torch.isnan(da[0]).all()) and bool(torch.isfinite(da[1:]).all())
+    assert bool(torch.isnan(db[0]).all()) and bool(torch.isfinite(db[1:]).all())
+    assert not bool(da[3].any()) and not bool(db[3].any())
+
+
+def test_outputs_may_be_left_out(cuda, tblib):
+    torch, tb = cuda, tblib
+    c = Case(torch, 40, 64, 72, 8, 2, who_of(torch, 40, 2, "runs"), 40)
+    ck = packed(torch, tb, c.x)
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    whole = [t.clone() for t in (c.dx, c.da, c.db)]
+    for t in (c.dx, c.da, c.db):
+        t.fill_(3.0)
+    tb.check(tb.adapter_backward(c.args(tb, da=None, db=None)))
+    assert torch.equal(c.dx, whole[0]) and bool((c.da == 3).all())
+    c.dx.fill_(3.0)
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s, dx=None, w=None)))
+    assert torch.equal(c.da, whole[1]) and torch.equal(c.db, whole[2]) and bool((c.dx == 3).all())
+    # no tokens: the gradients are zero
+    empty = packed(torch, tb, c.x)
+    empty.s.n = 0
+    tb.check(tb.adapter_backward(c.args(tb, n=0, x8=empty.s, dy=None)))
+    assert not bool(c.da[:, :64].any()) and not bool(c.db[:, :8].any())
+
+
+def test_calls_repeat_bit_for_bit_and_under_graphs(cuda, tblib):
+    torch, tb = cuda, tblib
+    sets = []
+    for i in range(2):
+        c = Case(torch, 600, 264, 392, 24, 5, who_of(torch, 600, 5, "mixed", i), 50 + i)
+        sets.append((c, packed(torch, tb, c.x)))
+
+    def go(k, stream=None):
+        c, ck = sets[k]
+        tb.check(tb.adapter_forward(c.args(tb), stream=stream))
+        tb.check(tb.adapter_backward(c.args(tb, x8=ck.s), stream=stream))
+
+    def outs(k):
+        c = sets[k][0]
+        return [c.y, c.dx, c.da, c.db]
+
+    want = []
+    for k in (0, 1):
+        go(k)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in outs(k)])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for t in outs(0) + outs(1):
+            t.fill_(3.0)
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            go(k, streams[k].cuda_stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for k in (0, 1) for a, b in zip(outs(k), want[k]))
+    graphs = []
+    for k in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            go(k, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for t in outs(0) + outs(1):
+        t.fill_(3.0)
+    for k in (0, 1, 1, 0):
+        graphs[k].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in (0, 1) for a, b in zip(outs(k), want[k]))
+
+
+def test_calibration_step_with_adapters(cuda, tblib):
+    """Forward with adapters, the checkpoint, the backward, and the shared projection's Fisher from the same tensors."""
+    torch, tb = cuda, tblib
+    n, d, r = 256, 256, 128
+    c = Case(torch, n, d, r, 16, 2, who_of(torch, n, 2, "runs"), 60)
+    ck = packed(torch, tb, c.x)
+    tb.check(tb.adapter_forward(c.args(tb)))
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    F = torch.empty(r, d, device="cuda")
+    sp = torch.tensor([[0, 128], [128, 256]], device="cuda")
+    tb.check(tb.act8_fisher(ck.s, c.dy.data_ptr(), tb.BF16, c.dy.stride(0), r, sp.data_ptr(), 2, F.data_ptr()))
+    w, m = torch.empty(r, d, device="cuda"), torch.empty(r * d // 4, device="cuda", dtype=torch.uint8)
+    a = tb.prune_args(weights=c.w.contiguous().data_ptr(), w_dtype=tb.BF16, grads=None, g_dtype=tb.F32, S=0, N=r * d,
+                      fisher_in=F.data_ptr(), fisher_steps_in=2, w_out=w.data_ptr(), mask_out=m.data_ptr())
+    tb.check(tb.score_mask_pack(a))
+    torch.cuda.synchronize()
+    assert float((w == 0).float().mean()) >= 0.5 and bool(torch.isfinite(c.y[:n, :r]).all())
