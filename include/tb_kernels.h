@@ -210,8 +210,8 @@ int tb_gemm_nt_tf32x3(const float* a_hi, const float* a_lo, long long lda, const
 int tb_gemm_nt_bf16(const void* a, long long lda, const void* b, long long ldb, int M, int N, int K,
                     float alpha, float beta, const float* c_in, long long ldcin, float* c, long long ldc,
                     int lower_only, void* stream);
-/* TB_ERR_TIMEOUT if a bounded pipeline wait inside a GEMM launched since the
- * last call expired (the kernel then skipped its output); synchronises. */
+/* TB_ERR_TIMEOUT if a bounded pipeline wait inside a GEMM, or inside a product
+ * of the checkpoint and adapter entries below, launched since the last call expired (the kernel then skipped its output); synchronises. */
 int tb_gemm_status(void* stream);
 
 /* ---- stage 3: column-block exact OBS against calibration activations ----- */
@@ -303,13 +303,18 @@ int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
  * 148-201) per sample, in their order, without the gradients in memory: with
  * G_s as above in FP32, the first step (first_step != 0, F not read) gives
- * F = (alpha g) g, the others F = beta F + ((alpha (1 - beta)) g) g.  fisher
- * is [r][d].  A sample without tokens is a step with g = 0. */
+ * F = (alpha g) g, the others F = beta F + ((alpha (1 - beta)) g) g, with the
+ * factors rounded to FP32 once.  (alpha and beta are double because 1 - beta
+ * of an FP32 0.99 is off by 1e-6; FP32 values give tb_fisher_ema_step's own
+ * factors.)  fisher is [r][d].  A sample without tokens is a step with g = 0. */
 int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r, const int64_t* samples,
-                   int S, float alpha, float beta, int first_step, float* fisher, void* stream);
+                   int S, double alpha, double beta, int first_step, float* fisher, void* stream);
 /* H = scale * Xhat^T Xhat (accumulate != 0: added to H): tb_obs_hessian_scaled
  * from a checkpoint, for any d and n.  H is [d][d]; only the 128x128 tiles on
- * or below the diagonal are written.  n = 0 gives zeros (accumulate: H stays). */
+ * or below the diagonal are written.  n = 0 gives zeros (accumulate: H stays).
+ * Within a block of 128 tokens the codes' products add up exactly in integers;
+ * the blocks' sums are added in FP32.  A feature with values beyond 2^100,
+ * whose diagonal overflows in any case, gives infinities or NaN in its row. */
 int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, void* stream);
 
 /* ---- low-rank adapters beside a shared projection ------------------------- */

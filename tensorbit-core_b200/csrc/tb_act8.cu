@@ -4,9 +4,8 @@
 #include <algorithm>
 
 #include "tb_act8.cuh"
-#include "tb_device.cuh"
+#include "tb_linear.cuh"
 #include "tb_runtime.h"
-#include "tb_simple_gemm.cuh"
 
 namespace tb {
 namespace act8 {
@@ -156,65 +155,48 @@ __global__ void __launch_bounds__(256) unpack_kernel(const View ck, void* __rest
     }
 }
 
-__device__ __forceinline__ float xhat(const View& ck, long long t, long long f) {
-    return static_cast<float>(ck.codes[t * ck.ldq + f]) * scale_f32(ck.exps[(t / kBlock) * ck.lde + f]);
-}
-__device__ __forceinline__ float value(const void* p, int dt, long long i) {
-    return dt == TB_F32 ? Elem<TB_F32>::load(p, i) : dt == TB_F16 ? Elem<TB_F16>::load(p, i) : Elem<TB_BF16>::load(p, i);
-}
-
-struct GradOp {
-    static constexpr bool kRowA = false, kRowB = true;
-    View ck;
-    const void* dy;
-    int dy_dtype;
-    long long lddy, M, N;
-    const int64_t* samples;
-    int S;
-    void* grads;
-    int g_dtype;
-    long long g_stride;
-    float* fisher;  // EMA over the samples instead of gradients
-    float alpha, beta;
-    int first_step;
-    __device__ bool wanted(long long, long long) const { return true; }
-    __device__ int first_unit(int z) const { return fisher ? 0 : z; }
-    __device__ int last_unit(int z) const { return fisher ? S : z + 1; }
-    __device__ long long k_begin(int s) const { return samples ? max(0ll, static_cast<long long>(samples[2 * s])) : 0; }
-    __device__ long long k_end(int s) const { return samples ? min(ck.n, static_cast<long long>(samples[2 * s + 1])) : ck.n; }
-    __device__ float a(long long m, long long t) const { return value(dy, dy_dtype, t * lddy + m); }
-    __device__ float b(long long t, long long n) const { return xhat(ck, t, n); }
-    __device__ void store(int s, long long m, long long n, float g) const {
-        if (fisher) {
-            float* F = fisher + m * N + n;
-            *F = (s == 0 && first_step) ? ema_first(alpha, g) : ema_next(*F, beta, alpha * (1.0f - beta), g);
-        } else if (g_dtype == TB_F32) {
-            static_cast<float*>(grads)[s * g_stride + m * N + n] = g;
+// dy as BF16 parts that add up to it exactly: the leading 8 bits, the next 8
+// and the last (FP32: three, F16: two; BF16 is copied, to aligned rows).  The
+// parts are cut off, not rounded, so the largest finite value stays finite.
+// The last part of a value below 2^-110 can fall below BF16's smallest, 2^-133.
+template <int DT, int PARTS>
+__global__ void __launch_bounds__(256) split_kernel(const void* __restrict__ dy, const long long lddy, const long long n,
+                                                    const int r, const bool vec, uint16_t* __restrict__ out,
+                                                    const long long ldo) {
+    const int groups = static_cast<int>(ldo / 4);
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n * groups; i += gridDim.x * 256ll) {
+        const long long t = i / groups;
+        const int c = static_cast<int>(i % groups) * 4;
+        float v[4];
+        if (vec && c + 4 <= r) {
+            if constexpr (DT == TB_F32) {
+                const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(dy) + t * lddy + c);
+                v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(dy) + t * lddy + c);
+                const uint16_t h[4] = {static_cast<uint16_t>(w.x), static_cast<uint16_t>(w.x >> 16), static_cast<uint16_t>(w.y), static_cast<uint16_t>(w.y >> 16)};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = Elem<DT>::load(h, k);
+            }
         } else {
-            static_cast<__nv_bfloat16*>(grads)[s * g_stride + m * N + n] = __float2bfloat16_rn(g);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = c + k < r ? Elem<DT>::load(dy, t * lddy + c + k) : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            uint16_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t bits = __float_as_uint(v[k]);
+                h[k] = static_cast<uint16_t>(bits >> 16);
+                if ((bits & 0x7FFFFFFFu) > 0x7F800000u) h[k] = 0x7FFFu;  // a NaN stays one
+                v[k] = (bits & 0x7F800000u) == 0x7F800000u ? 0.0f : v[k] - __uint_as_float(bits & 0xFFFF0000u);
+            }
+            *reinterpret_cast<uint2*>(out + (p * n + t) * ldo + c) =
+                make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
         }
     }
-};
-
-struct HessianOp {
-    static constexpr bool kRowA = false, kRowB = true;
-    View ck;
-    long long M, N;
-    float scale;
-    int accumulate;
-    float* H;
-    __device__ bool wanted(long long m0, long long n0) const { return m0 / 128 >= n0 / 128; }
-    __device__ int first_unit(int) const { return 0; }
-    __device__ int last_unit(int) const { return 1; }
-    __device__ long long k_begin(int) const { return 0; }
-    __device__ long long k_end(int) const { return ck.n; }
-    __device__ float a(long long m, long long t) const { return xhat(ck, t, m); }
-    __device__ float b(long long t, long long n) const { return xhat(ck, t, n); }
-    __device__ void store(int, long long m, long long n, float g) const {
-        float* h = H + m * N + n;
-        *h = accumulate ? *h + scale * g : scale * g;
-    }
-};
+}
 
 bool vectors(const void* p, long long ld, int esize) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * esize) % 16 == 0;
@@ -227,6 +209,26 @@ int check_dy(const char* who, const void* dy, int dtype, int64_t lddy, int r, in
         return fail(TB_ERR_ARG, "%s: S must be in 0..65535, and 1 where samples is NULL", who);
     if (n > 0 && S > 0 && (!dy || lddy < r)) return fail(TB_ERR_ARG, "%s: dy is null or lddy < r", who);
     return TB_OK;
+}
+
+// dy in the form that the tensor-core products read; *scratch is freed by the caller.
+int prepare_dy(const View& ck, const void* dy, int dtype, int64_t lddy, int r, cudaStream_t st, linear::Parts* out,
+               void** scratch) {
+    *out = {dy, lddy, 1};
+    if (ck.n == 0) return TB_OK;
+    const bool vec16 = vectors(dy, lddy, dtype == TB_F32 ? 4 : 2);
+    if (dtype == TB_BF16 && vec16) return TB_OK;
+    const int parts = dtype == TB_F32 ? 3 : dtype == TB_F16 ? 2 : 1;
+    const long long ld = (r + 7) / 8 * 8;
+    int rc = scratch_alloc(scratch, static_cast<size_t>(parts) * ck.n * ld * 2, st);
+    if (rc) return rc;
+    uint16_t* p = static_cast<uint16_t*>(*scratch);
+    *out = {p, ld, parts};
+    const unsigned grid = static_cast<unsigned>(std::min<long long>((ck.n * (ld / 4) + 255) / 256, 148 * 16));
+    if (dtype == TB_F32) split_kernel<TB_F32, 3><<<grid, 256, 0, st>>>(dy, lddy, ck.n, r, vec16, p, ld);
+    else if (dtype == TB_F16) split_kernel<TB_F16, 2><<<grid, 256, 0, st>>>(dy, lddy, ck.n, r, vec16, p, ld);
+    else split_kernel<TB_BF16, 1><<<grid, 256, 0, st>>>(dy, lddy, ck.n, r, vec16, p, ld);
+    return check_launch("split_kernel");
 }
 
 }  // namespace
@@ -304,13 +306,17 @@ extern "C" int tb_act8_weight_grad(const tb_act8* ckp, const void* dy, int dy_dt
     if (S == 0) return TB_OK;
     if (!grads) return fail(TB_ERR_ARG, "tb_act8_weight_grad: null gradients");
     if ((rc = require_device(nullptr))) return rc;
-    GradOp op{ck, dy, dy_dtype, lddy, r, ck.d, samples, S, grads, g_dtype, g_stride, nullptr, 0.0f, 0.0f, 0};
-    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (r + 63) / 64, S), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
-    return check_launch("act8 weight gradient");
+    auto st = static_cast<cudaStream_t>(stream);
+    linear::Parts parts{};
+    void* scratch = nullptr;
+    rc = prepare_dy(ck, dy, dy_dtype, lddy, r, st, &parts, &scratch);
+    if (!rc) rc = linear::weight_grad(ck, parts, r, samples, S, grads, g_dtype, g_stride, st);
+    scratch_free(scratch, st);
+    return rc;
 }
 
 extern "C" int tb_act8_fisher(const tb_act8* ckp, const void* dy, int dy_dtype, int64_t lddy, int r,
-                              const int64_t* samples, int S, float alpha, float beta, int first_step, float* fisher,
+                              const int64_t* samples, int S, double alpha, double beta, int first_step, float* fisher,
                               void* stream) {
     View ck;
     int rc = act8::check(ckp, "tb_act8_fisher", &ck);
@@ -319,9 +325,16 @@ extern "C" int tb_act8_fisher(const tb_act8* ckp, const void* dy, int dy_dtype, 
     if (S == 0) return TB_OK;
     if (!fisher) return fail(TB_ERR_ARG, "tb_act8_fisher: null Fisher state");
     if ((rc = require_device(nullptr))) return rc;
-    GradOp op{ck, dy, dy_dtype, lddy, r, ck.d, samples, S, nullptr, TB_F32, 0, fisher, alpha, beta, first_step};
-    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (r + 63) / 64, 1), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
-    return check_launch("act8 Fisher");
+    auto st = static_cast<cudaStream_t>(stream);
+    linear::Parts parts{};
+    void* scratch = nullptr;
+    rc = prepare_dy(ck, dy, dy_dtype, lddy, r, st, &parts, &scratch);
+    // 1 - beta loses a relative 1e-6 where beta is rounded to FP32 first: formed in double, rounded once
+    if (!rc)
+        rc = linear::fisher(ck, parts, r, samples, S, static_cast<float>(alpha), static_cast<float>(beta),
+                            static_cast<float>(alpha * (1.0 - beta)), first_step != 0, fisher, st);
+    scratch_free(scratch, st);
+    return rc;
 }
 
 extern "C" int tb_act8_hessian(const tb_act8* ckp, float scale, int accumulate, float* H, void* stream) {
@@ -330,7 +343,5 @@ extern "C" int tb_act8_hessian(const tb_act8* ckp, float scale, int accumulate, 
     if (rc) return rc;
     if (!H) return fail(TB_ERR_ARG, "tb_act8_hessian: null H");
     if ((rc = require_device(nullptr))) return rc;
-    HessianOp op{ck, ck.d, ck.d, scale, accumulate, H};
-    simple_gemm_kernel<<<dim3((ck.d + 63) / 64, (ck.d + 63) / 64, 1), 256, 0, static_cast<cudaStream_t>(stream)>>>(op);
-    return check_launch("act8 Hessian");
+    return linear::hessian(ck, scale, accumulate != 0, H, static_cast<cudaStream_t>(stream));
 }

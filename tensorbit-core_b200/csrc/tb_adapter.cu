@@ -3,8 +3,8 @@
 #include <algorithm>
 
 #include "tb_act8.cuh"
+#include "tb_linear.cuh"
 #include "tb_runtime.h"
-#include "tb_simple_gemm.cuh"
 
 namespace tb {
 namespace adapter {
@@ -50,45 +50,28 @@ __global__ void skinny_kernel(const Args g, const int mode, float* __restrict__ 
     u[i] = sum;
 }
 
-struct ForwardOp {
-    static constexpr bool kRowA = true, kRowB = false;
-    Args g;
-    const float* u;
-    long long M, N;
-    __device__ bool wanted(long long, long long) const { return true; }
-    __device__ int first_unit(int) const { return 0; }
-    __device__ int last_unit(int) const { return 1; }
-    __device__ long long k_begin(int) const { return 0; }
-    __device__ long long k_end(int) const { return g.d; }
-    __device__ float a(long long m, long long k) const { return __bfloat162float(g.x[m * g.ldx + k]); }
-    __device__ float b(long long k, long long n) const { return __bfloat162float(g.w[n * g.ldw + k]); }
-    __device__ void store(int, long long t, long long o, float y) const {
-        const int a = adapter_of(g, t);
-        if (a >= 0)
-            for (int k = 0; k < g.rank; ++k) y = fmaf(u[t * g.rank + k], __bfloat162float(g.b[(static_cast<long long>(a) * g.r + o) * g.ldb + k]), y);
-        g.y[t * g.ldy + o] = __float2bfloat16_rn(y);
+// The adapters that occur among 256 tokens, in order of first occurrence: the
+// count, then their numbers.
+__global__ void __launch_bounds__(256) list_kernel(const Args g, int32_t* __restrict__ lists) {
+    __shared__ int who[256], count[8];
+    const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
+    const long long t = blockIdx.x * 256ll + i;
+    who[i] = t < g.n ? adapter_of(g, t) : -1;
+    __syncthreads();
+    bool first = who[i] >= 0;
+    for (int j = 0; j < i && first; ++j) first = who[j] != who[i];
+    const unsigned m = __ballot_sync(~0u, first);
+    if (lane == 0) count[warp] = __popc(m);
+    __syncthreads();
+    int at = __popc(m & ((1u << lane) - 1)), total = 0;
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) at += count[w];
+        total += count[w];
     }
-};
-
-struct InputGradOp {
-    static constexpr bool kRowA = true, kRowB = true;
-    Args g;
-    const float* v;
-    long long M, N;
-    __device__ bool wanted(long long, long long) const { return true; }
-    __device__ int first_unit(int) const { return 0; }
-    __device__ int last_unit(int) const { return 1; }
-    __device__ long long k_begin(int) const { return 0; }
-    __device__ long long k_end(int) const { return g.r; }
-    __device__ float a(long long m, long long k) const { return __bfloat162float(g.dy[m * g.lddy + k]); }
-    __device__ float b(long long k, long long n) const { return __bfloat162float(g.w[k * g.ldw + n]); }
-    __device__ void store(int, long long t, long long c, float x) const {
-        const int a = adapter_of(g, t);
-        if (a >= 0)
-            for (int k = 0; k < g.rank; ++k) x = fmaf(v[t * g.rank + k], __bfloat162float(g.a[(static_cast<long long>(a) * g.rank + k) * g.lda + c]), x);
-        g.dx[t * g.lddx + c] = __float2bfloat16_rn(x);
-    }
-};
+    int32_t* out = lists + static_cast<long long>(blockIdx.x) * linear::kListPitch;
+    if (i == 0) out[0] = total;
+    if (first) out[1 + at] = who[i];
+}
 
 // da[a][k][c] = sum v[t][k] xhat[t][c]  (blockIdx.z = a, blockIdx.y = k)
 __global__ void grad_a_kernel(const Args g, const float* __restrict__ v) {
@@ -106,6 +89,24 @@ __global__ void grad_b_kernel(const Args g, const float* __restrict__ u) {
     for (long long t = 0; t < g.n; ++t)
         if (adapter_of(g, t) == a) sum = fmaf(u[t * g.rank + k], __bfloat162float(g.dy[t * g.lddy + o]), sum);
     g.db[(static_cast<long long>(a) * g.r + o) * g.ldb + k] = __float2bfloat16_rn(sum);
+}
+
+// One piece of scratch: the lists, u and v (freed through `lists`).  Empty without adapters or tokens.
+struct Scratch {
+    int32_t* lists;
+    float *u, *v;
+};
+int make_scratch(const Args& g, bool both, cudaStream_t st, Scratch* s) {
+    if (!g.na || !g.n) return TB_OK;
+    const size_t list = ((g.n + 255) / 256 * linear::kListPitch * sizeof(int32_t) + 255) / 256 * 256;
+    const size_t vals = (g.n * g.rank * sizeof(float) + 255) / 256 * 256;
+    void* p = nullptr;
+    const int rc = scratch_alloc(&p, list + (both ? 2 : 1) * vals, st);
+    if (rc) return rc;
+    s->lists = static_cast<int32_t*>(p);
+    s->v = reinterpret_cast<float*>(static_cast<char*>(p) + list);
+    s->u = both ? reinterpret_cast<float*>(reinterpret_cast<char*>(s->v) + vals) : s->v;
+    return TB_OK;
 }
 
 bool bad_rows(const void* p, int64_t ld, int64_t cols) {
@@ -162,15 +163,15 @@ extern "C" int tb_adapter_forward(const tb_adapter_args* p, void* stream) {
     g.ldy = p->ldy;
     if ((rc = require_device(nullptr))) return rc;
     auto st = static_cast<cudaStream_t>(stream);
-    float* u = nullptr;
+    Scratch s{};
+    if ((rc = make_scratch(g, false, st, &s))) return rc;
     if (g.na) {
-        if ((rc = scratch_alloc(reinterpret_cast<void**>(&u), g.n * g.rank * sizeof(float), st))) return rc;
-        skinny_kernel<<<static_cast<unsigned>((g.n * g.rank + 255) / 256), 256, 0, st>>>(g, 0, u);
+        skinny_kernel<<<static_cast<unsigned>((g.n * g.rank + 255) / 256), 256, 0, st>>>(g, 0, s.u);
+        list_kernel<<<static_cast<unsigned>((g.n + 255) / 256), 256, 0, st>>>(g, s.lists);
+        rc = check_launch("adapter down projection");
     }
-    ForwardOp op{g, u, g.n, g.r};
-    simple_gemm_kernel<<<dim3((g.r + 63) / 64, static_cast<unsigned>((g.n + 63) / 64)), 256, 0, st>>>(op);
-    rc = check_launch("adapter forward");
-    scratch_free(u, st);
+    if (!rc) rc = linear::adapter_forward({g.n, g.r, g.d, g.x, g.ldx, g.w, g.ldw, g.y, g.ldy, g.who, s.lists, s.u, g.b, g.ldb, g.rank, g.na}, st);
+    scratch_free(s.lists, st);
     return rc;
 }
 
@@ -194,24 +195,22 @@ extern "C" int tb_adapter_backward(const tb_adapter_args* p, void* stream) {
     g.db = static_cast<bf16*>(p->db);
     if ((rc = require_device(nullptr))) return rc;
     auto st = static_cast<cudaStream_t>(stream);
-    float *u = nullptr, *v = nullptr;
-    if (g.na && g.n) {
-        const size_t bytes = g.n * g.rank * sizeof(float);
-        if ((rc = scratch_alloc(reinterpret_cast<void**>(&v), 2 * bytes, st))) return rc;
-        u = v + g.n * g.rank;
+    Scratch s{};
+    if ((rc = make_scratch(g, grads, st, &s))) return rc;
+    if (s.lists) {
         const unsigned grid = static_cast<unsigned>((g.n * g.rank + 255) / 256);
-        skinny_kernel<<<grid, 256, 0, st>>>(g, 2, v);
-        if (grads) skinny_kernel<<<grid, 256, 0, st>>>(g, 1, u);
+        skinny_kernel<<<grid, 256, 0, st>>>(g, 2, s.v);
+        if (grads) skinny_kernel<<<grid, 256, 0, st>>>(g, 1, s.u);
+        list_kernel<<<static_cast<unsigned>((g.n + 255) / 256), 256, 0, st>>>(g, s.lists);
+        rc = check_launch("adapter down projection");
     }
-    if (g.dx && g.n) {
-        InputGradOp op{g, v, g.n, g.d};
-        simple_gemm_kernel<<<dim3((g.d + 63) / 64, static_cast<unsigned>((g.n + 63) / 64)), 256, 0, st>>>(op);
+    if (!rc && g.dx && g.n)
+        rc = linear::adapter_input_grad({g.n, g.d, g.r, g.dy, g.lddy, g.w, g.ldw, g.dx, g.lddx, g.who, s.lists, s.v, g.a, g.lda, g.rank, g.na}, st);
+    if (!rc && grads) {
+        grad_a_kernel<<<dim3((g.d + 255) / 256, g.rank, g.na), 256, 0, st>>>(g, s.v);
+        grad_b_kernel<<<dim3((g.r + 255) / 256, g.rank, g.na), 256, 0, st>>>(g, s.u);
+        rc = check_launch("adapter gradients");
     }
-    if (grads) {
-        grad_a_kernel<<<dim3((g.d + 255) / 256, g.rank, g.na), 256, 0, st>>>(g, v);
-        grad_b_kernel<<<dim3((g.r + 255) / 256, g.rank, g.na), 256, 0, st>>>(g, u);
-    }
-    rc = check_launch("adapter backward");
-    scratch_free(v, st);
+    scratch_free(s.lists, st);
     return rc;
 }

@@ -1,0 +1,819 @@
+// Products of the calibration operators on tcgen05 tensor cores (sm_100a).
+//
+// One persistent kernel skeleton, instantiated per mode.  A pair of CTAs
+// (cta_group::2) owns a 256 x NB output tile: each CTA holds its 128 rows of A
+// and NB/2 of the B columns of a K slice in shared memory, and its 128 x NB
+// half of the accumulator in TMEM.  Roles of a CTA's 16 warps:
+//   warp 12      TMA loads of K slices into a ring of stages;
+//   warps 8-11   "prepare" a stage: decode int8 codes to the BF16 operand,
+//                zero what lies behind a sample's end, or build the operands of
+//                an adapter; then tell the even CTA that the stage is ready;
+//   warp 13      (even CTA) issues tcgen05.mma for both CTAs;
+//   warps 0-7    take finished accumulators out of TMEM and store results.
+// The accumulator is double buffered, so the next sums run while a tile is
+// stored.  The tensor core's own additions truncate: the modes with FP32
+// results accumulate short groups of K in TMEM and add those into FP32
+// registers with round to nearest.  That needs 128 accumulators a thread, so
+// these modes move registers from the other roles to the epilogue's warps.
+//
+// Modes:
+//   kGrad    G_s = dY_s^T Xhat_s: A = dY (M-major by TMA), B = decoded codes
+//   kFisher  the same with the EMA of g^2 in registers, samples in order
+//   kHess    Xhat^T Xhat on int8 tensor cores: the codes of a block of 128
+//            tokens multiply exactly into int32, and the block's two
+//            power-of-two scales enter when its sum is added in FP32
+//   kFwd     X W^T, kDx: dY W, with one extra K slice of 64 for every 32 ranks
+//            of an adapter present in the tile: [u_hi | u_lo] of its tokens
+//            (zero for the others) times [E | E]
+// Every wait is bounded; on expiry the kernel records an error and leaves.
+#include <algorithm>
+#include <mutex>
+
+#include "tb_device.cuh"
+#include "tb_linear.cuh"
+#include "tb_runtime.h"
+#include "tb_tcgen05.cuh"
+
+namespace tb {
+namespace linear {
+namespace {
+
+using namespace tb::umma;
+using bf16 = __nv_bfloat16;
+
+enum Mode { kGrad = 0, kFisher = 1, kHess = 2, kFwd = 3, kDx = 4 };
+
+__device__ int g_linear_error;
+
+constexpr int kThreads = 512;
+constexpr int kEpiWarps = 8, kPrepWarp = 8, kTmaWarp = 12, kMmaWarp = 13;
+
+template <int MODE>
+struct Cfg {
+    static constexpr bool kCodes = MODE == kGrad || MODE == kFisher;   // B from codes
+    static constexpr bool kAdapter = MODE == kFwd || MODE == kDx;
+    static constexpr bool kPromote = !kAdapter;
+    static constexpr int NB = MODE == kFisher ? 128 : 256;             // columns of a pair's tile
+    static constexpr int kCols = NB / 2;                               // columns of an epilogue warp, and of a CTA's B
+    // K slices summed in TMEM before they are added in FP32: 256 tokens, or one block of codes
+    static constexpr int kGroup = kCodes ? 4 : MODE == kHess ? 1 : 1 << 30;
+    static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
+    static constexpr int kB = MODE == kHess ? 16384 : kCols * 128;
+    static constexpr int kRaw = kCodes ? 64 * kCols : 0;
+    static constexpr int kStage = kA + kB + kRaw;
+    static constexpr int kStages = MODE == kGrad ? 5 : MODE == kFisher ? 7 : 6;
+    static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
+    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kColScale + 1024 + 512;
+};
+
+struct Params {
+    long long M, N, K;
+    int tiles_m, tiles_n, items;
+    // checkpoint and samples
+    const uint8_t* exps;
+    long long lde, n;
+    const int64_t* samples;
+    int S, parts;
+    // results
+    void* out;
+    long long ldo, out_stride;
+    int out_bf16;
+    float alpha, beta, contrib, scale;
+    int first, accumulate;
+    // adapters
+    AdapterProduct ad;
+};
+
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer();
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (globaltimer() - t0 > kWaitNs) return false;
+    }
+}
+__device__ __forceinline__ void arrive_even(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar & kPeerMask) : "memory");
+}
+template <int MODE>
+__device__ __forceinline__ void mma_step(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (MODE == kHess)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+            ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+            ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
+}
+// 128-byte-swizzle operand descriptors.  K-major: 8-row atoms 1024 bytes apart.
+// MN-major: rows of K are 128 bytes of M or N, 8-row atoms 1024 bytes apart
+// along K, the next 128 bytes of M or N `kMnChunk` further.
+constexpr int kMnChunk = 64 * 128;
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
+    const uint64_t lbo = mn ? kMnChunk >> 4 : 1;
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (lbo << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two int8 codes in the low bytes of v's halves (the high bytes 0x43) times two
+// BF16 scales.  0x4300 | low7 is 128 + low7 and 0x4300 | sign is 128 or 256, so
+// their difference is the signed code; both steps are exact.
+__device__ __forceinline__ uint32_t decode2(uint32_t v, uint32_t scale2) {
+    const uint32_t hi = v & 0xFF7FFF7Fu, lo = v & 0xFF80FF80u;
+    const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
+    const __nv_bfloat162 x = __hmul2(q, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// ---- the walk over work items, units (one sum each) and K slices that every role shares ----
+struct Tile {
+    int tm, tn, s;
+};
+struct Unit {
+    long long lo, hi;   // K range
+    int slices;         // K slices of one part
+    int total;          // all slices
+    int rslices;        // adapters: slices of one adapter
+    const int32_t* list;
+};
+
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const Params& P, int item) {
+    Tile t{0, 0, 0};
+    if constexpr (MODE == kHess) {  // lower triangle, row by row
+        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(item) + 1.0f) - 1.0f) * 0.5f);
+        while (tm * (tm + 1) / 2 > item) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= item) ++tm;
+        t.tm = tm;
+        t.tn = item - tm * (tm + 1) / 2;
+    } else {
+        const int tiles = P.tiles_m * P.tiles_n;
+        if constexpr (MODE == kGrad) t.s = item / tiles;
+        const int i = item % tiles;
+        // bands of 8 tile rows, column by column inside, so that concurrent tiles share operands in L2
+        const int band = i / (8 * P.tiles_n), in = i % (8 * P.tiles_n);
+        const int rows = min(8, P.tiles_m - 8 * band);
+        t.tm = 8 * band + in % rows;
+        t.tn = in / rows;
+    }
+    return t;
+}
+
+template <int MODE>
+__device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
+    Unit u{0, P.K, 0, 0, 1, nullptr};
+    if constexpr (Cfg<MODE>::kCodes) {
+        if (P.samples) {
+            u.lo = max(0ll, static_cast<long long>(__ldg(P.samples + 2 * s)));
+            u.hi = max(u.lo, min(P.n, static_cast<long long>(__ldg(P.samples + 2 * s + 1))));
+        } else {
+            u.hi = P.n;
+        }
+        u.slices = static_cast<int>((u.hi - u.lo + 63) / 64);
+        u.total = u.slices * P.parts;
+    } else if constexpr (MODE == kHess) {
+        u.hi = P.n;
+        u.total = u.slices = static_cast<int>((P.n + 127) / 128);
+    } else {
+        u.total = u.slices = static_cast<int>((P.K + 63) / 64);
+        if (P.ad.lists) {
+            u.list = P.ad.lists + static_cast<long long>(t.tm) * kListPitch;
+            u.rslices = (P.ad.rank + 31) / 32;
+            u.total += __ldg(u.list) * u.rslices;
+        }
+    }
+    return u;
+}
+
+// Calls f(tile, unit, j) for every slice of this pair's items until it returns false.
+template <int MODE, class F>
+__device__ __forceinline__ bool walk(const Params& P, F&& f) {
+    for (int item = blockIdx.x >> 1; item < P.items; item += gridDim.x >> 1) {
+        const Tile t = tile_of<MODE>(P, item);
+        const int s1 = MODE == kFisher ? P.S : t.s + 1;
+        for (int s = t.s; s < s1; ++s) {
+            const Unit u = unit_of<MODE>(P, t, s);
+            for (int j = 0; j < u.total; ++j)
+                if (!f(t, u, j)) return false;
+        }
+    }
+    return true;
+}
+
+// ---- stores of one row's run of columns ------------------------------------------
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+template <int COLS>
+__device__ __forceinline__ void store_f32(float* p, const float (&v)[COLS], int valid) {
+    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+        for (int c = 0; c < COLS / 8; ++c) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * c + i]);
+            st_global32(p + 8 * c, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i)
+            if (i < valid) p[i] = v[i];
+    }
+}
+template <int COLS>
+__device__ __forceinline__ void store_bf16(bf16* p, const float (&v)[COLS], int valid) {
+    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+        for (int c = 0; c < COLS / 16; ++c) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[16 * c + 2 * i], v[16 * c + 2 * i + 1]);
+            st_global32(p + 16 * c, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i)
+            if (i < valid) p[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+// One result of an adapter product on its own.  An adapter's operands are zero
+// for the other tokens of its tile, but zero times an infinity or a NaN of that
+// adapter is not: a result that is not finite is formed again from what belongs
+// to its token alone.
+template <int MODE>
+__device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, long long o) {
+    float y = 0.0f;
+    for (int k = 0; k < p.K; ++k)
+        y = fmaf(__bfloat162float(p.in[t * p.ldin + k]),
+                 __bfloat162float(MODE == kFwd ? p.w[o * p.ldw + k] : p.w[k * p.ldw + o]), y);
+    const int a = p.who[t];
+    if (a >= 0 && a < p.na)
+        for (int j = 0; j < p.rank; ++j)
+            y = fmaf(p.u[t * p.rank + j],
+                     __bfloat162float(MODE == kFwd ? p.e[(static_cast<long long>(a) * p.N + o) * p.lde + j]
+                                                   : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o]),
+                     y);
+    return y;
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CUtensorMap tB,
+              const __grid_constant__ Params P) {
+    using C = Cfg<MODE>;
+    constexpr int NB = C::NB, kStages = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* col_scale = reinterpret_cast<float*>(smem + kStages * C::kStage);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * C::kStage + C::kColScale);
+    uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
+    uint64_t* empty = ready + kStages;    // stage read by the MMAs
+    uint64_t* accfull = empty + kStages;  // [2] accumulator finished
+    uint64_t* accempty = accfull + 2;     // [2] (even CTA) accumulator taken by both CTAs
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank());
+
+    if (threadIdx.x == kTmaWarp * 32 && P.n > 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tA)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tB)) : "memory");
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&ready[s]), 8);  // four prepare warps of each CTA
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&accfull[b]), 1);
+            mbar_init(smem_u32(&accempty[b]), 2 * kEpiWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(2 * NB));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    fence_before();
+    cluster_sync_all();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto stage_a = [&](int s) { return smem_u32(smem + s * C::kStage); };
+    auto stage_b = [&](int s) { return smem_u32(smem + s * C::kStage + C::kA); };
+    auto stage_raw = [&](int s) { return smem_u32(smem + s * C::kStage + C::kA + C::kB); };
+
+    // Register shares of the promoting modes: 8 warps x 200 + 8 warps x 56 = the launch's 16 x 128.
+    if (warp < kEpiWarps) {
+        if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        constexpr int COLS = C::kCols;
+        const int quad = warp & 3, half = warp >> 2;
+        const int row_in = rank * 128 + quad * 32 + lane;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * COLS);
+        bool ok = true;
+        int gc = 0;  // accumulator uses so far
+        for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
+            const Tile t = tile_of<MODE>(P, item);
+            const long long row = static_cast<long long>(t.tm) * 256 + row_in;
+            const long long col = static_cast<long long>(t.tn) * NB + half * COLS;
+            const int valid = row < P.M ? static_cast<int>(max(0ll, min(static_cast<long long>(COLS), P.N - col))) : 0;
+            if constexpr (C::kAdapter) {
+                const Unit u = unit_of<MODE>(P, t, 0);
+                const int b = gc & 1;
+                if (!mbar_wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
+                fence_after();
+                ++gc;
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    float v[32];
+                    tmem_ld32(lane_base + static_cast<uint32_t>(b * NB + c * 32), v);
+                    if (u.list) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < valid - 32 * c && !(fabsf(v[i]) <= 3.402823466e38f)) v[i] = lone_result<MODE>(P.ad, row, col + 32 * c + i);
+                    }
+                    store_bf16<32>(static_cast<bf16*>(P.out) + row * P.ldo + col + 32 * c, v, valid - 32 * c);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_even(smem_u32(&accempty[b]));
+            } else {
+                float F[MODE == kFisher ? COLS : 1];
+                if constexpr (MODE == kFisher) {
+                    const float* src = static_cast<const float*>(P.out) + row * P.ldo + col;
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i) F[i] = (!P.first && i < valid) ? src[i] : 0.0f;
+                }
+                const int s1 = MODE == kFisher ? P.S : t.s + 1;
+                for (int s = t.s; s < s1 && ok; ++s) {
+                    const Unit u = unit_of<MODE>(P, t, s);
+                    const int groups = (u.total + C::kGroup - 1) / C::kGroup;
+                    float acc[COLS];
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+                    float* scol = col_scale + warp * 2 * COLS;
+                    // kHess: exponent bytes of this lane's row and of four of the warp's columns, one group ahead
+                    uint32_t er = 0, ec = 0;
+                    auto load_exps = [&](int g) {
+                        if constexpr (MODE == kHess) {
+                            const uint8_t* e = P.exps + g * P.lde;
+                            er = row < P.M ? e[row] : 0u;
+                            ec = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (4 * lane + i < min(static_cast<long long>(COLS), P.N - col)) ec |= static_cast<uint32_t>(e[col + 4 * lane + i]) << (8 * i);
+                        }
+                    };
+                    if (groups > 0) load_exps(0);
+                    for (int g = 0; g < groups; ++g) {
+                        float srow = 0.0f;
+                        if constexpr (MODE == kHess) {
+                            srow = act8::scale_f32(er);
+                            float4 f = make_float4(act8::scale_f32(ec & 0xFF), act8::scale_f32((ec >> 8) & 0xFF),
+                                                   act8::scale_f32((ec >> 16) & 0xFF), act8::scale_f32(ec >> 24));
+                            __syncwarp();
+                            *reinterpret_cast<float4*>(scol + (g & 1) * COLS + 4 * lane) = f;
+                            __syncwarp();
+                            if (g + 1 < groups) load_exps(g + 1);
+                        }
+                        const int b = gc & 1;
+                        if (!mbar_wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
+                        fence_after();
+                        ++gc;
+#pragma unroll
+                        for (int c = 0; c < COLS / 32; ++c) {
+                            float v[32];
+                            tmem_ld32(lane_base + static_cast<uint32_t>(b * NB + c * 32), v);
+                            if constexpr (MODE == kHess) {
+                                // |block sum| <= 128 * 127^2 < 2^22: as the low bits of 1.5 * 2^23 it is an
+                                // exact FP32 value, and subtracting that base times the row's power of two too
+                                const float base = -12582912.0f * srow;
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) {
+                                    const float4 sc = *reinterpret_cast<const float4*>(scol + (g & 1) * COLS + c * 32 + 4 * q);
+                                    const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const float m = __uint_as_float(0x4B400000u + __float_as_uint(v[4 * q + i]));
+                                        const float x = fmaf(m, srow, base);
+                                        acc[c * 32 + 4 * q + i] = fmaf(x, s4[i], acc[c * 32 + 4 * q + i]);
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) acc[c * 32 + i] = __fadd_rn(acc[c * 32 + i], v[i]);
+                            }
+                        }
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_even(smem_u32(&accempty[b]));
+                    }
+                    if (!ok) break;
+                    if constexpr (MODE == kFisher) {
+                        const bool first = P.first && s == 0;
+#pragma unroll
+                        for (int i = 0; i < COLS; ++i) F[i] = first ? ema_first(P.alpha, acc[i]) : ema_next(F[i], P.beta, P.contrib, acc[i]);
+                    } else if constexpr (MODE == kGrad) {
+                        const long long at = t.s * P.out_stride + row * P.ldo + col;
+                        if (P.out_bf16) store_bf16<COLS>(static_cast<bf16*>(P.out) + at, acc, valid);
+                        else store_f32<COLS>(static_cast<float*>(P.out) + at, acc, valid);
+                    } else if (col / 128 <= row / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
+                        float* h = static_cast<float*>(P.out) + row * P.ldo + col;
+#pragma unroll
+                        for (int i = 0; i < COLS; ++i) acc[i] = P.accumulate && i < valid ? __fadd_rn(h[i], P.scale * acc[i]) : P.scale * acc[i];
+                        store_f32<COLS>(h, acc, valid);
+                    }
+                }
+                if constexpr (MODE == kFisher)
+                    if (ok) store_f32<COLS>(static_cast<float*>(P.out) + row * P.ldo + col, F, valid);
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            if (lane == 0) atomicExch(&g_linear_error, 1);
+        }
+    } else {
+        if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == kTmaWarp) {
+            if (lane == 0) {
+                int it = 0;
+                const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j) {
+                    const int s = it % kStages;
+                    if (it >= kStages && !mbar_wait(smem_u32(&empty[s]), ((it / kStages) - 1) & 1)) return false;
+                    if (*abort_flag) return false;
+                    const uint32_t bar = smem_u32(&full[s]);
+                    const int m0 = t.tm * 256 + rank * 128, n0 = t.tn * NB + rank * C::kCols;
+                    if (C::kAdapter && j >= u.slices) {  // the prepare warps fill this stage
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+                    } else if constexpr (C::kCodes) {
+                        const int part = j / u.slices;
+                        const int k = static_cast<int>(u.lo) + (j % u.slices) * 64;
+                        const int y = static_cast<int>(part * P.n) + k;
+                        mbar_expect_tx(bar, C::kA + C::kRaw);
+                        tma_load_2d(stage_a(s), &tA, m0, y, bar);
+                        tma_load_2d(stage_a(s) + kMnChunk, &tA, m0 + 64, y, bar);
+                        tma_load_2d(stage_raw(s), &tB, n0, k, bar);
+                    } else if constexpr (MODE == kHess) {
+                        mbar_expect_tx(bar, C::kA + C::kB);
+                        tma_load_2d(stage_a(s), &tA, m0, j * 128, bar);
+                        tma_load_2d(stage_b(s), &tB, n0, j * 128, bar);
+                    } else {
+                        mbar_expect_tx(bar, C::kA + C::kB);
+                        tma_load_2d(stage_a(s), &tA, j * 64, m0, bar);
+                        if constexpr (MODE == kFwd) {
+                            tma_load_2d(stage_b(s), &tB, j * 64, n0, bar);
+                        } else {
+                            tma_load_2d(stage_b(s), &tB, n0, j * 64, bar);
+                            tma_load_2d(stage_b(s) + kMnChunk, &tB, n0 + 64, j * 64, bar);
+                        }
+                    }
+                    ++it;
+                    return true;
+                });
+                if (!done) {
+                    *abort_flag = 1;
+                    for (int i = std::max(0, it - kStages); i < it; ++i)  // loads in flight, each waited for within a limit
+                        mbar_wait(smem_u32(&full[i % kStages]), (i / kStages) & 1);
+                }
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp) {
+            if (lane == 0 && rank == 0) {
+                constexpr bool kAmn = C::kCodes || MODE == kHess, kBmn = kAmn || MODE == kDx;
+                constexpr uint32_t kIdesc = ((MODE == kHess ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) |
+                                            (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((NB >> 3) << 17) | (16u << 24);
+                // descriptor steps of one MMA: K-major 32 bytes along a row; MN-major 16 (int8: 32) rows of 128 bytes
+                constexpr uint64_t kStepMn = MODE == kHess ? 4096 >> 4 : 2048 >> 4;
+                constexpr uint64_t kStepA = kAmn ? kStepMn : 2, kStepB = kBmn ? kStepMn : 2;
+                int it = 0, gc = 0;
+                const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int j) {
+                    const bool first = j % C::kGroup == 0;
+                    const int b = gc & 1;
+                    if (first) {
+                        if (gc >= 2 && !wait_cluster(smem_u32(&accempty[b]), ((gc >> 1) - 1) & 1)) return false;
+                    }
+                    const int s = it % kStages;
+                    if (*abort_flag || !wait_cluster(smem_u32(&ready[s]), (it / kStages) & 1)) return false;
+                    fence_after();
+                    const uint64_t a0 = operand_desc(stage_a(s), kAmn), b0 = operand_desc(stage_b(s), kBmn);
+                    const uint32_t d = tmem + static_cast<uint32_t>(b * NB);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_step<MODE>(d, a0 + kk * kStepA, b0 + kk * kStepB, kIdesc, !(first && kk == 0));
+                    commit_pair(smem_u32(&empty[s]));
+                    ++it;
+                    if (j + 1 == u.total || j % C::kGroup == C::kGroup - 1) {
+                        commit_pair(smem_u32(&accfull[b]));
+                        ++gc;
+                    }
+                    return true;
+                });
+                if (!done) {
+                    *abort_flag = 1;
+                    commit_pair(smem_u32(&accfull[0]));  // releases the waiting epilogues
+                    commit_pair(smem_u32(&accfull[1]));
+                }
+            }
+            __syncwarp();
+        } else if (warp >= kPrepWarp && warp < kTmaWarp) {
+            const int pt = threadIdx.x - kPrepWarp * 32;
+            int it = 0;
+            // kCodes: 8 consecutive features of every kRowStep-th token
+            constexpr int kLanesRow = C::kCodes ? C::kCols / 8 : 16, kRowStep = 128 / kLanesRow;
+            const int pc = pt % kLanesRow, pr = pt / kLanesRow;
+            uint2 e0 = make_uint2(0, 0), e1 = make_uint2(0, 0);
+            const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j) {
+                const int s = it % kStages;
+                const int n0 = t.tn * NB + rank * C::kCols;
+                int k0 = 0;
+                if constexpr (C::kCodes) {
+                    k0 = static_cast<int>(u.lo) + (j % u.slices) * 64;
+                    // the exponents of the slice's first and last token's blocks, fetched before the wait
+                    const long long f = n0 + 8 * pc;
+                    const int b0 = k0 >> 7, b1 = (static_cast<int>(min(u.hi, k0 + 64ll)) - 1) >> 7;
+                    if (f < P.N) {
+                        e0 = __ldg(reinterpret_cast<const uint2*>(P.exps + b0 * P.lde + f));
+                        e1 = b1 == b0 ? e0 : __ldg(reinterpret_cast<const uint2*>(P.exps + b1 * P.lde + f));
+                    }
+                }
+                if (*abort_flag || !mbar_wait(smem_u32(&full[s]), (it / kStages) & 1)) return false;
+                if constexpr (C::kCodes) {
+                    const int valid = static_cast<int>(min(64ll, u.hi - k0));
+                    const int border = (((k0 >> 7) + 1) << 7) - k0;  // first row of the second block
+                    uint32_t s0[4], s1[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = (i < 2 ? e0.x : e0.y) >> (16 * (i & 1)), y = (i < 2 ? e1.x : e1.y) >> (16 * (i & 1));
+                        s0[i] = act8::scale_bf16(x & 0xFF) | act8::scale_bf16((x >> 8) & 0xFF) << 16;
+                        s1[i] = act8::scale_bf16(y & 0xFF) | act8::scale_bf16((y >> 8) & 0xFF) << 16;
+                    }
+                    const uint32_t raw = stage_raw(s), dst = stage_b(s) + (pc >> 3) * kMnChunk;
+#pragma unroll
+                    for (int i = 0; i < 64 / kRowStep; ++i) {
+                        const int k = pr + i * kRowStep;
+                        uint2 w;
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(raw + k * C::kCols + pc * 8));
+                        const bool second = k >= border;
+                        uint4 o;
+                        o.x = decode2(prmt(w.x, 0x43434343u, 0x4140u), second ? s1[0] : s0[0]);
+                        o.y = decode2(prmt(w.x, 0x43434343u, 0x4342u), second ? s1[1] : s0[1]);
+                        o.z = decode2(prmt(w.y, 0x43434343u, 0x4140u), second ? s1[2] : s0[2]);
+                        o.w = decode2(prmt(w.y, 0x43434343u, 0x4342u), second ? s1[3] : s0[3]);
+                        if (k >= valid) o = make_uint4(0, 0, 0, 0);
+                        st_shared16(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4), o);
+                    }
+                    // tokens behind the sample's end: dY may hold anything there
+                    for (int i = pt; i < (64 - valid) * 16; i += 128)
+                        st_shared16(stage_a(s) + (i & 1) * kMnChunk + (valid + (i >> 4)) * 128 + ((i >> 1) & 7) * 16, make_uint4(0, 0, 0, 0));
+                } else if constexpr (C::kAdapter) {
+                    if (j >= u.slices) {
+                        const int x = j - u.slices;
+                        const int a = __ldg(u.list + 1 + x / u.rslices), r0 = (x % u.rslices) * 32;
+                        const int nr = min(32, P.ad.rank - r0);
+                        // A: this token's u as two BF16 parts, zero unless the adapter is its own
+                        const long long tok = static_cast<long long>(t.tm) * 256 + rank * 128 + pt;
+                        const bool mine = tok < P.M && __ldg(P.ad.who + tok) == a;
+                        const float* up = P.ad.u + tok * P.ad.rank + r0;
+                        const uint32_t arow = stage_a(s) + pt * 128;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int j0 = 8 * q + 2 * i;
+                                const float f0 = mine && j0 < nr ? up[j0] : 0.0f, f1 = mine && j0 + 1 < nr ? up[j0 + 1] : 0.0f;
+                                hi[i] = pack_bf16(f0, f1);
+                                lo[i] = pack_bf16(f0 - __uint_as_float(hi[i] << 16), f1 - __uint_as_float(hi[i] & 0xFFFF0000u));
+                            }
+                            st_shared16(arow + ((q ^ (pt & 7)) << 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                            st_shared16(arow + (((q + 4) ^ (pt & 7)) << 4), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                        }
+                        if constexpr (MODE == kFwd) {  // B: a row of b per output column, twice
+                            const long long o = n0 + pt;
+                            const uint16_t* bp = reinterpret_cast<const uint16_t*>(P.ad.e) + (static_cast<long long>(a) * P.N + o) * P.ad.lde + r0;
+                            const uint32_t brow = stage_b(s) + pt * 128;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t w[4] = {0, 0, 0, 0};
+                                if (o < P.N && 8 * q < nr) {
+                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(bp + 8 * q));
+                                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const int j0 = 8 * q + 2 * i;
+                                        w[i] = j0 + 1 < nr ? in[i] : j0 < nr ? in[i] & 0xFFFFu : 0u;
+                                    }
+                                }
+                                const uint4 v4 = make_uint4(w[0], w[1], w[2], w[3]);
+                                st_shared16(brow + ((q ^ (pt & 7)) << 4), v4);
+                                st_shared16(brow + (((q + 4) ^ (pt & 7)) << 4), v4);
+                            }
+                        } else {  // B: rows of a, the ranks along K, twice
+                            const int c = pt & 15;
+                            const long long f = n0 + 8 * c;
+                            const uint32_t dst = stage_b(s) + (c >> 3) * kMnChunk;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int k = (pt >> 4) + 8 * i;
+                                uint4 v = make_uint4(0, 0, 0, 0);
+                                if (f < P.N && k < nr)
+                                    v = __ldg(reinterpret_cast<const uint4*>(P.ad.e + (static_cast<long long>(a) * P.ad.rank + r0 + k) * P.ad.lde + f));
+                                const uint32_t unit = ((c & 7) ^ (k & 7)) << 4;
+                                st_shared16(dst + k * 128 + unit, v);
+                                st_shared16(dst + (k + 32) * 128 + unit, v);
+                            }
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive_even(smem_u32(&ready[s]));
+                ++it;
+                return true;
+            });
+            if (!done) *abort_flag = 1;
+        }
+    }
+    fence_before();
+    cluster_sync_all();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NB));
+    }
+}
+
+// Row-major [rows][cols] of `esize`-byte elements, boxes of box_cols x box_rows.
+int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long long rows, long long ld, int box_cols,
+             int box_rows, bool swizzle) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return fail(TB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esize};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(map, esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+                           const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+}
+
+template <int MODE>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& P, cudaStream_t st) {
+    using C = Cfg<MODE>;
+    // Per device: the shared-memory limit, and that the launch has the registers that the roles' shares add up to.
+    static std::mutex mu;
+    static uint64_t prepared = 0;
+    int dev = 0;
+    int rc = require_device(&dev);
+    if (rc) return rc;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 64 || !(prepared >> dev & 1)) {
+            cudaFuncAttributes fa{};
+            cudaError_t e = cudaFuncGetAttributes(&fa, linear_kernel<MODE>);
+            if (e == cudaSuccess && C::kPromote && fa.numRegs != 128)
+                return fail(TB_ERR_CUDA, "linear_kernel<%d> has %d registers a thread, not 128", MODE, fa.numRegs);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(linear_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+            if (e != cudaSuccess) return cuda_fail(e, "linear_kernel setup");
+            if (dev < 64) prepared |= 1ull << dev;
+        }
+    }
+    constexpr int kPairs = 74;  // one CTA on each of the 148 SMs
+    const int pairs = std::min(P.items, kPairs);
+    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, P);
+    return check_launch("linear_kernel");
+}
+
+int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
+
+// Items are counted in 32 bits.
+int set_items(Params* P, long long items, const char* who) {
+    if (items > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, items);
+    P->items = static_cast<int>(items);
+    return TB_OK;
+}
+
+template <int MODE>
+int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long long samples, const char* who, cudaStream_t st) {
+    using C = Cfg<MODE>;
+    if (ck.n * dy.parts > 0x7FFFFFFFll - 64) return fail(TB_ERR_CAPACITY, "%s: %lld tokens in %d parts", who, ck.n, dy.parts);
+    P.M = r;
+    P.N = ck.d;
+    P.tiles_m = tiles(r, 256);
+    P.tiles_n = tiles(ck.d, C::NB);
+    P.exps = ck.exps;
+    P.lde = ck.lde;
+    P.n = ck.n;
+    P.parts = dy.parts;
+    P.ldo = ck.d;
+    int rc = set_items(&P, static_cast<long long>(P.tiles_m) * P.tiles_n * samples, who);
+    CUtensorMap a{}, b{};
+    if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
+    if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
+    return rc ? rc : launch<MODE>(a, b, P, st);
+}
+
+}  // namespace
+
+int weight_grad(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, void* grads, int g_dtype,
+                long long g_stride, cudaStream_t st) {
+    Params P{};
+    P.samples = samples;
+    P.S = S;
+    P.out = grads;
+    P.out_bf16 = g_dtype == TB_BF16;
+    P.out_stride = g_stride;
+    return from_codes<kGrad>(ck, dy, r, P, S, "tb_act8_weight_grad", st);
+}
+
+int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, float alpha, float beta,
+           float contrib, bool first, float* F, cudaStream_t st) {
+    Params P{};
+    P.samples = samples;
+    P.S = S;
+    P.out = F;
+    P.alpha = alpha;
+    P.beta = beta;
+    P.contrib = contrib;
+    P.first = first;
+    return from_codes<kFisher>(ck, dy, r, P, 1, "tb_act8_fisher", st);
+}
+
+int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaStream_t st) {
+    Params P{};
+    P.M = P.N = ck.d;
+    P.tiles_m = P.tiles_n = tiles(ck.d, 256);
+    P.exps = ck.exps;
+    P.lde = ck.lde;
+    P.n = ck.n;
+    P.out = H;
+    P.ldo = ck.d;
+    P.scale = scale;
+    P.accumulate = accumulate;
+    int rc = set_items(&P, static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2, "tb_act8_hessian");
+    CUtensorMap a{};
+    if (!rc && ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
+    return rc ? rc : launch<kHess>(a, a, P, st);
+}
+
+template <int MODE>
+static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_t st) {
+    Params P{};
+    P.M = p.n;
+    P.N = p.N;
+    P.K = p.K;
+    P.n = p.n;
+    P.tiles_m = tiles(p.n, 256);
+    P.tiles_n = tiles(p.N, 256);
+    P.out = p.out;
+    P.ldo = p.ldout;
+    P.ad = p;
+    int rc = set_items(&P, static_cast<long long>(P.tiles_m) * P.tiles_n, who);
+    CUtensorMap a{}, b{};
+    if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
+    if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
+                               : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
+    return rc ? rc : launch<MODE>(a, b, P, st);
+}
+
+int adapter_forward(const AdapterProduct& p, cudaStream_t st) { return adapter_product<kFwd>(p, "tb_adapter_forward", st); }
+int adapter_input_grad(const AdapterProduct& p, cudaStream_t st) { return adapter_product<kDx>(p, "tb_adapter_backward", st); }
+
+int take_error(cudaStream_t st) {
+    int h = 0, zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&h, g_linear_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_linear_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    return e == cudaSuccess ? h : -1;
+}
+
+}  // namespace linear
+}  // namespace tb

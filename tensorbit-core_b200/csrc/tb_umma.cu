@@ -15,8 +15,10 @@
 #include <cstdio>
 #include <mutex>
 
+#include "tb_linear.cuh"
 #include "tb_pdl.cuh"
 #include "tb_runtime.h"
+#include "tb_tcgen05.cuh"
 #include "tb_umma.cuh"
 
 namespace tb {
@@ -27,46 +29,9 @@ constexpr int kTile = 128;              // rows of A / B per tile, M = N = 128
 // Operand K-slices are 128 rows x SW bytes, loaded by TMA with the SW-byte
 // swizzle (SW = 128 or 64): the canonical K-major layouts whose 8-row atoms
 // sit 8 * SW bytes apart.
-constexpr uint64_t kWaitNs = 2000000000ull;  // bounded waits: 2 s
 
 __device__ int g_umma_error;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ uint64_t globaltimer() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// Bounded wait for the barrier phase `parity` to complete.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    const uint64_t t0 = globaltimer();
-    while (true) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (globaltimer() - t0 > kWaitNs) return false;
-    }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 template <int SW>
 __device__ __forceinline__ uint64_t sw_desc(uint32_t addr) {
     constexpr uint64_t kLayout = (SW == 128) ? 2ull : 4ull;  // 128-byte / 64-byte swizzle
@@ -86,26 +51,6 @@ __device__ __forceinline__ void mma(uint32_t tmem, uint64_t a, uint64_t b, uint3
             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
             ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
     }
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
 }
 __device__ __forceinline__ float tf32_hi(float x) {
     uint32_t r;
@@ -407,7 +352,6 @@ gemm_nt_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ 
 // and both CTAs' epilogue warps arrive on its accumulator-empty barrier.
 // Operand loads carry no multicast.  All waits are bounded; a CTA that gives
 // up records the error and both CTAs still meet at the closing cluster barrier.
-constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // shared address of the even CTA's copy
 constexpr int kPairA = kTile * 128;           // 128 rows x 128 B
 
 template <int KIND, int NB> struct Pair {
@@ -420,14 +364,6 @@ template <int KIND, int NB> struct Pair {
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + 1024 + 256;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
                                                  uint32_t even_bar) {
     asm volatile(
@@ -449,13 +385,6 @@ __device__ __forceinline__ void mma_pair(uint32_t tmem, uint64_t a, uint64_t b, 
             ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
     }
 }
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(bar), "h"(static_cast<uint16_t>(3))
-        : "memory");
-}
-
 template <int KIND, int NB>
 __global__ void __launch_bounds__(Pair<KIND, NB>::kThreads, 1)
 gemm_nt_pair_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
@@ -635,22 +564,6 @@ gemm_nt_pair_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_consta
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NB));
     }
-}
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
 }
 
 // Row-major [rows, k] operand, 128-row x sw-byte boxes with the sw-byte swizzle.
@@ -862,7 +775,9 @@ extern "C" int tb_gemm_nt_bf16(const void* a, long long lda, const void* b, long
 extern "C" int tb_gemm_status(void* stream) {
     int rc = require_device(nullptr);
     if (rc) return rc;
-    const int e = umma::gemm_take_error(static_cast<cudaStream_t>(stream));
+    const int e1 = umma::gemm_take_error(static_cast<cudaStream_t>(stream));
+    const int e2 = linear::take_error(static_cast<cudaStream_t>(stream));
+    const int e = e1 < 0 || e2 < 0 ? -1 : e1 | e2;
     if (e < 0) return fail(TB_ERR_CUDA, "reading the GEMM status failed");
     return e ? fail(TB_ERR_TIMEOUT, "a tcgen05 GEMM pipeline wait expired") : TB_OK;
 }

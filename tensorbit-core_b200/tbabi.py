@@ -178,7 +178,7 @@ def lib() -> C.CDLL:
             "tb_act8_pack": ([C.POINTER(Act8), vp, i32, i64, vp, vp], i32),
             "tb_act8_unpack": ([C.POINTER(Act8), vp, i32, i64, vp], i32),
             "tb_act8_weight_grad": ([C.POINTER(Act8), vp, i32, i64, i32, vp, i32, vp, i32, i64, vp], i32),
-            "tb_act8_fisher": ([C.POINTER(Act8), vp, i32, i64, i32, vp, i32, f32, f32, i32, vp, vp], i32),
+            "tb_act8_fisher": ([C.POINTER(Act8), vp, i32, i64, i32, vp, i32, C.c_double, C.c_double, i32, vp, vp], i32),
             "tb_act8_hessian": ([C.POINTER(Act8), f32, i32, vp, vp], i32),
             "tb_adapter_forward": ([C.POINTER(AdapterArgs), vp], i32),
             "tb_adapter_backward": ([C.POINTER(AdapterArgs), vp], i32),
