@@ -5,9 +5,9 @@
 // and NB/2 of the B columns of a K slice in shared memory, and its 128 x NB
 // half of the accumulator in TMEM.  Roles of a CTA's 16 warps:
 //   warp 12      TMA loads of K slices into a ring of stages;
-//   warps 8-11   "prepare" a stage: decode int8 codes to the BF16 operand,
-//                zero what lies behind a sample's end, or build the operands of
-//                an adapter; then tell the even CTA that the stage is ready;
+//   warps 8-11   "prepare" stages that do not arrive as operands: decode int8
+//                codes to BF16 and zero what lies behind a sample's end, or
+//                build the operands of an adapter; then tell the even CTA;
 //   warp 13      (even CTA) issues tcgen05.mma for both CTAs;
 //   warps 0-7    take finished accumulators out of TMEM and store results.
 // The accumulator is double buffered, so the next sums run while a tile is
@@ -59,8 +59,12 @@ struct Cfg {
     static constexpr int kGroup = kCodes ? 4 : MODE == kHess ? 1 : 1 << 30;
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
     static constexpr int kB = MODE == kHess ? 16384 : kCols * 128;
-    static constexpr int kRaw = kCodes ? 64 * kCols : 0;
-    static constexpr int kStage = kA + kB + kRaw;
+    static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
+    static constexpr int kExps = kCodes ? 2 * kCols : 0;               // exponents of its first block and the next
+    static constexpr int kStage = kA + kB + (kRaw + kExps + 1023) / 1024 * 1024;
+    // Arrivals that make a stage ready: the prepare warps of both CTAs (codes), the even CTA's
+    // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
+    static constexpr int kReady = kCodes ? 8 : kAdapter ? 9 : 1;
     static constexpr int kStages = MODE == kGrad ? 5 : MODE == kFisher ? 7 : 6;
     static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kColScale + 1024 + 512;
@@ -84,23 +88,30 @@ struct Params {
     AdapterProduct ad;
 };
 
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity) {
-    const uint64_t t0 = globaltimer();
-    while (true) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (globaltimer() - t0 > kWaitNs) return false;
-    }
+// Waits for the barrier phase `parity`, at most about two seconds of SM cycles.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
+constexpr long long kWaitCycles = 4000000000ll;
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+    if (try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles)
+        if (try_wait(bar, parity)) return true;
+    return false;
+}
+// (An explicit .release.cluster here cost about 0.4 us per slice: 1235 against
+// 675 us for the 7000 x 4096 x 14336 forward.)
 __device__ __forceinline__ void arrive_even(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar & kPeerMask) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar & kPeerMask) : "memory");
 }
 template <int MODE>
 __device__ __forceinline__ void mma_step(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -123,8 +134,11 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
     const uint64_t lbo = mn ? kMnChunk >> 4 : 1;
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (lbo << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t even_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(even_bar)
+        : "memory");
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t r;
@@ -206,7 +220,9 @@ __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
     return u;
 }
 
-// Calls f(tile, unit, j) for every slice of this pair's items until it returns false.
+// Calls f(tile, unit, j, part, i) for every slice of this pair's items until it
+// returns false: slice i of a part of K, j counted over the whole unit; the
+// slices of a unit's adapters follow those of its K as the next part.
 template <int MODE, class F>
 __device__ __forceinline__ bool walk(const Params& P, F&& f) {
     for (int item = blockIdx.x >> 1; item < P.items; item += gridDim.x >> 1) {
@@ -214,8 +230,11 @@ __device__ __forceinline__ bool walk(const Params& P, F&& f) {
         const int s1 = MODE == kFisher ? P.S : t.s + 1;
         for (int s = t.s; s < s1; ++s) {
             const Unit u = unit_of<MODE>(P, t, s);
-            for (int j = 0; j < u.total; ++j)
-                if (!f(t, u, j)) return false;
+            for (int j = 0, part = 0; j < u.total; ++part) {
+                const int last = min(u.total, j + (Cfg<MODE>::kAdapter && part ? u.total : u.slices));
+                for (int i = 0; j < last; ++i, ++j)
+                    if (!f(t, u, j, part, i)) return false;
+            }
         }
     }
     return true;
@@ -280,10 +299,78 @@ __device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, 
     return y;
 }
 
+// Eight exponent bytes as four pairs of BF16 scales.
+__device__ __forceinline__ void scales8(uint2 e, uint32_t (&s)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = (i < 2 ? e.x : e.y) >> (16 * (i & 1));
+        s[i] = act8::scale_bf16(x & 0xFF) | act8::scale_bf16((x >> 8) & 0xFF) << 16;
+    }
+}
+
+// Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
+// tile's tokens' u as two BF16 parts, zero unless the adapter is their own; B is
+// the adapter's second factor, twice.
+template <int MODE>
+__device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, int r0, long long m0, int n0, uint8_t* sa,
+                                              uint8_t* sb, int pt) {
+    const int nr = min(32, p.rank - r0);
+    const long long tok = m0 + pt;
+    const bool mine = tok < p.n && __ldg(p.who + tok) == a;
+    const float* up = p.u + tok * p.rank + r0;
+    uint8_t* arow = sa + pt * 128;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 8 * q + 2 * i;
+            const float f0 = mine && j < nr ? up[j] : 0.0f, f1 = mine && j + 1 < nr ? up[j + 1] : 0.0f;
+            hi[i] = pack_bf16(f0, f1);
+            lo[i] = pack_bf16(f0 - __uint_as_float(hi[i] << 16), f1 - __uint_as_float(hi[i] & 0xFFFF0000u));
+        }
+        *reinterpret_cast<uint4*>(arow + ((q ^ (pt & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(arow + (((q + 4) ^ (pt & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    if constexpr (MODE == kFwd) {  // a row of b for each output column
+        const long long o = n0 + pt;
+        const uint16_t* bp = reinterpret_cast<const uint16_t*>(p.e) + (static_cast<long long>(a) * p.N + o) * p.lde + r0;
+        uint8_t* brow = sb + pt * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (o < p.N && 8 * q < nr) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(bp + 8 * q));
+                const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = 8 * q + 2 * i;
+                    w[i] = j + 1 < nr ? in[i] : j < nr ? in[i] & 0xFFFFu : 0u;
+                }
+            }
+            const uint4 v4 = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(brow + ((q ^ (pt & 7)) << 4)) = v4;
+            *reinterpret_cast<uint4*>(brow + (((q + 4) ^ (pt & 7)) << 4)) = v4;
+        }
+    } else {  // rows of a, the ranks along K
+        const int c = pt & 15, f = n0 + 8 * c;
+        uint8_t* dst = sb + (c >> 3) * kMnChunk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = (pt >> 4) + 8 * i;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (f < p.N && k < nr) v = __ldg(reinterpret_cast<const uint4*>(p.e + (static_cast<long long>(a) * p.rank + r0 + k) * p.lde + f));
+            const int unit = ((c & 7) ^ (k & 7)) << 4;
+            *reinterpret_cast<uint4*>(dst + k * 128 + unit) = v;
+            *reinterpret_cast<uint4*>(dst + (k + 32) * 128 + unit) = v;
+        }
+    }
+}
+
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CUtensorMap tB,
-              const __grid_constant__ Params P) {
+              const __grid_constant__ CUtensorMap tE, const __grid_constant__ Params P) {
     using C = Cfg<MODE>;
     constexpr int NB = C::NB, kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -306,7 +393,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&ready[s]), 8);  // four prepare warps of each CTA
+            mbar_init(smem_u32(&ready[s]), C::kReady);
             mbar_init(smem_u32(&empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -346,7 +433,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             if constexpr (C::kAdapter) {
                 const Unit u = unit_of<MODE>(P, t, 0);
                 const int b = gc & 1;
-                if (!mbar_wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
+                if (!wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
                 fence_after();
                 ++gc;
 #pragma unroll
@@ -403,7 +490,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                             if (g + 1 < groups) load_exps(g + 1);
                         }
                         const int b = gc & 1;
-                        if (!mbar_wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
+                        if (!wait(smem_u32(&accfull[b]), (gc >> 1) & 1) || *abort_flag) { ok = false; break; }
                         fence_after();
                         ++gc;
 #pragma unroll
@@ -463,34 +550,42 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
         if (warp == kTmaWarp) {
             if (lane == 0) {
                 int it = 0;
-                const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j) {
+                const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j, int part, int i) {
                     const int s = it % kStages;
-                    if (it >= kStages && !mbar_wait(smem_u32(&empty[s]), ((it / kStages) - 1) & 1)) return false;
+                    if (it >= kStages && !wait(smem_u32(&empty[s]), ((it / kStages) - 1) & 1)) return false;
                     if (*abort_flag) return false;
-                    const uint32_t bar = smem_u32(&full[s]);
                     const int m0 = t.tm * 256 + rank * 128, n0 = t.tn * NB + rank * C::kCols;
-                    if (C::kAdapter && j >= u.slices) {  // the prepare warps fill this stage
-                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-                    } else if constexpr (C::kCodes) {
-                        const int part = j / u.slices;
-                        const int k = static_cast<int>(u.lo) + (j % u.slices) * 64;
-                        const int y = static_cast<int>(part * P.n) + k;
-                        mbar_expect_tx(bar, C::kA + C::kRaw);
+                    if constexpr (C::kCodes) {
+                        const uint32_t bar = smem_u32(&full[s]);
+                        const int k = static_cast<int>(u.lo) + i * 64;
+                        // parts with fewer leading bits first: the large ones are then truncated least often
+                        const int y = static_cast<int>((P.parts - 1 - part) * P.n) + k;
+                        mbar_expect_tx(bar, C::kA + C::kRaw + C::kExps);
                         tma_load_2d(stage_a(s), &tA, m0, y, bar);
                         tma_load_2d(stage_a(s) + kMnChunk, &tA, m0 + 64, y, bar);
                         tma_load_2d(stage_raw(s), &tB, n0, k, bar);
-                    } else if constexpr (MODE == kHess) {
-                        mbar_expect_tx(bar, C::kA + C::kB);
-                        tma_load_2d(stage_a(s), &tA, m0, j * 128, bar);
-                        tma_load_2d(stage_b(s), &tB, n0, j * 128, bar);
+                        tma_load_2d(stage_raw(s) + C::kRaw, &tE, n0, k >> 7, bar);
                     } else {
-                        mbar_expect_tx(bar, C::kA + C::kB);
-                        tma_load_2d(stage_a(s), &tA, j * 64, m0, bar);
-                        if constexpr (MODE == kFwd) {
-                            tma_load_2d(stage_b(s), &tB, j * 64, n0, bar);
-                        } else {
-                            tma_load_2d(stage_b(s), &tB, n0, j * 64, bar);
-                            tma_load_2d(stage_b(s) + kMnChunk, &tB, n0 + 64, j * 64, bar);
+                        const uint32_t bar = smem_u32(&ready[s]) & kPeerMask;
+                        const bool built = C::kAdapter && part > 0;  // the prepare warps fill this stage
+                        if (built) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+                        if (rank == 0) {
+                            if (built) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+                            else {
+                                if (C::kAdapter) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 8;" ::"r"(bar) : "memory");
+                                mbar_expect_tx(bar, 2 * (C::kA + C::kB));
+                            }
+                        }
+                        if (!built) {
+                            const int k = i * (MODE == kHess ? 128 : 64);
+                            if constexpr (MODE == kHess) tma_load_pair(stage_a(s), &tA, m0, k, bar);
+                            else tma_load_pair(stage_a(s), &tA, k, m0, bar);
+                            if constexpr (MODE == kFwd) {
+                                tma_load_pair(stage_b(s), &tB, k, n0, bar);
+                            } else {
+                                tma_load_pair(stage_b(s), &tB, n0, k, bar);
+                                if constexpr (MODE == kDx) tma_load_pair(stage_b(s) + kMnChunk, &tB, n0 + 64, k, bar);
+                            }
                         }
                     }
                     ++it;
@@ -498,8 +593,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 });
                 if (!done) {
                     *abort_flag = 1;
-                    for (int i = std::max(0, it - kStages); i < it; ++i)  // loads in flight, each waited for within a limit
-                        mbar_wait(smem_u32(&full[i % kStages]), (i / kStages) & 1);
+                    // loads in flight, each waited for within a limit (the odd CTA's may count on the even one's barrier)
+                    for (int i = std::max(0, it - kStages); i < it && (C::kCodes || rank == 0); ++i)
+                        wait(smem_u32(C::kCodes ? &full[i % kStages] : &ready[i % kStages]), (i / kStages) & 1);
                 }
             }
             __syncwarp();
@@ -512,14 +608,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 constexpr uint64_t kStepMn = MODE == kHess ? 4096 >> 4 : 2048 >> 4;
                 constexpr uint64_t kStepA = kAmn ? kStepMn : 2, kStepB = kBmn ? kStepMn : 2;
                 int it = 0, gc = 0;
-                const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int j) {
+                const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int j, int, int) {
                     const bool first = j % C::kGroup == 0;
                     const int b = gc & 1;
                     if (first) {
-                        if (gc >= 2 && !wait_cluster(smem_u32(&accempty[b]), ((gc >> 1) - 1) & 1)) return false;
+                        if (gc >= 2 && !wait(smem_u32(&accempty[b]), ((gc >> 1) - 1) & 1)) return false;
                     }
                     const int s = it % kStages;
-                    if (*abort_flag || !wait_cluster(smem_u32(&ready[s]), (it / kStages) & 1)) return false;
+                    if (*abort_flag || !wait(smem_u32(&ready[s]), (it / kStages) & 1)) return false;
                     fence_after();
                     const uint64_t a0 = operand_desc(stage_a(s), kAmn), b0 = operand_desc(stage_b(s), kBmn);
                     const uint32_t d = tmem + static_cast<uint32_t>(b * NB);
@@ -541,116 +637,43 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 }
             }
             __syncwarp();
-        } else if (warp >= kPrepWarp && warp < kTmaWarp) {
-            const int pt = threadIdx.x - kPrepWarp * 32;
+        } else if (C::kCodes && warp >= kPrepWarp && warp < kTmaWarp) {
+            // 8 consecutive features (one 16-byte unit of the operand) of every kRowStep-th token
+            constexpr int kUnits = C::kCols / 8, kRowStep = 128 / kUnits, kSteps = 64 / kRowStep;
+            const int pt = threadIdx.x - kPrepWarp * 32, pc = pt % kUnits, pr = pt / kUnits;
             int it = 0;
-            // kCodes: 8 consecutive features of every kRowStep-th token
-            constexpr int kLanesRow = C::kCodes ? C::kCols / 8 : 16, kRowStep = 128 / kLanesRow;
-            const int pc = pt % kLanesRow, pr = pt / kLanesRow;
-            uint2 e0 = make_uint2(0, 0), e1 = make_uint2(0, 0);
-            const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j) {
+            const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int, int, int i) {
                 const int s = it % kStages;
-                const int n0 = t.tn * NB + rank * C::kCols;
-                int k0 = 0;
-                if constexpr (C::kCodes) {
-                    k0 = static_cast<int>(u.lo) + (j % u.slices) * 64;
-                    // the exponents of the slice's first and last token's blocks, fetched before the wait
-                    const long long f = n0 + 8 * pc;
-                    const int b0 = k0 >> 7, b1 = (static_cast<int>(min(u.hi, k0 + 64ll)) - 1) >> 7;
-                    if (f < P.N) {
-                        e0 = __ldg(reinterpret_cast<const uint2*>(P.exps + b0 * P.lde + f));
-                        e1 = b1 == b0 ? e0 : __ldg(reinterpret_cast<const uint2*>(P.exps + b1 * P.lde + f));
-                    }
+                const long long k0 = u.lo + i * 64ll;
+                const int valid = static_cast<int>(min(64ll, u.hi - k0));
+                const int border = 128 - static_cast<int>(k0 & 127);  // first token of the next block
+                if (*abort_flag || !wait(smem_u32(&full[s]), (it / kStages) & 1)) return false;
+                uint8_t* stage = smem + s * C::kStage;
+                const uint8_t* raw = stage + C::kA + C::kB;
+                uint2 w[kSteps];
+#pragma unroll
+                for (int q = 0; q < kSteps; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + q * kRowStep) * C::kCols + pc * 8);
+                const uint2 e0 = *reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8);
+                const uint2 e1 = *reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8);
+                uint32_t s0[4], s1[4];
+                scales8(e0, s0);
+                scales8(e1, s1);
+                uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
+#pragma unroll
+                for (int q = 0; q < kSteps; ++q) {
+                    const int k = pr + q * kRowStep;
+                    const bool second = k >= border;
+                    uint4 o;
+                    o.x = decode2(prmt(w[q].x, 0x43434343u, 0x4140u), second ? s1[0] : s0[0]);
+                    o.y = decode2(prmt(w[q].x, 0x43434343u, 0x4342u), second ? s1[1] : s0[1]);
+                    o.z = decode2(prmt(w[q].y, 0x43434343u, 0x4140u), second ? s1[2] : s0[2]);
+                    o.w = decode2(prmt(w[q].y, 0x43434343u, 0x4342u), second ? s1[3] : s0[3]);
+                    if (k >= valid) o = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = o;
                 }
-                if (*abort_flag || !mbar_wait(smem_u32(&full[s]), (it / kStages) & 1)) return false;
-                if constexpr (C::kCodes) {
-                    const int valid = static_cast<int>(min(64ll, u.hi - k0));
-                    const int border = (((k0 >> 7) + 1) << 7) - k0;  // first row of the second block
-                    uint32_t s0[4], s1[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t x = (i < 2 ? e0.x : e0.y) >> (16 * (i & 1)), y = (i < 2 ? e1.x : e1.y) >> (16 * (i & 1));
-                        s0[i] = act8::scale_bf16(x & 0xFF) | act8::scale_bf16((x >> 8) & 0xFF) << 16;
-                        s1[i] = act8::scale_bf16(y & 0xFF) | act8::scale_bf16((y >> 8) & 0xFF) << 16;
-                    }
-                    const uint32_t raw = stage_raw(s), dst = stage_b(s) + (pc >> 3) * kMnChunk;
-#pragma unroll
-                    for (int i = 0; i < 64 / kRowStep; ++i) {
-                        const int k = pr + i * kRowStep;
-                        uint2 w;
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(raw + k * C::kCols + pc * 8));
-                        const bool second = k >= border;
-                        uint4 o;
-                        o.x = decode2(prmt(w.x, 0x43434343u, 0x4140u), second ? s1[0] : s0[0]);
-                        o.y = decode2(prmt(w.x, 0x43434343u, 0x4342u), second ? s1[1] : s0[1]);
-                        o.z = decode2(prmt(w.y, 0x43434343u, 0x4140u), second ? s1[2] : s0[2]);
-                        o.w = decode2(prmt(w.y, 0x43434343u, 0x4342u), second ? s1[3] : s0[3]);
-                        if (k >= valid) o = make_uint4(0, 0, 0, 0);
-                        st_shared16(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4), o);
-                    }
-                    // tokens behind the sample's end: dY may hold anything there
-                    for (int i = pt; i < (64 - valid) * 16; i += 128)
-                        st_shared16(stage_a(s) + (i & 1) * kMnChunk + (valid + (i >> 4)) * 128 + ((i >> 1) & 7) * 16, make_uint4(0, 0, 0, 0));
-                } else if constexpr (C::kAdapter) {
-                    if (j >= u.slices) {
-                        const int x = j - u.slices;
-                        const int a = __ldg(u.list + 1 + x / u.rslices), r0 = (x % u.rslices) * 32;
-                        const int nr = min(32, P.ad.rank - r0);
-                        // A: this token's u as two BF16 parts, zero unless the adapter is its own
-                        const long long tok = static_cast<long long>(t.tm) * 256 + rank * 128 + pt;
-                        const bool mine = tok < P.M && __ldg(P.ad.who + tok) == a;
-                        const float* up = P.ad.u + tok * P.ad.rank + r0;
-                        const uint32_t arow = stage_a(s) + pt * 128;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int j0 = 8 * q + 2 * i;
-                                const float f0 = mine && j0 < nr ? up[j0] : 0.0f, f1 = mine && j0 + 1 < nr ? up[j0 + 1] : 0.0f;
-                                hi[i] = pack_bf16(f0, f1);
-                                lo[i] = pack_bf16(f0 - __uint_as_float(hi[i] << 16), f1 - __uint_as_float(hi[i] & 0xFFFF0000u));
-                            }
-                            st_shared16(arow + ((q ^ (pt & 7)) << 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                            st_shared16(arow + (((q + 4) ^ (pt & 7)) << 4), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                        }
-                        if constexpr (MODE == kFwd) {  // B: a row of b per output column, twice
-                            const long long o = n0 + pt;
-                            const uint16_t* bp = reinterpret_cast<const uint16_t*>(P.ad.e) + (static_cast<long long>(a) * P.N + o) * P.ad.lde + r0;
-                            const uint32_t brow = stage_b(s) + pt * 128;
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t w[4] = {0, 0, 0, 0};
-                                if (o < P.N && 8 * q < nr) {
-                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(bp + 8 * q));
-                                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const int j0 = 8 * q + 2 * i;
-                                        w[i] = j0 + 1 < nr ? in[i] : j0 < nr ? in[i] & 0xFFFFu : 0u;
-                                    }
-                                }
-                                const uint4 v4 = make_uint4(w[0], w[1], w[2], w[3]);
-                                st_shared16(brow + ((q ^ (pt & 7)) << 4), v4);
-                                st_shared16(brow + (((q + 4) ^ (pt & 7)) << 4), v4);
-                            }
-                        } else {  // B: rows of a, the ranks along K, twice
-                            const int c = pt & 15;
-                            const long long f = n0 + 8 * c;
-                            const uint32_t dst = stage_b(s) + (c >> 3) * kMnChunk;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int k = (pt >> 4) + 8 * i;
-                                uint4 v = make_uint4(0, 0, 0, 0);
-                                if (f < P.N && k < nr)
-                                    v = __ldg(reinterpret_cast<const uint4*>(P.ad.e + (static_cast<long long>(a) * P.ad.rank + r0 + k) * P.ad.lde + f));
-                                const uint32_t unit = ((c & 7) ^ (k & 7)) << 4;
-                                st_shared16(dst + k * 128 + unit, v);
-                                st_shared16(dst + (k + 32) * 128 + unit, v);
-                            }
-                        }
-                    }
-                }
+                // tokens behind the sample's end: dY may hold anything there
+                for (int q = pt; q < (64 - valid) * 16; q += 128)
+                    *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + (valid + (q >> 4)) * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&ready[s]));
@@ -658,6 +681,31 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 return true;
             });
             if (!done) *abort_flag = 1;
+        } else if (C::kAdapter && warp >= kPrepWarp && warp < kTmaWarp) {
+            // The TMA warp passes a free stage on through full[s]; every use of a stage for an adapter is one
+            // phase of that barrier.  (empty[s] cannot be waited on here: its parity says nothing to a waiter
+            // that skips phases.)
+            const int pt = threadIdx.x - kPrepWarp * 32;
+            int it = 0;
+            uint32_t phase = 0;  // a bit per stage
+            bool ok = true;
+            for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
+                const Tile t = tile_of<MODE>(P, item);
+                const Unit u = unit_of<MODE>(P, t, 0);
+                it += u.slices;
+                for (int x = 0; x < u.total - u.slices; ++x, ++it) {
+                    const int s = it % kStages;
+                    const int a = __ldg(u.list + 1 + x / u.rslices), r0 = (x % u.rslices) * 32;
+                    if (*abort_flag || !wait(smem_u32(&full[s]), (phase >> s) & 1)) { ok = false; break; }
+                    phase ^= 1u << s;
+                    build_adapter<MODE>(P.ad, a, r0, static_cast<long long>(t.tm) * 256 + rank * 128, t.tn * NB + rank * C::kCols,
+                                        smem + s * C::kStage, smem + s * C::kStage + C::kA, pt);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive_even(smem_u32(&ready[s]));
+                }
+            }
+            if (!ok) *abort_flag = 1;
         }
     }
     fence_before();
@@ -685,7 +733,7 @@ int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long
 }
 
 template <int MODE>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& P, cudaStream_t st) {
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const Params& P, cudaStream_t st) {
     using C = Cfg<MODE>;
     // Per device: the shared-memory limit, and that the launch has the registers that the roles' shares add up to.
     static std::mutex mu;
@@ -708,7 +756,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& P, cudaStre
     }
     constexpr int kPairs = 74;  // one CTA on each of the 148 SMs
     const int pairs = std::min(P.items, kPairs);
-    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, P);
+    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, P);
     return check_launch("linear_kernel");
 }
 
@@ -735,10 +783,11 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     P.parts = dy.parts;
     P.ldo = ck.d;
     int rc = set_items(&P, static_cast<long long>(P.tiles_m) * P.tiles_n * samples, who);
-    CUtensorMap a{}, b{};
+    CUtensorMap a{}, b{}, e{};
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
-    return rc ? rc : launch<MODE>(a, b, P, st);
+    if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 2, false);
+    return rc ? rc : launch<MODE>(a, b, e, P, st);
 }
 
 }  // namespace
@@ -781,7 +830,7 @@ int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaSt
     int rc = set_items(&P, static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2, "tb_act8_hessian");
     CUtensorMap a{};
     if (!rc && ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
-    return rc ? rc : launch<kHess>(a, a, P, st);
+    return rc ? rc : launch<kHess>(a, a, a, P, st);
 }
 
 template <int MODE>
@@ -801,7 +850,7 @@ static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_
     if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
     if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
                                : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
-    return rc ? rc : launch<MODE>(a, b, P, st);
+    return rc ? rc : launch<MODE>(a, b, b, P, st);
 }
 
 int adapter_forward(const AdapterProduct& p, cudaStream_t st) { return adapter_product<kFwd>(p, "tb_adapter_forward", st); }
