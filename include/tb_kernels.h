@@ -266,8 +266,9 @@ int tb_obs_sparsegpt_phase_times(float* ms_out, int n);
  * feature because calibration activations have heavy columns.  xhat has 7
  * significant bits, so it is exact in BF16, and every product formed from a
  * checkpoint below is the exact product of xhat.  A NaN or an infinity in a
- * block's kept tokens sets E = 255: the whole block of that feature reads
- * back as NaN. */
+ * block's kept tokens sets E = 255 and all its codes 0: the whole block of
+ * that feature reads back as NaN.  Other E are 1..249; checkpoints written by
+ * other means keep to both. */
 #define TB_ACT8_BLOCK 128
 typedef struct tb_act8 {
     uint32_t struct_size;  /* sizeof(tb_act8)                                          */

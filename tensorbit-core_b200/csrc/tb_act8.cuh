@@ -1,7 +1,7 @@
 // 8-bit activation checkpoints: the decode used by every kernel that reads one.
 // A value is q * 2^(E - 127) with an int8 code q and the exponent byte E of its
-// feature and block of TB_ACT8_BLOCK tokens; E = 255 marks a block that held a
-// NaN or an infinity and reads back as NaN.
+// feature and block of TB_ACT8_BLOCK tokens; E = 255 with codes 0 marks a block
+// that held a NaN or an infinity and reads back as NaN.
 #pragma once
 
 #include <cstdint>
@@ -28,12 +28,8 @@ struct View {
 // Status of a checkpoint description; fills `v`.
 int check(const tb_act8* ck, const char* who, View* v);
 
-// 2^(E - 127) in FP32 (E = 0, which packing never writes, is the subnormal 2^-127).
-__device__ __forceinline__ float scale_f32(uint32_t e) {
-    return __uint_as_float(e == 255u ? 0x7FFFFFFFu : e == 0u ? 0x00400000u : e << 23);
-}
-// The same as BF16 bits.
-__device__ __forceinline__ uint32_t scale_bf16(uint32_t e) { return e == 255u ? 0x7FFFu : e == 0u ? 0x0040u : e << 7; }
+// 2^(E - 127) in FP32.  E = 255 gives an infinity, and the zero codes of such a block times it NaN.
+__device__ __forceinline__ float scale_f32(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Exponent byte for a block whose largest |x| has the FP32 bits `amax`
 // (NaN and infinity order above every finite value): the smallest power of two

@@ -299,13 +299,17 @@ __device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, 
     return y;
 }
 
-// Eight exponent bytes as four pairs of BF16 scales.
+// Eight exponent bytes as four pairs of BF16 scales (255 is an infinity, and 0 times it NaN).
 __device__ __forceinline__ void scales8(uint2 e, uint32_t (&s)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t x = (i < 2 ? e.x : e.y) >> (16 * (i & 1));
-        s[i] = act8::scale_bf16(x & 0xFF) | act8::scale_bf16((x >> 8) & 0xFF) << 16;
-    }
+    s[0] = prmt(e.x, 0, 0x4140u) << 7;
+    s[1] = prmt(e.x, 0, 0x4342u) << 7;
+    s[2] = prmt(e.y, 0, 0x4140u) << 7;
+    s[3] = prmt(e.y, 0, 0x4342u) << 7;
+}
+// Eight codes times eight scales.
+__device__ __forceinline__ uint4 decode8(uint2 w, const uint32_t (&s)[4]) {
+    return make_uint4(decode2(prmt(w.x, 0x43434343u, 0x4140u), s[0]), decode2(prmt(w.x, 0x43434343u, 0x4342u), s[1]),
+                      decode2(prmt(w.y, 0x43434343u, 0x4140u), s[2]), decode2(prmt(w.y, 0x43434343u, 0x4342u), s[3]));
 }
 
 // Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
@@ -374,7 +378,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     using C = Cfg<MODE>;
     constexpr int NB = C::NB, kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // (by offset, so that the compiler still knows it for shared memory)
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     float* col_scale = reinterpret_cast<float*>(smem + kStages * C::kStage);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * C::kStage + C::kColScale);
     uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
@@ -465,16 +470,15 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 #pragma unroll
                     for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
                     float* scol = col_scale + warp * 2 * COLS;
-                    // kHess: exponent bytes of this lane's row and of four of the warp's columns, one group ahead
-                    uint32_t er = 0, ec = 0;
+                    // kHess: exponent bytes of this lane's row and of four of the warp's columns, fetched one
+                    // group ahead and not touched before (bytes behind the last column go to columns not stored)
+                    uint8_t er = 0;
+                    uint32_t ec = 0;
                     auto load_exps = [&](int g) {
                         if constexpr (MODE == kHess) {
                             const uint8_t* e = P.exps + g * P.lde;
-                            er = row < P.M ? e[row] : 0u;
-                            ec = 0;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (4 * lane + i < min(static_cast<long long>(COLS), P.N - col)) ec |= static_cast<uint32_t>(e[col + 4 * lane + i]) << (8 * i);
+                            if (row < P.M) er = __ldg(e + row);
+                            if (col + 4 * lane < P.N) ec = __ldg(reinterpret_cast<const uint32_t*>(e + col + 4 * lane));
                         }
                     };
                     if (groups > 0) load_exps(0);
@@ -482,8 +486,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         float srow = 0.0f;
                         if constexpr (MODE == kHess) {
                             srow = act8::scale_f32(er);
-                            float4 f = make_float4(act8::scale_f32(ec & 0xFF), act8::scale_f32((ec >> 8) & 0xFF),
-                                                   act8::scale_f32((ec >> 16) & 0xFF), act8::scale_f32(ec >> 24));
+                            const float4 f = make_float4(act8::scale_f32(ec & 0xFF), act8::scale_f32((ec >> 8) & 0xFF),
+                                                         act8::scale_f32((ec >> 16) & 0xFF), act8::scale_f32(ec >> 24));
                             __syncwarp();
                             *reinterpret_cast<float4*>(scol + (g & 1) * COLS + 4 * lane) = f;
                             __syncwarp();
@@ -653,23 +657,26 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 uint2 w[kSteps];
 #pragma unroll
                 for (int q = 0; q < kSteps; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + q * kRowStep) * C::kCols + pc * 8);
-                const uint2 e0 = *reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8);
-                const uint2 e1 = *reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8);
-                uint32_t s0[4], s1[4];
-                scales8(e0, s0);
-                scales8(e1, s1);
+                uint32_t s0[4];
+                scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8), s0);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
+                if (valid == 64 && border >= 64) {
 #pragma unroll
-                for (int q = 0; q < kSteps; ++q) {
-                    const int k = pr + q * kRowStep;
-                    const bool second = k >= border;
-                    uint4 o;
-                    o.x = decode2(prmt(w[q].x, 0x43434343u, 0x4140u), second ? s1[0] : s0[0]);
-                    o.y = decode2(prmt(w[q].x, 0x43434343u, 0x4342u), second ? s1[1] : s0[1]);
-                    o.z = decode2(prmt(w[q].y, 0x43434343u, 0x4140u), second ? s1[2] : s0[2]);
-                    o.w = decode2(prmt(w[q].y, 0x43434343u, 0x4342u), second ? s1[3] : s0[3]);
-                    if (k >= valid) o = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = o;
+                    for (int q = 0; q < kSteps; ++q) {
+                        const int k = pr + q * kRowStep;
+                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = decode8(w[q], s0);
+                    }
+                } else {  // a block's or the sample's end within the slice
+                    uint32_t s1[4];
+                    scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
+#pragma unroll
+                    for (int q = 0; q < kSteps; ++q) {
+                        const int k = pr + q * kRowStep;
+                        uint32_t sk[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
+                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = decode8(w[q], sk);
+                    }
                 }
                 // tokens behind the sample's end: dY may hold anything there
                 for (int q = pt; q < (64 - valid) * 16; q += 128)
