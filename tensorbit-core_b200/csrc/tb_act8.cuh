@@ -44,6 +44,34 @@ __device__ __forceinline__ uint32_t exponent_of(uint32_t amax) {
 // 2^(127 - E), the factor from values to codes (E of exponent_of, not 255).
 __device__ __forceinline__ float inverse_scale(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// Two int8 codes in the low bytes of v's halves (the high bytes 0x43) times two
+// BF16 scales.  0x4300 | low7 is 128 + low7 and 0x4300 | sign is 128 or 256, so
+// their difference is the signed code; both steps are exact.
+__device__ __forceinline__ uint32_t decode2(uint32_t v, uint32_t scale2) {
+    const uint32_t hi = v & 0xFF7FFF7Fu, lo = v & 0xFF80FF80u;
+    const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
+    const __nv_bfloat162 x = __hmul2(q, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Eight exponent bytes as four pairs of BF16 scales (255 is an infinity, and 0 times it NaN).
+__device__ __forceinline__ void scales8(uint2 e, uint32_t (&s)[4]) {
+    s[0] = prmt(e.x, 0, 0x4140u) << 7;
+    s[1] = prmt(e.x, 0, 0x4342u) << 7;
+    s[2] = prmt(e.y, 0, 0x4140u) << 7;
+    s[3] = prmt(e.y, 0, 0x4342u) << 7;
+}
+// Eight codes times eight scales.
+__device__ __forceinline__ uint4 decode8(uint2 w, const uint32_t (&s)[4]) {
+    return make_uint4(decode2(prmt(w.x, 0x43434343u, 0x4140u), s[0]), decode2(prmt(w.x, 0x43434343u, 0x4342u), s[1]),
+                      decode2(prmt(w.y, 0x43434343u, 0x4140u), s[2]), decode2(prmt(w.y, 0x43434343u, 0x4342u), s[3]));
+}
+
 // Element types as IEEE values.
 template <int DT>
 struct Elem;

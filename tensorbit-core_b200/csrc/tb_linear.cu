@@ -140,24 +140,9 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(even_bar)
         : "memory");
 }
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-    return r;
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// Two int8 codes in the low bytes of v's halves (the high bytes 0x43) times two
-// BF16 scales.  0x4300 | low7 is 128 + low7 and 0x4300 | sign is 128 or 256, so
-// their difference is the signed code; both steps are exact.
-__device__ __forceinline__ uint32_t decode2(uint32_t v, uint32_t scale2) {
-    const uint32_t hi = v & 0xFF7FFF7Fu, lo = v & 0xFF80FF80u;
-    const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
-    const __nv_bfloat162 x = __hmul2(q, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
-    return *reinterpret_cast<const uint32_t*>(&x);
 }
 
 // ---- the walk over work items, units (one sum each) and K slices that every role shares ----
@@ -297,19 +282,6 @@ __device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, 
                                                    : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o]),
                      y);
     return y;
-}
-
-// Eight exponent bytes as four pairs of BF16 scales (255 is an infinity, and 0 times it NaN).
-__device__ __forceinline__ void scales8(uint2 e, uint32_t (&s)[4]) {
-    s[0] = prmt(e.x, 0, 0x4140u) << 7;
-    s[1] = prmt(e.x, 0, 0x4342u) << 7;
-    s[2] = prmt(e.y, 0, 0x4140u) << 7;
-    s[3] = prmt(e.y, 0, 0x4342u) << 7;
-}
-// Eight codes times eight scales.
-__device__ __forceinline__ uint4 decode8(uint2 w, const uint32_t (&s)[4]) {
-    return make_uint4(decode2(prmt(w.x, 0x43434343u, 0x4140u), s[0]), decode2(prmt(w.x, 0x43434343u, 0x4342u), s[1]),
-                      decode2(prmt(w.y, 0x43434343u, 0x4140u), s[2]), decode2(prmt(w.y, 0x43434343u, 0x4342u), s[3]));
 }
 
 // Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
@@ -658,24 +630,24 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 #pragma unroll
                 for (int q = 0; q < kSteps; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + q * kRowStep) * C::kCols + pc * 8);
                 uint32_t s0[4];
-                scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8), s0);
+                act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8), s0);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
                 if (valid == 64 && border >= 64) {
 #pragma unroll
                     for (int q = 0; q < kSteps; ++q) {
                         const int k = pr + q * kRowStep;
-                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = decode8(w[q], s0);
+                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
                     }
                 } else {  // a block's or the sample's end within the slice
                     uint32_t s1[4];
-                    scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
+                    act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
 #pragma unroll
                     for (int q = 0; q < kSteps; ++q) {
                         const int k = pr + q * kRowStep;
                         uint32_t sk[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
-                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = decode8(w[q], sk);
+                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
                     }
                 }
                 // tokens behind the sample's end: dY may hold anything there
