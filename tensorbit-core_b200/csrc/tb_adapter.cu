@@ -4,7 +4,9 @@
 
 #include "tb_act8.cuh"
 #include "tb_linear.cuh"
+#include "tb_pdl.cuh"
 #include "tb_runtime.h"
+#include "tb_tcgen05.cuh"
 
 namespace tb {
 namespace adapter {
@@ -105,18 +107,31 @@ __device__ __forceinline__ uint4 row8(const Rows& s, long long t, int f) {
     return f + 8 <= s.cols ? v : first_of(v, s.cols - f);
 }
 
+// The value at `p`'s place in the shared memory of block `rank` of this cluster.
+__device__ __forceinline__ float load_peer(const float* p, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v)
+                 : "r"(umma::smem_u32(p)), "r"(rank)
+                 : "memory");
+    return v;
+}
+
 // u[t][k] = scale[a] sum_c row_t[c] M_a[k][c] for the tokens with an adapter:
 // 16 tokens and RC = 8 NT ranks per block, the features split over its 8 warps
 // in groups of 32 and the warps' sums joined in order.  One pass for each
 // adapter among the 16 tokens (runs of one request have one; a pass costs what
 // the 16 tokens of one adapter do, bound by reading M_a from L2).
 // ALONG: M_a = a [rank][lda], features along its rows; else M_a[k][c] = b [c][ldb].
-template <int NT, bool CODES, bool ALONG>
+// SPLIT > 1: a cluster of that many blocks shares the features of one tile and
+// joins its sums over distributed shared memory, in order.
+template <int NT, bool CODES, bool ALONG, int SPLIT>
 __device__ __forceinline__ void down_project(const Args& g, const Rows& src, float* __restrict__ u, float (*red)[16][8 * NT],
-                                             int* who) {
+                                             int* who, int passes, int mine_pass) {
     constexpr int RC = 8 * NT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-    const long long t0 = blockIdx.x * 16ll;
+    const int share = blockIdx.x % SPLIT;
+    const long long t0 = blockIdx.x / SPLIT * 16ll;
     const int rank0 = blockIdx.y * RC;
     if (threadIdx.x < 16) who[threadIdx.x] = t0 + threadIdx.x < g.n ? adapter_of(g, t0 + threadIdx.x) : -1;
     __syncthreads();
@@ -124,16 +139,17 @@ __device__ __forceinline__ void down_project(const Args& g, const Rows& src, flo
 #pragma unroll
     for (int i = 0; i < 16; ++i) rem |= who[i] >= 0 ? 1u << i : 0u;
     const int groups = (src.cols + 31) / 32;
-    while (rem) {
+    for (int pass = 0; rem; ++pass) {
         const int a = who[__ffs(rem) - 1];
         unsigned mine = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) mine |= who[i] == a ? 1u << i : 0u;
         rem &= ~mine;
+        if (pass % passes != mine_pass) continue;
         float acc[NT][4] = {};
         const bool r0 = mine >> gq & 1, r1 = mine >> (gq + 8) & 1;
-#pragma unroll 2
-        for (int kg = warp; kg < groups; kg += 8) {
+#pragma unroll(NT <= 4 ? 4 : 2)
+        for (int kg = share * 8 + warp; kg < groups; kg += 8 * SPLIT) {
             const int f = kg * 32 + 8 * tq;
             const bool in = f < src.cols;
             const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -184,32 +200,58 @@ __device__ __forceinline__ void down_project(const Args& g, const Rows& src, flo
 #pragma unroll
             for (int e = 0; e < 4; ++e) red[warp][gq + 8 * (e >> 1)][(2 * tq + (e & 1)) * NT + i] = acc[i][e];
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * RC; i += 256) {
-            const int row = i / RC, k = rank0 + i % RC;
-            float sum = 0.0f;
+        if constexpr (SPLIT == 1) {
+            for (int i = threadIdx.x; i < 16 * RC; i += 256) {
+                const int row = i / RC, k = rank0 + i % RC;
+                float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) sum += red[w][row][i % RC];
-            if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
+                for (int w = 0; w < 8; ++w) sum += red[w][row][i % RC];
+                if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
+            }
+            __syncthreads();
+        } else {
+            for (int i = threadIdx.x; i < 16 * RC; i += 256) {  // each sum has one thread: in place
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) sum += red[w][i / RC][i % RC];
+                red[0][i / RC][i % RC] = sum;
+            }
+            umma::cluster_sync_all();
+            for (int i = share * 256 + threadIdx.x; i < 16 * RC; i += SPLIT * 256) {
+                const int row = i / RC, k = rank0 + i % RC;
+                float v[SPLIT], sum = 0.0f;
+#pragma unroll
+                for (int q = 0; q < SPLIT; ++q) v[q] = load_peer(&red[0][row][i % RC], q);
+#pragma unroll
+                for (int q = 0; q < SPLIT; ++q) sum += v[q];
+                if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
+            }
+            umma::cluster_sync_all();  // no block writes its sums again, or leaves, before they have been read
         }
-        __syncthreads();
     }
 }
 
-// blockIdx.z = 0: the forward's u (from x) or the backward's v (from dy); 1: the backward's u (from the checkpoint).
-template <int NT, bool BACKWARD>
-__global__ void __launch_bounds__(256) down_kernel(const Args g, float* __restrict__ first, float* __restrict__ second,
-                                                   int32_t* __restrict__ lists) {
+// blockIdx.z = passes * q + p.  q = 0: the forward's u (from x) or the backward's
+// v (from dy); 1: the backward's u (from the checkpoint).  p: of a tile's
+// adapters, every passes-th.
+template <int NT, bool BACKWARD, int SPLIT>
+__global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(256) down_kernel(const Args g, const int passes,
+                                                                                float* __restrict__ first,
+                                                                                float* __restrict__ second,
+                                                                                int32_t* __restrict__ lists) {
     __shared__ float red[8][16][8 * NT];
     __shared__ int who[256];
+    const int p = blockIdx.z % passes;
+    asm volatile("griddepcontrol.launch_dependents;");  // few_tokens_kernel waits before it reads u
     if constexpr (!BACKWARD) {
-        down_project<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, first, red, who);
+        down_project<NT, false, true, SPLIT>(g, {g.x, g.ldx, {}, g.d}, first, red, who, passes, p);
     } else {
-        if (blockIdx.z == 0) down_project<NT, false, false>(g, {g.dy, g.lddy, {}, g.r}, first, red, who);
-        else down_project<NT, true, true>(g, {nullptr, 0, g.x8, g.d}, second, red, who);
+        if (static_cast<int>(blockIdx.z) < passes) down_project<NT, false, false, SPLIT>(g, {g.dy, g.lddy, {}, g.r}, first, red, who, passes, p);
+        else down_project<NT, true, true, SPLIT>(g, {nullptr, 0, g.x8, g.d}, second, red, who, passes, p);
     }
-    if (blockIdx.x % 16 == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    if (blockIdx.x % (16 * SPLIT) == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         __syncthreads();
-        list_adapters(g, blockIdx.x / 16, who, lists);
+        list_adapters(g, blockIdx.x / (16 * SPLIT), who, lists);
     }
 }
 
@@ -341,12 +383,92 @@ __global__ void __launch_bounds__(256) join_kernel(const Args g, const int cols,
     }
 }
 
+// The forward for few tokens: y = x W^T + u b^T, bound by reading W once.  A
+// block has 16 output features (rows of A in m16n8k16) and up to 8 NT tokens;
+// its 8 warps take every eighth group of 32 in features, so that the block reads
+// 512 consecutive bytes of each row at a time, and join their sums in order.
+// Launched while down_kernel still runs: u is not read before the wait.
+template <int NT>
+__global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const float* u) {
+    __shared__ float red[8][16][8 * NT + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+    const int o0 = blockIdx.x * 16, groups = (g.d + 31) / 32;
+    const bf16 *w0 = g.w + (o0 + gq) * g.ldw, *w1 = w0 + 8 * g.ldw;
+    const bool r0 = o0 + gq < g.r, r1 = o0 + gq + 8 < g.r;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    float acc[NT][4] = {};
+#pragma unroll(NT <= 2 ? 4 : 2)
+    for (int kg = warp; kg < groups; kg += 8) {
+        const int f = kg * 32 + 8 * tq;
+        const bool in = f < g.d;
+        uint4 a0 = in && r0 ? __ldcs(reinterpret_cast<const uint4*>(w0 + f)) : zero;
+        uint4 a1 = in && r1 ? __ldcs(reinterpret_cast<const uint4*>(w1 + f)) : zero;
+        uint4 x[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x[i] = in && 8 * i + gq < g.n ? __ldg(reinterpret_cast<const uint4*>(g.x + (8 * i + gq) * g.ldx + f)) : zero;
+        if (f + 8 > g.d) {
+            a0 = first_of(a0, g.d - f);
+            a1 = first_of(a1, g.d - f);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) x[i] = first_of(x[i], g.d - f);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            mma16816(acc[i], a0.x, a1.x, a0.y, a1.y, x[i].x, x[i].y);
+            mma16816(acc[i], a0.z, a1.z, a0.w, a1.w, x[i].z, x[i].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[warp][gq + 8 * (e >> 1)][8 * i + 2 * tq + (e & 1)] = acc[i][e];
+    __syncthreads();
+    pdl_wait();
+    for (int i = threadIdx.x; i < 16 * 8 * NT; i += 256) {
+        const int row = i & 15, t = i >> 4, o = o0 + row;
+        if (t >= g.n || o >= g.r) continue;
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) y += red[w][row][t];
+        const int a = adapter_of(g, t);
+        if (a >= 0) {
+            const bf16* b = g.b + (static_cast<long long>(a) * g.r + o) * g.ldb;
+            for (int k = 0; k < g.rank; k += 8) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(b + k));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (k + j < g.rank)
+                        y = fmaf(__ldcg(u + t * g.rank + k + j), __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16), y);
+            }
+        }
+        g.y[t * g.ldy + o] = __float2bfloat16_rn(y);
+    }
+}
+constexpr int kFewTokens = 32;
+
+template <int NT>
+cudaError_t launch_few(const Args& g, const float* u, cudaStream_t st) {
+    return launch_pdl(few_tokens_kernel<NT>, dim3((g.r + 15) / 16), dim3(256), 0, st, g, u);
+}
+
+template <int NT, bool BACKWARD>
+void launch_down(const Args& g, float* first, float* second, int32_t* lists, cudaStream_t st) {
+    const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16), chunks = (g.rank + 8 * NT - 1) / (8 * NT);
+    if (g.n <= 1024) {
+        // A small batch's tiles do not fill the GPU: a block for each adapter that a tile may hold, and
+        // eight for its features.  (One token, 4096 features, rank 16: 9.4 us with one block, READ_DOWN with eight.)
+        const int passes = std::min(16, g.na);
+        down_kernel<NT, BACKWARD, 8><<<dim3(8 * tiles, chunks, (second ? 2 : 1) * passes), 256, 0, st>>>(g, passes, first, second, lists);
+    } else {
+        down_kernel<NT, BACKWARD, 1><<<dim3(tiles, chunks, second ? 2 : 1), 256, 0, st>>>(g, 1, first, second, lists);
+    }
+}
 template <bool BACKWARD>
-int launch_down(const Args& g, float* first, float* second, int32_t* lists, cudaStream_t st) {
-    const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16), z = second ? 2 : 1;
-    if (g.rank <= 16) down_kernel<2, BACKWARD><<<dim3(tiles, 1, z), 256, 0, st>>>(g, first, second, lists);
-    else if (g.rank <= 32) down_kernel<4, BACKWARD><<<dim3(tiles, 1, z), 256, 0, st>>>(g, first, second, lists);
-    else down_kernel<8, BACKWARD><<<dim3(tiles, (g.rank + 63) / 64, z), 256, 0, st>>>(g, first, second, lists);
+int down(const Args& g, float* first, float* second, int32_t* lists, cudaStream_t st) {
+    if (g.rank <= 16) launch_down<2, BACKWARD>(g, first, second, lists, st);
+    else if (g.rank <= 32) launch_down<4, BACKWARD>(g, first, second, lists, st);
+    else launch_down<8, BACKWARD>(g, first, second, lists, st);
     return check_launch("down_kernel");
 }
 
@@ -456,9 +578,12 @@ extern "C" int tb_adapter_forward(const tb_adapter_args* p, void* stream) {
     Scratch s{};
     if ((rc = make_scratch(g, false, st, &s))) return rc;
     if (g.na) {
-        rc = launch_down<false>(g, s.u, nullptr, s.lists, st);
+        rc = down<false>(g, s.u, nullptr, s.lists, st);
     }
-    if (!rc) rc = linear::adapter_forward({g.n, g.r, g.d, g.x, g.ldx, g.w, g.ldw, g.y, g.ldy, g.who, s.lists, s.u, g.b, g.ldb, g.rank, g.na}, st);
+    if (!rc && g.n <= kFewTokens) {
+        const cudaError_t e = g.n <= 8 ? launch_few<1>(g, s.u, st) : g.n <= 16 ? launch_few<2>(g, s.u, st) : launch_few<4>(g, s.u, st);
+        rc = e == cudaSuccess ? check_launch("few_tokens_kernel") : cuda_fail(e, "few_tokens_kernel launch");
+    } else if (!rc) rc = linear::adapter_forward({g.n, g.r, g.d, g.x, g.ldx, g.w, g.ldw, g.y, g.ldy, g.who, s.lists, s.u, g.b, g.ldb, g.rank, g.na}, st);
     scratch_free(s.lists, st);
     return rc;
 }
@@ -486,7 +611,7 @@ extern "C" int tb_adapter_backward(const tb_adapter_args* p, void* stream) {
     Scratch s{};
     if ((rc = make_scratch(g, grads, st, &s))) return rc;
     if (s.lists) {
-        rc = launch_down<true>(g, s.v, grads ? s.u : nullptr, s.lists, st);
+        rc = down<true>(g, s.v, grads ? s.u : nullptr, s.lists, st);
     }
     if (!rc && g.dx && g.n)
         rc = linear::adapter_input_grad({g.n, g.d, g.r, g.dy, g.lddy, g.w, g.ldw, g.dx, g.lddx, g.who, s.lists, s.v, g.a, g.lda, g.rank, g.na}, st);
