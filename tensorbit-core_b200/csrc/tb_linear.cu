@@ -5,7 +5,7 @@
 // and NB/2 of the B columns of a K slice in shared memory, and its 128 x NB
 // half of the accumulator in TMEM.  Roles of a CTA's 16 warps:
 //   warp 12      TMA loads of K slices into a ring of stages;
-//   warps 8-11   "prepare" stages that do not arrive as operands: decode int8
+//   warps 8-11   (and 14-15) "prepare" stages that do not arrive as operands: decode int8
 //                codes to BF16 and zero what lies behind a sample's end, or
 //                build the operands of an adapter; then tell the even CTA;
 //   warp 13      (even CTA) issues tcgen05.mma for both CTAs;
@@ -47,6 +47,9 @@ __device__ int g_linear_error;
 
 constexpr int kThreads = 512;
 constexpr int kEpiWarps = 8, kPrepWarp = 8, kTmaWarp = 12, kMmaWarp = 13;
+// Codes are decoded by three groups of two warps (8-9, 10-11, 14-15), every third slice each: a
+// slice's chain of wait, loads, arithmetic, stores, fence and arrival overlaps the next ones'.
+constexpr int kDecodeGroups = 3;
 
 template <int MODE>
 struct Cfg {
@@ -62,9 +65,9 @@ struct Cfg {
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
     static constexpr int kExps = kCodes ? 2 * kCols : 0;               // exponents of its first block and the next
     static constexpr int kStage = kA + kB + (kRaw + kExps + 1023) / 1024 * 1024;
-    // Arrivals that make a stage ready: the prepare warps of both CTAs (codes), the even CTA's
+    // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
-    static constexpr int kReady = kCodes ? 8 : kAdapter ? 9 : 1;
+    static constexpr int kReady = kCodes ? 4 : kAdapter ? 9 : 1;
     static constexpr int kStages = MODE == kGrad ? 5 : MODE == kFisher ? 7 : 6;
     static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kColScale + 1024 + 512;
@@ -642,50 +645,60 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 }
             }
             __syncwarp();
-        } else if (C::kCodes && warp >= kPrepWarp && warp < kTmaWarp) {
+        } else if (C::kCodes) {
             // 8 consecutive features (one 16-byte unit of the operand) of every kRowStep-th token
-            constexpr int kUnits = C::kCols / 8, kRowStep = 128 / kUnits, kSteps = 64 / kRowStep;
-            const int pt = threadIdx.x - kPrepWarp * 32, pc = pt % kUnits, pr = pt / kUnits;
+            constexpr int kUnits = C::kCols / 8, kRowStep = 64 / kUnits, kSteps = 64 / kRowStep;
+            const int group = warp < kTmaWarp ? (warp - kPrepWarp) >> 1 : 2;
+            const int pt = (warp & 1) * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
             Ring<kStages> at;
+            int turn = 0;
             const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int, int, int i) {
                 const int s = at.s;
+                const uint32_t phase = at.phase;
+                at.next();
+                const bool mine = turn == group;
+                turn = turn == kDecodeGroups - 1 ? 0 : turn + 1;
+                if (!mine) return true;
                 const int k0 = u.lo + i * 64;
                 const int valid = min(64, u.hi - k0);
                 const int border = 128 - (k0 & 127);  // first token of the next block
-                if (!wait(smem_u32(&full[s]), at.phase, abort_flag)) return false;
+                if (!wait(smem_u32(&full[s]), phase, abort_flag)) return false;
                 uint8_t* stage = smem + s * C::kStage;
                 const uint8_t* raw = stage + C::kA + C::kB;
-                uint2 w[kSteps];
-#pragma unroll
-                for (int q = 0; q < kSteps; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + q * kRowStep) * C::kCols + pc * 8);
                 uint32_t s0[4];
                 act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8), s0);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
-                if (valid == 64 && border >= 64) {
+                const bool whole = valid == 64 && border >= 64;
+                uint32_t s1[4] = {0, 0, 0, 0};
+                if (!whole) act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
 #pragma unroll
-                    for (int q = 0; q < kSteps; ++q) {
-                        const int k = pr + q * kRowStep;
-                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
-                    }
-                } else {  // a block's or the sample's end within the slice
-                    uint32_t s1[4];
-                    act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
+                for (int h = 0; h < kSteps; h += 8) {
+                    uint2 w[8];
 #pragma unroll
-                    for (int q = 0; q < kSteps; ++q) {
-                        const int k = pr + q * kRowStep;
-                        uint32_t sk[4];
+                    for (int q = 0; q < 8; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + (h + q) * kRowStep) * C::kCols + pc * 8);
+                    if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
-                        *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
+                        for (int q = 0; q < 8; ++q) {
+                            const int k = pr + (h + q) * kRowStep;
+                            *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
+                        }
+                    } else {  // a block's or the sample's end within the slice
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const int k = pr + (h + q) * kRowStep;
+                            uint32_t sk[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
+                            *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
+                        }
                     }
                 }
                 // tokens behind the sample's end: dY may hold anything there
-                for (int q = pt; q < (64 - valid) * 16; q += 128)
+                for (int q = pt; q < (64 - valid) * 16; q += 64)
                     *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + (valid + (q >> 4)) * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&ready[s]));
-                at.next();
                 return true;
             });
             if (!done) give_up(abort_flag);
