@@ -57,11 +57,12 @@ struct Cfg {
     static constexpr bool kAdapter = MODE == kFwd || MODE == kDx;
     static constexpr bool kPromote = !kAdapter;
     static constexpr int NB = MODE == kFisher ? 128 : 256;             // columns of a pair's tile
+    static constexpr int kAcc = 512 / NB;                              // accumulators in TMEM
     static constexpr int kCols = NB / 2;                               // columns of an epilogue warp, and of a CTA's B
     // K slices summed in TMEM before they are added in FP32: 256 tokens, or one block of codes
     static constexpr int kGroup = kCodes ? 4 : MODE == kHess ? 1 : 1 << 30;
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
-    static constexpr int kB = MODE == kHess ? 16384 : kCols * 128;
+    static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
     static constexpr int kExps = kCodes ? 2 * kCols : 0;               // exponents of its first block and the next
     static constexpr int kStage = kA + kB + (kRaw + kExps + 1023) / 1024 * 1024;
@@ -140,14 +141,45 @@ __device__ __forceinline__ void mma_step(uint32_t tmem, uint64_t a, uint64_t b, 
             "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
             ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
 }
-// 128-byte-swizzle operand descriptors.  K-major: 8-row atoms 1024 bytes apart.
-// MN-major: rows of K are 128 bytes of M or N, 8-row atoms 1024 bytes apart
-// along K, the next 128 bytes of M or N `kMnChunk` further.
+// 128-byte-swizzle operand descriptors.  K-major: rows of M or N are 128 bytes of
+// K, 8-row atoms 1024 bytes apart.  MN-major: rows of K are 128 bytes of M or N,
+// 8-row atoms 1024 bytes apart along K, the next 128 bytes of M or N `kMnChunk`
+// further.
 constexpr int kMnChunk = 64 * 128;
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
     const uint64_t lbo = mn ? kMnChunk >> 4 : 1;
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (lbo << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
+// Sixteen accumulator columns of this lane's row: the read, and the wait for all reads under way.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// Two lanes of a += v, and of a += (m * row + base) * col, in packed FP32 (round to nearest).
+__device__ __forceinline__ void add2(float& a0, float& a1, uint32_t v0, uint32_t v1) {
+    asm("{\n\t.reg .b64 A, V;\n\tmov.b64 A, {%0, %1};\n\tmov.b64 V, {%2, %3};\n\t"
+        "add.rn.f32x2 A, A, V;\n\tmov.b64 {%0, %1}, A;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "r"(v0), "r"(v1));
+}
+__device__ __forceinline__ void scale_add2(float& a0, float& a1, uint32_t m0, uint32_t m1, float row, float base, float c0, float c1) {
+    asm("{\n\t.reg .b64 A, M, R, B, C;\n\tmov.b64 A, {%0, %1};\n\tmov.b64 M, {%2, %3};\n\t"
+        "mov.b64 R, {%4, %4};\n\tmov.b64 B, {%5, %5};\n\tmov.b64 C, {%6, %7};\n\t"
+        "fma.rn.f32x2 M, M, R, B;\n\tfma.rn.f32x2 A, M, C, A;\n\tmov.b64 {%0, %1}, A;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "r"(m0), "r"(m1), "f"(row), "f"(base), "f"(c0), "f"(c1));
+}
+// A load that counts on the even CTA's barrier.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t even_bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -174,7 +206,7 @@ struct Unit {
 template <int MODE>
 __device__ __forceinline__ Tile tile_of(const Params& P, int item) {
     Tile t{0, 0, 0};
-    if constexpr (MODE == kHess) {  // lower triangle, row by row
+    if constexpr (MODE == kHess) {  // tiles on or below the diagonal, row by row
         int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(item) + 1.0f) - 1.0f) * 0.5f);
         while (tm * (tm + 1) / 2 > item) --tm;
         while ((tm + 1) * (tm + 2) / 2 <= item) ++tm;
@@ -386,9 +418,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * C::kStage + C::kColScale);
     uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
     uint64_t* empty = ready + kStages;    // stage read by the MMAs
-    uint64_t* accfull = empty + kStages;  // [2] accumulator finished
-    uint64_t* accempty = accfull + 2;     // [2] (even CTA) accumulator taken by both CTAs
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    uint64_t* accfull = empty + kStages;      // [kAcc] accumulator finished
+    uint64_t* accempty = accfull + C::kAcc;   // [kAcc] (even CTA) accumulator taken by both CTAs
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + C::kAcc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
@@ -403,7 +435,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             mbar_init(smem_u32(&ready[s]), C::kReady);
             mbar_init(smem_u32(&empty[s]), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < C::kAcc; ++b) {
             mbar_init(smem_u32(&accfull[b]), 1);
             mbar_init(smem_u32(&accempty[b]), 2 * kEpiWarps);
         }
@@ -412,7 +444,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(tmem_slot)), "r"(2 * NB));
+                     ::"r"(smem_u32(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
     fence_before();
@@ -431,17 +463,17 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
         const int row_in = rank * 128 + quad * 32 + lane;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * COLS);
         bool ok = true;
-        int gc = 0;  // accumulator uses so far
+        Ring<C::kAcc> ac;
         for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
             const Tile t = tile_of<MODE>(P, item);
             const long long row = static_cast<long long>(t.tm) * 256 + row_in;
             const long long col = static_cast<long long>(t.tn) * NB + half * COLS;
             const int valid = row < P.M ? static_cast<int>(max(0ll, min(static_cast<long long>(COLS), P.N - col))) : 0;
             if constexpr (C::kAdapter) {
-                const int b = gc & 1;
-                if (!wait(smem_u32(&accfull[b]), (gc >> 1) & 1, abort_flag)) { ok = false; break; }
+                const int b = ac.s;
+                if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
                 fence_after();
-                ++gc;
+                ac.next();
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
                     float v[32];
@@ -498,43 +530,56 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                             __syncwarp();
                             if (g + 1 < groups) load_exps(g + 1);
                         }
-                        const int b = gc & 1;
-                        if (!wait(smem_u32(&accfull[b]), (gc >> 1) & 1, abort_flag)) { ok = false; break; }
+                        const int b = ac.s;
+                        if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
                         fence_after();
-                        ++gc;
+                        ac.next();
+                        // 16 columns at a time, the next read under way while these are added; the accumulator
+                        // is given back before the last are
+                        uint32_t v[2][16];
+                        const uint32_t from = lane_base + static_cast<uint32_t>(b * NB);
+                        tmem_ld16(from, v[0]);
 #pragma unroll
-                        for (int c = 0; c < COLS / 32; ++c) {
-                            float v[32];
-                            tmem_ld32(lane_base + static_cast<uint32_t>(b * NB + c * 32), v);
+                        for (int c = 0; c < COLS / 16; ++c) {
+                            uint32_t (&x)[16] = v[c & 1];
+                            tmem_wait16(x);
+                            if (c + 1 < COLS / 16) {
+                                tmem_ld16(from + static_cast<uint32_t>(16 * (c + 1)), v[(c + 1) & 1]);
+                            } else {
+                                fence_before();
+                                __syncwarp();
+                                if (lane == 0) arrive_even(smem_u32(&accempty[b]));
+                            }
                             if constexpr (MODE == kHess) {
                                 // |block sum| <= 128 * 127^2 < 2^22: as the low bits of 1.5 * 2^23 it is an
                                 // exact FP32 value, and subtracting that base times the row's power of two too
                                 const float base = -12582912.0f * srow;
 #pragma unroll
-                                for (int q = 0; q < 8; ++q) {
-                                    const float4 sc = *reinterpret_cast<const float4*>(scol + (g & 1) * COLS + c * 32 + 4 * q);
-                                    const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const float m = __uint_as_float(0x4B400000u + __float_as_uint(v[4 * q + i]));
-                                        const float x = fmaf(m, srow, base);
-                                        acc[c * 32 + 4 * q + i] = fmaf(x, s4[i], acc[c * 32 + 4 * q + i]);
-                                    }
+                                for (int q = 0; q < 4; ++q) {
+                                    const float4 sc = *reinterpret_cast<const float4*>(scol + (g & 1) * COLS + c * 16 + 4 * q);
+                                    float* to = acc + c * 16 + 4 * q;
+                                    scale_add2(to[0], to[1], 0x4B400000u + x[4 * q], 0x4B400000u + x[4 * q + 1], srow, base, sc.x, sc.y);
+                                    scale_add2(to[2], to[3], 0x4B400000u + x[4 * q + 2], 0x4B400000u + x[4 * q + 3], srow, base, sc.z, sc.w);
                                 }
                             } else {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) acc[c * 32 + i] = __fadd_rn(acc[c * 32 + i], v[i]);
+                                for (int i = 0; i < 16; i += 2) add2(acc[c * 16 + i], acc[c * 16 + i + 1], x[i], x[i + 1]);
                             }
                         }
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) arrive_even(smem_u32(&accempty[b]));
                     }
                     if (!ok) break;
                     if constexpr (MODE == kFisher) {
                         const bool first = P.first && s == 0;
+                        const uint64_t beta2 = pack2(P.beta, P.beta), contrib2 = pack2(P.contrib, P.contrib);
 #pragma unroll
-                        for (int i = 0; i < COLS; ++i) F[i] = first ? ema_first(P.alpha, acc[i]) : ema_next(F[i], P.beta, P.contrib, acc[i]);
+                        for (int i = 0; i < COLS; i += 2) {
+                            if (first) {
+                                F[i] = ema_first(P.alpha, acc[i]);
+                                F[i + 1] = ema_first(P.alpha, acc[i + 1]);
+                            } else {
+                                ema_next2(F[i], F[i + 1], beta2, contrib2, acc[i], acc[i + 1]);
+                            }
+                        }
                     } else if constexpr (MODE == kGrad) {
                         const long long at = t.s * P.out_stride + row * P.ldo + col;
                         if (P.out_bf16) store_bf16<COLS>(static_cast<bf16*>(P.out) + at, acc, valid);
@@ -609,19 +654,19 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             __syncwarp();
         } else if (warp == kMmaWarp) {
             if (lane == 0 && rank == 0) {
-                constexpr bool kAmn = C::kCodes || MODE == kHess, kBmn = kAmn || MODE == kDx;
+                constexpr bool kAmn = !C::kAdapter, kBmn = MODE != kFwd;
                 constexpr uint32_t kIdesc = ((MODE == kHess ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) |
                                             (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((NB >> 3) << 17) | (16u << 24);
-                // descriptor steps of one MMA: K-major 32 bytes along a row; MN-major 16 (int8: 32) rows of 128 bytes
-                constexpr uint64_t kStepMn = MODE == kHess ? 4096 >> 4 : 2048 >> 4;
+                // descriptor steps of one MMA: K-major 32 bytes along a row; MN-major 16 (int8: 32) rows
+                constexpr uint64_t kStepMn = (MODE == kHess ? 32 : 16) * 128 >> 4;
                 constexpr uint64_t kStepA = kAmn ? kStepMn : 2, kStepB = kBmn ? kStepMn : 2;
                 Ring<kStages> at;
-                int gc = 0;
+                Ring<C::kAcc> ac;
                 const uint64_t a_desc = operand_desc(stage_a(0), kAmn), b_desc = operand_desc(stage_b(0), kBmn);
                 const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int j, int, int) {
                     const bool first = j % C::kGroup == 0;
-                    const int b = gc & 1;
-                    if (first && !wait(smem_u32(&accempty[b]), ((gc >> 1) & 1) ^ 1, abort_flag)) return false;
+                    const int b = ac.s;
+                    if (first && !wait(smem_u32(&accempty[b]), ac.phase ^ 1, abort_flag)) return false;
                     const int s = at.s;
                     if (!wait(smem_u32(&ready[s]), at.phase, abort_flag)) return false;
                     fence_after();
@@ -634,14 +679,13 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     at.next();
                     if (j + 1 == u.total || j % C::kGroup == C::kGroup - 1) {
                         commit_pair(smem_u32(&accfull[b]));
-                        ++gc;
+                        ac.next();
                     }
                     return true;
                 });
                 if (!done) {
                     give_up(abort_flag);
-                    commit_pair(smem_u32(&accfull[0]));  // releases the waiting epilogues
-                    commit_pair(smem_u32(&accfull[1]));
+                    for (int b = 0; b < C::kAcc; ++b) commit_pair(smem_u32(&accfull[b]));  // releases the waiting epilogues
                 }
             }
             __syncwarp();
@@ -733,7 +777,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     cluster_sync_all();
     if (warp == 0) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NB));
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -757,7 +801,7 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant_
     }
 }
 
-// Row-major [rows][cols] of `esize`-byte elements, boxes of box_cols x box_rows.
+// Row-major [rows][cols] of `esize`-byte elements, boxes of box_cols x box_rows (128-byte swizzle or none).
 int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long long rows, long long ld, int box_cols,
              int box_rows, bool swizzle) {
     EncodeFn enc = encode_fn();
@@ -860,7 +904,7 @@ int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples,
 int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaStream_t st) {
     Params P{};
     P.M = P.N = ck.d;
-    P.tiles_m = P.tiles_n = tiles(ck.d, 256);
+    P.tiles_m = tiles(ck.d, 256);
     P.exps = ck.exps;
     P.lde = ck.lde;
     P.n = static_cast<int>(ck.n);
