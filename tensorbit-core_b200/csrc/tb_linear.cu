@@ -310,6 +310,24 @@ __device__ __forceinline__ void store_f32(float* p, const float (&v)[COLS], int 
     }
 }
 template <int COLS>
+__device__ __forceinline__ void add_f32(float (&v)[COLS], const float* p, int valid) {
+    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+        for (int c = 0; c < COLS / 8; ++c) {
+            float w[8];
+            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
+                         : "l"(p + 8 * c));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[8 * c + i] += w[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i)
+            if (i < valid) v[i] += p[i];
+    }
+}
+template <int COLS>
 __device__ __forceinline__ void store_bf16(bf16* p, const float (&v)[COLS], int valid) {
     if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
@@ -587,7 +605,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     } else if (col / 128 <= row / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
                         float* h = static_cast<float*>(P.out) + row * P.ldo + col;
 #pragma unroll
-                        for (int i = 0; i < COLS; ++i) acc[i] = P.accumulate && i < valid ? __fadd_rn(h[i], P.scale * acc[i]) : P.scale * acc[i];
+                        for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
+                        if (P.accumulate) add_f32<COLS>(acc, h, valid);
                         store_f32<COLS>(h, acc, valid);
                     }
                 }
