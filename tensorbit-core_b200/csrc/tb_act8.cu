@@ -25,38 +25,44 @@ int check(const tb_act8* ck, const char* who, View* v) {
 
 namespace {
 
-// One block of 256 threads holds 128 tokens x 128 features in registers, so X
-// is read once: thread (row, col) has 8 consecutive features of 8 tokens.
+// One block of 256 threads holds 128 tokens x 128 features in registers as they
+// are stored, so X is read once: thread (row, col) has 8 consecutive features of
+// 8 tokens.  Bound by memory: the largest magnitudes are found on the values'
+// own bits, and a code costs one multiply-add: x 2^(127-E) + 1.5 2^23 holds
+// rint(x 2^(127-E)), ties to even, in its low bits, the first product being exact.
 constexpr int kFeat = 128, kRowsPass = 16, kPasses = kBlock / kRowsPass;
 
+// Eight consecutive values as stored.
+template <int DT>
+struct Eight {
+    uint32_t w[DT == TB_F32 ? 8 : 4];
+    // value i's bits in FP32
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (DT == TB_F32) return __uint_as_float(w[i]);
+        else if constexpr (DT == TB_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(w[i >> 1] >> (16 * (i & 1)))));
+    }
+};
+
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* x, long long at, int valid, float (&v)[8]) {
-    using E = Elem<DT>;
+__device__ __forceinline__ Eight<DT> load8(const void* x, long long at, int valid) {
+    Eight<DT> v{};
     if (VEC && valid >= 8) {
-        if constexpr (DT == TB_F32) {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-            const float4 lo = p[0], hi = p[1];
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-        } else {
-            const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(x) + at * (DT == TB_F32 ? 4 : 2));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DT == TB_BF16) {
-                    v[2 * i] = __uint_as_float(w[i] << 16);
-                    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                }
-            }
+        for (int i = 0; i < (DT == TB_F32 ? 2 : 1); ++i) {
+            const uint4 q = __ldcs(p + i);
+            v.w[4 * i] = q.x; v.w[4 * i + 1] = q.y; v.w[4 * i + 2] = q.z; v.w[4 * i + 3] = q.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? E::load(x, at + i) : 0.0f;
+        for (int i = 0; i < 8; ++i) {
+            if (i >= valid) continue;
+            if constexpr (DT == TB_F32) v.w[i] = static_cast<const uint32_t*>(x)[at + i];
+            else v.w[i >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(x)[at + i]) << (16 * (i & 1));
+        }
     }
+    return v;
 }
 
 template <int DT, bool VEC>
@@ -67,56 +73,77 @@ __global__ void __launch_bounds__(256) pack_kernel(const View ck, const void* __
     const int f0 = blockIdx.x * kFeat + col * 8;
     const int valid = ck.d - f0;  // features of this thread (may be <= 0 or > 8)
     const long long t0 = static_cast<long long>(blockIdx.y) * kBlock;
-    float v[kPasses][8];
+    bool kept[kPasses];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const long long t = t0 + p * kRowsPass + row;
-        if (t < ck.n && valid > 0 && (!keep || keep[t])) load8<DT, VEC>(x, t * ldx + f0, valid, v[p]);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
+        kept[p] = t < ck.n && valid > 0 && (!keep || keep[t] != 0);
     }
+    Eight<DT> v[kPasses];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        uint32_t m = 0;
+    for (int p = 0; p < kPasses; ++p) {
+        v[p] = {};
+        if (kept[p]) v[p] = load8<DT, VEC>(x, (t0 + p * kRowsPass + row) * ldx + f0, valid);
+    }
+    if constexpr (DT == TB_F32) {
 #pragma unroll
-        for (int p = 0; p < kPasses; ++p) m = max(m, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
-        smax[row][col * 8 + i] = m;
+        for (int i = 0; i < 8; ++i) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) m = max(m, v[p].w[i] & 0x7FFFFFFFu);
+            smax[row][col * 8 + i] = m;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) m = __vmaxu2(m, v[p].w[i] & 0x7FFF7FFFu);
+            smax[row][col * 8 + 2 * i] = m & 0xFFFFu;
+            smax[row][col * 8 + 2 * i + 1] = m >> 16;
+        }
     }
     __syncthreads();
     if (threadIdx.x < kFeat) {
         uint32_t m = 0;
 #pragma unroll
         for (int r = 0; r < kRowsPass; ++r) m = max(m, smax[r][threadIdx.x]);
+        if constexpr (DT == TB_BF16) m <<= 16;
+        if constexpr (DT == TB_F16) m = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m)))) & 0x7FFFFFFFu;
         const uint32_t e = exponent_of(m);
-        smax[0][threadIdx.x] = e;
         const int f = blockIdx.x * kFeat + threadIdx.x;
         if (f < ck.d) ck.exps[blockIdx.y * ck.lde + f] = static_cast<uint8_t>(e);
+        smax[0][threadIdx.x] = e;
     }
     __syncthreads();
     if (valid <= 0) return;
-    uint32_t e[8];
     float inv[8];
+    uint32_t dead = 0;  // bytes of features whose block holds a NaN or an infinity: codes 0
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        e[i] = smax[0][col * 8 + i];
-        inv[i] = e[i] == 255u ? 0.0f : inverse_scale(e[i]);
+        const uint32_t e = smax[0][col * 8 + i];
+        dead |= e == 255u ? 1u << i : 0u;
+        inv[i] = e == 255u ? 0.0f : inverse_scale(e);
     }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const long long t = t0 + p * kRowsPass + row;
         if (t >= ck.n) break;
-        uint32_t w[2] = {0, 0};
+        uint32_t c[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int q = e[i] == 255u ? 0 : __float2int_rn(v[p][i] * inv[i]);
-            w[i >> 2] |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(fmaf(v[p].at(i), inv[i], 12582912.0f));
+        if (dead) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (dead >> i & 1) c[i] = 0;
         }
+        const uint32_t lo = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+        const uint32_t hi = prmt(prmt(c[4], c[5], 0x0040u), prmt(c[6], c[7], 0x0040u), 0x5410u);
         int8_t* out = ck.codes + t * ck.ldq + f0;
         if (valid >= 8) {
-            *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
         } else {
-            for (int i = 0; i < valid; ++i) out[i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
+            for (int i = 0; i < valid; ++i) out[i] = static_cast<int8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
         }
     }
 }
@@ -131,6 +158,8 @@ __global__ void __launch_bounds__(256) unpack_kernel(const View ck, void* __rest
     const long long t0 = static_cast<long long>(blockIdx.y) * kBlock;
     const uint2 ew = *reinterpret_cast<const uint2*>(ck.exps + blockIdx.y * ck.lde + f0);
     float s[8];
+    uint32_t s2[4];
+    scales8(ew, s2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = scale_f32(((i < 4 ? ew.x : ew.y) >> (8 * (i & 3))) & 0xFFu);
 #pragma unroll
@@ -138,11 +167,15 @@ __global__ void __launch_bounds__(256) unpack_kernel(const View ck, void* __rest
         const long long t = t0 + p * kRowsPass + row;
         if (t >= ck.n) break;
         const uint2 w = *reinterpret_cast<const uint2*>(ck.codes + t * ck.ldq + f0);
-        T o[8];
+        alignas(16) T o[8];
+        if constexpr (DT == TB_BF16) {
+            *reinterpret_cast<uint4*>(o) = decode8(w, s2);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int q = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-            o[i] = Elem<DT>::to(static_cast<float>(q) * s[i]);
+            for (int i = 0; i < 8; ++i) {
+                const int q = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+                o[i] = Elem<DT>::to(static_cast<float>(q) * s[i]);
+            }
         }
         T* dst = static_cast<T*>(out) + t * ldo + f0;
         if (VEC && valid >= 8) {

@@ -65,13 +65,17 @@ struct Cfg {
     static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
     static constexpr int kExps = kCodes ? 2 * kCols : 0;               // exponents of its first block and the next
-    static constexpr int kStage = kA + kB + (kRaw + kExps + 1023) / 1024 * 1024;
+    static constexpr int kStage = kA + kB + kRaw;
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
     static constexpr int kReady = kCodes ? 4 : kAdapter ? 9 : 1;
-    static constexpr int kStages = MODE == kGrad ? 5 : MODE == kFisher ? 7 : 6;
+    static constexpr int kStages = MODE == kGrad ? 4 : MODE == kFisher ? 7 : 6;
+    // Behind the stages: 8 KB a warp for results on their way out (kGrad), the exponents of each stage, column scales (kHess)
+    static constexpr int kOut = MODE == kGrad ? kEpiWarps * 8192 : 0;
     static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
-    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kColScale + 1024 + 512;
+    static constexpr int kExtra = kOut + kStages * kExps + kColScale;
+    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 512;
+    static_assert(kSmem <= 232448, "shared memory of a block");
 };
 
 struct Params {
@@ -86,7 +90,7 @@ struct Params {
     // results
     void* out;
     long long ldo, out_stride;
-    int out_bf16;
+    int out_bf16, out_tma;
     float alpha, beta, contrib, scale;
     int first, accumulate;
     // adapters; with splits > 1 the K range of a tile is shared out and FP32 sums go to part [splits][M][ldpart]
@@ -344,6 +348,39 @@ __device__ __forceinline__ void store_bf16(bf16* p, const float (&v)[COLS], int 
     }
 }
 
+// 32 rows x 128 columns of a sample's gradient through shared memory: a row of
+// 128 bytes a lane (128-byte swizzle), two pieces of 4 KB in flight.  Stored
+// straight from registers, one row a lane, the 537 MB of sixteen 4096 x 4096
+// gradients held the epilogue up: 400 us against 336.
+template <bool BF16>
+__device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, const float (&v)[128], int col, int row0, int s,
+                                          int N, int lane) {
+    constexpr int kPiece = BF16 ? 64 : 32;  // columns
+#pragma unroll
+    for (int c = 0; c < 128 / kPiece; ++c) {
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the piece before last has left its buffer
+        __syncwarp();
+        uint8_t* row = buf + (c & 1) * 4096 + lane * 128;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint4 w;
+            const float* x = v + c * kPiece + j * (kPiece / 8);
+            if constexpr (BF16) w = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            else w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+            *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = w;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            if (col + c * kPiece < N)
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                             "r"(col + c * kPiece), "r"(row0), "r"(s), "r"(smem_u32(buf + (c & 1) * 4096))
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
+
 // One result of an adapter product on its own.  An adapter's operands are zero
 // for the other tokens of its tile, but zero times an infinity or a NaN of that
 // adapter is not: a result that is not finite is formed again from what belongs
@@ -426,14 +463,17 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CUtensorMap tB,
-              const __grid_constant__ CUtensorMap tE, const __grid_constant__ Params P) {
+              const __grid_constant__ CUtensorMap tE, const __grid_constant__ CUtensorMap tO,
+              const __grid_constant__ Params P) {
     using C = Cfg<MODE>;
     constexpr int NB = C::NB, kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     // (by offset, so that the compiler still knows it for shared memory)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    float* col_scale = reinterpret_cast<float*>(smem + kStages * C::kStage);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * C::kStage + C::kColScale);
+    uint8_t* out_buf = smem + kStages * C::kStage;
+    uint8_t* exps_buf = out_buf + C::kOut;
+    float* col_scale = reinterpret_cast<float*>(exps_buf + kStages * C::kExps);
+    uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + C::kExtra);
     uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
     uint64_t* empty = ready + kStages;    // stage read by the MMAs
     uint64_t* accfull = empty + kStages;      // [kAcc] accumulator finished
@@ -600,7 +640,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         }
                     } else if constexpr (MODE == kGrad) {
                         const long long at = t.s * P.out_stride + row * P.ldo + col;
-                        if (P.out_bf16) store_bf16<COLS>(static_cast<bf16*>(P.out) + at, acc, valid);
+                        if (P.out_tma) {
+                            const int row0 = t.tm * 256 + rank * 128 + quad * 32;
+                            if (row0 < P.M && col < P.N) {
+                                uint8_t* buf = out_buf + warp * 8192;
+                                if (P.out_bf16) store_tma<true>(&tO, buf, acc, static_cast<int>(col), row0, t.s, static_cast<int>(P.N), lane);
+                                else store_tma<false>(&tO, buf, acc, static_cast<int>(col), row0, t.s, static_cast<int>(P.N), lane);
+                            }
+                        } else if (P.out_bf16) store_bf16<COLS>(static_cast<bf16*>(P.out) + at, acc, valid);
                         else store_f32<COLS>(static_cast<float*>(P.out) + at, acc, valid);
                     } else if (col / 128 <= row / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
                         float* h = static_cast<float*>(P.out) + row * P.ldo + col;
@@ -614,6 +661,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     if (ok) store_f32<COLS>(static_cast<float*>(P.out) + row * P.ldo + col, F, valid);
             }
         }
+        if constexpr (MODE == kGrad) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) give_up(abort_flag);
     } else {
         if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -633,7 +681,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         tma_load_2d(stage_a(s), &tA, m0, y, bar);
                         tma_load_2d(stage_a(s) + kMnChunk, &tA, m0 + 64, y, bar);
                         tma_load_2d(stage_raw(s), &tB, n0, k, bar);
-                        tma_load_2d(stage_raw(s) + C::kRaw, &tE, n0, k >> 7, bar);
+                        tma_load_2d(smem_u32(exps_buf + s * C::kExps), &tE, n0, k >> 7, bar);
                     } else {
                         const uint32_t bar = smem_u32(&ready[s]) & kPeerMask;
                         const bool built = C::kAdapter && part > 0;  // the prepare warps fill this stage
@@ -729,11 +777,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 uint8_t* stage = smem + s * C::kStage;
                 const uint8_t* raw = stage + C::kA + C::kB;
                 uint32_t s0[4];
-                act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + pc * 8), s0);
+                const uint8_t* exps = exps_buf + s * C::kExps + pc * 8;
+                act8::scales8(*reinterpret_cast<const uint2*>(exps), s0);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
                 const bool whole = valid == 64 && border >= 64;
                 uint32_t s1[4] = {0, 0, 0, 0};
-                if (!whole) act8::scales8(*reinterpret_cast<const uint2*>(raw + C::kRaw + C::kCols + pc * 8), s1);
+                if (!whole) act8::scales8(*reinterpret_cast<const uint2*>(exps + C::kCols), s1);
 #pragma unroll
                 for (int h = 0; h < kSteps; h += 8) {
                     uint2 w[8];
@@ -837,7 +886,7 @@ int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long
 }
 
 template <int MODE>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const Params& P, cudaStream_t st) {
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, const Params& P, cudaStream_t st) {
     using C = Cfg<MODE>;
     // Per device: the shared-memory limit, and that the launch has the registers that the roles' shares add up to.
     static std::mutex mu;
@@ -860,7 +909,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, con
     }
     constexpr int kPairs = 74;  // one CTA on each of the 148 SMs
     const int pairs = std::min(P.items, kPairs);
-    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, P);
+    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, o, P);
     return check_launch("linear_kernel");
 }
 
@@ -871,6 +920,21 @@ int set_items(Params* P, long long items, const char* who) {
     if (items > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, items);
     P->items = static_cast<int>(items);
     return TB_OK;
+}
+
+// Gradients [S][r][d] as boxes of 32 rows x 128 bytes, where every row starts on 16 bytes.
+int make_out_map(CUtensorMap* map, Params* P, int r, int d, int S) {
+    const int esize = P->out_bf16 ? 2 : 4;
+    P->out_tma = reinterpret_cast<uintptr_t>(P->out) % 16 == 0 && d * esize % 16 == 0 && P->out_stride * esize % 16 == 0;
+    EncodeFn enc = encode_fn();
+    if (!P->out_tma || !enc) return TB_OK;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(r), static_cast<cuuint64_t>(S)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(d) * esize, static_cast<cuuint64_t>(P->out_stride) * esize};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esize), 32, 1}, estr[3] = {1, 1, 1};
+    const CUresult e = enc(map, esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, P->out, dims,
+                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(e));
 }
 
 template <int MODE>
@@ -887,11 +951,12 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     P.parts = dy.parts;
     P.ldo = ck.d;
     int rc = set_items(&P, static_cast<long long>(P.tiles_m) * P.tiles_n * samples, who);
-    CUtensorMap a{}, b{}, e{};
+    CUtensorMap a{}, b{}, e{}, o{};
+    if (!rc && MODE == kGrad) rc = make_out_map(&o, &P, r, ck.d, static_cast<int>(samples));
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
     if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 2, false);
-    return rc ? rc : launch<MODE>(a, b, e, P, st);
+    return rc ? rc : launch<MODE>(a, b, e, o, P, st);
 }
 
 }  // namespace
@@ -934,7 +999,7 @@ int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaSt
     int rc = set_items(&P, static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2, "tb_act8_hessian");
     CUtensorMap a{};
     if (!rc && ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
-    return rc ? rc : launch<kHess>(a, a, a, P, st);
+    return rc ? rc : launch<kHess>(a, a, a, a, P, st);
 }
 
 template <int MODE>
@@ -962,7 +1027,7 @@ static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_
     if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
     if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
                                : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
-    if (!rc) rc = launch<MODE>(a, b, b, P, st);
+    if (!rc) rc = launch<MODE>(a, b, b, b, P, st);
     if (!rc && P.splits > 1) {
         const long long quads = P.M * ((P.N + 3) / 4);
         join_splits_kernel<MODE><<<static_cast<unsigned>(std::min((quads + 255) / 256, 148ll * 8)), 256, 0, st>>>(P);

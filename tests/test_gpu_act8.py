@@ -158,6 +158,23 @@ def test_weight_grad(cuda, tblib, n, r, d, dy_t, g_t, samples):
         check_sums(torch, out[s, : r * d].view(r, d), G, A, n * PARTS[dy_t], g_t == "bfloat16")
 
 
+@pytest.mark.parametrize("n,r,d,S", [(300, 130, 72, 3), (520, 300, 328, 2), (90, 33, 8, 4), (1000, 513, 264, 1), (64, 256, 1000, 2)])
+@pytest.mark.parametrize("g_t", ["float32", "bfloat16"])
+def test_weight_grad_densely_packed(cuda, tblib, n, r, d, S, g_t):
+    """Samples one behind the other without gaps, rows that start on 16 bytes: the results that leave by TMA."""
+    torch, tb = cuda, tblib
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, n))
+    dy = rows(torch, n, r, torch.bfloat16, n + 1, ref.up(r, 8), 1e-2, 0)
+    samples = [(i * n // S, (i + 1) * n // S) for i in range(S)]
+    out = torch.full((S * r * d + 64,), 3.0, device="cuda", dtype=getattr(torch, g_t))
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, pairs(torch, samples).data_ptr(), S,
+                                 out.data_ptr(), code(tb, torch, out.dtype)))
+    torch.cuda.synchronize()
+    assert bool((out[S * r * d:] == 3).all())
+    for s, (G, A) in enumerate(ref.gradients(torch, dy, c.values(torch), samples)):
+        check_sums(torch, out[s * r * d:(s + 1) * r * d].view(r, d), G, A, n, g_t == "bfloat16")
+
+
 def test_weight_grad_leaves_other_tokens_out(cuda, tblib):
     """NaN and infinities in tokens of no sample reach no gradient; those of one sample stay in it."""
     torch, tb = cuda, tblib
