@@ -107,6 +107,146 @@ __device__ __forceinline__ uint4 row8(const Rows& s, long long t, int f) {
     return f + 8 <= s.cols ? v : first_of(v, s.cols - f);
 }
 
+// The tokens of each adapter, in order, for batches of more than kSmallBatch
+// tokens: order[start ..] holds them, and every piece of 64 has an entry of
+// `tiles` at start / 64 + a + piece (adapters' entries cannot overlap there; an
+// entry without a piece has adapter -1).  One block per adapter: it counts the
+// tokens of lower adapters, then compacts its own.
+struct Order {
+    int2* span;     // [na] (start, count)
+    int2* tiles;    // [n / 64 + na] (adapter, piece)
+    int* tokens;    // [n]
+};
+constexpr int kSmallBatch = 1024;
+
+__global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o) {
+    __shared__ int scan[32], total[2];
+    const int a = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid < 2) total[tid] = 0;
+    __syncthreads();
+    int lower = 0, mine = 0;
+    for (long long t = tid; t < g.n; t += 1024) {
+        const int w = adapter_of(g, t);
+        lower += w >= 0 && w < a;
+        mine += w == a;
+    }
+    lower = __reduce_add_sync(~0u, lower);
+    mine = __reduce_add_sync(~0u, mine);
+    if (lane == 0) {
+        atomicAdd(&total[0], lower);
+        atomicAdd(&total[1], mine);
+    }
+    __syncthreads();
+    const int start = total[0], count = total[1];
+    if (tid == 0) o.span[a] = make_int2(start, count);
+    const int first = start / 64 + a, pieces = (count + 63) / 64, next = (start + count) / 64 + a + 1;
+    for (int p = tid; p < next - first; p += 1024) o.tiles[first + p] = make_int2(p < pieces ? a : -1, p);
+    if (a == g.na - 1)
+        for (long long p = next + tid; p < g.n / 64 + g.na; p += 1024) o.tiles[p] = make_int2(-1, 0);
+    int at = start;
+    for (long long base = 0; base < g.n; base += 4096) {  // four consecutive tokens a thread
+        int t[4], n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long q = base + 4 * tid + i;
+            if (q < g.n && adapter_of(g, q) == a) t[n++] = static_cast<int>(q);
+        }
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int v = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 31) scan[warp] = upto;
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int w = 0; w < 32; ++w) {
+            before += w < warp ? scan[w] : 0;
+            all += scan[w];
+        }
+        for (int i = 0; i < n; ++i) o.tokens[at + before + upto - n + i] = t[i];
+        at += all;
+        __syncthreads();
+    }
+}
+
+// acc[m][i] += rows of 16 tokens times ranks of adapter a, over every kstep-th
+// group of 32 features: lane (g, t) has features 8t..8t+7 of the group, rows
+// tok[2m], tok[2m+1] (-1: none) and ranks rank0 + g NT + i.  ALONG: M_a = a
+// [rank][lda], features along its rows; else M_a[k][c] = b [c][ldb].
+template <int NT, int MT, bool CODES, bool ALONG>
+__device__ __forceinline__ void accumulate(const Args& g, const Rows& src, int a, const int (&tok)[2 * MT], int rank0, int kg0,
+                                           int kstep, float (&acc)[MT][NT][4]) {
+    const int lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+    const int groups = (src.cols + 31) / 32;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll(MT == 1 && NT <= 4 ? 4 : 2)
+    for (int kg = kg0; kg < groups; kg += kstep) {
+        const int f = kg * 32 + 8 * tq;
+        const bool in = f < src.cols;
+        uint32_t x[2 * MT][4];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+            const uint4 v = in && tok[i] >= 0 ? row8<CODES>(src, tok[i], f) : zero;
+            x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+        }
+        if constexpr (ALONG) {
+            uint4 m[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int k = rank0 + gq * NT + i;
+                m[i] = in && k < g.rank ? __ldg(reinterpret_cast<const uint4*>(g.a + (static_cast<long long>(a) * g.rank + k) * g.lda + f)) : zero;
+                if (f + 8 > src.cols) m[i] = first_of(m[i], src.cols - f);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int q = 0; q < MT; ++q) {
+                    mma16816(acc[q][i], x[2 * q][0], x[2 * q + 1][0], x[2 * q][1], x[2 * q + 1][1], m[i].x, m[i].y);
+                    mma16816(acc[q][i], x[2 * q][2], x[2 * q + 1][2], x[2 * q][3], x[2 * q + 1][3], m[i].z, m[i].w);
+                }
+        } else {
+            // rows of b at eight consecutive features, NT ranks each
+            uint32_t m[8][NT / 2];
+            const int k0 = rank0 + gq * NT;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bf16* p = g.b + (static_cast<long long>(a) * g.r + f + j) * g.ldb + k0;
+                const bool have = f + j < src.cols;
+                if (have && k0 + NT <= g.rank) {
+                    load_words(p, m[j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NT / 2; ++i) {  // ranks behind the last are zeros (ldb is even)
+                        m[j][i] = have && k0 + 2 * i < g.rank ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+                        if (k0 + 2 * i + 1 >= g.rank) m[j][i] &= 0xFFFFu;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
+                const uint32_t b0 = __byte_perm(m[0][i / 2], m[1][i / 2], sel), b1 = __byte_perm(m[2][i / 2], m[3][i / 2], sel);
+                const uint32_t b2 = __byte_perm(m[4][i / 2], m[5][i / 2], sel), b3 = __byte_perm(m[6][i / 2], m[7][i / 2], sel);
+#pragma unroll
+                for (int q = 0; q < MT; ++q) {
+                    mma16816(acc[q][i], x[2 * q][0], x[2 * q + 1][0], x[2 * q][1], x[2 * q + 1][1], b0, b1);
+                    mma16816(acc[q][i], x[2 * q][2], x[2 * q + 1][2], x[2 * q][3], x[2 * q + 1][3], b2, b3);
+                }
+            }
+        }
+    }
+}
+// One warp's 16 x RC sums into its place of `red`: column 2t + e of fragment i is rank (2t + e) NT + i.
+template <int NT>
+__device__ __forceinline__ void stage_sums(float (*red)[16][8 * NT], const float (&acc)[NT][4]) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[warp][gq + 8 * (e >> 1)][(2 * tq + (e & 1)) * NT + i] = acc[i][e];
+}
+
 // The value at `p`'s place in the shared memory of block `rank` of this cluster.
 __device__ __forceinline__ float load_peer(const float* p, uint32_t rank) {
     float v;
@@ -117,28 +257,24 @@ __device__ __forceinline__ float load_peer(const float* p, uint32_t rank) {
     return v;
 }
 
-// u[t][k] = scale[a] sum_c row_t[c] M_a[k][c] for the tokens with an adapter:
-// 16 tokens and RC = 8 NT ranks per block, the features split over its 8 warps
-// in groups of 32 and the warps' sums joined in order.  One pass for each
-// adapter among the 16 tokens (runs of one request have one; a pass costs what
-// the 16 tokens of one adapter do, bound by reading M_a from L2).
-// ALONG: M_a = a [rank][lda], features along its rows; else M_a[k][c] = b [c][ldb].
-// SPLIT > 1: a cluster of that many blocks shares the features of one tile and
-// joins its sums over distributed shared memory, in order.
-template <int NT, bool CODES, bool ALONG, int SPLIT>
-__device__ __forceinline__ void down_project(const Args& g, const Rows& src, float* __restrict__ u, float (*red)[16][8 * NT],
-                                             int* who, int passes, int mine_pass) {
+// u[t][k] = scale[a] sum_c row_t[c] M_a[k][c] for the tokens with an adapter.
+
+// Small batches: 16 consecutive tokens per cluster of kSplit blocks, which share
+// their features out over 8 kSplit warps and join the sums in order, the blocks'
+// over distributed shared memory.  One pass for each adapter among the 16
+// tokens; blockIdx.z spreads the passes over blocks (every passes-th).
+constexpr int kSplit = 8;
+template <int NT, bool CODES, bool ALONG>
+__device__ __forceinline__ void down_small(const Args& g, const Rows& src, float* __restrict__ u, float (*red)[16][8 * NT],
+                                           int* who, int passes, int mine_pass) {
     constexpr int RC = 8 * NT;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-    const int share = blockIdx.x % SPLIT;
-    const long long t0 = blockIdx.x / SPLIT * 16ll;
-    const int rank0 = blockIdx.y * RC;
+    const int gq = (threadIdx.x & 31) >> 2, share = blockIdx.x % kSplit;
+    const int t0 = blockIdx.x / kSplit * 16, rank0 = blockIdx.y * RC;
     if (threadIdx.x < 16) who[threadIdx.x] = t0 + threadIdx.x < g.n ? adapter_of(g, t0 + threadIdx.x) : -1;
     __syncthreads();
     unsigned rem = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) rem |= who[i] >= 0 ? 1u << i : 0u;
-    const int groups = (src.cols + 31) / 32;
     for (int pass = 0; rem; ++pass) {
         const int a = who[__ffs(rem) - 1];
         unsigned mine = 0;
@@ -146,204 +282,209 @@ __device__ __forceinline__ void down_project(const Args& g, const Rows& src, flo
         for (int i = 0; i < 16; ++i) mine |= who[i] == a ? 1u << i : 0u;
         rem &= ~mine;
         if (pass % passes != mine_pass) continue;
-        float acc[NT][4] = {};
-        const bool r0 = mine >> gq & 1, r1 = mine >> (gq + 8) & 1;
-#pragma unroll(NT <= 4 ? 4 : 2)
-        for (int kg = share * 8 + warp; kg < groups; kg += 8 * SPLIT) {
-            const int f = kg * 32 + 8 * tq;
-            const bool in = f < src.cols;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const uint4 x0 = in && r0 ? row8<CODES>(src, t0 + gq, f) : zero, x1 = in && r1 ? row8<CODES>(src, t0 + gq + 8, f) : zero;
-            const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
-            if constexpr (ALONG) {
-                uint4 m[NT];
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const int k = rank0 + gq * NT + i;
-                    m[i] = in && k < g.rank ? __ldg(reinterpret_cast<const uint4*>(g.a + (static_cast<long long>(a) * g.rank + k) * g.lda + f)) : zero;
-                    if (f + 8 > src.cols) m[i] = first_of(m[i], src.cols - f);
-                }
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    mma16816(acc[i], w0[0], w1[0], w0[1], w1[1], m[i].x, m[i].y);
-                    mma16816(acc[i], w0[2], w1[2], w0[3], w1[3], m[i].z, m[i].w);
-                }
-            } else {
-                // rows of b at eight consecutive features, NT ranks each
-                uint32_t m[8][NT / 2];
-                const int k0 = rank0 + gq * NT;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bf16* p = g.b + (static_cast<long long>(a) * g.r + f + j) * g.ldb + k0;
-                    const bool have = f + j < src.cols;
-                    if (have && k0 + NT <= g.rank) {
-                        load_words(p, m[j]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NT / 2; ++i) {  // ranks behind the last are zeros (ldb is even)
-                            m[j][i] = have && k0 + 2 * i < g.rank ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
-                            if (k0 + 2 * i + 1 >= g.rank) m[j][i] &= 0xFFFFu;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
-                    mma16816(acc[i], w0[0], w1[0], w0[1], w1[1], __byte_perm(m[0][i / 2], m[1][i / 2], sel), __byte_perm(m[2][i / 2], m[3][i / 2], sel));
-                    mma16816(acc[i], w0[2], w1[2], w0[3], w1[3], __byte_perm(m[4][i / 2], m[5][i / 2], sel), __byte_perm(m[6][i / 2], m[7][i / 2], sel));
-                }
-            }
-        }
-        // column 2t + e of fragment i is rank (2t + e) NT + i
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) red[warp][gq + 8 * (e >> 1)][(2 * tq + (e & 1)) * NT + i] = acc[i][e];
+        float acc[1][NT][4] = {};
+        const int tok[2] = {mine >> gq & 1 ? t0 + gq : -1, mine >> (gq + 8) & 1 ? t0 + gq + 8 : -1};
+        accumulate<NT, 1, CODES, ALONG>(g, src, a, tok, rank0, share * 8 + (threadIdx.x >> 5), 8 * kSplit, acc);
+        stage_sums<NT>(red, acc[0]);
         __syncthreads();
-        if constexpr (SPLIT == 1) {
-            for (int i = threadIdx.x; i < 16 * RC; i += 256) {
-                const int row = i / RC, k = rank0 + i % RC;
-                float sum = 0.0f;
+        for (int i = threadIdx.x; i < 16 * RC; i += 256) {  // each sum has one thread: in place
+            float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 8; ++w) sum += red[w][row][i % RC];
-                if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
-            }
-            __syncthreads();
-        } else {
-            for (int i = threadIdx.x; i < 16 * RC; i += 256) {  // each sum has one thread: in place
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 8; ++w) sum += red[w][i / RC][i % RC];
-                red[0][i / RC][i % RC] = sum;
-            }
-            umma::cluster_sync_all();
-            for (int i = share * 256 + threadIdx.x; i < 16 * RC; i += SPLIT * 256) {
-                const int row = i / RC, k = rank0 + i % RC;
-                float v[SPLIT], sum = 0.0f;
-#pragma unroll
-                for (int q = 0; q < SPLIT; ++q) v[q] = load_peer(&red[0][row][i % RC], q);
-#pragma unroll
-                for (int q = 0; q < SPLIT; ++q) sum += v[q];
-                if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
-            }
-            umma::cluster_sync_all();  // no block writes its sums again, or leaves, before they have been read
+            for (int w = 0; w < 8; ++w) sum += red[w][i / RC][i % RC];
+            red[0][i / RC][i % RC] = sum;
         }
+        umma::cluster_sync_all();
+        for (int i = share * 256 + threadIdx.x; i < 16 * RC; i += kSplit * 256) {
+            const int row = i / RC, k = rank0 + i % RC;
+            float v[kSplit], sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < kSplit; ++q) v[q] = load_peer(&red[0][row][i % RC], q);
+#pragma unroll
+            for (int q = 0; q < kSplit; ++q) sum += v[q];
+            if ((mine >> row & 1) && k < g.rank) u[(t0 + row) * g.rank + k] = g.scale[a] * sum;
+        }
+        umma::cluster_sync_all();  // no block writes its sums again, or leaves, before they have been read
     }
 }
 
 // blockIdx.z = passes * q + p.  q = 0: the forward's u (from x) or the backward's
-// v (from dy); 1: the backward's u (from the checkpoint).  p: of a tile's
-// adapters, every passes-th.
-template <int NT, bool BACKWARD, int SPLIT>
-__global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(256) down_kernel(const Args g, const int passes,
-                                                                                float* __restrict__ first,
-                                                                                float* __restrict__ second,
-                                                                                int32_t* __restrict__ lists) {
+// v (from dy); 1: the backward's u (from the checkpoint).
+template <int NT, bool BACKWARD>
+__global__ void __cluster_dims__(kSplit, 1, 1) __launch_bounds__(256)
+down_small_kernel(const Args g, const int passes, float* __restrict__ first, float* __restrict__ second, int32_t* __restrict__ lists) {
     __shared__ float red[8][16][8 * NT];
     __shared__ int who[256];
     const int p = blockIdx.z % passes;
     asm volatile("griddepcontrol.launch_dependents;");  // few_tokens_kernel waits before it reads u
     if constexpr (!BACKWARD) {
-        down_project<NT, false, true, SPLIT>(g, {g.x, g.ldx, {}, g.d}, first, red, who, passes, p);
+        down_small<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, first, red, who, passes, p);
     } else {
-        if (static_cast<int>(blockIdx.z) < passes) down_project<NT, false, false, SPLIT>(g, {g.dy, g.lddy, {}, g.r}, first, red, who, passes, p);
-        else down_project<NT, true, true, SPLIT>(g, {nullptr, 0, g.x8, g.d}, second, red, who, passes, p);
+        if (static_cast<int>(blockIdx.z) < passes) down_small<NT, false, false>(g, {g.dy, g.lddy, {}, g.r}, first, red, who, passes, p);
+        else down_small<NT, true, true>(g, {nullptr, 0, g.x8, g.d}, second, red, who, passes, p);
     }
-    if (blockIdx.x % (16 * SPLIT) == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    if (blockIdx.x % (16 * kSplit) == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         __syncthreads();
-        list_adapters(g, blockIdx.x / (16 * SPLIT), who, lists);
+        list_adapters(g, blockIdx.x / (16 * kSplit), who, lists);
     }
 }
 
-// out_a[c][k] = sum over the tokens of adapter a of row_t[c] val_t[k]: 128
-// features and RC ranks per block, the tokens of the block's share compacted in
-// order and taken 64 at a time, 16 for each pair of warps; val enters as two
-// BF16 parts.  The four pairs' sums, and the shares' (grid z), join in order.
-// Bound by reading the rows once for each adapter that uses them.
-template <int NT, bool CODES>
-__global__ void __launch_bounds__(256) outer_kernel(const Args g, const Rows src, const float* __restrict__ val, const int shares,
-                                                    const int chunks, float* __restrict__ part, bf16* __restrict__ out) {
-    constexpr int RC = 8 * NT, kPitch = RC + 8, kScan = 1024;
-    __shared__ union {
-        uint32_t vp[2][32][kPitch];  // [part][pair of tokens][rank]
-        float sum[128][RC + 1];      // once the tokens are done
-    } sm;
-    __shared__ int list[kScan + 64];
-    __shared__ int warp_count[8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-    const int a = blockIdx.y, share = blockIdx.z / chunks, rank0 = (blockIdx.z % chunks) * RC;
-    const int f = blockIdx.x * 128 + (warp & 1) * 64 + 8 * gq;
-    const long long per = (g.n + shares - 1) / shares, t_end = min(g.n, (share + 1) * per);
-    float acc[4][NT][4] = {};
-    int have = 0;
-    for (long long base = share * per; base < t_end; base += kScan) {
-        bool hit[kScan / 256];
+// Larger batches: 64 tokens of one adapter per block (a piece of Order), which
+// read the adapter's factor once, the features over its 8 warps.  The first
+// blocks also list the adapters of the tiles of 256 tokens.
+template <int NT, bool CODES, bool ALONG>
+__device__ __forceinline__ void down_piece(const Args& g, const Rows& src, const Order& o, float* __restrict__ u, float (*red)[16][8 * NT]) {
+    constexpr int RC = 8 * NT, MT = 4;
+    const int2 tile = o.tiles[blockIdx.x];
+    const int a = tile.x;
+    if (a < 0) return;
+    const int2 span = o.span[a];
+    const int* tokens = o.tokens + span.x + 64 * tile.y;
+    const int count = min(64, span.y - 64 * tile.y), gq = (threadIdx.x & 31) >> 2, rank0 = blockIdx.y * RC;
+    int tok[2 * MT];
 #pragma unroll
-        for (int i = 0; i < kScan / 256; ++i) {
-            const long long t = base + i * 256 + threadIdx.x;
-            hit[i] = t < t_end && adapter_of(g, t) == a;
-        }
+    for (int i = 0; i < 2 * MT; ++i) tok[i] = 8 * i + gq < count ? tokens[8 * i + gq] : -1;
+    float acc[MT][NT][4] = {};
+    accumulate<NT, MT, CODES, ALONG>(g, src, a, tok, rank0, threadIdx.x >> 5, 8, acc);
 #pragma unroll
-        for (int i = 0; i < kScan / 256; ++i) {  // append this adapter's tokens, in order
-            const unsigned m = __ballot_sync(~0u, hit[i]);
-            if (lane == 0) warp_count[warp] = __popc(m);
-            __syncthreads();
-            int at = have + __popc(m & ((1u << lane) - 1));
-            for (int w = 0; w < 8; ++w) {
-                if (w < warp) at += warp_count[w];
-                have += warp_count[w];
-            }
-            if (hit[i]) list[at] = static_cast<int>(base + i * 256 + threadIdx.x);
-            __syncthreads();
-        }
-        const bool flush = base + kScan >= t_end;
-        int done = 0;
-        for (; have - done >= 64 || (flush && have > done); done += 64) {
-            // two tokens' values of a rank as one word, high parts and low parts
-            const int pair = threadIdx.x >> 3, i0 = done + 2 * pair;
-            const long long ta = i0 < have ? list[i0] : -1, tb = i0 + 1 < have ? list[i0 + 1] : -1;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int k = (threadIdx.x & 7) + 8 * i;
-                const bool in = rank0 + k < g.rank;
-                const float x = in && ta >= 0 ? val[ta * g.rank + rank0 + k] : 0.0f, y = in && tb >= 0 ? val[tb * g.rank + rank0 + k] : 0.0f;
-                const __nv_bfloat162 hi = __floats2bfloat162_rn(x, y);
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(x - __low2float(hi), y - __high2float(hi));
-                sm.vp[0][pair][k] = *reinterpret_cast<const uint32_t*>(&hi);
-                sm.vp[1][pair][k] = *reinterpret_cast<const uint32_t*>(&lo);
-            }
-            __syncthreads();
-            const int slot = done + (warp >> 1) * 16;
-            uint32_t w[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {  // tokens of k slots 2t, 2t+1, 2t+8, 2t+9
-                const int i = slot + 2 * tq + (j & 1) + 8 * (j >> 1);
-                const uint4 v = i < have && f < src.cols ? row8<CODES>(src, list[i], f) : make_uint4(0, 0, 0, 0);
-                w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
-            }
-            const int p = (warp >> 1) * 8 + tq;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const uint32_t h0 = sm.vp[0][p][8 * i + gq], h1 = sm.vp[0][p + 4][8 * i + gq];
-                const uint32_t l0 = sm.vp[1][p][8 * i + gq], l1 = sm.vp[1][p + 4][8 * i + gq];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {  // rows g, g+8 of tile m: features 2m, 2m+1 of the lane's eight
-                    const uint32_t a0 = __byte_perm(w[0][m], w[1][m], 0x5410), a1 = __byte_perm(w[0][m], w[1][m], 0x7632);
-                    const uint32_t a2 = __byte_perm(w[2][m], w[3][m], 0x5410), a3 = __byte_perm(w[2][m], w[3][m], 0x7632);
-                    mma16816(acc[m][i], a0, a1, a2, a3, l0, l1);
-                    mma16816(acc[m][i], a0, a1, a2, a3, h0, h1);
-                }
-            }
-            __syncthreads();
-        }
-        // what is left (fewer than 64) moves to the front
-        const int left = max(0, have - done);
-        const int keep = threadIdx.x < left ? list[done + threadIdx.x] : 0;
+    for (int q = 0; q < MT; ++q) {
         __syncthreads();
-        if (threadIdx.x < left) list[threadIdx.x] = keep;
-        have = left;
+        stage_sums<NT>(red, acc[q]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * RC; i += 256) {
+            const int row = 16 * q + i / RC, k = rank0 + i % RC;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) sum += red[w][i / RC][i % RC];
+            if (row < count && k < g.rank) u[static_cast<long long>(tokens[row]) * g.rank + k] = g.scale[a] * sum;
+        }
+    }
+}
+template <int NT, bool BACKWARD>
+__global__ void __launch_bounds__(256) down_kernel(const Args g, const Order o, float* __restrict__ first, float* __restrict__ second,
+                                                   int32_t* __restrict__ lists) {
+    __shared__ float red[8][16][8 * NT];
+    __shared__ int who[256];
+    if (blockIdx.y == 0 && blockIdx.z == 0 && blockIdx.x < (g.n + 255) / 256) {
+        list_adapters(g, blockIdx.x, who, lists);
         __syncthreads();
     }
+    if constexpr (!BACKWARD) {
+        down_piece<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, o, first, red);
+    } else {
+        if (blockIdx.z == 0) down_piece<NT, false, false>(g, {g.dy, g.lddy, {}, g.r}, o, first, red);
+        else down_piece<NT, true, true>(g, {nullptr, 0, g.x8, g.d}, o, second, red);
+    }
+}
+
+// Tokens of each of `shares` shares of `count`: whole pieces of 64.
+__device__ __forceinline__ int share_of(int count, int shares) { return ((count + 63) / 64 + shares - 1) / shares * 64; }
+// Where element (feature c, rank k) of adapter a's gradient is: of a, [rank][lda], or of b, [r][ldb].
+template <bool OF_A>
+__device__ __forceinline__ long long grad_at(const Args& g, int a, int c, int k) {
+    return OF_A ? (static_cast<long long>(a) * g.rank + k) * g.lda + c : (static_cast<long long>(a) * g.r + c) * g.ldb + k;
+}
+
+// The gradients of both factors: out_a[c][k] = sum over adapter a's tokens of
+// row_t[c] val_t[k], rows of the checkpoint with v for a, of dy with u for b.
+// A block has 128 features and RC ranks of one adapter and a share of its
+// tokens, taken 64 at a time, 16 for each pair of warps, the next 64 tokens'
+// rows and values fetched while these multiply; val enters as two BF16 parts.
+// The four pairs' sums, and the shares', join in a fixed order.
+template <int NT>
+struct OuterSmem {
+    union {
+        uint32_t vp[2][32][8 * NT + 8];  // [part][pair of tokens][rank]
+        float sum[128][8 * NT + 1];      // once the tokens are done
+    };
+    int list[kSmallBatch];  // a small batch's tokens of this adapter
+    int warp_count[8];
+};
+
+template <int NT, bool CODES>
+__device__ __forceinline__ void outer_product(const Args& g, const Rows& src, const float* __restrict__ val, const Order& o, int tile,
+                                              int share, int shares, int rank0, float* __restrict__ part, bf16* __restrict__ out,
+                                              OuterSmem<NT>& sm) {
+    constexpr int RC = 8 * NT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3, a = blockIdx.y;
+    const int f = tile * 128 + (warp & 1) * 64 + 8 * gq;
+    const int* tokens = sm.list;
+    int count = 0;
+    if (o.tokens) {
+        const int2 span = o.span[a];
+        tokens = o.tokens + span.x;
+        count = span.y;
+    } else {
+        for (int i = 0; i < kSmallBatch / 256; ++i) {  // compact them here
+            const int t = i * 256 + threadIdx.x;
+            const bool hit = t < g.n && adapter_of(g, t) == a;
+            const unsigned m = __ballot_sync(~0u, hit);
+            if (lane == 0) sm.warp_count[warp] = __popc(m);
+            __syncthreads();
+            int at = count + __popc(m & ((1u << lane) - 1));
+            for (int w = 0; w < 8; ++w) {
+                if (w < warp) at += sm.warp_count[w];
+                count += sm.warp_count[w];
+            }
+            if (hit) sm.list[at] = t;
+            __syncthreads();
+        }
+    }
+    const int per = share_of(count, shares), end = min(count, (share + 1) * per);
+    float acc[4][NT][4] = {};
+    uint32_t w[4][4];
+    float va[NT], vb[NT];
+    const int pair = threadIdx.x >> 3, k8 = threadIdx.x & 7;
+    auto fetch = [&](int from) {
+        const int i0 = from + 2 * pair;
+        const int ta = i0 < end ? tokens[i0] : -1, tb = i0 + 1 < end ? tokens[i0 + 1] : -1;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const bool in = rank0 + k8 + 8 * i < g.rank;
+            va[i] = in && ta >= 0 ? val[static_cast<long long>(ta) * g.rank + rank0 + k8 + 8 * i] : 0.0f;
+            vb[i] = in && tb >= 0 ? val[static_cast<long long>(tb) * g.rank + rank0 + k8 + 8 * i] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // tokens of k slots 2t, 2t+1, 2t+8, 2t+9
+            const int i = from + (warp >> 1) * 16 + 2 * tq + (j & 1) + 8 * (j >> 1);
+            const uint4 v = i < end && f < src.cols ? row8<CODES>(src, tokens[i], f) : make_uint4(0, 0, 0, 0);
+            w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+        }
+    };
+    const int begin = share * per;
+    if (begin < end) fetch(begin);
+    for (int from = begin; from < end; from += 64) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {  // two tokens' values of a rank as one word, high parts and low parts
+            const __nv_bfloat162 hi = __floats2bfloat162_rn(va[i], vb[i]);
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(va[i] - __low2float(hi), vb[i] - __high2float(hi));
+            sm.vp[0][pair][k8 + 8 * i] = *reinterpret_cast<const uint32_t*>(&hi);
+            sm.vp[1][pair][k8 + 8 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+        }
+        // rows g, g+8 of tile m: features 2m, 2m+1 of the lane's eight
+        uint32_t x[4][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            x[m][0] = __byte_perm(w[0][m], w[1][m], 0x5410);
+            x[m][1] = __byte_perm(w[0][m], w[1][m], 0x7632);
+            x[m][2] = __byte_perm(w[2][m], w[3][m], 0x5410);
+            x[m][3] = __byte_perm(w[2][m], w[3][m], 0x7632);
+        }
+        __syncthreads();
+        if (from + 64 < end) fetch(from + 64);
+        const int p = (warp >> 1) * 8 + tq;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const uint32_t h0 = sm.vp[0][p][8 * i + gq], h1 = sm.vp[0][p + 4][8 * i + gq];
+            const uint32_t l0 = sm.vp[1][p][8 * i + gq], l1 = sm.vp[1][p + 4][8 * i + gq];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                mma16816(acc[m][i], x[m][0], x[m][1], x[m][2], x[m][3], l0, l1);
+                mma16816(acc[m][i], x[m][0], x[m][1], x[m][2], x[m][3], h0, h1);
+            }
+        }
+    }
+    __syncthreads();
     for (int q = 0; q < 4; ++q) {
         if ((warp >> 1) == q) {
 #pragma unroll
@@ -358,28 +499,42 @@ __global__ void __launch_bounds__(256) outer_kernel(const Args g, const Rows src
         }
         __syncthreads();
     }
-    // CODES: the gradient of a, [rank][lda]; else of b, [r][ldb]
-    const int f0 = blockIdx.x * 128;
+    if (shares > 1 && begin >= end && share > 0) return;  // nothing of this share: join_kernel does not read it
+    const int f0 = tile * 128;
     for (int i = threadIdx.x; i < 128 * RC; i += 256) {
         const int c = CODES ? i % 128 : i / RC, k = CODES ? i / 128 : i % RC;
         if (f0 + c >= src.cols || rank0 + k >= g.rank) continue;
-        if (part) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = sm.sum[c][k];
-        else if (CODES) out[(static_cast<long long>(a) * g.rank + rank0 + k) * g.lda + f0 + c] = __float2bfloat16_rn(sm.sum[c][k]);
-        else out[(static_cast<long long>(a) * g.r + f0 + c) * g.ldb + rank0 + k] = __float2bfloat16_rn(sm.sum[c][k]);
+        if (shares > 1) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = sm.sum[c][k];
+        else out[grad_at<CODES>(g, a, f0 + c, rank0 + k)] = __float2bfloat16_rn(sm.sum[c][k]);
     }
 }
 
+// Blocks (tile of 128 features of a, then of b; adapter; share and rank chunk).
+template <int NT>
+__global__ void __launch_bounds__(256) outer_kernel(const Args g, const Order o, const float* __restrict__ v, const float* __restrict__ u,
+                                                    const int shares, const int chunks, float* __restrict__ part) {
+    __shared__ OuterSmem<NT> sm;
+    const int tiles_a = (g.d + 127) / 128, share = blockIdx.z / chunks, rank0 = blockIdx.z % chunks * 8 * NT;
+    const int tile = blockIdx.x;
+    if (tile < tiles_a) outer_product<NT, true>(g, {nullptr, 0, g.x8, g.d}, v, o, tile, share, shares, rank0, part, g.da, sm);
+    else outer_product<NT, false>(g, {g.dy, g.lddy, {}, g.r}, u, o, tile - tiles_a, share, shares, rank0,
+                                  part + static_cast<long long>(shares) * g.na * g.d * g.rank, g.db, sm);
+}
+
 // Joins the shares of outer_kernel in order.
-template <bool CODES>
-__global__ void __launch_bounds__(256) join_kernel(const Args g, const int cols, const int shares, const float* __restrict__ part,
-                                                   bf16* __restrict__ out) {
-    const long long each = static_cast<long long>(g.na) * cols * g.rank;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < each; i += gridDim.x * 256ll) {
-        float s = 0.0f;
-        for (int q = 0; q < shares; ++q) s += part[q * each + i];
-        const int k = static_cast<int>(i % g.rank);
-        const long long af = i / g.rank, a = af / cols, c = af % cols;
-        out[CODES ? (a * g.rank + k) * g.lda + c : (a * g.r + c) * g.ldb + k] = __float2bfloat16_rn(s);
+__global__ void __launch_bounds__(256) join_kernel(const Args g, const Order o, const int shares, const float* __restrict__ part) {
+    const long long each_a = static_cast<long long>(g.na) * g.d * g.rank, each_b = static_cast<long long>(g.na) * g.r * g.rank;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < each_a + each_b; i += gridDim.x * 256ll) {
+        const bool of_a = i < each_a;
+        const long long each = of_a ? each_a : each_b, j = of_a ? i : i - each_a;
+        const float* p = part + (of_a ? 0 : shares * each_a) + j;
+        const int k = static_cast<int>(j % g.rank), cols = of_a ? g.d : g.r;
+        const int a = static_cast<int>(j / g.rank / cols), c = static_cast<int>(j / g.rank % cols);
+        const int count = o.span[a].y, per = share_of(count, shares);
+        float s = p[0];
+        for (int q = 1; q < shares && q * per < count; ++q) s += p[q * each];
+        if (of_a) g.da[grad_at<true>(g, a, c, k)] = __float2bfloat16_rn(s);
+        else g.db[grad_at<false>(g, a, c, k)] = __float2bfloat16_rn(s);
     }
 }
 
@@ -452,73 +607,80 @@ cudaError_t launch_few(const Args& g, const float* u, cudaStream_t st) {
     return launch_pdl(few_tokens_kernel<NT>, dim3((g.r + 15) / 16), dim3(256), 0, st, g, u);
 }
 
-template <int NT, bool BACKWARD>
-void launch_down(const Args& g, float* first, float* second, int32_t* lists, cudaStream_t st) {
-    const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16), chunks = (g.rank + 8 * NT - 1) / (8 * NT);
-    if (g.n <= 1024) {
-        // A small batch's tiles do not fill the GPU: a block for each adapter that a tile may hold, and
-        // eight for its features.  (One token, 4096 features, rank 16: 9.4 us with one block, 4.7 with eight.)
-        const int passes = std::min(16, g.na);
-        down_kernel<NT, BACKWARD, 8><<<dim3(8 * tiles, chunks, (second ? 2 : 1) * passes), 256, 0, st>>>(g, passes, first, second, lists);
-    } else {
-        down_kernel<NT, BACKWARD, 1><<<dim3(tiles, chunks, second ? 2 : 1), 256, 0, st>>>(g, 1, first, second, lists);
-    }
-}
-template <bool BACKWARD>
-int down(const Args& g, float* first, float* second, int32_t* lists, cudaStream_t st) {
-    if (g.rank <= 16) launch_down<2, BACKWARD>(g, first, second, lists, st);
-    else if (g.rank <= 32) launch_down<4, BACKWARD>(g, first, second, lists, st);
-    else launch_down<8, BACKWARD>(g, first, second, lists, st);
-    return check_launch("down_kernel");
-}
-
-// Shares of the tokens for one gradient of `cols` features: enough blocks to
-// fill the GPU about four times, but no share below 512 tokens.
-int shares_of(const Args& g, int cols) {
-    const long long blocks = static_cast<long long>((cols + 127) / 128) * g.na * ((g.rank + 63) / 64);
-    return static_cast<int>(std::max(1ll, std::min((600 + blocks - 1) / blocks, g.n / 512)));
-}
-template <bool CODES>
-int launch_outer(const Args& g, const Rows& src, const float* val, float* part, bf16* out, cudaStream_t st) {
-    const int shares = shares_of(g, src.cols), chunks = (g.rank + 63) / 64;
-    const dim3 grid((src.cols + 127) / 128, g.na, shares * chunks);
-    float* p = shares > 1 ? part : nullptr;
-    if (g.rank <= 16) outer_kernel<2, CODES><<<grid, 256, 0, st>>>(g, src, val, shares, chunks, p, out);
-    else if (g.rank <= 32) outer_kernel<4, CODES><<<grid, 256, 0, st>>>(g, src, val, shares, chunks, p, out);
-    else outer_kernel<8, CODES><<<grid, 256, 0, st>>>(g, src, val, shares, chunks, p, out);
-    if (shares > 1) {
-        const long long each = static_cast<long long>(g.na) * src.cols * g.rank;
-        join_kernel<CODES><<<static_cast<unsigned>(std::min((each + 255) / 256, 148ll * 8)), 256, 0, st>>>(g, src.cols, shares, part, out);
-    }
-    return check_launch("outer_kernel");
-}
-
-// One piece of scratch: the lists, u and v, and the shares of a gradient (freed
-// through `lists`).  Empty without adapters or tokens.
+// One piece of scratch: the lists, u and v, the order of the tokens and the shares
+// of the gradients (freed through `lists`).  Empty without adapters or tokens.
 struct Scratch {
     int32_t* lists;
     float *u, *v, *part;
+    Order order;
+    int shares;
 };
 int make_scratch(const Args& g, bool grads, cudaStream_t st, Scratch* s) {
+    s->shares = 1;
     if (!g.na || !g.n) return TB_OK;
-    auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-    const size_t list = up((g.n + 255) / 256 * linear::kListPitch * sizeof(int32_t));
-    const size_t vals = up(g.n * g.rank * sizeof(float));
-    size_t part = 0;
-    if (grads)
-        for (const int cols : {g.d, g.r}) {
-            const int shares = shares_of(g, cols);
-            if (shares > 1) part = std::max(part, up(static_cast<size_t>(shares) * g.na * cols * g.rank * sizeof(float)));
-        }
+    const bool ordered = g.n > kSmallBatch;
+    if (grads && ordered) {
+        // Enough blocks to fill the GPU about four times, but no share of an even split below 512 tokens.
+        const long long blocks = static_cast<long long>((g.d + 127) / 128 + (g.r + 127) / 128) * g.na * ((g.rank + 63) / 64);
+        s->shares = static_cast<int>(std::max(1ll, std::min(600 / blocks, g.n / g.na / 512)));
+    }
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t lists = take((g.n + 255) / 256 * linear::kListPitch * sizeof(int32_t));
+    const size_t v = take(g.n * g.rank * sizeof(float)), u = grads ? take(g.n * g.rank * sizeof(float)) : v;
+    const size_t span = take(ordered ? g.na * sizeof(int2) : 0), tiles = take(ordered ? (g.n / 64 + g.na) * sizeof(int2) : 0);
+    const size_t tokens = take(ordered ? g.n * sizeof(int) : 0);
+    const size_t part = take(s->shares > 1 ? static_cast<size_t>(s->shares) * g.na * (static_cast<size_t>(g.d) + g.r) * g.rank * sizeof(float) : 0);
     void* p = nullptr;
-    const int rc = scratch_alloc(&p, list + (grads ? 2 : 1) * vals + part, st);
+    const int rc = scratch_alloc(&p, at, st);
     if (rc) return rc;
     char* c = static_cast<char*>(p);
-    s->lists = reinterpret_cast<int32_t*>(c);
-    s->v = reinterpret_cast<float*>(c + list);
-    s->u = grads ? reinterpret_cast<float*>(c + list + vals) : s->v;
-    s->part = reinterpret_cast<float*>(c + list + 2 * vals);
+    s->lists = reinterpret_cast<int32_t*>(c + lists);
+    s->v = reinterpret_cast<float*>(c + v);
+    s->u = reinterpret_cast<float*>(c + u);
+    if (ordered) s->order = {reinterpret_cast<int2*>(c + span), reinterpret_cast<int2*>(c + tiles), reinterpret_cast<int*>(c + tokens)};
+    s->part = reinterpret_cast<float*>(c + part);
     return TB_OK;
+}
+
+// u of the forward (into `first`), or v and u of the backward.
+template <int NT, bool BACKWARD>
+void launch_down(const Args& g, const Scratch& s, float* first, float* second, cudaStream_t st) {
+    const unsigned chunks = (g.rank + 8 * NT - 1) / (8 * NT), two = second ? 2 : 1;
+    if (g.n <= kSmallBatch) {
+        // A small batch's tiles do not fill the GPU: a block for each adapter that a tile may hold, and
+        // eight for its features.  (One token, 4096 features, rank 16: 9.4 us with one block, 4.7 with eight.)
+        const int passes = std::min(16, g.na);
+        const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16);
+        down_small_kernel<NT, BACKWARD><<<dim3(kSplit * tiles, chunks, two * passes), 256, 0, st>>>(g, passes, first, second, s.lists);
+    } else {
+        order_kernel<<<g.na, 1024, 0, st>>>(g, s.order);
+        down_kernel<NT, BACKWARD><<<dim3(static_cast<unsigned>(g.n / 64 + g.na), chunks, two), 256, 0, st>>>(g, s.order, first, second, s.lists);
+    }
+}
+template <bool BACKWARD>
+int down(const Args& g, const Scratch& s, float* first, float* second, cudaStream_t st) {
+    if (g.rank <= 16) launch_down<2, BACKWARD>(g, s, first, second, st);
+    else if (g.rank <= 32) launch_down<4, BACKWARD>(g, s, first, second, st);
+    else launch_down<8, BACKWARD>(g, s, first, second, st);
+    return check_launch("down_kernel");
+}
+
+int gradients(const Args& g, const Scratch& s, cudaStream_t st) {
+    const int chunks = (g.rank + 63) / 64;
+    const dim3 grid((g.d + 127) / 128 + (g.r + 127) / 128, g.na, s.shares * chunks);
+    if (g.rank <= 16) outer_kernel<2><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    else if (g.rank <= 32) outer_kernel<4><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    else outer_kernel<8><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    if (s.shares > 1) {
+        const long long all = static_cast<long long>(g.na) * (static_cast<long long>(g.d) + g.r) * g.rank;
+        join_kernel<<<static_cast<unsigned>(std::min((all + 255) / 256, 148ll * 8)), 256, 0, st>>>(g, s.order, s.shares, s.part);
+    }
+    return check_launch("outer_kernel");
 }
 
 bool bad_rows(const void* p, int64_t ld, int64_t cols) {
@@ -578,7 +740,7 @@ extern "C" int tb_adapter_forward(const tb_adapter_args* p, void* stream) {
     Scratch s{};
     if ((rc = make_scratch(g, false, st, &s))) return rc;
     if (g.na) {
-        rc = down<false>(g, s.u, nullptr, s.lists, st);
+        rc = down<false>(g, s, s.u, nullptr, st);
     }
     if (!rc && g.n <= kFewTokens) {
         const cudaError_t e = g.n <= 8 ? launch_few<1>(g, s.u, st) : g.n <= 16 ? launch_few<2>(g, s.u, st) : launch_few<4>(g, s.u, st);
@@ -611,14 +773,11 @@ extern "C" int tb_adapter_backward(const tb_adapter_args* p, void* stream) {
     Scratch s{};
     if ((rc = make_scratch(g, grads, st, &s))) return rc;
     if (s.lists) {
-        rc = down<true>(g, s.v, grads ? s.u : nullptr, s.lists, st);
+        rc = down<true>(g, s, s.v, grads ? s.u : nullptr, st);
     }
     if (!rc && g.dx && g.n)
         rc = linear::adapter_input_grad({g.n, g.d, g.r, g.dy, g.lddy, g.w, g.ldw, g.dx, g.lddx, g.who, s.lists, s.v, g.a, g.lda, g.rank, g.na}, st);
-    if (!rc && grads) {
-        rc = launch_outer<true>(g, {nullptr, 0, g.x8, g.d}, s.v, s.part, g.da, st);
-        if (!rc) rc = launch_outer<false>(g, {g.dy, g.lddy, {}, g.r}, s.u, s.part, g.db, st);
-    }
+    if (!rc && grads) rc = gradients(g, s, st);
     scratch_free(s.lists, st);
     return rc;
 }
