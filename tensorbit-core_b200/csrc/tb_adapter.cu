@@ -31,18 +31,18 @@ __device__ __forceinline__ int adapter_of(const Args& g, long long t) {
     return a >= 0 && a < g.na ? a : -1;
 }
 // The adapters that occur among 256 tokens, in order of first occurrence: their
-// count, then their numbers.
+// count, then their numbers.  Called by all threads of a block of 256 or more.
 __device__ __forceinline__ void list_adapters(const Args& g, int tile, int* who, int32_t* __restrict__ lists) {
     __shared__ int count[8];
     const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
     const long long t = tile * 256ll + i;
-    const int mine = t < g.n ? adapter_of(g, t) : -1;
-    who[i] = mine;
+    const int mine = i < 256 && t < g.n ? adapter_of(g, t) : -1;
+    if (i < 256) who[i] = mine;
     __syncthreads();
     bool first = mine >= 0;
     for (int j = 0; j < i && first; ++j) first = who[j] != mine;
     const unsigned m = __ballot_sync(~0u, first);
-    if (lane == 0) count[warp] = __popc(m);
+    if (lane == 0 && warp < 8) count[warp] = __popc(m);
     __syncthreads();
     int at = __popc(m & ((1u << lane) - 1)), total = 0;
     for (int w = 0; w < 8; ++w) {
@@ -111,7 +111,8 @@ __device__ __forceinline__ uint4 row8(const Rows& s, long long t, int f) {
 // tokens: order[start ..] holds them, and every piece of 64 has an entry of
 // `tiles` at start / 64 + a + piece (adapters' entries cannot overlap there; an
 // entry without a piece has adapter -1).  One block per adapter: it counts the
-// tokens of lower adapters, then compacts its own.
+// tokens of lower adapters, then compacts its own.  Further blocks list the
+// adapters of the tiles of 256 tokens.
 struct Order {
     int2* span;     // [na] (start, count)
     int2* tiles;    // [n / 64 + na] (adapter, piece)
@@ -119,8 +120,12 @@ struct Order {
 };
 constexpr int kSmallBatch = 1024;
 
-__global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o) {
-    __shared__ int scan[32], total[2];
+__global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o, int32_t* __restrict__ lists) {
+    __shared__ int scan[32], total[2], who[256];
+    if (static_cast<int>(blockIdx.x) >= g.na) {  // the blocks behind those of the adapters
+        list_adapters(g, blockIdx.x - g.na, who, lists);
+        return;
+    }
     const int a = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid < 2) total[tid] = 0;
     __syncthreads();
@@ -328,51 +333,61 @@ down_small_kernel(const Args g, const int passes, float* __restrict__ first, flo
     }
 }
 
-// Larger batches: 64 tokens of one adapter per block (a piece of Order), which
-// read the adapter's factor once, the features over its 8 warps.  The first
-// blocks also list the adapters of the tiles of 256 tokens.
+// Larger batches: 64 tokens of one adapter (a piece of Order) per cluster of
+// kPieceSplit blocks, 16 for each pair of a block's warps, which share the
+// features out over the blocks and the pair; the adapter's factor comes once
+// from L2 and four times from L1.  The pair's sums and the blocks' join in
+// order, the latter over distributed shared memory.  Bound by the latency of the
+// loads.  (8000 tokens, rank 64, v and u: 113 us with the features over all 8
+// warps of one block, each with all 64 tokens; 64 us like this.)
+constexpr int kPieceSplit = 4;
 template <int NT, bool CODES, bool ALONG>
-__device__ __forceinline__ void down_piece(const Args& g, const Rows& src, const Order& o, float* __restrict__ u, float (*red)[16][8 * NT]) {
-    constexpr int RC = 8 * NT, MT = 4;
-    const int2 tile = o.tiles[blockIdx.x];
-    const int a = tile.x;
+__device__ __forceinline__ void down_piece(const Args& g, const Rows& src, const Order& o, float* __restrict__ u, float (*sums)[8 * NT + 1]) {
+    constexpr int RC = 8 * NT;
+    const int2 tile = o.tiles[blockIdx.x / kPieceSplit];
+    const int a = tile.x, share = blockIdx.x % kPieceSplit;
     if (a < 0) return;
     const int2 span = o.span[a];
     const int* tokens = o.tokens + span.x + 64 * tile.y;
-    const int count = min(64, span.y - 64 * tile.y), gq = (threadIdx.x & 31) >> 2, rank0 = blockIdx.y * RC;
-    int tok[2 * MT];
+    const int warp = threadIdx.x >> 5, gq = (threadIdx.x & 31) >> 2, tq = threadIdx.x & 3;
+    const int count = min(64, span.y - 64 * tile.y), rank0 = blockIdx.y * RC;
+    const int row0 = 16 * (warp & 3) + gq, half = warp >> 2;
+    const int tok[2] = {row0 < count ? tokens[row0] : -1, row0 + 8 < count ? tokens[row0 + 8] : -1};
+    float acc[1][NT][4] = {};
+    accumulate<NT, 1, CODES, ALONG>(g, src, a, tok, rank0, share * 2 + half, 2 * kPieceSplit, acc);
+    for (int h = 0; h < 2; ++h) {
+        if (half == h) {
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) tok[i] = 8 * i + gq < count ? tokens[8 * i + gq] : -1;
-    float acc[MT][NT][4] = {};
-    accumulate<NT, MT, CODES, ALONG>(g, src, a, tok, rank0, threadIdx.x >> 5, 8, acc);
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-        __syncthreads();
-        stage_sums<NT>(red, acc[q]);
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * RC; i += 256) {
-            const int row = 16 * q + i / RC, k = rank0 + i % RC;
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) sum += red[w][i / RC][i % RC];
-            if (row < count && k < g.rank) u[static_cast<long long>(tokens[row]) * g.rank + k] = g.scale[a] * sum;
+                for (int e = 0; e < 4; ++e) {  // column 2t + e of fragment i is rank (2t + e) NT + i
+                    float& s = sums[row0 + 8 * (e >> 1)][(2 * tq + (e & 1)) * NT + i];
+                    s = h ? s + acc[0][i][e] : acc[0][i][e];
+                }
         }
+        __syncthreads();
     }
+    umma::cluster_sync_all();
+    for (int i = share * 256 + threadIdx.x; i < 64 * RC; i += kPieceSplit * 256) {
+        const int row = i / RC, k = rank0 + i % RC;
+        float v[kPieceSplit], sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kPieceSplit; ++q) v[q] = load_peer(&sums[row][i % RC], q);
+#pragma unroll
+        for (int q = 0; q < kPieceSplit; ++q) sum += v[q];
+        if (row < count && k < g.rank) u[static_cast<long long>(tokens[row]) * g.rank + k] = g.scale[a] * sum;
+    }
+    umma::cluster_sync_all();  // no block leaves before its sums have been read
 }
 template <int NT, bool BACKWARD>
-__global__ void __launch_bounds__(256) down_kernel(const Args g, const Order o, float* __restrict__ first, float* __restrict__ second,
-                                                   int32_t* __restrict__ lists) {
-    __shared__ float red[8][16][8 * NT];
-    __shared__ int who[256];
-    if (blockIdx.y == 0 && blockIdx.z == 0 && blockIdx.x < (g.n + 255) / 256) {
-        list_adapters(g, blockIdx.x, who, lists);
-        __syncthreads();
-    }
+__global__ void __cluster_dims__(kPieceSplit, 1, 1) __launch_bounds__(256)
+down_kernel(const Args g, const Order o, float* __restrict__ first, float* __restrict__ second) {
+    __shared__ float sums[64][8 * NT + 1];
     if constexpr (!BACKWARD) {
-        down_piece<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, o, first, red);
+        down_piece<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, o, first, sums);
     } else {
-        if (blockIdx.z == 0) down_piece<NT, false, false>(g, {g.dy, g.lddy, {}, g.r}, o, first, red);
-        else down_piece<NT, true, true>(g, {nullptr, 0, g.x8, g.d}, o, second, red);
+        if (blockIdx.z == 0) down_piece<NT, false, false>(g, {g.dy, g.lddy, {}, g.r}, o, first, sums);
+        else down_piece<NT, true, true>(g, {nullptr, 0, g.x8, g.d}, o, second, sums);
     }
 }
 
@@ -658,8 +673,8 @@ void launch_down(const Args& g, const Scratch& s, float* first, float* second, c
         const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16);
         down_small_kernel<NT, BACKWARD><<<dim3(kSplit * tiles, chunks, two * passes), 256, 0, st>>>(g, passes, first, second, s.lists);
     } else {
-        order_kernel<<<g.na, 1024, 0, st>>>(g, s.order);
-        down_kernel<NT, BACKWARD><<<dim3(static_cast<unsigned>(g.n / 64 + g.na), chunks, two), 256, 0, st>>>(g, s.order, first, second, s.lists);
+        order_kernel<<<static_cast<unsigned>(g.na + (g.n + 255) / 256), 1024, 0, st>>>(g, s.order, s.lists);
+        down_kernel<NT, BACKWARD><<<dim3(static_cast<unsigned>(kPieceSplit * (g.n / 64 + g.na)), chunks, two), 256, 0, st>>>(g, s.order, first, second);
     }
 }
 template <bool BACKWARD>
