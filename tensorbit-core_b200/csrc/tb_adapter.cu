@@ -636,7 +636,7 @@ int make_scratch(const Args& g, bool grads, cudaStream_t st, Scratch* s) {
     const bool ordered = g.n > kSmallBatch;
     if (grads && ordered) {
         // Enough blocks to fill the GPU about four times, but no share of an even split below 512 tokens.
-        const long long blocks = static_cast<long long>((g.d + 127) / 128 + (g.r + 127) / 128) * g.na * ((g.rank + 63) / 64);
+        const long long blocks = static_cast<long long>((g.d + 127) / 128 + (g.r + 127) / 128) * g.na * ((g.rank + 31) / 32);
         s->shares = static_cast<int>(std::max(1ll, std::min(600 / blocks, g.n / g.na / 512)));
     }
     size_t at = 0;
@@ -686,11 +686,11 @@ int down(const Args& g, const Scratch& s, float* first, float* second, cudaStrea
 }
 
 int gradients(const Args& g, const Scratch& s, cudaStream_t st) {
-    const int chunks = (g.rank + 63) / 64;
+    // 32 ranks a block at most: with 64 (206 registers, one block an SM) rank 64 took 125 + 18 us where this takes 102 us
+    const int chunks = (g.rank + 31) / 32;
     const dim3 grid((g.d + 127) / 128 + (g.r + 127) / 128, g.na, s.shares * chunks);
     if (g.rank <= 16) outer_kernel<2><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
-    else if (g.rank <= 32) outer_kernel<4><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
-    else outer_kernel<8><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    else outer_kernel<4><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
     if (s.shares > 1) {
         const long long all = static_cast<long long>(g.na) * (static_cast<long long>(g.d) + g.r) * g.rank;
         join_kernel<<<static_cast<unsigned>(std::min((all + 255) / 256, 148ll * 8)), 256, 0, st>>>(g, s.order, s.shares, s.part);
