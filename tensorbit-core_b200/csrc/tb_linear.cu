@@ -47,9 +47,13 @@ __device__ int g_linear_error;
 
 constexpr int kThreads = 512;
 constexpr int kEpiWarps = 8, kPrepWarp = 8, kTmaWarp = 12, kMmaWarp = 13;
-// Codes are decoded by three groups of two warps (8-9, 10-11, 14-15), every third slice each: a
-// slice's chain of wait, loads, arithmetic, stores, fence and arrival overlaps the next ones'.
-constexpr int kDecodeGroups = 3;
+// Codes are decoded by two groups of three warps (8-10 and 11, 14, 15), every
+// second slice each: a slice's chain of wait, loads, arithmetic, stores, fence and
+// arrival overlaps the next one's.  The number of stages is a multiple of the
+// groups, so a stage always has the same group: a barrier's parity says nothing
+// to a waiter that skips phases (TMA loads may complete out of order), so each
+// phase of full[s] has to be waited for by who waits for the next.
+constexpr int kDecodeGroups = 2, kGroupWarps = 3;
 
 template <int MODE>
 struct Cfg {
@@ -68,8 +72,9 @@ struct Cfg {
     static constexpr int kStage = kA + kB + kRaw;
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
-    static constexpr int kReady = kCodes ? 4 : kAdapter ? 9 : 1;
-    static constexpr int kStages = MODE == kGrad ? 4 : MODE == kFisher ? 7 : 6;
+    static constexpr int kReady = kCodes ? 2 * kGroupWarps : kAdapter ? 9 : 1;
+    static constexpr int kStages = MODE == kGrad ? 4 : 6;
+    static_assert(!kCodes || kStages % kDecodeGroups == 0, "a stage has one group of decoding warps");
     // Behind the stages: 8 KB a warp for results on their way out (kGrad), the exponents of each stage, column scales (kHess)
     static constexpr int kOut = MODE == kGrad ? kEpiWarps * 8192 : 0;
     static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
@@ -758,55 +763,55 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             __syncwarp();
         } else if (C::kCodes) {
             // 8 consecutive features (one 16-byte unit of the operand) of every kRowStep-th token
-            constexpr int kUnits = C::kCols / 8, kRowStep = 64 / kUnits, kSteps = 64 / kRowStep;
-            const int group = warp < kTmaWarp ? (warp - kPrepWarp) >> 1 : 2;
-            const int pt = (warp & 1) * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
+            constexpr int kThreadsGroup = 32 * kGroupWarps, kUnits = C::kCols / 8, kRowStep = kThreadsGroup / kUnits;
+            constexpr int kSteps = (64 + kRowStep - 1) / kRowStep, kBatch = 6;
+            const int nth = warp < kTmaWarp ? warp - kPrepWarp : warp - kMmaWarp + 3, group = nth / kGroupWarps;
+            const int pt = nth % kGroupWarps * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
             Ring<kStages> at;
-            int turn = 0;
             const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int, int, int i) {
                 const int s = at.s;
                 const uint32_t phase = at.phase;
                 at.next();
-                const bool mine = turn == group;
-                turn = turn == kDecodeGroups - 1 ? 0 : turn + 1;
-                if (!mine) return true;
+                if (s % kDecodeGroups != group) return true;
                 const int k0 = u.lo + i * 64;
                 const int valid = min(64, u.hi - k0);
                 const int border = 128 - (k0 & 127);  // first token of the next block
                 if (!wait(smem_u32(&full[s]), phase, abort_flag)) return false;
                 uint8_t* stage = smem + s * C::kStage;
                 const uint8_t* raw = stage + C::kA + C::kB;
-                uint32_t s0[4];
                 const uint8_t* exps = exps_buf + s * C::kExps + pc * 8;
+                uint32_t s0[4], s1[4] = {0, 0, 0, 0};
                 act8::scales8(*reinterpret_cast<const uint2*>(exps), s0);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
                 const bool whole = valid == 64 && border >= 64;
-                uint32_t s1[4] = {0, 0, 0, 0};
                 if (!whole) act8::scales8(*reinterpret_cast<const uint2*>(exps + C::kCols), s1);
 #pragma unroll
-                for (int h = 0; h < kSteps; h += 8) {
-                    uint2 w[8];
+                for (int h = 0; h < kSteps; h += kBatch) {
+                    uint2 w[kBatch];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + (h + q) * kRowStep) * C::kCols + pc * 8);
+                    for (int q = 0; q < kBatch; ++q) {
+                        const int k = pr + (h + q) * kRowStep;
+                        if (h + q < kSteps && k < 64) w[q] = *reinterpret_cast<const uint2*>(raw + k * C::kCols + pc * 8);
+                    }
                     if (whole) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
+                        for (int q = 0; q < kBatch; ++q) {
                             const int k = pr + (h + q) * kRowStep;
-                            *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
+                            if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
                         }
                     } else {  // a block's or the sample's end within the slice
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
+                        for (int q = 0; q < kBatch; ++q) {
                             const int k = pr + (h + q) * kRowStep;
                             uint32_t sk[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
-                            *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
+                            if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
                         }
                     }
                 }
                 // tokens behind the sample's end: dY may hold anything there
-                for (int q = pt; q < (64 - valid) * 16; q += 64)
+                for (int q = pt; q < (64 - valid) * 16; q += kThreadsGroup)
                     *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + (valid + (q >> 4)) * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

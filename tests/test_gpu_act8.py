@@ -175,6 +175,33 @@ def test_weight_grad_densely_packed(cuda, tblib, n, r, d, S, g_t):
         check_sums(torch, out[s * r * d:(s + 1) * r * d].view(r, d), G, A, n, g_t == "bfloat16")
 
 
+@pytest.mark.parametrize("dy_t", ["float32", "bfloat16"])
+def test_many_short_samples_on_many_tiles(cuda, tblib, dy_t):
+    """Many units of a few slices for each pair of blocks, the stages' ring wrapping at every phase: right, and the same
+    bits every time (gradients and Fisher)."""
+    torch, tb = cuda, tblib
+    n, r, d, S = 434, 1300, 1677, 10
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 7))
+    dy = rows(torch, n, r, getattr(torch, dy_t), 8, ref.up(r, 16), 1e-2, 0)
+    samples = [(i * n // S, (i + 1) * n // S) for i in range(S)]
+    sp = pairs(torch, samples)
+    outs = []
+    for _ in range(4):
+        G, F = torch.empty(S, r, d, device="cuda"), torch.empty(r, d, device="cuda")
+        tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), S,
+                                     G.data_ptr(), tb.F32))
+        tb.check(tb.act8_fisher(c.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), S, F.data_ptr()))
+        outs.append((G, F))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    assert all(torch.equal(a, b) for o in outs[1:] for a, b in zip(o, outs[0]))
+    ga = ref.gradients(torch, dy, c.values(torch), samples)
+    for s, (G, A) in enumerate(ga):
+        check_sums(torch, outs[0][0][s], G, A, 50 * PARTS[dy_t])
+    want = ref.fisher(torch, [G for G, _ in ga], 0.01, 0.99)
+    assert float((outs[0][1].double() - want).norm() / want.norm()) <= 4e-6
+
+
 def test_weight_grad_leaves_other_tokens_out(cuda, tblib):
     """NaN and infinities in tokens of no sample reach no gradient; those of one sample stay in it."""
     torch, tb = cuda, tblib
