@@ -73,12 +73,12 @@ struct Cfg {
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
     static constexpr int kReady = kCodes ? 2 * kGroupWarps : kAdapter ? 9 : 1;
-    static constexpr int kStages = MODE == kGrad ? 4 : 6;
+    static constexpr int kStages = MODE == kGrad ? 4 : MODE == kHess ? 5 : 6;
     static_assert(!kCodes || kStages % kDecodeGroups == 0, "a stage has one group of decoding warps");
-    // Behind the stages: 8 KB a warp for results on their way out (kGrad), the exponents of each stage, column scales (kHess)
-    static constexpr int kOut = MODE == kGrad ? kEpiWarps * 8192 : 0;
-    static constexpr int kColScale = MODE == kHess ? kEpiWarps * 2 * kCols * 4 : 0;
-    static constexpr int kExtra = kOut + kStages * kExps + kColScale;
+    // Behind the stages: pieces of results on their way out (for TMA two a warp), the exponents of each stage
+    static constexpr int kOutWarp = MODE == kGrad || MODE == kHess ? 8192 : 4096;
+    static constexpr int kOut = kEpiWarps * kOutWarp;
+    static constexpr int kExtra = kOut + kStages * kExps;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 512;
     static_assert(kSmem <= 232448, "shared memory of a block");
 };
@@ -98,8 +98,8 @@ struct Params {
     int out_bf16, out_tma;
     float alpha, beta, contrib, scale;
     int first, accumulate;
-    // adapters; with splits > 1 the K range of a tile is shared out and FP32 sums go to part [splits][M][ldpart]
     AdapterProduct ad;
+    // with splits > 1 the K range of a unit is shared out and FP32 sums go to part [splits][samples * M][ldpart]
     int splits;
     float* part;
     long long ldpart;
@@ -202,28 +202,38 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // ---- the walk over work items, units (one sum each) and K slices that every role shares ----
 struct Tile {
-    int tm, tn, s;
+    int tm, tn;
+    int s, q;           // sample; share of K
 };
 struct Unit {
     int lo, hi;         // K range
     int slices;         // K slices of one part
-    int total;          // all slices
-    int rslices;        // adapters: slices of one adapter
+    int first, total;   // the share's slices, counted over the parts
+    int extra;          // adapters: slices behind those of K,
+    int rslices;        // so many for each adapter
     const int32_t* list;
 };
 
 template <int MODE>
 __device__ __forceinline__ Tile tile_of(const Params& P, int item) {
-    Tile t{0, 0, 0};
+    Tile t{0, 0, 0, 0};
     if constexpr (MODE == kHess) {  // tiles on or below the diagonal, row by row
-        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(item) + 1.0f) - 1.0f) * 0.5f);
-        while (tm * (tm + 1) / 2 > item) --tm;
-        while ((tm + 1) * (tm + 2) / 2 <= item) ++tm;
+        const int tiles = P.tiles_m * (P.tiles_m + 1) / 2;
+        t.q = item / tiles;
+        const int i = item % tiles;
+        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(i) + 1.0f) - 1.0f) * 0.5f);
+        while (tm * (tm + 1) / 2 > i) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
         t.tm = tm;
-        t.tn = item - tm * (tm + 1) / 2;
+        t.tn = i - tm * (tm + 1) / 2;
     } else {
         const int tiles = P.tiles_m * P.tiles_n;
-        if constexpr (MODE != kFisher) t.s = item / tiles;  // sample, or share of K
+        if constexpr (MODE == kGrad) {
+            t.s = item / tiles % P.S;
+            t.q = item / tiles / P.S;
+        } else if constexpr (MODE != kFisher) {
+            t.q = item / tiles;
+        }
         const int i = item % tiles;
         // bands of 8 tile rows, column by column inside, so that concurrent tiles share operands in L2
         const int band = i / (8 * P.tiles_n), in = i % (8 * P.tiles_n);
@@ -234,9 +244,13 @@ __device__ __forceinline__ Tile tile_of(const Params& P, int item) {
     return t;
 }
 
+// The share `q` of `all` slices.
+__device__ __forceinline__ int share_begin(int all, int q, int splits) {
+    return static_cast<int>(static_cast<unsigned long long>(all) * static_cast<unsigned>(q) / static_cast<unsigned>(splits));
+}
 template <int MODE>
 __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
-    Unit u{0, P.K, 0, 0, 1, nullptr};
+    Unit u{0, P.K, 0, 0, 0, 0, 1, nullptr};
     if constexpr (Cfg<MODE>::kCodes) {
         u.hi = P.n;
         if (P.samples) {
@@ -246,18 +260,24 @@ __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
         }
         u.slices = (u.hi - u.lo + 63) / 64;
         u.total = u.slices * P.parts;
-    } else if constexpr (MODE == kHess) {
-        u.hi = P.n;
-        u.total = u.slices = (P.n + 127) / 128;
-    } else {
-        // every share has a slice: there are at least 8 times as many (at most 2^25 of them, 74 shares)
-        const unsigned all = (P.K + 63u) / 64u, first = all * s / P.splits;
-        u.lo = static_cast<int>(first * 64);
-        u.total = u.slices = static_cast<int>(all * (s + 1) / P.splits - first);
-        if (P.ad.lists && s == P.splits - 1) {
-            u.list = P.ad.lists + static_cast<long long>(t.tm) * kListPitch;
-            u.rslices = (P.ad.rank + 31) / 32;
-            u.total += __ldg(u.list) * u.rslices;
+        if (MODE != kFisher && P.splits > 1) {
+            u.first = share_begin(u.slices * P.parts, t.q, P.splits);
+            u.total = share_begin(u.slices * P.parts, t.q + 1, P.splits) - u.first;
+        }
+    } else {  // a share begins at its own `lo`
+        constexpr int kStep = MODE == kHess ? 128 : 64;
+        u.total = u.slices = ((MODE == kHess ? P.n : P.K) + kStep - 1) / kStep;
+        if (P.splits > 1) {
+            const int all = u.slices, first = share_begin(all, t.q, P.splits);
+            u.lo = first * kStep;
+            u.total = u.slices = share_begin(all, t.q + 1, P.splits) - first;
+        }
+        if constexpr (Cfg<MODE>::kAdapter) {
+            if (P.ad.lists && t.q == P.splits - 1) {
+                u.list = P.ad.lists + static_cast<long long>(t.tm) * kListPitch;
+                u.rslices = (P.ad.rank + 31) / 32;
+                u.extra = __ldg(u.list) * u.rslices;
+            }
         }
     }
     return u;
@@ -276,112 +296,176 @@ struct Ring {
     }
 };
 
-// Calls f(tile, unit, j, part, i) for every slice of this pair's items until it
-// returns false: slice i of a part of K, j counted over the whole unit; the
-// slices of a unit's adapters follow those of its K as the next part.
+// Calls f(tile, unit) for every unit of this pair's items until it returns false.
 template <int MODE, class F>
-__device__ __forceinline__ bool walk(const Params& P, F&& f) {
+__device__ __forceinline__ bool for_units(const Params& P, F&& f) {
     for (int item = blockIdx.x >> 1; item < P.items; item += gridDim.x >> 1) {
         const Tile t = tile_of<MODE>(P, item);
-        const int s1 = MODE == kFisher ? P.S : t.s + 1;
-        for (int s = t.s; s < s1; ++s) {
-            const Unit u = unit_of<MODE>(P, t, s);
-            for (int j = 0, part = 0; j < u.total; ++part) {
-                const int last = min(u.total, j + (Cfg<MODE>::kAdapter && part ? u.total : u.slices));
-                for (int i = 0; j < last; ++i, ++j)
-                    if (!f(t, u, j, part, i)) return false;
-            }
+        if constexpr (MODE == kFisher) {
+            for (int s = 0; s < P.S; ++s)
+                if (!f(t, unit_of<MODE>(P, t, s))) return false;
+        } else {
+            if (!f(t, unit_of<MODE>(P, t, t.s))) return false;
         }
     }
     return true;
 }
-
-// ---- stores of one row's run of columns ------------------------------------------
-__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-template <int COLS>
-__device__ __forceinline__ void store_f32(float* p, const float (&v)[COLS], int valid) {
-    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-#pragma unroll
-        for (int c = 0; c < COLS / 8; ++c) {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * c + i]);
-            st_global32(p + 8 * c, w);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i)
-            if (i < valid) p[i] = v[i];
+// Calls f(part, i, count) for the unit's runs of slices i .. i + count - 1 of one
+// part of K until it returns false.
+template <class F>
+__device__ __forceinline__ bool for_runs(const Unit& u, F&& f) {
+    int part = 0, i = 0;
+    if (u.first) {
+        part = u.first / u.slices;
+        i = u.first % u.slices;
     }
-}
-template <int COLS>
-__device__ __forceinline__ void add_f32(float (&v)[COLS], const float* p, int valid) {
-    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-#pragma unroll
-        for (int c = 0; c < COLS / 8; ++c) {
-            float w[8];
-            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
-                         : "l"(p + 8 * c));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[8 * c + i] += w[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i)
-            if (i < valid) v[i] += p[i];
+    for (int left = u.total; left > 0; ++part, i = 0) {
+        const int run = min(left, u.slices - i);
+        if (!f(part, i, run)) return false;
+        left -= run;
     }
-}
-template <int COLS>
-__device__ __forceinline__ void store_bf16(bf16* p, const float (&v)[COLS], int valid) {
-    if (valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-#pragma unroll
-        for (int c = 0; c < COLS / 16; ++c) {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[16 * c + 2 * i], v[16 * c + 2 * i + 1]);
-            st_global32(p + 16 * c, w);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i)
-            if (i < valid) p[i] = __float2bfloat16_rn(v[i]);
-    }
+    return true;
 }
 
-// 32 rows x 128 columns of a sample's gradient through shared memory: a row of
-// 128 bytes a lane (128-byte swizzle), two pieces of 4 KB in flight.  Stored
-// straight from registers, one row a lane, the 537 MB of sixteen 4096 x 4096
-// gradients held the epilogue up: 400 us against 336.
+// ---- results: a lane holds COLS columns of its row, memory wants rows --------------
+// They pass through shared memory in pieces of 32 rows x 128 bytes (32 FP32 or 64
+// BF16 columns) with 128-byte swizzle: written by 16-byte units of a row a lane,
+// read without conflicts by rows.  A piece leaves by TMA (gradients whose rows
+// start on 16 bytes), as 16-byte units of whole rows, or, where rows do not start
+// on 16 bytes or a piece is not whole, element by element, consecutive ones a
+// store.  rows, cols: how many of the warp's rows, of a piece's columns, exist.
+// (26 gradients of 14282 x 743, rows not on 16 bytes: 2417 us stored a row a lane, 320 so.)
+constexpr int kPieceBytes = 4096;
 template <bool BF16>
-__device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, const float (&v)[128], int col, int row0, int s,
-                                          int N, int lane) {
-    constexpr int kPiece = BF16 ? 64 : 32;  // columns
+struct Piece {
+    static constexpr int kCols = BF16 ? 64 : 32, kSize = BF16 ? 2 : 4;
+};
+template <bool BF16, int COLS>
+__device__ __forceinline__ void fill_piece(uint8_t* buf, const float (&v)[COLS], int c, int lane) {
+    uint8_t* row = buf + lane * 128;
 #pragma unroll
-    for (int c = 0; c < 128 / kPiece; ++c) {
+    for (int j = 0; j < 8; ++j) {
+        uint4 w;
+        const float* x = v + c * Piece<BF16>::kCols + j * (Piece<BF16>::kCols / 8);
+        if constexpr (BF16) w = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        else w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = w;
+    }
+}
+// Byte `at` of row r.
+__device__ __forceinline__ int piece_at(int r, int at) { return r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15); }
+
+template <bool BF16, bool ADD>
+__device__ __forceinline__ void store_piece(const uint8_t* buf, void* out, long long ld, int rows, int cols, int lane) {
+    constexpr int kSize = Piece<BF16>::kSize;
+    char* p = static_cast<char*>(out);
+    const long long pitch = ld * kSize;
+    const unsigned align = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) | pitch);
+    if (cols >= Piece<BF16>::kCols && align % 16 == 0) {
+        const int sub = lane >> 3, unit = (lane & 7) * 16;
+        float4 old[8];
+        if constexpr (ADD) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (4 * i + sub < rows) old[i] = *reinterpret_cast<const float4*>(p + (4 * i + sub) * pitch + unit);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + sub;
+            uint4 w = *reinterpret_cast<const uint4*>(buf + piece_at(r, unit));
+            if constexpr (ADD)
+                w = make_uint4(__float_as_uint(old[i].x + __uint_as_float(w.x)), __float_as_uint(old[i].y + __uint_as_float(w.y)),
+                               __float_as_uint(old[i].z + __uint_as_float(w.z)), __float_as_uint(old[i].w + __uint_as_float(w.w)));
+            if (r < rows) *reinterpret_cast<uint4*>(p + r * pitch + unit) = w;
+        }
+    } else if (!BF16 || align % 4 == 0) {  // a word a lane; a last odd BF16 column by itself
+        const int at = 4 * lane, left = cols * kSize - at;
+        if (left >= 4) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 16) {
+                float old[16];
+                if constexpr (ADD) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (r0 + r < rows) old[r] = *reinterpret_cast<const float*>(p + (r0 + r) * pitch + at);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    uint32_t w = *reinterpret_cast<const uint32_t*>(buf + piece_at(r0 + r, at));
+                    if constexpr (ADD) w = __float_as_uint(old[r] + __uint_as_float(w));
+                    if (r0 + r < rows) *reinterpret_cast<uint32_t*>(p + (r0 + r) * pitch + at) = w;
+                }
+            }
+        } else if (left == 2) {
+#pragma unroll 1
+            for (int r = 0; r < rows; ++r) *reinterpret_cast<uint16_t*>(p + r * pitch + at) = *reinterpret_cast<const uint16_t*>(buf + piece_at(r, at));
+        }
+    } else {
+#pragma unroll 1
+        for (int at = 2 * lane; at < 2 * cols; at += 64) {
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+                if (r >= rows) break;
+                *reinterpret_cast<uint16_t*>(p + r * pitch + at) = *reinterpret_cast<const uint16_t*>(buf + piece_at(r, at));
+            }
+        }
+    }
+}
+// The same as a function of its own, for the kernels that have several kinds of results.
+template <bool BF16>
+__device__ __noinline__ void store_piece_call(const uint8_t* buf, void* out, long long ld, int rows, int cols, int lane) {
+    store_piece<BF16, false>(buf, out, ld, rows, cols, lane);
+}
+// All of the warp's pieces; `out` is its first row and column.
+template <bool BF16, bool ADD, bool CALL, int COLS>
+__device__ __forceinline__ void store_rows(uint8_t* buf, const float (&v)[COLS], void* out, long long ld, int rows, int cols, int lane) {
+    if (rows <= 0) return;
+#pragma unroll
+    for (int c = 0; c < COLS / Piece<BF16>::kCols; ++c) {
+        if (c * Piece<BF16>::kCols >= cols) break;
+        __syncwarp();
+        fill_piece<BF16>(buf, v, c, lane);
+        __syncwarp();
+        if constexpr (CALL) store_piece_call<BF16>(buf, static_cast<char*>(out) + c * 128, ld, rows, cols - c * Piece<BF16>::kCols, lane);
+        else store_piece<BF16, ADD>(buf, static_cast<char*>(out) + c * 128, ld, rows, cols - c * Piece<BF16>::kCols, lane);
+    }
+}
+// The same by TMA, two pieces in flight: sixteen 4096 x 4096 gradients in 336 us, where straight
+// from registers, 32 bytes of a row a lane, they took 400.
+template <bool BF16, int COLS>
+__device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, const float (&v)[COLS], int col, int row0, int s, int N,
+                                          int lane) {
+#pragma unroll
+    for (int c = 0; c < COLS / Piece<BF16>::kCols; ++c) {
+        uint8_t* piece = buf + (c & 1) * kPieceBytes;
         asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the piece before last has left its buffer
         __syncwarp();
-        uint8_t* row = buf + (c & 1) * 4096 + lane * 128;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint4 w;
-            const float* x = v + c * kPiece + j * (kPiece / 8);
-            if constexpr (BF16) w = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-            else w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-            *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = w;
-        }
+        fill_piece<BF16>(piece, v, c, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-            if (col + c * kPiece < N)
+            if (col + c * Piece<BF16>::kCols < N)
                 asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
-                             "r"(col + c * kPiece), "r"(row0), "r"(s), "r"(smem_u32(buf + (c & 1) * 4096))
+                             "r"(col + c * Piece<BF16>::kCols), "r"(row0), "r"(s), "r"(smem_u32(piece))
                              : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
+// Reads FP32 rows.
+template <int COLS>
+__device__ __forceinline__ void load_rows(uint8_t* buf, float (&v)[COLS], const float* p, long long ld, int rows, int cols, int lane) {
+#pragma unroll
+    for (int c = 0; c < COLS / 32; ++c) {
+        __syncwarp();
+#pragma unroll 16
+        for (int r = 0; r < 32; ++r)
+            *reinterpret_cast<float*>(buf + piece_at(r, 4 * lane)) = r < rows && 32 * c + lane < cols ? p[r * ld + 32 * c + lane] : 0.0f;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float4 w = *reinterpret_cast<const float4*>(buf + piece_at(lane, 16 * j));
+            v[32 * c + 4 * j] = w.x; v[32 * c + 4 * j + 1] = w.y; v[32 * c + 4 * j + 2] = w.z; v[32 * c + 4 * j + 3] = w.w;
         }
     }
 }
@@ -404,6 +488,28 @@ __device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, 
                                                    : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o]),
                      y);
     return y;
+}
+
+// The results of one row that are not finite, formed again (not unrolled: it hardly ever runs).
+template <int MODE>
+__device__ __noinline__ void mend_row(const AdapterProduct& p, float* v, long long t, long long o, int cols) {
+    for (int i = 0; i < cols; ++i)
+        if (!(fabsf(v[32 * i]) <= 3.402823466e38f)) v[32 * i] = lone_result<MODE>(p, t, o + i);
+}
+template <int MODE>
+__device__ __forceinline__ void mend_results(const AdapterProduct& p, uint8_t* buf, float (&v)[64], long long row0, long long col,
+                                             int rows, int cols, int lane) {
+    float* x = reinterpret_cast<float*>(buf) + lane;  // column i of this lane's row at 32 i
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[32 * i] = v[32 * h + i];
+        if (lane < rows) mend_row<MODE>(p, x, row0 + lane, col + 32 * h, min(32, cols - 32 * h));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[32 * h + i] = x[32 * i];
+    }
+    __syncwarp();
 }
 
 // Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
@@ -477,7 +583,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* out_buf = smem + kStages * C::kStage;
     uint8_t* exps_buf = out_buf + C::kOut;
-    float* col_scale = reinterpret_cast<float*>(exps_buf + kStages * C::kExps);
     uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + C::kExtra);
     uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
     uint64_t* empty = ready + kStages;    // stage read by the MMAs
@@ -516,41 +621,47 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     const uint32_t tmem = *tmem_slot;
     auto stage_a = [&](int s) { return smem_u32(smem + s * C::kStage); };
     auto stage_b = [&](int s) { return smem_u32(smem + s * C::kStage + C::kA); };
-    auto stage_raw = [&](int s) { return smem_u32(smem + s * C::kStage + C::kA + C::kB); };
 
     // Register shares of the promoting modes: 8 warps x 200 + 8 warps x 56 = the launch's 16 x 128.
     if (warp < kEpiWarps) {
         if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         constexpr int COLS = C::kCols;
         const int quad = warp & 3, half = warp >> 2;
-        const int row_in = rank * 128 + quad * 32 + lane;
+        const int row_in = rank * 128 + quad * 32;
+        uint8_t* buf = out_buf + warp * C::kOutWarp;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * COLS);
         bool ok = true;
         Ring<C::kAcc> ac;
         for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
             const Tile t = tile_of<MODE>(P, item);
-            const long long row = static_cast<long long>(t.tm) * 256 + row_in;
+            const long long row0 = static_cast<long long>(t.tm) * 256 + row_in, row = row0 + lane;
             const long long col = static_cast<long long>(t.tn) * NB + half * COLS;
-            const int valid = row < P.M ? static_cast<int>(max(0ll, min(static_cast<long long>(COLS), P.N - col))) : 0;
+            const int rows = static_cast<int>(min(32ll, P.M - row0)), cols = static_cast<int>(min(static_cast<long long>(COLS), P.N - col));
             if constexpr (C::kAdapter) {
                 const int b = ac.s;
                 if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
                 fence_after();
                 ac.next();
+#pragma unroll 1
+                for (int c = 0; c < COLS && c < cols; c += 64) {
+                    float v[64];
 #pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
-                    float v[32];
-                    tmem_ld32(lane_base + static_cast<uint32_t>(b * NB + c * 32), v);
+                    for (int h = 0; h < 2; ++h) {
+                        float x[32];
+                        tmem_ld32(lane_base + static_cast<uint32_t>(b * NB + c + 32 * h), x);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[32 * h + i] = x[i];
+                    }
+                    const int left = cols - c;
                     if (P.splits > 1) {
-                        store_f32<32>(P.part + (t.s * P.M + row) * P.ldpart + col + 32 * c, v, valid - 32 * c);
+                        store_rows<false, false, true>(buf, v, P.part + (t.q * P.M + row0) * P.ldpart + col + c, P.ldpart, rows, left, lane);
                         continue;
                     }
-                    if (P.ad.lists) {
+                    bool odd = false;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < valid - 32 * c && !(fabsf(v[i]) <= 3.402823466e38f)) v[i] = lone_result<MODE>(P.ad, row, col + 32 * c + i);
-                    }
-                    store_bf16<32>(static_cast<bf16*>(P.out) + row * P.ldo + col + 32 * c, v, valid - 32 * c);
+                    for (int i = 0; i < 64; ++i) odd |= !(fabsf(v[i]) <= 3.402823466e38f);
+                    if (P.ad.lists && __any_sync(~0u, odd && lane < rows)) mend_results<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
+                    store_rows<true, false, true>(buf, v, static_cast<bf16*>(P.out) + row0 * P.ldo + col + c, P.ldo, rows, left, lane);
                 }
                 fence_before();
                 __syncwarp();
@@ -558,9 +669,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             } else {
                 float F[MODE == kFisher ? COLS : 1];
                 if constexpr (MODE == kFisher) {
-                    const float* src = static_cast<const float*>(P.out) + row * P.ldo + col;
+                    if (P.first) {
 #pragma unroll
-                    for (int i = 0; i < COLS; ++i) F[i] = (!P.first && i < valid) ? src[i] : 0.0f;
+                        for (int i = 0; i < COLS; ++i) F[i] = 0.0f;
+                    } else {
+                        load_rows(buf, F, static_cast<const float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
+                    }
                 }
                 const int s1 = MODE == kFisher ? P.S : t.s + 1;
                 for (int s = t.s; s < s1 && ok; ++s) {
@@ -569,19 +683,23 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     float acc[COLS];
 #pragma unroll
                     for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
-                    float* scol = col_scale + warp * 2 * COLS;
+                    float* scol = reinterpret_cast<float*>(buf);  // kHess: the columns' scales of two groups, until results leave
                     // kHess: exponent bytes of this lane's row and of four of the warp's columns, fetched one
                     // group ahead and not touched before (bytes behind the last column go to columns not stored)
                     uint8_t er = 0;
                     uint32_t ec = 0;
                     auto load_exps = [&](int g) {
                         if constexpr (MODE == kHess) {
-                            const uint8_t* e = P.exps + g * P.lde;
+                            const uint8_t* e = P.exps + (u.lo / 128 + g) * P.lde;
                             if (row < P.M) er = __ldg(e + row);
                             if (col + 4 * lane < P.N) ec = __ldg(reinterpret_cast<const uint32_t*>(e + col + 4 * lane));
                         }
                     };
                     if (groups > 0) load_exps(0);
+                    if constexpr (MODE == kHess) {  // the last results have left `scol`
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                    }
                     for (int g = 0; g < groups; ++g) {
                         float srow = 0.0f;
                         if constexpr (MODE == kHess) {
@@ -643,74 +761,84 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                                 ema_next2(F[i], F[i + 1], beta2, contrib2, acc[i], acc[i + 1]);
                             }
                         }
+                    } else if (P.splits > 1) {
+                        store_rows<false, false, MODE == kGrad>(buf, acc, P.part + ((t.q * max(1, P.S) + t.s) * P.M + row0) * P.ldpart + col, P.ldpart, rows, cols, lane);
                     } else if constexpr (MODE == kGrad) {
-                        const long long at = t.s * P.out_stride + row * P.ldo + col;
+                        const long long at = t.s * P.out_stride + row0 * P.ldo + col;
                         if (P.out_tma) {
-                            const int row0 = t.tm * 256 + rank * 128 + quad * 32;
-                            if (row0 < P.M && col < P.N) {
-                                uint8_t* buf = out_buf + warp * 8192;
-                                if (P.out_bf16) store_tma<true>(&tO, buf, acc, static_cast<int>(col), row0, t.s, static_cast<int>(P.N), lane);
-                                else store_tma<false>(&tO, buf, acc, static_cast<int>(col), row0, t.s, static_cast<int>(P.N), lane);
+                            if (rows > 0 && cols > 0) {
+                                if (P.out_bf16) store_tma<true>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), lane);
+                                else store_tma<false>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), lane);
                             }
-                        } else if (P.out_bf16) store_bf16<COLS>(static_cast<bf16*>(P.out) + at, acc, valid);
-                        else store_f32<COLS>(static_cast<float*>(P.out) + at, acc, valid);
-                    } else if (col / 128 <= row / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
-                        float* h = static_cast<float*>(P.out) + row * P.ldo + col;
+                        } else if (P.out_bf16) {
+                            store_rows<true, false, true>(buf, acc, static_cast<bf16*>(P.out) + at, P.ldo, rows, cols, lane);
+                        } else {
+                            store_rows<false, false, true>(buf, acc, static_cast<float*>(P.out) + at, P.ldo, rows, cols, lane);
+                        }
+                    } else if (col / 128 <= row0 / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
+                        float* h = static_cast<float*>(P.out) + row0 * P.ldo + col;
 #pragma unroll
                         for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
-                        if (P.accumulate) add_f32<COLS>(acc, h, valid);
-                        store_f32<COLS>(h, acc, valid);
+                        if (P.out_tma) store_tma<false>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), 0, static_cast<int>(P.N), lane);
+                        else if (P.accumulate) store_rows<false, true, false>(buf, acc, h, P.ldo, rows, cols, lane);
+                        else store_rows<false, false, false>(buf, acc, h, P.ldo, rows, cols, lane);
                     }
                 }
                 if constexpr (MODE == kFisher)
-                    if (ok) store_f32<COLS>(static_cast<float*>(P.out) + row * P.ldo + col, F, valid);
+                    if (ok) store_rows<false, false, false>(buf, F, static_cast<float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
             }
         }
-        if constexpr (MODE == kGrad) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if constexpr (MODE == kGrad || MODE == kHess) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) give_up(abort_flag);
     } else {
         if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kTmaWarp) {
             if (lane == 0) {
+                // (This loop and the MMA warp's bound the products: 60 cycles more a slice are 5 % of their time.)
                 Ring<kStages> at;
-                const bool done = walk<MODE>(P, [&](const Tile& t, const Unit& u, int j, int part, int i) {
-                    const int s = at.s;
-                    if (!wait(smem_u32(&empty[s]), at.phase ^ 1, abort_flag)) return false;  // (the first round passes at once)
+                const uint32_t full0 = smem_u32(full), ready0 = smem_u32(ready) & kPeerMask, empty0 = smem_u32(empty);
+                const bool done = for_units<MODE>(P, [&](const Tile& t, const Unit& u) {
                     const int m0 = t.tm * 256 + rank * 128, n0 = t.tn * NB + rank * C::kCols;
-                    if constexpr (C::kCodes) {
-                        const uint32_t bar = smem_u32(&full[s]);
-                        const int k = u.lo + i * 64;
+                    const bool ok = for_runs(u, [&](int part, int i, int count) {
+                        constexpr int kStep = MODE == kHess ? 128 : 64;
+                        int k = u.lo + i * kStep;
                         // parts with fewer leading bits first: the large ones are then truncated least often
-                        const int y = (P.parts - 1 - part) * P.n + k;
-                        mbar_expect_tx(bar, C::kA + C::kRaw + C::kExps);
-                        tma_load_2d(stage_a(s), &tA, m0, y, bar);
-                        tma_load_2d(stage_a(s) + kMnChunk, &tA, m0 + 64, y, bar);
-                        tma_load_2d(stage_raw(s), &tB, n0, k, bar);
-                        tma_load_2d(smem_u32(exps_buf + s * C::kExps), &tE, n0, k >> 7, bar);
-                    } else {
-                        const uint32_t bar = smem_u32(&ready[s]) & kPeerMask;
-                        const bool built = C::kAdapter && part > 0;  // the prepare warps fill this stage
-                        if (built) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[s])) : "memory");
-                        if (rank == 0) {
-                            if (built) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-                            else {
-                                if (C::kAdapter) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 8;" ::"r"(bar) : "memory");
-                                mbar_expect_tx(bar, 2 * (C::kA + C::kB));
-                            }
-                        }
-                        if (!built) {
-                            const int k = u.lo + i * (MODE == kHess ? 128 : 64);
-                            if constexpr (MODE == kHess) tma_load_pair(stage_a(s), &tA, m0, k, bar);
-                            else tma_load_pair(stage_a(s), &tA, k, m0, bar);
-                            if constexpr (MODE == kFwd) {
-                                tma_load_pair(stage_b(s), &tB, k, n0, bar);
+                        const int above = C::kCodes ? (P.parts - 1 - part) * P.n : 0;
+#pragma unroll 1
+                        for (; count > 0; --count, k += kStep, at.next()) {
+                            const uint32_t a = stage_a(0) + at.s * C::kStage, b = a + C::kA;
+                            if (!wait(empty0 + 8 * at.s, at.phase ^ 1, abort_flag)) return false;  // (the first round passes at once)
+                            if constexpr (C::kCodes) {
+                                const uint32_t bar = full0 + 8 * at.s;
+                                mbar_expect_tx(bar, C::kA + C::kRaw + C::kExps);
+                                tma_load_2d(a, &tA, m0, above + k, bar);
+                                tma_load_2d(a + kMnChunk, &tA, m0 + 64, above + k, bar);
+                                tma_load_2d(b + C::kB, &tB, n0, k, bar);
+                                tma_load_2d(smem_u32(exps_buf) + at.s * C::kExps, &tE, n0, k >> 7, bar);
                             } else {
-                                tma_load_pair(stage_b(s), &tB, n0, k, bar);
-                                if constexpr (MODE == kDx) tma_load_pair(stage_b(s) + kMnChunk, &tB, n0 + 64, k, bar);
+                                const uint32_t bar = ready0 + 8 * at.s;
+                                if (rank == 0) {
+                                    if (C::kAdapter) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 8;" ::"r"(bar) : "memory");
+                                    mbar_expect_tx(bar, 2 * (C::kA + C::kB));
+                                }
+                                if constexpr (MODE == kHess) tma_load_pair(a, &tA, m0, k, bar);
+                                else tma_load_pair(a, &tA, k, m0, bar);
+                                if constexpr (MODE == kFwd) {
+                                    tma_load_pair(b, &tB, k, n0, bar);
+                                } else {
+                                    tma_load_pair(b, &tB, n0, k, bar);
+                                    if constexpr (MODE == kDx) tma_load_pair(b + kMnChunk, &tB, n0 + 64, k, bar);
+                                }
                             }
                         }
+                        return true;
+                    });
+                    if (!ok) return false;
+                    for (int x = 0; C::kAdapter && x < u.extra; ++x, at.next()) {  // the prepare warps fill these stages
+                        if (!wait(empty0 + 8 * at.s, at.phase ^ 1, abort_flag)) return false;
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full0 + 8 * at.s) : "memory");
+                        if (rank == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ready0 + 8 * at.s) : "memory");
                     }
-                    at.next();
                     return true;
                 });
                 if (!done) {
@@ -735,22 +863,27 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 Ring<kStages> at;
                 Ring<C::kAcc> ac;
                 const uint64_t a_desc = operand_desc(stage_a(0), kAmn), b_desc = operand_desc(stage_b(0), kBmn);
-                const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int j, int, int) {
-                    const bool first = j % C::kGroup == 0;
-                    const int b = ac.s;
-                    if (first && !wait(smem_u32(&accempty[b]), ac.phase ^ 1, abort_flag)) return false;
-                    const int s = at.s;
-                    if (!wait(smem_u32(&ready[s]), at.phase, abort_flag)) return false;
-                    fence_after();
-                    const uint64_t a0 = a_desc + s * (C::kStage >> 4), b0 = b_desc + s * (C::kStage >> 4);
-                    const uint32_t d = tmem + static_cast<uint32_t>(b * NB);
+                const uint32_t ready0 = smem_u32(ready), empty0 = smem_u32(empty);
+                const bool done = for_units<MODE>(P, [&](const Tile&, const Unit& u) {
+                    for (int left = u.total + u.extra; left > 0;) {  // a group of slices sums in one accumulator
+                        const uint32_t d = tmem + static_cast<uint32_t>(ac.s * NB);
+                        int n = min(left, C::kGroup);
+                        left -= n;
+                        if (!wait(smem_u32(&accempty[ac.s]), ac.phase ^ 1, abort_flag)) return false;
+                        uint32_t more = 0;
+#pragma unroll 1
+                        for (; n > 0; --n, at.next()) {
+                            const uint64_t a0 = a_desc + at.s * (C::kStage >> 4), b0 = b_desc + at.s * (C::kStage >> 4);
+                            if (!wait(ready0 + 8 * at.s, at.phase, abort_flag)) return false;
+                            fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_step<MODE>(d, a0 + kk * kStepA, b0 + kk * kStepB, kIdesc, !(first && kk == 0));
-                    commit_pair(smem_u32(&empty[s]));
-                    at.next();
-                    if (j + 1 == u.total || j % C::kGroup == C::kGroup - 1) {
-                        commit_pair(smem_u32(&accfull[b]));
+                            for (int kk = 0; kk < 4; ++kk) {
+                                mma_step<MODE>(d, a0 + kk * kStepA, b0 + kk * kStepB, kIdesc, more);
+                                more = 1;
+                            }
+                            commit_pair(empty0 + 8 * at.s);
+                        }
+                        commit_pair(smem_u32(&accfull[ac.s]));
                         ac.next();
                     }
                     return true;
@@ -768,11 +901,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             const int nth = warp < kTmaWarp ? warp - kPrepWarp : warp - kMmaWarp + 3, group = nth / kGroupWarps;
             const int pt = nth % kGroupWarps * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
             Ring<kStages> at;
-            const bool done = walk<MODE>(P, [&](const Tile&, const Unit& u, int, int, int i) {
-                const int s = at.s;
-                const uint32_t phase = at.phase;
-                at.next();
-                if (s % kDecodeGroups != group) return true;
+            auto slice = [&](const Unit& u, int i, int s, uint32_t phase) {
                 const int k0 = u.lo + i * 64;
                 const int valid = min(64, u.hi - k0);
                 const int border = 128 - (k0 & 127);  // first token of the next block
@@ -817,6 +946,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&ready[s]));
                 return true;
+            };
+            const bool done = for_units<MODE>(P, [&](const Tile&, const Unit& u) {
+                return for_runs(u, [&](int, int i, int count) {
+#pragma unroll 1
+                    for (; count > 0; --count, ++i, at.next())
+                        if (at.s % kDecodeGroups == group && !slice(u, i, at.s, at.phase)) return false;
+                    return true;
+                });
             });
             if (!done) give_up(abort_flag);
         } else if (C::kAdapter && warp >= kPrepWarp && warp < kTmaWarp) {
@@ -829,9 +966,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             bool ok = true;
             for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
                 const Tile t = tile_of<MODE>(P, item);
-                const Unit u = unit_of<MODE>(P, t, t.s);
-                it += u.slices;
-                for (int x = 0; x < u.total - u.slices; ++x, ++it) {
+                const Unit u = unit_of<MODE>(P, t, 0);
+                it += u.total;
+                for (int x = 0; x < u.extra; ++x, ++it) {
                     const int s = it % kStages;
                     const int a = __ldg(u.list + 1 + x / u.rslices), r0 = (x % u.rslices) * 32;
                     if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag)) { ok = false; break; }
@@ -857,19 +994,28 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 // Joins the shares of K in order: four consecutive columns per thread.
 template <int MODE>
 __global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant__ Params P) {
-    const long long quads = (P.N + 3) / 4;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < P.M * quads; i += gridDim.x * 256ll) {
+    const long long quads = (P.N + 3) / 4, rows = P.M * max(1, P.S);
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * quads; i += gridDim.x * 256ll) {
         const long long row = i / quads, col = i % quads * 4;
+        if (MODE == kHess && col / 128 > row / 128) continue;
         float v[4] = {};
-        for (int s = 0; s < P.splits; ++s) {
-            const float4 f = *reinterpret_cast<const float4*>(P.part + (s * P.M + row) * P.ldpart + col);
+        for (int q = 0; q < P.splits; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(P.part + (q * rows + row) * P.ldpart + col);
             v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
         }
+        const long long at = MODE == kGrad ? row / P.M * P.out_stride + row % P.M * P.ldo + col : row * P.ldo + col;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (col + e >= P.N) break;
-            if (P.ad.lists && !(fabsf(v[e]) <= 3.402823466e38f)) v[e] = lone_result<MODE>(P.ad, row, col + e);
-            static_cast<bf16*>(P.out)[row * P.ldo + col + e] = __float2bfloat16_rn(v[e]);
+            if constexpr (MODE == kHess) {
+                float* h = static_cast<float*>(P.out) + at + e;
+                *h = P.accumulate ? *h + P.scale * v[e] : P.scale * v[e];
+            } else {
+                if constexpr (Cfg<MODE>::kAdapter)
+                    if (P.ad.lists && !(fabsf(v[e]) <= 3.402823466e38f)) v[e] = lone_result<MODE>(P.ad, row, col + e);
+                if (Cfg<MODE>::kAdapter || P.out_bf16) static_cast<bf16*>(P.out)[at + e] = __float2bfloat16_rn(v[e]);
+                else static_cast<float*>(P.out)[at + e] = v[e];
+            }
         }
     }
 }
@@ -889,6 +1035,8 @@ int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
 }
+
+constexpr long long kPairs = 74;  // one CTA on each of the 148 SMs
 
 template <int MODE>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, const Params& P, cudaStream_t st) {
@@ -912,22 +1060,41 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, con
             if (dev < 64) prepared |= 1ull << dev;
         }
     }
-    constexpr int kPairs = 74;  // one CTA on each of the 148 SMs
-    const int pairs = std::min(P.items, kPairs);
+    const int pairs = static_cast<int>(std::min<long long>(P.items, kPairs));
     linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, o, P);
     return check_launch("linear_kernel");
 }
 
-int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
-
-// Items are counted in 32 bits.
-int set_items(Params* P, long long items, const char* who) {
-    if (items > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, items);
-    P->items = static_cast<int>(items);
-    return TB_OK;
+// launch() of `units` sums of about `slices` K slices each.  Fewer than half as
+// many as pairs of SMs: their K is shared out, at least 8 slices a share, so that
+// all pairs work, and joined by a second kernel.  (64 tokens' forward, 4096 x
+// 4096: 33.6 us with one share, 19.3 with four and the join.)
+template <int MODE>
+int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, Params& P, long long units,
+                  long long slices, const char* who, cudaStream_t st) {
+    P.splits = MODE == kFisher ? 1 : static_cast<int>(std::max(1ll, std::min(kPairs / std::max(1ll, units), slices / 8)));
+    if (units * P.splits > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, units);
+    P.items = static_cast<int>(units * P.splits);
+    P.ldpart = (P.N + 7) / 8 * 8;
+    if (P.splits == 1) return launch<MODE>(a, b, e, o, P, st);
+    const long long rows = P.M * std::max(1, P.S);
+    void* part = nullptr;
+    int rc = scratch_alloc(&part, sizeof(float) * P.splits * rows * P.ldpart, st);
+    if (rc) return rc;
+    P.part = static_cast<float*>(part);
+    rc = launch<MODE>(a, b, e, o, P, st);
+    if (!rc) {
+        const long long quads = rows * ((P.N + 3) / 4);
+        join_splits_kernel<MODE><<<static_cast<unsigned>(std::min((quads + 255) / 256, 148ll * 8)), 256, 0, st>>>(P);
+        rc = check_launch("join_splits_kernel");
+    }
+    scratch_free(part, st);
+    return rc;
 }
 
-// Gradients [S][r][d] as boxes of 32 rows x 128 bytes, where every row starts on 16 bytes.
+int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
+
+// Results [S][r][d] as boxes of 32 rows x 128 bytes, where every row starts on 16 bytes (else out_tma stays 0).
 int make_out_map(CUtensorMap* map, Params* P, int r, int d, int S) {
     const int esize = P->out_bf16 ? 2 : 4;
     P->out_tma = reinterpret_cast<uintptr_t>(P->out) % 16 == 0 && d * esize % 16 == 0 && P->out_stride * esize % 16 == 0;
@@ -955,13 +1122,15 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     P.n = static_cast<int>(ck.n);
     P.parts = dy.parts;
     P.ldo = ck.d;
-    int rc = set_items(&P, static_cast<long long>(P.tiles_m) * P.tiles_n * samples, who);
+    int rc = TB_OK;
     CUtensorMap a{}, b{}, e{}, o{};
-    if (!rc && MODE == kGrad) rc = make_out_map(&o, &P, r, ck.d, static_cast<int>(samples));
+    if (MODE == kGrad) rc = make_out_map(&o, &P, r, ck.d, static_cast<int>(samples));
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
     if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 2, false);
-    return rc ? rc : launch<MODE>(a, b, e, o, P, st);
+    const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
+    // (the samples' lengths are on the device: an even split)
+    return rc ? rc : launch_shared<MODE>(a, b, e, o, P, units, ck.n / samples * dy.parts / 64, who, st);
 }
 
 }  // namespace
@@ -1001,10 +1170,15 @@ int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaSt
     P.ldo = ck.d;
     P.scale = scale;
     P.accumulate = accumulate;
-    int rc = set_items(&P, static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2, "tb_act8_hessian");
+    if (P.tiles_m > 46000) return fail(TB_ERR_CAPACITY, "tb_act8_hessian: %d features", ck.d);  // tiles are counted in 31 bits
+    int rc = TB_OK;
     CUtensorMap a{};
-    if (!rc && ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
-    return rc ? rc : launch<kHess>(a, a, a, a, P, st);
+    if (ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
+    CUtensorMap o{};
+    P.out_stride = static_cast<long long>(ck.d) * ck.d;
+    if (!rc && !accumulate) rc = make_out_map(&o, &P, ck.d, ck.d, 1);
+    const long long units = static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2;
+    return rc ? rc : launch_shared<kHess>(a, a, a, o, P, units, (ck.n + 127) / 128, "tb_act8_hessian", st);
 }
 
 template <int MODE>
@@ -1019,26 +1193,12 @@ static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_
     P.out = p.out;
     P.ldo = p.ldout;
     P.ad = p;
-    // Fewer tiles than half the pairs of SMs: share out K, at least 8 slices each, so that all work.
-    // (64 tokens, 4096 x 4096: one share 33.6 us, four 15 us with the join.)
-    const long long tiles_all = static_cast<long long>(P.tiles_m) * P.tiles_n;
-    P.splits = static_cast<int>(std::max(1ll, std::min<long long>(74 / std::max(1ll, tiles_all), (p.K + 63) / 64 / 8)));
-    P.ldpart = (P.N + 7) / 8 * 8;
-    void* part = nullptr;
-    int rc = set_items(&P, tiles_all * P.splits, who);
-    if (!rc && P.splits > 1) rc = scratch_alloc(&part, sizeof(float) * P.splits * P.M * P.ldpart, st);
-    P.part = static_cast<float*>(part);
+    int rc = TB_OK;
     CUtensorMap a{}, b{};
     if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
     if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
                                : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
-    if (!rc) rc = launch<MODE>(a, b, b, b, P, st);
-    if (!rc && P.splits > 1) {
-        const long long quads = P.M * ((P.N + 3) / 4);
-        join_splits_kernel<MODE><<<static_cast<unsigned>(std::min((quads + 255) / 256, 148ll * 8)), 256, 0, st>>>(P);
-        rc = check_launch("join_splits_kernel");
-    }
-    scratch_free(part, st);
+    if (!rc) rc = launch_shared<MODE>(a, b, b, b, P, static_cast<long long>(P.tiles_m) * P.tiles_n, (p.K + 63) / 64, who, st);
     return rc;
 }
 

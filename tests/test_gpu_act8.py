@@ -138,7 +138,9 @@ def check_sums(torch, got, want, mag, terms, bf16=False):
     (700, 129, 384, "float32", "float32", [(0, 127), (127, 500), (500, 700)]),
     (515, 200, 272, "float16", "float32", [(3, 130), (400, 512)]),
     (2000, 384, 640, "bfloat16", "bfloat16", [(0, 700), (650, 1400), (1400, 2000), (0, 2000), (0, 700)]),
-    (4100, 256, 256, "bfloat16", "float32", None), (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)])])
+    (4100, 256, 256, "bfloat16", "float32", None),
+    (3000, 100, 203, "float32", "bfloat16", [(0, 1500), (1500, 3000)]), (6000, 264, 130, "float16", "float32", [(7, 5900), (0, 10), (3, 3)]),
+    (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)])])
 def test_weight_grad(cuda, tblib, n, r, d, dy_t, g_t, samples):
     torch, tb = cuda, tblib
     c = packed(torch, tb, rows(torch, n, d, torch.float32, n))
@@ -267,7 +269,8 @@ def test_fisher_equals_its_steps(cuda, tblib):
 
 
 @pytest.mark.parametrize("n,d,acc", [(1, 1, False), (64, 128, False), (130, 200, True), (1000, 640, False),
-                                     (777, 515, True), (0, 96, False), (0, 96, True), (4096, 256, False), (300, 1100, True)])
+                                     (777, 515, True), (0, 96, False), (0, 96, True), (4096, 256, False), (300, 1100, True),
+                                     (5000, 300, True), (9000, 130, False)])
 def test_hessian(cuda, tblib, n, d, acc):
     torch, tb = cuda, tblib
     x = rows(torch, n, d, torch.float32, n + d)
