@@ -73,10 +73,10 @@ struct Cfg {
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
     static constexpr int kReady = kCodes ? 2 * kGroupWarps : kAdapter ? 9 : 1;
-    static constexpr int kStages = MODE == kGrad ? 4 : MODE == kHess ? 5 : 6;
+    static constexpr int kStages = MODE == kGrad ? 4 : 6;
     static_assert(!kCodes || kStages % kDecodeGroups == 0, "a stage has one group of decoding warps");
-    // Behind the stages: pieces of results on their way out (for TMA two a warp), the exponents of each stage
-    static constexpr int kOutWarp = MODE == kGrad || MODE == kHess ? 8192 : 4096;
+    // Behind the stages: pieces of results on their way out, the exponents of each stage
+    static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
     static constexpr int kOut = kEpiWarps * kOutWarp;
     static constexpr int kExtra = kOut + kStages * kExps;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 512;
@@ -99,7 +99,7 @@ struct Params {
     float alpha, beta, contrib, scale;
     int first, accumulate;
     AdapterProduct ad;
-    // with splits > 1 the K range of a unit is shared out and FP32 sums go to part [splits][samples * M][ldpart]
+    // with splits > 1 the K range of a unit is shared out; where `part` is given, FP32 sums go there, [splits][samples * M][ldpart]
     int splits;
     float* part;
     long long ldpart;
@@ -355,46 +355,27 @@ __device__ __forceinline__ void fill_piece(uint8_t* buf, const float (&v)[COLS],
 // Byte `at` of row r.
 __device__ __forceinline__ int piece_at(int r, int at) { return r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15); }
 
-template <bool BF16, bool ADD>
-__device__ __forceinline__ void store_piece(const uint8_t* buf, void* out, long long ld, int rows, int cols, int lane) {
+template <bool BF16>
+__device__ __noinline__ void store_piece(const uint8_t* buf, void* out, long long ld, int rows, int cols, int lane) {
     constexpr int kSize = Piece<BF16>::kSize;
     char* p = static_cast<char*>(out);
     const long long pitch = ld * kSize;
     const unsigned align = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) | pitch);
     if (cols >= Piece<BF16>::kCols && align % 16 == 0) {
         const int sub = lane >> 3, unit = (lane & 7) * 16;
-        float4 old[8];
-        if constexpr (ADD) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (4 * i + sub < rows) old[i] = *reinterpret_cast<const float4*>(p + (4 * i + sub) * pitch + unit);
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int r = 4 * i + sub;
-            uint4 w = *reinterpret_cast<const uint4*>(buf + piece_at(r, unit));
-            if constexpr (ADD)
-                w = make_uint4(__float_as_uint(old[i].x + __uint_as_float(w.x)), __float_as_uint(old[i].y + __uint_as_float(w.y)),
-                               __float_as_uint(old[i].z + __uint_as_float(w.z)), __float_as_uint(old[i].w + __uint_as_float(w.w)));
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + piece_at(r, unit));
             if (r < rows) *reinterpret_cast<uint4*>(p + r * pitch + unit) = w;
         }
     } else if (!BF16 || align % 4 == 0) {  // a word a lane; a last odd BF16 column by itself
         const int at = 4 * lane, left = cols * kSize - at;
         if (left >= 4) {
-#pragma unroll 1
-            for (int r0 = 0; r0 < rows; r0 += 16) {
-                float old[16];
-                if constexpr (ADD) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (r0 + r < rows) old[r] = *reinterpret_cast<const float*>(p + (r0 + r) * pitch + at);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    uint32_t w = *reinterpret_cast<const uint32_t*>(buf + piece_at(r0 + r, at));
-                    if constexpr (ADD) w = __float_as_uint(old[r] + __uint_as_float(w));
-                    if (r0 + r < rows) *reinterpret_cast<uint32_t*>(p + (r0 + r) * pitch + at) = w;
-                }
+#pragma unroll 16
+            for (int r = 0; r < 32; ++r) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + piece_at(r, at));
+                if (r < rows) *reinterpret_cast<uint32_t*>(p + r * pitch + at) = w;
             }
         } else if (left == 2) {
 #pragma unroll 1
@@ -403,21 +384,17 @@ __device__ __forceinline__ void store_piece(const uint8_t* buf, void* out, long 
     } else {
 #pragma unroll 1
         for (int at = 2 * lane; at < 2 * cols; at += 64) {
-#pragma unroll 8
+#pragma unroll 16
             for (int r = 0; r < 32; ++r) {
-                if (r >= rows) break;
-                *reinterpret_cast<uint16_t*>(p + r * pitch + at) = *reinterpret_cast<const uint16_t*>(buf + piece_at(r, at));
+                const uint16_t w = *reinterpret_cast<const uint16_t*>(buf + piece_at(r, at));
+                if (r < rows) *reinterpret_cast<uint16_t*>(p + r * pitch + at) = w;
             }
         }
     }
 }
-// The same as a function of its own, for the kernels that have several kinds of results.
-template <bool BF16>
-__device__ __noinline__ void store_piece_call(const uint8_t* buf, void* out, long long ld, int rows, int cols, int lane) {
-    store_piece<BF16, false>(buf, out, ld, rows, cols, lane);
-}
-// All of the warp's pieces; `out` is its first row and column.
-template <bool BF16, bool ADD, bool CALL, int COLS>
+// All of the warp's pieces; `out` is its first row and column.  (A piece's store is a function of its
+// own: inlined for every piece and kind of result, it cost the other roles 6 to 8 %.)
+template <bool BF16, int COLS>
 __device__ __forceinline__ void store_rows(uint8_t* buf, const float (&v)[COLS], void* out, long long ld, int rows, int cols, int lane) {
     if (rows <= 0) return;
 #pragma unroll
@@ -426,27 +403,32 @@ __device__ __forceinline__ void store_rows(uint8_t* buf, const float (&v)[COLS],
         __syncwarp();
         fill_piece<BF16>(buf, v, c, lane);
         __syncwarp();
-        if constexpr (CALL) store_piece_call<BF16>(buf, static_cast<char*>(out) + c * 128, ld, rows, cols - c * Piece<BF16>::kCols, lane);
-        else store_piece<BF16, ADD>(buf, static_cast<char*>(out) + c * 128, ld, rows, cols - c * Piece<BF16>::kCols, lane);
+        store_piece<BF16>(buf, static_cast<char*>(out) + c * 128, ld, rows, cols - c * Piece<BF16>::kCols, lane);
     }
 }
-// The same by TMA, two pieces in flight: sixteen 4096 x 4096 gradients in 336 us, where straight
-// from registers, 32 bytes of a row a lane, they took 400.
-template <bool BF16, int COLS>
+// The same by TMA, as many pieces in flight as there are buffers, stored or (FP32) added to what is
+// there: sixteen 4096 x 4096 gradients in 336 us, where straight from registers, 32 bytes of a row a
+// lane, they took 400.
+template <bool BF16, int PIECES, int COLS>
 __device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, const float (&v)[COLS], int col, int row0, int s, int N,
-                                          int lane) {
+                                          bool add, int lane) {
 #pragma unroll
     for (int c = 0; c < COLS / Piece<BF16>::kCols; ++c) {
-        uint8_t* piece = buf + (c & 1) * kPieceBytes;
-        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the piece before last has left its buffer
+        uint8_t* piece = buf + c % PIECES * kPieceBytes;
+        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PIECES - 1) : "memory");  // the buffer's last piece has left it
         __syncwarp();
         fill_piece<BF16>(piece, v, c, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-            if (col + c * Piece<BF16>::kCols < N)
+            const int x = col + c * Piece<BF16>::kCols;
+            if (x < N && add)
+                asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                             "r"(x), "r"(row0), "r"(s), "r"(smem_u32(piece))
+                             : "memory");
+            else if (x < N)
                 asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
-                             "r"(col + c * Piece<BF16>::kCols), "r"(row0), "r"(s), "r"(smem_u32(piece))
+                             "r"(x), "r"(row0), "r"(s), "r"(smem_u32(piece))
                              : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
@@ -654,14 +636,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     }
                     const int left = cols - c;
                     if (P.splits > 1) {
-                        store_rows<false, false, true>(buf, v, P.part + (t.q * P.M + row0) * P.ldpart + col + c, P.ldpart, rows, left, lane);
+                        store_rows<false>(buf, v, P.part + (t.q * P.M + row0) * P.ldpart + col + c, P.ldpart, rows, left, lane);
                         continue;
                     }
                     bool odd = false;
 #pragma unroll
                     for (int i = 0; i < 64; ++i) odd |= !(fabsf(v[i]) <= 3.402823466e38f);
                     if (P.ad.lists && __any_sync(~0u, odd && lane < rows)) mend_results<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
-                    store_rows<true, false, true>(buf, v, static_cast<bf16*>(P.out) + row0 * P.ldo + col + c, P.ldo, rows, left, lane);
+                    store_rows<true>(buf, v, static_cast<bf16*>(P.out) + row0 * P.ldo + col + c, P.ldo, rows, left, lane);
                 }
                 fence_before();
                 __syncwarp();
@@ -761,31 +743,27 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                                 ema_next2(F[i], F[i + 1], beta2, contrib2, acc[i], acc[i + 1]);
                             }
                         }
-                    } else if (P.splits > 1) {
-                        store_rows<false, false, MODE == kGrad>(buf, acc, P.part + ((t.q * max(1, P.S) + t.s) * P.M + row0) * P.ldpart + col, P.ldpart, rows, cols, lane);
-                    } else if constexpr (MODE == kGrad) {
-                        const long long at = t.s * P.out_stride + row0 * P.ldo + col;
-                        if (P.out_tma) {
-                            if (rows > 0 && cols > 0) {
-                                if (P.out_bf16) store_tma<true>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), lane);
-                                else store_tma<false>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), lane);
-                            }
-                        } else if (P.out_bf16) {
-                            store_rows<true, false, true>(buf, acc, static_cast<bf16*>(P.out) + at, P.ldo, rows, cols, lane);
-                        } else {
-                            store_rows<false, false, true>(buf, acc, static_cast<float*>(P.out) + at, P.ldo, rows, cols, lane);
-                        }
-                    } else if (col / 128 <= row0 / 128) {  // kHess: this 128 x 128 tile is on or below the diagonal
-                        float* h = static_cast<float*>(P.out) + row0 * P.ldo + col;
+                    } else {
+                        if constexpr (MODE == kHess) {
 #pragma unroll
-                        for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
-                        if (P.out_tma) store_tma<false>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), 0, static_cast<int>(P.N), lane);
-                        else if (P.accumulate) store_rows<false, true, false>(buf, acc, h, P.ldo, rows, cols, lane);
-                        else store_rows<false, false, false>(buf, acc, h, P.ldo, rows, cols, lane);
+                            for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
+                        }
+                        // kHess: only 128 x 128 tiles on or below the diagonal
+                        const bool wanted = rows > 0 && cols > 0 && (MODE == kGrad || col / 128 <= row0 / 128);
+                        const int z = P.part ? t.q * max(1, P.S) + t.s : t.s;
+                        if (MODE == kHess || P.out_tma) {
+                            if (!wanted) continue;
+                            if (MODE == kGrad && P.out_bf16 && !P.part) store_tma<true, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), z, static_cast<int>(P.N), false, lane);
+                            else store_tma<false, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), z, static_cast<int>(P.N), MODE == kHess && P.accumulate && !P.part, lane);
+                        } else if constexpr (MODE == kGrad) {
+                            const long long at = t.s * P.out_stride + row0 * P.ldo + col;
+                            if (P.out_bf16) store_rows<true>(buf, acc, static_cast<bf16*>(P.out) + at, P.ldo, rows, cols, lane);
+                            else store_rows<false>(buf, acc, static_cast<float*>(P.out) + at, P.ldo, rows, cols, lane);
+                        }
                     }
                 }
                 if constexpr (MODE == kFisher)
-                    if (ok) store_rows<false, false, false>(buf, F, static_cast<float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
+                    if (ok) store_rows<false>(buf, F, static_cast<float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
             }
         }
         if constexpr (MODE == kGrad || MODE == kHess) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1009,7 +987,7 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant_
             if (col + e >= P.N) break;
             if constexpr (MODE == kHess) {
                 float* h = static_cast<float*>(P.out) + at + e;
-                *h = P.accumulate ? *h + P.scale * v[e] : P.scale * v[e];
+                *h = P.accumulate ? *h + v[e] : v[e];
             } else {
                 if constexpr (Cfg<MODE>::kAdapter)
                     if (P.ad.lists && !(fabsf(v[e]) <= 3.402823466e38f)) v[e] = lone_result<MODE>(P.ad, row, col + e);
@@ -1065,24 +1043,48 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, con
     return check_launch("linear_kernel");
 }
 
+// Results [samples][rows][cols] in rows of ld, as boxes of 32 rows x 128 bytes.
+int make_out_map(CUtensorMap* map, void* base, bool bf16_out, long long cols, long long rows, long long samples, long long ld, long long stride) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return fail(TB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const int esize = bf16_out ? 2 : 4;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(samples)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * esize, static_cast<cuuint64_t>(stride) * esize};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esize), 32, 1}, estr[3] = {1, 1, 1};
+    const CUresult e = enc(map, bf16_out ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims,
+                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(e));
+}
+
 // launch() of `units` sums of about `slices` K slices each.  Fewer than half as
 // many as pairs of SMs: their K is shared out, at least 8 slices a share, so that
 // all pairs work, and joined by a second kernel.  (64 tokens' forward, 4096 x
-// 4096: 33.6 us with one share, 19.3 with four and the join.)
+// 4096: 33.6 us with one share, 19.3 with four and the join.)  The Hessian takes
+// that way too where its rows do not start on 16 bytes, as TMA wants them.
 template <int MODE>
-int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, Params& P, long long units,
-                  long long slices, const char* who, cudaStream_t st) {
+int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, Params& P, long long units, long long slices,
+                  const char* who, cudaStream_t st) {
+    constexpr bool kTma = MODE == kGrad || MODE == kHess;
+    const long long samples = std::max(1, P.S), rows = P.M * samples;
     P.splits = MODE == kFisher ? 1 : static_cast<int>(std::max(1ll, std::min(kPairs / std::max(1ll, units), slices / 8)));
     if (units * P.splits > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, units);
     P.items = static_cast<int>(units * P.splits);
     P.ldpart = (P.N + 7) / 8 * 8;
-    if (P.splits == 1) return launch<MODE>(a, b, e, o, P, st);
-    const long long rows = P.M * std::max(1, P.S);
+    const int esize = P.out_bf16 ? 2 : 4;
+    P.out_tma = kTma && reinterpret_cast<uintptr_t>(P.out) % 16 == 0 && P.ldo * esize % 16 == 0 && P.out_stride * esize % 16 == 0;
+    CUtensorMap o{};
+    if (P.splits == 1 && (MODE != kHess || P.out_tma)) {
+        const int rc = P.out_tma ? make_out_map(&o, P.out, P.out_bf16, P.N, P.M, samples, P.ldo, P.out_stride) : TB_OK;
+        return rc ? rc : launch<MODE>(a, b, e, o, P, st);
+    }
     void* part = nullptr;
     int rc = scratch_alloc(&part, sizeof(float) * P.splits * rows * P.ldpart, st);
     if (rc) return rc;
     P.part = static_cast<float*>(part);
-    rc = launch<MODE>(a, b, e, o, P, st);
+    P.out_tma = kTma;
+    if (kTma) rc = make_out_map(&o, part, false, P.N, P.M, samples * P.splits, P.ldpart, P.M * P.ldpart);
+    if (!rc) rc = launch<MODE>(a, b, e, o, P, st);
     if (!rc) {
         const long long quads = rows * ((P.N + 3) / 4);
         join_splits_kernel<MODE><<<static_cast<unsigned>(std::min((quads + 255) / 256, 148ll * 8)), 256, 0, st>>>(P);
@@ -1093,21 +1095,6 @@ int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap&
 }
 
 int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
-
-// Results [S][r][d] as boxes of 32 rows x 128 bytes, where every row starts on 16 bytes (else out_tma stays 0).
-int make_out_map(CUtensorMap* map, Params* P, int r, int d, int S) {
-    const int esize = P->out_bf16 ? 2 : 4;
-    P->out_tma = reinterpret_cast<uintptr_t>(P->out) % 16 == 0 && d * esize % 16 == 0 && P->out_stride * esize % 16 == 0;
-    EncodeFn enc = encode_fn();
-    if (!P->out_tma || !enc) return TB_OK;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(r), static_cast<cuuint64_t>(S)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(d) * esize, static_cast<cuuint64_t>(P->out_stride) * esize};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esize), 32, 1}, estr[3] = {1, 1, 1};
-    const CUresult e = enc(map, esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, P->out, dims,
-                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return e == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(e));
-}
 
 template <int MODE>
 int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long long samples, const char* who, cudaStream_t st) {
@@ -1123,14 +1110,13 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     P.parts = dy.parts;
     P.ldo = ck.d;
     int rc = TB_OK;
-    CUtensorMap a{}, b{}, e{}, o{};
-    if (MODE == kGrad) rc = make_out_map(&o, &P, r, ck.d, static_cast<int>(samples));
+    CUtensorMap a{}, b{}, e{};
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
     if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 2, false);
     const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
     // (the samples' lengths are on the device: an even split)
-    return rc ? rc : launch_shared<MODE>(a, b, e, o, P, units, ck.n / samples * dy.parts / 64, who, st);
+    return rc ? rc : launch_shared<MODE>(a, b, e, P, units, ck.n / samples * dy.parts / 64, who, st);
 }
 
 }  // namespace
@@ -1174,11 +1160,9 @@ int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaSt
     int rc = TB_OK;
     CUtensorMap a{};
     if (ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
-    CUtensorMap o{};
     P.out_stride = static_cast<long long>(ck.d) * ck.d;
-    if (!rc && !accumulate) rc = make_out_map(&o, &P, ck.d, ck.d, 1);
     const long long units = static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2;
-    return rc ? rc : launch_shared<kHess>(a, a, a, o, P, units, (ck.n + 127) / 128, "tb_act8_hessian", st);
+    return rc ? rc : launch_shared<kHess>(a, a, a, P, units, (ck.n + 127) / 128, "tb_act8_hessian", st);
 }
 
 template <int MODE>
@@ -1198,7 +1182,7 @@ static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_
     if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
     if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
                                : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
-    if (!rc) rc = launch_shared<MODE>(a, b, b, b, P, static_cast<long long>(P.tiles_m) * P.tiles_n, (p.K + 63) / 64, who, st);
+    if (!rc) rc = launch_shared<MODE>(a, b, b, P, static_cast<long long>(P.tiles_m) * P.tiles_n, (p.K + 63) / 64, who, st);
     return rc;
 }
 
