@@ -18,7 +18,7 @@
 //
 // Modes:
 //   kGrad    G_s = dY_s^T Xhat_s: A = dY (M-major by TMA), B = decoded codes
-//   kFisher  the same with the EMA of g^2 in registers, samples in order
+//   kFisher  the same with the Fisher state in registers, samples in order
 //   kHess    Xhat^T Xhat on int8 tensor cores: the codes of a block of 128
 //            tokens multiply exactly into int32, and the block's two
 //            power-of-two scales enter when its sum is added in FP32
@@ -60,11 +60,12 @@ struct Cfg {
     static constexpr bool kCodes = MODE == kGrad || MODE == kFisher;   // B from codes
     static constexpr bool kAdapter = MODE == kFwd || MODE == kDx;
     static constexpr bool kPromote = !kAdapter;
-    static constexpr int NB = MODE == kFisher ? 128 : 256;             // columns of a pair's tile
+    static constexpr int NB = 256;                                     // columns of a pair's tile
     static constexpr int kAcc = 512 / NB;                              // accumulators in TMEM
     static constexpr int kCols = NB / 2;                               // columns of an epilogue warp, and of a CTA's B
-    // K slices summed in TMEM before they are added in FP32: 256 tokens, or one block of codes
-    static constexpr int kGroup = kCodes ? 4 : MODE == kHess ? 1 : 1 << 30;
+    // K slices summed in TMEM before they are added in FP32: 512 tokens (kGrad), one block of codes
+    // (kHess), all (16-bit results).  kFisher: see kDirect.
+    static constexpr int kGroup = MODE == kGrad ? 8 : MODE == kFisher ? 4 : MODE == kHess ? 1 : 1 << 30;
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
     static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
@@ -73,7 +74,7 @@ struct Cfg {
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
     static constexpr int kReady = kCodes ? 2 * kGroupWarps : kAdapter ? 9 : 1;
-    static constexpr int kStages = MODE == kGrad ? 4 : 6;
+    static constexpr int kStages = kCodes ? 4 : 6;
     static_assert(!kCodes || kStages % kDecodeGroups == 0, "a stage has one group of decoding warps");
     // Behind the stages: pieces of results on their way out, the exponents of each stage
     static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
@@ -200,6 +201,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// kFisher has the Fisher state in the registers that would add a sample's groups
+// up.  A sample of at most kDirect slices (1024 tokens of BF16 dy) is summed in
+// TMEM alone: the tensor core's truncated additions then leave a relative 1e-7 in
+// g where signs are mixed, as an FP32 product's rounding does, and at most
+// 64 2^-24 where all terms have one sign.  For a longer one the state waits in
+// its place in memory, once, while groups of 256 tokens are added in FP32.
+constexpr int kDirect = 16;
+
 // ---- the walk over work items, units (one sum each) and K slices that every role shares ----
 struct Tile {
     int tm, tn;
@@ -209,6 +218,7 @@ struct Unit {
     int lo, hi;         // K range
     int slices;         // K slices of one part
     int first, total;   // the share's slices, counted over the parts
+    int group;          // slices summed in one accumulator
     int extra;          // adapters: slices behind those of K,
     int rslices;        // so many for each adapter
     const int32_t* list;
@@ -250,7 +260,7 @@ __device__ __forceinline__ int share_begin(int all, int q, int splits) {
 }
 template <int MODE>
 __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
-    Unit u{0, P.K, 0, 0, 0, 0, 1, nullptr};
+    Unit u{0, P.K, 0, 0, 0, Cfg<MODE>::kGroup, 0, 1, nullptr};
     if constexpr (Cfg<MODE>::kCodes) {
         u.hi = P.n;
         if (P.samples) {
@@ -260,6 +270,7 @@ __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
         }
         u.slices = (u.hi - u.lo + 63) / 64;
         u.total = u.slices * P.parts;
+        if (MODE == kFisher && u.total <= kDirect) u.group = kDirect;
         if (MODE != kFisher && P.splits > 1) {
             u.first = share_begin(u.slices * P.parts, t.q, P.splits);
             u.total = share_begin(u.slices * P.parts, t.q + 1, P.splits) - u.first;
@@ -434,21 +445,16 @@ __device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, 
         }
     }
 }
-// Reads FP32 rows.
-template <int COLS>
-__device__ __forceinline__ void load_rows(uint8_t* buf, float (&v)[COLS], const float* p, long long ld, int rows, int cols, int lane) {
-#pragma unroll
-    for (int c = 0; c < COLS / 32; ++c) {
-        __syncwarp();
+// Reads a piece of FP32 rows: 32 columns of the lane's row.
+__device__ __forceinline__ void load_piece(uint8_t* buf, float* v, const float* p, long long ld, int rows, int cols, int lane) {
+    __syncwarp();
 #pragma unroll 16
-        for (int r = 0; r < 32; ++r)
-            *reinterpret_cast<float*>(buf + piece_at(r, 4 * lane)) = r < rows && 32 * c + lane < cols ? p[r * ld + 32 * c + lane] : 0.0f;
-        __syncwarp();
+    for (int r = 0; r < 32; ++r) *reinterpret_cast<float*>(buf + piece_at(r, 4 * lane)) = r < rows && lane < cols ? p[r * ld + lane] : 0.0f;
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float4 w = *reinterpret_cast<const float4*>(buf + piece_at(lane, 16 * j));
-            v[32 * c + 4 * j] = w.x; v[32 * c + 4 * j + 1] = w.y; v[32 * c + 4 * j + 2] = w.z; v[32 * c + 4 * j + 3] = w.w;
-        }
+    for (int j = 0; j < 8; ++j) {
+        const float4 w = *reinterpret_cast<const float4*>(buf + piece_at(lane, 16 * j));
+        v[4 * j] = w.x; v[4 * j + 1] = w.y; v[4 * j + 2] = w.z; v[4 * j + 3] = w.w;
     }
 }
 
@@ -553,6 +559,27 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
     }
 }
 
+// f(c, x) for each 16 columns x of this lane's row of a finished accumulator, the
+// next read under way meanwhile; the accumulator is given back before the last.
+template <int COLS, class F>
+__device__ __forceinline__ void read_accumulator(uint32_t from, uint32_t accempty, int lane, F&& f) {
+    fence_after();
+    uint32_t v[2][16];
+    tmem_ld16(from, v[0]);
+#pragma unroll
+    for (int c = 0; c < COLS / 16; ++c) {
+        tmem_wait16(v[c & 1]);
+        if (c + 1 < COLS / 16) {
+            tmem_ld16(from + static_cast<uint32_t>(16 * (c + 1)), v[(c + 1) & 1]);
+        } else {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_even(accempty);
+        }
+        f(c, v[c & 1]);
+    }
+}
+
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CUtensorMap tB,
@@ -648,20 +675,66 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&accempty[b]));
-            } else {
-                float F[MODE == kFisher ? COLS : 1];
-                if constexpr (MODE == kFisher) {
-                    if (P.first) {
+            } else if constexpr (MODE == kFisher) {
+                float* out = static_cast<float*>(P.out) + row0 * P.ldo + col;
+                float F[COLS];
+                if (P.first) {
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i) F[i] = 0.0f;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) load_piece(buf, F + 32 * c, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
+                }
+                const uint64_t beta2 = pack2(P.beta, P.beta);
+                for (int s = 0; s < P.S && ok; ++s) {
+                    const Unit u = unit_of<MODE>(P, t, s);
+                    // the first step, (alpha g) g, is a later one from F = 0 with its own factor
+                    const float factor = P.first && s == 0 ? P.alpha : P.contrib;
+                    const uint64_t factor2 = pack2(factor, factor);
+                    if (u.total > kDirect) {
+                        store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
 #pragma unroll
                         for (int i = 0; i < COLS; ++i) F[i] = 0.0f;
-                    } else {
-                        load_rows(buf, F, static_cast<const float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
+                        for (int left = u.total; left > 0 && ok; left -= u.group) {
+                            const int b = ac.s;
+                            if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
+                            ac.next();
+                            read_accumulator<COLS>(lane_base + static_cast<uint32_t>(b * NB), smem_u32(&accempty[b]), lane, [&](int c, uint32_t (&x)[16]) {
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) add2(F[c * 16 + i], F[c * 16 + i + 1], x[i], x[i + 1]);
+                            });
+                        }
+#pragma unroll
+                        for (int c = 0; c < COLS / 32; ++c) {
+                            float old[32];
+                            load_piece(buf, old, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                ema_next2(old[i], old[i + 1], beta2, factor2, F[32 * c + i], F[32 * c + i + 1]);
+                                F[32 * c + i] = old[i];
+                                F[32 * c + i + 1] = old[i + 1];
+                            }
+                        }
+                    } else if (u.total > 0) {
+                        const int b = ac.s;
+                        if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
+                        ac.next();
+                        read_accumulator<COLS>(lane_base + static_cast<uint32_t>(b * NB), smem_u32(&accempty[b]), lane, [&](int c, uint32_t (&x)[16]) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                ema_next2(F[c * 16 + i], F[c * 16 + i + 1], beta2, factor2, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                        });
+                    } else {  // no tokens: g = 0
+#pragma unroll
+                        for (int i = 0; i < COLS; ++i) F[i] = __fmul_rn(P.beta, F[i]);
                     }
                 }
-                const int s1 = MODE == kFisher ? P.S : t.s + 1;
-                for (int s = t.s; s < s1 && ok; ++s) {
+                if (ok) store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
+            } else {
+                {
+                    const int s = t.s;
                     const Unit u = unit_of<MODE>(P, t, s);
-                    const int groups = (u.total + C::kGroup - 1) / C::kGroup;
+                    const int groups = (u.total + u.group - 1) / u.group;
                     float acc[COLS];
 #pragma unroll
                     for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
@@ -695,24 +768,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         }
                         const int b = ac.s;
                         if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
-                        fence_after();
                         ac.next();
-                        // 16 columns at a time, the next read under way while these are added; the accumulator
-                        // is given back before the last are
-                        uint32_t v[2][16];
-                        const uint32_t from = lane_base + static_cast<uint32_t>(b * NB);
-                        tmem_ld16(from, v[0]);
-#pragma unroll
-                        for (int c = 0; c < COLS / 16; ++c) {
-                            uint32_t (&x)[16] = v[c & 1];
-                            tmem_wait16(x);
-                            if (c + 1 < COLS / 16) {
-                                tmem_ld16(from + static_cast<uint32_t>(16 * (c + 1)), v[(c + 1) & 1]);
-                            } else {
-                                fence_before();
-                                __syncwarp();
-                                if (lane == 0) arrive_even(smem_u32(&accempty[b]));
-                            }
+                        read_accumulator<COLS>(lane_base + static_cast<uint32_t>(b * NB), smem_u32(&accempty[b]), lane, [&](int c, uint32_t (&x)[16]) {
                             if constexpr (MODE == kHess) {
                                 // |block sum| <= 128 * 127^2 < 2^22: as the low bits of 1.5 * 2^23 it is an
                                 // exact FP32 value, and subtracting that base times the row's power of two too
@@ -728,22 +785,10 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 #pragma unroll
                                 for (int i = 0; i < 16; i += 2) add2(acc[c * 16 + i], acc[c * 16 + i + 1], x[i], x[i + 1]);
                             }
-                        }
+                        });
                     }
                     if (!ok) break;
-                    if constexpr (MODE == kFisher) {
-                        const bool first = P.first && s == 0;
-                        const uint64_t beta2 = pack2(P.beta, P.beta), contrib2 = pack2(P.contrib, P.contrib);
-#pragma unroll
-                        for (int i = 0; i < COLS; i += 2) {
-                            if (first) {
-                                F[i] = ema_first(P.alpha, acc[i]);
-                                F[i + 1] = ema_first(P.alpha, acc[i + 1]);
-                            } else {
-                                ema_next2(F[i], F[i + 1], beta2, contrib2, acc[i], acc[i + 1]);
-                            }
-                        }
-                    } else {
+                    {
                         if constexpr (MODE == kHess) {
 #pragma unroll
                             for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
@@ -762,8 +807,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         }
                     }
                 }
-                if constexpr (MODE == kFisher)
-                    if (ok) store_rows<false>(buf, F, static_cast<float*>(P.out) + row0 * P.ldo + col, P.ldo, rows, cols, lane);
             }
         }
         if constexpr (MODE == kGrad || MODE == kHess) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -845,7 +888,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 const bool done = for_units<MODE>(P, [&](const Tile&, const Unit& u) {
                     for (int left = u.total + u.extra; left > 0;) {  // a group of slices sums in one accumulator
                         const uint32_t d = tmem + static_cast<uint32_t>(ac.s * NB);
-                        int n = min(left, C::kGroup);
+                        int n = min(left, u.group);
                         left -= n;
                         if (!wait(smem_u32(&accempty[ac.s]), ac.phase ^ 1, abort_flag)) return false;
                         uint32_t more = 0;

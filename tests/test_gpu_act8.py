@@ -227,7 +227,9 @@ def test_weight_grad_leaves_other_tokens_out(cuda, tblib):
 
 @pytest.mark.parametrize("n,r,d,dy_t,S,first", [
     (60, 128, 128, "float32", 8, True), (600, 130, 70, "bfloat16", 3, False), (1, 5, 9, "bfloat16", 1, True),
-    (900, 256, 640, "bfloat16", 7, True), (513, 384, 257, "float16", 4, False), (3000, 136, 264, "bfloat16", 2, True)])
+    (900, 256, 640, "bfloat16", 7, True), (513, 384, 257, "float16", 4, False), (3000, 136, 264, "bfloat16", 2, True),
+    (5000, 300, 515, "bfloat16", 3, False), (2600, 264, 136, "float32", 4, True), (1025, 72, 520, "bfloat16", 1, False),
+    (1024, 72, 520, "bfloat16", 1, True), (4000, 520, 300, "float16", 2, False)])
 def test_fisher(cuda, tblib, n, r, d, dy_t, S, first):
     """The EMA of the float64 gradients: each g is within its sum's bar, a square doubles that, and each step rounds four times."""
     torch, tb = cuda, tblib
