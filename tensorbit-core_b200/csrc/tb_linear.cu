@@ -69,7 +69,7 @@ struct Cfg {
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
     static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
-    static constexpr int kExps = kCodes ? 2 * kCols : 0;               // exponents of its first block and the next
+    static constexpr int kExps = kCodes ? kCols : 0;                   // exponents of its block
     static constexpr int kStage = kA + kB + kRaw;
     // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
@@ -215,7 +215,8 @@ struct Tile {
     int s, q;           // sample; share of K
 };
 struct Unit {
-    int lo, hi;         // K range
+    int lo, hi;         // K range (samples: lo rounded down to a whole slice,
+    int begin;          // begin the first token)
     int slices;         // K slices of one part
     int first, total;   // the share's slices, counted over the parts
     int group;          // slices summed in one accumulator
@@ -260,15 +261,16 @@ __device__ __forceinline__ int share_begin(int all, int q, int splits) {
 }
 template <int MODE>
 __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
-    Unit u{0, P.K, 0, 0, 0, Cfg<MODE>::kGroup, 0, 1, nullptr};
+    Unit u{0, P.K, 0, 0, 0, 0, Cfg<MODE>::kGroup, 0, 1, nullptr};
     if constexpr (Cfg<MODE>::kCodes) {
         u.hi = P.n;
         if (P.samples) {
             const long long b = __ldg(P.samples + 2 * s), e = __ldg(P.samples + 2 * s + 1);
-            u.lo = static_cast<int>(min(max(b, 0ll), static_cast<long long>(P.n)));
-            u.hi = static_cast<int>(max(min(e, static_cast<long long>(P.n)), static_cast<long long>(u.lo)));
+            u.begin = static_cast<int>(min(max(b, 0ll), static_cast<long long>(P.n)));
+            u.hi = static_cast<int>(max(min(e, static_cast<long long>(P.n)), static_cast<long long>(u.begin)));
+            u.lo = u.begin & ~63;  // a slice then lies in one block of codes
         }
-        u.slices = (u.hi - u.lo + 63) / 64;
+        u.slices = u.hi > u.begin ? (u.hi - u.lo + 63) / 64 : 0;
         u.total = u.slices * P.parts;
         if (MODE == kFisher && u.total <= kDirect) u.group = kDirect;
         if (MODE != kFisher && P.splits > 1) {
@@ -923,18 +925,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             const int pt = nth % kGroupWarps * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
             Ring<kStages> at;
             auto slice = [&](const Unit& u, int i, int s, uint32_t phase) {
-                const int k0 = u.lo + i * 64;
-                const int valid = min(64, u.hi - k0);
-                const int border = 128 - (k0 & 127);  // first token of the next block
+                // the slice's tokens first .. last - 1 are the sample's
+                const int k0 = u.lo + i * 64, first = max(0, u.begin - k0), last = min(64, u.hi - k0);
                 if (!wait(smem_u32(&full[s]), phase, abort_flag)) return false;
                 uint8_t* stage = smem + s * C::kStage;
                 const uint8_t* raw = stage + C::kA + C::kB;
-                const uint8_t* exps = exps_buf + s * C::kExps + pc * 8;
-                uint32_t s0[4], s1[4] = {0, 0, 0, 0};
-                act8::scales8(*reinterpret_cast<const uint2*>(exps), s0);
+                uint32_t scale[4];
+                act8::scales8(*reinterpret_cast<const uint2*>(exps_buf + s * C::kExps + pc * 8), scale);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
-                const bool whole = valid == 64 && border >= 64;
-                if (!whole) act8::scales8(*reinterpret_cast<const uint2*>(exps + C::kCols), s1);
 #pragma unroll
                 for (int h = 0; h < kSteps; h += kBatch) {
                     uint2 w[kBatch];
@@ -943,26 +941,19 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         const int k = pr + (h + q) * kRowStep;
                         if (h + q < kSteps && k < 64) w[q] = *reinterpret_cast<const uint2*>(raw + k * C::kCols + pc * 8);
                     }
-                    if (whole) {
 #pragma unroll
-                        for (int q = 0; q < kBatch; ++q) {
-                            const int k = pr + (h + q) * kRowStep;
-                            if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], s0);
-                        }
-                    } else {  // a block's or the sample's end within the slice
-#pragma unroll
-                        for (int q = 0; q < kBatch; ++q) {
-                            const int k = pr + (h + q) * kRowStep;
-                            uint32_t sk[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) sk[e] = k >= valid ? 0u : k >= border ? s1[e] : s0[e];
-                            if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], sk);
-                        }
+                    for (int q = 0; q < kBatch; ++q) {
+                        const int k = pr + (h + q) * kRowStep;
+                        if (k < first || k >= last) w[q] = make_uint2(0, 0);
+                        if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], scale);
                     }
                 }
-                // tokens behind the sample's end: dY may hold anything there
-                for (int q = pt; q < (64 - valid) * 16; q += kThreadsGroup)
-                    *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + (valid + (q >> 4)) * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                // the other tokens: dY may hold anything there.  (Their codes are zero now; a block that holds a
+                // NaN is infinitely scaled, but then it is NaN for the sample's tokens in it too.)
+                for (int q = pt; q < (first + 64 - last) * 16; q += kThreadsGroup) {
+                    const int r = q >> 4, k = r < first ? r : last + r - first;
+                    *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + k * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&ready[s]));
@@ -1156,7 +1147,7 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     CUtensorMap a{}, b{}, e{};
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
-    if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 2, false);
+    if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 1, false);
     const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
     // (the samples' lengths are on the device: an even split)
     return rc ? rc : launch_shared<MODE>(a, b, e, P, units, ck.n / samples * dy.parts / 64, who, st);
