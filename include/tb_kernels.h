@@ -304,10 +304,12 @@ int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
  * 148-201) per sample, in their order, without the gradients in memory: with
  * G_s as above in FP32, the first step (first_step != 0, F not read) gives
- * F = (alpha g) g, the others F = beta F + ((alpha (1 - beta)) g) g, with the
- * factors rounded to FP32 once.  (alpha and beta are double because 1 - beta
- * of an FP32 0.99 is off by 1e-6; FP32 values give tb_fisher_ema_step's own
- * factors.)  fisher is [r][d].  A sample without tokens is a step with g = 0. */
+ * F = alpha g^2, the others F = beta F + alpha (1 - beta) g^2.  Formed, as
+ * tb_fisher_weighted_sum does, as the sum of the samples' g^2 with the factors
+ * that these steps give them (in double, rounded to FP32 once): it agrees with
+ * the serial recurrence of tb_fisher_ema_step to FP32 rounding.  (alpha and beta
+ * are double because 1 - beta of an FP32 0.99 is off by 1e-6.)  fisher is [r][d].
+ * A sample without tokens is a step with g = 0. */
 int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r, const int64_t* samples,
                    int S, double alpha, double beta, int first_step, float* fisher, void* stream);
 /* H = scale * Xhat^T Xhat (accumulate != 0: added to H): tb_obs_hessian_scaled

@@ -362,10 +362,7 @@ extern "C" int tb_act8_fisher(const tb_act8* ckp, const void* dy, int dy_dtype, 
     linear::Parts parts{};
     void* scratch = nullptr;
     rc = prepare_dy(ck, dy, dy_dtype, lddy, r, st, &parts, &scratch);
-    // 1 - beta loses a relative 1e-6 where beta is rounded to FP32 first: formed in double, rounded once
-    if (!rc)
-        rc = linear::fisher(ck, parts, r, samples, S, static_cast<float>(alpha), static_cast<float>(beta),
-                            static_cast<float>(alpha * (1.0 - beta)), first_step != 0, fisher, st);
+    if (!rc) rc = linear::fisher(ck, parts, r, samples, S, alpha, beta, first_step != 0, fisher, st);
     scratch_free(scratch, st);
     return rc;
 }

@@ -18,7 +18,8 @@
 //
 // Modes:
 //   kGrad    G_s = dY_s^T Xhat_s: A = dY (M-major by TMA), B = decoded codes
-//   kFisher  the same with the Fisher state in registers, samples in order
+//   kFisher  the same with the Fisher state in registers: a sum of the samples' g^2
+//            with the factors that the EMA's steps give them, in order
 //   kHess    Xhat^T Xhat on int8 tensor cores: the codes of a block of 128
 //            tokens multiply exactly into int32, and the block's two
 //            power-of-two scales enter when its sum is added in FP32
@@ -79,7 +80,8 @@ struct Cfg {
     // Behind the stages: pieces of results on their way out, the exponents of each stage
     static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
     static constexpr int kOut = kEpiWarps * kOutWarp;
-    static constexpr int kExtra = kOut + kStages * kExps;
+    static constexpr int kFactors = MODE == kFisher ? 1024 : 0;        // samples whose factor is held in shared memory
+    static constexpr int kExtra = kOut + kStages * kExps + kFactors * 4;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 512;
     static_assert(kSmem <= 232448, "shared memory of a block");
 };
@@ -97,7 +99,8 @@ struct Params {
     void* out;
     long long ldo, out_stride;
     int out_bf16, out_tma;
-    float alpha, beta, contrib, scale;
+    double alpha, beta;
+    float scale;
     int first, accumulate;
     AdapterProduct ad;
     // with splits > 1 the K range of a unit is shared out; where `part` is given, FP32 sums go there, [splits][samples * M][ldpart]
@@ -561,6 +564,19 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
     }
 }
 
+// What the square of sample s's gradient counts for in the state after all S steps
+// F <- beta F + alpha (1 - beta) g^2, the first of which, on no state, is alpha g^2.
+__device__ __forceinline__ float fisher_factor(const Params& P, int s) {
+    return static_cast<float>(P.alpha * (P.first && s == 0 ? 1.0 : 1.0 - P.beta) * pow(P.beta, static_cast<double>(P.S - 1 - s)));
+}
+// Two lanes of F += (w g) g in packed FP32.
+__device__ __forceinline__ void square_add2(float& f0, float& f1, uint64_t w2, float g0, float g1) {
+    asm("{\n\t.reg .b64 F, G, T;\n\tmov.b64 F, {%0, %1};\n\tmov.b64 G, {%3, %4};\n\t"
+        "mul.rn.f32x2 T, %2, G;\n\tfma.rn.f32x2 F, T, G, F;\n\tmov.b64 {%0, %1}, F;\n\t}"
+        : "+f"(f0), "+f"(f1)
+        : "l"(w2), "f"(g0), "f"(g1));
+}
+
 // f(c, x) for each 16 columns x of this lane's row of a finished accumulator, the
 // next read under way meanwhile; the accumulator is given back before the last.
 template <int COLS, class F>
@@ -594,6 +610,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* out_buf = smem + kStages * C::kStage;
     uint8_t* exps_buf = out_buf + C::kOut;
+    float* factors = reinterpret_cast<float*>(exps_buf + kStages * C::kExps);
     uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + C::kExtra);
     uint64_t* ready = full + kStages;     // (even CTA) stage prepared by both CTAs
     uint64_t* empty = ready + kStages;    // stage read by the MMAs
@@ -621,6 +638,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if constexpr (MODE == kFisher)
+        for (int s = threadIdx.x; s < min(P.S, C::kFactors); s += kThreads) factors[s] = fisher_factor(P, s);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(512));
@@ -687,11 +706,13 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) load_piece(buf, F + 32 * c, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
                 }
-                const uint64_t beta2 = pack2(P.beta, P.beta);
+                const float decay = static_cast<float>(pow(P.beta, static_cast<double>(P.S)));  // of the state before
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) F[i] *= decay;
                 for (int s = 0; s < P.S && ok; ++s) {
                     const Unit u = unit_of<MODE>(P, t, s);
-                    // the first step, (alpha g) g, is a later one from F = 0 with its own factor
-                    const float factor = P.first && s == 0 ? P.alpha : P.contrib;
+                    if (u.total == 0) continue;  // no tokens: g = 0
+                    const float factor = s < C::kFactors ? factors[s] : fisher_factor(P, s);
                     const uint64_t factor2 = pack2(factor, factor);
                     if (u.total > kDirect) {
                         store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
@@ -712,23 +733,20 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                             load_piece(buf, old, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                ema_next2(old[i], old[i + 1], beta2, factor2, F[32 * c + i], F[32 * c + i + 1]);
+                                square_add2(old[i], old[i + 1], factor2, F[32 * c + i], F[32 * c + i + 1]);
                                 F[32 * c + i] = old[i];
                                 F[32 * c + i + 1] = old[i + 1];
                             }
                         }
-                    } else if (u.total > 0) {
+                    } else {
                         const int b = ac.s;
                         if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
                         ac.next();
                         read_accumulator<COLS>(lane_base + static_cast<uint32_t>(b * NB), smem_u32(&accempty[b]), lane, [&](int c, uint32_t (&x)[16]) {
 #pragma unroll
                             for (int i = 0; i < 16; i += 2)
-                                ema_next2(F[c * 16 + i], F[c * 16 + i + 1], beta2, factor2, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                square_add2(F[c * 16 + i], F[c * 16 + i + 1], factor2, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
                         });
-                    } else {  // no tokens: g = 0
-#pragma unroll
-                        for (int i = 0; i < COLS; ++i) F[i] = __fmul_rn(P.beta, F[i]);
                     }
                 }
                 if (ok) store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
@@ -1166,15 +1184,14 @@ int weight_grad(const act8::View& ck, const Parts& dy, int r, const int64_t* sam
     return from_codes<kGrad>(ck, dy, r, P, S, "tb_act8_weight_grad", st);
 }
 
-int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, float alpha, float beta,
-           float contrib, bool first, float* F, cudaStream_t st) {
+int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, double alpha, double beta, bool first,
+           float* F, cudaStream_t st) {
     Params P{};
     P.samples = samples;
     P.S = S;
     P.out = F;
     P.alpha = alpha;
     P.beta = beta;
-    P.contrib = contrib;
     P.first = first;
     return from_codes<kFisher>(ck, dy, r, P, 1, "tb_act8_fisher", st);
 }

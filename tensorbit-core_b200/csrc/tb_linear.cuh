@@ -21,8 +21,8 @@ struct Parts {
 
 int weight_grad(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, void* grads, int g_dtype,
                 long long g_stride, cudaStream_t st);
-int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, float alpha, float beta,
-           float contrib, bool first, float* F, cudaStream_t st);
+int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, double alpha, double beta, bool first,
+           float* F, cudaStream_t st);
 int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaStream_t st);
 
 constexpr int kListTokens = 256;              // tokens of one list of adapters
