@@ -48,13 +48,11 @@ __device__ int g_linear_error;
 
 constexpr int kThreads = 512;
 constexpr int kEpiWarps = 8, kPrepWarp = 8, kTmaWarp = 12, kMmaWarp = 13;
-// Codes are decoded by two groups of three warps (8-10 and 11, 14, 15), every
-// second slice each: a slice's chain of wait, loads, arithmetic, stores, fence and
-// arrival overlaps the next one's.  The number of stages is a multiple of the
-// groups, so a stage always has the same group: a barrier's parity says nothing
-// to a waiter that skips phases (TMA loads may complete out of order), so each
-// phase of full[s] has to be waited for by who waits for the next.
-constexpr int kDecodeGroups = 2, kGroupWarps = 3;
+// Codes are decoded by six warps (8-11, 14, 15).  (All six a slice: 313 us for
+// sixteen gradients of a q_proj, where two groups of three, every second slice
+// each, took 332.  Groups that skip a barrier's phases may not wait on its parity
+// in any case: TMA loads can complete out of order.)
+constexpr int kDecodeWarps = 6;
 
 template <int MODE>
 struct Cfg {
@@ -72,11 +70,10 @@ struct Cfg {
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
     static constexpr int kExps = kCodes ? kCols : 0;                   // exponents of its block
     static constexpr int kStage = kA + kB + kRaw;
-    // Arrivals that make a stage ready: a group of decoding warps of each CTA (codes), the even CTA's
+    // Arrivals that make a stage ready: the decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
-    static constexpr int kReady = kCodes ? 2 * kGroupWarps : kAdapter ? 9 : 1;
+    static constexpr int kReady = kCodes ? 2 * kDecodeWarps : kAdapter ? 9 : 1;
     static constexpr int kStages = kCodes ? 4 : 6;
-    static_assert(!kCodes || kStages % kDecodeGroups == 0, "a stage has one group of decoding warps");
     // Behind the stages: pieces of results on their way out, the exponents of each stage
     static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
     static constexpr int kOut = kEpiWarps * kOutWarp;
@@ -937,10 +934,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             __syncwarp();
         } else if (C::kCodes) {
             // 8 consecutive features (one 16-byte unit of the operand) of every kRowStep-th token
-            constexpr int kThreadsGroup = 32 * kGroupWarps, kUnits = C::kCols / 8, kRowStep = kThreadsGroup / kUnits;
-            constexpr int kSteps = (64 + kRowStep - 1) / kRowStep, kBatch = 6;
-            const int nth = warp < kTmaWarp ? warp - kPrepWarp : warp - kMmaWarp + 3, group = nth / kGroupWarps;
-            const int pt = nth % kGroupWarps * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
+            constexpr int kUnits = C::kCols / 8, kRowStep = 32 * kDecodeWarps / kUnits, kSteps = (64 + kRowStep - 1) / kRowStep;
+            const int pt = (warp < kTmaWarp ? warp - kPrepWarp : warp - kMmaWarp + 3) * 32 + lane, pc = pt % kUnits, pr = pt / kUnits;
             Ring<kStages> at;
             auto slice = [&](const Unit& u, int i, int s, uint32_t phase) {
                 // the slice's tokens first .. last - 1 are the sample's
@@ -951,24 +946,23 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 uint32_t scale[4];
                 act8::scales8(*reinterpret_cast<const uint2*>(exps_buf + s * C::kExps + pc * 8), scale);
                 uint8_t* dst = stage + C::kA + (pc >> 3) * kMnChunk;
+                uint2 w[kSteps];
 #pragma unroll
-                for (int h = 0; h < kSteps; h += kBatch) {
-                    uint2 w[kBatch];
+                for (int q = 0; q < kSteps; ++q)
+                    if (pr + q * kRowStep < 64) w[q] = *reinterpret_cast<const uint2*>(raw + (pr + q * kRowStep) * C::kCols + pc * 8);
+                if (first > 0 || last < 64) {
 #pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        const int k = pr + (h + q) * kRowStep;
-                        if (h + q < kSteps && k < 64) w[q] = *reinterpret_cast<const uint2*>(raw + k * C::kCols + pc * 8);
-                    }
+                    for (int q = 0; q < kSteps; ++q)
+                        if (pr + q * kRowStep < first || pr + q * kRowStep >= last) w[q] = make_uint2(0, 0);
+                }
 #pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        const int k = pr + (h + q) * kRowStep;
-                        if (k < first || k >= last) w[q] = make_uint2(0, 0);
-                        if (h + q < kSteps && k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], scale);
-                    }
+                for (int q = 0; q < kSteps; ++q) {
+                    const int k = pr + q * kRowStep;
+                    if (k < 64) *reinterpret_cast<uint4*>(dst + k * 128 + (((pc & 7) ^ (k & 7)) << 4)) = act8::decode8(w[q], scale);
                 }
                 // the other tokens: dY may hold anything there.  (Their codes are zero now; a block that holds a
                 // NaN is infinitely scaled, but then it is NaN for the sample's tokens in it too.)
-                for (int q = pt; q < (first + 64 - last) * 16; q += kThreadsGroup) {
+                for (int q = pt; q < (first + 64 - last) * 16; q += 32 * kDecodeWarps) {
                     const int r = q >> 4, k = r < first ? r : last + r - first;
                     *reinterpret_cast<uint4*>(stage + (q & 1) * kMnChunk + k * 128 + ((q >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -981,7 +975,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 return for_runs(u, [&](int, int i, int count) {
 #pragma unroll 1
                     for (; count > 0; --count, ++i, at.next())
-                        if (at.s % kDecodeGroups == group && !slice(u, i, at.s, at.phase)) return false;
+                        if (!slice(u, i, at.s, at.phase)) return false;
                     return true;
                 });
             });
