@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args g, const Order o, 
 // block has 16 output features (rows of A in m16n8k16) and up to 8 NT tokens;
 // its 8 warps take every eighth group of 32 in features, so that the block reads
 // 512 consecutive bytes of each row at a time, and join their sums in order.
-// Launched while down_kernel still runs: u is not read before the wait.
+// Launched while down_small_kernel still runs: u is not read before the wait, while
+// x and w, which no kernel here writes, are.
 template <int NT>
 __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const float* u) {
     __shared__ float red[8][16][8 * NT + 1];
@@ -619,6 +620,11 @@ constexpr int kFewTokens = 32;
 
 template <int NT>
 cudaError_t launch_few(const Args& g, const float* u, cudaStream_t st) {
+    // Without adapters the kernel before this one is the caller's, which may still be writing x when it lets go.
+    if (!g.na) {
+        few_tokens_kernel<NT><<<(g.r + 15) / 16, 256, 0, st>>>(g, u);
+        return cudaGetLastError();
+    }
     return launch_pdl(few_tokens_kernel<NT>, dim3((g.r + 15) / 16), dim3(256), 0, st, g, u);
 }
 

@@ -70,7 +70,7 @@ SHAPES = [
     (520, 1024, 384, 32, 5, "runs"), (100, 77, 51, 8, 2, "none"), (90, 200, 72, 12, 0, "none"),
     (1100, 256, 640, 100, 3, "runs"), (1024, 96, 80, 16, 3, "mixed"), (1025, 96, 80, 16, 3, "mixed"),
     (2500, 264, 392, 64, 2, "mixed"), (3000, 128, 136, 8, 1, "one"), (1500, 72, 40, 128, 20, "mixed"),
-    (2100, 136, 72, 24, 300, "mixed"), (1300, 64, 72, 16, 4, "none"), (2048, 72, 64, 40, 2, "wild")]
+    (5, 136, 200, 16, 0, "none"), (32, 264, 136, 16, 0, "none"), (2100, 136, 72, 24, 300, "mixed"), (1300, 64, 72, 16, 4, "none"), (2048, 72, 64, 40, 2, "wild")]
 
 
 @pytest.mark.parametrize("n,d,r,rank,na,kind", SHAPES)
@@ -216,6 +216,34 @@ def test_calls_repeat_bit_for_bit_and_under_graphs(cuda, tblib):
         graphs[k].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for k in (0, 1) for a, b in zip(outs(k), want[k]))
+
+
+@pytest.mark.parametrize("n,na", [(1, 3), (5, 0), (20, 3), (32, 3)])
+def test_few_tokens_under_graphs_and_on_two_streams(cuda, tblib, n, na):
+    """The forward that starts while its down projection runs: captured, replayed with new tokens, two at once."""
+    torch, tb = cuda, tblib
+    cases = [Case(torch, n, 520, 392, 24, na, who_of(torch, n, na, "mixed", i), 70 + i) for i in range(2)]
+    graphs = []
+    for c in cases:
+        tb.check(tb.adapter_forward(c.args(tb)))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.x.mul_(1.0)
+            tb.check(tb.adapter_forward(c.args(tb), stream=torch.cuda.current_stream().cuda_stream))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(4):
+        for k, c in enumerate(cases):
+            c.x.copy_(bf(torch, n, 520, 90 + 2 * i + k))
+            c.y.fill_(3.0)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for c in cases:
+            check(torch, c.y[:n, :392], c.ref.forward(c.x), c.ref.forward(c.x, True), 520 + 24)
+            assert bool((c.y[n:] == 3).all())
 
 
 def test_calibration_step_with_adapters(cuda, tblib):
