@@ -471,10 +471,7 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NT; ++i) {  // two tokens' values of a rank as one word, high parts and low parts
-            const __nv_bfloat162 hi = __floats2bfloat162_rn(va[i], vb[i]);
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(va[i] - __low2float(hi), vb[i] - __high2float(hi));
-            sm.vp[0][pair][k8 + 8 * i] = *reinterpret_cast<const uint32_t*>(&hi);
-            sm.vp[1][pair][k8 + 8 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+            linear::split_pair(va[i], vb[i], sm.vp[0][pair][k8 + 8 * i], sm.vp[1][pair][k8 + 8 * i]);
         }
         // rows g, g+8 of tile m: features 2m, 2m+1 of the lane's eight
         uint32_t x[4][4];

@@ -138,6 +138,16 @@ __device__ __forceinline__ void give_up(volatile int* abort_flag) {
 __device__ __forceinline__ void arrive_even(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar & kPeerMask) : "memory");
 }
+// Sets a flag of both CTAs, before what this warp tells anyone next.
+__device__ __forceinline__ void set_pair(volatile int* flag) {
+    const uint32_t here = smem_u32(const_cast<int*>(flag));
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.u32 [a], %1;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 1;\n\tst.shared::cluster.u32 [a], %1;\n\t"
+        "fence.acq_rel.cluster;\n\t}" ::"r"(here), "r"(1)
+        : "memory");
+}
 template <int MODE>
 __device__ __forceinline__ void mma_step(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     if constexpr (MODE == kHess)
@@ -460,42 +470,45 @@ __device__ __forceinline__ void load_piece(uint8_t* buf, float* v, const float* 
     }
 }
 
-// One result of an adapter product on its own.  An adapter's operands are zero
-// for the other tokens of its tile, but zero times an infinity or a NaN of that
-// adapter is not: a result that is not finite is formed again from what belongs
-// to its token alone.
+// An adapter's second factor enters the product for all tokens of a tile, times
+// zero for those of other adapters; zero times an infinity or a NaN is not zero.
+// Such values are therefore left out of the operand, which notes that there were
+// any, and the epilogue adds their terms to the results of the adapter's own tokens.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool& odd) {
+    if ((w & 0x7F80u) == 0x7F80u) {
+        w &= 0xFFFF0000u;
+        odd = true;
+    }
+    if ((w & 0x7F800000u) == 0x7F800000u) {
+        w &= 0xFFFFu;
+        odd = true;
+    }
+    return w;
+}
+// Result i of token t, feature o + i, is at v[32 i].  (Not unrolled: it hardly ever runs.)
 template <int MODE>
-__device__ __noinline__ float lone_result(const AdapterProduct& p, long long t, long long o) {
-    float y = 0.0f;
-    for (int k = 0; k < p.K; ++k)
-        y = fmaf(__bfloat162float(p.in[t * p.ldin + k]),
-                 __bfloat162float(MODE == kFwd ? p.w[o * p.ldw + k] : p.w[k * p.ldw + o]), y);
+__device__ __noinline__ void add_odd_row(const AdapterProduct& p, float* v, long long t, long long o, int cols) {
     const int a = p.who[t];
-    if (a >= 0 && a < p.na)
-        for (int j = 0; j < p.rank; ++j)
-            y = fmaf(p.u[t * p.rank + j],
-                     __bfloat162float(MODE == kFwd ? p.e[(static_cast<long long>(a) * p.N + o) * p.lde + j]
-                                                   : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o]),
-                     y);
-    return y;
-}
-
-// The results of one row that are not finite, formed again (not unrolled: it hardly ever runs).
-template <int MODE>
-__device__ __noinline__ void mend_row(const AdapterProduct& p, float* v, long long t, long long o, int cols) {
-    for (int i = 0; i < cols; ++i)
-        if (!(fabsf(v[32 * i]) <= 3.402823466e38f)) v[32 * i] = lone_result<MODE>(p, t, o + i);
+    if (a < 0 || a >= p.na) return;
+    for (int j = 0; j < p.rank; ++j) {
+        const float u = p.u[t * p.rank + j];
+        for (int i = 0; i < cols; ++i) {
+            const float e = __bfloat162float(MODE == kFwd ? p.e[(static_cast<long long>(a) * p.N + o + i) * p.lde + j]
+                                                          : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o + i]);
+            if (!(fabsf(e) <= 3.402823466e38f)) v[32 * i] = fmaf(u, e, v[32 * i]);
+        }
+    }
 }
 template <int MODE>
-__device__ __forceinline__ void mend_results(const AdapterProduct& p, uint8_t* buf, float (&v)[64], long long row0, long long col,
-                                             int rows, int cols, int lane) {
+__device__ __forceinline__ void add_odd_terms(const AdapterProduct& p, uint8_t* buf, float (&v)[64], long long row0, long long col,
+                                              int rows, int cols, int lane) {
     float* x = reinterpret_cast<float*>(buf) + lane;  // column i of this lane's row at 32 i
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[32 * i] = v[32 * h + i];
-        if (lane < rows) mend_row<MODE>(p, x, row0 + lane, col + 32 * h, min(32, cols - 32 * h));
+        if (lane < rows) add_odd_row<MODE>(p, x, row0 + lane, col + 32 * h, min(32, cols - 32 * h));
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[32 * h + i] = x[32 * i];
     }
@@ -504,10 +517,11 @@ __device__ __forceinline__ void mend_results(const AdapterProduct& p, uint8_t* b
 
 // Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
 // tile's tokens' u as two BF16 parts, zero unless the adapter is their own; B is
-// the adapter's second factor, twice.
+// the adapter's second factor, twice, its finite values.  True if it has others.
 template <int MODE>
-__device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, int r0, long long m0, int n0, uint8_t* sa,
+__device__ __forceinline__ bool build_adapter(const AdapterProduct& p, int a, int r0, long long m0, int n0, uint8_t* sa,
                                               uint8_t* sb, int pt) {
+    bool odd = false;
     const int nr = min(32, p.rank - r0);
     const long long tok = m0 + pt;
     const bool mine = tok < p.n && __ldg(p.who + tok) == a;
@@ -520,8 +534,7 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
         for (int i = 0; i < 4; ++i) {
             const int j = 8 * q + 2 * i;
             const float f0 = mine && j < nr ? up[j] : 0.0f, f1 = mine && j + 1 < nr ? up[j + 1] : 0.0f;
-            hi[i] = pack_bf16(f0, f1);
-            lo[i] = pack_bf16(f0 - __uint_as_float(hi[i] << 16), f1 - __uint_as_float(hi[i] & 0xFFFF0000u));
+            split_pair(f0, f1, hi[i], lo[i]);
         }
         *reinterpret_cast<uint4*>(arow + ((q ^ (pt & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(arow + (((q + 4) ^ (pt & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -539,7 +552,7 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = 8 * q + 2 * i;
-                    w[i] = j + 1 < nr ? in[i] : j < nr ? in[i] & 0xFFFFu : 0u;
+                    w[i] = finite_pair(j + 1 < nr ? in[i] : j < nr ? in[i] & 0xFFFFu : 0u, odd);
                 }
             }
             const uint4 v4 = make_uint4(w[0], w[1], w[2], w[3]);
@@ -554,11 +567,13 @@ __device__ __forceinline__ void build_adapter(const AdapterProduct& p, int a, in
             const int k = (pt >> 4) + 8 * i;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (f < p.N && k < nr) v = __ldg(reinterpret_cast<const uint4*>(p.e + (static_cast<long long>(a) * p.rank + r0 + k) * p.lde + f));
+            v = make_uint4(finite_pair(v.x, odd), finite_pair(v.y, odd), finite_pair(v.z, odd), finite_pair(v.w, odd));
             const int unit = ((c & 7) ^ (k & 7)) << 4;
             *reinterpret_cast<uint4*>(dst + k * 128 + unit) = v;
             *reinterpret_cast<uint4*>(dst + (k + 32) * 128 + unit) = v;
         }
     }
+    return odd;
 }
 
 // What the square of sample s's gradient counts for in the state after all S steps
@@ -615,6 +630,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint64_t* accempty = accfull + C::kAcc;   // [kAcc] (even CTA) accumulator taken by both CTAs
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + C::kAcc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* odd_flag = abort_flag + 1;  // an adapter's factor had values that are not finite (set in both CTAs, never reset)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
 
@@ -633,6 +649,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             mbar_init(smem_u32(&accempty[b]), 2 * kEpiWarps);
         }
         *abort_flag = 0;
+        *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if constexpr (MODE == kFisher)
@@ -669,6 +686,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
                 fence_after();
                 ac.next();
+                // (the adapters' slices are the last share's)
+                const bool odd = P.ad.lists && t.q == P.splits - 1 && __any_sync(~0u, *odd_flag);
 #pragma unroll 1
                 for (int c = 0; c < COLS && c < cols; c += 64) {
                     float v[64];
@@ -680,14 +699,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         for (int i = 0; i < 32; ++i) v[32 * h + i] = x[i];
                     }
                     const int left = cols - c;
+                    if (odd) add_odd_terms<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
                     if (P.splits > 1) {
                         store_rows<false>(buf, v, P.part + (t.q * P.M + row0) * P.ldpart + col + c, P.ldpart, rows, left, lane);
                         continue;
                     }
-                    bool odd = false;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) odd |= !(fabsf(v[i]) <= 3.402823466e38f);
-                    if (P.ad.lists && __any_sync(~0u, odd && lane < rows)) mend_results<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
                     store_rows<true>(buf, v, static_cast<bf16*>(P.out) + row0 * P.ldo + col + c, P.ldo, rows, left, lane);
                 }
                 fence_before();
@@ -997,8 +1013,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     const int a = __ldg(u.list + 1 + x / u.rslices), r0 = (x % u.rslices) * 32;
                     if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag)) { ok = false; break; }
                     phase ^= 1u << s;
-                    build_adapter<MODE>(P.ad, a, r0, static_cast<long long>(t.tm) * 256 + rank * 128, t.tn * NB + rank * C::kCols,
-                                        smem + s * C::kStage, smem + s * C::kStage + C::kA, pt);
+                    const bool odd = build_adapter<MODE>(P.ad, a, r0, static_cast<long long>(t.tm) * 256 + rank * 128, t.tn * NB + rank * C::kCols,
+                                                         smem + s * C::kStage, smem + s * C::kStage + C::kA, pt);
+                    if (__any_sync(~0u, odd)) set_pair(odd_flag);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) arrive_even(smem_u32(&ready[s]));
@@ -1035,8 +1052,6 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant_
                 float* h = static_cast<float*>(P.out) + at + e;
                 *h = P.accumulate ? *h + v[e] : v[e];
             } else {
-                if constexpr (Cfg<MODE>::kAdapter)
-                    if (P.ad.lists && !(fabsf(v[e]) <= 3.402823466e38f)) v[e] = lone_result<MODE>(P.ad, row, col + e);
                 if (Cfg<MODE>::kAdapter || P.out_bf16) static_cast<bf16*>(P.out)[at + e] = __float2bfloat16_rn(v[e]);
                 else static_cast<float*>(P.out)[at + e] = v[e];
             }

@@ -25,6 +25,23 @@ int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples,
            float* F, cudaStream_t st);
 int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaStream_t st);
 
+// Two FP32 values as pairs of BF16 parts that add up to them, to 2^-17 of each: hi
+// rounded, or cut off where rounding leaves the range; an infinity has no rest.
+__device__ __forceinline__ void split_pair(float f0, float f1, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f0, f1);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    float r0 = f0 - __uint_as_float(hi << 16), r1 = f1 - __uint_as_float(hi & 0xFFFF0000u);
+    if (fmaxf(fabsf(f0), fabsf(f1)) >= 3.39e38f) {  // (BF16 rounds to an infinity from 3.396e38)
+        constexpr uint32_t kInf = 0x7F80u;
+        if ((hi & 0x7FFFu) == kInf) hi = (hi & 0xFFFF0000u) | __float_as_uint(f0) >> 16;
+        if ((hi >> 16 & 0x7FFFu) == kInf) hi = (hi & 0xFFFFu) | (__float_as_uint(f1) & 0xFFFF0000u);
+        r0 = (hi & 0x7FFFu) == kInf ? 0.0f : f0 - __uint_as_float(hi << 16);
+        r1 = (hi >> 16 & 0x7FFFu) == kInf ? 0.0f : f1 - __uint_as_float(hi & 0xFFFF0000u);
+    }
+    const __nv_bfloat162 l = __floats2bfloat162_rn(r0, r1);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 constexpr int kListTokens = 256;              // tokens of one list of adapters
 constexpr int kListPitch = kListTokens + 1;   // its count, then its adapters
 

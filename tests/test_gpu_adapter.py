@@ -154,6 +154,74 @@ def test_values_of_other_tokens_stay_out(cuda, tblib):
     assert not bool(da[3].any()) and not bool(db[3].any())
 
 
+@pytest.mark.parametrize("n", [20, 60, 150, 700, 1500])
+def test_infinities_of_an_adapter_keep_their_sign(cuda, tblib, n):
+    """An infinity in a row of b or a column of a gives its own tokens' results the infinity that the formula gives,
+    and leaves every other result within its bar.  (A result with two is of their signs or NaN; b and a get one each.)"""
+    torch, tb = cuda, tblib
+    d, r, rank, na = 200, 392, 24, 3
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, "mixed"), 80)
+    want, mag = c.ref.forward(c.x), c.ref.forward(c.x, True)
+    c.b[1 * r + 300, 7] = math.inf
+    c.b[2 * r + 17, 20] = -math.inf
+    tb.check(tb.adapter_forward(c.args(tb)))
+    y = c.y[:n, :r]
+    u = [c.scale[k].double() * (c.x.double() @ c.a[k * rank:(k + 1) * rank].double().t()) for k in range(na)]
+    hit = torch.zeros(n, r, dtype=torch.bool, device="cuda")
+    for k, o, j, sign in ((1, 300, 7, 1), (2, 17, 20, -1)):
+        t = c.ref.tokens(k)
+        hit[t, o] = True
+        assert torch.equal(y[t, o].double(), sign * torch.sign(u[k][t, j]) * math.inf)
+    check(torch, y[~hit], want[~hit], mag[~hit], d + rank)
+    dx, mx = (c.ref.backward(c.dy, c.x.double(), m)[0] for m in (False, True))
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, "mixed"), 80)
+    c.a[1 * rank + 9, 130] = -math.inf
+    tb.check(tb.adapter_backward(c.args(tb, da=None, db=None)))
+    t = c.ref.tokens(1)
+    v = c.dy.double()[t] @ c.b[r:2 * r, 9].double()
+    got = c.dx[:n, :d]
+    assert torch.equal(got[t, 130].double(), -torch.sign(v) * math.inf)
+    hit = torch.zeros(n, d, dtype=torch.bool, device="cuda")
+    hit[t, 130] = True
+    check(torch, got[~hit], dx[~hit], mx[~hit], r + rank)
+
+
+def test_large_values_and_tokens_without_numbers(cuda, tblib):
+    """u and v that round to an infinity in BF16 but are none count as what they are; tokens that are all NaN, and an
+    adapter that is, cost no more time than others: the products' bounded waits do not run out."""
+    torch, tb = cuda, tblib
+    c = Case(torch, 200, 64, 72, 8, 2, who_of(torch, 200, 2, "one"), 85)
+    c.w.zero_()
+    c.a.zero_()
+    c.b.zero_()
+    c.scale.fill_(1.0)
+    c.a[0, :2] = torch.tensor([1.0, 2.0 ** -8], device="cuda", dtype=torch.bfloat16)
+    c.x.zero_()
+    c.x[:, :2] = torch.finfo(torch.bfloat16).max  # u = max (1 + 2^-8), still an FP32 value
+    c.b[:72, 0] = 2.0 ** -10
+    tb.check(tb.adapter_forward(c.args(tb)))
+    u = torch.finfo(torch.bfloat16).max * (1 + 2.0 ** -8)
+    assert u < torch.finfo(torch.float32).max
+    assert float((c.y[:200, :72].double() / (u * 2.0 ** -10) - 1).abs().max()) <= 2.0 ** -8 + 2.0 ** -16
+    n, d, r = 4000, 2048, 2048
+    c = Case(torch, n, d, r, 16, 3, who_of(torch, n, 3, "mixed"), 86)
+    want, mag = c.ref.forward(c.x), c.ref.forward(c.x, True)
+    c.b[r:2 * r] = math.nan
+    tb.check(tb.adapter_forward(c.args(tb)))
+    tb.check(tb.lib().tb_gemm_status(None))
+    own = c.who == 1
+    y = c.y[:n, :r]
+    assert bool(torch.isnan(y[own]).all())
+    check(torch, y[~own], want[~own], mag[~own], d + 16)
+    c.x.fill_(math.nan)
+    ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    ev[0].record()
+    tb.check(tb.adapter_forward(c.args(tb)))
+    ev[1].record()
+    tb.check(tb.lib().tb_gemm_status(None))
+    assert bool(torch.isnan(y).all()) and ev[0].elapsed_time(ev[1]) < 1000.0
+
+
 def test_outputs_may_be_left_out(cuda, tblib):
     torch, tb = cuda, tblib
     c = Case(torch, 40, 64, 72, 8, 2, who_of(torch, 40, 2, "runs"), 40)
