@@ -211,7 +211,8 @@ int tb_gemm_nt_bf16(const void* a, long long lda, const void* b, long long ldb, 
                     float alpha, float beta, const float* c_in, long long ldcin, float* c, long long ldc,
                     int lower_only, void* stream);
 /* TB_ERR_TIMEOUT if a bounded pipeline wait inside a GEMM, or inside a product
- * of the checkpoint and adapter entries below, launched since the last call expired (the kernel then skipped its output); synchronises. */
+ * of the checkpoint and adapter entries below, launched since the last call
+ * expired (the kernel then skipped its output); synchronises. */
 int tb_gemm_status(void* stream);
 
 /* ---- stage 3: column-block exact OBS against calibration activations ----- */
@@ -298,7 +299,9 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * no sample are not read into any.  Sums are in FP32 and every product is
  * exact: FP32 (F16) dy is split into three (two) BF16 parts, in scratch of
  * 6 (4) bytes per value from the library's per-device pool; rows of a BF16 dy
- * that are not 16-byte aligned are first copied to such scratch. */
+ * that are not 16-byte aligned are first copied to such scratch.  Where the
+ * gradients have few 256 x 256 tiles, shares of their sums also wait there, at
+ * most 74 tiles of FP32. */
 int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
                         const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride, void* stream);
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
@@ -317,7 +320,10 @@ int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy
  * or below the diagonal are written.  n = 0 gives zeros (accumulate: H stays).
  * Within a block of 128 tokens the codes' products add up exactly in integers;
  * the blocks' sums are added in FP32.  A feature with values beyond 2^100,
- * whose diagonal overflows in any case, gives infinities or NaN in its row. */
+ * whose diagonal overflows in any case, gives infinities or NaN in its row.
+ * Added to H, a sum below FP32's smallest normal value counts as zero.  Scratch
+ * where H has few 256 x 256 tiles, or rows (d not a multiple of 4) or an address
+ * that are not 16-byte aligned: FP32 shares of H, at most 74 tiles or one H. */
 int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, void* stream);
 
 /* ---- low-rank adapters beside a shared projection ------------------------- */
@@ -359,13 +365,19 @@ typedef struct tb_adapter_args {
 /* y_t = W x_t + scale[a] B_a (A_a x_t).  All inputs 16-byte aligned with row
  * strides that are multiples of 8; outputs may have any stride.  Columns
  * behind the last one (d..lda-1 and so on) are neither used nor written.
- * Scratch: 4 bytes per token and rank, from the library's per-device pool. */
+ * An infinity or a NaN in a token or an adapter reaches that token's, or that
+ * adapter's tokens', results alone.  Scratch from the library's per-device pool:
+ * 4 bytes per token and rank and 8 per token, and, where y has few 256 x 256
+ * tiles, shares of their sums, at most 74 tiles of FP32. */
 int tb_adapter_forward(const tb_adapter_args* args, void* stream);
 /* With v_t = scale[a] B_a^T dy_t and u_t = scale[a] A_a xhat_t:
  *     dx_t = W^T dy_t + A_a^T v_t,   da_a = sum v_t xhat_t^T,   db_a = sum dy_t u_t^T
  * over the tokens of adapter a (zero where it has none).  da and db do not
  * depend on the order in which blocks run: their sums have a fixed order.
- * With dx NULL, w may be NULL; with da and db NULL, x8 may be NULL. */
+ * With dx NULL, w may be NULL; with da and db NULL, x8 may be NULL.  Scratch:
+ * as the forward's, twice the bytes per token and rank, and FP32 shares of da
+ * and db where batches are long and these are small (at most 600 blocks of 128
+ * features by 32 ranks). */
 int tb_adapter_backward(const tb_adapter_args* args, void* stream);
 
 /* ---- fused score -> mask -> pack pass ------------------------------------ */

@@ -10,7 +10,7 @@ three and two times the additions.  A BF16 result adds half a step, 2^-8 of the
 value.  Beside that bound, which grows with n, the 2-norm error of FP32 results
 stays below 2e-6: rounding errors of n terms add like sqrt(n), and both sides
 of the ratio do, so it is a few times 2^-24 times the depth of one partial sum
-(16 tensor-core steps) whatever n."""
+(32 tensor-core steps) whatever n."""
 import math
 
 import pytest
@@ -403,3 +403,34 @@ def test_calibration_end_to_end(cuda, tblib):
     mask = torch.empty(r * d // 4, device="cuda", dtype=torch.uint8)
     tb.check(tb.lib().tb_obs_sparsegpt(W.data_ptr(), r, d, H.data_ptr(), 0.01, 2, 4, mask.data_ptr(), None, None))
     assert float((W == 0).float().mean()) == 0.5
+
+
+def test_corners_of_the_state(cuda, tblib):
+    """No tokens added to H leave it, subnormals too; a first step does not read F, whatever beta's powers."""
+    torch, tb = cuda, tblib
+    H = torch.full((40, 40), 1e-40, device="cuda")
+    H[3, 4] = math.nan
+    before = H.clone()
+    ck = packed(torch, tb, rows(torch, 4, 40, torch.float32, 0))
+    ck.s.n = 0
+    tb.check(tb.act8_hessian(ck.s, 1.0, H.data_ptr(), accumulate=True))
+    torch.cuda.synchronize()
+    assert torch.equal(H.view(torch.int32), before.view(torch.int32))
+    ck = packed(torch, tb, rows(torch, 150, 24, torch.float32, 1))
+    dy = rows(torch, 150, 16, torch.bfloat16, 2, 16, 1e-3)
+    sp = torch.tensor([[i, i + 1] for i in range(150)], device="cuda")
+    for beta in (0.0, 2.0):
+        F = torch.full((16, 24), math.nan, device="cuda")
+        S = 150 if beta == 0.0 else 128  # (beta^S alone is beyond FP32)
+        tb.check(tb.act8_fisher(ck.s, dy.data_ptr(), tb.BF16, 16, 16, sp.data_ptr(), S, F.data_ptr(), alpha=0.5, beta=beta))
+        want = torch.zeros(16, 24, device="cuda", dtype=torch.float64)
+        xh = ck.values(torch)
+        for s in range(S):
+            g = torch.outer(dy[s].double(), xh[s])
+            want = 0.5 * g * g if s == 0 else beta * want + 0.5 * (1 - beta) * g * g
+        # terms of both signs (1 - beta = -1): S additions and a few roundings of each term, of their magnitudes
+        mag = torch.zeros_like(want)
+        for s in range(S):
+            g = torch.outer(dy[s].double(), xh[s])
+            mag = 0.5 * g * g if s == 0 else beta * mag + 0.5 * abs(1 - beta) * g * g
+        assert bool(((F.double() - want).abs() <= (S + 8) * 2.0 ** -23 * mag + 1e-38).all())
