@@ -28,6 +28,7 @@
 //            (zero for the others) times [E | E]
 // Every wait is bounded; on expiry the kernel records an error and leaves.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "tb_device.cuh"
@@ -97,14 +98,15 @@ struct Params {
     long long ldo, out_stride;
     int out_bf16, out_tma;
     double alpha, beta;
-    float scale;
+    float scale, decay;  // decay: beta^S
     int first, accumulate;
     AdapterProduct ad;
-    // with splits > 1 the K range of a unit is shared out; where `part` is given, FP32 sums go there, [splits][samples * M][ldpart]
-    int splits;
+    // The first `whole` units are items of their own; each of the `tail` units behind them is `splits` items,
+    // shares of its K (kFisher: of its samples), whose sums go to `part`, [splits][tail][256][256] FP32.
+    int whole, tail, splits;
     float* part;
-    long long ldpart;
 };
+constexpr int kPartTile = 256 * 256;
 
 // Waits for the barrier phase `parity`, at most about two seconds of SM cycles.
 __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
@@ -222,7 +224,9 @@ constexpr int kDirect = 16;
 // ---- the walk over work items, units (one sum each) and K slices that every role shares ----
 struct Tile {
     int tm, tn;
-    int s, q;           // sample; share of K
+    int s;              // sample
+    int q, splits;      // share
+    int slot;           // its place in `part`, or -1
 };
 struct Unit {
     int lo, hi;         // K range (samples: lo rounded down to a whole slice,
@@ -237,25 +241,23 @@ struct Unit {
 
 template <int MODE>
 __device__ __forceinline__ Tile tile_of(const Params& P, int item) {
-    Tile t{0, 0, 0, 0};
+    Tile t{0, 0, 0, 0, 1, -1};
+    int unit = item;
+    if (item >= P.whole) {
+        t.slot = item - P.whole;
+        t.q = t.slot / P.tail;
+        t.splits = P.splits;
+        unit = P.whole + t.slot % P.tail;
+    }
     if constexpr (MODE == kHess) {  // tiles on or below the diagonal, row by row
-        const int tiles = P.tiles_m * (P.tiles_m + 1) / 2;
-        t.q = item / tiles;
-        const int i = item % tiles;
-        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(i) + 1.0f) - 1.0f) * 0.5f);
-        while (tm * (tm + 1) / 2 > i) --tm;
-        while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
+        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(unit) + 1.0f) - 1.0f) * 0.5f);
+        while (tm * (tm + 1) / 2 > unit) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= unit) ++tm;
         t.tm = tm;
-        t.tn = i - tm * (tm + 1) / 2;
+        t.tn = unit - tm * (tm + 1) / 2;
     } else {
-        const int tiles = P.tiles_m * P.tiles_n;
-        if constexpr (MODE == kGrad) {
-            t.s = item / tiles % P.S;
-            t.q = item / tiles / P.S;
-        } else if constexpr (MODE != kFisher) {
-            t.q = item / tiles;
-        }
-        const int i = item % tiles;
+        const int tiles = P.tiles_m * P.tiles_n, i = MODE == kGrad ? unit % tiles : unit;
+        if constexpr (MODE == kGrad) t.s = unit / tiles;
         // bands of 8 tile rows, column by column inside, so that concurrent tiles share operands in L2
         const int band = i / (8 * P.tiles_n), in = i % (8 * P.tiles_n);
         const int rows = min(8, P.tiles_m - 8 * band);
@@ -283,20 +285,20 @@ __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
         u.slices = u.hi > u.begin ? (u.hi - u.lo + 63) / 64 : 0;
         u.total = u.slices * P.parts;
         if (MODE == kFisher && u.total <= kDirect) u.group = kDirect;
-        if (MODE != kFisher && P.splits > 1) {
-            u.first = share_begin(u.slices * P.parts, t.q, P.splits);
-            u.total = share_begin(u.slices * P.parts, t.q + 1, P.splits) - u.first;
+        if (MODE != kFisher && t.splits > 1) {
+            u.first = share_begin(u.slices * P.parts, t.q, t.splits);
+            u.total = share_begin(u.slices * P.parts, t.q + 1, t.splits) - u.first;
         }
     } else {  // a share begins at its own `lo`
         constexpr int kStep = MODE == kHess ? 128 : 64;
         u.total = u.slices = ((MODE == kHess ? P.n : P.K) + kStep - 1) / kStep;
-        if (P.splits > 1) {
-            const int all = u.slices, first = share_begin(all, t.q, P.splits);
+        if (t.splits > 1) {
+            const int all = u.slices, first = share_begin(all, t.q, t.splits);
             u.lo = first * kStep;
-            u.total = u.slices = share_begin(all, t.q + 1, P.splits) - first;
+            u.total = u.slices = share_begin(all, t.q + 1, t.splits) - first;
         }
         if constexpr (Cfg<MODE>::kAdapter) {
-            if (P.ad.lists && t.q == P.splits - 1) {
+            if (P.ad.lists && t.q == t.splits - 1) {
                 u.list = P.ad.lists + static_cast<long long>(t.tm) * kListPitch;
                 u.rslices = (P.ad.rank + 31) / 32;
                 u.extra = __ldg(u.list) * u.rslices;
@@ -325,7 +327,7 @@ __device__ __forceinline__ bool for_units(const Params& P, F&& f) {
     for (int item = blockIdx.x >> 1; item < P.items; item += gridDim.x >> 1) {
         const Tile t = tile_of<MODE>(P, item);
         if constexpr (MODE == kFisher) {
-            for (int s = 0; s < P.S; ++s)
+            for (int s = share_begin(P.S, t.q, t.splits), end = share_begin(P.S, t.q + 1, t.splits); s < end; ++s)
                 if (!f(t, unit_of<MODE>(P, t, s))) return false;
         } else {
             if (!f(t, unit_of<MODE>(P, t, t.s))) return false;
@@ -614,7 +616,7 @@ template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CUtensorMap tB,
               const __grid_constant__ CUtensorMap tE, const __grid_constant__ CUtensorMap tO,
-              const __grid_constant__ Params P) {
+              const __grid_constant__ CUtensorMap tP, const __grid_constant__ Params P) {
     using C = Cfg<MODE>;
     constexpr int NB = C::NB, kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -687,7 +689,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 fence_after();
                 ac.next();
                 // (the adapters' slices are the last share's)
-                const bool odd = P.ad.lists && t.q == P.splits - 1 && __any_sync(~0u, *odd_flag);
+                const bool odd = P.ad.lists && t.q == t.splits - 1 && __any_sync(~0u, *odd_flag);
 #pragma unroll 1
                 for (int c = 0; c < COLS && c < cols; c += 64) {
                     float v[64];
@@ -700,8 +702,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     }
                     const int left = cols - c;
                     if (odd) add_odd_terms<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
-                    if (P.splits > 1) {
-                        store_rows<false>(buf, v, P.part + (t.q * P.M + row0) * P.ldpart + col + c, P.ldpart, rows, left, lane);
+                    if (t.slot >= 0) {
+                        store_rows<false>(buf, v, P.part + static_cast<long long>(t.slot) * kPartTile + row_in * 256 + half * COLS + c, 256, rows, left, lane);
                         continue;
                     }
                     store_rows<true>(buf, v, static_cast<bf16*>(P.out) + row0 * P.ldo + col + c, P.ldo, rows, left, lane);
@@ -710,25 +712,28 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&accempty[b]));
             } else if constexpr (MODE == kFisher) {
-                float* out = static_cast<float*>(P.out) + row0 * P.ldo + col;
+                // A share is a state of its own, begun at 0.
+                float* out = t.slot < 0 ? static_cast<float*>(P.out) + row0 * P.ldo + col
+                                        : P.part + static_cast<long long>(t.slot) * kPartTile + row_in * 256 + half * COLS;
+                const int ld = t.slot < 0 ? static_cast<int>(P.ldo) : 256;
                 float F[COLS];
-                if (P.first) {
+                if (P.first || t.slot >= 0) {
 #pragma unroll
                     for (int i = 0; i < COLS; ++i) F[i] = 0.0f;
                 } else {
-                    const float decay = static_cast<float>(pow(P.beta, static_cast<double>(P.S)));  // of the state before
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) load_piece(buf, F + 32 * c, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
+                    for (int c = 0; c < COLS / 32; ++c) load_piece(buf, F + 32 * c, out + 32 * c, ld, rows, cols - 32 * c, lane);
 #pragma unroll
-                    for (int i = 0; i < COLS; ++i) F[i] *= decay;
+                    for (int i = 0; i < COLS; ++i) F[i] *= P.decay;
                 }
-                for (int s = 0; s < P.S && ok; ++s) {
+                const int s_end = share_begin(P.S, t.q + 1, t.splits);
+                for (int s = share_begin(P.S, t.q, t.splits); s < s_end && ok; ++s) {
                     const Unit u = unit_of<MODE>(P, t, s);
                     if (u.total == 0) continue;  // no tokens: g = 0
                     const float factor = s < C::kFactors ? factors[s] : fisher_factor(P, s);
                     const uint64_t factor2 = pack2(factor, factor);
                     if (u.total > kDirect) {
-                        store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
+                        store_rows<false>(buf, F, out, ld, rows, cols, lane);
 #pragma unroll
                         for (int i = 0; i < COLS; ++i) F[i] = 0.0f;
                         for (int left = u.total; left > 0 && ok; left -= u.group) {
@@ -743,7 +748,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
 #pragma unroll
                         for (int c = 0; c < COLS / 32; ++c) {
                             float old[32];
-                            load_piece(buf, old, out + 32 * c, P.ldo, rows, cols - 32 * c, lane);
+                            load_piece(buf, old, out + 32 * c, ld, rows, cols - 32 * c, lane);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 square_add2(old[i], old[i + 1], factor2, F[32 * c + i], F[32 * c + i + 1]);
@@ -762,7 +767,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         });
                     }
                 }
-                if (ok) store_rows<false>(buf, F, out, P.ldo, rows, cols, lane);
+                if (ok) {
+                    store_rows<false>(buf, F, out, ld, rows, cols, lane);
+                }
             } else {
                 {
                     const int s = t.s;
@@ -828,11 +835,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         }
                         // kHess: only 128 x 128 tiles on or below the diagonal
                         const bool wanted = rows > 0 && cols > 0 && (MODE == kGrad || col / 128 <= row0 / 128);
-                        const int z = P.part ? t.q * max(1, P.S) + t.s : t.s;
-                        if (MODE == kHess || P.out_tma) {
+                        if (t.slot >= 0) {
+                            if (wanted) store_tma<false, C::kPieces>(&tP, buf, acc, half * COLS, row_in, t.slot, 256, false, lane);
+                        } else if (MODE == kHess || P.out_tma) {
                             if (!wanted) continue;
-                            if (MODE == kGrad && P.out_bf16 && !P.part) store_tma<true, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), z, static_cast<int>(P.N), false, lane);
-                            else store_tma<false, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), z, static_cast<int>(P.N), MODE == kHess && P.accumulate && !P.part, lane);
+                            if (MODE == kGrad && P.out_bf16) store_tma<true, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), false, lane);
+                            else store_tma<false, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), MODE == kHess && P.accumulate, lane);
                         } else if constexpr (MODE == kGrad) {
                             const long long at = t.s * P.out_stride + row0 * P.ldo + col;
                             if (P.out_bf16) store_rows<true>(buf, acc, static_cast<bf16*>(P.out) + at, P.ldo, rows, cols, lane);
@@ -1032,30 +1040,30 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     }
 }
 
-// Joins the shares of K in order: four consecutive columns per thread.
+// Joins the shares of the units behind the whole ones, in order: four consecutive columns per thread.
 template <int MODE>
-__global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant__ Params P) {
-    const long long quads = (P.N + 3) / 4, rows = P.M * max(1, P.S);
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * quads; i += gridDim.x * 256ll) {
-        const long long row = i / quads, col = i % quads * 4;
-        if (MODE == kHess && col / 128 > row / 128) continue;
-        float v[4] = {};
-        for (int q = 0; q < P.splits; ++q) {
-            const float4 f = *reinterpret_cast<const float4*>(P.part + (q * rows + row) * P.ldpart + col);
-            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-        }
-        const long long at = MODE == kGrad ? row / P.M * P.out_stride + row % P.M * P.ldo + col : row * P.ldo + col;
+__global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant__ Params P, const int from) {
+    const int unit = from + blockIdx.y;
+    const Tile t = tile_of<MODE>(P, P.whole + unit);
+    const int at_tile = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const long long row = t.tm * 256ll + at_tile / 256, col = t.tn * 256ll + at_tile % 256;
+    if (row >= P.M || col >= P.N || (MODE == kHess && col / 128 > row / 128)) return;
+    const float* part = P.part + static_cast<long long>(unit) * kPartTile + at_tile;
+    float v[4] = {};
+#pragma unroll 4
+    for (int q = 0; q < P.splits; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(part + static_cast<long long>(q) * P.tail * kPartTile);
+        v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+    }
+    const long long at = (MODE == kGrad ? t.s * P.out_stride : 0) + row * P.ldo + col;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (col + e >= P.N) break;
-            if constexpr (MODE == kHess) {
-                float* h = static_cast<float*>(P.out) + at + e;
-                *h = P.accumulate ? *h + v[e] : v[e];
-            } else {
-                if (Cfg<MODE>::kAdapter || P.out_bf16) static_cast<bf16*>(P.out)[at + e] = __float2bfloat16_rn(v[e]);
-                else static_cast<float*>(P.out)[at + e] = v[e];
-            }
-        }
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= P.N) break;
+        float* to = static_cast<float*>(P.out) + at + e;
+        if constexpr (MODE == kHess) *to = P.accumulate ? *to + v[e] : v[e];
+        else if constexpr (MODE == kFisher) *to = P.first ? v[e] : fmaf(P.decay, *to, v[e]);
+        else if (Cfg<MODE>::kAdapter || P.out_bf16) static_cast<bf16*>(P.out)[at + e] = __float2bfloat16_rn(v[e]);
+        else *to = v[e];
     }
 }
 
@@ -1078,7 +1086,7 @@ int make_map(CUtensorMap* map, const void* base, int esize, long long cols, long
 constexpr long long kPairs = 74;  // one CTA on each of the 148 SMs
 
 template <int MODE>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, const Params& P, cudaStream_t st) {
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, const CUtensorMap& o, const CUtensorMap& part, const Params& P, cudaStream_t st) {
     using C = Cfg<MODE>;
     // Per device: the shared-memory limit, and that the launch has the registers that the roles' shares add up to.
     static std::mutex mu;
@@ -1100,7 +1108,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, con
         }
     }
     const int pairs = static_cast<int>(std::min<long long>(P.items, kPairs));
-    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, o, P);
+    linear_kernel<MODE><<<2 * pairs, kThreads, C::kSmem, st>>>(a, b, e, o, part, P);
     return check_launch("linear_kernel");
 }
 
@@ -1118,37 +1126,46 @@ int make_out_map(CUtensorMap* map, void* base, bool bf16_out, long long cols, lo
     return e == CUDA_SUCCESS ? TB_OK : fail(TB_ERR_ARG, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(e));
 }
 
-// launch() of `units` sums of about `slices` K slices each.  Fewer than half as
-// many as pairs of SMs: their K is shared out, at least 8 slices a share, so that
-// all pairs work, and joined by a second kernel.  (64 tokens' forward, 4096 x
-// 4096: 33.6 us with one share, 19.3 with four and the join.)  The Hessian takes
-// that way too where its rows do not start on 16 bytes, as TMA wants them.
+// launch() of `units` sums of about `slices` K slices each, in waves of one a pair
+// of SMs.  The units of a last wave that is not full, or of an only one, are
+// shared out where that is sooner: s shares of at most `shares` parts, two waves
+// of them at most, s chosen for the fewest slices one after another, the second
+// kernel that joins them counted as ten and an eighth for each share's tile (a
+// slice takes 0.25 us, the join 2.5).  (64 tokens' forward, 4096 x 4096, 16
+// units: 33.6 us with one share, 19.3 with four.)  The Hessian goes by way of
+// `part` too where its rows do not start on 16 bytes, as TMA wants them.
 template <int MODE>
 int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, Params& P, long long units, long long slices,
-                  const char* who, cudaStream_t st) {
+                  long long shares, const char* who, cudaStream_t st) {
     constexpr bool kTma = MODE == kGrad || MODE == kHess;
-    const long long samples = std::max(1, P.S), rows = P.M * samples;
-    P.splits = MODE == kFisher ? 1 : static_cast<int>(std::max(1ll, std::min(kPairs / std::max(1ll, units), slices / 8)));
-    if (units * P.splits > 0x7FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, units);
-    P.items = static_cast<int>(units * P.splits);
-    P.ldpart = (P.N + 7) / 8 * 8;
+    if (units > 0x3FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, units);
     const int esize = P.out_bf16 ? 2 : 4;
     P.out_tma = kTma && reinterpret_cast<uintptr_t>(P.out) % 16 == 0 && P.ldo * esize % 16 == 0 && P.out_stride * esize % 16 == 0;
-    CUtensorMap o{};
-    if (P.splits == 1 && (MODE != kHess || P.out_tma)) {
-        const int rc = P.out_tma ? make_out_map(&o, P.out, P.out_bf16, P.N, P.M, samples, P.ldo, P.out_stride) : TB_OK;
-        return rc ? rc : launch<MODE>(a, b, e, o, P, st);
+    const long long tail = units % kPairs;
+    long long best = slices, splits = 1;
+    for (long long s = 2; tail && s <= shares && tail * s <= 2 * kPairs; ++s) {
+        const long long cost = (tail * s + kPairs - 1) / kPairs * ((slices + s - 1) / s) + 10 + tail * s / 8;
+        if (cost < best) best = cost, splits = s;
     }
+    P.tail = static_cast<int>(MODE == kHess && !P.out_tma ? units : splits > 1 ? tail : 0);
+    P.splits = static_cast<int>(P.tail == tail ? splits : 1);
+    P.whole = static_cast<int>(units - P.tail);
+    P.items = P.whole + P.tail * P.splits;
+    CUtensorMap o{}, parts{};
+    if (P.out_tma && P.whole) {
+        const int rc = make_out_map(&o, P.out, P.out_bf16, P.N, P.M, std::max(1, P.S), P.ldo, P.out_stride);
+        if (rc) return rc;
+    }
+    if (!P.tail) return launch<MODE>(a, b, e, o, parts, P, st);
     void* part = nullptr;
-    int rc = scratch_alloc(&part, sizeof(float) * P.splits * rows * P.ldpart, st);
+    const long long slots = static_cast<long long>(P.tail) * P.splits;
+    int rc = scratch_alloc(&part, sizeof(float) * slots * kPartTile, st);
     if (rc) return rc;
     P.part = static_cast<float*>(part);
-    P.out_tma = kTma;
-    if (kTma) rc = make_out_map(&o, part, false, P.N, P.M, samples * P.splits, P.ldpart, P.M * P.ldpart);
-    if (!rc) rc = launch<MODE>(a, b, e, o, P, st);
-    if (!rc) {
-        const long long quads = rows * ((P.N + 3) / 4);
-        join_splits_kernel<MODE><<<static_cast<unsigned>(std::min((quads + 255) / 256, 148ll * 8)), 256, 0, st>>>(P);
+    if (kTma) rc = make_out_map(&parts, part, false, 256, 256, slots, 256, kPartTile);
+    if (!rc) rc = launch<MODE>(a, b, e, o, parts, P, st);
+    for (int u = 0; !rc && u < P.tail; u += 65535) {  // (a grid's y extent)
+        join_splits_kernel<MODE><<<dim3(64, std::min(P.tail - u, 65535)), 256, 0, st>>>(P, u);
         rc = check_launch("join_splits_kernel");
     }
     scratch_free(part, st);
@@ -1176,8 +1193,9 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
     if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 1, false);
     const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
-    // (the samples' lengths are on the device: an even split)
-    return rc ? rc : launch_shared<MODE>(a, b, e, P, units, ck.n / samples * dy.parts / 64, who, st);
+    // (The samples' lengths are on the device: as if they were even.)  A unit of the Fisher mode has all samples.
+    const long long each = (ck.n / std::max(1, P.S) + 63) / 64 * dy.parts, slices = MODE == kFisher ? P.S * each : each;
+    return rc ? rc : launch_shared<MODE>(a, b, e, P, units, slices, MODE == kFisher ? P.S : slices, who, st);
 }
 
 }  // namespace
@@ -1202,6 +1220,7 @@ int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples,
     P.alpha = alpha;
     P.beta = beta;
     P.first = first;
+    P.decay = static_cast<float>(pow(beta, static_cast<double>(S)));
     return from_codes<kFisher>(ck, dy, r, P, 1, "tb_act8_fisher", st);
 }
 
@@ -1223,7 +1242,7 @@ int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaSt
     if (ck.n > 0) rc = make_map(&a, ck.codes, 1, ck.d, ck.n, ck.ldq, 128, 128, true);
     P.out_stride = static_cast<long long>(ck.d) * ck.d;
     const long long units = static_cast<long long>(P.tiles_m) * (P.tiles_m + 1) / 2;
-    return rc ? rc : launch_shared<kHess>(a, a, a, P, units, (ck.n + 127) / 128, "tb_act8_hessian", st);
+    return rc ? rc : launch_shared<kHess>(a, a, a, P, units, (ck.n + 127) / 128, (ck.n + 127) / 128, "tb_act8_hessian", st);
 }
 
 template <int MODE>
@@ -1243,7 +1262,7 @@ static int adapter_product(const AdapterProduct& p, const char* who, cudaStream_
     if (!rc) rc = make_map(&a, p.in, 2, p.K, p.n, p.ldin, 64, 128, true);
     if (!rc) rc = MODE == kFwd ? make_map(&b, p.w, 2, p.K, p.N, p.ldw, 64, 128, true)
                                : make_map(&b, p.w, 2, p.N, p.K, p.ldw, 64, 64, true);
-    if (!rc) rc = launch_shared<MODE>(a, b, b, P, static_cast<long long>(P.tiles_m) * P.tiles_n, (p.K + 63) / 64, who, st);
+    if (!rc) rc = launch_shared<MODE>(a, b, b, P, static_cast<long long>(P.tiles_m) * P.tiles_n, (p.K + 63) / 64, (p.K + 63) / 64, who, st);
     return rc;
 }
 

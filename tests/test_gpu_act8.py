@@ -434,3 +434,57 @@ def test_corners_of_the_state(cuda, tblib):
             g = torch.outer(dy[s].double(), xh[s])
             mag = 0.5 * g * g if s == 0 else beta * mag + 0.5 * abs(1 - beta) * g * g
         assert bool(((F.double() - want).abs() <= (S + 8) * 2.0 ** -23 * mag + 1e-38).all())
+
+
+@pytest.mark.parametrize("n,r,d,S,first", [(40, 60, 52, 8, True), (700, 264, 300, 5, False), (3000, 200, 136, 2, False),
+                                           (900, 2600, 2600, 6, True), (1500, 2600, 2304, 3, False)])
+def test_fisher_of_few_tiles_and_of_last_waves(cuda, tblib, n, r, d, S, first):
+    """Tiles whose samples are shared out (all of few, the last ones of 110 or 90), long samples among them."""
+    torch, tb = cuda, tblib
+    ck = packed(torch, tb, rows(torch, n, d, torch.float32, 7))
+    dy = rows(torch, n, r, torch.bfloat16, 8, ref.up(r, 8), 0.1)
+    cuts = [0] + [n * (i + 1) * (i + 2) // (S * (S + 1)) for i in range(S)]
+    sp = torch.tensor([[a, b] for a, b in zip(cuts, cuts[1:])], device="cuda")
+    F = torch.rand(r, d, device="cuda")
+    old = F.double()
+    tb.check(tb.act8_fisher(ck.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), S, F.data_ptr(), first_step=first))
+    again = old.float()
+    tb.check(tb.act8_fisher(ck.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), S, again.data_ptr(), first_step=first))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    xh = ck.values(torch)
+    want, bar = (None, torch.zeros_like(old)) if first else (old, old * 0.0)
+    for a, b in sp.tolist():
+        g, m = dy[a:b].double().t() @ xh[a:b], dy[a:b].double().abs().t() @ xh[a:b].abs()
+        e = (b - a) * 2.0 ** -23 * m
+        w = 0.01 if want is None else 0.01 * 0.01
+        bar = 0.99 * bar + w * (2 * m * e + e * e)
+        want = 0.01 * g * g if want is None else 0.99 * want + w * g * g
+    bar = bar + (2 * S + 6) * 2.0 ** -23 * want  # the state's own multiplications and additions, at most
+    assert bool(((F.double() - want).abs() <= bar * 1.01 + 1e-40).all())
+    assert float((F.double() - want).norm() / want.norm()) <= 2e-6
+    assert torch.equal(F, again)
+
+
+@pytest.mark.parametrize("n,r,d,S", [(2100, 2600, 2600, 1), (1100, 500, 1300, 9)])
+@pytest.mark.parametrize("g_t", ["float32", "bfloat16"])
+def test_gradients_of_last_waves(cuda, tblib, n, r, d, S, g_t):
+    """121 and 108 units: those behind the first wave have their K shared out, rows on 16 bytes or not."""
+    torch, tb = cuda, tblib
+    ck = packed(torch, tb, rows(torch, n, d, torch.float32, 9))
+    dy = rows(torch, n, r, torch.bfloat16, 10, ref.up(r, 8), 0.1)
+    sp = torch.tensor([[n * i // S, n * (i + 1) // S] for i in range(S)], device="cuda")
+    dt = getattr(torch, g_t)
+    for pad in (0, 1):
+        G = torch.full((S, r * d + pad), 3.0, device="cuda", dtype=dt)
+        tb.check(tb.act8_weight_grad(ck.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), S, G.data_ptr(), code(tb, torch, dt),
+                                     g_stride=r * d + pad))
+        torch.cuda.synchronize()
+        tb.check(tb.lib().tb_gemm_status(None))
+        xh = ck.values(torch)
+        for s, (a, b) in enumerate(sp.tolist()):
+            g, m = dy[a:b].double().t() @ xh[a:b], dy[a:b].double().abs().t() @ xh[a:b].abs()
+            half = 2.0 ** -8 if g_t == "bfloat16" else 0.0
+            got = G[s, :r * d].view(r, d).double()
+            assert bool(((got - g).abs() <= half * g.abs() + (b - a) * 2.0 ** -23 * 1.01 * m + 1e-40).all())
+        assert pad == 0 or bool((G[:, r * d] == 3).all())
