@@ -556,9 +556,10 @@ __global__ void __launch_bounds__(256) join_kernel(const Args g, const Order o, 
 // 512 consecutive bytes of each row at a time, and join their sums in order.
 // Launched while down_small_kernel still runs: u is not read before the wait, while
 // x and w, which no kernel here writes, are.
+constexpr int kMaxRank = 128;
 template <int NT>
 __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const float* u) {
-    __shared__ float red[8][16][8 * NT + 1];
+    __shared__ float red[8][16][8 * NT + 1], su[8 * NT * kMaxRank];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
     const int o0 = blockIdx.x * 16, groups = (g.d + 31) / 32;
     const bf16 *w0 = g.w + (o0 + gq) * g.ldw, *w1 = w0 + 8 * g.ldw;
@@ -590,8 +591,10 @@ __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const flo
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) red[warp][gq + 8 * (e >> 1)][8 * i + 2 * tq + (e & 1)] = acc[i][e];
-    __syncthreads();
     pdl_wait();
+    // (Read from memory for each output, 19 tokens at rank 128 took 48 us, 10163 features, and 28 so.)
+    for (int i = threadIdx.x; i < g.n * g.rank; i += 256) su[i] = __ldcg(u + i);
+    __syncthreads();
     for (int i = threadIdx.x; i < 16 * 8 * NT; i += 256) {
         const int row = i & 15, t = i >> 4, o = o0 + row;
         if (t >= g.n || o >= g.r) continue;
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const flo
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (k + j < g.rank)
-                        y = fmaf(__ldcg(u + t * g.rank + k + j), __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16), y);
+                        y = fmaf(su[t * g.rank + k + j], __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16), y);
             }
         }
         g.y[t * g.ldy + o] = __float2bfloat16_rn(y);
@@ -714,7 +717,7 @@ int check_common(const char* who, const tb_adapter_args* p, bool need_w, Args* g
     if (p->n_adapters < 0 || p->n_adapters > 65535) return fail(TB_ERR_ARG, "%s: %d adapters", who, p->n_adapters);
     if (need_w && bad_rows(p->w, p->ldw, p->d)) return fail(TB_ERR_ARG, "%s: w must be 16-byte aligned, ldw >= d a multiple of 8", who);
     if (p->n_adapters) {
-        if (p->rank < 1 || p->rank > 128) return fail(TB_ERR_SHAPE, "%s: rank %d outside 1..128", who, p->rank);
+        if (p->rank < 1 || p->rank > kMaxRank) return fail(TB_ERR_SHAPE, "%s: rank %d outside 1..%d", who, p->rank, kMaxRank);
         if (bad_rows(p->a, p->lda, p->d) || bad_rows(p->b, p->ldb, p->rank))
             return fail(TB_ERR_ARG, "%s: a and b must be 16-byte aligned with row strides that are multiples of 8", who);
         if (!p->scale || (p->n > 0 && !p->token_adapter)) return fail(TB_ERR_ARG, "%s: null scale or token_adapter", who);
