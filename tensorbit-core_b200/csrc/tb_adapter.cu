@@ -1,6 +1,7 @@
 // Low-rank adapters of many requests beside a shared projection: forward and
 // backward (contract in include/tb_kernels.h).
 #include <algorithm>
+#include <atomic>
 
 #include "tb_act8.cuh"
 #include "tb_linear.cuh"
@@ -399,14 +400,25 @@ __device__ __forceinline__ long long grad_at(const Args& g, int a, int c, int k)
     return OF_A ? (static_cast<long long>(a) * g.rank + k) * g.lda + c : (static_cast<long long>(a) * g.r + c) * g.ldb + k;
 }
 
+// A copy of BYTES that this thread waits for by itself, or as many zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool have) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(have ? BYTES : 0) : "memory");
+}
+
 // The gradients of both factors: out_a[c][k] = sum over adapter a's tokens of
 // row_t[c] val_t[k], rows of the checkpoint with v for a, of dy with u for b.
 // A block has 128 features and RC ranks of one adapter and a share of its
-// tokens, taken 64 at a time, 16 for each pair of warps, the next 64 tokens'
-// rows and values fetched while these multiply; val enters as two BF16 parts.
-// The four pairs' sums, and the shares', join in a fixed order.
+// tokens, taken 64 at a time, 16 for each pair of warps; val enters as two BF16
+// parts.  Bound by the latency of the rows and values: each thread copies what it
+// will read itself kAhead steps ahead, through shared memory (8000 tokens, rank
+// 64: 104 us one step ahead in registers, READ_OUTER so).  The four pairs' sums,
+// and the shares', join in a fixed order.
+constexpr int kAhead = 2, kRing = kAhead + 1;
 template <int NT>
 struct OuterSmem {
+    uint4 rows[kRing][4][256];        // (codes: 8 bytes of them, 8 of their exponents)
+    float vals[kRing][2 * NT][256];
     union {
         uint32_t vp[2][32][8 * NT + 8];  // [part][pair of tokens][rank]
         float sum[128][8 * NT + 1];      // once the tokens are done
@@ -444,34 +456,61 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
             __syncthreads();
         }
     }
-    const int per = share_of(count, shares), end = min(count, (share + 1) * per);
+    const int per = share_of(count, shares), end = min(count, (share + 1) * per), begin = share * per;
     float acc[4][NT][4] = {};
-    uint32_t w[4][4];
-    float va[NT], vb[NT];
     const int pair = threadIdx.x >> 3, k8 = threadIdx.x & 7;
-    auto fetch = [&](int from) {
-        const int i0 = from + 2 * pair;
-        const int ta = i0 < end ? tokens[i0] : -1, tb = i0 + 1 < end ? tokens[i0 + 1] : -1;
+    // Tokens of this thread in the 64 from `from` on, -1 behind the last: four rows, k slots 2t, 2t+1, 2t+8,
+    // 2t+9 of the fragments, and two tokens' values.
+    int tok[6];
+    auto find = [&](int from) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const bool in = rank0 + k8 + 8 * i < g.rank;
-            va[i] = in && ta >= 0 ? val[static_cast<long long>(ta) * g.rank + rank0 + k8 + 8 * i] : 0.0f;
-            vb[i] = in && tb >= 0 ? val[static_cast<long long>(tb) * g.rank + rank0 + k8 + 8 * i] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // tokens of k slots 2t, 2t+1, 2t+8, 2t+9
-            const int i = from + (warp >> 1) * 16 + 2 * tq + (j & 1) + 8 * (j >> 1);
-            const uint4 v = i < end && f < src.cols ? row8<CODES>(src, tokens[i], f) : make_uint4(0, 0, 0, 0);
-            w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+        for (int j = 0; j < 6; ++j) {
+            const int i = from + (j < 4 ? (warp >> 1) * 16 + 2 * tq + (j & 1) + 8 * (j >> 1) : 2 * pair + j - 4);
+            tok[j] = i < end ? tokens[i] : -1;
         }
     };
-    const int begin = share * per;
-    if (begin < end) fetch(begin);
-    for (int from = begin; from < end; from += 64) {
-        __syncthreads();
+    auto fetch = [&](int stage) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {  // two tokens' values of a rank as one word, high parts and low parts
-            linear::split_pair(va[i], vb[i], sm.vp[0][pair][k8 + 8 * i], sm.vp[1][pair][k8 + 8 * i]);
+        for (int j = 0; j < 4; ++j) {
+            const bool have = tok[j] >= 0 && f < src.cols;
+            const long long t = have ? tok[j] : 0;
+            const int at = have ? f : 0;
+            const uint32_t dst = umma::smem_u32(&sm.rows[stage][j][threadIdx.x]);
+            if constexpr (CODES) {
+                copy_async<8>(dst, src.x8.codes + t * src.x8.ldq + at, have);
+                copy_async<8>(dst + 8, src.x8.exps + t / act8::kBlock * src.x8.lde + at, have);
+            } else {
+                copy_async<16>(dst, src.x + t * src.ld + at, have);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+            const int k = rank0 + k8 + 8 * (i >> 1), t = tok[4 + (i & 1)];
+            const bool have = k < g.rank && t >= 0;
+            copy_async<4>(umma::smem_u32(&sm.vals[stage][i][threadIdx.x]), have ? val + static_cast<long long>(t) * g.rank + k : val, have);
+        }
+    };
+    int stage = 0;
+    find(begin);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        if (begin + 64 * i < end) fetch(i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        find(begin + 64 * (i + 1));
+    }
+    for (int from = begin; from < end; from += 64) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        uint32_t w[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint4 v = sm.rows[stage][j][threadIdx.x];
+            if constexpr (CODES) {
+                uint32_t sc[4];
+                act8::scales8(make_uint2(v.z, v.w), sc);
+                v = act8::decode8(make_uint2(v.x, v.y), sc);
+            }
+            if (f + 8 > src.cols) v = first_of(v, src.cols - f);
+            w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
         }
         // rows g, g+8 of tile m: features 2m, 2m+1 of the lane's eight
         uint32_t x[4][4];
@@ -483,7 +522,15 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
             x[m][3] = __byte_perm(w[2][m], w[3][m], 0x7632);
         }
         __syncthreads();
-        if (from + 64 < end) fetch(from + 64);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)  // two tokens' values of a rank as one word, high parts and low parts
+            linear::split_pair(sm.vals[stage][2 * i][threadIdx.x], sm.vals[stage][2 * i + 1][threadIdx.x], sm.vp[0][pair][k8 + 8 * i],
+                               sm.vp[1][pair][k8 + 8 * i]);
+        __syncthreads();
+        if (from + 64 * kAhead < end) fetch(stage == 0 ? kRing - 1 : stage - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        find(from + 64 * (kAhead + 1));
+        stage = stage == kRing - 1 ? 0 : stage + 1;
         const int p = (warp >> 1) * 8 + tq;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -525,7 +572,8 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
 template <int NT>
 __global__ void __launch_bounds__(256) outer_kernel(const Args g, const Order o, const float* __restrict__ v, const float* __restrict__ u,
                                                     const int shares, const int chunks, float* __restrict__ part) {
-    __shared__ OuterSmem<NT> sm;
+    extern __shared__ uint4 outer_smem[];
+    OuterSmem<NT>& sm = *reinterpret_cast<OuterSmem<NT>*>(outer_smem);
     const int tiles_a = (g.d + 127) / 128, share = blockIdx.z / chunks, rank0 = blockIdx.z % chunks * 8 * NT;
     const int tile = blockIdx.x;
     if (tile < tiles_a) outer_product<NT, true>(g, {nullptr, 0, g.x8, g.d}, v, o, tile, share, shares, rank0, part, g.da, sm);
@@ -691,17 +739,32 @@ int down(const Args& g, const Scratch& s, float* first, float* second, cudaStrea
     return check_launch("down_kernel");
 }
 
+template <int NT>
+int launch_outer(const Args& g, const Scratch& s, int chunks, cudaStream_t st) {
+    constexpr int kBytes = sizeof(OuterSmem<NT>);
+    static std::atomic<uint64_t> prepared{0};  // per device: the shared-memory limit
+    int dev = 0;
+    const int rc = require_device(&dev);
+    if (rc) return rc;
+    if (dev >= 64 || !(prepared.load() >> dev & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute(outer_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e != cudaSuccess) return cuda_fail(e, "outer_kernel setup");
+        if (dev < 64) prepared |= 1ull << dev;
+    }
+    const dim3 grid((g.d + 127) / 128 + (g.r + 127) / 128, g.na, s.shares * chunks);
+    outer_kernel<NT><<<grid, 256, kBytes, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    return check_launch("outer_kernel");
+}
 int gradients(const Args& g, const Scratch& s, cudaStream_t st) {
     // 32 ranks a block at most: with 64 (206 registers, one block an SM) rank 64 took 125 + 18 us where this takes 102 us
     const int chunks = (g.rank + 31) / 32;
-    const dim3 grid((g.d + 127) / 128 + (g.r + 127) / 128, g.na, s.shares * chunks);
-    if (g.rank <= 16) outer_kernel<2><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
-    else outer_kernel<4><<<grid, 256, 0, st>>>(g, s.order, s.v, s.u, s.shares, chunks, s.part);
+    const int rc = g.rank <= 16 ? launch_outer<2>(g, s, chunks, st) : launch_outer<4>(g, s, chunks, st);
+    if (rc) return rc;
     if (s.shares > 1) {
         const long long all = static_cast<long long>(g.na) * (static_cast<long long>(g.d) + g.r) * g.rank;
         join_kernel<<<static_cast<unsigned>(std::min((all + 255) / 256, 148ll * 8)), 256, 0, st>>>(g, s.order, s.shares, s.part);
     }
-    return check_launch("outer_kernel");
+    return check_launch("join_kernel");
 }
 
 bool bad_rows(const void* p, int64_t ld, int64_t cols) {
