@@ -86,6 +86,18 @@ __device__ __forceinline__ void load_words(const bf16* p, uint32_t (&w)[4]) {
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
 }
 
+// NT values of shared memory, aligned to as many.
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[2]) {
+    const float2 f = *reinterpret_cast<const float2*>(p);
+    v[0] = f.x; v[1] = f.y;
+}
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+}
+__device__ __forceinline__ void store_words(uint32_t* p, const uint32_t (&w)[2]) { *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]); }
+__device__ __forceinline__ void store_words(uint32_t* p, const uint32_t (&w)[4]) { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+
 // Eight values of row t at feature f: BF16 rows, or a checkpoint decoded to BF16 (exact).
 struct Rows {
     const bf16* x;   // NULL: the checkpoint
@@ -412,13 +424,13 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool h
 // tokens, taken 64 at a time, 16 for each pair of warps; val enters as two BF16
 // parts.  Bound by the latency of the rows and values: each thread copies what it
 // will read itself kAhead steps ahead, through shared memory (8000 tokens, rank
-// 64: 104 us one step ahead in registers, READ_OUTER so).  The four pairs' sums,
+// 64: 104 us one step ahead in registers, 77 so).  The four pairs' sums,
 // and the shares', join in a fixed order.
 constexpr int kAhead = 2, kRing = kAhead + 1;
 template <int NT>
 struct OuterSmem {
     uint4 rows[kRing][4][256];        // (codes: 8 bytes of them, 8 of their exponents)
-    float vals[kRing][2 * NT][256];
+    float vals[kRing][2][256][NT];    // NT ranks of two tokens
     union {
         uint32_t vp[2][32][8 * NT + 8];  // [part][pair of tokens][rank]
         float sum[128][8 * NT + 1];      // once the tokens are done
@@ -458,7 +470,8 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
     }
     const int per = share_of(count, shares), end = min(count, (share + 1) * per), begin = share * per;
     float acc[4][NT][4] = {};
-    const int pair = threadIdx.x >> 3, k8 = threadIdx.x & 7;
+    const int pair = threadIdx.x >> 3, k8 = threadIdx.x & 7, k0 = rank0 + k8 * NT;
+    const bool whole = g.rank % NT == 0;  // copies of NT ranks are aligned
     // Tokens of this thread in the 64 from `from` on, -1 behind the last: four rows, k slots 2t, 2t+1, 2t+8,
     // 2t+9 of the fragments, and two tokens' values.
     int tok[6];
@@ -484,10 +497,16 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-            const int k = rank0 + k8 + 8 * (i >> 1), t = tok[4 + (i & 1)];
-            const bool have = k < g.rank && t >= 0;
-            copy_async<4>(umma::smem_u32(&sm.vals[stage][i][threadIdx.x]), have ? val + static_cast<long long>(t) * g.rank + k : val, have);
+        for (int i = 0; i < 2; ++i) {
+            const int t = tok[4 + i];
+            const uint32_t dst = umma::smem_u32(sm.vals[stage][i][threadIdx.x]);
+            const float* from = val + static_cast<long long>(max(t, 0)) * g.rank;
+            if (whole) {  // (k0 < rank then holds for all NT or none)
+                copy_async<4 * NT>(dst, from + (k0 < g.rank ? k0 : 0), t >= 0 && k0 < g.rank);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) copy_async<4>(dst + 4 * j, from + (k0 + j < g.rank ? k0 + j : 0), t >= 0 && k0 + j < g.rank);
+            }
         }
     };
     int stage = 0;
@@ -522,10 +541,14 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
             x[m][3] = __byte_perm(w[2][m], w[3][m], 0x7632);
         }
         __syncthreads();
+        uint32_t hi[NT], lo[NT];  // two tokens' values of a rank as one word, high parts and low parts
+        float va[NT], vb[NT];
+        load_floats(sm.vals[stage][0][threadIdx.x], va);
+        load_floats(sm.vals[stage][1][threadIdx.x], vb);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)  // two tokens' values of a rank as one word, high parts and low parts
-            linear::split_pair(sm.vals[stage][2 * i][threadIdx.x], sm.vals[stage][2 * i + 1][threadIdx.x], sm.vp[0][pair][k8 + 8 * i],
-                               sm.vp[1][pair][k8 + 8 * i]);
+        for (int i = 0; i < NT; ++i) linear::split_pair(va[i], vb[i], hi[i], lo[i]);
+        store_words(&sm.vp[0][pair][k8 * NT], hi);
+        store_words(&sm.vp[1][pair][k8 * NT], lo);
         __syncthreads();
         if (from + 64 * kAhead < end) fetch(stage == 0 ? kRing - 1 : stage - 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -756,7 +779,7 @@ int launch_outer(const Args& g, const Scratch& s, int chunks, cudaStream_t st) {
     return check_launch("outer_kernel");
 }
 int gradients(const Args& g, const Scratch& s, cudaStream_t st) {
-    // 32 ranks a block at most: with 64 (206 registers, one block an SM) rank 64 took 125 + 18 us where this takes 102 us
+    // 32 ranks a block at most: with 64 (206 registers, one block an SM) rank 64 took 125 + 18 us where this took 102 us
     const int chunks = (g.rank + 31) / 32;
     const int rc = g.rank <= 16 ? launch_outer<2>(g, s, chunks, st) : launch_outer<4>(g, s, chunks, st);
     if (rc) return rc;
