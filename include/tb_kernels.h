@@ -300,8 +300,8 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * exact: FP32 (F16) dy is split into three (two) BF16 parts, in scratch of
  * 6 (4) bytes per value from the library's per-device pool; rows of a BF16 dy
  * that are not 16-byte aligned are first copied to such scratch.  Where the
- * gradients have few 256 x 256 tiles, shares of their sums also wait there, at
- * most 74 tiles of FP32. */
+ * gradients' 256 x 256 tiles do not fill the GPU's last wave, FP32 shares of
+ * their sums also wait there, at most 148 tiles (39 MB). */
 int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
                         const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride, void* stream);
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
@@ -312,7 +312,7 @@ int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t
  * that these steps give them (in double, rounded to FP32 once): it agrees with
  * the serial recurrence of tb_fisher_ema_step to FP32 rounding.  (alpha and beta
  * are double because 1 - beta of an FP32 0.99 is off by 1e-6.)  fisher is [r][d].
- * A sample without tokens is a step with g = 0. */
+ * A sample without tokens is a step with g = 0.  Scratch as for the gradients. */
 int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r, const int64_t* samples,
                    int S, double alpha, double beta, int first_step, float* fisher, void* stream);
 /* H = scale * Xhat^T Xhat (accumulate != 0: added to H): tb_obs_hessian_scaled
@@ -321,9 +321,9 @@ int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy
  * Within a block of 128 tokens the codes' products add up exactly in integers;
  * the blocks' sums are added in FP32.  A feature with values beyond 2^100,
  * whose diagonal overflows in any case, gives infinities or NaN in its row.
- * Added to H, a sum below FP32's smallest normal value counts as zero.  Scratch
- * where H has few 256 x 256 tiles, or rows (d not a multiple of 4) or an address
- * that are not 16-byte aligned: FP32 shares of H, at most 74 tiles or one H. */
+ * Added to H, a sum below FP32's smallest normal value counts as zero.  Scratch:
+ * FP32 shares of H as for the gradients, or, where its rows or address are not
+ * 16-byte aligned (d not a multiple of 4), all its 256 x 256 tiles. */
 int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, void* stream);
 
 /* ---- low-rank adapters beside a shared projection ------------------------- */
@@ -367,8 +367,8 @@ typedef struct tb_adapter_args {
  * behind the last one (d..lda-1 and so on) are neither used nor written.
  * An infinity or a NaN in a token or an adapter reaches that token's, or that
  * adapter's tokens', results alone.  Scratch from the library's per-device pool:
- * 4 bytes per token and rank and 8 per token, and, where y has few 256 x 256
- * tiles, shares of their sums, at most 74 tiles of FP32. */
+ * 4 bytes per token and rank and 8 per token, and, where y's 256 x 256 tiles do
+ * not fill the GPU's last wave, FP32 shares of their sums, at most 148 tiles. */
 int tb_adapter_forward(const tb_adapter_args* args, void* stream);
 /* With v_t = scale[a] B_a^T dy_t and u_t = scale[a] A_a xhat_t:
  *     dx_t = W^T dy_t + A_a^T v_t,   da_a = sum v_t xhat_t^T,   db_a = sum dy_t u_t^T

@@ -272,7 +272,7 @@ def test_fisher_equals_its_steps(cuda, tblib):
 
 @pytest.mark.parametrize("n,d,acc", [(1, 1, False), (64, 128, False), (130, 200, True), (1000, 640, False),
                                      (777, 515, True), (0, 96, False), (0, 96, True), (4096, 256, False), (300, 1100, True),
-                                     (5000, 300, True), (9000, 130, False)])
+                                     (5000, 300, True), (9000, 130, False), (4000, 2900, True), (4000, 2899, False)])
 def test_hessian(cuda, tblib, n, d, acc):
     torch, tb = cuda, tblib
     x = rows(torch, n, d, torch.float32, n + d)

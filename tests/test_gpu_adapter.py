@@ -70,7 +70,9 @@ SHAPES = [
     (520, 1024, 384, 32, 5, "runs"), (100, 77, 51, 8, 2, "none"), (90, 200, 72, 12, 0, "none"),
     (1100, 256, 640, 100, 3, "runs"), (1024, 96, 80, 16, 3, "mixed"), (1025, 96, 80, 16, 3, "mixed"),
     (2500, 264, 392, 64, 2, "mixed"), (3000, 128, 136, 8, 1, "one"), (1500, 72, 40, 128, 20, "mixed"),
-    (5, 136, 200, 16, 0, "none"), (32, 264, 136, 16, 0, "none"), (2100, 136, 72, 24, 300, "mixed"), (1300, 64, 72, 16, 4, "none"), (2048, 72, 64, 40, 2, "wild")]
+    (2500, 2100, 2000, 16, 4, "mixed"), (5, 136, 200, 16, 0, "none"), (32, 264, 136, 16, 0, "none"),
+    (2100, 136, 72, 24, 300, "mixed"),
+    (1300, 64, 72, 16, 4, "none"), (2048, 72, 64, 40, 2, "wild")]
 
 
 @pytest.mark.parametrize("n,d,r,rank,na,kind", SHAPES)
