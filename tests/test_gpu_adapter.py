@@ -64,7 +64,7 @@ def who_of(torch, n, na, kind, seed=0):
 
 
 SHAPES = [
-    (1, 64, 64, 8, 1, "one"), (1, 4096, 1024, 16, 4, "mixed"), (3, 40, 24, 1, 2, "runs"), (8, 520, 136, 16, 8, "runs"),
+    (1, 1, 1, 1, 1, "one"), (40, 1, 1, 1, 1, "one"), (1100, 3, 2, 1, 2, "mixed"), (1, 64, 64, 8, 1, "one"), (1, 4096, 1024, 16, 4, "mixed"), (3, 40, 24, 1, 2, "runs"), (8, 520, 136, 16, 8, "runs"),
     (17, 256, 264, 5, 3, "mixed"), (33, 136, 1000, 64, 2, "runs"), (64, 512, 256, 128, 3, "mixed"),
     (130, 384, 520, 33, 4, "runs"), (300, 264, 136, 16, 40, "mixed"), (257, 128, 256, 24, 2, "wild"),
     (520, 1024, 384, 32, 5, "runs"), (100, 77, 51, 8, 2, "none"), (90, 200, 72, 12, 0, "none"),
@@ -333,3 +333,50 @@ def test_calibration_step_with_adapters(cuda, tblib):
     tb.check(tb.score_mask_pack(a))
     torch.cuda.synchronize()
     assert float((w == 0).float().mean()) >= 0.5 and bool(torch.isfinite(c.y[:n, :r]).all())
+
+
+def test_offsets_beyond_32_bits(cuda, tblib):
+    """270000 tokens of 8192 features, all but the first 50 and the last 300 zero: x, its codes and dx pass 2^31 values."""
+    torch, tb = cuda, tblib
+    n, d, r, rank, last = 270000, 8192, 64, 16, 300
+    x = torch.zeros(n, d, device="cuda", dtype=torch.bfloat16)
+    dy = torch.zeros(n, r, device="cuda", dtype=torch.bfloat16)
+    for rows_of, cols, seed, scale in ((x, d, 1, 1.0), (dy, r, 3, 0.1)):
+        rows_of[:50] = bf(torch, 50, cols, seed, scale)
+        rows_of[n - last:] = bf(torch, last, cols, seed + 1, scale)
+    who = torch.full((n,), -1)
+    who[:50], who[n - last:] = 0, 1
+    who = who.to(torch.int32).cuda()
+    w, a, b = bf(torch, r, d, 5, 0.05), bf(torch, 2 * rank, d, 6, 0.01), bf(torch, 2 * r, rank, 7, 0.3)
+    scale = torch.tensor([1.0, 0.5], device="cuda")
+    ck = packed(torch, tb, x)
+    b0 = (n - last) // 128 * 128
+    q, e = ref.pack(torch, x[b0:])
+    assert torch.equal(ck.codes[b0:], q) and torch.equal(ck.exps[b0 // 128:], e)
+    dx = torch.full((n, d), 3.0, device="cuda", dtype=torch.bfloat16)
+    tb.check(tb.act8_unpack(ck.s, dx.data_ptr(), tb.BF16, d))
+    assert torch.equal(dx[b0:].double(), ref.values(torch, q, e)) and not bool(dx[1000:b0:997].any())
+    y = torch.full((n, r), 3.0, device="cuda", dtype=torch.bfloat16)
+    da, db = torch.empty_like(a), torch.empty_like(b)
+    args = tb.adapter_args(n=n, d=d, r=r, rank=rank, n_adapters=2, w=w.data_ptr(), ldw=d, a=a.data_ptr(), lda=d, b=b.data_ptr(),
+                           ldb=rank, scale=scale.data_ptr(), token_adapter=who.data_ptr(), x=x.data_ptr(), ldx=d, y=y.data_ptr(),
+                           ldy=r, dy=dy.data_ptr(), lddy=r, x8=ck.s, dx=dx.data_ptr(), lddx=d, da=da.data_ptr(), db=db.data_ptr())
+    tb.check(tb.adapter_forward(args))
+    tb.check(tb.adapter_backward(args))
+    G = torch.empty(r, d, device="cuda")
+    sp = torch.tensor([[n - last, n]], device="cuda")
+    tb.check(tb.act8_weight_grad(ck.s, dy.data_ptr(), tb.BF16, r, r, sp.data_ptr(), 1, G.data_ptr(), tb.F32))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    at = torch.cat([torch.arange(50), torch.arange(n - last, n)]).cuda()
+    R = ref.Adapters(torch, w, a.reshape(2, rank, d), b.reshape(2, r, rank), scale, who[at])
+    check(torch, y[at], R.forward(x[at]), R.forward(x[at], True), d + rank)
+    assert not bool(y[50:n - last].any()) and not bool(dx[50:n - last:997].any())
+    q0, e0 = ref.pack(torch, x[:128])
+    xh = torch.cat([ref.values(torch, q0, e0)[:50], ref.values(torch, q, e)[n - last - b0:]])
+    want, mag = R.backward(dy[at], xh), R.backward(dy[at], xh, True)
+    check(torch, dx[at], want[0], mag[0], r + rank)
+    check(torch, da.reshape(2, rank, d), want[1], mag[1], n + r)
+    check(torch, db.reshape(2, r, rank), want[2], mag[2], n + d)
+    g = dy[n - last:].double().t() @ xh[50:]
+    assert float((G.double() - g).norm() / g.norm()) <= 2e-6
