@@ -281,6 +281,24 @@ int prepare_dy(const View& ck, const void* dy, int dtype, int64_t lddy, int r, c
 }
 
 }  // namespace
+
+int unpack(const View& ck, void* out, int dtype, long long ldo, cudaStream_t st) {
+    const long long blocks = (ck.n + kBlock - 1) / kBlock;
+    for (long long b0 = 0; b0 < blocks; b0 += 65535) {
+        const long long nb = std::min(blocks - b0, 65535ll), t0 = b0 * kBlock;
+        const View v{ck.codes + t0 * ck.ldq, ck.exps + b0 * ck.lde, ck.ldq, ck.lde, ck.n - t0, ck.d};
+        const dim3 grid((ck.d + kFeat - 1) / kFeat, static_cast<unsigned>(nb));
+        void* op = static_cast<char*>(out) + t0 * ldo * (dtype == TB_F32 ? 4 : 2);
+        const bool vec = vectors(out, ldo, dtype == TB_F32 ? 4 : 2);
+        switch (dtype) {
+        case TB_F32: vec ? unpack_kernel<TB_F32, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F32, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        case TB_F16: vec ? unpack_kernel<TB_F16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        default: vec ? unpack_kernel<TB_BF16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_BF16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
+        }
+    }
+    return check_launch("unpack_kernel");
+}
+
 }  // namespace act8
 }  // namespace tb
 
@@ -323,21 +341,7 @@ extern "C" int tb_act8_unpack(const tb_act8* ckp, void* out, int dtype, int64_t 
     if (ck.n == 0) return TB_OK;
     if (!out || ldo < ck.d) return fail(TB_ERR_ARG, "tb_act8_unpack: out is null or ldo < d");
     if ((rc = require_device(nullptr))) return rc;
-    const long long blocks = (ck.n + kBlock - 1) / kBlock;
-    auto st = static_cast<cudaStream_t>(stream);
-    for (long long b0 = 0; b0 < blocks; b0 += 65535) {
-        const long long nb = std::min(blocks - b0, 65535ll), t0 = b0 * kBlock;
-        const View v{ck.codes + t0 * ck.ldq, ck.exps + b0 * ck.lde, ck.ldq, ck.lde, ck.n - t0, ck.d};
-        const dim3 grid((ck.d + kFeat - 1) / kFeat, static_cast<unsigned>(nb));
-        void* op = static_cast<char*>(out) + t0 * ldo * (dtype == TB_F32 ? 4 : 2);
-        const bool vec = vectors(out, ldo, dtype == TB_F32 ? 4 : 2);
-        switch (dtype) {
-        case TB_F32: vec ? unpack_kernel<TB_F32, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F32, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
-        case TB_F16: vec ? unpack_kernel<TB_F16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_F16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
-        default: vec ? unpack_kernel<TB_BF16, true><<<grid, 256, 0, st>>>(v, op, ldo) : unpack_kernel<TB_BF16, false><<<grid, 256, 0, st>>>(v, op, ldo); break;
-        }
-    }
-    return check_launch("unpack_kernel");
+    return act8::unpack(ck, out, dtype, ldo, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tb_act8_weight_grad(const tb_act8* ckp, const void* dy, int dy_dtype, int64_t lddy, int r,

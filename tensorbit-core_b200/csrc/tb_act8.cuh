@@ -27,6 +27,8 @@ struct View {
 
 // Status of a checkpoint description; fills `v`.
 int check(const tb_act8* ck, const char* who, View* v);
+// Enqueues the reading back of n > 0 tokens.
+int unpack(const View& ck, void* out, int dtype, long long ldo, cudaStream_t st);
 
 // 2^(E - 127) in FP32.  E = 255 gives an infinity, and the zero codes of such a block times it NaN.
 __device__ __forceinline__ float scale_f32(uint32_t e) { return __uint_as_float(e << 23); }

@@ -43,7 +43,8 @@ namespace {
 using namespace tb::umma;
 using bf16 = __nv_bfloat16;
 
-enum Mode { kGrad = 0, kFisher = 1, kHess = 2, kFwd = 3, kDx = 4 };
+enum Mode { kGrad = 0, kFisher = 1, kHess = 2, kFwd = 3, kDx = 4, kGradX = 5, kFisherX = 6 };
+__host__ __device__ constexpr int kind(int mode) { return mode == kGradX ? kGrad : mode == kFisherX ? kFisher : mode; }
 
 __device__ int g_linear_error;
 
@@ -57,7 +58,9 @@ constexpr int kDecodeWarps = 6;
 
 template <int MODE>
 struct Cfg {
-    static constexpr bool kCodes = MODE == kGrad || MODE == kFisher;   // B from codes
+    static constexpr bool kCodes = MODE == kGrad || MODE == kFisher;   // B decoded from codes here
+    static constexpr bool kTails = MODE == kGradX || MODE == kFisherX; // B in BF16; a sample's last slice is cut off in shared memory
+    static constexpr bool kSamples = kCodes || kTails;
     static constexpr bool kAdapter = MODE == kFwd || MODE == kDx;
     static constexpr bool kPromote = !kAdapter;
     static constexpr int NB = 256;                                     // columns of a pair's tile
@@ -65,7 +68,7 @@ struct Cfg {
     static constexpr int kCols = NB / 2;                               // columns of an epilogue warp, and of a CTA's B
     // K slices summed in TMEM before they are added in FP32: 512 tokens (kGrad), one block of codes
     // (kHess), all (16-bit results).  kFisher: see kDirect.
-    static constexpr int kGroup = MODE == kGrad ? 8 : MODE == kFisher ? 4 : MODE == kHess ? 1 : 1 << 30;
+    static constexpr int kGroup = kind(MODE) == kGrad ? 8 : kind(MODE) == kFisher ? 4 : MODE == kHess ? 1 : 1 << 30;
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
     static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
@@ -73,12 +76,12 @@ struct Cfg {
     static constexpr int kStage = kA + kB + kRaw;
     // Arrivals that make a stage ready: the decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
-    static constexpr int kReady = kCodes ? 2 * kDecodeWarps : kAdapter ? 9 : 1;
-    static constexpr int kStages = kCodes ? 4 : 6;
+    static constexpr int kReady = kCodes ? 2 * kDecodeWarps : kAdapter || kTails ? 9 : 1;
+    static constexpr int kStages = kCodes ? 4 : kTails ? 5 : 6;
     // Behind the stages: pieces of results on their way out, the exponents of each stage
-    static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
+    static constexpr int kPieces = kind(MODE) == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
     static constexpr int kOut = kEpiWarps * kOutWarp;
-    static constexpr int kFactors = MODE == kFisher ? 1024 : 0;        // samples whose factor is held in shared memory
+    static constexpr int kFactors = kind(MODE) == kFisher ? 1024 : 0;        // samples whose factor is held in shared memory
     static constexpr int kExtra = kOut + kStages * kExps + kFactors * 4;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 512;
     static_assert(kSmem <= 232448, "shared memory of a block");
@@ -256,8 +259,8 @@ __device__ __forceinline__ Tile tile_of(const Params& P, int item) {
         t.tm = tm;
         t.tn = unit - tm * (tm + 1) / 2;
     } else {
-        const int tiles = P.tiles_m * P.tiles_n, i = MODE == kGrad ? unit % tiles : unit;
-        if constexpr (MODE == kGrad) t.s = unit / tiles;
+        const int tiles = P.tiles_m * P.tiles_n, i = kind(MODE) == kGrad ? unit % tiles : unit;
+        if constexpr (kind(MODE) == kGrad) t.s = unit / tiles;
         // bands of 8 tile rows, column by column inside, so that concurrent tiles share operands in L2
         const int band = i / (8 * P.tiles_n), in = i % (8 * P.tiles_n);
         const int rows = min(8, P.tiles_m - 8 * band);
@@ -274,18 +277,18 @@ __device__ __forceinline__ int share_begin(int all, int q, int splits) {
 template <int MODE>
 __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
     Unit u{0, P.K, 0, 0, 0, 0, Cfg<MODE>::kGroup, 0, 1, nullptr};
-    if constexpr (Cfg<MODE>::kCodes) {
+    if constexpr (Cfg<MODE>::kSamples) {
         u.hi = P.n;
         if (P.samples) {
             const long long b = __ldg(P.samples + 2 * s), e = __ldg(P.samples + 2 * s + 1);
             u.begin = static_cast<int>(min(max(b, 0ll), static_cast<long long>(P.n)));
             u.hi = static_cast<int>(max(min(e, static_cast<long long>(P.n)), static_cast<long long>(u.begin)));
-            u.lo = u.begin & ~63;  // a slice then lies in one block of codes
+            u.lo = Cfg<MODE>::kCodes ? u.begin & ~63 : u.begin;  // (codes: a slice then lies in one block)
         }
         u.slices = u.hi > u.begin ? (u.hi - u.lo + 63) / 64 : 0;
         u.total = u.slices * P.parts;
-        if (MODE == kFisher && u.total <= kDirect) u.group = kDirect;
-        if (MODE != kFisher && t.splits > 1) {
+        if (kind(MODE) == kFisher && u.total <= kDirect) u.group = kDirect;
+        if (kind(MODE) != kFisher && t.splits > 1) {
             u.first = share_begin(u.slices * P.parts, t.q, t.splits);
             u.total = share_begin(u.slices * P.parts, t.q + 1, t.splits) - u.first;
         }
@@ -326,7 +329,7 @@ template <int MODE, class F>
 __device__ __forceinline__ bool for_units(const Params& P, F&& f) {
     for (int item = blockIdx.x >> 1; item < P.items; item += gridDim.x >> 1) {
         const Tile t = tile_of<MODE>(P, item);
-        if constexpr (MODE == kFisher) {
+        if constexpr (kind(MODE) == kFisher) {
             for (int s = share_begin(P.S, t.q, t.splits), end = share_begin(P.S, t.q + 1, t.splits); s < end; ++s)
                 if (!f(t, unit_of<MODE>(P, t, s))) return false;
         } else {
@@ -669,7 +672,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if constexpr (MODE == kFisher)
+    if constexpr (kind(MODE) == kFisher)
         for (int s = threadIdx.x; s < min(P.S, C::kFactors); s += kThreads) factors[s] = fisher_factor(P, s);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -726,7 +729,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_even(smem_u32(&accempty[b]));
-            } else if constexpr (MODE == kFisher) {
+            } else if constexpr (kind(MODE) == kFisher) {
                 // A share is a state of its own, begun at 0.
                 float* out = t.slot < 0 ? static_cast<float*>(P.out) + row0 * P.ldo + col
                                         : P.part + static_cast<long long>(t.slot) * kPartTile + row_in * 256 + half * COLS;
@@ -849,14 +852,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                             for (int i = 0; i < COLS; ++i) acc[i] *= P.scale;
                         }
                         // kHess: only 128 x 128 tiles on or below the diagonal
-                        const bool wanted = rows > 0 && cols > 0 && (MODE == kGrad || col / 128 <= row0 / 128);
+                        const bool wanted = rows > 0 && cols > 0 && (kind(MODE) == kGrad || col / 128 <= row0 / 128);
                         if (t.slot >= 0) {
                             if (wanted) store_tma<false, C::kPieces>(&tP, buf, acc, half * COLS, row_in, t.slot, 256, false, lane);
                         } else if (MODE == kHess || P.out_tma) {
                             if (!wanted) continue;
-                            if (MODE == kGrad && P.out_bf16) store_tma<true, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), false, lane);
+                            if (kind(MODE) == kGrad && P.out_bf16) store_tma<true, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), false, lane);
                             else store_tma<false, C::kPieces>(&tO, buf, acc, static_cast<int>(col), static_cast<int>(row0), t.s, static_cast<int>(P.N), MODE == kHess && P.accumulate, lane);
-                        } else if constexpr (MODE == kGrad) {
+                        } else if constexpr (kind(MODE) == kGrad) {
                             const long long at = t.s * P.out_stride + row0 * P.ldo + col;
                             if (P.out_bf16) store_rows<true>(buf, acc, static_cast<bf16*>(P.out) + at, P.ldo, rows, cols, lane);
                             else store_rows<false>(buf, acc, static_cast<float*>(P.out) + at, P.ldo, rows, cols, lane);
@@ -865,7 +868,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 }
             }
         }
-        if constexpr (MODE == kGrad || MODE == kHess) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if constexpr (kind(MODE) == kGrad || MODE == kHess) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) give_up(abort_flag);
     } else {
         if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -873,6 +876,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             if (lane == 0) {
                 // (This loop and the MMA warp's bound the products: 60 cycles more a slice are 5 % of their time.)
                 Ring<kStages> at;
+                uint32_t tails = 0, tailed = 0;  // a bit per stage: parity of its cut slices, whether it had any
                 const uint32_t full0 = smem_u32(full), ready0 = smem_u32(ready) & kPeerMask, empty0 = smem_u32(empty);
                 const bool done = for_units<MODE>(P, [&](const Tile& t, const Unit& u) {
                     const int m0 = t.tm * 256 + rank * 128, n0 = t.tn * NB + rank * C::kCols;
@@ -880,7 +884,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         constexpr int kStep = MODE == kHess ? 128 : 64;
                         int k = u.lo + i * kStep;
                         // parts with fewer leading bits first: the large ones are then truncated least often
-                        const int above = C::kCodes ? (P.parts - 1 - part) * P.n : 0;
+                        const int above = C::kSamples ? (P.parts - 1 - part) * P.n : 0;
 #pragma unroll 1
                         for (; count > 0; --count, k += kStep, at.next()) {
                             const uint32_t a = stage_a(0) + at.s * C::kStage, b = a + C::kA;
@@ -892,19 +896,35 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                                 tma_load_2d(a + kMnChunk, &tA, m0 + 64, above + k, bar);
                                 tma_load_2d(b + C::kB, &tB, n0, k, bar);
                                 tma_load_2d(smem_u32(exps_buf) + at.s * C::kExps, &tE, n0, k >> 7, bar);
+                            } else if (C::kTails && k + 64 > u.hi) {  // the sample ends in this slice: the prepare warps cut it off
+                                const uint32_t bar = full0 + 8 * at.s;
+                                if (rank == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ready0 + 8 * at.s) : "memory");
+                                mbar_expect_tx(bar, C::kA + C::kB);
+                                tma_load_2d(a, &tA, m0, above + k, bar);
+                                tma_load_2d(a + kMnChunk, &tA, m0 + 64, above + k, bar);
+                                tma_load_2d(b, &tB, n0, k, bar);
+                                tma_load_2d(b + kMnChunk, &tB, n0 + 64, k, bar);
+                                tails ^= 1u << at.s;
+                                tailed |= 1u << at.s;
                             } else {
                                 const uint32_t bar = ready0 + 8 * at.s;
                                 if (rank == 0) {
-                                    if (C::kAdapter) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 8;" ::"r"(bar) : "memory");
+                                    if (C::kAdapter || C::kTails) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 8;" ::"r"(bar) : "memory");
                                     mbar_expect_tx(bar, 2 * (C::kA + C::kB));
                                 }
-                                if constexpr (MODE == kHess) tma_load_pair(a, &tA, m0, k, bar);
-                                else tma_load_pair(a, &tA, k, m0, bar);
+                                if constexpr (MODE == kHess) {
+                                    tma_load_pair(a, &tA, m0, k, bar);
+                                } else if constexpr (C::kTails) {
+                                    tma_load_pair(a, &tA, m0, above + k, bar);
+                                    tma_load_pair(a + kMnChunk, &tA, m0 + 64, above + k, bar);
+                                } else {
+                                    tma_load_pair(a, &tA, k, m0, bar);
+                                }
                                 if constexpr (MODE == kFwd) {
                                     tma_load_pair(b, &tB, k, n0, bar);
                                 } else {
                                     tma_load_pair(b, &tB, n0, k, bar);
-                                    if constexpr (MODE == kDx) tma_load_pair(b + kMnChunk, &tB, n0 + 64, k, bar);
+                                    if constexpr (MODE == kDx || C::kTails) tma_load_pair(b + kMnChunk, &tB, n0 + 64, k, bar);
                                 }
                             }
                         }
@@ -926,6 +946,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         const bool used = i < at.s || at.phase;
                         if (used) wait(smem_u32(C::kCodes ? &full[i] : &ready[i]), i < at.s ? at.phase : at.phase ^ 1, nullptr);
                     }
+                    for (int i = 0; C::kTails && i < kStages; ++i)
+                        if (tailed >> i & 1) wait(smem_u32(&full[i]), (tails >> i & 1) ^ 1, nullptr);
                 }
             }
             __syncwarp();
@@ -1019,6 +1041,29 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 });
             });
             if (!done) give_up(abort_flag);
+        } else if (C::kTails && warp >= kPrepWarp && warp < kTmaWarp) {
+            // Zeros for the tokens behind the sample's end in both operands (either may hold anything there).
+            const int pt = threadIdx.x - kPrepWarp * 32;
+            int it = 0;
+            uint32_t phase = 0;  // a bit per stage, for its cut slices only
+            const bool done = for_units<MODE>(P, [&](const Tile&, const Unit& u) {
+                return for_runs(u, [&](int, int i, int count) {
+                    it += count;
+                    const int last = u.hi - u.lo - (u.slices - 1) * 64;
+                    if (i + count < u.slices || last == 64) return true;
+                    const int s = (it - 1) % kStages;
+                    if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag)) return false;
+                    phase ^= 1u << s;
+                    uint8_t* stage = smem + s * C::kStage;  // two chunks of A, two of B, rows of 128 bytes
+                    for (int q = pt; q < (64 - last) * 32; q += 128)
+                        *reinterpret_cast<uint4*>(stage + (q & 3) * kMnChunk + (last + (q >> 5)) * 128 + ((q >> 2) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive_even(smem_u32(&ready[s]));
+                    return true;
+                });
+            });
+            if (!done) give_up(abort_flag);
         } else if (C::kAdapter && warp >= kPrepWarp && warp < kTmaWarp) {
             // The TMA warp passes a free stage on through full[s]; every use of a stage for an adapter is one
             // phase of that barrier.  (empty[s] cannot be waited on here: its parity says nothing to a waiter
@@ -1075,13 +1120,13 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant_
         const float4 f = *reinterpret_cast<const float4*>(part + static_cast<long long>(q) * P.tail * kPartTile);
         v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
     }
-    const long long at = (MODE == kGrad ? t.s * P.out_stride : 0) + row * P.ldo + col;
+    const long long at = (kind(MODE) == kGrad ? t.s * P.out_stride : 0) + row * P.ldo + col;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (col + e >= P.N) break;
         float* to = static_cast<float*>(P.out) + at + e;
         if constexpr (MODE == kHess) *to = P.accumulate ? *to + v[e] : v[e];
-        else if constexpr (MODE == kFisher) *to = P.first ? v[e] : fmaf(P.decay, *to, v[e]);
+        else if constexpr (kind(MODE) == kFisher) *to = P.first ? v[e] : fmaf(P.decay, *to, v[e]);
         else if (Cfg<MODE>::kAdapter || P.out_bf16) static_cast<bf16*>(P.out)[at + e] = __float2bfloat16_rn(v[e]);
         else *to = v[e];
     }
@@ -1157,7 +1202,7 @@ int make_out_map(CUtensorMap* map, void* base, bool bf16_out, long long cols, lo
 template <int MODE>
 int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& e, Params& P, long long units, long long slices,
                   long long shares, const char* who, cudaStream_t st) {
-    constexpr bool kTma = MODE == kGrad || MODE == kHess;
+    constexpr bool kTma = kind(MODE) == kGrad || MODE == kHess;
     if (units > 0x3FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %lld output tiles", who, units);
     const int esize = P.out_bf16 ? 2 : 4;
     P.out_tma = kTma && reinterpret_cast<uintptr_t>(P.out) % 16 == 0 && P.ldo * esize % 16 == 0 && P.out_stride * esize % 16 == 0;
@@ -1194,14 +1239,21 @@ int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap&
 
 int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
 
-template <int MODE>
+// Gradients and Fisher decode their codes once for each tile of rows and part of
+// dY.  Where that is four times or more, the values are written out as BF16 first,
+// to scratch, and the products read them without a decode between TMA and MMA.
+// (Sixteen gradients of 4096 x 4096, sixteen tiles of rows: 313 us decoded in the
+// product, 258 and 17 for the values so; 64 samples' Fisher 752 against 561 and 37; the
+// gradient of 1024 x 4096 from FP32 dY, twelve times, 20.6 against 17.7 and 2.5.)
+constexpr long long kValuesMax = 1ll << 31;  // bytes of them at most
+
+template <int MODE, int VALUES>
 int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long long samples, const char* who, cudaStream_t st) {
-    using C = Cfg<MODE>;
     if (ck.n * dy.parts > 0x7FFFFFFFll - 64) return fail(TB_ERR_CAPACITY, "%s: %lld tokens in %d parts", who, ck.n, dy.parts);
     P.M = r;
     P.N = ck.d;
     P.tiles_m = tiles(r, 256);
-    P.tiles_n = tiles(ck.d, C::NB);
+    P.tiles_n = tiles(ck.d, 256);
     P.exps = ck.exps;
     P.lde = ck.lde;
     P.n = static_cast<int>(ck.n);
@@ -1209,13 +1261,24 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     P.ldo = ck.d;
     int rc = TB_OK;
     CUtensorMap a{}, b{}, e{};
+    const long long ld = (ck.d + 7) / 8 * 8;
+    const bool values = ck.n > 0 && static_cast<long long>(P.tiles_m) * P.parts >= 4 && 2 * ck.n * ld <= kValuesMax;
+    void* x = nullptr;
+    if (values) {
+        rc = scratch_alloc(&x, static_cast<size_t>(2 * ck.n * ld), st);
+        if (!rc) rc = act8::unpack(ck, x, TB_BF16, ld, st);
+    }
     if (!rc && ck.n > 0) rc = make_map(&a, dy.base, 2, r, ck.n * dy.parts, dy.ld, 64, 64, true);
-    if (!rc && ck.n > 0) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, C::kCols, 64, false);
-    if (!rc && ck.n > 0) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, C::kCols, 1, false);
+    if (!rc && values) rc = make_map(&b, x, 2, ck.d, ck.n, ld, 64, 64, true);
+    if (!rc && ck.n > 0 && !values) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, Cfg<MODE>::kCols, 64, false);
+    if (!rc && ck.n > 0 && !values) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, Cfg<MODE>::kCols, 1, false);
     const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
     // (The samples' lengths are on the device: as if they were even.)  A unit of the Fisher mode has all samples.
     const long long each = (ck.n / std::max(1, P.S) + 63) / 64 * dy.parts, slices = MODE == kFisher ? P.S * each : each;
-    return rc ? rc : launch_shared<MODE>(a, b, e, P, units, slices, MODE == kFisher ? P.S : slices, who, st);
+    const long long shares = MODE == kFisher ? P.S : slices;
+    if (!rc) rc = values ? launch_shared<VALUES>(a, b, b, P, units, slices, shares, who, st) : launch_shared<MODE>(a, b, e, P, units, slices, shares, who, st);
+    scratch_free(x, st);
+    return rc;
 }
 
 }  // namespace
@@ -1228,7 +1291,7 @@ int weight_grad(const act8::View& ck, const Parts& dy, int r, const int64_t* sam
     P.out = grads;
     P.out_bf16 = g_dtype == TB_BF16;
     P.out_stride = g_stride;
-    return from_codes<kGrad>(ck, dy, r, P, S, "tb_act8_weight_grad", st);
+    return from_codes<kGrad, kGradX>(ck, dy, r, P, S, "tb_act8_weight_grad", st);
 }
 
 int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples, int S, double alpha, double beta, bool first,
@@ -1241,7 +1304,7 @@ int fisher(const act8::View& ck, const Parts& dy, int r, const int64_t* samples,
     P.beta = beta;
     P.first = first;
     P.decay = static_cast<float>(pow(beta, static_cast<double>(S)));
-    return from_codes<kFisher>(ck, dy, r, P, 1, "tb_act8_fisher", st);
+    return from_codes<kFisher, kFisherX>(ck, dy, r, P, 1, "tb_act8_fisher", st);
 }
 
 int hessian(const act8::View& ck, float scale, bool accumulate, float* H, cudaStream_t st) {

@@ -140,7 +140,10 @@ def check_sums(torch, got, want, mag, terms, bf16=False):
     (2000, 384, 640, "bfloat16", "bfloat16", [(0, 700), (650, 1400), (1400, 2000), (0, 2000), (0, 700)]),
     (4100, 256, 256, "bfloat16", "float32", None),
     (3000, 100, 203, "float32", "bfloat16", [(0, 1500), (1500, 3000)]), (6000, 264, 130, "float16", "float32", [(7, 5900), (0, 10), (3, 3)]),
-    (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)])])
+    (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)]),
+    (700, 1100, 264, "bfloat16", "float32", [(0, 1), (1, 64), (64, 64), (64, 333), (333, 700)]),
+    (515, 600, 272, "float16", "bfloat16", [(3, 130), (400, 512)]), (333, 520, 100, "float32", "float32", [(5, 70), (70, 200), (0, 333)]),
+    (5, 1000, 9, "bfloat16", "bfloat16", [(0, 3), (3, 5)]), (256, 1030, 72, "float32", "float32", [(-5, 128), (200, 999), (90, 20)])])
 def test_weight_grad(cuda, tblib, n, r, d, dy_t, g_t, samples):
     torch, tb = cuda, tblib
     c = packed(torch, tb, rows(torch, n, d, torch.float32, n))
@@ -488,3 +491,36 @@ def test_gradients_of_last_waves(cuda, tblib, n, r, d, S, g_t):
             got = G[s, :r * d].view(r, d).double()
             assert bool(((got - g).abs() <= half * g.abs() + (b - a) * 2.0 ** -23 * 1.01 * m + 1e-40).all())
         assert pad == 0 or bool((G[:, r * d] == 3).all())
+
+
+@pytest.mark.parametrize("dy_t", ["float32", "bfloat16"])
+def test_samples_of_many_rows_leave_other_tokens_out(cuda, tblib, dy_t):
+    """Rows enough that the values are written out first: NaN before, between and behind the samples reaches none."""
+    torch, tb = cuda, tblib
+    n, r, d = 600, 1100, 200
+    samples = [(3, 130), (131, 200), (210, 211), (220, 539)]
+    x, dy = rows(torch, n, d, torch.float32, 30), rows(torch, n, r, getattr(torch, dy_t), 31, ref.up(r, 8), 0.1, 0)
+    inside = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for a, b in samples:
+        inside[a:b] = True
+    dy[~inside] = math.nan
+    x[560:] = math.nan  # blocks 0 .. 3 stay numbers
+    x[512:560] = 0.0
+    ck = packed(torch, tb, x, (torch.arange(n, device="cuda") < 560).to(torch.uint8))
+    sp = pairs(torch, samples)
+    G = torch.full((4, r, d), 3.0, device="cuda")
+    tb.check(tb.act8_weight_grad(ck.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), 4, G.data_ptr(), tb.F32))
+    F = torch.full((r, d), math.nan, device="cuda")
+    tb.check(tb.act8_fisher(ck.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), 4, F.data_ptr()))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    want = None
+    for s, (g, m) in enumerate(ref.gradients(torch, dy, ck.values(torch), samples)):
+        check_sums(torch, G[s], g, m, n * PARTS[dy_t])
+        want = 0.01 * g * g if want is None else 0.99 * want + 0.01 * 0.01 * g * g
+    assert float((F.double() - want).norm() / want.norm()) <= 4e-6  # a square doubles g's 2e-6
+    x[225, 7] = math.nan  # a number no longer in block 1: the feature of that block is NaN, for the samples in it
+    ck = packed(torch, tb, x, (torch.arange(n, device="cuda") < 560).to(torch.uint8))
+    tb.check(tb.act8_weight_grad(ck.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), 4, G.data_ptr(), tb.F32))
+    assert not bool(torch.isnan(G[0][:, :7]).any()) and bool(torch.isnan(G[1][:, 7]).all()) and bool(torch.isnan(G[3][:, 7]).all())
+    assert int(torch.isnan(G).sum()) == sum(r for a, b in samples if a < 256 and b > 128)
