@@ -77,9 +77,9 @@ struct Cfg {
     // Arrivals that make a stage ready: the decoding warps of each CTA (codes), the even CTA's
     // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
     static constexpr int kReady = kCodes ? 2 * kDecodeWarps : kAdapter || kTails ? 9 : 1;
-    static constexpr int kStages = kCodes ? 4 : kTails ? 5 : 6;
+    static constexpr int kStages = kCodes ? 4 : MODE == kFisherX ? 5 : 6;
     // Behind the stages: pieces of results on their way out, the exponents of each stage
-    static constexpr int kPieces = kind(MODE) == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
+    static constexpr int kPieces = MODE == kGrad ? 2 : 1, kOutWarp = kPieces * 4096;
     static constexpr int kOut = kEpiWarps * kOutWarp;
     static constexpr int kFactors = kind(MODE) == kFisher ? 1024 : 0;        // samples whose factor is held in shared memory
     static constexpr int kExtra = kOut + kStages * kExps + kFactors * 4;
