@@ -299,9 +299,11 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * no sample are not read into any.  Sums are in FP32 and every product is
  * exact: FP32 (F16) dy is split into three (two) BF16 parts, in scratch of
  * 6 (4) bytes per value from the library's per-device pool; rows of a BF16 dy
- * that are not 16-byte aligned are first copied to such scratch.  Where the
- * gradients' 256 x 256 tiles do not fill the GPU's last wave, FP32 shares of
- * their sums also wait there, at most 148 tiles (39 MB). */
+ * that are not 16-byte aligned are first copied to such scratch.  Large products
+ * with r beyond 1024 (F16: 512, FP32: 256) write xhat out there as BF16, 2 bytes
+ * per value, unless that is more than 2 GiB.  Where the gradients' 256 x 256
+ * tiles do not fill the GPU's last wave, FP32 shares of their sums also wait
+ * there, at most 148 tiles (39 MB). */
 int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
                         const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride, void* stream);
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:

@@ -6,8 +6,8 @@
 // half of the accumulator in TMEM.  Roles of a CTA's 16 warps:
 //   warp 12      TMA loads of K slices into a ring of stages;
 //   warps 8-11   (and 14-15) "prepare" stages that do not arrive as operands: decode int8
-//                codes to BF16 and zero what lies behind a sample's end, or
-//                build the operands of an adapter; then tell the even CTA;
+//                codes to BF16, zero what lies behind a sample's end, or build
+//                the operands of an adapter; then tell the even CTA;
 //   warp 13      (even CTA) issues tcgen05.mma for both CTAs;
 //   warps 0-7    take finished accumulators out of TMEM and store results.
 // The accumulator is double buffered, so the next sums run while a tile is
@@ -20,6 +20,7 @@
 //   kGrad    G_s = dY_s^T Xhat_s: A = dY (M-major by TMA), B = decoded codes
 //   kFisher  the same with the Fisher state in registers: a sum of the samples' g^2
 //            with the factors that the EMA's steps give them, in order
+//   kGradX, kFisherX  the same two with B = Xhat in BF16, decoded beforehand
 //   kHess    Xhat^T Xhat on int8 tensor cores: the codes of a block of 128
 //            tokens multiply exactly into int32, and the block's two
 //            power-of-two scales enter when its sum is added in FP32
@@ -75,7 +76,7 @@ struct Cfg {
     static constexpr int kExps = kCodes ? kCols : 0;                   // exponents of its block
     static constexpr int kStage = kA + kB + kRaw;
     // Arrivals that make a stage ready: the decoding warps of each CTA (codes), the even CTA's
-    // TMA thread (bytes of both CTAs), or either (an adapter's slice is built by the prepare warps)
+    // TMA thread (bytes of both CTAs), or either (an adapter's or a sample's last slice is the prepare warps')
     static constexpr int kReady = kCodes ? 2 * kDecodeWarps : kAdapter || kTails ? 9 : 1;
     static constexpr int kStages = kCodes ? 4 : MODE == kFisherX ? 5 : 6;
     // Behind the stages: pieces of results on their way out, the exponents of each stage
@@ -435,7 +436,7 @@ __device__ __forceinline__ void store_rows(uint8_t* buf, const float (&v)[COLS],
     }
 }
 // The same by TMA, as many pieces in flight as there are buffers, stored or (FP32) added to what is
-// there: sixteen 4096 x 4096 gradients in 336 us (now 313), where straight from registers, 32 bytes of a row a
+// there: sixteen 4096 x 4096 gradients in 336 us, where straight from registers, 32 bytes of a row a
 // lane, they took 400.
 template <bool BF16, int PIECES, int COLS>
 __device__ __forceinline__ void store_tma(const CUtensorMap* map, uint8_t* buf, const float (&v)[COLS], int col, int row0, int s, int N,
@@ -1240,11 +1241,13 @@ int launch_shared(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap&
 int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
 
 // Gradients and Fisher decode their codes once for each tile of rows and part of
-// dY.  Where that is four times or more, the values are written out as BF16 first,
-// to scratch, and the products read them without a decode between TMA and MMA.
-// (Sixteen gradients of 4096 x 4096, sixteen tiles of rows: 313 us decoded in the
-// product, 258 and 17 for the values so; 64 samples' Fisher 752 against 561 and 37; the
-// gradient of 1024 x 4096 from FP32 dY, twelve times, 20.6 against 17.7 and 2.5.)
+// dY.  Where that is five times or more, the values are written out as BF16 first,
+// to scratch, and the products read them without a decode between TMA and MMA; not
+// where a pair of SMs has fewer than 32 slices, for which one launch more is not
+// worth it.  (Kernels, 4096 features, decoded in the product against written out:
+// 16 gradients of 4096 rows 313 and 248 + 17 us; 2048 rows, with all launches, 157
+// and 145; 1024 rows 87 and 87; 512 rows 53 and 59.  One gradient of 500 tokens and
+// 2048 rows 16.0 and 17.4.  64 samples' Fisher of 4096 rows 752 and 561 + 37.)
 constexpr long long kValuesMax = 1ll << 31;  // bytes of them at most
 
 template <int MODE, int VALUES>
@@ -1262,7 +1265,11 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     int rc = TB_OK;
     CUtensorMap a{}, b{}, e{};
     const long long ld = (ck.d + 7) / 8 * 8;
-    const bool values = ck.n > 0 && static_cast<long long>(P.tiles_m) * P.parts >= 4 && 2 * ck.n * ld <= kValuesMax;
+    const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
+    // (The samples' lengths are on the device: as if they were even.)  A unit of the Fisher mode has all samples.
+    const long long each = (ck.n / std::max(1, P.S) + 63) / 64 * dy.parts, slices = MODE == kFisher ? P.S * each : each;
+    const long long shares = MODE == kFisher ? P.S : slices;
+    const bool values = static_cast<long long>(P.tiles_m) * P.parts >= 5 && units * slices >= 32 * kPairs && 2 * ck.n * ld <= kValuesMax;
     void* x = nullptr;
     if (values) {
         rc = scratch_alloc(&x, static_cast<size_t>(2 * ck.n * ld), st);
@@ -1272,10 +1279,6 @@ int from_codes(const act8::View& ck, const Parts& dy, int r, Params& P, long lon
     if (!rc && values) rc = make_map(&b, x, 2, ck.d, ck.n, ld, 64, 64, true);
     if (!rc && ck.n > 0 && !values) rc = make_map(&b, ck.codes, 1, ck.d, ck.n, ck.ldq, Cfg<MODE>::kCols, 64, false);
     if (!rc && ck.n > 0 && !values) rc = make_map(&e, ck.exps, 1, ck.d, (ck.n + 127) / 128, ck.lde, Cfg<MODE>::kCols, 1, false);
-    const long long units = static_cast<long long>(P.tiles_m) * P.tiles_n * samples;
-    // (The samples' lengths are on the device: as if they were even.)  A unit of the Fisher mode has all samples.
-    const long long each = (ck.n / std::max(1, P.S) + 63) / 64 * dy.parts, slices = MODE == kFisher ? P.S * each : each;
-    const long long shares = MODE == kFisher ? P.S : slices;
     if (!rc) rc = values ? launch_shared<VALUES>(a, b, b, P, units, slices, shares, who, st) : launch_shared<MODE>(a, b, e, P, units, slices, shares, who, st);
     scratch_free(x, st);
     return rc;

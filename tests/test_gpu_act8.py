@@ -143,7 +143,10 @@ def check_sums(torch, got, want, mag, terms, bf16=False):
     (256, 40, 1030, "float32", "bfloat16", [(-5, 100), (200, 999), (90, 20)]),
     (700, 1100, 264, "bfloat16", "float32", [(0, 1), (1, 64), (64, 64), (64, 333), (333, 700)]),
     (515, 600, 272, "float16", "bfloat16", [(3, 130), (400, 512)]), (333, 520, 100, "float32", "float32", [(5, 70), (70, 200), (0, 333)]),
-    (5, 1000, 9, "bfloat16", "bfloat16", [(0, 3), (3, 5)]), (256, 1030, 72, "float32", "float32", [(-5, 128), (200, 999), (90, 20)])])
+    (5, 1000, 9, "bfloat16", "bfloat16", [(0, 3), (3, 5)]), (256, 1030, 72, "float32", "float32", [(-5, 128), (200, 999), (90, 20)]),
+    # large enough that the values are written out first
+    (1000, 1300, 2000, "float32", "float32", [(3, 130), (130, 131), (131, 400), (400, 400), (400, 999), (0, 1000)]),
+    (3000, 1100, 2610, "bfloat16", "bfloat16", [(301 * i, 300 * i + 290 - 7 * i) for i in range(10)])])
 def test_weight_grad(cuda, tblib, n, r, d, dy_t, g_t, samples):
     torch, tb = cuda, tblib
     c = packed(torch, tb, rows(torch, n, d, torch.float32, n))
@@ -494,10 +497,11 @@ def test_gradients_of_last_waves(cuda, tblib, n, r, d, S, g_t):
 
 
 @pytest.mark.parametrize("dy_t", ["float32", "bfloat16"])
-def test_samples_of_many_rows_leave_other_tokens_out(cuda, tblib, dy_t):
-    """Rows enough that the values are written out first: NaN before, between and behind the samples reaches none."""
+@pytest.mark.parametrize("d", [200, 10000])
+def test_samples_of_many_rows_leave_other_tokens_out(cuda, tblib, dy_t, d):
+    """NaN before, between and behind the samples reaches none; with 10000 features the values are written out first."""
     torch, tb = cuda, tblib
-    n, r, d = 600, 1100, 200
+    n, r = 600, 1100
     samples = [(3, 130), (131, 200), (210, 211), (220, 539)]
     x, dy = rows(torch, n, d, torch.float32, 30), rows(torch, n, r, getattr(torch, dy_t), 31, ref.up(r, 8), 0.1, 0)
     inside = torch.zeros(n, dtype=torch.bool, device="cuda")
