@@ -318,8 +318,9 @@ int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t
 int tb_act8_fisher(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r, const int64_t* samples,
                    int S, double alpha, double beta, int first_step, float* fisher, void* stream);
 /* H = scale * Xhat^T Xhat (accumulate != 0: added to H): tb_obs_hessian_scaled
- * from a checkpoint, for any d and n.  H is [d][d]; only the 128x128 tiles on
- * or below the diagonal are written.  n = 0 gives zeros (accumulate: H stays).
+ * from a checkpoint, for any d and n up to 2^31 - 128 (more are TB_ERR_SHAPE).
+ * H is [d][d]; only the 128x128 tiles on or below the diagonal are written.
+ * n = 0 gives zeros (accumulate: H stays).
  * Within a block of 128 tokens the codes' products add up exactly in integers;
  * the blocks' sums are added in FP32.  A feature with values beyond 2^100,
  * whose diagonal overflows in any case, gives infinities or NaN in its row.

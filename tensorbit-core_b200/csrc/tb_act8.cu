@@ -392,6 +392,8 @@ extern "C" int tb_act8_hessian(const tb_act8* ckp, float scale, int accumulate, 
     int rc = act8::check(ckp, "tb_act8_hessian", &ck);
     if (rc) return rc;
     if (!H) return fail(TB_ERR_ARG, "tb_act8_hessian: null H");
+    // (The product's token indexes, rounded up to its K step of 128, are 32 bits wide.)
+    if (ck.n > 0x7FFFFFFFll - 127) return fail(TB_ERR_SHAPE, "tb_act8_hessian: %lld tokens", static_cast<long long>(ck.n));
     if ((rc = require_device(nullptr))) return rc;
     return linear::hessian(ck, scale, accumulate != 0, H, static_cast<cudaStream_t>(stream));
 }

@@ -93,3 +93,10 @@ def test_adapter_backward_refusals(tblib):
                      (dict(x8=ck(n=5)), tb.TB_ERR_SHAPE), (dict(x8=ck(n=4, d=48)), tb.TB_ERR_SHAPE)]:
         assert tb.adapter_backward(adapters(**{**ok, **kw})) == code, kw
     assert tb.adapter_forward(adapters(n=0, x=None, y=None, token_adapter=None)) == tb.TB_OK
+
+
+@pytest.mark.parametrize("n", [(1 << 31) - 127, (1 << 31) - 65])
+def test_hessian_refuses_tokens_that_its_steps_cannot_count(tblib, n):
+    """Tokens whose number, rounded up to the Hessian's step of 128, passes 31 bits (the other entries take them)."""
+    assert tb.act8_hessian(ck(n=n), 1.0, P) == tb.TB_ERR_SHAPE
+    assert tb.act8_hessian(ck(n=n), 1.0, P, accumulate=True) == tb.TB_ERR_SHAPE
