@@ -273,7 +273,7 @@ int tb_obs_sparsegpt_phase_times(float* ms_out, int n);
 #define TB_ACT8_BLOCK 128
 typedef struct tb_act8 {
     uint32_t struct_size;  /* sizeof(tb_act8)                                          */
-    int32_t  d;            /* features                                                 */
+    int32_t  d;            /* features, up to 2^31 - 256 (as r below)                  */
     int64_t  n;            /* tokens, below 2^31 - 64                                  */
     int8_t*  codes;        /* [n][ldq], device, 16-byte aligned                        */
     int64_t  ldq;          /* >= d, a multiple of 16                                   */
@@ -340,7 +340,7 @@ typedef struct tb_adapter_args {
     uint32_t struct_size;  /* sizeof(tb_adapter_args)                                    */
     int32_t  dtype;        /* of w, a, b, x, y, dy, dx, da, db: TB_BF16                  */
     int64_t  n;            /* tokens, below 2^31 - 256                                   */
-    int32_t  d, r;         /* in and out features                                        */
+    int32_t  d, r;         /* in and out features, each up to 2^31 - 256                 */
     int32_t  rank;         /* 1..128                                                     */
     int32_t  n_adapters;   /* 0: the projection alone                                    */
     const void* w;         /* [r][ldw]                                                   */

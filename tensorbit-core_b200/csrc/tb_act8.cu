@@ -13,6 +13,7 @@ namespace act8 {
 int check(const tb_act8* ck, const char* who, View* v) {
     if (!ck || ck->struct_size != sizeof(tb_act8)) return fail(TB_ERR_ARG, "%s: null checkpoint or bad struct_size", who);
     if (ck->d <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: a checkpoint has at least one feature", who);
+    if (ck->d > kMaxFeatures) return fail(TB_ERR_SHAPE, "%s: %d features", who, ck->d);
     if (ck->n < 0 || ck->n > 0x7FFFFFFFll - 64) return fail(TB_ERR_SHAPE, "%s: %lld tokens", who, static_cast<long long>(ck->n));
     if (ck->ldq < ck->d || ck->ldq % 16 || ck->lde < ck->d || ck->lde % 16)
         return fail(TB_ERR_ARG, "%s: ldq and lde must be multiples of 16 and at least d", who);
@@ -254,6 +255,7 @@ bool vectors(const void* p, long long ld, int esize) {
 int check_dy(const char* who, const void* dy, int dtype, int64_t lddy, int r, int64_t n, const int64_t* samples, int S) {
     if (dtype < TB_F32 || dtype > TB_BF16) return fail(TB_ERR_ARG, "%s: bad dy dtype %d", who, dtype);
     if (r <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: r must be positive", who);
+    if (r > kMaxFeatures) return fail(TB_ERR_SHAPE, "%s: %d rows of a gradient", who, r);
     if (S < 0 || S > 65535 || (!samples && S != 1))
         return fail(TB_ERR_ARG, "%s: S must be in 0..65535, and 1 where samples is NULL", who);
     if (n > 0 && S > 0 && (!dy || lddy < r)) return fail(TB_ERR_ARG, "%s: dy is null or lddy < r", who);

@@ -16,6 +16,9 @@ namespace act8 {
 
 constexpr int kBlock = TB_ACT8_BLOCK;
 
+// Features at most, in and out: the kernels round their indexes up to tiles of 256 in 32 bits.
+constexpr int kMaxFeatures = 0x7FFFFFFF - 255;
+
 // What the kernels need of a tb_act8.
 struct View {
     int8_t* codes;

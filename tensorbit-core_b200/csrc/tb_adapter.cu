@@ -800,6 +800,7 @@ int check_common(const char* who, const tb_adapter_args* p, bool need_w, Args* g
     if (!p || p->struct_size != sizeof(tb_adapter_args)) return fail(TB_ERR_ARG, "%s: null args or bad struct_size", who);
     if (p->dtype != TB_BF16) return fail(TB_ERR_UNSUPPORTED, "%s: TB_BF16 only (dtype %d)", who, p->dtype);
     if (p->d <= 0 || p->r <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: empty projection", who);
+    if (p->d > act8::kMaxFeatures || p->r > act8::kMaxFeatures) return fail(TB_ERR_SHAPE, "%s: %d in and %d out features", who, p->d, p->r);
     if (p->n < 0 || p->n > 0x7FFFFFFFll - 65536) return fail(TB_ERR_SHAPE, "%s: %lld tokens", who, static_cast<long long>(p->n));
     if (p->n_adapters < 0 || p->n_adapters > 65535) return fail(TB_ERR_ARG, "%s: %d adapters", who, p->n_adapters);
     if (need_w && bad_rows(p->w, p->ldw, p->d)) return fail(TB_ERR_ARG, "%s: w must be 16-byte aligned, ldw >= d a multiple of 8", who);

@@ -100,3 +100,19 @@ def test_hessian_refuses_tokens_that_its_steps_cannot_count(tblib, n):
     """Tokens whose number, rounded up to the Hessian's step of 128, passes 31 bits (the other entries take them)."""
     assert tb.act8_hessian(ck(n=n), 1.0, P) == tb.TB_ERR_SHAPE
     assert tb.act8_hessian(ck(n=n), 1.0, P, accumulate=True) == tb.TB_ERR_SHAPE
+
+
+@pytest.mark.parametrize("many", [(1 << 31) - 255, (1 << 31) - 1])
+def test_features_that_tiles_cannot_count_are_refused(tblib, many):
+    """In or out features whose number, rounded up to a tile of 256, passes 31 bits."""
+    ld = 1 << 31
+    c = ck(n=1, d=many, ldq=ld, lde=ld)
+    assert tb.act8_pack(c, P, tb.F32, ld) == tb.TB_ERR_SHAPE
+    assert tb.act8_unpack(c, P, tb.F32, ld) == tb.TB_ERR_SHAPE
+    assert tb.act8_hessian(c, 1.0, P) == tb.TB_ERR_SHAPE
+    for k, r in ((c, 8), (ck(n=1), many)):
+        assert tb.act8_weight_grad(k, P, tb.F32, ld, r, None, 1, P, tb.F32) == tb.TB_ERR_SHAPE
+        assert tb.act8_fisher(k, P, tb.F32, ld, r, None, 1, P) == tb.TB_ERR_SHAPE
+    for kw in (dict(d=many, ldw=ld, lda=ld, ldx=ld), dict(r=many, ldy=ld, lddy=ld)):
+        assert tb.adapter_forward(adapters(**kw)) == tb.TB_ERR_SHAPE
+        assert tb.adapter_backward(adapters(dy=P, lddy=ld, dx=P, lddx=ld, **{k: v for k, v in kw.items() if k != "lddy"})) == tb.TB_ERR_SHAPE
