@@ -413,6 +413,24 @@ __device__ __forceinline__ long long grad_at(const Args& g, int a, int c, int k)
     return OF_A ? (static_cast<long long>(a) * g.rank + k) * g.lda + c : (static_cast<long long>(a) * g.r + c) * g.ldb + k;
 }
 
+// Feature c's sum with rank k over tokens[begin .. end), products whole, one after
+// another: for a sum of the parts' products that is a NaN.  Times an infinity of
+// the row, a value's second part makes one (where it is zero, or of the other
+// sign) although the product is an infinity.  Ends at the first NaN of its own.
+template <bool CODES>
+__device__ __noinline__ float whole_sum(const Rows& src, const float* val, int rank, const int* tokens, int begin, int end, int c, int k) {
+    float s = 0.0f;
+    for (int i = begin; i < end && s == s; ++i) {
+        const long long t = tokens[i];
+        float x;
+        if constexpr (CODES)
+            x = static_cast<float>(src.x8.codes[t * src.x8.ldq + c]) * act8::scale_f32(src.x8.exps[t / act8::kBlock * src.x8.lde + c]);
+        else x = __bfloat162float(src.x[t * src.ld + c]);
+        s = fmaf(x, val[t * rank + k], s);
+    }
+    return s;
+}
+
 // A copy of BYTES that this thread waits for by itself, or as many zeros.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool have) {
@@ -587,8 +605,10 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
     for (int i = threadIdx.x; i < 128 * RC; i += 256) {
         const int c = CODES ? i % 128 : i / RC, k = CODES ? i / 128 : i % RC;
         if (f0 + c >= src.cols || rank0 + k >= g.rank) continue;
-        if (shares > 1) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = sm.sum[c][k];
-        else out[grad_at<CODES>(g, a, f0 + c, rank0 + k)] = __float2bfloat16_rn(sm.sum[c][k]);
+        float s = sm.sum[c][k];
+        if (s != s) s = whole_sum<CODES>(src, val, g.rank, tokens, begin, end, f0 + c, rank0 + k);
+        if (shares > 1) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = s;
+        else out[grad_at<CODES>(g, a, f0 + c, rank0 + k)] = __float2bfloat16_rn(s);
     }
 }
 

@@ -188,6 +188,31 @@ def test_infinities_of_an_adapter_keep_their_sign(cuda, tblib, n):
     check(torch, got[~hit], dx[~hit], mx[~hit], r + rank)
 
 
+@pytest.mark.parametrize("n", [20, 150, 1500, 4000])
+def test_infinities_of_dy_keep_their_sign_in_db(cuda, tblib, n):
+    """An infinity in dy gives its feature's row of its adapter's db the infinities that the formula gives (a NaN where two
+    of them cancel), and leaves every other entry within its bar."""
+    torch, tb = cuda, tblib
+    d, r, rank, na = 200, 136, 24, 2
+    c = Case(torch, n, d, r, rank, na, torch.arange(n) % 2, 90)
+    ck = packed(torch, tb, c.x)
+    _, _, want = c.ref.backward(c.dy, ck.values(torch))
+    _, _, mag = c.ref.backward(c.dy, ck.values(torch), True)
+    u = [c.scale[k].double() * (ck.values(torch) @ c.a[k * rank:(k + 1) * rank].double().t()) for k in range(na)]
+    hit = torch.zeros(na, r, dtype=torch.bool, device="cuda")
+    for t, o, sign in ((0, 7, 1), (n - 1, 9, -1), (n - 2, 130, 1), (2, 130, 1)):
+        c.dy[t, o] = sign * math.inf
+        hit[t % 2, o] = True
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    db = c.db[:, :rank].reshape(na, r, rank)
+    assert torch.equal(db[0, 7].double(), torch.sign(u[0][0]) * math.inf)
+    assert torch.equal(db[1, 9].double(), -torch.sign(u[1][n - 1]) * math.inf)
+    two, first = torch.sign(u[0][n - 2]), torch.sign(u[0][2])
+    assert torch.equal(db[0, 130][two == first].double(), (two * math.inf)[two == first])
+    assert bool(torch.isnan(db[0, 130][two != first]).all())
+    check(torch, db[~hit], want[~hit], mag[~hit], n + d)
+
+
 def test_large_values_and_tokens_without_numbers(cuda, tblib):
     """u and v that round to an infinity in BF16 but are none count as what they are; tokens that are all NaN, and an
     adapter that is, cost no more time than others: the products' bounded waits do not run out."""
