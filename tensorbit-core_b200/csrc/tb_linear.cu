@@ -125,11 +125,16 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 constexpr long long kWaitCycles = 4000000000ll;
+// A role that passes over work which needs nothing of it waits at once for the next
+// that does.  Its limit grows with what lies between: so much for each slice (of
+// about 2^10 cycles).  The TMA warp beside it, which takes every slice,
+// has the plain limit and ends that wait if it gives up.
+constexpr long long kPassedCycles = 1 << 14;
 // False once that is over, or as soon as another role of the CTA has given up.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long passed = 0) {
     if (try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (clock64() - t0 < kWaitCycles) {
+    const long long t0 = clock64(), limit = kWaitCycles + passed * kPassedCycles;
+    while (clock64() - t0 < limit) {
         if (try_wait(bar, parity)) return true;
         if (abort_flag && *abort_flag) return false;
     }
@@ -1045,7 +1050,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
         } else if (C::kTails && warp >= kPrepWarp && warp < kTmaWarp) {
             // Zeros for the tokens behind the sample's end in both operands (either may hold anything there).
             const int pt = threadIdx.x - kPrepWarp * 32;
-            int it = 0;
+            int it = 0, waited = 0;  // slices so far, and at the last wait
             uint32_t phase = 0;  // a bit per stage, for its cut slices only
             const bool done = for_units<MODE>(P, [&](const Tile&, const Unit& u) {
                 return for_runs(u, [&](int, int i, int count) {
@@ -1053,7 +1058,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     const int last = u.hi - u.lo - (u.slices - 1) * 64;
                     if (i + count < u.slices || last == 64) return true;
                     const int s = (it - 1) % kStages;
-                    if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag)) return false;
+                    if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag, it - waited)) return false;
+                    waited = it;
                     phase ^= 1u << s;
                     uint8_t* stage = smem + s * C::kStage;  // two chunks of A, two of B, rows of 128 bytes
                     for (int q = pt; q < (64 - last) * 32; q += 128)
@@ -1070,7 +1076,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             // phase of that barrier.  (empty[s] cannot be waited on here: its parity says nothing to a waiter
             // that skips phases.)
             const int pt = threadIdx.x - kPrepWarp * 32;
-            int it = 0;
+            int it = 0, waited = 0;  // slices so far, and at the last wait
             uint32_t phase = 0;  // a bit per stage
             bool ok = true;
             for (int item = blockIdx.x >> 1; item < P.items && ok; item += gridDim.x >> 1) {
@@ -1085,7 +1091,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 for (int x = 0; x < u.extra; ++x, ++it) {
                     const int s = it % kStages, next = x + 1;
                     const int a = next < u.extra ? __ldg(u.list + 1 + next / u.rslices) : 0;
-                    if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag)) { ok = false; break; }
+                    if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag, it - waited)) { ok = false; break; }
+                    waited = it;
                     phase ^= 1u << s;
                     const bool odd = slice.build(smem + s * C::kStage, smem + s * C::kStage + C::kA, pt);
                     if (__any_sync(~0u, odd)) set_pair(odd_flag);

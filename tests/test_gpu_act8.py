@@ -472,6 +472,34 @@ def test_fisher_of_few_tiles_and_of_last_waves(cuda, tblib, n, r, d, S, first):
     assert torch.equal(F, again)
 
 
+def test_a_cut_slice_behind_seconds_of_whole_ones(cuda, tblib):
+    """65534 samples of 128 whole slices, then one that ends inside a slice: what cuts that slice waits for all the others,
+    several seconds, longer than a bounded wait for one slice lasts.  74 tiles, so that no sample is shared out, and
+    enough rows that the values are written out first.
+
+    All samples but the last have one gradient g, so the state is alpha (c g^2 + (1 - beta) g_last^2) with c = beta (1 -
+    beta) (1 + beta + ...) + beta^(S-1), whose sum is beta up to terms below 1e-280.  The additions' roundings: each is 2^-24
+    of the state so far, and those are F beta^(S-j), which add to F / (1 - beta) = 100 F."""
+    torch, tb = cuda, tblib
+    n, r, d, S, whole = 65536, 74 * 256, 256, 65535, 128 * 64
+    ck = packed(torch, tb, rows(torch, n, d, torch.float32, 50, heavy=0))
+    dy = rows(torch, n, r, torch.bfloat16, 51, r, 0.1, 0)
+    sp = torch.tensor([[0, whole]], device="cuda").repeat(S, 1)
+    sp[S - 1, 1] = whole + 37
+    F = torch.full((r, d), math.nan, device="cuda")
+    tb.check(tb.act8_fisher(ck.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), S, F.data_ptr()))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    xh, part = ck.values(torch), dy[:whole + 37].double()
+    g, last = part[:whole].t() @ xh[:whole], part.t() @ xh[:whole + 37]
+    mag = part.abs().t() @ xh[:whole + 37].abs()
+    want = 0.01 * (0.99 * g * g + 0.01 * last * last)
+    e = whole * 2.0 ** -23 * mag
+    bar = 0.01 * (2 * mag * e + e * e) + (100 + 8) * 2.0 ** -24 * want
+    assert bool(((F.double() - want).abs() <= bar).all())
+    assert float((F.double() - want).norm() / want.norm()) <= 2e-5  # 100 2^-24, and twice g's own 2e-6
+
+
 @pytest.mark.parametrize("n,r,d,S", [(2100, 2600, 2600, 1), (1100, 500, 1300, 9)])
 @pytest.mark.parametrize("g_t", ["float32", "bfloat16"])
 def test_gradients_of_last_waves(cuda, tblib, n, r, d, S, g_t):
