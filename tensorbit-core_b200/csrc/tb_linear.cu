@@ -417,7 +417,7 @@ __device__ __noinline__ void store_piece(const uint8_t* buf, void* out, long lon
         }
     } else {
 #pragma unroll 1
-        for (int at = 2 * lane; at < 2 * cols; at += 64) {
+        for (int at = 2 * lane; at < 2 * min(cols, Piece<BF16>::kCols); at += 64) {  // (`cols` may go on behind the piece)
 #pragma unroll 16
             for (int r = 0; r < 32; ++r) {
                 const uint16_t w = *reinterpret_cast<const uint16_t*>(buf + piece_at(r, at));
