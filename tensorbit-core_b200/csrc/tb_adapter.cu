@@ -132,6 +132,7 @@ struct Order {
     int* tokens;    // [n]
 };
 constexpr int kSmallBatch = 1024;
+constexpr int kFewTokens = 32;  // at most, of few_tokens_kernel
 
 __global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o, int32_t* __restrict__ lists) {
     __shared__ int scan[32], total[2], who[256];
@@ -334,7 +335,8 @@ down_small_kernel(const Args g, const int passes, float* __restrict__ first, flo
     __shared__ float red[8][16][8 * NT];
     __shared__ int who[256];
     const int p = blockIdx.z % passes;
-    asm volatile("griddepcontrol.launch_dependents;");  // few_tokens_kernel waits before it reads u
+    // Only where few_tokens_kernel follows, which waits before it reads u (see launch_pdl's contract).
+    if (!BACKWARD && g.n <= kFewTokens) asm volatile("griddepcontrol.launch_dependents;");
     if constexpr (!BACKWARD) {
         down_small<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, first, red, who, passes, p);
     } else {
@@ -708,8 +710,6 @@ __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const flo
         g.y[t * g.ldy + o] = __float2bfloat16_rn(y);
     }
 }
-constexpr int kFewTokens = 32;
-
 template <int NT>
 cudaError_t launch_few(const Args& g, const float* u, cudaStream_t st) {
     // Without adapters the kernel before this one is the caller's, which may still be writing x when it lets go.

@@ -8,9 +8,17 @@
 // and only then reads or writes global memory.  A kernel launched without the
 // attribute returns from pdl_wait() at once.
 //
-// No kernel issues griddepcontrol.launch_dependents: its successor is released
-// only when it exits.  With the trigger issued right after pdl_wait() in every
-// kernel (successors resident early), the exact-OBS chain of a 14336-wide
+// No kernel but one issues griddepcontrol.launch_dependents: its successor is
+// released only when it exits.  The exception is down_small_kernel of the
+// adapters, and it only where few_tokens_kernel is the next launch: that one's
+// reads before its pdl_wait() are of x, W, b and the tokens' adapters, which
+// nothing writes between the ordinary launch of down_small_kernel, itself behind
+// everything that wrote them, and its own end; what down_small_kernel writes, u,
+// it reads behind the wait and through L2 (__ldcg), not the read-only path.  A
+// kernel that does not keep to both may not follow one that triggers.
+//
+// Elsewhere the trigger is left out.  With it issued right after pdl_wait() in
+// every kernel (successors resident early), the exact-OBS chain of a 14336-wide
 // layer gave results that differed from run to run on B200, some with a failed
 // Cholesky pivot, although every event and stream ordering of the schedule
 // checks out.  The edge the trigger breaks is a cache contract, not an
