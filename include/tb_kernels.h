@@ -339,7 +339,7 @@ int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, vo
 typedef struct tb_adapter_args {
     uint32_t struct_size;  /* sizeof(tb_adapter_args)                                    */
     int32_t  dtype;        /* of w, a, b, x, y, dy, dx, da, db: TB_BF16                  */
-    int64_t  n;            /* tokens, below 2^31 - 256                                   */
+    int64_t  n;            /* tokens, up to 2^31 - 65537                                 */
     int32_t  d, r;         /* in and out features, each up to 2^31 - 256                 */
     int32_t  rank;         /* 1..128                                                     */
     int32_t  n_adapters;   /* 0: the projection alone                                    */

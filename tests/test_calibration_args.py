@@ -116,3 +116,12 @@ def test_features_that_tiles_cannot_count_are_refused(tblib, many):
     for kw in (dict(d=many, ldw=ld, lda=ld, ldx=ld), dict(r=many, ldy=ld, lddy=ld)):
         assert tb.adapter_forward(adapters(**kw)) == tb.TB_ERR_SHAPE
         assert tb.adapter_backward(adapters(dy=P, lddy=ld, dx=P, lddx=ld, **{k: v for k, v in kw.items() if k != "lddy"})) == tb.TB_ERR_SHAPE
+
+
+def test_adapters_refuse_tokens_beyond_their_limit(tblib):
+    """The largest batch is 2^31 - 65537 tokens, as the header states."""
+    text = open(tb.HEADER).read()
+    assert "tokens, up to 2^31 - 65537 " in text[text.index("typedef struct tb_adapter_args"):]
+    for n in ((1 << 31) - 65536, (1 << 31) - 256, 1 << 31):
+        assert tb.adapter_forward(adapters(n=n)) == tb.TB_ERR_SHAPE
+        assert tb.adapter_backward(adapters(n=n, dy=P, lddy=32, dx=P, lddx=64)) == tb.TB_ERR_SHAPE
