@@ -269,7 +269,9 @@ int tb_obs_sparsegpt_phase_times(float* ms_out, int n);
  * checkpoint below is the exact product of xhat.  A NaN or an infinity in a
  * block's kept tokens sets E = 255 and all its codes 0: the whole block of
  * that feature reads back as NaN.  Other E are 1..249; checkpoints written by
- * other means keep to both. */
+ * other means keep to both.  Where a block's largest magnitude reaches 255 * 2^120
+ * (BF16's largest value), E is 249, and its values from 254 * 2^120 on round to
+ * 2^128: they read back, and count in every product below, as infinities. */
 #define TB_ACT8_BLOCK 128
 typedef struct tb_act8 {
     uint32_t struct_size;  /* sizeof(tb_act8)                                          */

@@ -93,6 +93,24 @@ def test_pack_borders(cuda, tblib):
     assert torch.equal(c.codes[:3, : len(vals)], q) and torch.equal(c.exps[:, : len(vals)], e)
 
 
+def test_values_that_round_beyond_the_range_read_back_as_infinities(cuda, tblib):
+    """A block that reaches 255 * 2^120 has steps of 2^122: from 254 * 2^120 on its values round to 2^128.  One below keeps
+    all its values finite."""
+    torch, tb = cuda, tblib
+    x = torch.zeros(4, 3, device="cuda")
+    x[:, 0] = torch.tensor([255 * 2.0 ** 120, -254 * 2.0 ** 120, 253.9 * 2.0 ** 120, 2.0 ** 121], device="cuda")
+    x[:, 1] = torch.tensor([-254.9 * 2.0 ** 120, 254 * 2.0 ** 120, 2.0 ** 119, 0.0], device="cuda")
+    x[:, 2] = torch.finfo(torch.bfloat16).min
+    c = packed(torch, tb, x)
+    assert c.exps[0, :3].tolist() == [249, 248, 249]
+    for dt in (torch.float32, torch.bfloat16):
+        out = torch.empty(4, 3, device="cuda", dtype=dt)
+        tb.check(tb.act8_unpack(c.s, out.data_ptr(), code(tb, torch, dt), 3))
+        assert out[:, 0].tolist() == [math.inf, -math.inf, 63 * 2.0 ** 122, 0.0]  # 2^121: half a step, to even
+        assert out[:, 1].tolist() == [-127 * 2.0 ** 121, 127 * 2.0 ** 121, 0.0, 0.0]
+        assert bool((out[:, 2] == -math.inf).all())
+
+
 def test_padding_and_values_that_are_no_numbers(cuda, tblib):
     torch, tb = cuda, tblib
     n, d = 300, 40
