@@ -298,19 +298,22 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * dy [n][lddy] is of dy_dtype.  samples: device array of S (begin, end) token
  * pairs, clamped to [0, n], in any order, overlapping or not; NULL means one
  * sample of all tokens (S = 1).  An empty sample's gradient is zero; tokens of
- * no sample are not read into any.  Sums are in FP32 and every product is
- * exact: FP32 (F16) dy is split into three (two) BF16 parts, in scratch of
- * 6 (4) bytes per value from the library's per-device pool; rows of a BF16 dy
- * that are not 16-byte aligned are first copied to such scratch.  Large products
- * with r beyond 1024 (F16: 512, FP32: 256) write xhat out there as BF16, 2 bytes
- * per value, unless that is more than 2 GiB.  Where the gradients' 256 x 256
- * tiles do not fill the GPU's last wave, FP32 shares of their sums also wait
- * there, at most 148 tiles (39 MB). */
+ * no sample are not read into any.  Sums are in FP32: up to 512 tokens in the
+ * tensor core, whose additions cut off instead of rounding (2.6e-7 of the sum
+ * where all terms have one sign), and those added with rounding.  Every product
+ * is exact: FP32 (F16) dy is split into three (two) BF16 parts, but for bits
+ * below 2^-133, in scratch of 6 (4) bytes per value from the library's per-device
+ * pool; rows of a BF16 dy that are not 16-byte aligned are first copied to such
+ * scratch.  Large products with r beyond 1024 (F16: 512, FP32: 256) write xhat out
+ * there as BF16, 2 bytes per value, unless that is more than 2 GiB.  Where the
+ * gradients' 256 x 256 tiles do not fill the GPU's last wave, FP32 shares of their
+ * sums also wait there, at most 148 tiles (39 MB). */
 int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
                         const int64_t* samples, int S, void* grads, int g_dtype, int64_t g_stride, void* stream);
 /* The Fisher state after one EHAPPruner::accumulate_fisher step (ehap.hpp:
  * 148-201) per sample, in their order, without the gradients in memory: with
- * G_s as above in FP32, the first step (first_step != 0, F not read) gives
+ * G_s as above in FP32 (groups of 256 tokens where a sample has more than 1024,
+ * for F16 dy 512, for FP32 320), the first step (first_step != 0, F not read) gives
  * F = alpha g^2, the others F = beta F + alpha (1 - beta) g^2.  Formed, as
  * tb_fisher_weighted_sum does, as the sum of the samples' g^2 with the factors
  * that these steps give them (in double, rounded to FP32 once): it agrees with

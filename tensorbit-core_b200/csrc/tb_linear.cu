@@ -57,6 +57,8 @@ constexpr int kEpiWarps = 8, kPrepWarp = 8, kTmaWarp = 12, kMmaWarp = 13;
 // in any case: TMA loads can complete out of order.)
 constexpr int kDecodeWarps = 6;
 
+constexpr int kGradGroup = 8;  // slices that kGrad sums in TMEM
+
 template <int MODE>
 struct Cfg {
     static constexpr bool kCodes = MODE == kGrad || MODE == kFisher;   // B decoded from codes here
@@ -69,7 +71,7 @@ struct Cfg {
     static constexpr int kCols = NB / 2;                               // columns of an epilogue warp, and of a CTA's B
     // K slices summed in TMEM before they are added in FP32: 512 tokens (kGrad), one block of codes
     // (kHess), all (16-bit results).  kFisher: see kDirect.
-    static constexpr int kGroup = kind(MODE) == kGrad ? 8 : kind(MODE) == kFisher ? 4 : MODE == kHess ? 1 : 1 << 30;
+    static constexpr int kGroup = kind(MODE) == kGrad ? kGradGroup : kind(MODE) == kFisher ? 4 : MODE == kHess ? 1 : 1 << 30;
     static constexpr int kA = 16384;                                   // 128 rows x 128 bytes of K (or 128 int8 tokens)
     static constexpr int kB = kCols * 128;
     static constexpr int kRaw = kCodes ? 64 * kCols : 0;               // codes of the slice
@@ -196,6 +198,17 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
+// Eight columns of each of two accumulators, waited for.
+__device__ __forceinline__ void tmem_ld8x2(uint32_t from0, uint32_t from1, uint32_t (&x)[8], uint32_t (&y)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3]), "=&r"(x[4]), "=&r"(x[5]), "=&r"(x[6]), "=&r"(x[7]),
+          "=&r"(y[0]), "=&r"(y[1]), "=&r"(y[2]), "=&r"(y[3]), "=&r"(y[4]), "=&r"(y[5]), "=&r"(y[6]), "=&r"(y[7])
+        : "r"(from0), "r"(from1)
+        : "memory");
+}
 // Two lanes of a += v, and of a += (m * row + base) * col, in packed FP32 (round to nearest).
 __device__ __forceinline__ void add2(float& a0, float& a1, uint32_t v0, uint32_t v1) {
     asm("{\n\t.reg .b64 A, V;\n\tmov.b64 A, {%0, %1};\n\tmov.b64 V, {%2, %3};\n\t"
@@ -223,11 +236,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // kFisher has the Fisher state in the registers that would add a sample's groups
-// up.  A sample of at most kDirect slices (1024 tokens of BF16 dy) is summed in
-// TMEM alone: the tensor core's truncated additions then leave a relative 1e-7 in
-// g where signs are mixed, as an FP32 product's rounding does, and at most
-// 64 2^-24 where all terms have one sign.  For a longer one the state waits in
-// its place in memory, once, while groups of 256 tokens are added in FP32.
+// up.  A sample of at most kDirect slices over all parts comes out of TMEM whole:
+// one sum where that is at most kGradGroup slices of tokens, as in a group of kGrad,
+// else (more than 512 tokens of BF16 dy) two, in both accumulators, added as they are
+// read.  Each of a slice's four steps cuts off less than 2^-23 of the sum so far; the
+// parts before the leading one count little.  (Of g^2, 2-norm against float64, 1000
+// tokens with terms of one sign: 1.5e-6 in one sum, 5e-7 in two, 2e-7 where signs
+// are mixed.)  For a longer one the state waits in its place in memory, once, while
+// groups of 256 tokens are added in FP32.
 constexpr int kDirect = 16;
 
 // ---- the walk over work items, units (one sum each) and K slices that every role shares ----
@@ -293,7 +309,7 @@ __device__ __forceinline__ Unit unit_of(const Params& P, const Tile& t, int s) {
         }
         u.slices = u.hi > u.begin ? (u.hi - u.lo + 63) / 64 : 0;
         u.total = u.slices * P.parts;
-        if (kind(MODE) == kFisher && u.total <= kDirect) u.group = kDirect;
+        if (kind(MODE) == kFisher && u.total <= kDirect) u.group = u.slices <= kGradGroup ? kDirect : kGradGroup;
         if (kind(MODE) != kFisher && t.splits > 1) {
             u.first = share_begin(u.slices * P.parts, t.q, t.splits);
             u.total = share_begin(u.slices * P.parts, t.q + 1, t.splits) - u.first;
@@ -778,6 +794,32 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                                 square_add2(old[i], old[i + 1], factor2, F[32 * c + i], F[32 * c + i + 1]);
                                 F[32 * c + i] = old[i];
                                 F[32 * c + i + 1] = old[i + 1];
+                            }
+                        }
+                    } else if (u.total > u.group) {  // two sums, one in each accumulator
+                        const int b = ac.s;
+                        if (!wait(smem_u32(&accfull[b]), ac.phase, abort_flag)) { ok = false; break; }
+                        ac.next();
+                        if (!wait(smem_u32(&accfull[b ^ 1]), ac.phase, abort_flag)) { ok = false; break; }
+                        ac.next();
+                        fence_after();
+#pragma unroll
+                        for (int c = 0; c < COLS / 8; ++c) {
+                            uint32_t x[8], y[8];
+                            tmem_ld8x2(lane_base + static_cast<uint32_t>(b * NB + 8 * c), lane_base + static_cast<uint32_t>((b ^ 1) * NB + 8 * c), x, y);
+                            if (c + 1 == COLS / 8) {
+                                fence_before();
+                                __syncwarp();
+                                if (lane == 0) {
+                                    arrive_even(smem_u32(&accempty[0]));
+                                    arrive_even(smem_u32(&accempty[1]));
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; i += 2) {
+                                float g0 = __uint_as_float(x[i]), g1 = __uint_as_float(x[i + 1]);
+                                add2(g0, g1, y[i], y[i + 1]);
+                                square_add2(F[c * 8 + i], F[c * 8 + i + 1], factor2, g0, g1);
                             }
                         }
                     } else {

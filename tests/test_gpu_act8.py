@@ -276,6 +276,25 @@ def test_fisher(cuda, tblib, n, r, d, dy_t, S, first):
     assert float((F.double() - want).norm() / want.norm()) <= 4e-6
 
 
+@pytest.mark.parametrize("n", [500, 513, 1000, 1024])
+@pytest.mark.parametrize("d", [256, 512])
+def test_fisher_of_terms_of_one_sign(cuda, tblib, n, d):
+    """The tensor core cuts its sums off, which terms of one sign do not even out.  Fisher's g are the very sums that the
+    gradients are, groups of 512 tokens (32 steps) added in FP32: a step cuts off half of 2^-23 of the sum so far on
+    average, and those are half the group's on average, so g loses at most 32 2^-25 of itself, and a rounding.  (74 and
+    148 tiles, so that neither call shares a sum out; with 512 features the values are written out first.)"""
+    torch, tb = cuda, tblib
+    r = 74 * 256
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 1, heavy=0).abs())
+    dy = rows(torch, n, r, torch.bfloat16, 2, r, 1e-2, 0).abs()
+    F, G = torch.empty(r, d, device="cuda"), torch.empty(r, d, device="cuda")
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, r, r, None, 1, F.data_ptr(), alpha=1.0))
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, r, r, None, 1, G.data_ptr(), tb.F32))
+    assert torch.equal(F, G * G)
+    want = dy.double().t() @ c.values(torch)
+    assert float((G.double() - want).norm() / want.norm()) <= 32 * 2.0 ** -25 + 2.0 ** -24
+
+
 def test_fisher_equals_its_steps(cuda, tblib):
     """One fused call and tb_fisher_ema_step over the FP32 gradients of the same call's family agree to rounding of g."""
     torch, tb = cuda, tblib
