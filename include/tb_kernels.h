@@ -296,8 +296,9 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * tb_fisher_ema_step read.  TB_F16 is TB_ERR_UNSUPPORTED: the passes that read
  * F16 gradients decode subnormals as the reference does, not as IEEE values.
  * dy [n][lddy] is of dy_dtype.  samples: device array of S (begin, end) token
- * pairs, clamped to [0, n], in any order, overlapping or not; NULL means one
- * sample of all tokens (S = 1).  An empty sample's gradient is zero; tokens of
+ * pairs, S at most 65535, clamped to [0, n], in any order, overlapping or not;
+ * NULL means one sample of all tokens (S = 1).  n times the parts of dy (below)
+ * ends at 2^31 - 65 (TB_ERR_CAPACITY).  An empty sample's gradient is zero; tokens of
  * no sample are not read into any.  Sums are in FP32: up to 512 tokens in the
  * tensor core, whose additions cut off instead of rounding (2.6e-7 of the sum
  * where all terms have one sign), and those added with rounding.  Every product

@@ -125,3 +125,12 @@ def test_adapters_refuse_tokens_beyond_their_limit(tblib):
     for n in ((1 << 31) - 65536, (1 << 31) - 256, 1 << 31):
         assert tb.adapter_forward(adapters(n=n)) == tb.TB_ERR_SHAPE
         assert tb.adapter_backward(adapters(n=n, dy=P, lddy=32, dx=P, lddx=64)) == tb.TB_ERR_SHAPE
+
+
+def test_samples_end_at_their_limit(tblib):
+    """At most 65535 samples in a call, as the header states."""
+    text = open(tb.HEADER).read()
+    assert "S at most 65535" in text[text.index("Weight gradients of y"):text.index("int tb_act8_weight_grad")]
+    c = ck()
+    assert tb.act8_weight_grad(c, P, tb.BF16, 64, 64, P, 65536, P, tb.F32) == tb.TB_ERR_ARG
+    assert tb.act8_fisher(c, P, tb.BF16, 64, 64, P, 65536, P) == tb.TB_ERR_ARG
