@@ -100,5 +100,16 @@ inline EncodeFn encode_fn() {
     return fn;
 }
 
+// The encoding fails without a current driver context.  A host thread has one only
+// after a runtime call that binds its current device's, which the first entry that a
+// thread calls may not have made.
+template <typename... Args>
+CUresult encode_tiled(EncodeFn fn, Args... args) {
+    const CUresult r = fn(args...);
+    int dev = 0;
+    if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return r;
+    return fn(args...);
+}
+
 }  // namespace umma
 }  // namespace tb

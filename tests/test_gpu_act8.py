@@ -593,3 +593,40 @@ def test_samples_of_many_rows_leave_other_tokens_out(cuda, tblib, dy_t, d):
     tb.check(tb.act8_weight_grad(ck.s, dy.data_ptr(), code(tb, torch, dy.dtype), dy.stride(0), r, sp.data_ptr(), 4, G.data_ptr(), tb.F32))
     assert not bool(torch.isnan(G[0][:, :7]).any()) and bool(torch.isnan(G[1][:, 7]).all()) and bool(torch.isnan(G[3][:, 7]).all())
     assert int(torch.isnan(G).sum()) == sum(r for a, b in samples if a < 256 and b > 128)
+
+
+def test_first_call_of_a_host_thread(cuda, tblib):
+    """A thread that has made no CUDA call before: every entry that encodes tensor maps, among them products that allocate no
+    scratch first (an aligned BF16 dy, 74 or fewer tiles of one K step; adapters' forward without adapters; a GEMM)."""
+    import threading
+    torch, tb = cuda, tblib
+    c = packed(torch, tb, rows(torch, 64, 256, torch.float32, 100))
+    dy = rows(torch, 64, 256, torch.bfloat16, 101, None, 0.1, 0)
+    x, w = rows(torch, 64, 256, torch.bfloat16, 102, heavy=0), rows(torch, 256, 256, torch.bfloat16, 103, None, 0.05, 0)
+    outs = [torch.empty(256, 256, device="cuda") for _ in range(4)] + [torch.empty(64, 256, device="cuda", dtype=torch.bfloat16)]
+    G, F, H, P, y = outs
+    calls = [
+        lambda: tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, 256, 256, None, 1, G.data_ptr(), tb.F32),
+        lambda: tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, 256, 256, None, 1, F.data_ptr()),
+        lambda: tb.act8_hessian(c.s, 1.0, H.data_ptr()),
+        lambda: tb.lib().tb_gemm_nt_bf16(w.data_ptr(), 256, w.data_ptr(), 256, 256, 256, 256, 1.0, 0.0, None, 0, P.data_ptr(), 256, 0, None),
+        lambda: tb.adapter_forward(tb.adapter_args(n=64, d=256, r=256, rank=0, n_adapters=0, w=w.data_ptr(), ldw=256,
+                                                   x=x.data_ptr(), ldx=256, y=y.data_ptr(), ldy=256))]
+
+    def all_outs():
+        torch.cuda.synchronize()
+        return [torch.tril(t) if t is H else t.clone() for t in outs]
+
+    for f in calls:
+        tb.check(f())
+    want = all_outs()
+    for t in outs:
+        t.zero_()
+    torch.cuda.synchronize()
+    codes = []
+    for f in calls:
+        t = threading.Thread(target=lambda: codes.append(f()))
+        t.start()
+        t.join()
+    assert codes == [tb.TB_OK] * len(calls)
+    assert all(torch.equal(a, b) for a, b in zip(all_outs(), want))
