@@ -630,3 +630,189 @@ def test_first_call_of_a_host_thread(cuda, tblib):
         t.join()
     assert codes == [tb.TB_OK] * len(calls)
     assert all(torch.equal(a, b) for a, b in zip(all_outs(), want))
+
+
+@pytest.mark.parametrize("r,d,first", [(264, 264, True), (1300, 300, False), (256, 74 * 256, False), (74 * 256, 256, True)])
+def test_fisher_of_more_samples_than_factors_are_kept(cuda, tblib, r, d, first):
+    """1500 samples, factors from the 1025th on formed as they are needed: shared out over blocks or not (74 tiles), from
+    codes or from values written out first (1300 and 18944 rows).  The bars of test_fisher; the state's additions are
+    2^-24 of the state so far, and those are F beta^(S-j), which add to 100 F."""
+    torch, tb = cuda, tblib
+    n, S = 3000, 1500
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 60, heavy=0))
+    dy = rows(torch, n, r, torch.bfloat16, 61, ref.up(r, 8), 0.1, 0)
+    samples = [(2 * i, 2 * i + 2) for i in range(S - 1)] + [(700, 1100)]
+    F = torch.full((r, d), math.nan, device="cuda") if first else torch.rand(r, d, device="cuda")
+    want = None if first else F.double()
+    mag = torch.zeros(r, d, device="cuda", dtype=torch.float64)
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, pairs(torch, samples).data_ptr(), S, F.data_ptr(),
+                            first_step=first))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    xh, dyd = c.values(torch), dy.double()
+    for a, b in samples:
+        g = dyd[a:b].t() @ xh[a:b]
+        e = (b - a) * 2.0 ** -23 * (dyd[a:b].abs().t() @ xh[a:b].abs())
+        w = 0.01 if want is None else 0.01 * 0.01
+        want = w * g * g if want is None else want.mul_(0.99).addcmul_(g, g, value=w)
+        mag.mul_(0.99).add_(2 * g.abs() * e + e * e, alpha=w)
+    bar = mag + (100 + 8) * 2.0 ** -24 * want
+    assert bool(((F.double() - want).abs() <= bar * 1.01 + 1e-40).all())
+    assert float((F.double() - want).norm() / want.norm()) <= 4e-6 + (100 + 8) * 2.0 ** -24
+
+
+def test_values_beyond_their_scratch_are_decoded_in_the_product(cuda, tblib):
+    """140000 tokens of 8192 features are more than 2 GiB as BF16: 1300 rows of gradients read the codes all the same."""
+    torch, tb = cuda, tblib
+    n, d, r, m = 140000, 8192, 1300, 333
+    c = Checkpoint(torch, tb, n, d)
+    c.codes.zero_()
+    c.exps.fill_(1)
+    dy = torch.zeros(n, ref.up(r, 8), device="cuda", dtype=torch.bfloat16)[:, :r]
+    at = [(128 * 50 + 3, 128 * 50 + 3 + m), (n - m, n)]
+    for i, (a, b) in enumerate(at):
+        x = rows(torch, 512, d, torch.float32, 70 + i, heavy=0)
+        q, e = ref.pack(torch, x)
+        lo, k = a // 128 * 128, min(512, n - a // 128 * 128)
+        c.codes[lo:lo + k] = q[:k]
+        c.exps[lo // 128:lo // 128 + -(-k // 128)] = e[:-(-k // 128)]
+        dy[a:b] = rows(torch, m, r, torch.bfloat16, 72 + i, None, 0.1, 0)
+    G, F = torch.empty(2, r, d, device="cuda"), torch.empty(r, d, device="cuda")
+    sp = pairs(torch, at)
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), 2, G.data_ptr(), tb.F32))
+    tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), 2, F.data_ptr()))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    grads = []
+    for s, (a, b) in enumerate(at):
+        lo = a // 128 * 128
+        xh = ref.values(torch, c.codes[lo:b], c.exps[lo // 128:])[a - lo:]
+        g, A = dy[a:b].double().t() @ xh, dy[a:b].double().abs().t() @ xh.abs()
+        check_sums(torch, G[s], g, A, m)
+        grads.append(g)
+    want = ref.fisher(torch, grads, 0.01, 0.99)
+    assert float((F.double() - want).norm() / want.norm()) <= 4e-6
+
+
+def test_hessian_of_more_tiles_than_a_grid_has_rows(cuda, tblib):
+    """92417 features, whose rows of H do not start on 16 bytes: all 65703 tiles of 256 x 256 go through scratch and are
+    written by a second kernel in two launches.  Spot rows; what is above the diagonal stays."""
+    torch, tb = cuda, tblib
+    n, d = 3, 361 * 256 + 1
+    c = packed(torch, tb, rows(torch, n, d, torch.float32, 80))
+    H = torch.full((d, d), 7.0, device="cuda")
+    tb.check(tb.act8_hessian(c.s, 0.5, H.data_ptr()))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    xh = c.values(torch)
+    for i in (0, 127, 128, 255, 256, 40000, 65535, 92159, 92160, 92415, 92416):
+        k = min(d, i // 128 * 128 + 128)
+        want, mag = 0.5 * xh[:, i] @ xh[:, :k], 0.5 * xh[:, i].abs() @ xh[:, :k].abs()
+        assert bool(((H[i, :k].double() - want).abs() <= (n + 3) * 2.0 ** -23 * mag).all())
+        assert bool((H[i, k:] == 7).all())
+
+
+def test_two_host_threads(cuda, tblib):
+    """Calls from two threads at once, each on a stream of its own, give what the same calls give one behind another."""
+    import threading
+    torch, tb = cuda, tblib
+    n, d = 700, 520
+    work = []
+    for i in range(2):
+        r = (264, 1500)[i]  # the latter's values are written out first
+        c = packed(torch, tb, rows(torch, n, d, torch.float32, 90 + i))
+        dy = rows(torch, n, r, torch.bfloat16, 92 + i, ref.up(r, 8), 0.1, 0)
+        sp = pairs(torch, [(j * n // 40, (j + 1) * n // 40) for j in range(40)])
+        out = [torch.zeros(40, r, d, device="cuda"), torch.zeros(r, d, device="cuda"), torch.zeros(d, d, device="cuda"),
+               torch.zeros(n, d, device="cuda", dtype=torch.bfloat16), torch.zeros(n, r, device="cuda", dtype=torch.bfloat16)]
+        w = rows(torch, r, d, torch.bfloat16, 94 + i, None, 0.05, 0)
+        a, b = rows(torch, 16, d, torch.bfloat16, 96, None, 0.05, 0), rows(torch, 2 * r, 8, torch.bfloat16, 97, None, 0.3, 0)
+        who = (torch.arange(n, device="cuda") % 3 - 1).to(torch.int32)
+        work.append((r, c, dy, sp, out, w, a, b, who, torch.ones(2, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def go(k):
+        r, c, dy, sp, (G, F, H, X, Y), w, a, b, who, scale, st = work[k]
+        s = st.cuda_stream
+        tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), 40, G.data_ptr(), tb.F32, stream=s))
+        tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.BF16, dy.stride(0), r, sp.data_ptr(), 40, F.data_ptr(), stream=s))
+        tb.check(tb.act8_hessian(c.s, 1.0, H.data_ptr(), stream=s))
+        tb.check(tb.act8_unpack(c.s, X.data_ptr(), tb.BF16, d, stream=s))
+        for m in (20, n):
+            tb.check(tb.adapter_forward(tb.adapter_args(
+                n=m, d=d, r=r, rank=8, n_adapters=2, w=w.data_ptr(), ldw=d, a=a.data_ptr(), lda=d, b=b.data_ptr(), ldb=8,
+                scale=scale.data_ptr(), token_adapter=who.data_ptr(), x=X.data_ptr(), ldx=d, y=Y.data_ptr(), ldy=r), stream=s))
+
+    want = []
+    for k in (0, 1):
+        go(k)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in work[k][4]])
+    failed = []
+
+    def loop(k):
+        try:
+            for _ in range(30):
+                go(k)
+            work[k][10].synchronize()
+        except Exception as e:  # (handed to the test's own thread)
+            failed.append(e)
+
+    for _ in range(3):
+        for k in (0, 1):
+            for t in work[k][4]:
+                t.zero_()
+        torch.cuda.synchronize()
+        threads = [threading.Thread(target=loop, args=(k,)) for k in (0, 1)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not failed, failed
+        assert all(torch.equal(x, y) for k in (0, 1) for x, y in zip(work[k][4], want[k]))
+    tb.check(tb.lib().tb_gemm_status(None))
+
+
+def test_values_written_out_first_under_graphs(cuda, tblib):
+    """Two captured graphs whose calls write their values to scratch first, replayed on two streams at once with new sample
+    bounds and new dy, against single calls."""
+    torch, tb = cuda, tblib
+    n, r, d, S = 900, 1400, 1300, 4
+    sets, graphs = [], []
+    for i in range(2):
+        c = packed(torch, tb, rows(torch, n, d, torch.float32, 110 + i))
+        dy = rows(torch, n, r, torch.float32, 112 + i, r, 1e-2, 0)
+        sp = pairs(torch, [(j * 200, j * 200 + 190 + i) for j in range(S)])
+        sets.append((c, dy, sp, torch.empty(S, r, d, device="cuda"), torch.empty(r, d, device="cuda")))
+
+    def go(k, stream=None):
+        c, dy, sp, G, F = sets[k]
+        tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.F32, r, r, sp.data_ptr(), S, G.data_ptr(), tb.F32, stream=stream))
+        tb.check(tb.act8_fisher(c.s, dy.data_ptr(), tb.F32, r, r, sp.data_ptr(), S, F.data_ptr(), stream=stream))
+
+    for k in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            go(k, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for t in range(3):
+        for k, (c, dy, sp, G, F) in enumerate(sets):
+            dy.copy_(rows(torch, n, r, torch.float32, 120 + 2 * t + k, r, 1e-2, 0))
+            sp.copy_(pairs(torch, [(j * 210 + t, j * 210 + 130 + 9 * t + k) for j in range(S)]))
+            G.fill_(-1.0)
+            F.fill_(-1.0)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        got = [(G.clone(), F.clone()) for _, _, _, G, F in sets]
+        for k in (0, 1):
+            go(k)
+            torch.cuda.synchronize()
+            assert torch.equal(got[k][0], sets[k][3]) and torch.equal(got[k][1], sets[k][4])
+            xh = sets[k][0].values(torch)
+            for s, (G, A) in enumerate(ref.gradients(torch, sets[k][1], xh, sets[k][2].tolist())):
+                check_sums(torch, got[k][0][s], G, A, 200 * 3)
