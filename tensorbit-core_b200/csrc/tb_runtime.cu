@@ -74,6 +74,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();  // reported here: the next launch's check must not find it again
     return fail(TB_ERR_CUDA, "%s: %s (%d)", what, cudaGetErrorString(e), static_cast<int>(e));
 }
 

@@ -816,3 +816,16 @@ def test_values_written_out_first_under_graphs(cuda, tblib):
             xh = sets[k][0].values(torch)
             for s, (G, A) in enumerate(ref.gradients(torch, sets[k][1], xh, sets[k][2].tolist())):
                 check_sums(torch, got[k][0][s], G, A, 200 * 3)
+
+
+def test_scratch_that_cannot_be_had_fails_its_call_alone(cuda, tblib):
+    """A call whose scratch (here 2 PB) is refused by the allocator returns before any launch; the next call is fine."""
+    torch, tb = cuda, tblib
+    c = packed(torch, tb, rows(torch, 40, 64, torch.float32, 130))
+    unread = torch.zeros(64, device="cuda", dtype=torch.uint8).data_ptr()
+    big = tb.act8(n=1 << 30, d=16, codes=unread, ldq=16, exps=unread, lde=16)
+    assert tb.act8_weight_grad(big, unread + 2, tb.BF16, 1 << 20, 1 << 20, None, 1, unread, tb.F32) == tb.TB_ERR_CUDA
+    assert b"memory" in tb.lib().tb_last_error()
+    out = torch.zeros(40, 64, device="cuda")
+    assert tb.act8_unpack(c.s, out.data_ptr(), tb.F32, 64) == tb.TB_OK
+    assert torch.equal(out.double(), c.values(torch))
