@@ -45,11 +45,15 @@ int scratch_alloc(void** ptr, size_t bytes, cudaStream_t stream) {
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;
             props.location.id = dev;
+            // The first call may be one that a stream captures.  Making the pool is no stream's
+            // work: this thread lets it through for as long as that takes.
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaThreadExchangeStreamCaptureMode(&mode);
             cudaError_t e = cudaMemPoolCreate(&pool, &props);
-            if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolCreate(scratch)");
             uint64_t keep = UINT64_MAX;
-            e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
-            if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolSetAttribute(scratch)");
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return cuda_fail(e, "scratch pool");
             g_pools[dev] = pool;
         } else {
             pool = it->second;

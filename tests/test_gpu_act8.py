@@ -829,3 +829,50 @@ def test_scratch_that_cannot_be_had_fails_its_call_alone(cuda, tblib):
     out = torch.zeros(40, 64, device="cuda")
     assert tb.act8_unpack(c.s, out.data_ptr(), tb.F32, 64) == tb.TB_OK
     assert torch.equal(out.double(), c.values(torch))
+
+
+FIRST_CALL_CAPTURED = """
+import sys
+import torch
+import tbabi as tb
+n, d, r, what = 700, 512, 256, sys.argv[1]
+g = torch.Generator(device="cuda").manual_seed(1)
+codes = torch.randint(-127, 128, (n, d), device="cuda", generator=g, dtype=torch.int8)
+exps = torch.full((6, d), 120, device="cuda", dtype=torch.uint8)
+ck = tb.act8(n=n, d=d, codes=codes.data_ptr(), ldq=d, exps=exps.data_ptr(), lde=d)
+half = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+x, w, a, b = half(n, d), half(r, d), half(16, d), half(2 * r, 8)
+dy, G, H = torch.randn(n, r, device="cuda", generator=g), torch.zeros(r, d, device="cuda"), torch.zeros(d, d, device="cuda")
+who, scale = torch.zeros(n, device="cuda", dtype=torch.int32), torch.ones(2, device="cuda")
+y = torch.zeros(n, r, device="cuda", dtype=torch.bfloat16)
+def go():
+    s = torch.cuda.current_stream().cuda_stream
+    if what == "gradient":
+        tb.check(tb.act8_weight_grad(ck, dy.data_ptr(), tb.F32, r, r, None, 1, G.data_ptr(), tb.F32, stream=s))
+    elif what == "hessian":
+        tb.check(tb.act8_hessian(ck, 1.0, H.data_ptr(), stream=s))
+    else:
+        tb.check(tb.adapter_forward(tb.adapter_args(n=int(what), d=d, r=r, rank=8, n_adapters=2, w=w.data_ptr(), ldw=d, a=a.data_ptr(),
+            lda=d, b=b.data_ptr(), ldb=8, scale=scale.data_ptr(), token_adapter=who.data_ptr(), x=x.data_ptr(), ldx=d,
+            y=y.data_ptr(), ldy=r), stream=s))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    go()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (G, H, y)]
+go()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, (G, H, y))) and any(bool(t.any()) for t in got)
+"""
+
+
+@pytest.mark.parametrize("what", ["gradient", "hessian", "20", "700"])
+def test_a_process_first_call_may_be_captured(cuda, tblib, what):
+    """In a process of its own: the library's pool and its kernels' settings are made while a stream captures."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(tblib.__file__))
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, what], env=env, capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]
