@@ -876,3 +876,34 @@ def test_a_process_first_call_may_be_captured(cuda, tblib, what):
     env = dict(os.environ, PYTHONPATH=os.path.dirname(tblib.__file__))
     p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, what], env=env, capture_output=True, text=True, timeout=300)
     assert p.returncode == 0, p.stderr[-2000:]
+
+
+def test_more_blocks_of_tokens_than_a_grid_has_rows(cuda, tblib):
+    """65535 blocks of 128 tokens and 300 tokens more: packing and reading back in two launches, and sums over all of them.
+    A sum's groups (512 tokens; the Hessian's 128 are exact) lose at most 32 2^-23 of their terms' magnitudes in the tensor
+    core; the one tile has 74 to 148 shares, the additions of whose groups, and of the shares, round by 2^-24 of the
+    magnitudes each."""
+    torch, tb = cuda, tblib
+    n, d, r = 65535 * 128 + 300, 9, 5
+    x = rows(torch, n, d, torch.float32, 140, heavy=0)
+    keep = (torch.arange(n, device="cuda") % 1000 < 990).to(torch.uint8)
+    c = packed(torch, tb, x, keep)
+    lo = 65533 * 128  # the last blocks of the first launch, and the second
+    q, e = ref.pack(torch, x[lo:], keep[lo:])
+    assert torch.equal(c.codes[lo:n, :d], q) and torch.equal(c.exps[65533:, :d], e)
+    q, e = ref.pack(torch, x[:1024], keep[:1024])
+    assert torch.equal(c.codes[:1024, :d], q) and torch.equal(c.exps[:8, :d], e)
+    xh = c.values(torch)
+    out = torch.full((n, d), 9.0, device="cuda")
+    tb.check(tb.act8_unpack(c.s, out.data_ptr(), tb.F32, d))
+    assert torch.equal(out.double(), xh)
+    dy = rows(torch, n, r, torch.bfloat16, 141, 8, 1e-2, 0)
+    G, H = torch.empty(r, d, device="cuda"), torch.empty(d, d, device="cuda")
+    tb.check(tb.act8_weight_grad(c.s, dy.data_ptr(), tb.BF16, 8, r, None, 1, G.data_ptr(), tb.F32))
+    tb.check(tb.act8_hessian(c.s, 1.0, H.data_ptr()))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    for got, a, groups in ((G, dy.double(), n // 512), (H, xh, n // 128)):
+        want, mag = a.t() @ xh, a.abs().t() @ xh.abs()
+        bar = (64 + groups // 74 + 1 + 148 + 2) * 2.0 ** -24 * mag
+        assert bool(((got.double() - want).abs() <= bar).all())

@@ -313,6 +313,54 @@ def test_calls_repeat_bit_for_bit_and_under_graphs(cuda, tblib):
     assert all(torch.equal(a, b) for k in (0, 1) for a, b in zip(outs(k), want[k]))
 
 
+def test_larger_batches_under_graphs_with_new_tokens(cuda, tblib):
+    """Batches whose tokens are ordered by adapter, with shares of the gradients: two captured graphs, replayed on two
+    streams at once with new rows and new adapters of the tokens, against single calls and the formula."""
+    torch, tb = cuda, tblib
+    n, d, r, rank, na = 2600, 264, 392, 40, 3
+    cases, cks, graphs = [], [], []
+    for i in range(2):
+        c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, "mixed", i), 100 + i)
+        cases.append(c)
+        cks.append(packed(torch, tb, c.x))
+
+    def go(k, stream=None):
+        c, ck = cases[k], cks[k]
+        tb.check(tb.adapter_forward(c.args(tb), stream=stream))
+        tb.check(tb.adapter_backward(c.args(tb, x8=ck.s), stream=stream))
+
+    for k in (0, 1):
+        go(k)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            go(k, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for t, kind in enumerate(("runs", "mixed", "none", "one")):
+        for k, c in enumerate(cases):
+            c.x.copy_(bf(torch, n, d, 110 + 2 * t + k))
+            c.who.copy_(who_of(torch, n, na, kind, 9 + t + k).to(torch.int32))
+            ck = packed(torch, tb, c.x)
+            cks[k].codes.copy_(ck.codes)
+            cks[k].exps.copy_(ck.exps)
+            for o in (c.y, c.dx, c.da, c.db):
+                o.fill_(3.0)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for k, c in enumerate(cases):
+            got = [o.clone() for o in (c.y, c.dx, c.da, c.db)]
+            go(k)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, (c.y, c.dx, c.da, c.db)))
+            check(torch, c.y[:n, :r], c.ref.forward(c.x), c.ref.forward(c.x, True), d + rank)
+            want, mag = (c.ref.backward(c.dy, cks[k].values(torch), m) for m in (False, True))
+            check(torch, c.da[:, :d].reshape(na, rank, d), want[1], mag[1], n + r)
+            check(torch, c.db[:, :rank].reshape(na, r, rank), want[2], mag[2], n + d)
+
+
 @pytest.mark.parametrize("n,na", [(1, 3), (5, 0), (20, 3), (32, 3)])
 def test_few_tokens_under_graphs_and_on_two_streams(cuda, tblib, n, na):
     """The forward that starts while its down projection runs: captured, replayed with new tokens, two at once."""
