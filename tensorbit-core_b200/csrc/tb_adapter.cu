@@ -132,7 +132,6 @@ struct Order {
     int* tokens;    // [n]
 };
 constexpr int kSmallBatch = 1024;
-constexpr int kFewTokens = 32;  // at most, of few_tokens_kernel
 
 __global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o, int32_t* __restrict__ lists) {
     __shared__ int scan[32], total[2], who[256];
@@ -331,12 +330,13 @@ __device__ __forceinline__ void down_small(const Args& g, const Rows& src, float
 // v (from dy); 1: the backward's u (from the checkpoint).
 template <int NT, bool BACKWARD>
 __global__ void __cluster_dims__(kSplit, 1, 1) __launch_bounds__(256)
-down_small_kernel(const Args g, const int passes, float* __restrict__ first, float* __restrict__ second, int32_t* __restrict__ lists) {
+down_small_kernel(const Args g, const int passes, const bool few, float* __restrict__ first, float* __restrict__ second,
+                  int32_t* __restrict__ lists) {
     __shared__ float red[8][16][8 * NT];
     __shared__ int who[256];
     const int p = blockIdx.z % passes;
     // Only where few_tokens_kernel follows, which waits before it reads u (see launch_pdl's contract).
-    if (!BACKWARD && g.n <= kFewTokens) asm volatile("griddepcontrol.launch_dependents;");
+    if (few) asm volatile("griddepcontrol.launch_dependents;");
     if constexpr (!BACKWARD) {
         down_small<NT, false, true>(g, {g.x, g.ldx, {}, g.d}, first, red, who, passes, p);
     } else {
@@ -710,6 +710,21 @@ __global__ void __launch_bounds__(256) few_tokens_kernel(const Args g, const flo
         g.y[t * g.ldy + o] = __float2bfloat16_rn(y);
     }
 }
+// Where it is the sooner: up to 16 tokens, or 32 with at most 2^25 weights or from
+// eight adapters on (each in a tile is a slice of its own, about 2.6 us); without
+// adapters not where W's rows are longer than 8192.  (us of a call, W from memory,
+// tokens of eight adapters of rank 16 mixed, or without adapters; this kernel against
+// tiles: 4096 -> 4096, 16 tokens 15.7 and 34.6, without 14.3 and 17.1; 32 tokens 22.6
+// and 35.8, without 15.8 and 17.8.  4096 -> 14336, 16 tokens 32.1 and 49.9, without
+// 29.8 and 28.8; 24 tokens 47.3 and 50.3, without 42.5 and 29.0.  8192 -> 8192, one
+// token 31.4 and 53.0, without 29.6 and 46.9; 24 tokens 59.3 and 58.6, without 55.2
+// and 36.2.  14336 -> 4096, one token 44.7 and 47.7, without 43.4 and 36.8; 16 tokens
+// 46.1 and 56.7, without 44.4 and 31.7; 32 tokens 59.6 and 57.6, without 48.9 and 32.9.)
+bool few_tokens(const Args& g) {
+    if (!g.na && g.d > 8192) return false;
+    return g.n <= 16 || (g.n <= 32 && (g.na >= 8 || static_cast<long long>(g.r) * g.d <= 1ll << 25));
+}
+
 template <int NT>
 cudaError_t launch_few(const Args& g, const float* u, cudaStream_t st) {
     // Without adapters the kernel before this one is the caller's, which may still be writing x when it lets go.
@@ -762,24 +777,24 @@ int make_scratch(const Args& g, bool grads, cudaStream_t st, Scratch* s) {
 
 // u of the forward (into `first`), or v and u of the backward.
 template <int NT, bool BACKWARD>
-void launch_down(const Args& g, const Scratch& s, float* first, float* second, cudaStream_t st) {
+void launch_down(const Args& g, const Scratch& s, bool few, float* first, float* second, cudaStream_t st) {
     const unsigned chunks = (g.rank + 8 * NT - 1) / (8 * NT), two = second ? 2 : 1;
     if (g.n <= kSmallBatch) {
         // A small batch's tiles do not fill the GPU: a block for each adapter that a tile may hold, and
         // eight for its features.  (One token, 4096 features, rank 16: 9.4 us with one block, 4.7 with eight.)
         const int passes = std::min(16, g.na);
         const unsigned tiles = static_cast<unsigned>((g.n + 15) / 16);
-        down_small_kernel<NT, BACKWARD><<<dim3(kSplit * tiles, chunks, two * passes), 256, 0, st>>>(g, passes, first, second, s.lists);
+        down_small_kernel<NT, BACKWARD><<<dim3(kSplit * tiles, chunks, two * passes), 256, 0, st>>>(g, passes, few, first, second, s.lists);
     } else {
         order_kernel<<<static_cast<unsigned>(g.na + (g.n + 255) / 256), 1024, 0, st>>>(g, s.order, s.lists);
         down_kernel<NT, BACKWARD><<<dim3(static_cast<unsigned>(kPieceSplit * (g.n / 64 + g.na)), chunks, two), 256, 0, st>>>(g, s.order, first, second);
     }
 }
 template <bool BACKWARD>
-int down(const Args& g, const Scratch& s, float* first, float* second, cudaStream_t st) {
-    if (g.rank <= 16) launch_down<2, BACKWARD>(g, s, first, second, st);
-    else if (g.rank <= 32) launch_down<4, BACKWARD>(g, s, first, second, st);
-    else launch_down<8, BACKWARD>(g, s, first, second, st);
+int down(const Args& g, const Scratch& s, bool few, float* first, float* second, cudaStream_t st) {
+    if (g.rank <= 16) launch_down<2, BACKWARD>(g, s, few, first, second, st);
+    else if (g.rank <= 32) launch_down<4, BACKWARD>(g, s, few, first, second, st);
+    else launch_down<8, BACKWARD>(g, s, few, first, second, st);
     return check_launch("down_kernel");
 }
 
@@ -868,10 +883,11 @@ extern "C" int tb_adapter_forward(const tb_adapter_args* p, void* stream) {
     auto st = static_cast<cudaStream_t>(stream);
     Scratch s{};
     if ((rc = make_scratch(g, false, st, &s))) return rc;
+    const bool few = few_tokens(g);
     if (g.na) {
-        rc = down<false>(g, s, s.u, nullptr, st);
+        rc = down<false>(g, s, few, s.u, nullptr, st);
     }
-    if (!rc && g.n <= kFewTokens) {
+    if (!rc && few) {
         const cudaError_t e = g.n <= 8 ? launch_few<1>(g, s.u, st) : g.n <= 16 ? launch_few<2>(g, s.u, st) : launch_few<4>(g, s.u, st);
         rc = e == cudaSuccess ? check_launch("few_tokens_kernel") : cuda_fail(e, "few_tokens_kernel launch");
     } else if (!rc) rc = linear::adapter_forward({g.n, g.r, g.d, g.x, g.ldx, g.w, g.ldw, g.y, g.ldy, g.who, s.lists, s.u, g.b, g.ldb, g.rank, g.na}, st);
@@ -902,7 +918,7 @@ extern "C" int tb_adapter_backward(const tb_adapter_args* p, void* stream) {
     Scratch s{};
     if ((rc = make_scratch(g, grads, st, &s))) return rc;
     if (s.lists) {
-        rc = down<true>(g, s, s.v, grads ? s.u : nullptr, st);
+        rc = down<true>(g, s, false, s.v, grads ? s.u : nullptr, st);
     }
     if (!rc && g.dx && g.n)
         rc = linear::adapter_input_grad({g.n, g.d, g.r, g.dy, g.lddy, g.w, g.ldw, g.dx, g.lddx, g.who, s.lists, s.v, g.a, g.lda, g.rank, g.na}, st);

@@ -86,6 +86,20 @@ def test_forward(cuda, tblib, n, d, r, rank, na, kind):
     assert bool((c.y[n:] == 3).all()) and bool((c.y[:, r:] == 3).all())
 
 
+@pytest.mark.parametrize("n,d,r,rank,na,kind", [
+    (16, 8200, 4104, 16, 3, "mixed"), (17, 8200, 4104, 16, 3, "mixed"), (32, 8192, 4096, 24, 3, "runs"), (32, 8192, 4104, 24, 3, "runs"), (32, 8192, 4104, 24, 8, "mixed"),
+    (1, 8192, 136, 16, 0, "none"), (1, 8200, 136, 16, 0, "none"), (1, 8200, 136, 16, 1, "one"), (16, 9000, 4000, 8, 0, "none")])
+def test_forward_of_few_tokens_on_both_sides_of_its_rule(cuda, tblib, n, d, r, rank, na, kind):
+    """Few tokens of large projections, by the kernel of few tokens and by tiles."""
+    torch, tb = cuda, tblib
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, kind), 3)
+    tb.check(tb.adapter_forward(c.args(tb)))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    check(torch, c.y[:n, :r], c.ref.forward(c.x), c.ref.forward(c.x, True), d + rank)
+    assert bool((c.y[n:] == 3).all()) and bool((c.y[:, r:] == 3).all())
+
+
 @pytest.mark.parametrize("n,d,r,rank,na,kind", SHAPES)
 def test_backward(cuda, tblib, n, d, r, rank, na, kind):
     torch, tb = cuda, tblib
