@@ -1296,7 +1296,12 @@ int tiles(long long v, int t) { return static_cast<int>((v + t - 1) / t); }
 // worth it.  (Kernels, 4096 features, decoded in the product against written out:
 // 16 gradients of 4096 rows 313 and 248 + 17 us; 2048 rows, with all launches, 157
 // and 145; 1024 rows 87 and 87; 512 rows 53 and 59.  One gradient of 500 tokens and
-// 2048 rows 16.0 and 17.4.  64 samples' Fisher of 4096 rows 752 and 561 + 37.)
+// 2048 rows 16.0 and 17.4.  64 samples' Fisher of 4096 rows 752 and 561 + 37.  Between
+// and for other types, 16 gradients, calls: BF16 of 1280 rows, five uses, 135 and 123;
+// F16 of 512 rows, four, 105 and 103, of 768, six, 147 and 137; FP32 of 256, three, 88
+// and 89, of 512, six, 140 and 128.  16 samples' Fisher: BF16 of 1280 rows 110 and 110,
+// F16 of 768 180 and 165, FP32 of 512 187 and 178.  One FP32 gradient of 509 tokens and
+// 1024 rows 29 and 31.)
 constexpr long long kValuesMax = 1ll << 31;  // bytes of them at most
 
 template <int MODE, int VALUES>
