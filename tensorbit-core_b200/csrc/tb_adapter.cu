@@ -120,8 +120,8 @@ __device__ __forceinline__ uint4 row8(const Rows& s, long long t, int f) {
     return f + 8 <= s.cols ? v : first_of(v, s.cols - f);
 }
 
-// The tokens of each adapter, in order, for batches of more than kSmallBatch
-// tokens: order[start ..] holds them, and every piece of 64 has an entry of
+// The tokens of each adapter, in order, for batches that are not small (see
+// small_batch()): order[start ..] holds them, and every piece of 64 has an entry of
 // `tiles` at start / 64 + a + piece (adapters' entries cannot overlap there; an
 // entry without a piece has adapter -1).  One block per adapter: it counts the
 // tokens of lower adapters, then compacts its own.  Further blocks list the
@@ -131,7 +131,7 @@ struct Order {
     int2* tiles;    // [n / 64 + na] (adapter, piece)
     int* tokens;    // [n]
 };
-constexpr int kSmallBatch = 1024;
+constexpr int kSmallBatch = 1024;  // tokens at most
 
 __global__ void __launch_bounds__(1024) order_kernel(const Args g, const Order o, int32_t* __restrict__ lists) {
     __shared__ int scan[32], total[2], who[256];
@@ -743,10 +743,22 @@ struct Scratch {
     Order order;
     int shares;
 };
+// Batches whose tokens are taken as they lie, 16 at a time, with a pass for each
+// adapter among them, against ordered by adapter first, two launches for one.  The
+// passes grow with the tokens and, where those of many adapters are mixed, with the
+// adapters; the ordering with the adapters alone.  (Time of whole calls, ordered over
+// as they lie, geometric mean of forward and backward, 1024 -> 512 to 4096 -> 14336,
+// ranks 8 to 128.  In runs of one adapter each: 4 adapters, 512 tokens 1.10, 768 0.98;
+// 16 adapters, 128 tokens 1.06, 256 1.06, 512 0.93, 1024 0.69.  Mixed: 4 adapters, 256
+// tokens 0.94, 512 0.75; 16 adapters, 64 tokens 0.87, 128 0.69, 1024 0.22; 64 adapters,
+// 64 tokens 0.95, 256 0.74.  An adapter each: 2048 adapters, 130 tokens 0.98,
+// 1024 0.82; 8192, forward, 130 tokens 1.47, 1024 1.03.)
+bool small_batch(const Args& g) { return g.n <= (g.na > 2048 ? kSmallBatch : g.na < 16 ? 512 : 128); }
+
 int make_scratch(const Args& g, bool grads, cudaStream_t st, Scratch* s) {
     s->shares = 1;
     if (!g.na || !g.n) return TB_OK;
-    const bool ordered = g.n > kSmallBatch;
+    const bool ordered = !small_batch(g);
     if (grads && ordered) {
         // Enough blocks to fill the GPU about four times, but no share of an even split below 512 tokens.
         const long long blocks = static_cast<long long>((g.d + 127) / 128 + (g.r + 127) / 128) * g.na * ((g.rank + 31) / 32);
@@ -779,7 +791,7 @@ int make_scratch(const Args& g, bool grads, cudaStream_t st, Scratch* s) {
 template <int NT, bool BACKWARD>
 void launch_down(const Args& g, const Scratch& s, bool few, float* first, float* second, cudaStream_t st) {
     const unsigned chunks = (g.rank + 8 * NT - 1) / (8 * NT), two = second ? 2 : 1;
-    if (g.n <= kSmallBatch) {
+    if (small_batch(g)) {
         // A small batch's tiles do not fill the GPU: a block for each adapter that a tile may hold, and
         // eight for its features.  (One token, 4096 features, rank 16: 9.4 us with one block, 4.7 with eight.)
         const int passes = std::min(16, g.na);

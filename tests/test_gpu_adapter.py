@@ -119,6 +119,28 @@ def test_backward(cuda, tblib, n, d, r, rank, na, kind):
         assert bool((c.da[:, d:] == 3).all()) and bool((c.db[:, rank:] == 3).all())
 
 
+@pytest.mark.parametrize("n,d,r,rank,na,kind", [
+    (512, 264, 392, 16, 15, "mixed"), (513, 264, 392, 16, 15, "mixed"), (128, 264, 392, 40, 16, "mixed"), (129, 264, 392, 40, 16, "mixed"),
+    (512, 136, 72, 8, 1, "one"), (513, 136, 72, 8, 1, "one"), (1024, 72, 40, 3, 2049, "runs"), (1025, 72, 40, 3, 2049, "runs"),
+    (600, 72, 40, 8, 2048, "mixed"), (129, 2000, 1000, 128, 20, "wild")])
+def test_batches_on_both_sides_of_the_ordering_rule(cuda, tblib, n, d, r, rank, na, kind):
+    """Tokens taken as they lie, and ordered by adapter first."""
+    torch, tb = cuda, tblib
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, kind, 1), 120)
+    ck = packed(torch, tb, c.x)
+    tb.check(tb.adapter_forward(c.args(tb)))
+    tb.check(tb.adapter_backward(c.args(tb, x8=ck.s)))
+    torch.cuda.synchronize()
+    tb.check(tb.lib().tb_gemm_status(None))
+    check(torch, c.y[:n, :r], c.ref.forward(c.x), c.ref.forward(c.x, True), d + rank)
+    xh = ck.values(torch)
+    want, mag = c.ref.backward(c.dy, xh), c.ref.backward(c.dy, xh, True)
+    check(torch, c.dx[:n, :d], want[0], mag[0], r + rank)
+    check(torch, c.da[:, :d].reshape(na, rank, d), want[1], mag[1], n + r)
+    check(torch, c.db[:, :rank].reshape(na, r, rank), want[2], mag[2], n + d)
+    assert bool((c.y[n:] == 3).all()) and bool((c.y[:, r:] == 3).all()) and bool((c.dx[n:] == 3).all()) and bool((c.dx[:, d:] == 3).all())
+
+
 def test_gradients_against_differences(cuda, tblib):
     """The loss sum(dy * y(xhat)) in float64, differenced along random directions of x, A and B, against the kernels'
     gradients: y is linear in each of them alone, so a central difference is exact to float64 rounding, and the
