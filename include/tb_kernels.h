@@ -305,8 +305,8 @@ int tb_act8_unpack(const tb_act8* ck, void* out, int dtype, int64_t ldo, void* s
  * is exact: FP32 (F16) dy is split into three (two) BF16 parts, but for bits
  * below 2^-133, in scratch of 6 (4) bytes per value from the library's per-device
  * pool; rows of a BF16 dy that are not 16-byte aligned are first copied to such
- * scratch.  Large products with r beyond 1024 (F16: 512, FP32: 256) write xhat out
- * there as BF16, 2 bytes per value, unless that is more than 2 GiB.  Where the
+ * scratch.  Large products with r beyond 1024 (F16: 512, FP32: 256) write all of
+ * xhat out there as BF16, 2 bytes per value, unless that is more than 2 GiB.  Where the
  * gradients' 256 x 256 tiles do not fill the GPU's last wave, FP32 shares of their
  * sums also wait there, at most 148 tiles (39 MB). */
 int tb_act8_weight_grad(const tb_act8* ck, const void* dy, int dy_dtype, int64_t lddy, int r,
@@ -340,8 +340,9 @@ int tb_act8_hessian(const tb_act8* ck, float scale, int accumulate, float* H, vo
  * none: token t of adapter a = token_adapter[t] sees W + scale[a] B_a A_a.
  * The calibration of such a projection runs its forward with the adapters in
  * place and its backward from the 8-bit checkpoint of x.  No reference
- * counterpart.  BF16 operands, FP32 sums; A x and B^T dy stay in FP32 and
- * enter the second product as two BF16 parts (a relative 2^-17). */
+ * counterpart.  BF16 operands, FP32 sums (in the tensor core, whose additions
+ * cut off instead of rounding); A x and B^T dy stay in FP32 and enter the second
+ * product as two BF16 parts (a relative 2^-17). */
 typedef struct tb_adapter_args {
     uint32_t struct_size;  /* sizeof(tb_adapter_args)                                    */
     int32_t  dtype;        /* of w, a, b, x, y, dy, dx, da, db: TB_BF16                  */
