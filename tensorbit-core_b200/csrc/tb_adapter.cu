@@ -415,22 +415,11 @@ __device__ __forceinline__ long long grad_at(const Args& g, int a, int c, int k)
     return OF_A ? (static_cast<long long>(a) * g.rank + k) * g.lda + c : (static_cast<long long>(a) * g.r + c) * g.ldb + k;
 }
 
-// Feature c's sum with rank k over tokens[begin .. end), products whole, one after
-// another: for a sum of the parts' products that is a NaN.  Times an infinity of
-// the row, a value's second part makes one (where it is zero, or of the other
-// sign) although the product is an infinity.  Ends at the first NaN of its own.
-template <bool CODES>
-__device__ __noinline__ float whole_sum(const Rows& src, const float* val, int rank, const int* tokens, int begin, int end, int c, int k) {
-    float s = 0.0f;
-    for (int i = begin; i < end && s == s; ++i) {
-        const long long t = tokens[i];
-        float x;
-        if constexpr (CODES)
-            x = static_cast<float>(src.x8.codes[t * src.x8.ldq + c]) * act8::scale_f32(src.x8.exps[t / act8::kBlock * src.x8.lde + c]);
-        else x = __bfloat162float(src.x[t * src.ld + c]);
-        s = fmaf(x, val[t * rank + k], s);
-    }
-    return s;
+// Zeros for those of two BF16 values that are not finite.
+__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
+    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
+    return w;
 }
 
 // A copy of BYTES that this thread waits for by itself, or as many zeros.
@@ -576,6 +565,29 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
         find(from + 64 * (kAhead + 1));
         stage = stage == kRing - 1 ? 0 : stage + 1;
         const int p = (warp >> 1) * 8 + tq;
+        // Times an infinity of the row a value's low part, which may be zero or of the other sign, would make a
+        // NaN of it: such rows have their low products apart, without it.  (An exponent of all ones carries out
+        // of the exponent's bits.)
+        uint32_t odd = 0;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) odd |= (x[m][j] & 0x7F807F80u) + 0x00800080u;
+        if (__any_sync(~0u, odd & 0x80008000u)) {
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+                        mma16816(acc[m][i], x[m][0], x[m][1], x[m][2], x[m][3], sm.vp[part][p][8 * i + gq], sm.vp[part][p + 4][8 * i + gq]);
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[m][j] = finite_of(x[m][j]);
+            }
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const uint32_t h0 = sm.vp[0][p][8 * i + gq], h1 = sm.vp[0][p + 4][8 * i + gq];
@@ -607,10 +619,8 @@ __device__ __forceinline__ void outer_product(const Args& g, const Rows& src, co
     for (int i = threadIdx.x; i < 128 * RC; i += 256) {
         const int c = CODES ? i % 128 : i / RC, k = CODES ? i / 128 : i % RC;
         if (f0 + c >= src.cols || rank0 + k >= g.rank) continue;
-        float s = sm.sum[c][k];
-        if (s != s) s = whole_sum<CODES>(src, val, g.rank, tokens, begin, end, f0 + c, rank0 + k);
-        if (shares > 1) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = s;
-        else out[grad_at<CODES>(g, a, f0 + c, rank0 + k)] = __float2bfloat16_rn(s);
+        if (shares > 1) part[((static_cast<long long>(share) * g.na + a) * src.cols + f0 + c) * g.rank + rank0 + k] = sm.sum[c][k];
+        else out[grad_at<CODES>(g, a, f0 + c, rank0 + k)] = __float2bfloat16_rn(sm.sum[c][k]);
     }
 }
 

@@ -249,6 +249,31 @@ def test_infinities_of_dy_keep_their_sign_in_db(cuda, tblib, n):
     check(torch, db[~hit], want[~hit], mag[~hit], n + d)
 
 
+def test_gradients_of_rows_without_numbers_cost_no_more(cuda, tblib):
+    """One infinity, one token of NaN: the factors' gradients take about the time that they take without (the bar is 4 times)."""
+    torch, tb = cuda, tblib
+    n, d, r = 4000, 2048, 2048
+    c = Case(torch, n, d, r, 32, 2, who_of(torch, n, 2, "runs"), 95)
+    ck = packed(torch, tb, c.x)
+
+    def time():
+        times = []
+        for _ in range(8):
+            ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            ev[0].record()
+            tb.check(tb.adapter_backward(c.args(tb, x8=ck.s, dx=None)))
+            ev[1].record()
+            torch.cuda.synchronize()
+            times.append(ev[0].elapsed_time(ev[1]))
+        return min(times)
+
+    plain = time()
+    c.dy[n - 5, 9] = math.inf
+    assert time() <= 4 * plain and bool(torch.isinf(c.db[r + 9, :32]).all())
+    c.dy[n - 700] = math.nan
+    assert time() <= 4 * plain and bool(torch.isnan(c.db[r:, :32]).all())
+
+
 def test_large_values_and_tokens_without_numbers(cuda, tblib):
     """u and v that round to an infinity in BF16 but are none count as what they are; tokens that are all NaN, and an
     adapter that is, cost no more time than others: the products' bounded waits do not run out."""
