@@ -151,14 +151,13 @@ __device__ __forceinline__ void give_up(volatile int* abort_flag) {
 __device__ __forceinline__ void arrive_even(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar & kPeerMask) : "memory");
 }
-// Sets a flag of both CTAs, before what this warp tells anyone next.
-__device__ __forceinline__ void set_pair(volatile int* flag) {
-    const uint32_t here = smem_u32(const_cast<int*>(flag));
+// Sets bits of a word of both CTAs, before what this warp tells anyone next.
+__device__ __forceinline__ void set_pair(uint32_t* word, uint32_t bits) {
     asm volatile(
         "{\n\t.reg .b32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.u32 [a], %1;\n\t"
-        "mapa.shared::cluster.u32 a, %0, 1;\n\tst.shared::cluster.u32 [a], %1;\n\t"
-        "fence.acq_rel.cluster;\n\t}" ::"r"(here), "r"(1)
+        "mapa.shared::cluster.u32 a, %0, 0;\n\tred.relaxed.cluster.shared::cluster.or.b32 [a], %1;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 1;\n\tred.relaxed.cluster.shared::cluster.or.b32 [a], %1;\n\t"
+        "fence.acq_rel.cluster;\n\t}" ::"r"(smem_u32(word)), "r"(bits)
         : "memory");
 }
 template <int MODE>
@@ -499,43 +498,74 @@ __device__ __forceinline__ void load_piece(uint8_t* buf, float* v, const float* 
 
 // An adapter's second factor enters the product for all tokens of a tile, times
 // zero for those of other adapters; zero times an infinity or a NaN is not zero.
-// Such values are therefore left out of the operand, which notes that there were
-// any, and the epilogue adds their terms to the results of the adapter's own tokens.
+// Such values are ones of their sign in the operand, which notes their adapter, and
+// the epilogue adds their own terms to the results of the adapter's own tokens.
+// (Beside those a one's does not count; an infinity of the token, which with a zero
+// would be a NaN, keeps its sign.)
 __device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool& odd) {
     if ((w & 0x7F80u) == 0x7F80u) {
-        w &= 0xFFFF0000u;
+        w = (w & 0xFFFF8000u) | 0x3F80u;
         odd = true;
     }
     if ((w & 0x7F800000u) == 0x7F800000u) {
-        w &= 0xFFFFu;
+        w = (w & 0x8000FFFFu) | 0x3F800000u;
         odd = true;
     }
     return w;
 }
-// Result i of token t, feature o + i, is at v[32 i].  (Not unrolled: it hardly ever runs.)
+// The bit that stands for adapter a among those noted (for others too, whose factors then are looked through).
+__device__ __forceinline__ uint32_t odd_bit(int a) { return 1u << (a & 31); }
+
+// Result i of this lane's token, feature o + i, is at v[32 i].  A lane looks one
+// feature's ranks through for all tokens of an adapter.  (8000 x 4096 x 4096 forward,
+// four adapters of rank 64, 268 us: with one value an infinity 10991 looked through
+// token by token and 365 so, with a whole adapter NaN 12089 and 437.)
 template <int MODE>
-__device__ __noinline__ void add_odd_row(const AdapterProduct& p, float* v, long long t, long long o, int cols) {
-    const int a = p.who[t];
-    if (a < 0 || a >= p.na) return;
-    for (int j = 0; j < p.rank; ++j) {
-        const float u = p.u[t * p.rank + j];
-        for (int i = 0; i < cols; ++i) {
-            const float e = __bfloat162float(MODE == kFwd ? p.e[(static_cast<long long>(a) * p.N + o + i) * p.lde + j]
-                                                          : p.e[(static_cast<long long>(a) * p.rank + j) * p.lde + o + i]);
-            if (!(fabsf(e) <= 3.402823466e38f)) v[32 * i] = fmaf(u, e, v[32 * i]);
+__device__ __noinline__ void add_odd_columns(const AdapterProduct& p, const uint32_t* noted, float* v, long long row0, int rows, long long o,
+                                             int cols, int lane) {
+    const long long t = row0 + lane;
+    int own = lane < rows ? __ldg(p.who + t) : -1;  // this lane's adapter if it is one of those noted, else -1
+    if (own < 0 || own >= p.na || !(*const_cast<const volatile uint32_t*>(noted) & odd_bit(own))) own = -1;
+    const long long step = MODE == kFwd ? 1 : p.lde;  // from rank to rank
+    for (unsigned left = __ballot_sync(~0u, own >= 0); left;) {
+        const int a = __shfl_sync(~0u, own, __ffs(left) - 1);
+        left &= ~__ballot_sync(~0u, own == a);
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(p.e) +
+                            (MODE == kFwd ? (static_cast<long long>(a) * p.N + o) * p.lde : static_cast<long long>(a) * p.rank * p.lde + o);
+        bool nan = false, inf = false;
+        if (lane < cols) {
+            const uint16_t* mine = e + (MODE == kFwd ? lane * p.lde : lane);
+#pragma unroll 8
+            for (int j = 0; j < p.rank; ++j) {
+                const uint32_t magnitude = __ldg(mine + j * step) & 0x7FFFu;
+                nan |= magnitude > 0x7F80u;
+                inf |= magnitude == 0x7F80u;
+            }
+        }
+        const unsigned nans = __ballot_sync(~0u, nan), infs = __ballot_sync(~0u, inf) & ~nans;
+        if (own != a) continue;
+        for (unsigned m = nans; m; m &= m - 1) v[32 * (__ffs(m) - 1)] = __uint_as_float(0x7FFFFFFFu);
+        for (unsigned m = infs; m; m &= m - 1) {
+            const int i = __ffs(m) - 1;
+            float s = v[32 * i];
+            for (int j = 0; j < p.rank && s == s; ++j) {
+                const uint32_t x = __ldg(e + (MODE == kFwd ? i * p.lde : i) + j * step);
+                if ((x & 0x7FFFu) == 0x7F80u) s = fmaf(p.u[t * p.rank + j], __uint_as_float(x << 16), s);
+            }
+            v[32 * i] = s;
         }
     }
 }
 template <int MODE>
-__device__ __forceinline__ void add_odd_terms(const AdapterProduct& p, uint8_t* buf, float (&v)[64], long long row0, long long col,
-                                              int rows, int cols, int lane) {
+__device__ __forceinline__ void add_odd_terms(const AdapterProduct& p, const uint32_t* noted, uint8_t* buf, float (&v)[64], long long row0,
+                                              long long col, int rows, int cols, int lane) {
     float* x = reinterpret_cast<float*>(buf) + lane;  // column i of this lane's row at 32 i
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[32 * i] = v[32 * h + i];
-        if (lane < rows) add_odd_row<MODE>(p, x, row0 + lane, col + 32 * h, min(32, cols - 32 * h));
+        add_odd_columns<MODE>(p, noted, x, row0, rows, col + 32 * h, min(32, cols - 32 * h), lane);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[32 * h + i] = x[32 * i];
     }
@@ -544,7 +574,7 @@ __device__ __forceinline__ void add_odd_terms(const AdapterProduct& p, uint8_t* 
 
 // Ranks r0.. of adapter `a` as one K slice of 64 (thread pt of 128): A is the
 // tile's tokens' u as two BF16 parts, zero unless the adapter is their own; B is
-// the adapter's second factor, twice, its finite values.  What it needs is fetched
+// the adapter's second factor, twice, as finite_pair has it.  What it needs is fetched
 // ahead: into registers before the stage is free.  (7000 x 4096 x 14336 forward
 // with one adapter in most tiles: 584 us fetched once the stage was free, 560 so.)
 template <int MODE>
@@ -672,7 +702,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint64_t* accempty = accfull + C::kAcc;   // [kAcc] (even CTA) accumulator taken by both CTAs
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + C::kAcc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* odd_flag = abort_flag + 1;  // an adapter's factor had values that are not finite (set in both CTAs, never reset)
+    uint32_t* odd_flag = tmem_slot + 2;  // a bit for each adapter whose factor had values that are not finite (set in both CTAs, never reset)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
 
@@ -729,7 +759,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 fence_after();
                 ac.next();
                 // (the adapters' slices are the last share's)
-                const bool odd = P.ad.lists && t.q == t.splits - 1 && __any_sync(~0u, *odd_flag);
+                const bool odd = P.ad.lists && t.q == t.splits - 1 && __any_sync(~0u, *const_cast<volatile uint32_t*>(odd_flag));
 #pragma unroll 1
                 for (int c = 0; c < COLS && c < cols; c += 64) {
                     float v[64];
@@ -741,7 +771,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                         for (int i = 0; i < 32; ++i) v[32 * h + i] = x[i];
                     }
                     const int left = cols - c;
-                    if (odd) add_odd_terms<MODE>(P.ad, buf, v, row0, col + c, rows, left, lane);
+                    if (odd) add_odd_terms<MODE>(P.ad, odd_flag, buf, v, row0, col + c, rows, left, lane);
                     if (t.slot >= 0) {
                         store_rows<false>(buf, v, P.part + static_cast<long long>(t.slot) * kPartTile + row_in * 256 + half * COLS + c, 256, rows, left, lane);
                         continue;
@@ -1129,18 +1159,20 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                 const long long m0 = static_cast<long long>(t.tm) * 256 + rank * 128;
                 const int n0 = t.tn * NB + rank * C::kCols, own = m0 + pt < P.ad.n ? __ldg(P.ad.who + m0 + pt) : -1;
                 AdapterSlice<MODE> slice;
-                slice.fetch(P.ad, own, __ldg(u.list + 1), 0, m0, n0, pt);
+                int a = __ldg(u.list + 1);
+                slice.fetch(P.ad, own, a, 0, m0, n0, pt);
                 for (int x = 0; x < u.extra; ++x, ++it) {
                     const int s = it % kStages, next = x + 1;
-                    const int a = next < u.extra ? __ldg(u.list + 1 + next / u.rslices) : 0;
+                    const int following = next < u.extra ? __ldg(u.list + 1 + next / u.rslices) : 0;
                     if (!wait(smem_u32(&full[s]), (phase >> s) & 1, abort_flag, it - waited)) { ok = false; break; }
                     waited = it;
                     phase ^= 1u << s;
                     const bool odd = slice.build(smem + s * C::kStage, smem + s * C::kStage + C::kA, pt);
-                    if (__any_sync(~0u, odd)) set_pair(odd_flag);
+                    if (odd) set_pair(odd_flag, odd_bit(a));
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) arrive_even(smem_u32(&ready[s]));
+                    a = following;
                     if (next < u.extra) slice.fetch(P.ad, own, a, next % u.rslices * 32, m0, n0, pt);
                 }
             }

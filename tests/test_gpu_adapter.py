@@ -249,6 +249,59 @@ def test_infinities_of_dy_keep_their_sign_in_db(cuda, tblib, n):
     check(torch, db[~hit], want[~hit], mag[~hit], n + d)
 
 
+@pytest.mark.parametrize("n", [20, 60, 1500])
+def test_infinities_of_token_and_adapter_at_once(cuda, tblib, n):
+    """All values positive but for the infinities' signs: a token with one times a factor with one is an infinity, in y and dx."""
+    torch, tb = cuda, tblib
+    d, r, rank, na, t = 200, 392, 24, 3, 7
+    c = Case(torch, n, d, r, rank, na, torch.arange(n) % na, 130)
+    for m in (c.w, c.a, c.b, c.x, c.dy):
+        m.abs_()
+    c.w.clamp_(min=1e-3)
+    c.x[t, 9], c.b[(t % na) * r + 300, 7] = math.inf, math.inf
+    tb.check(tb.adapter_forward(c.args(tb)))
+    y = c.y[:n, :r]
+    own = c.who == t % na
+    assert bool((y[t] == math.inf).all()) and bool((y[own, 300] == math.inf).all())
+    assert int(torch.isinf(y).sum()) == r + int(own.sum()) - 1 and not bool(torch.isnan(y).any())
+    c.b[(t % na) * r + 300, 7] = 0.5
+    c.dy[t, 9], c.a[(t % na) * rank + 5, 130] = math.inf, -math.inf
+    c.w[:, 130] = 0.0
+    tb.check(tb.adapter_backward(c.args(tb, da=None, db=None)))
+    dx = c.dx[:n, :d]
+    assert bool((dx[own, 130][c.who[own] >= 0] == -math.inf).sum() == int(own.sum()) - 1) and bool(torch.isnan(dx[t, 130]))
+    rest = torch.ones(d, dtype=torch.bool, device="cuda")
+    rest[130] = False
+    assert bool((dx[t, rest] == math.inf).all()) and int(torch.isinf(dx).sum()) == d - 1 + int(own.sum()) - 1
+
+
+def test_products_of_an_adapter_without_numbers_cost_no_more(cuda, tblib):
+    """One infinity in each factor, then an adapter of NaN: forward and input gradients take about the time that they take
+    without, but for the adapter's own tokens (the bar is 4 times)."""
+    torch, tb = cuda, tblib
+    n, d, r, rank, na = 4000, 2048, 2048, 32, 8
+    c = Case(torch, n, d, r, rank, na, who_of(torch, n, na, "runs"), 96)
+
+    def time(f):
+        times = []
+        for _ in range(8):
+            ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            ev[0].record()
+            tb.check(f())
+            ev[1].record()
+            torch.cuda.synchronize()
+            times.append(ev[0].elapsed_time(ev[1]))
+        return min(times)
+
+    calls = (lambda: tb.adapter_forward(c.args(tb)), lambda: tb.adapter_backward(c.args(tb, da=None, db=None)))
+    plain = [time(f) for f in calls]
+    c.b[r + 9, 5] = c.a[rank + 5, 9] = math.inf
+    assert all(time(f) <= 4 * p for f, p in zip(calls, plain))
+    c.b[r:2 * r] = math.nan
+    c.a[rank:2 * rank] = math.nan
+    assert all(time(f) <= 4 * p for f, p in zip(calls, plain))
+
+
 def test_gradients_of_rows_without_numbers_cost_no_more(cuda, tblib):
     """One infinity, one token of NaN: the factors' gradients take about the time that they take without (the bar is 4 times)."""
     torch, tb = cuda, tblib
