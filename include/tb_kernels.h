@@ -271,7 +271,8 @@ int tb_obs_sparsegpt_phase_times(float* ms_out, int n);
  * that feature reads back as NaN.  Other E are 1..249; checkpoints written by
  * other means keep to both.  Where a block's largest magnitude reaches 255 * 2^120
  * (BF16's largest value), E is 249, and its values from 254 * 2^120 on round to
- * 2^128: they read back, and count in every product below, as infinities. */
+ * 2^128: they read back as infinities, and count in the products below as those
+ * (with FP32 and F16 dy, whose parts may be zero, or as NaN). */
 #define TB_ACT8_BLOCK 128
 typedef struct tb_act8 {
     uint32_t struct_size;  /* sizeof(tb_act8)                                          */
