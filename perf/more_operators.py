@@ -31,29 +31,29 @@ MAX_LOSS, MAX_GRADS, MAX_STEP = 8000 * 4096 * 128000, 4001 * 8192 * 128000, 8192
 def listed():
     return [
         # The next token of one evaluated request: launch latency and one pass over the head.
-        dict(name="loss, one token", op="loss", n=1, d=4096, vocab=32000, left=0.0, cap=0.0),
+        dict(name="loss: one token", op="loss", n=1, d=4096, vocab=32000, left=0.0, cap=0.0),
         # A batch of calibration text at the 32000-entry head.
-        dict(name="loss, calibration batch", op="loss", n=2048, d=4096, vocab=32000, left=0.0, cap=0.0),
+        dict(name="loss: calibration batch", op="loss", n=2048, d=4096, vocab=32000, left=0.0, cap=0.0),
         # Perplexity over a long batch with a large vocabulary, prompts left out, capped logits.
-        dict(name="loss, large vocabulary", op="loss", n=8000, d=4096, vocab=128000, left=0.25, cap=30.0),
+        dict(name="loss: large vocabulary", op="loss", n=8000, d=4096, vocab=128000, left=0.25, cap=30.0),
         # One short sample's loss and gradients.
-        dict(name="gradients, short sample", op="grads", n=37, d=4096, vocab=32000, left=0.0, cap=0.0, dlse=False),
+        dict(name="gradients: short sample", op="grads", n=37, d=4096, vocab=32000, left=0.0, cap=0.0, dlse=False),
         # A batch of recovery training, prompts left out, with a penalty on lse.
-        dict(name="gradients, batch", op="grads", n=2048, d=4096, vocab=32000, left=0.25, cap=0.0, dlse=True),
+        dict(name="gradients: batch", op="grads", n=2048, d=4096, vocab=32000, left=0.25, cap=0.0, dlse=True),
         # The 8192-wide model with a large vocabulary, an odd number of tokens.
-        dict(name="gradients, 8192 wide", op="grads", n=4001, d=8192, vocab=128000, left=0.0, cap=30.0, dlse=False),
+        dict(name="gradients: 8192 wide", op="grads", n=4001, d=8192, vocab=128000, left=0.0, cap=30.0, dlse=False),
         # The 128 x 128 mock tensor's gradient.
-        dict(name="orthogonalise, mock", op="ortho", r=128, d=128, g="f32"),
+        dict(name="orthogonalise: mock", op="ortho", r=128, d=128, g="f32"),
         # A k_proj's gradient.
-        dict(name="orthogonalise, k_proj", op="ortho", r=1024, d=4096, g="bf16"),
+        dict(name="orthogonalise: k_proj", op="ortho", r=1024, d=4096, g="bf16"),
         # A gate_proj's, which is tall.
-        dict(name="orthogonalise, gate_proj", op="ortho", r=14336, d=4096, g="bf16"),
+        dict(name="orthogonalise: gate_proj", op="ortho", r=14336, d=4096, g="bf16"),
         # The step of the 128 x 128 mock tensor under its 2:4 mask.
-        dict(name="step, mock", op="step", r=128, d=128, g="f32", w="f32", m=4),
+        dict(name="step: mock", op="step", r=128, d=128, g="f32", w="f32", m=4),
         # A pruned q_proj in FP32, as the pruning pass leaves it.
-        dict(name="step, q_proj", op="step", r=4096, d=4096, g="bf16", w="f32", m=4),
+        dict(name="step: q_proj", op="step", r=4096, d=4096, g="bf16", w="f32", m=4),
         # The 8192-wide model's down_proj in BF16, 4:8.
-        dict(name="step, 28672 wide", op="step", r=8192, d=28672, g="bf16", w="bf16", m=8),
+        dict(name="step: 28672 wide", op="step", r=8192, d=28672, g="bf16", w="bf16", m=8),
     ]
 
 
