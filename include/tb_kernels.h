@@ -211,8 +211,8 @@ int tb_gemm_nt_bf16(const void* a, long long lda, const void* b, long long ldb, 
                     float alpha, float beta, const float* c_in, long long ldcin, float* c, long long ldc,
                     int lower_only, void* stream);
 /* TB_ERR_TIMEOUT if a bounded pipeline wait inside a GEMM, or inside a product
- * of the checkpoint and adapter entries below, launched since the last call
- * expired (the kernel then skipped its output); synchronises. */
+ * of the checkpoint, adapter, loss and update entries below, launched since the
+ * last call expired (the kernel then skipped its output); synchronises. */
 int tb_gemm_status(void* stream);
 
 /* ---- stage 3: column-block exact OBS against calibration activations ----- */
@@ -390,6 +390,54 @@ int tb_adapter_forward(const tb_adapter_args* args, void* stream);
  * and db where batches are long and these are small (at most 600 blocks of 128
  * features by 32 ranks). */
 int tb_adapter_backward(const tb_adapter_args* args, void* stream);
+
+/* ---- the loss at the LM head ---------------------------------------------- */
+/* Where the first dy of a calibration or recovery pass comes from: softmax cross
+ * entropy over the vocabulary and its gradients, without the logits in memory.
+ * No reference counterpart: the reference takes gradients from its caller
+ * (ehap.hpp:148-201).  For token t and entry v of the vocabulary
+ *     z_tv = cap(h_t . w_v),  cap(x) = x, or softcap * tanh(x / softcap)
+ *     lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,target[t].
+ * A token whose target lies outside [0, vocab) is left out: its loss, lse and dh
+ * are zeros, it adds nothing to dw, and it costs next to nothing, whatever its row
+ * of h (dloss, dlse) holds.  An infinity or a NaN in a token kept reaches that
+ * token's results and dw; one in w reaches all tokens. */
+typedef struct tb_lm_loss_args {
+    uint32_t struct_size;  /* sizeof(tb_lm_loss_args)                                    */
+    int32_t  dtype;        /* of h, w, dh, dw: TB_BF16                                   */
+    int64_t  n;            /* tokens, up to 2^31 - 65537                                 */
+    int32_t  d, vocab;     /* features and entries, each up to 2^31 - 257                */
+    const void* h;         /* [n][ldh], 16-byte aligned, ldh a multiple of 8             */
+    int64_t  ldh;
+    const void* w;         /* [vocab][ldw], 16-byte aligned, ldw a multiple of 8         */
+    int64_t  ldw;
+    const int64_t* target; /* [n], device                                                */
+    float    softcap;      /* 0: none                                                    */
+    float*   loss;         /* [n], device; forward only                                  */
+    float*   lse;          /* [n], device: written by the forward, read by the backward  */
+    /* backward */
+    const float* dloss;    /* [n], device                                                */
+    const float* dlse;     /* [n], device, or NULL (zeros): a penalty on lse, say        */
+    void*    dh;           /* [n][lddh], any stride, or NULL                             */
+    int64_t  lddh;
+    void*    dw;           /* [vocab][lddw], any stride, or NULL                         */
+    int64_t  lddw;
+} tb_lm_loss_args;
+/* loss and lse.  Logits are sums in FP32, up to 512 terms in the tensor core,
+ * whose additions cut off (2.6e-7 of the sum where all terms have one sign), and
+ * those added with rounding.  Scratch from the library's per-device pool: 2 bytes
+ * per value of h, and 16 bytes per token and 256 entries. */
+int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
+/* Gradients of sum_t dloss_t loss_t + dlse_t lse_t, with lse from the forward on the
+ * same h, w and targets:
+ *     g_tv = cap'(h_t . w_v) ((dloss_t + dlse_t) exp(z_tv - lse_t) - dloss_t [v = target[t]])
+ *     dh_t = sum_v g_tv w_v,   dw_v = sum_t g_tv h_t.
+ * The vocabulary is gone through in pieces whose g enters both products as BF16
+ * (2^-8 of each value).  dh and dw overwrite what is there; each sum has a fixed
+ * order.  n = 0 gives a dw of zeros.  Scratch: as above, 128 MB of g (more beyond
+ * 2^18 tokens), and 4 bytes per value of dh, up to 37 times that where few tokens
+ * and features make few tiles. */
+int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
 
 /* ---- fused score -> mask -> pack pass ------------------------------------ */
 /* One pass over a tensor: Fisher EMA over S gradient samples, importance,

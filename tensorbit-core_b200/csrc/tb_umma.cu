@@ -16,6 +16,7 @@
 #include <mutex>
 
 #include "tb_linear.cuh"
+#include "tb_lm_loss.cuh"
 #include "tb_pdl.cuh"
 #include "tb_runtime.h"
 #include "tb_tcgen05.cuh"
@@ -777,7 +778,8 @@ extern "C" int tb_gemm_status(void* stream) {
     if (rc) return rc;
     const int e1 = umma::gemm_take_error(static_cast<cudaStream_t>(stream));
     const int e2 = linear::take_error(static_cast<cudaStream_t>(stream));
-    const int e = e1 < 0 || e2 < 0 ? -1 : e1 | e2;
+    const int e3 = loss::take_error(static_cast<cudaStream_t>(stream));
+    const int e = e1 < 0 || e2 < 0 || e3 < 0 ? -1 : e1 | e2 | e3;
     if (e < 0) return fail(TB_ERR_CUDA, "reading the GEMM status failed");
     return e ? fail(TB_ERR_TIMEOUT, "a tcgen05 GEMM pipeline wait expired") : TB_OK;
 }

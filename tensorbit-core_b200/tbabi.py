@@ -109,6 +109,30 @@ class AdapterArgs(C.Structure):
     ]
 
 
+class LmLossArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("n", C.c_int64),
+        ("d", C.c_int32),
+        ("vocab", C.c_int32),
+        ("h", C.c_void_p),
+        ("ldh", C.c_int64),
+        ("w", C.c_void_p),
+        ("ldw", C.c_int64),
+        ("target", C.c_void_p),
+        ("softcap", C.c_float),
+        ("loss", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("dloss", C.c_void_p),
+        ("dlse", C.c_void_p),
+        ("dh", C.c_void_p),
+        ("lddh", C.c_int64),
+        ("dw", C.c_void_p),
+        ("lddw", C.c_int64),
+    ]
+
+
 def header_symbols() -> list[str]:
     """Names of every function declared in include/tb_kernels.h."""
     txt = open(HEADER).read()
@@ -182,6 +206,8 @@ def lib() -> C.CDLL:
             "tb_act8_hessian": ([C.POINTER(Act8), f32, i32, vp, vp], i32),
             "tb_adapter_forward": ([C.POINTER(AdapterArgs), vp], i32),
             "tb_adapter_backward": ([C.POINTER(AdapterArgs), vp], i32),
+            "tb_lm_loss": ([C.POINTER(LmLossArgs), vp], i32),
+            "tb_lm_loss_backward": ([C.POINTER(LmLossArgs), vp], i32),
             "tb_score_mask_pack": ([C.POINTER(PruneArgs), vp], i32),
             "tb_fisher_partial_scatter": ([vp, i32, sz, sz, sz, vp, i32, C.POINTER(C.c_uint64), C.POINTER(vp), i32,
                                            vp], i32),
@@ -290,3 +316,17 @@ def adapter_forward(args: AdapterArgs, stream=None) -> int:
 
 def adapter_backward(args: AdapterArgs, stream=None) -> int:
     return lib().tb_adapter_backward(C.byref(args), stream)
+
+
+def lm_loss_args(*, n, d, vocab, h, ldh, w, ldw, target, lse, loss=None, softcap=0.0, dloss=None, dlse=None, dh=None,
+                 lddh=0, dw=None, lddw=0, dtype=BF16) -> LmLossArgs:
+    return LmLossArgs(C.sizeof(LmLossArgs), dtype, n, d, vocab, h, ldh, w, ldw, target, softcap, loss, lse, dloss, dlse,
+                      dh, lddh, dw, lddw)
+
+
+def lm_loss(args: LmLossArgs, stream=None) -> int:
+    return lib().tb_lm_loss(C.byref(args), stream)
+
+
+def lm_loss_backward(args: LmLossArgs, stream=None) -> int:
+    return lib().tb_lm_loss_backward(C.byref(args), stream)
