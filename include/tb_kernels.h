@@ -439,6 +439,46 @@ int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
  * and features make few tiles. */
 int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
 
+/* ---- orthogonalised updates ------------------------------------------------ */
+/* O(U) by Newton-Schulz products: X = U / (|U|_F + eps), then `steps` (1..32, 5 is
+ * usual) times
+ *     X <- a X + (b A + c A^2) X,  A = X X^T,  (a, b, c) = (3.4445, -4.7750, 2.0315),
+ * which brings U's singular values near 1 and keeps its singular vectors.  No
+ * reference counterpart.  x is [r][ldx] of TB_F32 or TB_BF16, out [r][ldo] of
+ * TB_BF16, any strides; the shorter side ends at 32768.  Products keep 22 bits (two
+ * FP16 parts of each operand, FP32 sums): the result is within 5e-4 (2-norm) of the
+ * formula's, before it is rounded to BF16.  A zero matrix gives zeros; a NaN or an infinity makes all of out NaN.
+ * Scratch from the library's per-device pool: 8 bytes per value of x (4 up to three
+ * steps) and 24 for each of min(r, d)^2. */
+int tb_orthogonalize(const void* x, int x_dtype, int64_t ldx, int r, int d, void* out, int out_dtype, int64_t ldo,
+                     int steps, float eps, void* stream);
+/* One step of a pruned weight W [r][d] with gradient g:
+ *     m <- mask (beta m + g)
+ *     U =  mask (g + beta m) with nesterov, else m
+ *     W <- mask ((1 - lr weight_decay) W - lr scale O(U))
+ * Whatever a pruned weight, its gradient or its momentum held, its W and m are zeros
+ * afterwards.  Scratch as above. */
+typedef struct tb_muon_args {
+    uint32_t struct_size;  /* sizeof(tb_muon_args)                                       */
+    int32_t  r, d;         /* rows, columns                                              */
+    int32_t  g_dtype;      /* TB_F32 or TB_BF16, as tb_act8_weight_grad writes           */
+    const void* grad;      /* [r][ldg]                                                   */
+    int64_t  ldg;          /* 0 means d, as ldm and ldw                                  */
+    float*   momentum;     /* [r][ldm], or NULL: U = mask g                              */
+    int64_t  ldm;
+    void*    w;            /* [r][ldw]                                                   */
+    int64_t  ldw;
+    int32_t  w_dtype;      /* TB_F32 or TB_BF16                                          */
+    int32_t  nm_m;         /* weights of a byte of the mask, 1..8; r * d a multiple      */
+    const uint8_t* mask;   /* [r * d / nm_m], the .tb mask section, or NULL              */
+    float    beta, lr, weight_decay, scale;
+    float    eps;
+    int32_t  nesterov;
+    int32_t  steps;
+    int32_t  reserved;     /* 0                                                          */
+} tb_muon_args;
+int tb_muon_step(const tb_muon_args* args, void* stream);
+
 /* ---- fused score -> mask -> pack pass ------------------------------------ */
 /* One pass over a tensor: Fisher EMA over S gradient samples, importance,
  * CORING N:M mask, apply, redistribution, and emission of the .tb weight and

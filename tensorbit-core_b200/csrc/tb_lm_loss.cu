@@ -19,7 +19,7 @@
 #include "tb_pair_product.cuh"
 
 #ifndef TBG
-#define TBG 8
+#define TBG 16
 #endif
 namespace tb {
 namespace loss {
@@ -268,7 +268,7 @@ struct Logits {
 // 2^-8 of each of its values at most, which are summed with signs that do not depend on the errors'.
 struct Gradient {
     static constexpr bool kAMn = false, kBMn = false, kF16 = false;
-    static constexpr int kParts = 1, kGroup = 8;
+    static constexpr int kParts = 1, kGroup = 1 << 30;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return kept_tiles(p) * p.tiles_n; }

@@ -1,0 +1,610 @@
+// Orthogonalised updates by Newton-Schulz products, and the masked step of a pruned
+// weight that uses them.
+//
+//   X = U / (|U| + eps);  `steps` times X <- (a I + b A + c A^2) X,  A = X X^T
+//
+// on the shorter side of U (X^T X and X (...) where U is tall).  The polynomials
+// P(A) commute with A, so that several steps need X once:
+//
+//   P = a I + b A + c A^2,  Q <- P Q,  A <- P A P,  ...,  X <- Q X
+//
+// which takes symmetric products of the short side only, half of whose tiles are
+// computed.  What rounding adds to A grows by up to a^2 = 11.9 with each step that A is
+// carried through, in the directions whose singular values are far below the norm:
+// X is formed anew after at most three steps, and A from it.  (Five steps in one
+// go, with FP32's roundings: up to 6e-3 of the result for spectra that fall off; as three and
+// two 2e-4; BF16 results are off by 1.7e-3 in any case.  For k x d, products counted
+// by their tiles: 6 k^2 d + 14 k^3 so, 15 k^2 d + 5 k^3 with X formed in each step.)
+//
+// Operands are pairs of FP16 parts, hi + lo, of the values times a power of two that
+// each matrix has for good: 22 bits, as FP32 has 24, at the tensor core's FP16 rate; a
+// single FP16 (BF16) part would put 2e-3 (2e-2) of A's error into the directions
+// above.  Entries: |X|, |A|, |P A| <= 1.5, |P| <= 3.5, |Q| <= 3.5^3, which FP16's 65504 bounds.
+#include <algorithm>
+#include <cuda_fp16.h>
+
+#include "tb_muon.cuh"
+#include "tb_pair_product.cuh"
+
+namespace tb {
+namespace muon {
+namespace {
+
+using namespace tb::pair;
+using bf16 = __nv_bfloat16;
+
+__device__ int g_muon_error;
+
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr int kExpX = 14, kExpK = 13, kExpQ = 10;  // the powers of two of X; of A, P and P A; of Q
+constexpr int kSegment = 3;                        // steps between two formings of X
+
+// hi + lo of an FP32 value, as two FP16 in one word.
+__device__ __forceinline__ uint32_t split16(float x) {
+    const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
+    return static_cast<uint32_t>(__half_as_ushort(h)) | static_cast<uint32_t>(__half_as_ushort(l)) << 16;
+}
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+
+// ---- U, and X from it ---------------------------------------------------------------
+struct Source {
+    int r, d;
+    const void* g;
+    int g_bf16;
+    long long ldg;
+    float* m;         // momentum, or NULL
+    long long ldm;
+    float beta;
+    int nesterov;
+    const uint8_t* mask;
+    int group;        // weights of one mask byte
+    int shift;        // its logarithm, or -1
+};
+__device__ __forceinline__ bool kept(const Source& s, long long i) {
+    if (!s.mask) return true;
+    const long long at = s.shift >= 0 ? i >> s.shift : static_cast<long long>(static_cast<unsigned long long>(i) / static_cast<unsigned>(s.group));
+    return __ldg(s.mask + at) >> static_cast<int>(i - at * s.group) & 1;
+}
+// Four columns from `col`, zeros behind the row's end and for pruned weights.
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int col, int d, bool wide, float (&v)[4]) {
+    if (wide && col + 4 <= d) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(row + col);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+            const uint2 f = *reinterpret_cast<const uint2*>(row + col);
+            v[0] = __uint_as_float(f.x << 16); v[1] = __uint_as_float(f.x & 0xFFFF0000u);
+            v[2] = __uint_as_float(f.y << 16); v[3] = __uint_as_float(f.y & 0xFFFF0000u);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = col + e < d ? static_cast<float>(row[col + e]) : 0.0f;
+}
+__device__ __forceinline__ bool wide_rows(const void* p, long long ld, int size) {
+    return ((reinterpret_cast<uintptr_t>(p) | static_cast<unsigned long long>(ld) * size) & (4 * size - 1)) == 0;
+}
+// The momentum's new value (written if UPDATE) and U.
+template <bool UPDATE>
+__device__ __forceinline__ void update4(const Source& s, long long row, int col, float (&u)[4]) {
+    const bool g_wide = wide_rows(s.g, s.ldg, s.g_bf16 ? 2 : 4);
+    if (s.g_bf16) load4(static_cast<const bf16*>(s.g) + row * s.ldg, col, s.d, g_wide, u);
+    else load4(static_cast<const float*>(s.g) + row * s.ldg, col, s.d, g_wide, u);
+    bool keep[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        keep[e] = col + e < s.d && kept(s, row * s.d + col + e);
+        if (!keep[e]) u[e] = 0.0f;
+    }
+    if (!s.m) return;
+    float* at = s.m + row * s.ldm;
+    const bool m_wide = wide_rows(s.m, s.ldm, 4);
+    float m[4];
+    load4(at, col, s.d, m_wide, m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (UPDATE) m[e] = keep[e] ? fmaf(s.beta, m[e], u[e]) : 0.0f;
+        u[e] = s.nesterov ? fmaf(s.beta, m[e], u[e]) : m[e];
+    }
+    if constexpr (UPDATE) {
+        if (m_wide && col + 4 <= s.d) *reinterpret_cast<float4*>(at + col) = make_float4(m[0], m[1], m[2], m[3]);
+        else
+            for (int e = 0; e < 4 && col + e < s.d; ++e) at[col + e] = m[e];
+    }
+}
+constexpr int kNormBlocks = 592;
+// Of 256 threads, in a fixed order; for all of them.
+__device__ __forceinline__ double block_sum(double v, double* shared) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += shared[i];
+    return s;
+}
+// The momentum's step, and each block's part of |U|^2.  (In 64 bits: the squares of small gradients
+// leave FP32's range.)
+__global__ void __launch_bounds__(256) norm_kernel(const Source s, double* partial) {
+    __shared__ double shared[8];
+    const int units = (s.d + 3) / 4;
+    const long long all = static_cast<long long>(s.r) * units;
+    double sum = 0.0;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+        const long long row = static_cast<unsigned long long>(i) / static_cast<unsigned>(units);
+        float u[4];
+        update4<true>(s, row, 4 * static_cast<int>(i - row * units), u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fma(static_cast<double>(u[e]), static_cast<double>(u[e]), sum);
+    }
+    sum = block_sum(sum, shared);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+// X's parts, in rows of ld.
+__global__ void __launch_bounds__(256) scale_kernel(const Source s, const double* partial, const int parts, const float eps, uint16_t* hi, uint16_t* lo,
+                                                    const long long ld) {
+    __shared__ double shared[8];
+    pdl_wait();
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) sum += partial[i];
+    sum = block_sum(sum, shared);
+    const double scale = static_cast<double>(1 << kExpX) / (sqrt(sum) + static_cast<double>(eps));
+    const int units = (s.d + 3) / 4;
+    const long long all = static_cast<long long>(s.r) * units;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+        const long long row = static_cast<unsigned long long>(i) / static_cast<unsigned>(units);
+        const int col = 4 * static_cast<int>(i - row * units);
+        float u[4];
+        update4<false>(s, row, col, u);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = split16(sum == 0.0 ? 0.0f : static_cast<float>(u[e] * scale));
+        const long long at = row * ld + col;
+        *reinterpret_cast<uint2*>(hi + at) = make_uint2(low_halves(w[0], w[1]), low_halves(w[2], w[3]));
+        *reinterpret_cast<uint2*>(lo + at) = make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]));
+    }
+}
+
+// ---- products -----------------------------------------------------------------------
+struct Params {
+    int m, n, k;          // of the product
+    int tiles_m, tiles_n;
+    int products;
+    float alpha[2];       // powers of two (times c): of what the sums are multiplied by
+    float beta, diagonal; // P: of A and I
+    const uint16_t* c[2]; // P: A's parts
+    uint16_t* out[2][2];  // [product][part]
+    long long ld;         // of c and out
+    // results
+    void* result;
+    long long ldr;
+    const uint8_t* mask;
+    int group, shift, w_bf16;
+    float decay, step;    // W <- mask (decay W - step O)
+};
+
+// Fills a piece of 64 columns x 32 rows with one part of `v`.
+template <bool LO>
+__device__ __forceinline__ void fill_part(uint8_t* buf, const uint32_t* v, int lane) {
+    uint8_t* row = buf + lane * 128;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t* x = v + 8 * j;
+        uint4 w;
+        if constexpr (LO) w = make_uint4(high_halves(x[0], x[1]), high_halves(x[2], x[3]), high_halves(x[4], x[5]), high_halves(x[6], x[7]));
+        else w = make_uint4(low_halves(x[0], x[1]), low_halves(x[2], x[3]), low_halves(x[4], x[5]), low_halves(x[6], x[7]));
+        *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = w;
+    }
+}
+__device__ __forceinline__ void store_part(const CUtensorMap* map, uint8_t* buf, int col, int row, int lane) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(col),
+                     "r"(row), "r"(0), "r"(smem_u32(buf))
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+// The lane's row of 128 columns, split, as rows of both parts.
+__device__ __forceinline__ void store_split(const CUtensorMap (&maps)[2], uint8_t* buf, const uint32_t (&v)[128], int col, int row0, int n, int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        if (col + 64 * c >= n) break;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+            if (part) fill_part<true>(buf, v + 64 * c, lane);
+            else fill_part<false>(buf, v + 64 * c, lane);
+            store_part(&maps[part], buf, col + 64 * c, row0, lane);
+        }
+    }
+}
+
+// A symmetric matrix: its tiles on and below the diagonal, each written where it is
+// and mirrored.  MN: operands in memory along M and N (X^T X).  Sums of 256 terms in the
+// tensor core.
+template <bool MN>
+struct Symmetric {
+    static constexpr bool kAMn = MN, kBMn = MN, kF16 = true;
+    static constexpr int kParts = 2, kGroup = 4;
+    using Params = muon::Params;
+    static __device__ __forceinline__ int* error() { return &g_muon_error; }
+    static __device__ __forceinline__ int items(const Params& p) { return p.tiles_m * (p.tiles_m + 1) / 2 * p.products; }
+    static __device__ __forceinline__ Work work(const Params& p, int item) {
+        const int unit = p.products > 1 ? item >> 1 : item;
+        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(unit) + 1.0f) - 1.0f) * 0.5f);
+        while (tm * (tm + 1) / 2 > unit) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= unit) ++tm;
+        return Work{tm, unit - tm * (tm + 1) / 2, 0, (p.k + 63) / 64, p.products > 1 ? item & 1 : 0, -1};
+    }
+    static __device__ __forceinline__ void finish(const Launch<Symmetric>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
+        const Params& p = L.p;
+        const int row0 = w.tm * 256 + row_in, row = row0 + lane, col = w.tn * 256 + half * 128;
+        if (col / 128 > row0 / 128 || row0 >= p.m || col >= p.n) return;
+        const float alpha = p.alpha[w.which];
+        uint32_t v[128];
+        if (p.c[0] && row < p.m) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (col + 8 * j >= p.n) break;  // (rows of ld, a multiple of 8)
+                const long long at = row * p.ld + col + 8 * j;
+                const uint4 h = *reinterpret_cast<const uint4*>(p.c[0] + at), l = *reinterpret_cast<const uint4*>(p.c[1] + at);
+                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
+                    float& x = acc[8 * j + 2 * e];
+                    float& y = acc[8 * j + 2 * e + 1];
+                    x = fmaf(p.beta, hf.x, fmaf(p.beta, lf.x, x * alpha));
+                    y = fmaf(p.beta, hf.y, fmaf(p.beta, lf.y, y * alpha));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] + (col + i == row ? p.diagonal : 0.0f));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] * alpha);
+        }
+        store_split(L.o[w.which], buf, v, col, row0, p.n, lane);
+        if (col / 128 == row0 / 128) return;
+        // mirrored: two lanes exchange, so that each has two rows of one column
+        uint16_t* hi = p.out[w.which][0];
+        uint16_t* lo = p.out[w.which][1];
+        const bool odd = lane & 1, whole = row0 + 32 <= p.m;
+#pragma unroll
+        for (int i = 0; i < 128; i += 2) {
+            const uint32_t other = __shfl_xor_sync(~0u, odd ? v[i] : v[i + 1], 1);
+            const uint32_t first = odd ? other : v[i], second = odd ? v[i + 1] : other;
+            const long long at = (col + i + odd) * p.ld + (row & ~1);
+            if (whole || (row | 1) < p.m) {
+                *reinterpret_cast<uint32_t*>(hi + at) = low_halves(first, second);
+                *reinterpret_cast<uint32_t*>(lo + at) = high_halves(first, second);
+            } else if ((row & ~1) < p.m) {
+                hi[at] = static_cast<uint16_t>(first & 0xFFFFu);
+                lo[at] = static_cast<uint16_t>(first >> 16);
+            }
+        }
+    }
+};
+
+// X's product with Q: X's parts again, BF16 results, or the weights' step.  BMN: Q X, else X Q.
+enum Out { kSplit = 0, kBf16 = 1, kWeights = 2 };
+template <bool BMN, int OUT>
+struct Apply {
+    static constexpr bool kAMn = false, kBMn = BMN, kF16 = true;
+    static constexpr int kParts = 2, kGroup = 4;
+    using Params = muon::Params;
+    static __device__ __forceinline__ int* error() { return &g_muon_error; }
+    static __device__ __forceinline__ int items(const Params& p) { return p.tiles_m * p.tiles_n; }
+    static __device__ __forceinline__ Work work(const Params& p, int item) {
+        Work w{0, 0, 0, (p.k + 63) / 64, 0, -1};
+        band_tile(item, p.tiles_m, p.tiles_n, w.tm, w.tn);
+        return w;
+    }
+    static __device__ __forceinline__ void finish(const Launch<Apply>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
+        const Params& p = L.p;
+        const int row0 = w.tm * 256 + row_in, col = w.tn * 256 + half * 128;
+        const int rows = min(32, p.m - row0), cols = p.n - col;
+        if (rows <= 0 || cols <= 0) return;
+        const float alpha = p.alpha[0];
+        if constexpr (OUT == kSplit) {
+            uint32_t v[128];
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] * alpha);
+            store_split(L.o[0], buf, v, col, row0, p.n, lane);
+        } else if constexpr (OUT == kBf16) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i] *= alpha;
+            store_rows<true>(buf, acc, static_cast<bf16*>(p.result) + row0 * p.ldr + col, p.ldr, rows, cols, lane);
+        } else {
+            const float step = p.step * alpha;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (32 * c >= cols) break;
+                __syncwarp();
+                fill_piece<false>(buf, acc, c, lane);
+                __syncwarp();
+                update_rows(p, buf, row0, col + 32 * c + lane, rows, 32 * c + lane < cols, step, lane);
+            }
+        }
+    }
+    // One column of up to 32 rows of weights a lane.
+    static __device__ __noinline__ void update_rows(const Params& p, const uint8_t* buf, int row0, int col, int rows, bool inside, float step, int lane) {
+        if (!inside) return;
+        constexpr int kBatch = 16;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += kBatch) {
+            float w[kBatch];
+            uint32_t bits[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int r = min(r0 + i, rows - 1);
+                const long long at = (row0 + r) * p.ldr + col;
+                w[i] = p.w_bf16 ? __bfloat162float(static_cast<const bf16*>(p.result)[at]) : static_cast<const float*>(p.result)[at];
+                bits[i] = 1;
+                if (p.mask) {
+                    const long long flat = static_cast<long long>(row0 + r) * p.n + col;
+                    const long long group = p.shift >= 0 ? flat >> p.shift : static_cast<long long>(static_cast<unsigned long long>(flat) / static_cast<unsigned>(p.group));
+                    bits[i] = __ldg(p.mask + group) >> static_cast<int>(flat - group * p.group);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int r = r0 + i;
+                if (r >= rows) break;
+                const float o = *reinterpret_cast<const float*>(buf + piece_at(r, 4 * lane));
+                const float x = bits[i] & 1 ? fmaf(-step, o, p.decay * w[i]) : 0.0f;
+                const long long at = (row0 + r) * p.ldr + col;
+                if (p.w_bf16) static_cast<bf16*>(p.result)[at] = __float2bfloat16_rn(x);
+                else static_cast<float*>(p.result)[at] = x;
+            }
+        }
+    }
+};
+
+long long up(long long v, long long m) { return (v + m - 1) / m * m; }
+
+struct Matrix {
+    uint16_t* part[2];
+    long long rows, cols, ld;
+    int exp;
+};
+float power(int e) { return ldexpf(1.0f, e); }
+
+int operand_maps(CUtensorMap (&maps)[2], const Matrix& x, bool mn) {
+    int rc = TB_OK;
+    for (int q = 0; q < 2 && !rc; ++q) rc = operand_map(&maps[q], x.part[q], x.rows, x.cols, x.ld, mn);
+    return rc;
+}
+int out_maps(CUtensorMap (&maps)[2], const Matrix& x) {
+    int rc = TB_OK;
+    for (int q = 0; q < 2 && !rc; ++q) rc = make_out_map(&maps[q], x.part[q], true, x.cols, x.rows, 1, x.ld, x.ld * x.rows);
+    return rc;
+}
+
+// out = scale A B^T (MN: scale A^T B), a symmetric matrix; plus beta C + diagonal I where C is given.
+// With a second B and out, two products with the same A.
+template <bool MN>
+int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, const Matrix* c, float beta, float diagonal, const Matrix* b2, const Matrix* out2,
+              cudaStream_t st) {
+    Launch<Symmetric<MN>> L{};
+    Params& p = L.p;
+    p.m = p.n = static_cast<int>(out.rows);
+    p.k = static_cast<int>(MN ? a.rows : a.cols);
+    p.tiles_m = tiles(p.m, 256);
+    p.products = b2 ? 2 : 1;
+    p.ld = out.ld;
+    int rc = operand_maps(L.a, a, MN);
+    if (!rc) rc = operand_maps(L.b[0], b, MN);
+    if (!rc) rc = out_maps(L.o[0], out);
+    if (!rc && b2) rc = operand_maps(L.b[1], *b2, MN);
+    if (!rc && b2) rc = out_maps(L.o[1], *out2);
+    if (rc) return rc;
+    p.alpha[0] = scale * power(out.exp - a.exp - b.exp);
+    if (b2) p.alpha[1] = scale * power(out2->exp - a.exp - b2->exp);
+    for (int q = 0; q < 2; ++q) {
+        p.out[0][q] = out.part[q];
+        if (b2) p.out[1][q] = out2->part[q];
+        if (c) p.c[q] = c->part[q];
+    }
+    if (c) {
+        p.beta = beta * power(out.exp - c->exp);
+        p.diagonal = diagonal * power(out.exp);
+    }
+    return launch_product(L, static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * p.products, st);
+}
+
+struct Result {
+    void* out;
+    long long ld;
+    const uint8_t* mask;
+    int group, shift, w_bf16;
+    float decay, step;
+};
+// X (Q X, tall: X Q) into `out`, or into the result.
+template <bool BMN, int OUT>
+int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
+    Launch<Apply<BMN, OUT>> L{};
+    Params& p = L.p;
+    p.m = static_cast<int>(x.rows);
+    p.n = static_cast<int>(x.cols);
+    p.k = static_cast<int>(q.rows);
+    p.tiles_m = tiles(p.m, 256);
+    p.tiles_n = tiles(p.n, 256);
+    int rc = operand_maps(L.a, BMN ? q : x, false);
+    if (!rc) rc = operand_maps(L.b[0], BMN ? x : q, BMN);
+    if (!rc && OUT == kSplit) rc = out_maps(L.o[0], out);
+    if (rc) return rc;
+    p.alpha[0] = power((OUT == kSplit ? out.exp : 0) - q.exp - x.exp);
+    p.result = res.out;
+    p.ldr = res.ld;
+    p.mask = res.mask;
+    p.group = res.group;
+    p.shift = res.shift;
+    p.w_bf16 = res.w_bf16;
+    p.decay = res.decay;
+    p.step = res.step;
+    return launch_product(L, static_cast<long long>(p.tiles_m) * p.tiles_n, st);
+}
+template <int OUT>
+int apply(bool tall, const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
+    return tall ? apply<false, OUT>(q, x, out, res, st) : apply<true, OUT>(q, x, out, res, st);
+}
+
+// O(U) to the result.
+template <int OUT>
+int orthogonalize(const Source& s, int steps, float eps, const Result& res, cudaStream_t st) {
+    const bool tall = s.r > s.d;
+    const long long k = std::min(s.r, s.d), ldx = up(s.d, 8), ldk = up(k, 8);
+    const size_t x_bytes = up(2 * s.r * ldx, 256), k_bytes = up(2 * k * ldk, 256);
+    const int segments = (steps + kSegment - 1) / kSegment;
+    void* base = nullptr;
+    int rc = scratch_alloc(&base, 8 * kNormBlocks + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
+    if (rc) return rc;
+    char* at = static_cast<char*>(base);
+    double* partial = reinterpret_cast<double*>(at);
+    at += up(8 * kNormBlocks, 256);
+    auto matrix = [&](long long rows, long long cols, long long ld, size_t bytes, int exp) {
+        Matrix x{{reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + bytes)}, rows, cols, ld, exp};
+        at += 2 * bytes;
+        return x;
+    };
+    Matrix x = matrix(s.r, s.d, ldx, x_bytes, kExpX), x2 = x;
+    if (segments > 1) x2 = matrix(s.r, s.d, ldx, x_bytes, kExpX);
+    Matrix A = matrix(k, k, ldk, k_bytes, kExpK), T = matrix(k, k, ldk, k_bytes, kExpK);
+    Matrix P[2] = {matrix(k, k, ldk, k_bytes, kExpK), matrix(k, k, ldk, k_bytes, kExpK)};
+    Matrix Q[2] = {matrix(k, k, ldk, k_bytes, kExpQ), matrix(k, k, ldk, k_bytes, kExpQ)};
+
+    const long long units = static_cast<long long>(s.r) * ((s.d + 3) / 4);
+    const unsigned blocks = static_cast<unsigned>(std::min<long long>((units + 255) / 256, kNormBlocks));
+    norm_kernel<<<blocks, 256, 0, st>>>(s, partial);
+    rc = check_launch("norm_kernel");
+    if (!rc) {
+        const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx);
+        rc = e == cudaSuccess ? check_launch("scale_kernel") : cuda_fail(e, "scale_kernel launch");
+    }
+    for (int seg = 0; seg < segments && !rc; ++seg) {
+        const int n = steps * (seg + 1) / segments - steps * seg / segments;
+        rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+        Matrix q = P[0];
+        for (int i = 0; i < n && !rc; ++i) {
+            const Matrix& p = P[i & 1];
+            rc = symmetric<false>(A, A, p, kC, &A, kB, kA, nullptr, nullptr, st);
+            const Matrix& next = Q[i & 1];
+            const bool last = i == n - 1;
+            if (!rc && !last) rc = i ? symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, &q, &next, st) : symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+            if (!rc && !last) rc = symmetric<false>(p, T, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+            if (!rc && last && i) rc = symmetric<false>(p, q, next, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+            if (i) q = next;
+        }
+        if (rc) break;
+        if (seg < segments - 1) {
+            rc = apply<kSplit>(tall, q, x, x2, res, st);
+            std::swap(x, x2);
+        } else {
+            rc = apply<OUT>(tall, q, x, x, res, st);
+        }
+    }
+    scratch_free(base, st);
+    return rc;
+}
+
+int shift_of(int m) { return m == 1 ? 0 : m == 2 ? 1 : m == 4 ? 2 : m == 8 ? 3 : -1; }
+
+int check_shape(const char* who, int r, int d, int steps, float eps) {
+    if (r <= 0 || d <= 0) return fail(TB_ERR_ZERO_SIZE, "%s: empty matrix", who);
+    if (r > 0x7FFFFFFF - 256 || d > 0x7FFFFFFF - 256) return fail(TB_ERR_SHAPE, "%s: %d x %d", who, r, d);
+    if (std::min(r, d) > 32768) return fail(TB_ERR_CAPACITY, "%s: %d x %d: the shorter side ends at 32768", who, r, d);
+    if (static_cast<long long>((r + 255) / 256) * ((d + 255) / 256) > 0x3FFFFFFFll) return fail(TB_ERR_CAPACITY, "%s: %d x %d", who, r, d);
+    if (steps < 1 || steps > 32) return fail(TB_ERR_CONFIG, "%s: %d steps", who, steps);
+    if (!(eps >= 0.0f && eps < INFINITY)) return fail(TB_ERR_CONFIG, "%s: eps %g", who, eps);
+    return TB_OK;
+}
+bool misaligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == TB_F32 ? 4 : 2) != 0; }
+
+}  // namespace
+
+int take_error(cudaStream_t st) {
+    int h = 0, zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&h, g_muon_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_muon_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    return e == cudaSuccess ? h : -1;
+}
+
+}  // namespace muon
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" int tb_orthogonalize(const void* x, int x_dtype, int64_t ldx, int r, int d, void* out, int out_dtype, int64_t ldo, int steps, float eps,
+                                void* stream) {
+    constexpr const char* who = "tb_orthogonalize";
+    if (x_dtype != TB_F32 && x_dtype != TB_BF16) return fail(x_dtype == TB_F16 ? TB_ERR_UNSUPPORTED : TB_ERR_ARG, "%s: x of dtype %d", who, x_dtype);
+    if (out_dtype != TB_BF16) return fail(out_dtype == TB_F16 || out_dtype == TB_F32 ? TB_ERR_UNSUPPORTED : TB_ERR_ARG, "%s: out of dtype %d", who, out_dtype);
+    int rc = muon::check_shape(who, r, d, steps, eps);
+    if (rc) return rc;
+    if (!x || !out || muon::misaligned(x, x_dtype) || muon::misaligned(out, out_dtype)) return fail(TB_ERR_ARG, "%s: null or misaligned pointer", who);
+    if (ldx < d || ldo < d) return fail(TB_ERR_ARG, "%s: a row stride below d", who);
+    if ((rc = require_device(nullptr))) return rc;
+    muon::Source s{};
+    s.r = r;
+    s.d = d;
+    s.g = x;
+    s.g_bf16 = x_dtype == TB_BF16;
+    s.ldg = ldx;
+    muon::Result res{};
+    res.out = out;
+    res.ld = ldo;
+    return muon::orthogonalize<muon::kBf16>(s, steps, eps, res, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tb_muon_step(const tb_muon_args* p, void* stream) {
+    constexpr const char* who = "tb_muon_step";
+    if (!p || p->struct_size != sizeof(tb_muon_args)) return fail(TB_ERR_ARG, "%s: null args or bad struct_size", who);
+    if (p->g_dtype != TB_F32 && p->g_dtype != TB_BF16) return fail(p->g_dtype == TB_F16 ? TB_ERR_UNSUPPORTED : TB_ERR_ARG, "%s: gradient of dtype %d", who, p->g_dtype);
+    if (p->w_dtype != TB_F32 && p->w_dtype != TB_BF16) return fail(p->w_dtype == TB_F16 ? TB_ERR_UNSUPPORTED : TB_ERR_ARG, "%s: weights of dtype %d", who, p->w_dtype);
+    int rc = muon::check_shape(who, p->r, p->d, p->steps, p->eps);
+    if (rc) return rc;
+    if (!p->grad || !p->w || muon::misaligned(p->grad, p->g_dtype) || muon::misaligned(p->w, p->w_dtype) || muon::misaligned(p->momentum, TB_F32))
+        return fail(TB_ERR_ARG, "%s: null or misaligned pointer", who);
+    const int64_t ldg = p->ldg ? p->ldg : p->d, ldm = p->ldm ? p->ldm : p->d, ldw = p->ldw ? p->ldw : p->d;
+    if (ldg < p->d || ldm < p->d || ldw < p->d) return fail(TB_ERR_ARG, "%s: a row stride below d", who);
+    if (p->mask) {
+        if (p->nm_m < 1) return fail(TB_ERR_CONFIG, "%s: a mask of groups of %d", who, p->nm_m);
+        if (p->nm_m > 8) return fail(TB_ERR_UNSUPPORTED, "%s: M=%d > 8: masks hold one byte per group", who, p->nm_m);
+        if (static_cast<int64_t>(p->r) * p->d % p->nm_m) return fail(TB_ERR_SHAPE, "%s: %d x %d is not a multiple of %d", who, p->r, p->d, p->nm_m);
+    }
+    for (float v : {p->beta, p->lr, p->weight_decay, p->scale})
+        if (!(v > -INFINITY && v < INFINITY)) return fail(TB_ERR_CONFIG, "%s: a factor that is not finite", who);
+    if ((rc = require_device(nullptr))) return rc;
+    muon::Source s{};
+    s.r = p->r;
+    s.d = p->d;
+    s.g = p->grad;
+    s.g_bf16 = p->g_dtype == TB_BF16;
+    s.ldg = ldg;
+    s.m = p->momentum;
+    s.ldm = ldm;
+    s.beta = p->beta;
+    s.nesterov = p->nesterov;
+    s.mask = p->mask;
+    s.group = p->nm_m;
+    s.shift = muon::shift_of(p->nm_m);
+    muon::Result res{};
+    res.out = p->w;
+    res.ld = ldw;
+    res.mask = p->mask;
+    res.group = p->nm_m;
+    res.shift = s.shift;
+    res.w_bf16 = p->w_dtype == TB_BF16;
+    res.decay = static_cast<float>(1.0 - static_cast<double>(p->lr) * p->weight_decay);
+    res.step = static_cast<float>(static_cast<double>(p->lr) * p->scale);
+    return muon::orthogonalize<muon::kWeights>(s, p->steps, p->eps, res, static_cast<cudaStream_t>(stream));
+}

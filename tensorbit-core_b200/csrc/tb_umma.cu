@@ -17,6 +17,7 @@
 
 #include "tb_linear.cuh"
 #include "tb_lm_loss.cuh"
+#include "tb_muon.cuh"
 #include "tb_pdl.cuh"
 #include "tb_runtime.h"
 #include "tb_tcgen05.cuh"
@@ -779,7 +780,8 @@ extern "C" int tb_gemm_status(void* stream) {
     const int e1 = umma::gemm_take_error(static_cast<cudaStream_t>(stream));
     const int e2 = linear::take_error(static_cast<cudaStream_t>(stream));
     const int e3 = loss::take_error(static_cast<cudaStream_t>(stream));
-    const int e = e1 < 0 || e2 < 0 || e3 < 0 ? -1 : e1 | e2 | e3;
+    const int e4 = muon::take_error(static_cast<cudaStream_t>(stream));
+    const int e = e1 < 0 || e2 < 0 || e3 < 0 || e4 < 0 ? -1 : e1 | e2 | e3 | e4;
     if (e < 0) return fail(TB_ERR_CUDA, "reading the GEMM status failed");
     return e ? fail(TB_ERR_TIMEOUT, "a tcgen05 GEMM pipeline wait expired") : TB_OK;
 }

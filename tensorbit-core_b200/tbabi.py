@@ -133,6 +133,32 @@ class LmLossArgs(C.Structure):
     ]
 
 
+class MuonArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("r", C.c_int32),
+        ("d", C.c_int32),
+        ("g_dtype", C.c_int32),
+        ("grad", C.c_void_p),
+        ("ldg", C.c_int64),
+        ("momentum", C.c_void_p),
+        ("ldm", C.c_int64),
+        ("w", C.c_void_p),
+        ("ldw", C.c_int64),
+        ("w_dtype", C.c_int32),
+        ("nm_m", C.c_int32),
+        ("mask", C.c_void_p),
+        ("beta", C.c_float),
+        ("lr", C.c_float),
+        ("weight_decay", C.c_float),
+        ("scale", C.c_float),
+        ("eps", C.c_float),
+        ("nesterov", C.c_int32),
+        ("steps", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 def header_symbols() -> list[str]:
     """Names of every function declared in include/tb_kernels.h."""
     txt = open(HEADER).read()
@@ -208,6 +234,8 @@ def lib() -> C.CDLL:
             "tb_adapter_backward": ([C.POINTER(AdapterArgs), vp], i32),
             "tb_lm_loss": ([C.POINTER(LmLossArgs), vp], i32),
             "tb_lm_loss_backward": ([C.POINTER(LmLossArgs), vp], i32),
+            "tb_orthogonalize": ([vp, i32, i64, i32, i32, vp, i32, i64, i32, f32, vp], i32),
+            "tb_muon_step": ([C.POINTER(MuonArgs), vp], i32),
             "tb_score_mask_pack": ([C.POINTER(PruneArgs), vp], i32),
             "tb_fisher_partial_scatter": ([vp, i32, sz, sz, sz, vp, i32, C.POINTER(C.c_uint64), C.POINTER(vp), i32,
                                            vp], i32),
@@ -330,3 +358,17 @@ def lm_loss(args: LmLossArgs, stream=None) -> int:
 
 def lm_loss_backward(args: LmLossArgs, stream=None) -> int:
     return lib().tb_lm_loss_backward(C.byref(args), stream)
+
+
+def orthogonalize(x, x_dtype, ldx, r, d, out, out_dtype, ldo, *, steps=5, eps=1e-7, stream=None) -> int:
+    return lib().tb_orthogonalize(x, x_dtype, ldx, r, d, out, out_dtype, ldo, steps, eps, stream)
+
+
+def muon_args(*, r, d, grad, g_dtype, w, w_dtype, lr, momentum=None, mask=None, nm_m=0, beta=0.95, weight_decay=0.0,
+              scale=1.0, nesterov=True, steps=5, eps=1e-7, ldg=0, ldm=0, ldw=0) -> MuonArgs:
+    return MuonArgs(C.sizeof(MuonArgs), r, d, g_dtype, grad, ldg, momentum, ldm, w, ldw, w_dtype, nm_m, mask, beta, lr,
+                    weight_decay, scale, eps, int(nesterov), steps, 0)
+
+
+def muon_step(args: MuonArgs, stream=None) -> int:
+    return lib().tb_muon_step(C.byref(args), stream)
