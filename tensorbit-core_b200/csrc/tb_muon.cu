@@ -25,6 +25,7 @@
 
 #include "tb_muon.cuh"
 #include "tb_pair_product.cuh"
+#include "tb_split_product.cuh"
 
 namespace tb {
 namespace muon {
@@ -226,6 +227,14 @@ __device__ __forceinline__ void store_split(const CUtensorMap (&maps)[2], uint8_
     }
 }
 
+// Tile `unit` of those on and below the diagonal, row by row.
+__device__ __forceinline__ void lower_tile(int unit, int& tm, int& tn) {
+    tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(unit) + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > unit) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= unit) ++tm;
+    tn = unit - tm * (tm + 1) / 2;
+}
+
 // A symmetric matrix: its tiles on and below the diagonal, each written where it is
 // and mirrored.  MN: operands in memory along M and N (X^T X).  Sums of 256 terms in the
 // tensor core.
@@ -237,11 +246,49 @@ struct Symmetric {
     static __device__ __forceinline__ int* error() { return &g_muon_error; }
     static __device__ __forceinline__ int items(const Params& p) { return p.tiles_m * (p.tiles_m + 1) / 2 * p.products; }
     static __device__ __forceinline__ Work work(const Params& p, int item) {
-        const int unit = p.products > 1 ? item >> 1 : item;
-        int tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(unit) + 1.0f) - 1.0f) * 0.5f);
-        while (tm * (tm + 1) / 2 > unit) --tm;
-        while ((tm + 1) * (tm + 2) / 2 <= unit) ++tm;
-        return Work{tm, unit - tm * (tm + 1) / 2, 0, (p.k + 63) / 64, p.products > 1 ? item & 1 : 0, -1};
+        Work w{0, 0, 0, (p.k + 63) / 64, p.products > 1 ? item & 1 : 0, -1};
+        lower_tile(p.products > 1 ? item >> 1 : item, w.tm, w.tn);
+        return w;
+    }
+    static __device__ __forceinline__ Work split_work(const Params& p, int item) { return work(p, item); }
+    static constexpr bool kMirror = true;
+    static __device__ __forceinline__ void finish_quad(const Launch<Symmetric>& L, const Work& w, int row, int col, const float4& v, uint4& words) {
+        const Params& p = L.p;
+        const float alpha = p.alpha[w.which];
+        const bool inside = row < p.m && col < p.n;
+        const long long at = row * p.ld + col;  // (rows of ld, a multiple of 8)
+        float x[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
+        if (p.c[0] && inside) {
+            const uint2 h = *reinterpret_cast<const uint2*>(p.c[0] + at), l = *reinterpret_cast<const uint2*>(p.c[1] + at);
+            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+            const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&l.x)), l1 = __half22float2(*reinterpret_cast<const __half2*>(&l.y));
+            const float hs[4] = {h0.x, h0.y, h1.x, h1.y}, ls[4] = {l0.x, l0.y, l1.x, l1.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(p.beta, hs[e], fmaf(p.beta, ls[e], x[e])) + (row == col + e ? p.diagonal : 0.0f);
+        }
+        words = make_uint4(split16(x[0]), split16(x[1]), split16(x[2]), split16(x[3]));
+        if (inside) {
+            *reinterpret_cast<uint2*>(p.out[w.which][0] + at) = make_uint2(low_halves(words.x, words.y), low_halves(words.z, words.w));
+            *reinterpret_cast<uint2*>(p.out[w.which][1] + at) = make_uint2(high_halves(words.x, words.y), high_halves(words.z, words.w));
+        }
+    }
+    // Two rows of a column at a time (columns left of the diagonal's tile all exist).
+    static __device__ __forceinline__ void mirror(const Launch<Symmetric>& L, const Work& w, const uint32_t* words, int pitch, int row0, int rows, int thread) {
+        if (w.tm == w.tn) return;
+        const Params& p = L.p;
+        uint16_t* hi = p.out[w.which][0];
+        uint16_t* lo = p.out[w.which][1];
+        const int pairs = min(rows, p.m - row0 + 1) / 2;
+        for (int r = 2 * (thread / 64); r < 2 * pairs; r += 6) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = thread % 64 + 64 * h;
+                const uint32_t a = words[r * pitch + c], b = words[(r + 1) * pitch + c];
+                const long long at = (w.tn * 128 + c) * p.ld + row0 + r;
+                *reinterpret_cast<uint32_t*>(hi + at) = low_halves(a, b);
+                *reinterpret_cast<uint32_t*>(lo + at) = high_halves(a, b);
+            }
+        }
     }
     static __device__ __forceinline__ void finish(const Launch<Symmetric>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
         const Params& p = L.p;
@@ -334,6 +381,52 @@ struct Apply {
             }
         }
     }
+    static __device__ __forceinline__ Work split_work(const Params& p, int tile) {
+        const int tiles = (p.n + 127) / 128;
+        return Work{tile / tiles, tile % tiles, 0, (p.k + 63) / 64, 0, -1};
+    }
+    static constexpr bool kMirror = false;
+    static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, uint4&) {
+        const Params& p = L.p;
+        if (row >= p.m || col >= p.n) return;
+        const float factor = OUT == kWeights ? p.alpha[0] * p.step : p.alpha[0];
+        const float x[4] = {v.x * factor, v.y * factor, v.z * factor, v.w * factor};
+        if constexpr (OUT == kSplit) {
+            const uint32_t w0 = split16(x[0]), w1 = split16(x[1]), w2 = split16(x[2]), w3 = split16(x[3]);
+            const long long at = row * p.ld + col;
+            *reinterpret_cast<uint2*>(p.out[0][0] + at) = make_uint2(low_halves(w0, w1), low_halves(w2, w3));
+            *reinterpret_cast<uint2*>(p.out[0][1] + at) = make_uint2(high_halves(w0, w1), high_halves(w2, w3));
+        } else if constexpr (OUT == kBf16) {
+            bf16* out = static_cast<bf16*>(p.result) + row * p.ldr + col;
+            if (col + 4 <= p.n && reinterpret_cast<uintptr_t>(out) % 8 == 0) {
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < p.n) out[e] = __float2bfloat16_rn(x[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < p.n) update_weight(p, row, col + e, x[e]);
+        }
+    }
+    static __device__ __forceinline__ void update_weight(const Params& p, int row, int col, float change) {
+        bool keep = true;
+        if (p.mask) {
+            const long long flat = static_cast<long long>(row) * p.n + col;
+            const long long group = p.shift >= 0 ? flat >> p.shift : static_cast<long long>(static_cast<unsigned long long>(flat) / static_cast<unsigned>(p.group));
+            keep = __ldg(p.mask + group) >> static_cast<int>(flat - group * p.group) & 1;
+        }
+        const long long at = row * p.ldr + col;
+        if (p.w_bf16) {
+            bf16* w = static_cast<bf16*>(p.result) + at;
+            *w = __float2bfloat16_rn(keep ? fmaf(p.decay, __bfloat162float(*w), -change) : 0.0f);
+        } else {
+            float* w = static_cast<float*>(p.result) + at;
+            *w = keep ? fmaf(p.decay, *w, -change) : 0.0f;
+        }
+    }
     // One column of up to 32 rows of weights a lane.
     static __device__ __noinline__ void update_rows(const Params& p, const uint8_t* buf, int row0, int col, int rows, bool inside, float step, int lane) {
         if (!inside) return;
@@ -359,7 +452,7 @@ struct Apply {
                 const int r = r0 + i;
                 if (r >= rows) break;
                 const float o = *reinterpret_cast<const float*>(buf + piece_at(r, 4 * lane));
-                const float x = bits[i] & 1 ? fmaf(-step, o, p.decay * w[i]) : 0.0f;
+                const float x = bits[i] & 1 ? fmaf(p.decay, w[i], -(step * o)) : 0.0f;
                 const long long at = (row0 + r) * p.ldr + col;
                 if (p.w_bf16) static_cast<bf16*>(p.result)[at] = __float2bfloat16_rn(x);
                 else static_cast<float*>(p.result)[at] = x;
@@ -417,7 +510,8 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
         p.beta = beta * power(out.exp - c->exp);
         p.diagonal = diagonal * power(out.exp);
     }
-    return launch_product(L, static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * p.products, st);
+    const long long t = (p.m + 127) / 128, pairs = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * p.products, units = t * (t + 1) / 2 * p.products;
+    return launch_either(L, units, pairs, (p.k + 63) / 64, st);
 }
 
 struct Result {
@@ -430,7 +524,7 @@ struct Result {
 // X (Q X, tall: X Q) into `out`, or into the result.
 template <bool BMN, int OUT>
 int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
-    Launch<Apply<BMN, OUT>> L{};
+    pair::Launch<Apply<BMN, OUT>> L{};
     Params& p = L.p;
     p.m = static_cast<int>(x.rows);
     p.n = static_cast<int>(x.cols);
@@ -450,7 +544,12 @@ int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res
     p.w_bf16 = res.w_bf16;
     p.decay = res.decay;
     p.step = res.step;
-    return launch_product(L, static_cast<long long>(p.tiles_m) * p.tiles_n, st);
+    if (OUT == kSplit) {
+        p.ld = out.ld;
+        for (int q = 0; q < 2; ++q) p.out[0][q] = out.part[q];
+    }
+    const long long pairs = static_cast<long long>(p.tiles_m) * p.tiles_n, units = static_cast<long long>((p.m + 127) / 128) * ((p.n + 127) / 128);
+    return launch_either(L, units, pairs, (p.k + 63) / 64, st);
 }
 template <int OUT>
 int apply(bool tall, const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
