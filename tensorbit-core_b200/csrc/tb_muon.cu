@@ -279,7 +279,7 @@ struct Symmetric {
         uint16_t* hi = p.out[w.which][0];
         uint16_t* lo = p.out[w.which][1];
         const int pairs = min(rows, p.m - row0 + 1) / 2;
-        for (int r = 2 * (thread / 64); r < 2 * pairs; r += 6) {
+        for (int r = 2 * (thread / 64); r < 2 * pairs; r += kSplitThreads / 32) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int c = thread % 64 + 64 * h;
@@ -461,6 +461,172 @@ struct Apply {
     }
 };
 
+// ---- short sides up to 128: a segment's k x k products in one launch ----------------------
+// One CTA with A (then P A), P and Q as operands in shared memory, 64 KB each; every product
+// is one 128 x 128 tile.  A thread turns 64 columns of a row of the accumulator into the
+// next operand's parts.  (Three steps, k = 128: CORE_US, of which the tensor core works CORE_MMA; as eight launches 76.)
+constexpr int kCoreThreads = 288, kCoreMatrix = 65536, kCorePart = 16384;  // warps 0-7 results, 8 loads and MMAs
+constexpr size_t kCoreSmem = 3 * kCoreMatrix + 1024 + 64;
+struct CoreMaps {
+    CUtensorMap a[2];
+};
+struct CoreParams {
+    int k, steps;
+    uint16_t* out[2];
+    long long ld;
+};
+__global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_constant__ CoreMaps maps, const __grid_constant__ CoreParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + 3 * kCoreMatrix);
+    uint64_t* done = loaded + 1;  // [2] one of each accumulator
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(loaded), 1);
+        mbar_init(smem_u32(&done[0]), 1);
+        mbar_init(smem_u32(&done[1]), 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    const bool issuer = warp == 8 && lane == 0;
+    if (issuer) {
+        mbar_expect_tx(smem_u32(loaded), kCoreMatrix);
+        for (int q = 0; q < 2; ++q)
+            for (int half = 0; half < 2; ++half)
+                tma_load_2d(smem_u32(smem + (2 * half + q) * kCorePart), &maps.a[q], 64 * half, 0, smem_u32(loaded));
+        if (!wait(smem_u32(loaded), 0, nullptr)) {
+            *abort_flag = 1;
+            atomicExch(&g_muon_error, 1);
+        }
+    }
+    __syncthreads();
+
+    // accumulator `d` = X Y^T of the matrices in buffers x and y (slices of 64 columns: hi, lo)
+    auto product = [&](int d, int x, int y) {
+        if (!issuer || *abort_flag) return;
+        constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | (8u << 24);
+        const uint64_t xd = operand_desc(smem_u32(smem + x * kCoreMatrix), false), yd = operand_desc(smem_u32(smem + y * kCoreMatrix), false);
+        constexpr uint64_t kLo = kCorePart >> 4;
+        for (int half = 0; half < (p.k > 64 ? 2 : 1); ++half)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t a = xd + half * 2 * kLo + 2 * kk, b = yd + half * 2 * kLo + 2 * kk;
+                mma_one16<true>(tmem + 128 * d, a + kLo, b, kIdesc, half | kk);
+                mma_one16<true>(tmem + 128 * d, a, b + kLo, kIdesc, 1);
+                mma_one16<true>(tmem + 128 * d, a, b, kIdesc, 1);
+            }
+        mma_commit(smem_u32(&done[d]));
+    };
+    const int row = (warp & 3) * 32 + lane, half = (warp >> 2) & 1;  // of a thread with results: columns 64 half ..
+    uint32_t phase[2] = {0, 0};
+    uint32_t v[64];
+    // this thread's values of a finished accumulator, times alpha (plus beta C + diagonal I), split
+    auto take = [&](int d, float alpha, int c, float beta, float diagonal) {
+        if (warp >= 8) return;
+        if (!wait(smem_u32(&done[d]), phase[d], abort_flag)) {
+            *abort_flag = 1;
+            atomicExch(&g_muon_error, 1);
+        }
+        phase[d] ^= 1;
+        fence_after();
+        uint32_t x[2][32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float f[32];
+            tmem_ld32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(128 * d + 64 * half + 32 * i), f);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[i][e] = __float_as_uint(f[e] * alpha);
+        }
+        fence_before();
+        const uint8_t* at = smem + c * kCoreMatrix + 2 * half * kCorePart + row * 128;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __uint_as_float(x[j >> 2][(8 * j + e) & 31]);
+            if (c >= 0) {
+                const uint4 h = *reinterpret_cast<const uint4*>(at + ((j ^ (row & 7)) << 4)), l = *reinterpret_cast<const uint4*>(at + kCorePart + ((j ^ (row & 7)) << 4));
+                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
+                    w[2 * e] = fmaf(beta, hf.x, fmaf(beta, lf.x, w[2 * e]));
+                    w[2 * e + 1] = fmaf(beta, hf.y, fmaf(beta, lf.y, w[2 * e + 1]));
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (64 * half + 8 * j + e == row && row < p.k) w[e] += diagonal;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[8 * j + e] = split16(w[e]);
+        }
+    };
+    auto put = [&](int to) {  // as an operand
+        if (warp >= 8) return;
+        uint8_t* at = smem + to * kCoreMatrix + 2 * half * kCorePart;
+        fill_part<false>(at + (row - lane) * 128, v, lane);
+        fill_part<true>(at + kCorePart + (row - lane) * 128, v, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    };
+    auto meet = [&] {
+        fence_before();
+        __syncthreads();
+        fence_after();
+    };
+    constexpr float kDown = 1.0f / (1 << kExpK);  // A, P and P A all have this power of two
+    int P = 1, Q = 1;
+    for (int i = 0; i < p.steps; ++i) {
+        const bool last = i == p.steps - 1;
+        if (i) P = 3 - Q;
+        product(0, 0, 0);
+        take(0, kC * kDown, 0, kB, kA * (1 << kExpK));
+        if (last && i == 0) break;
+        put(P);
+        meet();
+        if (last) {
+            product(0, P, Q);
+            take(0, i == 1 ? 1.0f / (1 << (2 * kExpK - kExpQ)) : kDown, -1, 0, 0);
+            break;
+        }
+        product(0, P, 0);
+        if (i) product(1, P, Q);
+        take(0, kDown, -1, 0, 0);
+        put(0);  // (the products that read A, and Q, ...
+        if (i) {
+            take(1, i == 1 ? 1.0f / (1 << (2 * kExpK - kExpQ)) : kDown, -1, 0, 0);
+            put(Q);  // ... are done)
+        }
+        meet();
+        product(0, P, 0);
+        take(0, kDown, -1, 0, 0);
+        put(0);
+        meet();
+    }
+    if (warp < 8 && row < p.k && !*abort_flag) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int col = 64 * half + 8 * j;
+            if (col >= p.ld) break;
+            const uint32_t* x = v + 8 * j;
+            *reinterpret_cast<uint4*>(p.out[0] + row * p.ld + col) = make_uint4(low_halves(x[0], x[1]), low_halves(x[2], x[3]), low_halves(x[4], x[5]), low_halves(x[6], x[7]));
+            *reinterpret_cast<uint4*>(p.out[1] + row * p.ld + col) = make_uint4(high_halves(x[0], x[1]), high_halves(x[2], x[3]), high_halves(x[4], x[5]), high_halves(x[6], x[7]));
+        }
+    }
+    meet();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+}
+
 long long up(long long v, long long m) { return (v + m - 1) / m * m; }
 
 struct Matrix {
@@ -512,6 +678,28 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
     }
     const long long t = (p.m + 127) / 128, pairs = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * p.products, units = t * (t + 1) / 2 * p.products;
     return launch_either(L, units, pairs, (p.k + 63) / 64, st);
+}
+
+// Q of `steps` steps from A, for k up to 128.
+int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
+    static std::mutex mu;
+    static uint64_t prepared = 0;  // per device: the shared-memory limit
+    int dev = 0;
+    int rc = require_device(&dev);
+    if (rc) return rc;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 64 || !(prepared >> dev & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(core_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCoreSmem));
+            if (e != cudaSuccess) return cuda_fail(e, "core_kernel setup");
+            if (dev < 64) prepared |= 1ull << dev;
+        }
+    }
+    CoreMaps maps{};
+    if ((rc = operand_maps(maps.a, A, false))) return rc;
+    const CoreParams p{static_cast<int>(A.rows), steps, {q.part[0], q.part[1]}, q.ld};
+    const cudaError_t e = launch_pdl(core_kernel, dim3(1), dim3(kCoreThreads), kCoreSmem, st, maps, p);
+    return e == cudaSuccess ? check_launch("core_kernel") : cuda_fail(e, "core_kernel launch");
 }
 
 struct Result {
@@ -592,7 +780,12 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
         const int n = steps * (seg + 1) / segments - steps * seg / segments;
         rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
         Matrix q = P[0];
-        for (int i = 0; i < n && !rc; ++i) {
+        const bool small = k <= 128;
+        if (!rc && small) {
+            if (n > 1) q = Q[0];
+            rc = core(A, q, n, st);
+        }
+        for (int i = 0; i < n && !rc && !small; ++i) {
             const Matrix& p = P[i & 1];
             rc = symmetric<false>(A, A, p, kC, &A, kB, kA, nullptr, nullptr, st);
             const Matrix& next = Q[i & 1];

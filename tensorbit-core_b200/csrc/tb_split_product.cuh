@@ -19,7 +19,7 @@
 namespace tb {
 namespace pair {
 
-constexpr int kSplitThreads = 192;  // warps 0-3 sums and results, 4 loads, 5 MMAs
+constexpr int kSplitThreads = 384;  // warps 0-3 sums, 4 loads, 5 MMAs, all of them results
 constexpr int kSplitPitch = 132;    // floats of a row of sums: 16-byte accesses without bank conflicts
 constexpr int kSplitMost = 8;       // CTAs of a cluster
 
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp == 5) {
         if (lane == 0) {
             constexpr uint32_t kFormat = OP::kF16 ? 0u : 1u;
             constexpr uint32_t kIdesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | (OP::kAMn ? 1u << 15 : 0u) |
