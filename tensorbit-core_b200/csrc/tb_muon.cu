@@ -279,16 +279,17 @@ struct Symmetric {
         uint16_t* hi = p.out[w.which][0];
         uint16_t* lo = p.out[w.which][1];
         const int pairs = min(rows, p.m - row0 + 1) / 2;
-        for (int r = 2 * (thread / 64); r < 2 * pairs; r += kSplitThreads / 32) {
+        for (int c = 4 * (thread >> 5); c < 128; c += kSplitThreads / 8)
+            for (int r = 2 * (thread & 31); r < 2 * pairs; r += 64) {  // (a warp writes consecutive rows of four columns)
+                const uint4 a = *reinterpret_cast<const uint4*>(words + r * pitch + c), b = *reinterpret_cast<const uint4*>(words + (r + 1) * pitch + c);
+                const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+                long long at = (w.tn * 128 + c) * p.ld + row0 + r;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = thread % 64 + 64 * h;
-                const uint32_t a = words[r * pitch + c], b = words[(r + 1) * pitch + c];
-                const long long at = (w.tn * 128 + c) * p.ld + row0 + r;
-                *reinterpret_cast<uint32_t*>(hi + at) = low_halves(a, b);
-                *reinterpret_cast<uint32_t*>(lo + at) = high_halves(a, b);
+                for (int e = 0; e < 4; ++e, at += p.ld) {
+                    *reinterpret_cast<uint32_t*>(hi + at) = low_halves(x[e], y[e]);
+                    *reinterpret_cast<uint32_t*>(lo + at) = high_halves(x[e], y[e]);
+                }
             }
-        }
     }
     static __device__ __forceinline__ void finish(const Launch<Symmetric>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
         const Params& p = L.p;
