@@ -40,10 +40,13 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int kExpX = 14, kExpK = 13, kExpQ = 10;  // the powers of two of X; of A, P and P A; of Q
 constexpr int kSegment = 3;                        // steps between two formings of X
 
-// hi + lo of an FP32 value, as two FP16 in one word.
-__device__ __forceinline__ uint32_t split16(float x) {
-    const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
-    return static_cast<uint32_t>(__half_as_ushort(h)) | static_cast<uint32_t>(__half_as_ushort(l)) << 16;
+// The FP16 parts hi + lo of two FP32 values: hi parts in one word, lo parts in another.
+__device__ __forceinline__ void split16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
@@ -161,12 +164,14 @@ __global__ void __launch_bounds__(256) scale_kernel(const Source s, const double
         const int col = 4 * static_cast<int>(i - row * units);
         float u[4];
         update4<false>(s, row, col, u);
-        uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = split16(sum == 0.0 ? 0.0f : static_cast<float>(u[e] * scale));
+        for (int e = 0; e < 4; ++e) u[e] = sum == 0.0 ? 0.0f : static_cast<float>(u[e] * scale);
+        uint2 h, l;
+        split16x2(u[0], u[1], h.x, l.x);
+        split16x2(u[2], u[3], h.y, l.y);
         const long long at = row * ld + col;
-        *reinterpret_cast<uint2*>(hi + at) = make_uint2(low_halves(w[0], w[1]), low_halves(w[2], w[3]));
-        *reinterpret_cast<uint2*>(lo + at) = make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]));
+        *reinterpret_cast<uint2*>(hi + at) = h;
+        *reinterpret_cast<uint2*>(lo + at) = l;
     }
 }
 
@@ -188,18 +193,11 @@ struct Params {
     float decay, step;    // W <- mask (decay W - step O)
 };
 
-// Fills a piece of 64 columns x 32 rows with one part of `v`.
-template <bool LO>
-__device__ __forceinline__ void fill_part(uint8_t* buf, const uint32_t* v, int lane) {
+// Fills a piece of 64 columns x 32 rows with the lane's row of one part.
+__device__ __forceinline__ void fill_part(uint8_t* buf, const uint32_t (&v)[32], int lane) {
     uint8_t* row = buf + lane * 128;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t* x = v + 8 * j;
-        uint4 w;
-        if constexpr (LO) w = make_uint4(high_halves(x[0], x[1]), high_halves(x[2], x[3]), high_halves(x[4], x[5]), high_halves(x[6], x[7]));
-        else w = make_uint4(low_halves(x[0], x[1]), low_halves(x[2], x[3]), low_halves(x[4], x[5]), low_halves(x[6], x[7]));
-        *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = w;
-    }
+    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
 __device__ __forceinline__ void store_part(const CUtensorMap* map, uint8_t* buf, int col, int row, int lane) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -211,20 +209,16 @@ __device__ __forceinline__ void store_part(const CUtensorMap* map, uint8_t* buf,
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
 }
-// The lane's row of 128 columns, split, as rows of both parts.
-__device__ __forceinline__ void store_split(const CUtensorMap (&maps)[2], uint8_t* buf, const uint32_t (&v)[128], int col, int row0, int n, int lane) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        if (col + 64 * c >= n) break;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-            if (part) fill_part<true>(buf, v + 64 * c, lane);
-            else fill_part<false>(buf, v + 64 * c, lane);
-            store_part(&maps[part], buf, col + 64 * c, row0, lane);
-        }
-    }
+// The lane's row of 64 columns as rows of both parts.
+__device__ __forceinline__ void store_split(const CUtensorMap (&maps)[2], uint8_t* buf, const uint32_t (&hi)[32], const uint32_t (&lo)[32], int col, int row0, int lane) {
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    fill_part(buf, hi, lane);
+    store_part(&maps[0], buf, col, row0, lane);
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    fill_part(buf, lo, lane);
+    store_part(&maps[1], buf, col, row0, lane);
 }
 
 // Tile `unit` of those on and below the diagonal, row by row.
@@ -266,10 +260,13 @@ struct Symmetric {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = fmaf(p.beta, hs[e], fmaf(p.beta, ls[e], x[e])) + (row == col + e ? p.diagonal : 0.0f);
         }
-        words = make_uint4(split16(x[0]), split16(x[1]), split16(x[2]), split16(x[3]));
+        uint2 hi, lo;
+        split16x2(x[0], x[1], hi.x, lo.x);
+        split16x2(x[2], x[3], hi.y, lo.y);
+        words = make_uint4(hi.x, hi.y, lo.x, lo.y);
         if (inside) {
-            *reinterpret_cast<uint2*>(p.out[w.which][0] + at) = make_uint2(low_halves(words.x, words.y), low_halves(words.z, words.w));
-            *reinterpret_cast<uint2*>(p.out[w.which][1] + at) = make_uint2(high_halves(words.x, words.y), high_halves(words.z, words.w));
+            *reinterpret_cast<uint2*>(p.out[w.which][0] + at) = hi;
+            *reinterpret_cast<uint2*>(p.out[w.which][1] + at) = lo;
         }
     }
     // Two rows of a column at a time (columns left of the diagonal's tile all exist).
@@ -285,9 +282,11 @@ struct Symmetric {
                 const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
                 long long at = (w.tn * 128 + c) * p.ld + row0 + r;
 #pragma unroll
-                for (int e = 0; e < 4; ++e, at += p.ld) {
+                for (int e = 0; e < 2; ++e, at += 2 * p.ld) {
                     *reinterpret_cast<uint32_t*>(hi + at) = low_halves(x[e], y[e]);
-                    *reinterpret_cast<uint32_t*>(lo + at) = high_halves(x[e], y[e]);
+                    *reinterpret_cast<uint32_t*>(hi + at + p.ld) = high_halves(x[e], y[e]);
+                    *reinterpret_cast<uint32_t*>(lo + at) = low_halves(x[2 + e], y[2 + e]);
+                    *reinterpret_cast<uint32_t*>(lo + at + p.ld) = high_halves(x[2 + e], y[2 + e]);
                 }
             }
     }
@@ -296,46 +295,68 @@ struct Symmetric {
         const int row0 = w.tm * 256 + row_in, row = row0 + lane, col = w.tn * 256 + half * 128;
         if (col / 128 > row0 / 128 || row0 >= p.m || col >= p.n) return;
         const float alpha = p.alpha[w.which];
-        uint32_t v[128];
-        if (p.c[0] && row < p.m) {
+        const bool mirrored = col / 128 != row0 / 128, odd = lane & 1;
+        // selectors of the halves that a lane sends to its neighbour, and of what it makes of those that it gets
+        const uint32_t send = odd ? 0x5410u : 0x7632u, take_hi = odd ? 0x3254u : 0x5410u, take_lo = odd ? 0x3276u : 0x7610u;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (col + 8 * j >= p.n) break;  // (rows of ld, a multiple of 8)
-                const long long at = row * p.ld + col + 8 * j;
-                const uint4 h = *reinterpret_cast<const uint4*>(p.c[0] + at), l = *reinterpret_cast<const uint4*>(p.c[1] + at);
-                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+        for (int c = 0; c < 2; ++c) {
+            const int col0 = col + 64 * c;
+            if (col0 >= p.n) break;
+            float* x = acc + 64 * c;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
-                    float& x = acc[8 * j + 2 * e];
-                    float& y = acc[8 * j + 2 * e + 1];
-                    x = fmaf(p.beta, hf.x, fmaf(p.beta, lf.x, x * alpha));
-                    y = fmaf(p.beta, hf.y, fmaf(p.beta, lf.y, y * alpha));
+            for (int i = 0; i < 64; ++i) x[i] *= alpha;
+            if (p.c[0]) {  // (rows of ld, a multiple of 8)
+                const long long at = min(row, p.m - 1) * p.ld + col0;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint4 h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool inside = col0 + 32 * q + 8 * j < p.n;
+                        h[j] = l[j] = make_uint4(0, 0, 0, 0);
+                        if (inside) h[j] = *reinterpret_cast<const uint4*>(p.c[0] + at + 32 * q + 8 * j);
+                        if (inside) l[j] = *reinterpret_cast<const uint4*>(p.c[1] + at + 32 * q + 8 * j);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t hw[4] = {h[j].x, h[j].y, h[j].z, h[j].w}, lw[4] = {l[j].x, l[j].y, l[j].z, l[j].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
+                            float* to = x + 32 * q + 8 * j + 2 * e;
+                            to[0] = fmaf(p.beta, hf.x, fmaf(p.beta, lf.x, to[0]));
+                            to[1] = fmaf(p.beta, hf.y, fmaf(p.beta, lf.y, to[1]));
+                        }
+                    }
+                }
+                if (!mirrored) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) x[i] += col0 + i == row ? p.diagonal : 0.0f;
                 }
             }
+            uint32_t hi[32], lo[32];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] + (col + i == row ? p.diagonal : 0.0f));
-        } else {
+            for (int i = 0; i < 32; ++i) split16x2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+            store_split(L.o[w.which], buf, hi, lo, col0, row0, lane);
+            if (!mirrored) continue;
+            // two lanes exchange, so that each has two rows of one column
+            const long long at = (col0 + odd) * p.ld + (row & ~1);
+            uint16_t* out_hi = p.out[w.which][0] + at;
+            uint16_t* out_lo = p.out[w.which][1] + at;
+            const bool both = (row | 1) < p.m, one = (row & ~1) < p.m;
 #pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] * alpha);
-        }
-        store_split(L.o[w.which], buf, v, col, row0, p.n, lane);
-        if (col / 128 == row0 / 128) return;
-        // mirrored: two lanes exchange, so that each has two rows of one column
-        uint16_t* hi = p.out[w.which][0];
-        uint16_t* lo = p.out[w.which][1];
-        const bool odd = lane & 1, whole = row0 + 32 <= p.m;
-#pragma unroll
-        for (int i = 0; i < 128; i += 2) {
-            const uint32_t other = __shfl_xor_sync(~0u, odd ? v[i] : v[i + 1], 1);
-            const uint32_t first = odd ? other : v[i], second = odd ? v[i + 1] : other;
-            const long long at = (col + i + odd) * p.ld + (row & ~1);
-            if (whole || (row | 1) < p.m) {
-                *reinterpret_cast<uint32_t*>(hi + at) = low_halves(first, second);
-                *reinterpret_cast<uint32_t*>(lo + at) = high_halves(first, second);
-            } else if ((row & ~1) < p.m) {
-                hi[at] = static_cast<uint16_t>(first & 0xFFFFu);
-                lo[at] = static_cast<uint16_t>(first >> 16);
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t other = __shfl_xor_sync(~0u, __byte_perm(hi[i], lo[i], send), 1);
+                const uint32_t h = __byte_perm(hi[i], other, take_hi), l = __byte_perm(lo[i], other, take_lo);
+                if (both) {
+                    *reinterpret_cast<uint32_t*>(out_hi) = h;
+                    *reinterpret_cast<uint32_t*>(out_lo) = l;
+                } else if (one) {
+                    *out_hi = static_cast<uint16_t>(h);
+                    *out_lo = static_cast<uint16_t>(l);
+                }
+                out_hi += 2 * p.ld;
+                out_lo += 2 * p.ld;
             }
         }
     }
@@ -362,10 +383,14 @@ struct Apply {
         if (rows <= 0 || cols <= 0) return;
         const float alpha = p.alpha[0];
         if constexpr (OUT == kSplit) {
-            uint32_t v[128];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] = split16(acc[i] * alpha);
-            store_split(L.o[0], buf, v, col, row0, p.n, lane);
+            for (int c = 0; c < 2; ++c) {
+                if (64 * c >= cols) break;
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) split16x2(acc[64 * c + 2 * i] * alpha, acc[64 * c + 2 * i + 1] * alpha, hi[i], lo[i]);
+                store_split(L.o[0], buf, hi, lo, col + 64 * c, row0, lane);
+            }
         } else if constexpr (OUT == kBf16) {
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] *= alpha;
@@ -393,10 +418,12 @@ struct Apply {
         const float factor = OUT == kWeights ? p.alpha[0] * p.step : p.alpha[0];
         const float x[4] = {v.x * factor, v.y * factor, v.z * factor, v.w * factor};
         if constexpr (OUT == kSplit) {
-            const uint32_t w0 = split16(x[0]), w1 = split16(x[1]), w2 = split16(x[2]), w3 = split16(x[3]);
+            uint2 hi, lo;
+            split16x2(x[0], x[1], hi.x, lo.x);
+            split16x2(x[2], x[3], hi.y, lo.y);
             const long long at = row * p.ld + col;
-            *reinterpret_cast<uint2*>(p.out[0][0] + at) = make_uint2(low_halves(w0, w1), low_halves(w2, w3));
-            *reinterpret_cast<uint2*>(p.out[0][1] + at) = make_uint2(high_halves(w0, w1), high_halves(w2, w3));
+            *reinterpret_cast<uint2*>(p.out[0][0] + at) = hi;
+            *reinterpret_cast<uint2*>(p.out[0][1] + at) = lo;
         } else if constexpr (OUT == kBf16) {
             bf16* out = static_cast<bf16*>(p.result) + row * p.ldr + col;
             if (col + 4 <= p.n && reinterpret_cast<uintptr_t>(out) % 8 == 0) {
@@ -531,7 +558,7 @@ __global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_cons
     };
     const int row = (warp & 3) * 32 + lane, half = (warp >> 2) & 1;  // of a thread with results: columns 64 half ..
     uint32_t phase[2] = {0, 0};
-    uint32_t v[64];
+    uint32_t vh[32], vl[32];
     // this thread's values of a finished accumulator, times alpha (plus beta C + diagonal I), split
     auto take = [&](int d, float alpha, int c, float beta, float diagonal) {
         if (warp >= 8) return;
@@ -570,14 +597,14 @@ __global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_cons
                     if (64 * half + 8 * j + e == row && row < p.k) w[e] += diagonal;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[8 * j + e] = split16(w[e]);
+            for (int e = 0; e < 4; ++e) split16x2(w[2 * e], w[2 * e + 1], vh[4 * j + e], vl[4 * j + e]);
         }
     };
     auto put = [&](int to) {  // as an operand
         if (warp >= 8) return;
         uint8_t* at = smem + to * kCoreMatrix + 2 * half * kCorePart;
-        fill_part<false>(at + (row - lane) * 128, v, lane);
-        fill_part<true>(at + kCorePart + (row - lane) * 128, v, lane);
+        fill_part(at + (row - lane) * 128, vh, lane);
+        fill_part(at + kCorePart + (row - lane) * 128, vl, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
     auto meet = [&] {
@@ -619,9 +646,8 @@ __global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_cons
         for (int j = 0; j < 8; ++j) {
             const int col = 64 * half + 8 * j;
             if (col >= p.ld) break;
-            const uint32_t* x = v + 8 * j;
-            *reinterpret_cast<uint4*>(p.out[0] + row * p.ld + col) = make_uint4(low_halves(x[0], x[1]), low_halves(x[2], x[3]), low_halves(x[4], x[5]), low_halves(x[6], x[7]));
-            *reinterpret_cast<uint4*>(p.out[1] + row * p.ld + col) = make_uint4(high_halves(x[0], x[1]), high_halves(x[2], x[3]), high_halves(x[4], x[5]), high_halves(x[6], x[7]));
+            *reinterpret_cast<uint4*>(p.out[0] + row * p.ld + col) = make_uint4(vh[4 * j], vh[4 * j + 1], vh[4 * j + 2], vh[4 * j + 3]);
+            *reinterpret_cast<uint4*>(p.out[1] + row * p.ld + col) = make_uint4(vl[4 * j], vl[4 * j + 1], vl[4 * j + 2], vl[4 * j + 3]);
         }
     }
     meet();
