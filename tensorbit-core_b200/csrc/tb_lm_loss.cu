@@ -17,6 +17,7 @@
 
 #include "tb_lm_loss.cuh"
 #include "tb_pair_product.cuh"
+#include "tb_split_product.cuh"
 
 #ifndef TBG
 #define TBG 16
@@ -312,6 +313,7 @@ struct InputGrad {
     }
     static __device__ __forceinline__ void finish(const Launch<InputGrad>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
         const int row0 = w.tm * 256 + row_in, col = w.tn * 256 + half * 128;
+        if (row0 >= *L.p.count) return;
         store_tma<false, 1>(&L.o[0][0], buf, acc, col, row0, w.slot, L.p.cols, !L.p.first, lane);
     }
 };
@@ -371,29 +373,28 @@ __global__ void __launch_bounds__(256) join_loss_kernel(const Args a, const Scra
         a.loss[t] = (m - s.top[r]) + rest;  // (the difference of like logits first: it is exact)
     }
 }
-// dh from its shares, in order: a row a warp.
+// dh from its shares, in order: 1024 columns of a row a block.
 __global__ void __launch_bounds__(256) join_dh_kernel(const Args a, const Scratch s, const int splits) {
     pdl_wait();
-    const long long r = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (r >= *s.count) return;
-    const int lane = threadIdx.x & 31;
+    const int chunks = (a.d + 1023) / 1024;
+    const long long r = blockIdx.x / chunks;
+    const int i = static_cast<int>(blockIdx.x % chunks) * 1024 + 4 * threadIdx.x;
+    if (r >= *s.count || i >= a.d) return;
     const float unit = *s.unit;
-    const float* part = s.part + r * s.ldp;
-    bf16* out = a.dh + s.token[r] * a.lddh;
-    const bool wide = (reinterpret_cast<uintptr_t>(out) & 7) == 0;
-    for (int i = 4 * lane; i < a.d; i += 128) {
-        float4 v = *reinterpret_cast<const float4*>(part + i);
-        for (int q = 1; q < splits; ++q) {
-            const float4 x = *reinterpret_cast<const float4*>(part + q * s.rows * s.ldp + i);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        }
-        v.x *= unit; v.y *= unit; v.z *= unit; v.w *= unit;
-        if (wide && i + 4 <= a.d) {
-            *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-        } else {
-            const float x[4] = {v.x, v.y, v.z, v.w};
-            for (int e = 0; e < 4 && i + e < a.d; ++e) out[i + e] = __float2bfloat16_rn(x[e]);
-        }
+    const float* part = s.part + r * s.ldp + i;
+    float4 v = *reinterpret_cast<const float4*>(part);
+#pragma unroll 4
+    for (int q = 1; q < splits; ++q) {
+        const float4 x = *reinterpret_cast<const float4*>(part + q * s.rows * s.ldp);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    v.x *= unit; v.y *= unit; v.z *= unit; v.w *= unit;
+    bf16* out = a.dh + s.token[r] * a.lddh + i;
+    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0 && i + 4 <= a.d) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    } else {
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        for (int e = 0; e < 4 && i + e < a.d; ++e) out[e] = __float2bfloat16_rn(x[e]);
     }
 }
 
@@ -433,7 +434,343 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
     return e == cudaSuccess ? check_launch(what) : cuda_fail(e, what);
 }
 
+// ---- few tokens: one pass over w --------------------------------------------------------
+// Up to 128 tokens leave the logits bound by the reading of w.  Tokens are the N of the
+// product here and the vocabulary is M: a CTA takes `tile` rows of w (up to 256, two MMAs of 128), a
+// share that is even over all SMs, and streams them past the tokens' slices; a thread has one entry of the
+// vocabulary and all tokens.  Sums of 256 terms in the tensor core.
+// (32000 x 4096, kernel: ONE_US for 1 token, FEW_US for 37; w at the measured copy rate 41.)
+constexpr int kFewMost = 128;
+constexpr int kFewThreads = 320;  // warps 0-7 results, 8 loads, 9 MMAs
+constexpr int kFewGroup = 4;
+template <int NT>
+struct FewCfg {
+    static constexpr int kStage = 32768 + NT * 128;
+    static constexpr int kStages = NT <= 32 ? 6 : NT <= 64 ? 5 : 4;
+    static constexpr int kExtra = 8 * NT * 8 + NT * 16;  // the warps' maxima and sums; the tokens' rows
+    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kExtra + 1024 + 256;
+    static_assert(kSmem <= 232448, "shared memory of a block");
+};
+struct FewParams {
+    int tile, tiles, vocab, d;
+    int n;             // forward: tokens as they are
+    const int* count;  // backward: those kept
+    const int64_t* target;
+    const Row* row;
+    float cap;
+    float* top;        // [NT]
+    float2* stats;     // [tiles][NT]
+    bf16* g;           // [NT][ldg]
+    long long ldg;
+};
+struct FewMaps {
+    CUtensorMap w, h;
+};
+template <int NT, bool GRAD>
+__global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewParams p) {
+    using C = FewCfg<NT>;
+    constexpr int kStages = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float2* joined = reinterpret_cast<float2*>(smem + kStages * C::kStage);  // [8][NT]
+    Row* rows = reinterpret_cast<Row*>(joined + 8 * NT);
+    uint64_t* ready = reinterpret_cast<uint64_t*>(rows + NT);
+    uint64_t* empty = ready + kStages;
+    uint64_t* accfull = empty + kStages;  // [2]
+    uint64_t* accempty = accfull + 2;     // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr uint32_t kColumns = 4 * NT < 32 ? 32 : 4 * NT;  // two sums of two halves
+
+    if (threadIdx.x == 8 * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.h)) : "memory");
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&ready[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&accfull[b]), 1);
+            mbar_init(smem_u32(&accempty[b]), 8);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kColumns));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();  // nothing above touched memory that an earlier kernel writes
+    if (threadIdx.x < NT) {
+        const int t = threadIdx.x;
+        Row r{0.0f, 0.0f, 0.0f, -1};
+        if (GRAD) {
+            if (t < *p.count) r = p.row[t];
+        } else if (t < p.n) {
+            const int64_t y = p.target[t];
+            if (y >= 0 && y < p.vocab) r.target = static_cast<int>(y);
+        }
+        rows[t] = r;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int slices = (p.d + 63) / 64;
+
+    if (warp < 8) {
+        const int quad = warp & 3, half = warp >> 2;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * NT);
+        Ring<2> ac;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+            float z[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) z[i] = 0.0f;
+            for (int left = slices; left > 0; left -= kFewGroup) {
+                if (!wait(smem_u32(&accfull[ac.s]), ac.phase, abort_flag)) { ok = false; break; }
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < NT / 16; ++c) {
+                    uint32_t x[16];
+                    tmem_ld16(lane_base + static_cast<uint32_t>(ac.s * 2 * NT + 16 * c), x);
+                    tmem_wait16(x);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) add2(z[16 * c + i], z[16 * c + i + 1], x[i], x[i + 1]);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&accempty[ac.s])) : "memory");
+                ac.next();
+            }
+            if (!ok) break;
+            const int in = half * 128 + quad * 32 + lane;
+            const long long entry = static_cast<long long>(tile) * p.tile + in;
+            const bool inside = in < p.tile && entry < p.vocab;
+            const float inverse = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+            if constexpr (GRAD) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const Row r = rows[i];
+                    float x = z[i], slope = 1.0f;
+                    if (p.cap > 0.0f) {
+                        const float t = tanhf(x * inverse);
+                        x = p.cap * t;
+                        slope = fmaf(-t, t, 1.0f);
+                    }
+                    float g = r.both * exp2f(fmaf(x, kLog2e, -r.lse2));
+                    if (r.target == entry) g -= r.dloss;
+                    // (a token behind the last kept one, of which z is what w times zeros gives, counts as zero)
+                    if (inside) p.g[i * p.ldg + entry] = __float2bfloat16_rn(i < *p.count ? g * slope : 0.0f);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    float x = z[i];
+                    if (p.cap > 0.0f) x = p.cap * tanhf(x * inverse);
+                    if (inside && rows[i].target == entry) p.top[i] = x;
+                    if (!inside) x = -INFINITY;
+                    float m = x;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                    const float base = m == -INFINITY ? 0.0f : m * kLog2e;
+                    float e = exp2f(fmaf(x, kLog2e, -base));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(~0u, e, o);
+                    if (lane == 0) joined[warp * NT + i] = make_float2(m, e);
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (threadIdx.x < NT) {
+                    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) m = fmaxf(m, joined[q * NT + threadIdx.x].x);
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const float2 x = joined[q * NT + threadIdx.x];
+                        sum += x.y * exp2f((x.x - base) * kLog2e);
+                    }
+                    p.stats[static_cast<long long>(tile) * NT + threadIdx.x] = make_float2(m, sum);
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            atomicExch(&g_loss_error, 1);
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            Ring<kStages> at;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+#pragma unroll 1
+                for (int i = 0; i < slices; ++i, at.next()) {
+                    if (!wait(smem_u32(&empty[at.s]), at.phase ^ 1, abort_flag)) { ok = false; break; }  // (the first round passes at once)
+                    const uint32_t stage = smem_u32(smem + at.s * C::kStage), bar = smem_u32(&ready[at.s]);
+                    mbar_expect_tx(bar, static_cast<uint32_t>(p.tile) * 128 + NT * 128);
+                    tma_load_2d(stage, &maps.w, 64 * i, tile * p.tile, bar);
+                    tma_load_2d(stage + 32768, &maps.h, 64 * i, 0, bar);
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(&g_loss_error, 1);
+                for (int i = 0; i < kStages; ++i)  // loads in flight, within a limit
+                    if (i < at.s || at.phase) wait(smem_u32(&ready[i]), i < at.s ? at.phase : at.phase ^ 1, nullptr);
+            }
+        }
+        __syncwarp();
+    } else {
+        if (lane == 0) {
+            constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NT >> 3) << 17) | (8u << 24);
+            Ring<kStages> at;
+            Ring<2> ac;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+                for (int left = slices; left > 0 && ok;) {
+                    int n = min(left, kFewGroup);
+                    left -= n;
+                    if (!wait(smem_u32(&accempty[ac.s]), ac.phase ^ 1, abort_flag)) { ok = false; break; }
+                    fence_after();
+                    uint32_t more = 0;
+#pragma unroll 1
+                    for (; n > 0; --n, at.next()) {
+                        if (!wait(smem_u32(&ready[at.s]), at.phase, abort_flag)) { ok = false; break; }
+                        fence_after();
+                        const uint64_t a = operand_desc(smem_u32(smem + at.s * C::kStage), false), b = a + (32768 >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            mma_one16<false>(tmem + ac.s * 2 * NT, a + 2 * kk, b + 2 * kk, kIdesc, more);
+                            if (p.tile > 128) mma_one16<false>(tmem + ac.s * 2 * NT + NT, a + (16384 >> 4) + 2 * kk, b + 2 * kk, kIdesc, more);
+                            more = 1;
+                        }
+                        mma_commit(smem_u32(&empty[at.s]));
+                    }
+                    mma_commit(smem_u32(&accfull[ac.s]));
+                    ac.next();
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(&g_loss_error, 1);
+                for (int b = 0; b < 2; ++b) mma_commit(smem_u32(&accfull[b]));  // releases the waiting warps
+            }
+        }
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns));
+    }
+}
+// A token a block: its tiles' maxima and sums.
+__global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float* top, const float2* stats, const int tiles, const int pitch) {
+    __shared__ float2 shared[8];
+    pdl_wait();
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (!kept(a, t)) {
+        if (threadIdx.x == 0) a.loss[t] = a.lse[t] = 0.0f;
+        return;
+    }
+    float m = -INFINITY, sum = 0.0f;
+    auto add = [&](float2 x) {
+        const float most = fmaxf(m, x.x), base = most == -INFINITY ? 0.0f : most;
+        sum = sum * exp2f((m - base) * kLog2e) + x.y * exp2f((x.x - base) * kLog2e);
+        m = most;
+    };
+#pragma unroll 4
+    for (int i = threadIdx.x; i < tiles; i += 256) add(stats[static_cast<long long>(i) * pitch + t]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float x = __shfl_xor_sync(~0u, m, o), y = __shfl_xor_sync(~0u, sum, o);
+        // (the same result in both lanes: the lower one's first)
+        const float m0 = lane & o ? x : m, s0 = lane & o ? y : sum, m1 = lane & o ? m : x, s1 = lane & o ? sum : y;
+        m = m0;
+        sum = s0;
+        add(make_float2(m1, s1));
+    }
+    if (lane == 0) shared[warp] = make_float2(m, sum);
+    __syncthreads();
+    if (threadIdx.x) return;
+    m = shared[0].x;
+    sum = shared[0].y;
+    for (int q = 1; q < 8; ++q) add(shared[q]);
+    const float rest = logf(sum);
+    a.lse[t] = m + rest;
+    a.loss[t] = (m - top[t]) + rest;  // (the difference of like logits first: it is exact)
+}
+
+int few_tokens(long long n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+template <int NT, bool GRAD>
+int launch_few(const FewMaps& maps, const FewParams& p, cudaStream_t st) {
+    static std::mutex mu;
+    static uint64_t prepared = 0;  // per device: the shared-memory limit
+    int dev = 0;
+    const int rc = require_device(&dev);
+    if (rc) return rc;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 64 || !(prepared >> dev & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(few_logits_kernel<NT, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(FewCfg<NT>::kSmem));
+            if (e != cudaSuccess) return cuda_fail(e, "few_logits_kernel setup");
+            if (dev < 64) prepared |= 1ull << dev;
+        }
+    }
+    const cudaError_t e = launch_pdl(few_logits_kernel<NT, GRAD>, dim3(std::min(p.tiles, 148)), dim3(kFewThreads), FewCfg<NT>::kSmem, st, maps, p);
+    return e == cudaSuccess ? check_launch("few_logits_kernel") : cuda_fail(e, "few_logits_kernel launch");
+}
+// The shares of the vocabulary: as few passes of up to 256 entries as 148 CTAs need, each as even as eights allow.
+template <bool GRAD>
+int few_logits(const Args& a, const bf16* h, long long ldh, FewParams& p, cudaStream_t st) {
+    const int nt = few_tokens(a.n);
+    FewMaps maps{};
+    int rc = make_map(&maps.w, a.w, 2, a.d, a.vocab, a.ldw, 64, p.tile, true);
+    if (!rc) rc = make_map(&maps.h, h, 2, a.d, a.n, ldh, 64, nt, true);
+    if (rc) return rc;
+    switch (nt) {
+        case 16: return launch_few<16, GRAD>(maps, p, st);
+        case 32: return launch_few<32, GRAD>(maps, p, st);
+        case 64: return launch_few<64, GRAD>(maps, p, st);
+        default: return launch_few<128, GRAD>(maps, p, st);
+    }
+}
+FewParams few_params(const Args& a) {
+    FewParams p{};
+    const long long passes = (a.vocab + 148 * 256ll - 1) / (148 * 256ll), share = (a.vocab + 148 * passes - 1) / (148 * passes);
+    p.tile = static_cast<int>((share + 7) / 8 * 8);
+    p.tiles = static_cast<int>((a.vocab + static_cast<long long>(p.tile) - 1) / p.tile);
+    p.vocab = a.vocab;
+    p.d = a.d;
+    p.n = static_cast<int>(a.n);
+    p.target = a.target;
+    p.cap = a.cap;
+    return p;
+}
+int forward_few(const Args& a, cudaStream_t st) {
+    FewParams p = few_params(a);
+    const int nt = few_tokens(a.n);
+    void* base = nullptr;
+    int rc = scratch_alloc(&base, 512 + sizeof(float2) * nt * static_cast<size_t>(p.tiles), st);
+    if (rc) return rc;
+    p.top = static_cast<float*>(base);
+    p.stats = reinterpret_cast<float2*>(static_cast<char*>(base) + 512);
+    rc = few_logits<false>(a, a.h, a.ldh, p, st);
+    if (!rc) {
+        const cudaError_t e = launch_pdl(join_few_kernel, dim3(static_cast<unsigned>(a.n)), dim3(256), 0, st, a, p.top, p.stats, p.tiles, nt);
+        rc = e == cudaSuccess ? check_launch("join_few_kernel") : cuda_fail(e, "join_few_kernel launch");
+    }
+    scratch_free(base, st);
+    return rc;
+}
+
 int forward(const Args& a, cudaStream_t st) {
+    if (a.n <= kFewMost) return forward_few(a, st);
     const int tiles_m = tiles(a.n, 256), tiles_n = tiles(a.vocab, 256);
     if (static_cast<long long>(tiles_m) * tiles_n > 0x3FFFFFFFll) return fail(TB_ERR_CAPACITY, "tb_lm_loss: %lld tiles", static_cast<long long>(tiles_m) * tiles_n);
     Scratch s{};
@@ -463,22 +800,34 @@ int forward(const Args& a, cudaStream_t st) {
     return rc;
 }
 
+// Shares of K for each of dh's tiles: those whose last wave wastes least, a share's FP32 sums
+// (a tile written and read again) counted as the time of 8 slices.
+int dh_splits(long long tiles, long long slices) {
+    double best = 0;
+    int splits = 1;
+    for (int s = 1; s <= 32 && s <= slices; ++s) {
+        const double cost = static_cast<double>((tiles * s + kPairs - 1) / kPairs) * ((slices + s - 1) / s + 8);
+        if (s == 1 || cost < 0.97 * best) best = cost, splits = s;
+    }
+    return splits;
+}
 constexpr long long kPieceG = 128ll << 20;  // bytes of G in one piece of the vocabulary
 
 int backward(const Args& a, cudaStream_t st) {
     const int tiles_m = tiles(a.n, 256), tiles_d = tiles(a.d, 256);
     const long long rows = up(a.n, 256);
-    const long long piece = std::min(up(a.vocab, 256), std::max(256ll, kPieceG / (2 * rows) / 256 * 256));
+    const bool few = a.n <= kFewMost;
+    const long long g_rows = few ? few_tokens(a.n) : rows;
+    const long long piece = few ? up(a.vocab, 8) : std::min(up(a.vocab, 256), std::max(256ll, kPieceG / (2 * rows) / 256 * 256));
     if (tiles_m * (piece / 256) > 0x3FFFFFFFll || tiles_m * static_cast<long long>(tiles_d) * kPairs > 0x3FFFFFFFll || piece / 256 * tiles_d > 0x3FFFFFFFll)
         return fail(TB_ERR_CAPACITY, "tb_lm_loss_backward: %lld tokens of %d", a.n, a.d);
     // dh's tiles share out their K where they do not fill the GPU
-    int splits = 1;
-    while (2ll * splits * tiles_m * tiles_d <= kPairs && piece / 64 / (2 * splits) >= 4) splits *= 2;
+    const int splits = dh_splits(static_cast<long long>(tiles_m) * tiles_d, (piece + 63) / 64);
     Scratch s{};
     void* base = nullptr;
     char* rest = nullptr;
     const long long ldp = up(a.d, 4);
-    const size_t g_bytes = sizeof(bf16) * rows * piece, part_bytes = a.dh ? sizeof(float) * splits * rows * ldp : 0;
+    const size_t g_bytes = up(sizeof(bf16) * g_rows * piece, 256), part_bytes = a.dh ? sizeof(float) * splits * rows * ldp : 0;
     int rc = make_scratch(a, g_bytes + part_bytes, &s, &base, &rest, st);
     if (rc) return rc;
     s.g = reinterpret_cast<bf16*>(rest);
@@ -494,7 +843,14 @@ int backward(const Args& a, cudaStream_t st) {
         p.cap = a.cap;
         p.rows = rows;
         p.row = s.row;
-        {
+        if (few) {
+            FewParams q = few_params(a);
+            q.count = s.count;
+            q.row = s.row;
+            q.g = s.g;
+            q.ldg = piece;
+            rc = few_logits<true>(a, s.h, s.ld, q, st);
+        } else {
             pair::Launch<Gradient> L{};
             L.p = p;
             L.p.tiles_n = tiles(cols, 256);
@@ -515,7 +871,7 @@ int backward(const Args& a, cudaStream_t st) {
             L.p.k = cols;
             L.p.splits = splits;
             L.p.first = v0 == 0;
-            rc = operand_map(&L.a[0], s.g, rows, cols, piece, false);
+            rc = operand_map(&L.a[0], s.g, g_rows, cols, piece, false);
             if (!rc) rc = operand_map(&L.b[0][0], w, cols, a.d, a.ldw, true);
             if (!rc) rc = make_out_map(&L.o[0][0], s.part, false, a.d, rows, splits, ldp, rows * ldp);
             if (!rc) rc = launch_product(L, static_cast<long long>(tiles_m) * tiles_d * splits, st);
@@ -530,13 +886,13 @@ int backward(const Args& a, cudaStream_t st) {
             L.p.ldo = a.lddw;
             // (a TMA store writes whole 16 bytes of a row, whatever the row's length)
             L.p.out_tma = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && a.lddw % 8 == 0 && a.d % 8 == 0;
-            rc = operand_map(&L.a[0], s.g, rows, cols, piece, true);
+            rc = operand_map(&L.a[0], s.g, g_rows, cols, piece, true);
             if (!rc) rc = operand_map(&L.b[0][0], s.h, rows, a.d, s.ld, true);
             if (!rc && L.p.out_tma) rc = make_out_map(&L.o[0][0], L.p.out, true, a.d, cols, 1, a.lddw, a.lddw * cols);
             if (!rc) rc = launch_product(L, static_cast<long long>(tiles(cols, 256)) * tiles_d, st);
         }
     }
-    if (!rc && a.dh) rc = launch_small("join_dh_kernel", join_dh_kernel, (a.n + 7) / 8, st, a, s, splits);
+    if (!rc && a.dh) rc = launch_small("join_dh_kernel", join_dh_kernel, a.n * ((a.d + 1023) / 1024), st, a, s, splits);
     scratch_free(base, st);
     return rc;
 }
