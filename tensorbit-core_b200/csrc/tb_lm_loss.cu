@@ -86,7 +86,7 @@ struct Scratch {
 };
 
 constexpr int kScan = 4096;    // targets that are counted ahead in one piece
-constexpr int kGather = 8;     // tokens of a gathering block, one a warp
+constexpr int kFewGather = 512; // up to so many tokens, a gathering block has one, of which each warp copies a part; else eight, one a warp
 
 __device__ __forceinline__ bool kept(const Args& a, long long t) {
     const int64_t y = __ldg(a.target + t);
@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(256) tally_kernel(const Args a, Tally* tallies
 }
 // Copies the kept tokens' rows together and zeros behind them up to the end of a tile;
 // results of tokens left out are zeros.
-template <bool BACKWARD>
+template <bool BACKWARD, bool ONE>
 __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch s) {
     __shared__ Tally shared[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long t0 = static_cast<long long>(blockIdx.x) * kGather;
+    const long long t0 = static_cast<long long>(blockIdx.x) * (ONE ? 1 : 8);
     Tally before{0, 0.0f, 0.0f}, all{0, 0.0f, 0.0f};
     if (s.tallies) {
         const int blocks = static_cast<int>((a.n + kScan - 1) / kScan), own = static_cast<int>(t0 / kScan);
@@ -161,18 +161,20 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
         *s.count = all.kept;
         *s.unit = usual ? unit : 1.0f;
     }
-    const long long t = t0 + warp;
+    const long long t = t0 + (ONE ? 0 : warp);
+    const int part = ONE ? threadIdx.x : lane;  // of a row's units
+    constexpr int kParts = ONE ? 256 : 32;
     const bool mine = t < a.n && kept(a, t);
     if (t < a.n) {
         const int units = (a.d + 7) / 8;
         if (mine) {
             long long to = before.kept;
-            for (int i = 0; i < warp; ++i) to += kept(a, t0 + i);
+            for (int i = 0; !ONE && i < warp; ++i) to += kept(a, t0 + i);
             const uint4* from = reinterpret_cast<const uint4*>(a.h + t * a.ldh);
             uint4* dst = reinterpret_cast<uint4*>(s.h + to * s.ld);
 #pragma unroll 8
-            for (int i = lane; i < units; i += 32) dst[i] = __ldg(from + i);
-            if (lane == 0) {
+            for (int i = part; i < units; i += kParts) dst[i] = __ldg(from + i);
+            if (part == 0) {
                 s.token[to] = t;
                 Row r{0.0f, 0.0f, 0.0f, static_cast<int>(a.target[t])};
                 if (BACKWARD) {
@@ -185,15 +187,15 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
             }
         } else if (BACKWARD) {
             if (a.dh)
-                for (int i = lane; i < a.d; i += 32) a.dh[t * a.lddh + i] = __float2bfloat16_rn(0.0f);
-        } else if (lane == 0) {
+                for (int i = part; i < a.d; i += kParts) a.dh[t * a.lddh + i] = __float2bfloat16_rn(0.0f);
+        } else if (part == 0) {
             a.loss[t] = 0.0f;
             a.lse[t] = 0.0f;
         }
     }
     // rows behind the last token, each warp's share
     const long long end = (all.kept + 255) / 256 * 256;
-    for (long long r = all.kept + t0 + warp; r < end; r += static_cast<long long>(gridDim.x) * kGather) {
+    for (long long r = all.kept + blockIdx.x * 8ll + warp; r < end; r += gridDim.x * 8ll) {
         uint4* dst = reinterpret_cast<uint4*>(s.h + r * s.ld);
         for (int i = lane; i < s.ld / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
         if (lane == 0) s.row[r] = Row{0.0f, 0.0f, 0.0f, -1};
@@ -425,7 +427,8 @@ int make_scratch(const Args& a, size_t more, Scratch* s, void** base, char** res
 template <bool BACKWARD>
 int gather(const Args& a, const Scratch& s, cudaStream_t st) {
     if (s.tallies) tally_kernel<BACKWARD><<<static_cast<unsigned>((a.n + kScan - 1) / kScan), 256, 0, st>>>(a, s.tallies);
-    gather_kernel<BACKWARD><<<static_cast<unsigned>((a.n + kGather - 1) / kGather), 256, 0, st>>>(a, s);
+    if (a.n <= kFewGather) gather_kernel<BACKWARD, true><<<static_cast<unsigned>(a.n), 256, 0, st>>>(a, s);
+    else gather_kernel<BACKWARD, false><<<static_cast<unsigned>((a.n + 7) / 8), 256, 0, st>>>(a, s);
     return check_launch("gather_kernel");
 }
 template <typename... P, typename... A>
@@ -466,6 +469,26 @@ struct FewParams {
 struct FewMaps {
     CUtensorMap w, h;
 };
+// N columns (16 or 32) over a warp's 32 rows: column `lane` % N of this lane in the end.  Each step halves
+// the columns that a lane has (37 tokens' forward: 64 us with five exchanges a column, FEW_US so).
+template <int N, class F>
+__device__ __forceinline__ float reduce_columns(float (&v)[N], int lane, F&& f) {
+    if constexpr (N == 16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = f(v[i], __shfl_xor_sync(~0u, v[i], 16));
+    }
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float keep = upper ? v[i + o] : v[i], send = upper ? v[i] : v[i + o];
+            v[i] = f(keep, __shfl_xor_sync(~0u, send, o));
+        }
+    }
+    return v[0];
+}
+
 template <int NT, bool GRAD>
 __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewParams p) {
     using C = FewCfg<NT>;
@@ -481,7 +504,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr uint32_t kColumns = 4 * NT < 32 ? 32 : 4 * NT;  // two sums of two halves
+    constexpr uint32_t kColumns = NT <= 16 ? 64 : NT <= 32 ? 128 : NT <= 64 ? 256 : 512;  // two sums of two halves
 
     if (threadIdx.x == 8 * 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w)) : "memory");
@@ -519,7 +542,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int slices = (p.d + 63) / 64;
+    const int slices = (p.d + 63) / 64, kept = GRAD ? *p.count : 0;
 
     if (warp < 8) {
         const int quad = warp & 3, half = warp >> 2;
@@ -564,23 +587,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                     float g = r.both * exp2f(fmaf(x, kLog2e, -r.lse2));
                     if (r.target == entry) g -= r.dloss;
                     // (a token behind the last kept one, of which z is what w times zeros gives, counts as zero)
-                    if (inside) p.g[i * p.ldg + entry] = __float2bfloat16_rn(i < *p.count ? g * slope : 0.0f);
+                    if (inside) p.g[i * p.ldg + entry] = __float2bfloat16_rn(i < kept ? g * slope : 0.0f);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    float x = z[i];
-                    if (p.cap > 0.0f) x = p.cap * tanhf(x * inverse);
-                    if (inside && rows[i].target == entry) p.top[i] = x;
-                    if (!inside) x = -INFINITY;
-                    float m = x;
+                    if (p.cap > 0.0f) z[i] = p.cap * tanhf(z[i] * inverse);
+                    if (inside && rows[i].target == entry) p.top[i] = z[i];
+                    if (!inside) z[i] = -INFINITY;
+                }
+                constexpr int N = NT % 32 ? 16 : 32;
+                float2* mine = joined + warp * NT;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                    const float base = m == -INFINITY ? 0.0f : m * kLog2e;
-                    float e = exp2f(fmaf(x, kLog2e, -base));
+                for (int c = 0; c < NT; c += N) {
+                    float v[N];
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(~0u, e, o);
-                    if (lane == 0) joined[warp * NT + i] = make_float2(m, e);
+                    for (int i = 0; i < N; ++i) v[i] = z[c + i];
+                    const float most = reduce_columns(v, lane, [](float x, float y) { return fmaxf(x, y); });
+                    if (lane < N) mine[c + lane].x = most;
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float m = mine[c + i].x;
+                        v[i] = exp2f((z[c + i] - (m == -INFINITY ? 0.0f : m)) * kLog2e);
+                    }
+                    const float sum = reduce_columns(v, lane, [](float x, float y) { return x + y; });
+                    if (lane < N) mine[c + lane].y = sum;
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (threadIdx.x < NT) {
@@ -706,7 +738,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float
     a.loss[t] = (m - top[t]) + rest;  // (the difference of like logits first: it is exact)
 }
 
-int few_tokens(long long n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+int few_tokens(long long n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 48 ? 48 : n <= 64 ? 64 : n <= 96 ? 96 : 128; }
 template <int NT, bool GRAD>
 int launch_few(const FewMaps& maps, const FewParams& p, cudaStream_t st) {
     static std::mutex mu;
@@ -736,7 +768,9 @@ int few_logits(const Args& a, const bf16* h, long long ldh, FewParams& p, cudaSt
     switch (nt) {
         case 16: return launch_few<16, GRAD>(maps, p, st);
         case 32: return launch_few<32, GRAD>(maps, p, st);
+        case 48: return launch_few<48, GRAD>(maps, p, st);
         case 64: return launch_few<64, GRAD>(maps, p, st);
+        case 96: return launch_few<96, GRAD>(maps, p, st);
         default: return launch_few<128, GRAD>(maps, p, st);
     }
 }
@@ -760,6 +794,7 @@ int forward_few(const Args& a, cudaStream_t st) {
     if (rc) return rc;
     p.top = static_cast<float*>(base);
     p.stats = reinterpret_cast<float2*>(static_cast<char*>(base) + 512);
+    pdl_fence(st);  // the caller may have queued a cross-stream wait
     rc = few_logits<false>(a, a.h, a.ldh, p, st);
     if (!rc) {
         const cudaError_t e = launch_pdl(join_few_kernel, dim3(static_cast<unsigned>(a.n)), dim3(256), 0, st, a, p.top, p.stats, p.tiles, nt);
@@ -900,6 +935,7 @@ int backward(const Args& a, cudaStream_t st) {
 bool bad_rows(const void* p, int64_t ld, int64_t cols) {
     return !p || reinterpret_cast<uintptr_t>(p) % 16 || ld < cols || ld % 8;
 }
+bool misaligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
 int check_args(const char* who, const tb_lm_loss_args* p, Args* a) {
     if (!p || p->struct_size != sizeof(tb_lm_loss_args)) return fail(TB_ERR_ARG, "%s: null args or bad struct_size", who);
     if (p->dtype != TB_BF16) return fail(TB_ERR_UNSUPPORTED, "%s: TB_BF16 only (dtype %d)", who, p->dtype);
@@ -910,7 +946,7 @@ int check_args(const char* who, const tb_lm_loss_args* p, Args* a) {
     if (bad_rows(p->w, p->ldw, p->d)) return fail(TB_ERR_ARG, "%s: w must be 16-byte aligned, ldw >= d a multiple of 8", who);
     if (p->n > 0) {
         if (bad_rows(p->h, p->ldh, p->d)) return fail(TB_ERR_ARG, "%s: h must be 16-byte aligned, ldh >= d a multiple of 8", who);
-        if (!p->target || !p->lse) return fail(TB_ERR_ARG, "%s: null target or lse", who);
+        if (!p->target || !p->lse || misaligned(p->target, 8) || misaligned(p->lse, 4)) return fail(TB_ERR_ARG, "%s: null or misaligned target or lse", who);
     }
     a->n = p->n;
     a->d = p->d;
@@ -952,7 +988,7 @@ extern "C" int tb_lm_loss(const tb_lm_loss_args* p, void* stream) {
     int rc = loss::check_args("tb_lm_loss", p, &a);
     if (rc) return rc;
     if (a.n == 0) return TB_OK;
-    if (!a.loss) return fail(TB_ERR_ARG, "tb_lm_loss: null loss");
+    if (!a.loss || loss::misaligned(a.loss, 4)) return fail(TB_ERR_ARG, "tb_lm_loss: null or misaligned loss");
     if ((rc = require_device(nullptr))) return rc;
     return loss::forward(a, static_cast<cudaStream_t>(stream));
 }
@@ -961,9 +997,9 @@ extern "C" int tb_lm_loss_backward(const tb_lm_loss_args* p, void* stream) {
     loss::Args a{};
     int rc = loss::check_args("tb_lm_loss_backward", p, &a);
     if (rc) return rc;
-    if (a.n > 0 && !a.dloss) return fail(TB_ERR_ARG, "tb_lm_loss_backward: null dloss");
-    if (a.dh && a.lddh < a.d) return fail(TB_ERR_ARG, "tb_lm_loss_backward: lddh < d");
-    if (a.dw && a.lddw < a.d) return fail(TB_ERR_ARG, "tb_lm_loss_backward: lddw < d");
+    if (a.n > 0 && (!a.dloss || loss::misaligned(a.dloss, 4) || loss::misaligned(a.dlse, 4))) return fail(TB_ERR_ARG, "tb_lm_loss_backward: null or misaligned dloss or dlse");
+    if (a.dh && (a.lddh < a.d || loss::misaligned(a.dh, 2))) return fail(TB_ERR_ARG, "tb_lm_loss_backward: dh is misaligned or lddh < d");
+    if (a.dw && (a.lddw < a.d || loss::misaligned(a.dw, 2))) return fail(TB_ERR_ARG, "tb_lm_loss_backward: dw is misaligned or lddw < d");
     if ((!a.dh || a.n == 0) && !a.dw) return TB_OK;
     if ((rc = require_device(nullptr))) return rc;
     auto st = static_cast<cudaStream_t>(stream);

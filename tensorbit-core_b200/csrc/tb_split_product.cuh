@@ -273,55 +273,60 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
     }
 }
 
-// How many clusters of `ctas` CTAs the device holds at once: SMs belong together in groups whose
-// numbers are not all multiples of `ctas` (clusters of four: 32 to 36, not 37).
+// How many clusters of 1 .. kSplitMost CTAs the device holds at once: SMs belong together in groups
+// whose numbers are not all multiples of them (clusters of four: fewer than 37).
+struct SplitClusters {
+    int most[kSplitMost + 1];
+};
 template <class OP>
-int split_setup(int ctas, int* clusters) {
+int split_setup(SplitClusters* out) {
     using C = SplitCfg<OP>;
     static std::mutex mu;
-    static int known[64][kSplitMost + 1] = {};
+    static SplitClusters known[64] = {};
     int dev = 0;
     int rc = require_device(&dev);
     if (rc) return rc;
     std::lock_guard<std::mutex> lk(mu);
-    int other = 0;
-    int& n = dev < 64 ? known[dev][ctas] : other;
-    if (!n) {
+    SplitClusters other{};
+    SplitClusters& n = dev < 64 ? known[dev] : other;
+    if (!n.most[0]) {
+        SplitClusters x{};
         cudaError_t e = cudaFuncSetAttribute(split_product_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-        cfg.blockDim = dim3(kSplitThreads);
-        cfg.dynamicSmemBytes = C::kSmem;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = static_cast<unsigned>(ctas);
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, split_product_kernel<OP>, &cfg);
+        for (int ctas = 1; ctas <= kSplitMost && e == cudaSuccess; ++ctas) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+            cfg.blockDim = dim3(kSplitThreads);
+            cfg.dynamicSmemBytes = C::kSmem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&x.most[ctas], split_product_kernel<OP>, &cfg);
+        }
         if (e != cudaSuccess) return cuda_fail(e, "split_product_kernel setup");
-        n = std::max(n, 1);
+        x.most[0] = 1;
+        n = x;
     }
-    *clusters = n;
+    *out = n;
     return TB_OK;
 }
 
 // CTAs of a cluster with which `units` tiles of 128 x 128 of `slices` each are sooner done than `pairs`
 // tiles of 256 x 256 by the pair kernel; 0 if with none.  In us (two parts): a slice takes a pair 0.82, and a CTA
-// 0.42, or 0.008 for each CTA at work; sums joined, 1.
-template <class OP>
-int choose_split(long long units, long long pairs, long long slices, int* ctas) {
+// 0.42, or 0.008 for each CTA at work; sums joined, 1.  (k = 1024, both sides measured: Q Q 13 us by clusters of
+// two, 22 by pairs; 4096: 300 and 110.)
+inline int choose_split(const SplitClusters& clusters, long long units, long long pairs, long long slices) {
     double best = 0.82 * slices * ((pairs + kPairs - 1) / kPairs);
-    *ctas = 0;
+    int ctas = 0;
     for (int c = 1; c <= kSplitMost && c <= slices; ++c) {
-        int clusters = 0;
-        const int rc = split_setup<OP>(c, &clusters);
-        if (rc) return rc;
-        const long long waves = (units + clusters - 1) / clusters;
-        const double cost = waves * ((slices + c - 1) / c) * std::max(0.42, 0.008 * std::min<long long>(units, clusters) * c) + (c > 1 ? 1.0 : 0.0);
-        if (cost < best) best = cost, *ctas = c;
+        const long long most = clusters.most[c];
+        if (most < 1) continue;
+        const double cost = (units + most - 1) / most * ((slices + c - 1) / c) * std::max(0.42, 0.008 * std::min(units, most) * c) + (c > 1 ? 1.0 : 0.0);
+        if (cost < best) best = cost, ctas = c;
     }
-    return TB_OK;
+    return ctas;
 }
 
 // Launches for `units` tiles of 128 x 128, each by `ctas` CTAs.
@@ -348,9 +353,10 @@ int launch_split(const Launch<OP>& L, long long units, int ctas, cudaStream_t st
 // By the sooner of the two.
 template <class OP>
 int launch_either(const Launch<OP>& L, long long units, long long pairs, long long slices, cudaStream_t st) {
-    int ctas = 0;
-    const int rc = choose_split<OP>(units, pairs, slices, &ctas);
+    SplitClusters clusters{};
+    const int rc = split_setup<OP>(&clusters);
     if (rc) return rc;
+    const int ctas = choose_split(clusters, units, pairs, slices);
     return ctas ? launch_split(L, units, ctas, st) : launch_product(L, pairs, st);
 }
 

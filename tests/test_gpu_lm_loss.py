@@ -92,3 +92,177 @@ def test_gradients(cuda, n, d, vocab, left, cap, with_dlse):
     for buf, r in ((dhb, n), (dwb, vocab)):  # what lies behind rows and their ends stays
         assert (buf[r:] == 3.0).all() and (buf[:, d:] == 3.0).all()
     status()
+
+
+@pytest.mark.parametrize("n,d,vocab", [(40, 72, 500), (300, 72, 500)])  # in one pass over w, and by tiles
+def test_left_out_tokens_reach_nothing(cuda, n, d, vocab):
+    """Whatever a token that is left out holds: as if its row were zeros."""
+    h, w, target, dloss, dlse = make(n, d, vocab, left=0.4, seed=2)
+    out = (target < 0) | (target >= vocab)
+    assert out.any() and not out.all()
+    ref = reference(h, w, target, 0.0, dloss, dlse)
+    h[out] = float("nan")
+    h[torch.nonzero(out)[0]] = float("inf")
+    dloss[out] = float("inf")
+    dlse[out] = float("nan")
+    dh, dw = torch.full((n, d), 3.0, device="cuda", dtype=BF), torch.full((vocab, d), 3.0, device="cuda", dtype=BF)
+    loss, lse = call(h, w, target, 0.0, dloss, dlse, dh, dw, backward=True)
+    for name, got in (("lse", lse), ("loss", loss), ("dh", dh), ("dw", dw)):
+        assert_within(got, ref, name)
+    assert (loss[out] == 0).all() and (lse[out] == 0).all() and (dh[out] == 0).all()
+
+
+@pytest.mark.parametrize("n", [30, 400])
+def test_all_tokens_left_out(cuda, n):
+    h, w, target, dloss, _ = make(n, 64, 200)
+    target[:] = -1
+    target[::2] = 1 << 40
+    dh, dw = torch.full((n, 64), 3.0, device="cuda", dtype=BF), torch.full((200, 64), 3.0, device="cuda", dtype=BF)
+    loss, lse = call(h, w, target, 0.0, dloss, None, dh, dw, backward=True)
+    for x in (loss, lse, dh, dw):
+        assert (x == 0).all()
+    status()
+
+
+def test_no_tokens(cuda):
+    w = torch.randn(50, 64, device="cuda").to(BF)
+    buf = torch.full((51, 80), 3.0, device="cuda", dtype=BF)
+    args = tb.lm_loss_args(n=0, d=64, vocab=50, h=None, ldh=64, w=w.data_ptr(), ldw=64, target=None, lse=None, dw=buf.data_ptr(), lddw=80)
+    tb.check(tb.lm_loss_backward(args, stream=torch.cuda.current_stream().cuda_stream))
+    assert (buf[:50, :64] == 0).all() and (buf[50:] == 3.0).all() and (buf[:, 64:] == 3.0).all()
+
+
+@pytest.mark.parametrize("n", [20, 300])
+def test_infinities_stay_with_their_token(cuda, n):
+    d, vocab = 64, 300
+    h, w, target, dloss, _ = make(n, d, vocab)
+    ref = reference(h, w, target, 0.0, dloss)
+    h[3, 5] = float("inf")
+    h[7, 1] = float("nan")
+    dloss[9] = float("inf")
+    dh = torch.empty(n, d, device="cuda", dtype=BF)
+    loss, lse = call(h, w, target, 0.0, dloss, None, dh, None, backward=True)
+    fine = torch.ones(n, device="cuda", dtype=torch.bool)
+    fine[[3, 7]] = False
+    for name, got in (("lse", lse), ("loss", loss)):
+        assert_within(got[fine], {k: v[fine] for k, v in ref.items() if k.startswith(name)}, name)
+        assert not torch.isfinite(got[~fine]).any()
+    fine[9] = False
+    # (the unit that the tokens' factors share is the largest finite one, with or without token 9)
+    assert_within(dh[fine], {k: v[fine] for k, v in ref.items() if k.startswith("dh")}, "dh")
+    assert not torch.isfinite(dh[9]).all()
+
+
+@pytest.mark.parametrize("n,d,vocab", [(33, 100, 257), (300, 264, 500)])
+@pytest.mark.parametrize("which", ["dh", "dw"])
+def test_one_gradient_in_rows_of_any_stride(cuda, n, d, vocab, which):
+    h, w, target, dloss, _ = make(n, d, vocab, left=0.2)
+    r = n if which == "dh" else vocab
+    buf = torch.full((r * (d + 3) + 2,), 3.0, device="cuda", dtype=BF)
+    out = torch.as_strided(buf, (r, d), (d + 3, 1), 1)  # rows that start on two bytes
+    call(h, w, target, 0.0, dloss, None, backward=True, **{which: out})
+    assert_within(out, reference(h, w, target, 0.0, dloss), which)
+    out.fill_(3.0)
+    assert (buf == 3.0).all()
+
+
+@pytest.mark.parametrize("n", [60, 700])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_gradients_against_differences(cuda, n, cap):
+    """dh and dw along random directions against central differences of the loss in 64 bits."""
+    d, vocab, eps = 96, 400, 1e-5
+    h, w, target, dloss, dlse = make(n, d, vocab, left=0.2, seed=5)
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    call(h, w, target, cap, dloss, dlse, dh, dw, backward=True)
+    ref = reference(h, w, target, cap, dloss, dlse)
+    kept = (target >= 0) & (target < vocab)
+
+    def total(hh, ww):
+        z = hh[kept] @ ww.t()
+        z = cap * torch.tanh(z / cap) if cap else z
+        lse = torch.logsumexp(z, 1)
+        loss = lse - z.gather(1, target[kept][:, None])[:, 0]
+        return (loss * dloss[kept].double() + lse * dlse[kept].double()).sum()
+
+    for got, name, x in ((dh, "dh", h), (dw, "dw", w)):
+        u = torch.randn(x.shape, device="cuda", dtype=torch.float64)
+        moved = [(h.double() + s * eps * u, w.double()) if name == "dh" else (h.double(), w.double() + s * eps * u) for s in (1, -1)]
+        slope = (total(*moved[0]) - total(*moved[1])) / (2 * eps)
+        along = (got.double() * u).sum()
+        # the values' bounds, and what differences leave: eps^2 of a third derivative of order one, 2^-50 / eps
+        assert abs(along - slope) <= (ref[name + "_bound"] * u.abs()).sum() + 1e-8
+
+
+@pytest.mark.parametrize("n", [48, 900])
+def test_same_bits_again(cuda, n):
+    h, w, target, dloss, dlse = make(n, 200, 3000, left=0.2)
+    got = []
+    for _ in range(3):
+        dh, dw = torch.empty(n, 200, device="cuda", dtype=BF), torch.empty(3000, 200, device="cuda", dtype=BF)
+        got.append((*call(h, w, target, 0.0, dloss, dlse, dh, dw, backward=True), dh, dw))
+    for other in got[1:]:
+        for x, y in zip(got[0], other):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n", [5, 500])
+def test_captured_and_replayed(cuda, n):
+    """Two graphs of one call, replayed in turn with other tokens and targets."""
+    d, vocab = 128, 700
+    h, w, target, dloss, _ = make(n, d, vocab, left=0.3)
+    graphs = []
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            loss, lse = call(h, w, target, 0.0, dloss, None, dh, dw, backward=True)
+            g.capture_end()
+        graphs.append((g, loss, lse, dh, dw))
+    torch.cuda.synchronize()
+    for seed in range(4):
+        h2, _, target2, dloss2, _ = make(n, d, vocab, left=0.1 * seed, seed=seed + 10)
+        h.copy_(h2)
+        target.copy_(target2)
+        dloss.copy_(dloss2)
+        ref = reference(h, w, target, 0.0, dloss)
+        for g, loss, lse, dh, dw in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, loss, lse, dh, dw in graphs:
+            for name, got in (("lse", lse), ("loss", loss), ("dh", dh), ("dw", dw)):
+                assert_within(got, ref, name)
+
+
+def test_two_streams_at_once(cuda):
+    cases = [make(n, 256, 2000, left=0.2, seed=n) for n in (90, 600)]
+    refs = [reference(c[0], c[1], c[2], 0.0, c[3]) for c in cases]
+    outs = [(torch.empty(c[0].shape, device="cuda", dtype=BF), torch.empty(c[1].shape, device="cuda", dtype=BF)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(3):
+        results = []
+        for c, (dh, dw), s in zip(cases, outs, streams):
+            with torch.cuda.stream(s):
+                results.append(call(c[0], c[1], c[2], 0.0, c[3], None, dh, dw, backward=True))
+    torch.cuda.synchronize()
+    for ref, (dh, dw), (loss, lse) in zip(refs, outs, results):
+        for name, got in (("lse", lse), ("loss", loss), ("dh", dh), ("dw", dw)):
+            assert_within(got, ref, name)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """h's rows lie 2^31 bytes and more apart."""
+    n, d, vocab = 4, 64, 300
+    ld = 1 << 30
+    buf = torch.empty(3 * ld + 128, device="cuda", dtype=BF)
+    h, w, target, dloss, _ = make(n, d, vocab)
+    far = torch.as_strided(buf, (n, d), (ld, 1))
+    far.copy_(h)
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    loss, lse = call(far, w, target, 0.0, dloss, None, dh, dw, backward=True)
+    ref = reference(h, w, target, 0.0, dloss)
+    for name, got in (("lse", lse), ("loss", loss), ("dh", dh), ("dw", dw)):
+        assert_within(got, ref, name)

@@ -88,3 +88,80 @@ def test_step(cuda, r, d, g, w, m, nesterov, pad):
     assert_near(mom[:r, :d], want_m, (clean[2].double().abs() + clean[1].double().abs()) * 2.0 ** -23, 0.0, "momentum")
     assert (W[r:] == 5.0).all() and (W[:, d:] == 5.0).all() and (mom[r:] == 5.0).all() and (mom[:, d:] == 5.0).all()
     assert (W[:r, :d][~keep] == 0).all() and (mom[:r, :d][~keep] == 0).all()
+
+
+@pytest.mark.parametrize("r,d", [(1500, 2100), (2100, 1501), (4097, 1700), (3100, 3000), (3300, 3300)])  # by clusters, and by pairs of CTAs
+def test_larger(cuda, r, d):
+    x = gradient(r, d, "falling")
+    want = ortho(x)
+    assert_near(run_ortho(x, pad=1), want, want.abs() * 2.0 ** -8, OFF * want.norm().item(), "larger")
+
+
+@pytest.mark.parametrize("r,d", [(40, 90), (300, 200)])
+def test_zeros_and_ranges(cuda, r, d):
+    z = torch.zeros(r, d, device="cuda")
+    assert (run_ortho(z) == 0).all()
+    assert (run_ortho(z, eps=0.0) == 0).all()
+    x = gradient(r, d, "noise")
+    want = ortho(x, eps=0.0)
+    for scale in (2.0 ** -100, 2.0 ** 100):  # (the squares leave FP32's range)
+        assert_near(run_ortho(x * scale, eps=0.0), want, want.abs() * 2.0 ** -8, OFF * want.norm().item(), f"times {scale:g}")
+    tiny = run_ortho(x * 2.0 ** -100)  # far below eps
+    assert (tiny.float().abs() <= 1e-20).all()
+    for bad in (float("nan"), float("inf")):
+        y = x.clone()
+        y[r // 2, d // 3] = bad
+        assert torch.isnan(run_ortho(y)).all()
+
+
+@pytest.mark.parametrize("r,d", [(100, 300), (700, 900)])
+def test_same_bits_again(cuda, r, d):
+    x = gradient(r, d, "falling")
+    first = run_ortho(x).clone()
+    for _ in range(3):
+        assert torch.equal(run_ortho(x), first)
+
+
+@pytest.mark.parametrize("r,d", [(64, 200), (600, 520)])
+def test_step_captured_and_replayed(cuda, r, d):
+    """Steps of a graph follow steps of the formula, new gradients each."""
+    m = 4
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    W = torch.randn(r, d, device="cuda", generator=gen) * 0.02
+    mom = torch.zeros(r, d, device="cuda")
+    mask = torch.randint(0, 16, (r * d // m,), device="cuda", generator=gen, dtype=torch.uint8)
+    keep = unpack_mask(mask, r, d, m)
+    grad = torch.zeros(r, d, device="cuda")
+    how = dict(beta=0.9, lr=0.01, weight_decay=0.1, scale=1.0)
+    args = tb.muon_args(r=r, d=d, grad=grad.data_ptr(), g_dtype=tb.F32, momentum=mom.data_ptr(), w=W.data_ptr(), w_dtype=tb.F32, mask=mask.data_ptr(), nm_m=m, **how)
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        g.capture_begin()
+        tb.check(tb.muon_step(args, stream=torch.cuda.current_stream().cuda_stream))
+        g.capture_end()
+    torch.cuda.synchronize()
+    for i in range(3):
+        grad.copy_(gradient(r, d, "falling", seed=20 + i))
+        want_w, want_m, o = step(W, grad, mom, keep, **how)
+        before = W.double().abs()
+        g.replay()
+        torch.cuda.synchronize()
+        assert_near(W, want_w, (before + 0.01 * o.abs()) * 2.0 ** -22, 0.01 * OFF * o.norm().item(), f"step {i}")
+        assert_near(mom, want_m, want_m.abs() * 2.0 ** -22 + grad.double().abs() * 2.0 ** -22, 0.0, f"momentum {i}")
+
+
+def test_two_streams_at_once(cuda):
+    xs = [gradient(*s, "falling") for s in ((100, 400), (900, 500))]
+    wants = [ortho(x) for x in xs]
+    outs = [torch.empty(x.shape, device="cuda", dtype=torch.bfloat16) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for x, o, s in zip(xs, outs, streams):
+            r, d = x.shape
+            tb.check(tb.orthogonalize(x.data_ptr(), tb.F32, d, r, d, o.data_ptr(), tb.BF16, d, stream=s.cuda_stream))
+    torch.cuda.synchronize()
+    for o, want in zip(outs, wants):
+        assert_near(o, want, want.abs() * 2.0 ** -8, OFF * want.norm().item(), "beside another")
+    status()
