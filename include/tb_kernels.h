@@ -423,9 +423,9 @@ typedef struct tb_lm_loss_args {
     void*    dw;           /* [vocab][lddw], any stride, or NULL                         */
     int64_t  lddw;
 } tb_lm_loss_args;
-/* loss and lse.  Logits are sums in FP32, up to 512 terms in the tensor core,
- * whose additions cut off (2.6e-7 of the sum where all terms have one sign), and
- * those added with rounding.  Scratch from the library's per-device pool: 2 bytes
+/* loss and lse.  Logits are sums in FP32, up to 1024 terms (64 where there are at
+ * most 128 tokens) in the tensor core, whose additions cut off, and those added with
+ * rounding: 7e-7 of the loss (2-norm) at 4096 features, as with FP32 products.  Scratch from the library's per-device pool: 2 bytes
  * per value of h, and 16 bytes per token and 256 entries. */
 int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
 /* Gradients of sum_t dloss_t loss_t + dlse_t lse_t, with lse from the forward on the

@@ -19,9 +19,6 @@
 #include "tb_pair_product.cuh"
 #include "tb_split_product.cuh"
 
-#ifndef TBG
-#define TBG 16
-#endif
 namespace tb {
 namespace loss {
 namespace {
@@ -223,10 +220,12 @@ struct Params {
 };
 __device__ __forceinline__ int kept_tiles(const Params& p) { return (*p.count + 255) / 256; }
 
-// Sums of 512 terms in the tensor core: a logit is off by 2.6e-7 of its terms' magnitude at most.
+// Sums of 1024 terms in the tensor core.  (2048 tokens, 4096 features, 2-norm of the loss's error: 1.6e-7 with
+// sums of 256, 3.1e-7 of 512, 6.5e-7 of 1024, which is what FP32 products have too, 3.1e-6 with one of all; tiles
+// of 35200 cycles with 1024, 34200 with one, of which the products need 32768.)
 struct Logits {
     static constexpr bool kAMn = false, kBMn = false, kF16 = false;
-    static constexpr int kParts = 1, kGroup = TBG;
+    static constexpr int kParts = 1, kGroup = 16;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return kept_tiles(p) * p.tiles_n; }
@@ -441,11 +440,11 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
 // Up to 128 tokens leave the logits bound by the reading of w.  Tokens are the N of the
 // product here and the vocabulary is M: a CTA takes `tile` rows of w (up to 256, two MMAs of 128), a
 // share that is even over all SMs, and streams them past the tokens' slices; a thread has one entry of the
-// vocabulary and all tokens.  Sums of 256 terms in the tensor core.
+// vocabulary and all tokens.  Sums of 64 terms in the tensor core, which costs nothing here.
 // (32000 x 4096, kernel: ONE_US for 1 token, FEW_US for 37; w at the measured copy rate 41.)
 constexpr int kFewMost = 128;
 constexpr int kFewThreads = 320;  // warps 0-7 results, 8 loads, 9 MMAs
-constexpr int kFewGroup = 4;
+constexpr int kFewGroup = 1;
 template <int NT>
 struct FewCfg {
     static constexpr int kStage = 32768 + NT * 128;

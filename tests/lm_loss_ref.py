@@ -1,10 +1,10 @@
 """The loss at the LM head and its gradients in 64 bits, with bounds on what the
 kernels' arithmetic may add, from the unit roundoffs alone.
 
-A logit is a sum of exact products: groups of 512 terms in the tensor core, whose 32
-steps of 16 terms each cut off less than 2^-23 of what the terms' magnitudes have
-added up to (and within a step as much again, counted as two steps more), then FP32
-additions of the groups.  A rounding to BF16, whose values have 8 bits, is off by at
+A logit is a sum of exact products: groups of 1024 terms in the tensor core (in the
+backward one of all), whose steps of 16 terms each cut off less than 2^-23 of what the
+terms' magnitudes have added up to (and within a step as much again, counted as two
+steps more), then FP32 additions of the groups.  A rounding to BF16, whose values have 8 bits, is off by at
 most half a step, 2^-8 of the value.  exp, log and the capping's tanh add a few units of 2^-24 and
 their arguments' roundings."""
 import torch
@@ -24,11 +24,13 @@ def reference(h, w, target, cap=0.0, dloss=None, dlse=None):
     i = torch.arange(len(t), device=h.device)
     raw = hd @ wd.t()
     size = hd.abs() @ wd.abs().t()
-    off = size * (34 * 2.0 ** -23 + (d / 512 + 1) * 2.0 ** -24)
+    off = size * ((min(d, 1024) / 16 + 2) * 2.0 ** -23 + (d / 1024 + 1) * 2.0 ** -24)
+    off_backward = size * (d / 16 + 2) * 2.0 ** -23
     z = raw
     if cap:
         z = cap * torch.tanh(raw / cap)
         off = off + raw.abs() * 2.0 ** -22 + z.abs() * 2.0 ** -21
+        off_backward = off_backward + raw.abs() * 2.0 ** -22 + z.abs() * 2.0 ** -21
     lse = torch.logsumexp(z, 1)
     worst = off.amax(1)
     lse_off = worst + 2.0 ** -21 * (4 + z.abs().amax(1) + lse.abs())
@@ -53,10 +55,10 @@ def reference(h, w, target, cap=0.0, dloss=None, dlse=None):
     g = slope * (both[:, None] * p - dl[:, None] * hot)
     g_size = both.abs()[:, None] * p + dl.abs()[:, None] * hot
     # p's relative error, then the rounding to BF16 and those of FP32; the slope's own error
-    p_off = off + lse_off[:, None] + 2.0 ** -21 * (4 + z.abs() + lse.abs()[:, None])
+    p_off = off_backward + lse_off[:, None] + 2.0 ** -21 * (4 + z.abs() + lse.abs()[:, None])
     g_off = slope * (both.abs()[:, None] * p * p_off + g_size * 2.0 ** -22) + g.abs() * 2.0 ** -8 + g_size * 2.0 ** -22 + 2.0 ** -133
     if cap:
-        g_off = g_off + g_size * 2 * (off + 2.0 ** -21 * z.abs()) / cap
+        g_off = g_off + g_size * 2 * (off_backward + 2.0 ** -21 * z.abs()) / cap
 
     def product(a, a_off, b):
         v = a @ b
