@@ -52,6 +52,26 @@ __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return 
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 
 // ---- U, and X from it ---------------------------------------------------------------
+// The .tb mask: a byte for each `group` weights, in the order of rows, bit k for the k-th; NULL keeps all.
+struct Mask {
+    const uint8_t* bytes;
+    int group, shift;  // shift: the group's logarithm, or -1
+};
+// Bits 0..3: whether weights i .. i + 3 are kept (of those that exist).
+__device__ __forceinline__ uint32_t kept4(const Mask& m, long long i, int exist) {
+    if (!m.bytes) return 15u;
+    if (m.shift == 2 && i % 4 == 0) return __ldg(m.bytes + (i >> 2));
+    if (m.shift == 3 && i % 4 == 0) return __ldg(m.bytes + (i >> 3)) >> (i & 4);
+    uint32_t bits = 0;
+    long long at = m.shift >= 0 ? i >> m.shift : static_cast<long long>(static_cast<unsigned long long>(i) / static_cast<unsigned>(m.group));
+    int in = static_cast<int>(i - at * m.group);
+    for (int e = 0; e < 4 && e < exist; ++e) {
+        bits |= (__ldg(m.bytes + at) >> in & 1u) << e;
+        if (++in == m.group) in = 0, ++at;
+    }
+    return bits;
+}
+
 struct Source {
     int r, d;
     const void* g;
@@ -61,15 +81,8 @@ struct Source {
     long long ldm;
     float beta;
     int nesterov;
-    const uint8_t* mask;
-    int group;        // weights of one mask byte
-    int shift;        // its logarithm, or -1
+    Mask mask;
 };
-__device__ __forceinline__ bool kept(const Source& s, long long i) {
-    if (!s.mask) return true;
-    const long long at = s.shift >= 0 ? i >> s.shift : static_cast<long long>(static_cast<unsigned long long>(i) / static_cast<unsigned>(s.group));
-    return __ldg(s.mask + at) >> static_cast<int>(i - at * s.group) & 1;
-}
 // Four columns from `col`, zeros behind the row's end and for pruned weights.
 template <typename T>
 __device__ __forceinline__ void load4(const T* row, int col, int d, bool wide, float (&v)[4]) {
@@ -96,12 +109,10 @@ __device__ __forceinline__ void update4(const Source& s, long long row, int col,
     const bool g_wide = wide_rows(s.g, s.ldg, s.g_bf16 ? 2 : 4);
     if (s.g_bf16) load4(static_cast<const bf16*>(s.g) + row * s.ldg, col, s.d, g_wide, u);
     else load4(static_cast<const float*>(s.g) + row * s.ldg, col, s.d, g_wide, u);
-    bool keep[4];
+    const uint32_t keep = kept4(s.mask, row * s.d + col, s.d - col);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        keep[e] = col + e < s.d && kept(s, row * s.d + col + e);
-        if (!keep[e]) u[e] = 0.0f;
-    }
+    for (int e = 0; e < 4; ++e)
+        if (!(keep >> e & 1)) u[e] = 0.0f;
     if (!s.m) return;
     float* at = s.m + row * s.ldm;
     const bool m_wide = wide_rows(s.m, s.ldm, 4);
@@ -109,7 +120,7 @@ __device__ __forceinline__ void update4(const Source& s, long long row, int col,
     load4(at, col, s.d, m_wide, m);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (UPDATE) m[e] = keep[e] ? fmaf(s.beta, m[e], u[e]) : 0.0f;
+        if (UPDATE) m[e] = keep >> e & 1 ? fmaf(s.beta, m[e], u[e]) : 0.0f;
         u[e] = s.nesterov ? fmaf(s.beta, m[e], u[e]) : m[e];
     }
     if constexpr (UPDATE) {
@@ -188,10 +199,79 @@ struct Params {
     // results
     void* result;
     long long ldr;
-    const uint8_t* mask;
-    int group, shift, w_bf16;
+    Mask mask;
+    int w_bf16;
     float decay, step;    // W <- mask (decay W - step O)
 };
+// Four weights' step; `exist` of them are the row's.
+__device__ __forceinline__ void update_weights(const Mask& mask, long long flat, bool w_bf16, void* row, int col, int exist, float decay, const float (&change)[4]) {
+    const uint32_t keep = kept4(mask, flat, exist);
+    if (w_bf16) {
+        bf16* w = static_cast<bf16*>(row) + col;
+        if (exist >= 4 && reinterpret_cast<uintptr_t>(w) % 8 == 0) {
+            const uint2 x = *reinterpret_cast<const uint2*>(w);
+            const float f[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xFFFF0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xFFFF0000u)};
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = keep >> e & 1 ? fmaf(decay, f[e], -change[e]) : 0.0f;
+            *reinterpret_cast<uint2*>(w) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        } else {
+            for (int e = 0; e < 4 && e < exist; ++e) w[e] = __float2bfloat16_rn(keep >> e & 1 ? fmaf(decay, __bfloat162float(w[e]), -change[e]) : 0.0f);
+        }
+    } else {
+        float* w = static_cast<float*>(row) + col;
+        if (exist >= 4 && reinterpret_cast<uintptr_t>(w) % 16 == 0) {
+            const float4 x = *reinterpret_cast<const float4*>(w);
+            const float f[4] = {x.x, x.y, x.z, x.w};
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = keep >> e & 1 ? fmaf(decay, f[e], -change[e]) : 0.0f;
+            *reinterpret_cast<float4*>(w) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+            for (int e = 0; e < 4 && e < exist; ++e) w[e] = keep >> e & 1 ? fmaf(decay, w[e], -change[e]) : 0.0f;
+        }
+    }
+}
+// Where rows of weights are whole sixteen (BF16: eight) bytes, `rows` of 32 columns from a piece of O: four columns
+// of every fourth row a lane, all loads before the first store.  (A column a lane, its parameters read again for each
+// weight, made the 4096 x 4096 step's last product 600 us; so STEP_US, and 282 where it is not a step.)
+template <bool BF16>
+__device__ __forceinline__ void update_piece(const uint8_t* buf, const Mask& mask, char* w, long long pitch, long long flat, int n, int rows, float decay, float step, int lane) {
+    const int sub = lane >> 3, unit = lane & 7;
+    uint4 x[8];
+    uint32_t keep[8];
+    constexpr int kUnit = BF16 ? 8 : 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = min(4 * i + sub, rows - 1);
+        if constexpr (BF16) {
+            const uint2 v = *reinterpret_cast<const uint2*>(w + r * pitch + unit * kUnit);
+            x[i].x = v.x;
+            x[i].y = v.y;
+        } else {
+            x[i] = *reinterpret_cast<const uint4*>(w + r * pitch + unit * kUnit);
+        }
+        keep[i] = kept4(mask, flat + static_cast<long long>(r) * n + 4 * unit, 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + sub;
+        const float4 o = *reinterpret_cast<const float4*>(buf + piece_at(r, 16 * unit));
+        const float change[4] = {step * o.x, step * o.y, step * o.z, step * o.w};
+        float f[4], y[4];
+        if constexpr (BF16) {
+            f[0] = __uint_as_float(x[i].x << 16); f[1] = __uint_as_float(x[i].x & 0xFFFF0000u);
+            f[2] = __uint_as_float(x[i].y << 16); f[3] = __uint_as_float(x[i].y & 0xFFFF0000u);
+        } else {
+            f[0] = __uint_as_float(x[i].x); f[1] = __uint_as_float(x[i].y); f[2] = __uint_as_float(x[i].z); f[3] = __uint_as_float(x[i].w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = keep[i] >> e & 1 ? fmaf(decay, f[e], -change[e]) : 0.0f;
+        if (r >= rows) continue;
+        if constexpr (BF16) *reinterpret_cast<uint2*>(w + r * pitch + unit * kUnit) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        else *reinterpret_cast<float4*>(w + r * pitch + unit * kUnit) = make_float4(y[0], y[1], y[2], y[3]);
+    }
+}
 
 // Fills a piece of 64 columns x 32 rows with the lane's row of one part.
 __device__ __forceinline__ void fill_part(uint8_t* buf, const uint32_t (&v)[32], int lane) {
@@ -396,14 +476,33 @@ struct Apply {
             for (int i = 0; i < 128; ++i) acc[i] *= alpha;
             store_rows<true>(buf, acc, static_cast<bf16*>(p.result) + row0 * p.ldr + col, p.ldr, rows, cols, lane);
         } else {
-            const float step = p.step * alpha;
+            const Mask mask = p.mask;
+            const float step = p.step * alpha, decay = p.decay;
+            const bool w_bf16 = p.w_bf16;
+            const int n = p.n, size = w_bf16 ? 2 : 4;
+            const long long pitch = p.ldr * size;
+            char* w0 = static_cast<char*>(p.result) + row0 * pitch;
+            const bool whole = (reinterpret_cast<uintptr_t>(p.result) | pitch) % (4 * size) == 0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                if (32 * c >= cols) break;
+                const int col0 = col + 32 * c, left = cols - 32 * c;
+                if (left <= 0) break;
                 __syncwarp();
                 fill_piece<false>(buf, acc, c, lane);
                 __syncwarp();
-                update_rows(p, buf, row0, col + 32 * c + lane, rows, 32 * c + lane < cols, step, lane);
+                const long long flat = static_cast<long long>(row0) * n + col0;
+                if (whole && left >= 32) {
+                    if (w_bf16) update_piece<true>(buf, mask, w0 + col0 * 2, pitch, flat, n, rows, decay, step, lane);
+                    else update_piece<false>(buf, mask, w0 + col0 * 4, pitch, flat, n, rows, decay, step, lane);
+                } else {
+                    const int unit = 4 * (lane & 7);
+#pragma unroll 1
+                    for (int r = lane >> 3; r < rows && unit < left; r += 4) {
+                        const float4 o = *reinterpret_cast<const float4*>(buf + piece_at(r, 4 * unit));
+                        const float change[4] = {step * o.x, step * o.y, step * o.z, step * o.w};
+                        update_weights(mask, flat + static_cast<long long>(r) * n + unit, w_bf16, w0 + r * pitch, col0 + unit, left - unit, decay, change);
+                    }
+                }
             }
         }
     }
@@ -434,57 +533,8 @@ struct Apply {
                     if (col + e < p.n) out[e] = __float2bfloat16_rn(x[e]);
             }
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < p.n) update_weight(p, row, col + e, x[e]);
-        }
-    }
-    static __device__ __forceinline__ void update_weight(const Params& p, int row, int col, float change) {
-        bool keep = true;
-        if (p.mask) {
-            const long long flat = static_cast<long long>(row) * p.n + col;
-            const long long group = p.shift >= 0 ? flat >> p.shift : static_cast<long long>(static_cast<unsigned long long>(flat) / static_cast<unsigned>(p.group));
-            keep = __ldg(p.mask + group) >> static_cast<int>(flat - group * p.group) & 1;
-        }
-        const long long at = row * p.ldr + col;
-        if (p.w_bf16) {
-            bf16* w = static_cast<bf16*>(p.result) + at;
-            *w = __float2bfloat16_rn(keep ? fmaf(p.decay, __bfloat162float(*w), -change) : 0.0f);
-        } else {
-            float* w = static_cast<float*>(p.result) + at;
-            *w = keep ? fmaf(p.decay, *w, -change) : 0.0f;
-        }
-    }
-    // One column of up to 32 rows of weights a lane.
-    static __device__ __noinline__ void update_rows(const Params& p, const uint8_t* buf, int row0, int col, int rows, bool inside, float step, int lane) {
-        if (!inside) return;
-        constexpr int kBatch = 16;
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += kBatch) {
-            float w[kBatch];
-            uint32_t bits[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int r = min(r0 + i, rows - 1);
-                const long long at = (row0 + r) * p.ldr + col;
-                w[i] = p.w_bf16 ? __bfloat162float(static_cast<const bf16*>(p.result)[at]) : static_cast<const float*>(p.result)[at];
-                bits[i] = 1;
-                if (p.mask) {
-                    const long long flat = static_cast<long long>(row0 + r) * p.n + col;
-                    const long long group = p.shift >= 0 ? flat >> p.shift : static_cast<long long>(static_cast<unsigned long long>(flat) / static_cast<unsigned>(p.group));
-                    bits[i] = __ldg(p.mask + group) >> static_cast<int>(flat - group * p.group);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int r = r0 + i;
-                if (r >= rows) break;
-                const float o = *reinterpret_cast<const float*>(buf + piece_at(r, 4 * lane));
-                const float x = bits[i] & 1 ? fmaf(p.decay, w[i], -(step * o)) : 0.0f;
-                const long long at = (row0 + r) * p.ldr + col;
-                if (p.w_bf16) static_cast<bf16*>(p.result)[at] = __float2bfloat16_rn(x);
-                else static_cast<float*>(p.result)[at] = x;
-            }
+            char* w = static_cast<char*>(p.result) + row * p.ldr * (p.w_bf16 ? 2 : 4);
+            update_weights(p.mask, static_cast<long long>(row) * p.n + col, p.w_bf16, w, col, p.n - col, p.decay, x);
         }
     }
 };
@@ -732,8 +782,8 @@ int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
 struct Result {
     void* out;
     long long ld;
-    const uint8_t* mask;
-    int group, shift, w_bf16;
+    Mask mask;
+    int w_bf16;
     float decay, step;
 };
 // X (Q X, tall: X Q) into `out`, or into the result.
@@ -754,8 +804,6 @@ int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res
     p.result = res.out;
     p.ldr = res.ld;
     p.mask = res.mask;
-    p.group = res.group;
-    p.shift = res.shift;
     p.w_bf16 = res.w_bf16;
     p.decay = res.decay;
     p.step = res.step;
@@ -913,15 +961,11 @@ extern "C" int tb_muon_step(const tb_muon_args* p, void* stream) {
     s.ldm = ldm;
     s.beta = p->beta;
     s.nesterov = p->nesterov;
-    s.mask = p->mask;
-    s.group = p->nm_m;
-    s.shift = muon::shift_of(p->nm_m);
+    s.mask = {p->mask, p->nm_m, muon::shift_of(p->nm_m)};
     muon::Result res{};
     res.out = p->w;
     res.ld = ldw;
-    res.mask = p->mask;
-    res.group = p->nm_m;
-    res.shift = s.shift;
+    res.mask = s.mask;
     res.w_bf16 = p->w_dtype == TB_BF16;
     res.decay = static_cast<float>(1.0 - static_cast<double>(p->lr) * p->weight_decay);
     res.step = static_cast<float>(static_cast<double>(p->lr) * p->scale);
