@@ -539,32 +539,72 @@ struct Apply {
     }
 };
 
-// ---- short sides up to 128: a segment's k x k products in one launch ----------------------
-// One CTA with A (then P A), P and Q as operands in shared memory, 64 KB each; every product
-// is one 128 x 128 tile.  A thread turns 64 columns of a row of the accumulator into the
-// next operand's parts.  (Three steps, k = 128: CORE_US, of which the tensor core works CORE_MMA; as eight launches 76.)
-constexpr int kCoreThreads = 288, kCoreMatrix = 65536, kCorePart = 16384;  // warps 0-7 results, 8 loads and MMAs
-constexpr size_t kCoreSmem = 3 * kCoreMatrix + 1024 + 64;
-struct CoreMaps {
-    CUtensorMap a[2];
+// ---- short sides up to 128 -----------------------------------------------------------------
+// All of the iteration in one launch, by a cluster of up to 8 CTAs that share the long side out.
+// Each sums its part of A; the cluster's CTAs add up a share of A's rows each, through distributed shared memory,
+// and copy the others'; then each forms Q by itself, and its own part of Q X.
+//
+// A (then P A), P and Q lie in shared memory as operands, 64 KB each, every product of them one 128 x 128
+// tile; a thread turns 32 columns of a row of the accumulator into the next operand's parts.  A chunk of X, 128 of its long side, is
+// four tiles of 64 columns x 128 rows (hi, hi, lo, lo) in the places of P and Q, which are not needed then.  The same
+// tile in memory is an operand along its rows and one along its columns.
+// (128 x 128, all: SHORT_US us; as eight launches 72.)  With `core` the kernel forms Q from A alone: long sides beyond
+// 4096 are better shared out over all SMs.
+constexpr int kShortThreads = 512, kShortMatrix = 65536, kShortTile = 16384;  // thread 0 also loads and issues MMAs
+constexpr int kShortChunks = 8;  // of 128: the most that the whole iteration is done here with
+constexpr size_t kShortSmem = 3 * kShortMatrix + 1024 + 128;
+struct ShortMaps {
+    CUtensorMap x[2];  // X's parts, or A's
 };
-struct CoreParams {
-    int k, steps;
-    uint16_t* out[2];
+struct ShortParams {
+    int k, r, d, tall, chunks;
+    int steps, segments;
+    int core;
+    uint16_t* x[2];    // X's parts, written anew between segments; or Q's
     long long ld;
+    void* result;
+    long long ldr;
+    Mask mask;
+    int w_bf16;
+    float decay, step;
 };
-__global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_constant__ CoreMaps maps, const __grid_constant__ CoreParams p) {
+__device__ __forceinline__ uint4 load_cluster_u4(uint32_t addr, uint32_t rank) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+        "ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
+// Place of 8 columns from `col` of row r in a matrix's operand: slices of 64 columns, each a tile of hi and one of lo parts.
+__device__ __forceinline__ int operand_at(int r, int col, int part) {
+    return (2 * (col >> 6) + part) * kShortTile + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4);
+}
+template <int OUT>
+__global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_constant__ ShortMaps maps, const __grid_constant__ ShortParams p, const int ctas) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + 3 * kCoreMatrix);
-    uint64_t* done = loaded + 1;  // [2] one of each accumulator
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+    uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + 3 * kShortMatrix);  // [2] a chunk's buffer filled
+    uint64_t* used = loaded + 2;                                            // [2] and read
+    uint64_t* done = used + 2;                                              // [2] an accumulator finished
+    uint64_t* taken = done + 2;                                             // [2] and read (products with X)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank());
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x[0])) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x[1])) : "memory");
+    }
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(loaded), 1);
-        mbar_init(smem_u32(&done[0]), 1);
-        mbar_init(smem_u32(&done[1]), 1);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&loaded[b]), 1);
+            mbar_init(smem_u32(&used[b]), 1);
+            mbar_init(smem_u32(&done[b]), 1);
+            mbar_init(smem_u32(&taken[b]), 16);
+        }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -577,130 +617,340 @@ __global__ void __launch_bounds__(kCoreThreads, 1) core_kernel(const __grid_cons
     fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
-    const bool issuer = warp == 8 && lane == 0;
-    if (issuer) {
-        mbar_expect_tx(smem_u32(loaded), kCoreMatrix);
-        for (int q = 0; q < 2; ++q)
-            for (int half = 0; half < 2; ++half)
-                tma_load_2d(smem_u32(smem + (2 * half + q) * kCorePart), &maps.a[q], 64 * half, 0, smem_u32(loaded));
-        if (!wait(smem_u32(loaded), 0, nullptr)) {
-            *abort_flag = 1;
-            atomicExch(&g_muon_error, 1);
-        }
-    }
-    __syncthreads();
 
-    // accumulator `d` = X Y^T of the matrices in buffers x and y (slices of 64 columns: hi, lo)
-    auto product = [&](int d, int x, int y) {
-        if (!issuer || *abort_flag) return;
-        constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | (8u << 24);
-        const uint64_t xd = operand_desc(smem_u32(smem + x * kCoreMatrix), false), yd = operand_desc(smem_u32(smem + y * kCoreMatrix), false);
-        constexpr uint64_t kLo = kCorePart >> 4;
-        for (int half = 0; half < (p.k > 64 ? 2 : 1); ++half)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-                const uint64_t a = xd + half * 2 * kLo + 2 * kk, b = yd + half * 2 * kLo + 2 * kk;
-                mma_one16<true>(tmem + 128 * d, a + kLo, b, kIdesc, half | kk);
-                mma_one16<true>(tmem + 128 * d, a, b + kLo, kIdesc, 1);
-                mma_one16<true>(tmem + 128 * d, a, b, kIdesc, 1);
-            }
-        mma_commit(smem_u32(&done[d]));
+    const bool issuer = threadIdx.x == 0;
+    const int row = (warp & 3) * 32 + lane, part4 = warp >> 2;  // a thread has columns 32 part4 .. of `row`
+    const int first = share_at(p.chunks, rank, ctas), own = share_at(p.chunks, rank + 1, ctas) - first;
+    constexpr uint32_t kIdesc = (1u << 4) | (8u << 24);  // FP16 operands, FP32 sums, M = 128
+    constexpr uint32_t kN128 = (128u >> 3) << 17, kAlongM = 1u << 15, kAlongN = 1u << 16;
+    constexpr uint64_t kLoMatrix = kShortTile >> 4, kLoChunk = 2 * kShortTile >> 4;  // from hi to lo: of a matrix's slice, of a chunk's tile
+    auto buffer = [&](int b) { return smem_u32(smem + b * kShortMatrix); };
+    // columns along memory's rows: K steps of 32 bytes; rows along K: steps of 16 rows, chunks of M or N a tile apart
+    auto tile_desc = [&](uint32_t at, bool mn) {
+        return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(mn ? kShortTile >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
     };
-    const int row = (warp & 3) * 32 + lane, half = (warp >> 2) & 1;  // of a thread with results: columns 64 half ..
-    uint32_t phase[2] = {0, 0};
-    uint32_t vh[32], vl[32];
-    // this thread's values of a finished accumulator, times alpha (plus beta C + diagonal I), split
-    auto take = [&](int d, float alpha, int c, float beta, float diagonal) {
-        if (warp >= 8) return;
-        if (!wait(smem_u32(&done[d]), phase[d], abort_flag)) {
-            *abort_flag = 1;
-            atomicExch(&g_muon_error, 1);
+    auto gave_up = [&] {
+        *abort_flag = 1;
+        atomicExch(&g_muon_error, 1);
+    };
+    // the issuer's counts: loads into each buffer, products with X into each accumulator
+    int loads[2] = {0, 0}, products[2] = {0, 0};
+    auto load_chunk = [&](int i, int b) {  // X's chunk `first` + i into buffer 1 + b
+        if (*abort_flag) return;
+        if (loads[b] && !wait(smem_u32(&used[b]), (loads[b] - 1) & 1, abort_flag)) return gave_up();
+        mbar_expect_tx(smem_u32(&loaded[b]), kShortMatrix);
+        const int at = 128 * (first + i);
+        for (int q = 0; q < 4; ++q)
+            tma_load_2d(buffer(1 + b) + q * kShortTile, &maps.x[q >> 1], (p.tall ? 0 : at) + 64 * (q & 1), p.tall ? at : 0, smem_u32(&loaded[b]));
+        ++loads[b];
+    };
+    auto chunk_ready = [&](int b) {
+        if (*abort_flag) return false;
+        if (!wait(smem_u32(&loaded[b]), (loads[b] - 1) & 1, abort_flag)) {
+            gave_up();
+            return false;
         }
-        phase[d] ^= 1;
         fence_after();
-        uint32_t x[2][32];
+        return true;
+    };
+    uint32_t phase[2] = {0, 0};  // of `done`
+    auto finished = [&](int d) {
+        if (!wait(smem_u32(&done[d]), phase[d], abort_flag) && !*abort_flag) gave_up();
+        phase[d] ^= 1;
+        __syncwarp();
+        fence_after();
+    };
+    float f[32];
+    auto read_sums = [&](int d) { tmem_ld32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(128 * d + 32 * part4), f); };
+    uint32_t hi[16], lo[16];
+    auto split_sums = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float f[32];
-            tmem_ld32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(128 * d + 64 * half + 32 * i), f);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[i][e] = __float_as_uint(f[e] * alpha);
-        }
-        fence_before();
-        const uint8_t* at = smem + c * kCoreMatrix + 2 * half * kCorePart + row * 128;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = __uint_as_float(x[j >> 2][(8 * j + e) & 31]);
-            if (c >= 0) {
-                const uint4 h = *reinterpret_cast<const uint4*>(at + ((j ^ (row & 7)) << 4)), l = *reinterpret_cast<const uint4*>(at + kCorePart + ((j ^ (row & 7)) << 4));
-                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
-                    w[2 * e] = fmaf(beta, hf.x, fmaf(beta, lf.x, w[2 * e]));
-                    w[2 * e + 1] = fmaf(beta, hf.y, fmaf(beta, lf.y, w[2 * e + 1]));
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (64 * half + 8 * j + e == row && row < p.k) w[e] += diagonal;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split16x2(w[2 * e], w[2 * e + 1], vh[4 * j + e], vl[4 * j + e]);
-        }
+        for (int i = 0; i < 16; ++i) split16x2(f[2 * i], f[2 * i + 1], hi[i], lo[i]);
     };
     auto put = [&](int to) {  // as an operand
-        if (warp >= 8) return;
-        uint8_t* at = smem + to * kCoreMatrix + 2 * half * kCorePart;
-        fill_part(at + (row - lane) * 128, vh, lane);
-        fill_part(at + kCorePart + (row - lane) * 128, vl, lane);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        uint8_t* at = smem + to * kShortMatrix;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<uint4*>(at + operand_at(row, 32 * part4 + 8 * j, 0)) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+            *reinterpret_cast<uint4*>(at + operand_at(row, 32 * part4 + 8 * j, 1)) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+        }
     };
-    auto meet = [&] {
+    auto meet = [&](bool x_too) {  // what was written here (and to X) may be read by MMAs (and TMA), and the accumulators be written
+        if (x_too) asm volatile("fence.proxy.async;" ::: "memory");
+        else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
         __syncthreads();
         fence_after();
     };
-    constexpr float kDown = 1.0f / (1 << kExpK);  // A, P and P A all have this power of two
-    int P = 1, Q = 1;
-    for (int i = 0; i < p.steps; ++i) {
-        const bool last = i == p.steps - 1;
-        if (i) P = 3 - Q;
-        product(0, 0, 0);
-        take(0, kC * kDown, 0, kB, kA * (1 << kExpK));
-        if (last && i == 0) break;
-        put(P);
-        meet();
-        if (last) {
-            product(0, P, Q);
-            take(0, i == 1 ? 1.0f / (1 << (2 * kExpK - kExpQ)) : kDown, -1, 0, 0);
-            break;
-        }
-        product(0, P, 0);
-        if (i) product(1, P, Q);
-        take(0, kDown, -1, 0, 0);
-        put(0);  // (the products that read A, and Q, ...
-        if (i) {
-            take(1, i == 1 ? 1.0f / (1 << (2 * kExpK - kExpQ)) : kDown, -1, 0, 0);
-            put(Q);  // ... are done)
-        }
-        meet();
-        product(0, P, 0);
-        take(0, kDown, -1, 0, 0);
-        put(0);
-        meet();
-    }
-    if (warp < 8 && row < p.k && !*abort_flag) {
+    // accumulator d = the product of the matrices in buffers x and y
+    auto product = [&](int d, int x, int y) {
+        if (!issuer || *abort_flag) return;
+        const uint64_t xd = tile_desc(buffer(x), false), yd = tile_desc(buffer(y), false);
+        for (int s = 0; s < (p.k > 64 ? 2 : 1); ++s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int col = 64 * half + 8 * j;
-            if (col >= p.ld) break;
-            *reinterpret_cast<uint4*>(p.out[0] + row * p.ld + col) = make_uint4(vh[4 * j], vh[4 * j + 1], vh[4 * j + 2], vh[4 * j + 3]);
-            *reinterpret_cast<uint4*>(p.out[1] + row * p.ld + col) = make_uint4(vl[4 * j], vl[4 * j + 1], vl[4 * j + 2], vl[4 * j + 3]);
+            for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t a = xd + s * 2 * kLoMatrix + 2 * kk, b = yd + s * 2 * kLoMatrix + 2 * kk;
+                mma_one16<true>(tmem + 128 * d, a + kLoMatrix, b, kIdesc | kN128, s | kk);
+                mma_one16<true>(tmem + 128 * d, a, b + kLoMatrix, kIdesc | kN128, 1);
+                mma_one16<true>(tmem + 128 * d, a, b, kIdesc | kN128, 1);
+            }
+        mma_commit(smem_u32(&done[d]));
+    };
+    // the accumulator's values times alpha (plus beta C + diagonal I), split
+    auto take = [&](int d, float alpha, int c, float beta, float diagonal) {
+        finished(d);
+        read_sums(d);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] *= alpha;
+        if (c >= 0) {
+            const uint8_t* at = smem + c * kShortMatrix;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 h = *reinterpret_cast<const uint4*>(at + operand_at(row, 32 * part4 + 8 * j, 0)), l = *reinterpret_cast<const uint4*>(at + operand_at(row, 32 * part4 + 8 * j, 1));
+                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hw[e])), lf = __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
+                    f[8 * j + 2 * e] = fmaf(beta, hf.x, fmaf(beta, lf.x, f[8 * j + 2 * e]));
+                    f[8 * j + 2 * e + 1] = fmaf(beta, hf.y, fmaf(beta, lf.y, f[8 * j + 2 * e + 1]));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] += 32 * part4 + i == row && row < p.k ? diagonal : 0.0f;
         }
+        split_sums();
+    };
+
+    constexpr float kDown = 1.0f / (1 << kExpK);  // A, P and P A all have this power of two
+    constexpr float kGram = 1.0f / (1 << (2 * kExpX - kExpK));
+    for (int seg = 0; seg < p.segments; ++seg) {
+        // ---- A into buffer 0 ----
+        if (p.core) {
+            if (issuer) {
+                mbar_expect_tx(smem_u32(&loaded[0]), kShortMatrix);
+                for (int q = 0; q < 4; ++q) tma_load_2d(buffer(0) + q * kShortTile, &maps.x[q & 1], 64 * (q >> 1), 0, smem_u32(&loaded[0]));
+                ++loads[0];
+                chunk_ready(0);
+            }
+            meet(false);
+        } else {
+            if (issuer) {
+                load_chunk(0, 0);
+                for (int i = 0; i < own; ++i) {
+                    const int b = i & 1;
+                    if (i + 1 < own) load_chunk(i + 1, b ^ 1);
+                    if (!chunk_ready(b)) break;
+                    // (two accumulators, so that no sum has more than half of the chunks)
+                    for (int s = 0; s < (p.tall || 64 < p.d - 128 * (first + i) ? 2 : 1); ++s)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint64_t x = p.tall ? tile_desc(buffer(1 + b), true) + (4 * s + kk) * 128 : tile_desc(buffer(1 + b) + s * kShortTile, false) + 2 * kk;
+                            const uint32_t idesc = kIdesc | kN128 | (p.tall ? kAlongM | kAlongN : 0u);
+                            mma_one16<true>(tmem + 128 * b, x + kLoChunk, x, idesc, i >= 2 || s || kk);
+                            mma_one16<true>(tmem + 128 * b, x, x + kLoChunk, idesc, 1);
+                            mma_one16<true>(tmem + 128 * b, x, x, idesc, 1);
+                        }
+                    mma_commit(smem_u32(&used[b]));
+                }
+                mma_commit(smem_u32(&done[0]));
+                if (own > 1) mma_commit(smem_u32(&done[1]));
+            }
+            __syncwarp();
+            finished(0);
+            read_sums(0);
+            if (own > 1) {
+                finished(1);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t x[16];
+                    tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(128 + 32 * part4 + 16 * c), x);
+                    tmem_wait16(x);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) add2(f[16 * c + i], f[16 * c + i + 1], x[i], x[i + 1]);
+                }
+            }
+            if (ctas == 1) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) f[i] *= kGram;
+                split_sums();
+                put(0);
+            }
+            if (ctas > 1) {
+                float* sums = reinterpret_cast<float*>(smem + kShortMatrix);  // rows of kSplitPitch, where the chunks were
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(sums + row * kSplitPitch + 32 * part4 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                __syncwarp();
+                cluster_arrive();
+                cluster_wait();
+                const int row0 = 2 * share_at(64, rank, ctas), rows = 2 * share_at(64, rank + 1, ctas) - row0;
+                for (int i = threadIdx.x; i < rows * 32; i += kShortThreads) {
+                    const int r = row0 + (i >> 5), c = 4 * (i & 31);
+                    float4 v[kSplitMost];
+#pragma unroll
+                    for (int q = 0; q < kSplitMost; ++q)
+                        if (q < ctas) v[q] = load_cluster4(smem_u32(sums + r * kSplitPitch + c), static_cast<uint32_t>(q));
+#pragma unroll
+                    for (int q = 1; q < kSplitMost; ++q)
+                        if (q < ctas) { v[0].x += v[q].x; v[0].y += v[q].y; v[0].z += v[q].z; v[0].w += v[q].w; }
+                    uint2 h, l;
+                    split16x2(v[0].x * kGram, v[0].y * kGram, h.x, l.x);
+                    split16x2(v[0].z * kGram, v[0].w * kGram, h.y, l.y);
+                    *reinterpret_cast<uint2*>(smem + operand_at(r, c, 0) + (c & 4) * 2) = h;
+                    *reinterpret_cast<uint2*>(smem + operand_at(r, c, 1) + (c & 4) * 2) = l;
+                }
+                __syncwarp();
+                cluster_arrive();
+                cluster_wait();
+                for (int i = threadIdx.x; i < 128 * 32; i += kShortThreads) {
+                    const int r = i >> 5, unit = i & 31;
+                    if (r >= row0 && r < row0 + rows) continue;
+                    int owner = 0;
+                    while (2 * share_at(64, owner + 1, ctas) <= r) ++owner;
+                    const int at = operand_at(r, 8 * (unit & 15), unit >> 4);
+                    *reinterpret_cast<uint4*>(smem + at) = load_cluster_u4(smem_u32(smem + at), static_cast<uint32_t>(owner));
+                }
+                __syncwarp();
+                cluster_arrive();  // (nobody's A, nor sums, change before all have read them)
+                cluster_wait();
+            }
+            meet(false);
+        }
+        // ---- Q of this segment's steps into buffer 0 ----
+        const int steps = p.steps * (seg + 1) / p.segments - p.steps * seg / p.segments;
+        int P = 1, Q = 1;
+        for (int i = 0; i < steps; ++i) {
+            const bool last = i == steps - 1;
+            if (i) P = 3 - Q;
+            product(0, 0, 0);
+            take(0, kC * kDown, 0, kB, kA * (1 << kExpK));
+            put(last && i == 0 ? 0 : P);  // (buffer 0: what a thread writes there it alone has read)
+            meet(false);
+            if (last && i == 0) break;
+            const float down_q = i == 1 ? 1.0f / (1 << (2 * kExpK - kExpQ)) : kDown;
+            if (last) {
+                product(0, P, Q);
+                take(0, down_q, -1, 0, 0);
+                put(0);
+                meet(false);
+                break;
+            }
+            product(0, P, 0);
+            if (i) product(1, P, Q);
+            take(0, kDown, -1, 0, 0);
+            put(0);  // (the products that read A, and Q, ...
+            if (i) {
+                take(1, down_q, -1, 0, 0);
+                put(Q);  // ... are done)
+            }
+            meet(false);
+            product(0, P, 0);
+            take(0, kDown, -1, 0, 0);
+            put(0);
+            meet(false);
+        }
+        if (p.core) {
+            if (row < p.k && !*abort_flag) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = 32 * part4 + 8 * j;
+                    if (col >= p.ld) break;
+                    *reinterpret_cast<uint4*>(p.x[0] + row * p.ld + col) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+                    *reinterpret_cast<uint4*>(p.x[1] + row * p.ld + col) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+                }
+            }
+            continue;
+        }
+        // ---- this CTA's part of Q X (tall: X Q) ----
+        const int exp_q = steps > 1 ? kExpQ : kExpK;
+        const bool end = seg == p.segments - 1;
+        const float alpha = 1.0f / static_cast<float>(1 << (end ? exp_q + kExpX - 13 : exp_q)) * (end ? 1.0f / 8192 : 1.0f);
+        auto multiply = [&](int i) {
+            const int b = i & 1;
+            if (!chunk_ready(b)) return;
+            if (products[b] && !wait(smem_u32(&taken[b]), (products[b] - 1) & 1, abort_flag)) return gave_up();
+            ++products[b];
+            fence_after();
+            const uint64_t qd = tile_desc(buffer(0), false);
+            const uint64_t x = tile_desc(buffer(1 + b), !p.tall);
+            const uint32_t idesc = kIdesc | kN128 | (p.tall ? 0u : kAlongN);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+                if (kk == 4 && p.k <= 64) break;
+                const uint64_t q = qd + (kk >> 2) * 2 * kLoMatrix + 2 * (kk & 3);
+                const uint64_t at = x + (p.tall ? (kk >> 2) * (kShortTile >> 4) + 2 * (kk & 3) : kk * 128);
+                if (p.tall) {
+                    mma_one16<true>(tmem + 128 * b, at + kLoChunk, q, idesc, kk);
+                    mma_one16<true>(tmem + 128 * b, at, q + kLoMatrix, idesc, 1);
+                    mma_one16<true>(tmem + 128 * b, at, q, idesc, 1);
+                } else {
+                    mma_one16<true>(tmem + 128 * b, q + kLoMatrix, at, idesc, kk);
+                    mma_one16<true>(tmem + 128 * b, q, at + kLoChunk, idesc, 1);
+                    mma_one16<true>(tmem + 128 * b, q, at, idesc, 1);
+                }
+            }
+            mma_commit(smem_u32(&used[b]));
+            mma_commit(smem_u32(&done[b]));
+        };
+        if (issuer) {
+            load_chunk(0, 0);
+            if (own > 1) load_chunk(1, 1);
+            multiply(0);
+        }
+        for (int i = 0; i < own; ++i) {
+            const int b = i & 1, at = 128 * (first + i);
+            if (issuer && i + 1 < own) {
+                multiply(i + 1);
+                if (i + 2 < own) load_chunk(i + 2, b);
+            }
+            __syncwarp();
+            finished(b);
+            if (*abort_flag) break;
+            read_sums(b);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&taken[b])) : "memory");
+            const int r = p.tall ? at + row : row, col = (p.tall ? 0 : at) + 32 * part4;
+            if (r >= p.r || col >= p.d) continue;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] *= alpha;
+            if (!end) {  // (rows of ld, a multiple of 8)
+                split_sums();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (col + 8 * j >= p.d) break;
+                    *reinterpret_cast<uint4*>(p.x[0] + r * p.ld + col + 8 * j) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+                    *reinterpret_cast<uint4*>(p.x[1] + r * p.ld + col + 8 * j) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+                }
+            } else if constexpr (OUT == kBf16) {
+                bf16* out = static_cast<bf16*>(p.result) + r * p.ldr + col;
+                const bool wide = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float* x = f + 8 * j;
+                    if (wide && col + 8 * j + 8 <= p.d) {
+                        *reinterpret_cast<uint4*>(out + 8 * j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (col + 8 * j + e < p.d) out[8 * j + e] = __float2bfloat16_rn(x[e]);
+                    }
+                }
+            } else if constexpr (OUT == kWeights) {
+                char* w = static_cast<char*>(p.result) + r * p.ldr * (p.w_bf16 ? 2 : 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (col + 4 * j >= p.d) break;
+                    const float change[4] = {p.step * f[4 * j], p.step * f[4 * j + 1], p.step * f[4 * j + 2], p.step * f[4 * j + 3]};
+                    update_weights(p.mask, static_cast<long long>(r) * p.d + col + 4 * j, p.w_bf16, w, col + 4 * j, p.d - col - 4 * j, p.decay, change);
+                }
+            }
+        }
+        meet(true);
     }
-    meet();
+    if (issuer && *abort_flag)  // loads in flight, within a limit
+        for (int b = 0; b < 2; ++b)
+            if (loads[b]) wait(smem_u32(&loaded[b]), (loads[b] - 1) & 1, nullptr);
+    meet(false);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
 }
 
@@ -757,28 +1007,6 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
     return launch_either(L, units, pairs, (p.k + 63) / 64, st);
 }
 
-// Q of `steps` steps from A, for k up to 128.
-int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
-    static std::mutex mu;
-    static uint64_t prepared = 0;  // per device: the shared-memory limit
-    int dev = 0;
-    int rc = require_device(&dev);
-    if (rc) return rc;
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (dev >= 64 || !(prepared >> dev & 1)) {
-            const cudaError_t e = cudaFuncSetAttribute(core_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCoreSmem));
-            if (e != cudaSuccess) return cuda_fail(e, "core_kernel setup");
-            if (dev < 64) prepared |= 1ull << dev;
-        }
-    }
-    CoreMaps maps{};
-    if ((rc = operand_maps(maps.a, A, false))) return rc;
-    const CoreParams p{static_cast<int>(A.rows), steps, {q.part[0], q.part[1]}, q.ld};
-    const cudaError_t e = launch_pdl(core_kernel, dim3(1), dim3(kCoreThreads), kCoreSmem, st, maps, p);
-    return e == cudaSuccess ? check_launch("core_kernel") : cuda_fail(e, "core_kernel launch");
-}
-
 struct Result {
     void* out;
     long long ld;
@@ -819,6 +1047,79 @@ int apply(bool tall, const Matrix& q, const Matrix& x, const Matrix& out, const 
     return tall ? apply<false, OUT>(q, x, out, res, st) : apply<true, OUT>(q, x, out, res, st);
 }
 
+template <int OUT>
+int launch_short(const ShortMaps& maps, const ShortParams& p, int ctas, cudaStream_t st) {
+    static std::mutex mu;
+    static uint64_t prepared = 0;  // per device: the shared-memory limit
+    int dev = 0;
+    const int rc = require_device(&dev);
+    if (rc) return rc;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 64 || !(prepared >> dev & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(short_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kShortSmem));
+            if (e != cudaSuccess) return cuda_fail(e, "short_kernel setup");
+            if (dev < 64) prepared |= 1ull << dev;
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(kShortThreads);
+    cfg.dynamicSmemBytes = kShortSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = pdl_allowed(st) ? 1 : 0;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, short_kernel<OUT>, maps, p, ctas);
+    return e == cudaSuccess ? check_launch("short_kernel") : cuda_fail(e, "short_kernel launch");
+}
+// Q of `steps` steps from A, for k up to 128.
+int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
+    ShortMaps maps{};
+    const int rc = operand_maps(maps.x, A, false);
+    if (rc) return rc;
+    ShortParams p{};
+    p.k = static_cast<int>(A.rows);
+    p.steps = steps;
+    p.segments = 1;
+    p.core = 1;
+    p.x[0] = q.part[0];
+    p.x[1] = q.part[1];
+    p.ld = q.ld;
+    return launch_short<kSplit>(maps, p, 1, st);
+}
+// All of it.
+template <int OUT>
+int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res, cudaStream_t st) {
+    ShortMaps maps{};
+    const int rc = operand_maps(maps.x, x, false);
+    if (rc) return rc;
+    ShortParams p{};
+    p.r = static_cast<int>(x.rows);
+    p.d = static_cast<int>(x.cols);
+    p.tall = tall;
+    p.k = std::min(p.r, p.d);
+    p.chunks = tiles(std::max(p.r, p.d), 128);
+    p.steps = steps;
+    p.segments = segments;
+    p.x[0] = x.part[0];
+    p.x[1] = x.part[1];
+    p.ld = x.ld;
+    p.result = res.out;
+    p.ldr = res.ld;
+    p.mask = res.mask;
+    p.w_bf16 = res.w_bf16;
+    p.decay = res.decay;
+    p.step = res.step;
+    return launch_short<OUT>(maps, p, std::min(kSplitMost, (p.chunks + 1) / 2), st);
+}
+
 // O(U) to the result.
 template <int OUT>
 int orthogonalize(const Source& s, int steps, float eps, const Result& res, cudaStream_t st) {
@@ -851,11 +1152,16 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
         const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx);
         rc = e == cudaSuccess ? check_launch("scale_kernel") : cuda_fail(e, "scale_kernel launch");
     }
+    const bool small = k <= 128;
+    if (!rc && small && std::max(s.r, s.d) <= 128 * kShortChunks) {
+        rc = whole<OUT>(x, tall, steps, segments, res, st);
+        scratch_free(base, st);
+        return rc;
+    }
     for (int seg = 0; seg < segments && !rc; ++seg) {
         const int n = steps * (seg + 1) / segments - steps * seg / segments;
         rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
         Matrix q = P[0];
-        const bool small = k <= 128;
         if (!rc && small) {
             if (n > 1) q = Q[0];
             rc = core(A, q, n, st);
