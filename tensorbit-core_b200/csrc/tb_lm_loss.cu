@@ -51,7 +51,7 @@ struct Args {
 // What is known of a kept token.  The backward's factors are relative to a unit that
 // all tokens share, the largest |dloss|, which dh and dW are multiplied by in FP32:
 // where all tokens count the same, the target's -1 is then exact in BF16.  (Tokens of
-// 1/1536 each: 2-norm of dW's error 2.6e-3 without a unit, UNIT_ERR with it, 1.7e-3 of
+// 1/1536 each: 2-norm of dW's error 2.6e-3 without a unit, 1.9e-3 with it, 1.7e-3 of
 // that the rounding of dW itself.)
 struct __align__(16) Row {
     float lse2;   // lse in powers of two
@@ -441,7 +441,8 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
 // product here and the vocabulary is M: a CTA takes `tile` rows of w (up to 256, two MMAs of 128), a
 // share that is even over all SMs, and streams them past the tokens' slices; a thread has one entry of the
 // vocabulary and all tokens.  Sums of 64 terms in the tensor core, which costs nothing here.
-// (32000 x 4096, kernel: ONE_US for 1 token, FEW_US for 37; w at the measured copy rate 41.)
+// (32000 x 4096, whole calls: 52 us for 1 token, 56 for 37, 68 for 128, by tiles of 256 tokens 70; w at the measured
+// copy rate 41.  128000 x 4096, 8 tokens: 167, at that rate 162.)
 constexpr int kFewMost = 128;
 constexpr int kFewThreads = 320;  // warps 0-7 results, 8 loads, 9 MMAs
 constexpr int kFewGroup = 1;
@@ -455,6 +456,7 @@ struct FewCfg {
 };
 struct FewParams {
     int tile, tiles, vocab, d;
+    int back;          // features from the last to the first
     int n;             // forward: tokens as they are
     const int* count;  // backward: those kept
     const int64_t* target;
@@ -469,7 +471,7 @@ struct FewMaps {
     CUtensorMap w, h;
 };
 // N columns (16 or 32) over a warp's 32 rows: column `lane` % N of this lane in the end.  Each step halves
-// the columns that a lane has (37 tokens' forward: 64 us with five exchanges a column, FEW_US so).
+// the columns that a lane has (37 tokens' forward, 64 columns: 64 us with five exchanges a column, 55 so).
 template <int N, class F>
 __device__ __forceinline__ float reduce_columns(float (&v)[N], int lane, F&& f) {
     if constexpr (N == 16) {
@@ -643,8 +645,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                     if (!wait(smem_u32(&empty[at.s]), at.phase ^ 1, abort_flag)) { ok = false; break; }  // (the first round passes at once)
                     const uint32_t stage = smem_u32(smem + at.s * C::kStage), bar = smem_u32(&ready[at.s]);
                     mbar_expect_tx(bar, static_cast<uint32_t>(p.tile) * 128 + NT * 128);
-                    tma_load_2d(stage, &maps.w, 64 * i, tile * p.tile, bar);
-                    tma_load_2d(stage + 32768, &maps.h, 64 * i, 0, bar);
+                    const int x = 64 * (p.back ? slices - 1 - i : i);
+                    tma_load_2d(stage, &maps.w, x, tile * p.tile, bar);
+                    tma_load_2d(stage + 32768, &maps.h, x, 0, bar);
                 }
             }
             if (!ok) {
@@ -845,6 +848,7 @@ int dh_splits(long long tiles, long long slices) {
     }
     return splits;
 }
+constexpr long long kBack = 512ll << 20;  // bytes of w
 constexpr long long kPieceG = 128ll << 20;  // bytes of G in one piece of the vocabulary
 
 int backward(const Args& a, cudaStream_t st) {
@@ -883,6 +887,9 @@ int backward(const Args& a, cudaStream_t st) {
             q.row = s.row;
             q.g = s.g;
             q.ldg = piece;
+            // The forward, which came before, has left w's last features in L2.  (37 tokens with gradients, 32000 x 4096: 229 us
+            // in the forward's order, 222 backwards; 16 tokens, 128000 x 4096, of which little is left: 700 and 720.)
+            q.back = 2ll * a.vocab * a.d <= kBack;
             rc = few_logits<true>(a, s.h, s.ld, q, st);
         } else {
             pair::Launch<Gradient> L{};

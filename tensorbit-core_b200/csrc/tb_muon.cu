@@ -133,8 +133,8 @@ __device__ __forceinline__ void update_four(const Source& s, bool m_wide, long l
             for (int e = 0; e < 4 && col + e < s.d; ++e) at[e] = x.m[e];
     }
 }
-// f(row, col, u) for all of U, by the threads of the grid: kBatch fours a thread at a time.  (A four at a time: 55 us for
-// the 4096 x 4096 step's first pass, NORM_US so, 27 at the measured copy rate.)
+// f(row, col, u) for all of U, by the threads of the grid: kBatch fours a thread at a time.  (The 4096 x 4096 step's first pass:
+// 55 us one at a time, 44 so, 65 with four in 76 registers; 27 at the measured copy rate.)
 template <bool UPDATE, class F>
 __device__ __forceinline__ void for_update(const Source& s, F&& f) {
     constexpr int kBatch = 2;
@@ -262,7 +262,7 @@ __device__ __forceinline__ void update_weights(const Mask& mask, long long flat,
 }
 // Where rows of weights are whole sixteen (BF16: eight) bytes, `rows` of 32 columns from a piece of O: four columns
 // of every fourth row a lane, all loads before the first store.  (A column a lane, its parameters read again for each
-// weight, made the 4096 x 4096 step's last product 600 us; so STEP_US, and 282 where it is not a step.)
+// weight, made the 4096 x 4096 step's last product 600 us; so 309, and 282 where it is not a step.)
 template <bool BF16>
 __device__ __forceinline__ void update_piece(const uint8_t* buf, const Mask& mask, char* w, long long pitch, long long flat, int n, int rows, float decay, float step, int lane) {
     const int sub = lane >> 3, unit = lane & 7;
@@ -576,8 +576,8 @@ struct Apply {
 // tile; a thread turns 32 columns of a row of the accumulator into the next operand's parts.  A chunk of X, 128 of its long side, is
 // four tiles of 64 columns x 128 rows (hi, hi, lo, lo) in the places of P and Q, which are not needed then.  The same
 // tile in memory is an operand along its rows and one along its columns.
-// (128 x 128, all: SHORT_US us; as eight launches 72.)  With `core` the kernel forms Q from A alone: long sides beyond
-// 4096 are better shared out over all SMs.
+// (128 x 128, whole call: 56 us, of which a product of the chain takes 1.65; as eight launches 79.  16 x 512: 61 and 66; 128 x 1024: 80
+// and 81; 128 x 2048: 89 and 83.)  With `core` the kernel forms Q from A alone: longer sides are better shared out over all SMs.
 constexpr int kShortThreads = 512, kShortMatrix = 65536, kShortTile = 16384;  // thread 0 also loads and issues MMAs
 constexpr int kShortChunks = 8;  // of 128: the most that the whole iteration is done here with
 constexpr size_t kShortSmem = 3 * kShortMatrix + 1024 + 128;
