@@ -457,7 +457,8 @@ int tb_orthogonalize(const void* x, int x_dtype, int64_t ldx, int r, int d, void
  *     U =  mask (g + beta m) with nesterov, else m
  *     W <- mask ((1 - lr weight_decay) W - lr scale O(U))
  * Whatever a pruned weight, its gradient or its momentum held, its W and m are zeros
- * afterwards.  Scratch as above. */
+ * afterwards; a NaN or an infinity in a kept one's U makes all kept weights NaN.
+ * Scratch as above. */
 typedef struct tb_muon_args {
     uint32_t struct_size;  /* sizeof(tb_muon_args)                                       */
     int32_t  r, d;         /* rows, columns                                              */

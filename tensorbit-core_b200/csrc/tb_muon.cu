@@ -1153,7 +1153,7 @@ template <int OUT>
 int orthogonalize(const Source& s, int steps, float eps, const Result& res, cudaStream_t st) {
     const bool tall = s.r > s.d;
     const long long k = std::min(s.r, s.d), ldx = up(s.d, 8), ldk = up(k, 8);
-    const size_t x_bytes = up(2 * s.r * ldx, 256), k_bytes = up(2 * k * ldk, 256);
+    const size_t x_bytes = up(2ll * s.r * ldx, 256), k_bytes = up(2ll * k * ldk, 256);
     const int segments = (steps + kSegment - 1) / kSegment;
     void* base = nullptr;
     int rc = scratch_alloc(&base, 8 * kNormBlocks + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
