@@ -82,7 +82,7 @@ struct Scratch {
     long long ldp;
 };
 
-constexpr int kScan = 4096;    // targets that are counted ahead in one piece
+constexpr int kScan = 1024;    // targets that are counted ahead in one piece, from two such pieces on (8000 tokens of 100 features: every block counting all 27 us, so 14)
 constexpr int kFewGather = 512; // up to so many tokens, a gathering block has one, of which each warp copies a part; else eight, one a warp
 
 __device__ __forceinline__ bool kept(const Args& a, long long t) {
@@ -199,6 +199,42 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
     }
 }
 
+// tanh of each of v / c, in place: the odd polynomial of degree 9 nearest to it up to 1/2 (1.4e-8 of the value; fitted at
+// Chebyshev points in 64 bits) where all of the lane's neighbours' values lie there, which takes a quarter of tanhf's time.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void tanh_of(float* v, float inverse) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] *= inverse;
+        most = fmaxf(most, fabsf(v[i]));
+        if (!(v[i] == v[i])) most = INFINITY;
+    }
+    if (__any_sync(~0u, most > 0.5f)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = tanhf(v[i]);
+        return;
+    }
+    const uint64_t c1 = pack2(-0.3333307206630707f, -0.3333307206630707f), c2 = pack2(0.13324828445911407f, 0.13324828445911407f);
+    const uint64_t c3 = pack2(-0.05298924073576927f, -0.05298924073576927f), c4 = pack2(0.017141319811344147f, 0.017141319811344147f), zero = pack2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t x = pack2(v[i], v[i + 1]), y = fma2(x, x, zero);
+        const uint64_t t = fma2(fma2(fma2(fma2(fma2(c4, y, c3), y, c2), y, c1), y, zero), x, x);  // x + x (c1 y + ...)
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(t));
+    }
+}
+
 struct Params {
     const int* count;
     const float* unit;
@@ -206,7 +242,7 @@ struct Params {
     int cols;          // columns of the product that exist
     int k;             // K of the product (dW: counted on the device)
     int col0;          // first entry of the vocabulary of this piece
-    int splits;        // dh
+    int splits;        // shares of K of dh's tiles, and of dW's
     int first;         // dh: the piece is the first
     float cap;
     long long rows;
@@ -241,7 +277,9 @@ struct Logits {
         if (p.cap > 0.0f) {
             const float inverse = 1.0f / p.cap;
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = p.cap * tanhf(acc[i] * inverse);
+            for (int c = 0; c < 128; c += 32) tanh_of<32>(acc + c, inverse);
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i] *= p.cap;
         }
         if (cols < 128) {
 #pragma unroll
@@ -281,18 +319,25 @@ struct Gradient {
         const Row r = p.row[row0 + lane];
         const int at = r.target - p.col0 - col;
         const bool hit = at >= 0 && at < 128;
-        const float inverse = 1.0f / p.cap;
+        if (p.cap > 0.0f) {
+            const float inverse = 1.0f / p.cap;
 #pragma unroll
-        for (int i = 0; i < 128; ++i) {
-            float z = acc[i], slope = 1.0f;
-            if (p.cap > 0.0f) {
-                const float t = tanhf(z * inverse);
-                z = p.cap * t;
-                slope = fmaf(-t, t, 1.0f);
+            for (int c = 0; c < 128; c += 32) {
+                tanh_of<32>(acc + c, inverse);
+#pragma unroll
+                for (int i = c; i < c + 32; ++i) {
+                    const float t = acc[i];
+                    float g = r.both * exp2f(fmaf(p.cap * t, kLog2e, -r.lse2));
+                    if (hit && i == at) g -= r.dloss;
+                    acc[i] = g * fmaf(-t, t, 1.0f);
+                }
             }
-            float g = r.both * exp2f(fmaf(z, kLog2e, -r.lse2));
-            if (hit && i == at) g -= r.dloss;
-            acc[i] = p.cap > 0.0f ? g * slope : g;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+                const float g = r.both * exp2f(fmaf(acc[i], kLog2e, -r.lse2));
+                acc[i] = hit && i == at ? g - r.dloss : g;
+            }
         }
         store_tma<true, 1>(&L.o[0][0], buf, acc, col, row0, 0, static_cast<int>(p.ldo), false, lane);
     }
@@ -325,10 +370,12 @@ struct WeightGrad {
     static constexpr int kParts = 1, kGroup = 1 << 30;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
-    static __device__ __forceinline__ int items(const Params& p) { return (p.out_rows + 255) / 256 * p.tiles_n; }
+    static __device__ __forceinline__ int items(const Params& p) { return (p.out_rows + 255) / 256 * p.tiles_n * p.splits; }
     static __device__ __forceinline__ Work work(const Params& p, int item) {
-        Work w{0, 0, 0, (*p.count + 63) / 64, 0, -1};
-        band_tile(item, (p.out_rows + 255) / 256, p.tiles_n, w.tm, w.tn);
+        const int all = (*p.count + 63) / 64, q = item % p.splits;
+        Work w{0, 0, share_at(all, q, p.splits), 0, 0, q};
+        w.slices = share_at(all, q + 1, p.splits) - w.k0;
+        band_tile(item / p.splits, (p.out_rows + 255) / 256, p.tiles_n, w.tm, w.tn);
         return w;
     }
     static __device__ __forceinline__ void finish(const Launch<WeightGrad>& L, const Work& w, float (&acc)[128], uint8_t* buf, int row_in, int half, int lane) {
@@ -336,6 +383,10 @@ struct WeightGrad {
         const int row0 = w.tm * 256 + row_in, col = w.tn * 256 + half * 128;
         const int rows = min(32, p.out_rows - row0), cols = p.cols - col;
         if (rows <= 0 || cols <= 0) return;
+        if (p.splits > 1) {
+            store_tma<false, 1>(&L.o[0][0], buf, acc, col, row0, w.slot, p.cols, false, lane);
+            return;
+        }
         const float unit = *p.unit;
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] *= unit;
@@ -397,6 +448,22 @@ __global__ void __launch_bounds__(256) join_dh_kernel(const Args a, const Scratc
         const float x[4] = {v.x, v.y, v.z, v.w};
         for (int e = 0; e < 4 && i + e < a.d; ++e) out[e] = __float2bfloat16_rn(x[e]);
     }
+}
+
+// A piece's dW from its shares, in order: 1024 columns of a row a block.
+__global__ void __launch_bounds__(256) join_dw_kernel(const float* part, const long long ldp, const int rows, const int d, const int splits, const float* unit, bf16* out,
+                                                      const long long ldo) {
+    pdl_wait();
+    const int chunks = (d + 1023) / 1024, r = blockIdx.x / chunks, i = static_cast<int>(blockIdx.x % chunks) * 1024 + 4 * threadIdx.x;
+    if (i >= d) return;
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int q = 0; q < splits; ++q) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (static_cast<long long>(q) * rows + r) * ldp + i);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    const float f[4] = {v.x * *unit, v.y * *unit, v.z * *unit, v.w * *unit};
+    for (int e = 0; e < 4 && i + e < d; ++e) out[r * ldo + i + e] = __float2bfloat16_rn(f[e]);
 }
 
 long long up(long long v, long long m) { return (v + m - 1) / m * m; }
@@ -574,16 +641,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             const int in = half * 128 + quad * 32 + lane;
             const long long entry = static_cast<long long>(tile) * p.tile + in;
             const bool inside = in < p.tile && entry < p.vocab;
-            const float inverse = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+            if (p.cap > 0.0f) {
+                const float inverse = 1.0f / p.cap;
+#pragma unroll
+                for (int c = 0; c < NT; c += 16) tanh_of<16>(z + c, inverse);
+            }
             if constexpr (GRAD) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const Row r = rows[i];
                     float x = z[i], slope = 1.0f;
                     if (p.cap > 0.0f) {
-                        const float t = tanhf(x * inverse);
-                        x = p.cap * t;
-                        slope = fmaf(-t, t, 1.0f);
+                        slope = fmaf(-x, x, 1.0f);
+                        x *= p.cap;
                     }
                     float g = r.both * exp2f(fmaf(x, kLog2e, -r.lse2));
                     if (r.target == entry) g -= r.dloss;
@@ -593,7 +663,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             } else {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    if (p.cap > 0.0f) z[i] = p.cap * tanhf(z[i] * inverse);
+                    if (p.cap > 0.0f) z[i] *= p.cap;
                     if (inside && rows[i].target == entry) p.top[i] = z[i];
                     if (!inside) z[i] = -INFINITY;
                 }
@@ -865,9 +935,16 @@ int backward(const Args& a, cudaStream_t st) {
     void* base = nullptr;
     char* rest = nullptr;
     const long long ldp = up(a.d, 4);
-    const size_t g_bytes = up(sizeof(bf16) * g_rows * piece, 256), part_bytes = a.dh ? sizeof(float) * splits * rows * ldp : 0;
-    int rc = make_scratch(a, g_bytes + part_bytes, &s, &base, &rest, st);
+    // dW's tiles share out theirs, the tokens, where there are many and the tiles leave most SMs idle (small heads):
+    // sixteen slices each, as the kernel that joins them takes the time of thirty.  (With gradients, 8000 tokens, 130 x 100: 122 us
+    // without shares, 89 with; 1000 tokens, 1000 x 200: 63 and 80.)
+    const long long dw_tiles = piece >= a.vocab ? tiles(a.vocab, 256) * static_cast<long long>(tiles_d) : kPairs, dw_slices = (a.n + 63) / 64;
+    const int dw_splits = dw_slices < 64 ? 1 : static_cast<int>(std::max(1ll, std::min(kPairs / dw_tiles, dw_slices / 16)));
+    const size_t g_bytes = up(sizeof(bf16) * g_rows * piece, 256), part_bytes = a.dh ? up(sizeof(float) * splits * rows * ldp, 256) : 0;
+    const size_t dw_bytes = a.dw && dw_splits > 1 ? sizeof(float) * dw_splits * a.vocab * ldp : 0;
+    int rc = make_scratch(a, g_bytes + part_bytes + dw_bytes, &s, &base, &rest, st);
     if (rc) return rc;
+    float* dw_part = reinterpret_cast<float*>(rest + g_bytes + part_bytes);
     s.g = reinterpret_cast<bf16*>(rest);
     s.part = reinterpret_cast<float*>(rest + g_bytes);
     s.ldp = ldp;
@@ -929,8 +1006,12 @@ int backward(const Args& a, cudaStream_t st) {
             L.p.out_tma = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && a.lddw % 8 == 0 && a.d % 8 == 0;
             rc = operand_map(&L.a[0], s.g, g_rows, cols, piece, true);
             if (!rc) rc = operand_map(&L.b[0][0], s.h, rows, a.d, s.ld, true);
-            if (!rc && L.p.out_tma) rc = make_out_map(&L.o[0][0], L.p.out, true, a.d, cols, 1, a.lddw, a.lddw * cols);
-            if (!rc) rc = launch_product(L, static_cast<long long>(tiles(cols, 256)) * tiles_d, st);
+            L.p.splits = dw_splits;
+            if (!rc && dw_splits > 1) rc = make_out_map(&L.o[0][0], dw_part, false, a.d, cols, dw_splits, ldp, ldp * cols);
+            else if (!rc && L.p.out_tma) rc = make_out_map(&L.o[0][0], L.p.out, true, a.d, cols, 1, a.lddw, a.lddw * cols);
+            if (!rc) rc = launch_product(L, static_cast<long long>(tiles(cols, 256)) * tiles_d * dw_splits, st);
+            if (!rc && dw_splits > 1)
+                rc = launch_small("join_dw_kernel", join_dw_kernel, static_cast<long long>(cols) * ((a.d + 1023) / 1024), st, dw_part, ldp, cols, a.d, dw_splits, s.unit, a.dw, a.lddw);
         }
     }
     if (!rc && a.dh) rc = launch_small("join_dh_kernel", join_dh_kernel, a.n * ((a.d + 1023) / 1024), st, a, s, splits);
