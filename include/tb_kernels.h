@@ -425,8 +425,9 @@ typedef struct tb_lm_loss_args {
 } tb_lm_loss_args;
 /* loss and lse.  Logits are sums in FP32, up to 1024 terms (64 where there are at
  * most 128 tokens) in the tensor core, whose additions cut off, and those added with
- * rounding: 7e-7 of the loss (2-norm) at 4096 features, as with FP32 products.  Scratch from the library's per-device pool: 2 bytes
- * per value of h, and 16 bytes per token and 256 entries. */
+ * rounding: 7e-7 of the loss (2-norm) at 4096 features, as with FP32 products.
+ * Scratch from the library's per-device pool: 2 bytes per value of h, and 16 bytes
+ * per token and 256 entries. */
 int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
 /* Gradients of sum_t dloss_t loss_t + dlse_t lse_t, with lse from the forward on the
  * same h, w and targets:
@@ -434,9 +435,11 @@ int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
  *     dh_t = sum_v g_tv w_v,   dw_v = sum_t g_tv h_t.
  * The vocabulary is gone through in pieces whose g enters both products as BF16
  * (2^-8 of each value).  dh and dw overwrite what is there; each sum has a fixed
- * order.  n = 0 gives a dw of zeros.  Scratch: as above, 128 MB of g (more beyond
- * 2^18 tokens), and 4 bytes per value of dh, up to 37 times that where few tokens
- * and features make few tiles. */
+ * order.  dh may be h's own memory, with its stride.  n = 0 gives a dw of zeros.
+ * Scratch: 2 bytes per value of h, up to 128 MB of g (more beyond 2^18 tokens), 4
+ * bytes per value of dh, up to 32 times that where its 256 x 256 tiles leave much of
+ * the GPU's last wave idle, and for dw at most 74 such tiles in FP32 where it has
+ * fewer than half as many. */
 int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
 
 /* ---- orthogonalised updates ------------------------------------------------ */
@@ -447,7 +450,8 @@ int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
  * reference counterpart.  x is [r][ldx] of TB_F32 or TB_BF16, out [r][ldo] of
  * TB_BF16, any strides; the shorter side ends at 32768.  Products keep 22 bits (two
  * FP16 parts of each operand, FP32 sums): the result is within 5e-4 (2-norm) of the
- * formula's, before it is rounded to BF16.  A zero matrix gives zeros; a NaN or an infinity makes all of out NaN.
+ * formula's, before it is rounded to BF16.  A zero matrix gives zeros; a NaN or an
+ * infinity makes all of out NaN.
  * Scratch from the library's per-device pool: 8 bytes per value of x (4 up to three
  * steps) and 24 for each of min(r, d)^2. */
 int tb_orthogonalize(const void* x, int x_dtype, int64_t ldx, int r, int d, void* out, int out_dtype, int64_t ldo,

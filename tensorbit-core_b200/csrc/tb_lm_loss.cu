@@ -151,12 +151,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
     }
     before = block_tally(before, shared);
     all = block_tally(all, shared);
-    const float unit = all.dloss > 0.0f ? all.dloss : all.dlse;
-    const bool usual = unit > 1e-30f && unit < 1e30f;  // (whose reciprocal exists)
-    const float inverse = usual ? 1.0f / unit : 1.0f;
+    const float most = all.dloss > 1e-15f * all.dlse ? all.dloss : all.dlse;  // (with dlse far above dloss, that)
+    const float unit = most > 1e-30f && most < 1e30f ? most : 1.0f, inverse = 1.0f / unit;  // (a reciprocal that exists)
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *s.count = all.kept;
-        *s.unit = usual ? unit : 1.0f;
+        *s.unit = unit;
     }
     const long long t = t0 + (ONE ? 0 : warp);
     const int part = ONE ? threadIdx.x : lane;  // of a row's units

@@ -266,3 +266,26 @@ def test_offsets_beyond_32_bits(cuda):
     ref = reference(h, w, target, 0.0, dloss)
     for name, got in (("lse", lse), ("loss", loss), ("dh", dh), ("dw", dw)):
         assert_within(got, ref, name)
+
+
+@pytest.mark.parametrize("n", [21, 333])
+def test_gradient_in_the_tokens_place(cuda, n):
+    h, w, target, dloss, dlse = make(n, 104, 600, left=0.3)
+    ref = reference(h, w, target, 0.0, dloss, dlse)
+    call(h, w, target, 0.0, dloss, dlse, h, None, backward=True)
+    assert_within(h, ref, "dh")
+
+
+@pytest.mark.parametrize("n", [21, 333])
+@pytest.mark.parametrize("size,penalty", [(1e-20, 1e20), (0.0, 1.0), (1e30, 1.0), (1e-38, 0.0)])
+def test_factors_of_any_size(cuda, n, size, penalty):
+    """dloss and dlse far apart, or far from one."""
+    h, w, target, dloss, dlse = make(n, 96, 500, left=0.2)
+    dloss, dlse = dloss * size, dlse * penalty
+    dh, dw = torch.empty(n, 96, device="cuda", dtype=BF), torch.empty(500, 96, device="cuda", dtype=BF)
+    call(h, w, target, 0.0, dloss, dlse, dh, dw, backward=True)
+    ref = reference(h, w, target, 0.0, dloss, dlse)
+    for name, got in (("dh", dh), ("dw", dw)):
+        # (a dloss 2^-133 below the unit, and results below FP32's smallest normal value, may be zero)
+        ref[name + "_bound"] = ref[name + "_bound"] + 2.0 ** -126 + 2.0 ** -120 * max(float(dloss.abs().max()), float(dlse.abs().max()))
+        assert_within(got, ref, name)
