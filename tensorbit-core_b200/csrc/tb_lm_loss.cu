@@ -303,11 +303,12 @@ struct Logits {
     }
 };
 
-// The same product, turned into G.  G enters its products as BF16, as every operand does: an error of
+// The same product, turned into G, in sums of 8192 terms (up to 4e-5 of a logit where all terms have one sign: G is
+// rounded to 2^-8).  G enters its products as BF16, as every operand does: an error of
 // 2^-8 of each of its values at most, which are summed with signs that do not depend on the errors'.
 struct Gradient {
     static constexpr bool kAMn = false, kBMn = false, kF16 = false;
-    static constexpr int kParts = 1, kGroup = 1 << 30;
+    static constexpr int kParts = 1, kGroup = 128;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return kept_tiles(p) * p.tiles_n; }
@@ -342,10 +343,10 @@ struct Gradient {
     }
 };
 
-// A piece's part of dh, added in FP32.
+// A piece's part of dh, in sums of 4096 entries, added in FP32.
 struct InputGrad {
     static constexpr bool kAMn = false, kBMn = true, kF16 = false;
-    static constexpr int kParts = 1, kGroup = 1 << 30;
+    static constexpr int kParts = 1, kGroup = 64;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return kept_tiles(p) * p.tiles_n * p.splits; }
@@ -363,10 +364,10 @@ struct InputGrad {
     }
 };
 
-// A piece's rows of dW, over all kept tokens.
+// A piece's rows of dW, over all kept tokens, in sums of 4096 of them (each of whose 256 steps cuts off up to 2^-23).
 struct WeightGrad {
     static constexpr bool kAMn = true, kBMn = true, kF16 = false;
-    static constexpr int kParts = 1, kGroup = 1 << 30;
+    static constexpr int kParts = 1, kGroup = 64;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return (p.out_rows + 255) / 256 * p.tiles_n * p.splits; }

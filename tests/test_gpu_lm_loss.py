@@ -289,3 +289,51 @@ def test_factors_of_any_size(cuda, n, size, penalty):
         # (a dloss 2^-133 below the unit, and results below FP32's smallest normal value, may be zero)
         ref[name + "_bound"] = ref[name + "_bound"] + 2.0 ** -126 + 2.0 ** -120 * max(float(dloss.abs().max()), float(dlse.abs().max()))
         assert_within(got, ref, name)
+
+
+def test_more_than_31_bits_of_weights(cuda):
+    """w and dw of 2.2e9 values: the last entries of the vocabulary, and all of them together in lse and dh."""
+    n, d, vocab = 3, 4096, 530000
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(vocab, d, device="cuda", dtype=BF).normal_(generator=g).mul_(0.02)
+    h = torch.randn(n, d, device="cuda", generator=g).to(BF)
+    target = torch.tensor([0, vocab - 1, 524288], device="cuda")
+    dloss = torch.ones(n, device="cuda")
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    loss, lse = call(h, w, target, 0.0, dloss, None, dh, dw, backward=True)
+    status()
+    z = torch.cat([h.double() @ part.double().t() for part in w.split(20000)], 1)
+    want = torch.logsumexp(z, 1)
+    top = z.gather(1, target[:, None])[:, 0]
+    # (bounds as in lm_loss_ref, with |h| . |w| at most 100 here)
+    off = 100 * (6 * 2.0 ** -23 + 65 * 2.0 ** -24) + 2.0 ** -21 * 40
+    assert ((lse.double() - want).abs() <= off).all() and ((loss.double() - want + top).abs() <= 2 * off).all()
+    p = torch.exp(z - want[:, None])
+    p.scatter_add_(1, target[:, None], torch.full((n, 1), -1.0, device="cuda", dtype=torch.float64))
+    size = torch.exp(z - want[:, None])
+    size.scatter_add_(1, target[:, None], torch.ones(n, 1, device="cuda", dtype=torch.float64))
+    for rows in (slice(0, 300), slice(524288, 524600), slice(vocab - 300, vocab)):
+        dw_want, terms = p[:, rows].t() @ h.double(), size[:, rows].t() @ h.double().abs()
+        assert ((dw[rows].double() - dw_want).abs() <= dw_want.abs() * 2.0 ** -8 * 1.01 + terms * (2.0 ** -8 + 4 * off) + 2.0 ** -133).all()
+    dh_want = sum(p[:, i:i + 20000] @ w[i:i + 20000].double() for i in range(0, vocab, 20000))
+    terms = sum(size[:, i:i + 20000] @ w[i:i + 20000].double().abs() for i in range(0, vocab, 20000))
+    assert ((dh.double() - dh_want).abs() <= dh_want.abs() * 2.0 ** -8 * 1.01 + terms * (2.0 ** -8 + 4 * off + vocab / 16 / 32 * 2.0 ** -23)).all()
+
+
+def test_gradients_of_many_tokens_of_one_sign(cuda):
+    """Sums over 200000 tokens whose terms all have one sign, which the tensor core's additions cut off."""
+    n, d, vocab = 200000, 32, 64
+    h = torch.full((n, d), 1.0, device="cuda", dtype=BF)
+    h[:, ::2] = 0.75
+    w = torch.zeros(vocab, d, device="cuda", dtype=BF)
+    w[0] = 0.25
+    target = torch.zeros(n, device="cuda", dtype=torch.int64)
+    dloss = torch.full((n,), 1.0, device="cuda")
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    call(h, w, target, 0.0, dloss, None, dh, dw, backward=True)
+    z = h[:1].double() @ w.double().t()
+    p = torch.softmax(z, 1)[0]
+    p[0] -= 1.0
+    want = n * p[:, None] * h[0].double()
+    # G's rounding and dW's own, and 300 steps cut off at 2^-24 on average
+    assert ((dw.double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -8 + 300 * 2.0 ** -23)).all()

@@ -165,3 +165,27 @@ def test_two_streams_at_once(cuda):
     for o, want in zip(outs, wants):
         assert_near(o, want, want.abs() * 2.0 ** -8, OFF * want.norm().item(), "beside another")
     status()
+
+
+@pytest.mark.parametrize("tall", [False, True])
+def test_more_than_31_bits_of_values(cuda, tall):
+    """2.2e9 values: by way of the short side's 64 x 64 matrices, at the long side's ends."""
+    k, D = 64, (1 << 25) + 11
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty((D, k) if tall else (k, D), device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    (x[:, :9] if tall else x[:9]).mul_(30)
+    got = run_ortho(x)
+    long = x if tall else x.t()
+    A = torch.zeros(k, k, device="cuda", dtype=torch.float64)
+    for i in range(0, D, 1 << 20):
+        part = long[i:i + (1 << 20)].double()
+        A += part.t() @ part
+    norm = A.trace().sqrt() + 1e-7
+    A, Q, eye = A / norm ** 2, torch.eye(k, device="cuda", dtype=torch.float64), torch.eye(k, device="cuda", dtype=torch.float64)
+    for _ in range(5):
+        P = 3.4445 * eye - 4.7750 * A + 2.0315 * A @ A
+        Q, A = P @ Q, P @ A @ P
+    for rows in (slice(0, 2000), slice((1 << 25) - 500, D)):
+        want = (long[rows].double() / norm) @ Q
+        part = (got[rows] if tall else got[:, rows].t())
+        assert_near(part, want, want.abs() * 2.0 ** -8, OFF * want.norm().item(), str(rows))
