@@ -354,16 +354,23 @@ struct Symmetric {
     }
     static __device__ __forceinline__ Work split_work(const Params& p, int item) { return work(p, item); }
     static constexpr bool kMirror = true;
-    static __device__ __forceinline__ void finish_quad(const Launch<Symmetric>& L, const Work& w, int row, int col, const float4& v, uint4& words) {
+    // C's parts
+    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Symmetric>& L, int row, int col) {
+        const Params& p = L.p;
+        if (!p.c[0] || row >= p.m || col >= p.n) return make_uint4(0, 0, 0, 0);
+        const long long at = row * p.ld + col;  // (rows of ld, a multiple of 8)
+        const uint2 h = *reinterpret_cast<const uint2*>(p.c[0] + at), l = *reinterpret_cast<const uint2*>(p.c[1] + at);
+        return make_uint4(h.x, h.y, l.x, l.y);
+    }
+    static __device__ __forceinline__ void finish_quad(const Launch<Symmetric>& L, const Work& w, int row, int col, const float4& v, const uint4& c, uint4& words) {
         const Params& p = L.p;
         const float alpha = p.alpha[w.which];
         const bool inside = row < p.m && col < p.n;
         const long long at = row * p.ld + col;  // (rows of ld, a multiple of 8)
         float x[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
         if (p.c[0] && inside) {
-            const uint2 h = *reinterpret_cast<const uint2*>(p.c[0] + at), l = *reinterpret_cast<const uint2*>(p.c[1] + at);
-            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-            const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&l.x)), l1 = __half22float2(*reinterpret_cast<const __half2*>(&l.y));
+            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&c.x)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&c.y));
+            const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&c.z)), l1 = __half22float2(*reinterpret_cast<const __half2*>(&c.w));
             const float hs[4] = {h0.x, h0.y, h1.x, h1.y}, ls[4] = {l0.x, l0.y, l1.x, l1.y};
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = fmaf(p.beta, hs[e], fmaf(p.beta, ls[e], x[e])) + (row == col + e ? p.diagonal : 0.0f);
@@ -539,7 +546,8 @@ struct Apply {
         return Work{tile / tiles, tile % tiles, 0, (p.k + 63) / 64, 0, -1};
     }
     static constexpr bool kMirror = false;
-    static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, uint4&) {
+    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Apply>&, int, int) { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, const uint4&, uint4&) {
         const Params& p = L.p;
         if (row >= p.m || col >= p.n) return;
         const float factor = OUT == kWeights ? p.alpha[0] * p.step : p.alpha[0];

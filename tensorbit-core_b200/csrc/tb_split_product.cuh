@@ -10,7 +10,8 @@
 //
 // Operations as for the pair kernel, with tiles of 128 from
 //   split_work(P, tile)
-//   finish_quad(L, w, row, col, v, words)   four columns; `words` go on to, where kMirror,
+//   fetch_quad(L, row, col)        what four columns need from memory, fetched while their sums arrive
+//   finish_quad(L, w, row, col, v, fetched, words)   four columns; `words` go on to, where kMirror,
 //   mirror(L, w, words, pitch, row, rows, thread)   the rows' words in shared memory
 #pragma once
 
@@ -233,10 +234,12 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
         constexpr int kBatch = 2;  // quads of a thread whose loads are under way together
         for (int i0 = threadIdx.x; i0 < rows * 32; i0 += kBatch * kSplitThreads) {
             float4 v[kBatch][kSplitMost];
+            uint4 ahead[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int i = min(i0 + b * kSplitThreads, rows * 32 - 1);
                 float* at = sums + (row + (i >> 5)) * kSplitPitch + 4 * (i & 31);
+                ahead[b] = OP::fetch_quad(L, w.tm * 128 + row + (i >> 5), w.tn * 128 + 4 * (i & 31));
                 if (ctas == 1) {
                     v[b][0] = *reinterpret_cast<float4*>(at);
                 } else {
@@ -255,7 +258,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
                     if (q < ctas) { x.x += v[b][q].x; x.y += v[b][q].y; x.z += v[b][q].z; x.w += v[b][q].w; }
                 const int r = i >> 5, c = 4 * (i & 31);
                 uint4 out;
-                OP::finish_quad(L, w, w.tm * 128 + row + r, w.tn * 128 + c, x, out);
+                OP::finish_quad(L, w, w.tm * 128 + row + r, w.tn * 128 + c, x, ahead[b], out);
                 if constexpr (OP::kMirror) *reinterpret_cast<uint4*>(words + r * kSplitPitch + c) = out;
             }
         }
