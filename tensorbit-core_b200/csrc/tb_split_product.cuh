@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
 }
 
 // How many clusters of 1 .. kSplitMost CTAs the device holds at once: SMs belong together in groups
-// whose numbers are not all multiples of them (clusters of four: fewer than 37).
+// whose numbers are not all multiples of them (clusters of four: 33, not 37).
 struct SplitClusters {
     int most[kSplitMost + 1];
 };
