@@ -426,6 +426,7 @@ typedef struct tb_lm_loss_args {
 /* loss and lse.  Logits are sums in FP32, up to 1024 terms (64 where there are at
  * most 128 tokens) in the tensor core, whose additions cut off, and those added with
  * rounding: 7e-7 of the loss (2-norm) at 4096 features, as with FP32 products.
+ * A loss is never below zero: exponentials are of exact differences from the largest logit.
  * Scratch from the library's per-device pool: 2 bytes per value of h, and 16 bytes
  * per token and 256 entries. */
 int tb_lm_loss(const tb_lm_loss_args* args, void* stream);

@@ -234,6 +234,20 @@ __device__ __forceinline__ void tanh_of(float* v, float inverse) {
     }
 }
 
+// exp(v - from) for `v` in place.  The difference first: it is exact where the two are alike, so that a maximum's exponential
+// is 1, where the difference of rounded products with log2(e) is off by up to |from| 2^-24.
+template <int N>
+__device__ __forceinline__ void exp_below(float (&v)[N], float from) {
+    const uint64_t one = pack2(1.0f, 1.0f), minus = pack2(-from, -from), log2e = pack2(kLog2e, kLog2e), zero = pack2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t x = fma2(fma2(pack2(v[i], v[i + 1]), one, minus), log2e, zero);
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(x));
+        v[i] = exp2f(v[i]);
+        v[i + 1] = exp2f(v[i + 1]);
+    }
+}
+
 struct Params {
     const int* count;
     const float* unit;
@@ -288,11 +302,6 @@ struct Logits {
         float m = acc[0];
 #pragma unroll
         for (int i = 1; i < 128; ++i) m = fmaxf(m, acc[i]);
-        const float base = m == -INFINITY ? 0.0f : m * kLog2e;
-        float s[4] = {};
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i & 3] += exp2f(fmaf(acc[i], kLog2e, -base));
-        p.stats[(2 * w.tn + half) * p.rows + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
         const int at = p.row[row].target - col;
         if (at >= 0 && at < 128) {
             float z = 0.0f;
@@ -300,6 +309,11 @@ struct Logits {
             for (int i = 0; i < 128; ++i) z = i == at ? acc[i] : z;
             p.top[row] = z;
         }
+        exp_below(acc, m == -INFINITY ? 0.0f : m);
+        float s[4] = {};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i & 3] += acc[i];
+        p.stats[(2 * w.tn + half) * p.rows + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
     }
 };
 
@@ -422,7 +436,7 @@ __global__ void __launch_bounds__(256) join_loss_kernel(const Args a, const Scra
         const float rest = logf(sum);
         const long long t = s.token[r];
         a.lse[t] = m + rest;
-        a.loss[t] = (m - s.top[r]) + rest;  // (the difference of like logits first: it is exact)
+        a.loss[t] = (m - s.top[r]) + rest;  // (the difference of like logits first: it is exact; neither is below zero, as the maximum's exponential is 1)
     }
 }
 // dh from its shares, in order: 1024 columns of a row a block.
