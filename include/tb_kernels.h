@@ -434,6 +434,7 @@ int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
  * same h, w and targets:
  *     g_tv = cap'(h_t . w_v) ((dloss_t + dlse_t) exp(z_tv - lse_t) - dloss_t [v = target[t]])
  *     dh_t = sum_v g_tv w_v,   dw_v = sum_t g_tv h_t.
+ * with logits summed as the forward's are (which depends on n, not on the tokens).
  * The vocabulary is gone through in pieces whose g enters both products as BF16
  * (2^-8 of each value).  dh and dw overwrite what is there; each sum has a fixed
  * order.  dh may be h's own memory, with its stride.  n = 0 gives a dw of zeros.

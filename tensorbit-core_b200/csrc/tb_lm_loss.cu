@@ -54,7 +54,7 @@ struct Args {
 // 1/1536 each: 2-norm of dW's error 2.6e-3 without a unit, 1.9e-3 with it, 1.7e-3 of
 // that the rounding of dW itself.)
 struct __align__(16) Row {
-    float lse2;   // lse in powers of two
+    float lse;
     float both;   // dloss + dlse
     float dloss;
     int target;   // -1 behind the last token
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
                 s.token[to] = t;
                 Row r{0.0f, 0.0f, 0.0f, static_cast<int>(a.target[t])};
                 if (BACKWARD) {
-                    r.lse2 = a.lse[t] * kLog2e;
+                    r.lse = a.lse[t];
                     const float dl = a.dloss[t];
                     r.dloss = dl == unit ? 1.0f : dl * inverse;
                     r.both = a.dlse ? fmaf(a.dlse[t], inverse, r.dloss) : r.dloss;
@@ -317,12 +317,14 @@ struct Logits {
     }
 };
 
-// The same product, turned into G, in sums of 8192 terms (up to 4e-5 of a logit where all terms have one sign: G is
-// rounded to 2^-8).  G enters its products as BF16, as every operand does: an error of
+// The same product in the same sums, so that its logits are the forward's to the last bit, turned into G.  What the tensor
+// core cuts off has one sign where the terms have: logits that are low beside lse make every p low, and p - 1 of a
+// token that is nearly certain a multiple of what it is.  (8192 terms of one sign in one sum, a logit of 60: p low by 6e-4,
+// where p - 1 may be 1e-4.)  G enters its products as BF16, as every operand does: an error of
 // 2^-8 of each of its values at most, which are summed with signs that do not depend on the errors'.
 struct Gradient {
     static constexpr bool kAMn = false, kBMn = false, kF16 = false;
-    static constexpr int kParts = 1, kGroup = 128;
+    static constexpr int kParts = 1, kGroup = Logits::kGroup;
     using Params = loss::Params;
     static __device__ __forceinline__ int* error() { return &g_loss_error; }
     static __device__ __forceinline__ int items(const Params& p) { return kept_tiles(p) * p.tiles_n; }
@@ -338,18 +340,23 @@ struct Gradient {
 #pragma unroll
             for (int c = 0; c < 128; c += 32) {
                 tanh_of<32>(acc + c, inverse);
+                float e[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) e[i] = p.cap * acc[c + i];
+                exp_below(e, r.lse);
 #pragma unroll
                 for (int i = c; i < c + 32; ++i) {
                     const float t = acc[i];
-                    float g = r.both * exp2f(fmaf(p.cap * t, kLog2e, -r.lse2));
+                    float g = r.both * e[i - c];
                     if (hit && i == at) g -= r.dloss;
                     acc[i] = g * fmaf(-t, t, 1.0f);
                 }
             }
         } else {
+            exp_below(acc, r.lse);
 #pragma unroll
             for (int i = 0; i < 128; ++i) {
-                const float g = r.both * exp2f(fmaf(acc[i], kLog2e, -r.lse2));
+                const float g = r.both * acc[i];
                 acc[i] = hit && i == at ? g - r.dloss : g;
             }
         }
@@ -521,7 +528,9 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
 // Up to 128 tokens leave the logits bound by the reading of w.  Tokens are the N of the
 // product here and the vocabulary is M: a CTA takes `tile` rows of w (up to 256, two MMAs of 128), a
 // share that is even over all SMs, and streams them past the tokens' slices; a thread has one entry of the
-// vocabulary and all tokens.  Sums of 64 terms in the tensor core, which costs nothing here.
+// vocabulary and all tokens.  Sums of 64 terms in the tensor core, which costs nothing here, added in one order in both
+// directions: p is of the difference of the backward's logits and the forward's lse.  (The backward from the last features on, which
+// L2 still has, is 3 % sooner for 37 tokens, 4096 x 32000, with gradients, but adds in another order: 3e-5 of a logit of 60.)
 // (32000 x 4096, whole calls: 52 us for 1 token, 56 for 37, 68 for 128, by tiles of 256 tokens 70; w at the measured
 // copy rate 41.  128000 x 4096, 8 tokens: 167, at that rate 162.)
 constexpr int kFewMost = 128;
@@ -537,7 +546,6 @@ struct FewCfg {
 };
 struct FewParams {
     int tile, tiles, vocab, d;
-    int back;          // features from the last to the first
     int n;             // forward: tokens as they are
     const int* count;  // backward: those kept
     const int64_t* target;
@@ -669,7 +677,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                         slope = fmaf(-x, x, 1.0f);
                         x *= p.cap;
                     }
-                    float g = r.both * exp2f(fmaf(x, kLog2e, -r.lse2));
+                    float g = r.both * exp2f((x - r.lse) * kLog2e);
                     if (r.target == entry) g -= r.dloss;
                     // (a token behind the last kept one, of which z is what w times zeros gives, counts as zero)
                     if (inside) p.g[i * p.ldg + entry] = __float2bfloat16_rn(i < kept ? g * slope : 0.0f);
@@ -729,9 +737,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                     if (!wait(smem_u32(&empty[at.s]), at.phase ^ 1, abort_flag)) { ok = false; break; }  // (the first round passes at once)
                     const uint32_t stage = smem_u32(smem + at.s * C::kStage), bar = smem_u32(&ready[at.s]);
                     mbar_expect_tx(bar, static_cast<uint32_t>(p.tile) * 128 + NT * 128);
-                    const int x = 64 * (p.back ? slices - 1 - i : i);
-                    tma_load_2d(stage, &maps.w, x, tile * p.tile, bar);
-                    tma_load_2d(stage + 32768, &maps.h, x, 0, bar);
+                    tma_load_2d(stage, &maps.w, 64 * i, tile * p.tile, bar);
+                    tma_load_2d(stage + 32768, &maps.h, 64 * i, 0, bar);
                 }
             }
             if (!ok) {
@@ -932,7 +939,6 @@ int dh_splits(long long tiles, long long slices) {
     }
     return splits;
 }
-constexpr long long kBack = 512ll << 20;  // bytes of w
 constexpr long long kPieceG = 128ll << 20;  // bytes of G in one piece of the vocabulary
 
 int backward(const Args& a, cudaStream_t st) {
@@ -978,9 +984,6 @@ int backward(const Args& a, cudaStream_t st) {
             q.row = s.row;
             q.g = s.g;
             q.ldg = piece;
-            // The forward, which came before, has left w's last features in L2.  (37 tokens with gradients, 32000 x 4096: 229 us
-            // in the forward's order, 222 backwards; 16 tokens, 128000 x 4096, of which little is left: 700 and 720.)
-            q.back = 2ll * a.vocab * a.d <= kBack;
             rc = few_logits<true>(a, s.h, s.ld, q, st);
         } else {
             pair::Launch<Gradient> L{};

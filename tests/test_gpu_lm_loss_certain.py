@@ -9,13 +9,16 @@ pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
 
-def call(h, w, target, cap=0.0):
+def call(h, w, target, cap=0.0, dloss=None, dh=None, dw=None):
     n, d = h.shape
     loss, lse = torch.full((n,), 7.0, device="cuda"), torch.full((n,), 7.0, device="cuda")
     args = tb.lm_loss_args(n=n, d=d, vocab=w.shape[0], h=h.data_ptr(), ldh=h.stride(0), w=w.data_ptr(), ldw=w.stride(0), target=target.data_ptr(),
                            softcap=cap, loss=loss.data_ptr(), lse=lse.data_ptr())
     stream = torch.cuda.current_stream().cuda_stream
     tb.check(tb.lm_loss(args, stream=stream))
+    if dloss is not None:
+        args.dloss, args.dh, args.lddh, args.dw, args.lddw = dloss.data_ptr(), dh.data_ptr(), dh.stride(0), dw.data_ptr(), dw.stride(0)
+        tb.check(tb.lm_loss_backward(args, stream=stream))
     tb.check(tb.call("tb_gemm_status", stream))
     return loss, lse
 
@@ -54,3 +57,43 @@ def test_nearly_certain_tokens(cuda, n, lo, hi):
     # logits and gap are exact (sums of 20 bits at most); two exponentials of two units of 2^-23 each, products with log2(e) and a few sums
     off = 2.0 ** -21 * (1 + want)
     assert (loss >= 0).all() and ((loss.double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("n", [100, 700])
+@pytest.mark.parametrize("cap", [0.0, 4000.0])
+@pytest.mark.parametrize("size", [60, 1000])
+def test_gradients_of_nearly_certain_tokens(cuda, n, cap, size):
+    """8192 terms of one sign, which the tensor core's additions cut off: p - 1 of a target with p near 1 is a small difference."""
+    d, vocab, at, other = 8192, 300, 20, 290
+    g = torch.Generator(device="cuda").manual_seed(0)
+    h = (0.5 + torch.rand(n, d, device="cuda", generator=g)).to(BF)
+    w = torch.zeros(vocab, d, device="cuda", dtype=BF)
+    w[at] = ((0.5 + torch.rand(d, device="cuda", generator=g)) * size / d).to(BF)
+    w[other] = (w[at].float() * (1 - 9.2 / size)).to(BF)
+    target = torch.full((n,), at, device="cuda")
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    call(h, w, target, cap, torch.ones(n, device="cuda"), dh, dw)
+    hd, wd = h.double(), w.double()
+    raw = hd @ wd.t()
+    z = cap * torch.tanh(raw / cap) if cap else raw
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    slope = 1 - (z / cap) ** 2 if cap else torch.ones_like(z)
+    one = p.clone()
+    one[:, at] -= 1.0
+    assert (one[:, at] > -1e-3).all() and (one[:, at] < -1e-5).all()
+    # Forward and backward cut the same sums off (of 1024 terms at most, up to 66 steps of 2^-23, and nine additions), and two logits'
+    # difference moves p by p (1 - p) of it; tanh and the cap round z twice more, by a few 2^-24.  lse is held to half of its last place;
+    # the argument's product with log2(e) and the exponential are off by a few 2^-23.
+    moved = 2 * raw.amax(1, keepdim=True) * (66 * 2.0 ** -23 + 9 * 2.0 ** -24) + (4 * 2.0 ** -22 * z.abs().amax(1, keepdim=True) if cap else 0.0)
+    p_off = p * ((1 - p) * moved + lse.abs() * 2.0 ** -24 + 2.0 ** -20)
+    if cap:  # (the forward's and the backward's z are the same values here too: only the difference to the definition's)
+        p_off = p_off + p * (1 - p) * moved
+    off = slope * p_off + one.abs() * slope * (2.0 ** -8 + 2.0 ** -20) + one.abs() * 2.0 ** -21
+    grad = one * slope
+    dh_want, dw_want = grad @ wd, grad.t() @ hd
+    dh_off = off @ wd.abs() * 1.01 + grad.abs() @ wd.abs() * (vocab / 16 + 8) * 2.0 ** -23 + dh_want.abs() * 2.0 ** -8 * 1.01
+    dw_off = off.t() @ hd.abs() * 1.01 + grad.abs().t() @ hd.abs() * (n / 16 + 8) * 2.0 ** -23 + dw_want.abs() * 2.0 ** -8 * 1.01
+    for got, want, bound, name in ((dh, dh_want, dh_off, "dh"), (dw, dw_want, dw_off, "dw")):
+        err = (got.double() - want).abs()
+        assert (err <= bound + 2.0 ** -133).all(), f"{name}: worst {float((err / (bound + 2.0 ** -133)).max()):.3g} of its bound"
