@@ -546,6 +546,7 @@ struct FewCfg {
 };
 struct FewParams {
     int tile, tiles, vocab, d;
+    int col0;          // first entry of the vocabulary; `vocab` counts from it
     int n;             // forward: tokens as they are
     const int* count;  // backward: those kept
     const int64_t* target;
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             if (t < *p.count) r = p.row[t];
         } else if (t < p.n) {
             const int64_t y = p.target[t];
-            if (y >= 0 && y < p.vocab) r.target = static_cast<int>(y);
+            if (y >= 0 && y < p.vocab) r.target = static_cast<int>(y);  // (all of the vocabulary, from 0)
         }
         rows[t] = r;
     }
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                         x *= p.cap;
                     }
                     float g = r.both * exp2f((x - r.lse) * kLog2e);
-                    if (r.target == entry) g -= r.dloss;
+                    if (r.target - p.col0 == entry) g -= r.dloss;
                     // (a token behind the last kept one, of which z is what w times zeros gives, counts as zero)
                     if (inside) p.g[i * p.ldg + entry] = __float2bfloat16_rn(i < kept ? g * slope : 0.0f);
                 }
@@ -852,10 +853,10 @@ int launch_few(const FewMaps& maps, const FewParams& p, cudaStream_t st) {
 }
 // The shares of the vocabulary: as few passes of up to 256 entries as 148 CTAs need, each as even as eights allow.
 template <bool GRAD>
-int few_logits(const Args& a, const bf16* h, long long ldh, FewParams& p, cudaStream_t st) {
+int few_logits(const Args& a, const bf16* h, long long ldh, const bf16* w, FewParams& p, cudaStream_t st) {
     const int nt = few_tokens(a.n);
     FewMaps maps{};
-    int rc = make_map(&maps.w, a.w, 2, a.d, a.vocab, a.ldw, 64, p.tile, true);
+    int rc = make_map(&maps.w, w, 2, a.d, p.vocab, a.ldw, 64, p.tile, true);
     if (!rc) rc = make_map(&maps.h, h, 2, a.d, a.n, ldh, 64, nt, true);
     if (rc) return rc;
     switch (nt) {
@@ -867,12 +868,13 @@ int few_logits(const Args& a, const bf16* h, long long ldh, FewParams& p, cudaSt
         default: return launch_few<128, GRAD>(maps, p, st);
     }
 }
-FewParams few_params(const Args& a) {
+FewParams few_params(const Args& a, int col0, int cols) {
     FewParams p{};
-    const long long passes = (a.vocab + 148 * 256ll - 1) / (148 * 256ll), share = (a.vocab + 148 * passes - 1) / (148 * passes);
+    const long long passes = (cols + 148 * 256ll - 1) / (148 * 256ll), share = (cols + 148 * passes - 1) / (148 * passes);
     p.tile = static_cast<int>((share + 7) / 8 * 8);
-    p.tiles = static_cast<int>((a.vocab + static_cast<long long>(p.tile) - 1) / p.tile);
-    p.vocab = a.vocab;
+    p.tiles = static_cast<int>((cols + static_cast<long long>(p.tile) - 1) / p.tile);
+    p.vocab = cols;
+    p.col0 = col0;
     p.d = a.d;
     p.n = static_cast<int>(a.n);
     p.target = a.target;
@@ -880,7 +882,7 @@ FewParams few_params(const Args& a) {
     return p;
 }
 int forward_few(const Args& a, cudaStream_t st) {
-    FewParams p = few_params(a);
+    FewParams p = few_params(a, 0, a.vocab);
     const int nt = few_tokens(a.n);
     void* base = nullptr;
     int rc = scratch_alloc(&base, 512 + sizeof(float2) * nt * static_cast<size_t>(p.tiles), st);
@@ -888,7 +890,7 @@ int forward_few(const Args& a, cudaStream_t st) {
     p.top = static_cast<float*>(base);
     p.stats = reinterpret_cast<float2*>(static_cast<char*>(base) + 512);
     pdl_fence(st);  // the caller may have queued a cross-stream wait
-    rc = few_logits<false>(a, a.h, a.ldh, p, st);
+    rc = few_logits<false>(a, a.h, a.ldh, a.w, p, st);
     if (!rc) {
         const cudaError_t e = launch_pdl(join_few_kernel, dim3(static_cast<unsigned>(a.n)), dim3(256), 0, st, a, p.top, p.stats, p.tiles, nt);
         rc = e == cudaSuccess ? check_launch("join_few_kernel") : cuda_fail(e, "join_few_kernel launch");
@@ -946,7 +948,7 @@ int backward(const Args& a, cudaStream_t st) {
     const long long rows = up(a.n, 256);
     const bool few = a.n <= kFewMost;
     const long long g_rows = few ? few_tokens(a.n) : rows;
-    const long long piece = few ? up(a.vocab, 8) : std::min(up(a.vocab, 256), std::max(256ll, kPieceG / (2 * rows) / 256 * 256));
+    const long long piece = std::min(up(a.vocab, few ? 8 : 256), std::max(256ll, kPieceG / (2 * g_rows) / 256 * 256));
     if (tiles_m * (piece / 256) > 0x3FFFFFFFll || tiles_m * static_cast<long long>(tiles_d) * kPairs > 0x3FFFFFFFll || piece / 256 * tiles_d > 0x3FFFFFFFll)
         return fail(TB_ERR_CAPACITY, "tb_lm_loss_backward: %lld tokens of %d", a.n, a.d);
     // dh's tiles share out their K where they do not fill the GPU
@@ -979,12 +981,12 @@ int backward(const Args& a, cudaStream_t st) {
         p.rows = rows;
         p.row = s.row;
         if (few) {
-            FewParams q = few_params(a);
+            FewParams q = few_params(a, static_cast<int>(v0), cols);
             q.count = s.count;
             q.row = s.row;
             q.g = s.g;
             q.ldg = piece;
-            rc = few_logits<true>(a, s.h, s.ld, q, st);
+            rc = few_logits<true>(a, s.h, s.ld, w, q, st);
         } else {
             pair::Launch<Gradient> L{};
             L.p = p;
