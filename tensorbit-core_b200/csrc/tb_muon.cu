@@ -1164,11 +1164,12 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
     const size_t x_bytes = up(2ll * s.r * ldx, 256), k_bytes = up(2ll * k * ldk, 256);
     const int segments = (steps + kSegment - 1) / kSegment;
     void* base = nullptr;
-    int rc = scratch_alloc(&base, 8 * kNormBlocks + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
+    const size_t partial_bytes = up(sizeof(double) * kNormBlocks, 256);
+    int rc = scratch_alloc(&base, partial_bytes + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
     if (rc) return rc;
     char* at = static_cast<char*>(base);
     double* partial = reinterpret_cast<double*>(at);
-    at += up(8 * kNormBlocks, 256);
+    at += partial_bytes;
     auto matrix = [&](long long rows, long long cols, long long ld, size_t bytes, int exp) {
         Matrix x{{reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + bytes)}, rows, cols, ld, exp};
         at += 2 * bytes;
