@@ -452,7 +452,8 @@ int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
  * reference counterpart.  x is [r][ldx] of TB_F32 or TB_BF16, out [r][ldo] of
  * TB_BF16, any strides; the shorter side ends at 32768.  Products keep 22 bits (two
  * FP16 parts of each operand, FP32 sums): the result is within 5e-4 (2-norm) of the
- * formula's, before it is rounded to BF16.  A zero matrix gives zeros; a NaN or an
+ * formula's, before it is rounded to BF16, whether |U| is above eps or far below it
+ * (down to 2^-70 of it; what is smaller tends to zeros).  A zero matrix gives zeros; a NaN or an
  * infinity makes all of out NaN.
  * Scratch from the library's per-device pool: 8 bytes per value of x (4 up to three
  * steps) and 24 for each of min(r, d)^2. */

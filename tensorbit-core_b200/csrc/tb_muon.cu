@@ -20,6 +20,8 @@
 // each matrix has for good: 22 bits, as FP32 has 24, at the tensor core's FP16 rate; a
 // single FP16 (BF16) part would put 2e-3 (2e-2) of A's error into the directions
 // above.  Entries: |X|, |A|, |P A| <= 1.5, |P| <= 3.5, |Q| <= 3.5^3, which FP16's 65504 bounds.
+// Where |U| is far below eps, so is |X| below 1, and FP16 ends at 2^-24: X then has another power of two 2^s beside its
+// own, which brings |X| to one, less 2^6 with each forming of X anew, in which three steps make it 3.5^3 times larger at most.
 #include <algorithm>
 #include <cuda_fp16.h>
 
@@ -39,6 +41,13 @@ __device__ int g_muon_error;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int kExpX = 14, kExpK = 13, kExpQ = 10;  // the powers of two of X; of A, P and P A; of Q
 constexpr int kSegment = 3;                        // steps between two formings of X
+constexpr int kGrowth = 6;                         // 2^6 > 3.5^kSegment
+constexpr int kMostShift = 60;                     // of s: its factors stay in FP32's range
+constexpr int kMostSegments = (32 + kSegment - 1) / kSegment;
+// What a segment's sums are multiplied by on account of s: those of X X^T, those of the next X, those of the result.
+struct Factors {
+    float gram, next, result;
+};
 
 // The FP16 parts hi + lo of two FP32 values: hi parts in one word, lo parts in another.
 __device__ __forceinline__ void split16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -191,15 +200,22 @@ __global__ void __launch_bounds__(256, 4) norm_kernel(const Source s, double* pa
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
-// X's parts, in rows of ld.
+// X's parts, in rows of ld, and the segments' factors.
 __global__ void __launch_bounds__(256, 4) scale_kernel(const Source s, const double* partial, const int parts, const float eps, uint16_t* hi, uint16_t* lo,
-                                                    const long long ld) {
+                                                    const long long ld, Factors* factors, const int segments) {
     __shared__ double shared[8];
     pdl_wait();
     double sum = 0.0;
     for (int i = threadIdx.x; i < parts; i += 256) sum += partial[i];
     sum = block_sum(sum, shared);
-    const double scale = static_cast<double>(1 << kExpX) / (sqrt(sum) + static_cast<double>(eps));
+    const double size = sqrt(sum), below = size + static_cast<double>(eps);
+    const bool some = size > 0.0 && size < INFINITY;
+    const int shift = some ? min(max(-ilogb(size / below) - 1, 0), kMostShift) : 0;
+    if (blockIdx.x == 0 && threadIdx.x < segments) {
+        const int now = max(shift - kGrowth * static_cast<int>(threadIdx.x), 0), then = max(now - kGrowth, 0);
+        factors[threadIdx.x] = Factors{ldexpf(1.0f, -2 * now), ldexpf(1.0f, then - now), ldexpf(1.0f, -now)};
+    }
+    const double scale = ldexp(1.0, kExpX + shift) / below;
     const bool usual = scale > 1e-30 && scale < 1e30;
     const float factor = static_cast<float>(scale);
     for_update<false>(s, [&](long long row, int col, float (&u)[4]) {
@@ -220,6 +236,7 @@ struct Params {
     int tiles_m, tiles_n;
     int products;
     float alpha[2];       // powers of two (times c): of what the sums are multiplied by
+    const float* factor;  // one more factor of them, in device memory, or NULL
     float beta, diagonal; // P: of A and I
     const uint16_t* c[2]; // P: A's parts
     uint16_t* out[2][2];  // [product][part]
@@ -354,9 +371,10 @@ struct Symmetric {
     }
     static __device__ __forceinline__ Work split_work(const Params& p, int item) { return work(p, item); }
     static constexpr bool kMirror = true;
-    // C's parts
+    // C's parts; without C, the factor
     static __device__ __forceinline__ uint4 fetch_quad(const Launch<Symmetric>& L, int row, int col) {
         const Params& p = L.p;
+        if (p.factor) return make_uint4(__float_as_uint(*p.factor), 0, 0, 0);
         if (!p.c[0] || row >= p.m || col >= p.n) return make_uint4(0, 0, 0, 0);
         const long long at = row * p.ld + col;  // (rows of ld, a multiple of 8)
         const uint2 h = *reinterpret_cast<const uint2*>(p.c[0] + at), l = *reinterpret_cast<const uint2*>(p.c[1] + at);
@@ -364,7 +382,7 @@ struct Symmetric {
     }
     static __device__ __forceinline__ void finish_quad(const Launch<Symmetric>& L, const Work& w, int row, int col, const float4& v, const uint4& c, uint4& words) {
         const Params& p = L.p;
-        const float alpha = p.alpha[w.which];
+        const float alpha = p.alpha[w.which] * (p.factor ? __uint_as_float(c.x) : 1.0f);
         const bool inside = row < p.m && col < p.n;
         const long long at = row * p.ld + col;  // (rows of ld, a multiple of 8)
         float x[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
@@ -409,7 +427,7 @@ struct Symmetric {
         const Params& p = L.p;
         const int row0 = w.tm * 256 + row_in, row = row0 + lane, col = w.tn * 256 + half * 128;
         if (col / 128 > row0 / 128 || row0 >= p.m || col >= p.n) return;
-        const float alpha = p.alpha[w.which];
+        const float alpha = p.alpha[w.which] * (p.factor ? *p.factor : 1.0f);
         const bool mirrored = col / 128 != row0 / 128, odd = lane & 1;
         // selectors of the halves that a lane sends to its neighbour, and of what it makes of those that it gets
         const uint32_t send = odd ? 0x5410u : 0x7632u, take_hi = odd ? 0x3254u : 0x5410u, take_lo = odd ? 0x3276u : 0x7610u;
@@ -496,7 +514,7 @@ struct Apply {
         const int row0 = w.tm * 256 + row_in, col = w.tn * 256 + half * 128;
         const int rows = min(32, p.m - row0), cols = p.n - col;
         if (rows <= 0 || cols <= 0) return;
-        const float alpha = p.alpha[0];
+        const float alpha = p.alpha[0] * *p.factor;
         if constexpr (OUT == kSplit) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -546,11 +564,11 @@ struct Apply {
         return Work{tile / tiles, tile % tiles, 0, (p.k + 63) / 64, 0, -1};
     }
     static constexpr bool kMirror = false;
-    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Apply>&, int, int) { return make_uint4(0, 0, 0, 0); }
-    static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, const uint4&, uint4&) {
+    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Apply>& L, int, int) { return make_uint4(__float_as_uint(*L.p.factor), 0, 0, 0); }
+    static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, const uint4& c, uint4&) {
         const Params& p = L.p;
         if (row >= p.m || col >= p.n) return;
-        const float factor = OUT == kWeights ? p.alpha[0] * p.step : p.alpha[0];
+        const float alpha = p.alpha[0] * __uint_as_float(c.x), factor = OUT == kWeights ? alpha * p.step : alpha;
         const float x[4] = {v.x * factor, v.y * factor, v.z * factor, v.w * factor};
         if constexpr (OUT == kSplit) {
             uint2 hi, lo;
@@ -596,6 +614,7 @@ struct ShortParams {
     int k, r, d, tall, chunks;
     int steps, segments;
     int core;
+    const Factors* factors;  // each segment's
     uint16_t* x[2];    // X's parts, written anew between segments; or Q's
     long long ld;
     void* result;
@@ -760,6 +779,8 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
     constexpr float kDown = 1.0f / (1 << kExpK);  // A, P and P A all have this power of two
     constexpr float kGram = 1.0f / (1 << (2 * kExpX - kExpK));
     for (int seg = 0; seg < p.segments; ++seg) {
+        const Factors factors = p.core ? Factors{1.0f, 1.0f, 1.0f} : p.factors[seg];
+        const float gram = kGram * factors.gram;
         // ---- A into buffer 0 ----
         if (p.core) {
             if (issuer) {
@@ -807,7 +828,7 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
             }
             if (ctas == 1) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) f[i] *= kGram;
+                for (int i = 0; i < 32; ++i) f[i] *= gram;
                 split_sums();
                 put(0);
             }
@@ -829,8 +850,8 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
                     for (int q = 1; q < kSplitMost; ++q)
                         if (q < ctas) { v[0].x += v[q].x; v[0].y += v[q].y; v[0].z += v[q].z; v[0].w += v[q].w; }
                     uint2 h, l;
-                    split16x2(v[0].x * kGram, v[0].y * kGram, h.x, l.x);
-                    split16x2(v[0].z * kGram, v[0].w * kGram, h.y, l.y);
+                    split16x2(v[0].x * gram, v[0].y * gram, h.x, l.x);
+                    split16x2(v[0].z * gram, v[0].w * gram, h.y, l.y);
                     *reinterpret_cast<uint2*>(smem + operand_at(r, c, 0) + (c & 4) * 2) = h;
                     *reinterpret_cast<uint2*>(smem + operand_at(r, c, 1) + (c & 4) * 2) = l;
                 }
@@ -899,7 +920,7 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
         // ---- this CTA's part of Q X (tall: X Q) ----
         const int exp_q = steps > 1 ? kExpQ : kExpK;
         const bool end = seg == p.segments - 1;
-        const float alpha = 1.0f / static_cast<float>(1 << (end ? exp_q + kExpX - 13 : exp_q)) * (end ? 1.0f / 8192 : 1.0f);
+        const float alpha = 1.0f / static_cast<float>(1 << (end ? exp_q + kExpX - 13 : exp_q)) * (end ? factors.result / 8192 : factors.next);
         auto multiply = [&](int i) {
             const int b = i & 1;
             if (!chunk_ready(b)) return;
@@ -1011,10 +1032,10 @@ int out_maps(CUtensorMap (&maps)[2], const Matrix& x) {
 }
 
 // out = scale A B^T (MN: scale A^T B), a symmetric matrix; plus beta C + diagonal I where C is given.
-// With a second B and out, two products with the same A.
+// With a second B and out, two products with the same A; with a factor (in device memory), that too.
 template <bool MN>
 int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, const Matrix* c, float beta, float diagonal, const Matrix* b2, const Matrix* out2,
-              cudaStream_t st) {
+              cudaStream_t st, const float* factor = nullptr) {
     Launch<Symmetric<MN>> L{};
     Params& p = L.p;
     p.m = p.n = static_cast<int>(out.rows);
@@ -1028,6 +1049,7 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
     if (!rc && b2) rc = operand_maps(L.b[1], *b2, MN);
     if (!rc && b2) rc = out_maps(L.o[1], *out2);
     if (rc) return rc;
+    p.factor = factor;
     p.alpha[0] = scale * power(out.exp - a.exp - b.exp);
     if (b2) p.alpha[1] = scale * power(out2->exp - a.exp - b2->exp);
     for (int q = 0; q < 2; ++q) {
@@ -1052,7 +1074,7 @@ struct Result {
 };
 // X (Q X, tall: X Q) into `out`, or into the result.
 template <bool BMN, int OUT>
-int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
+int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, const Factors* factors, cudaStream_t st) {
     pair::Launch<Apply<BMN, OUT>> L{};
     Params& p = L.p;
     p.m = static_cast<int>(x.rows);
@@ -1064,6 +1086,7 @@ int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res
     if (!rc) rc = operand_maps(L.b[0], BMN ? x : q, BMN);
     if (!rc && OUT == kSplit) rc = out_maps(L.o[0], out);
     if (rc) return rc;
+    p.factor = OUT == kSplit ? &factors->next : &factors->result;
     p.alpha[0] = power((OUT == kSplit ? out.exp : 0) - q.exp - x.exp);
     p.result = res.out;
     p.ldr = res.ld;
@@ -1079,8 +1102,8 @@ int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res
     return launch_either(L, units, pairs, (p.k + 63) / 64, st);
 }
 template <int OUT>
-int apply(bool tall, const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, cudaStream_t st) {
-    return tall ? apply<false, OUT>(q, x, out, res, st) : apply<true, OUT>(q, x, out, res, st);
+int apply(bool tall, const Matrix& q, const Matrix& x, const Matrix& out, const Result& res, const Factors* factors, cudaStream_t st) {
+    return tall ? apply<false, OUT>(q, x, out, res, factors, st) : apply<true, OUT>(q, x, out, res, factors, st);
 }
 
 template <int OUT>
@@ -1132,7 +1155,7 @@ int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
 }
 // All of it.
 template <int OUT>
-int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res, cudaStream_t st) {
+int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res, const Factors* factors, cudaStream_t st) {
     ShortMaps maps{};
     const int rc = operand_maps(maps.x, x, false);
     if (rc) return rc;
@@ -1144,6 +1167,7 @@ int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res
     p.chunks = tiles(std::max(p.r, p.d), 128);
     p.steps = steps;
     p.segments = segments;
+    p.factors = factors;
     p.x[0] = x.part[0];
     p.x[1] = x.part[1];
     p.ld = x.ld;
@@ -1164,12 +1188,14 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
     const size_t x_bytes = up(2ll * s.r * ldx, 256), k_bytes = up(2ll * k * ldk, 256);
     const int segments = (steps + kSegment - 1) / kSegment;
     void* base = nullptr;
-    const size_t partial_bytes = up(sizeof(double) * kNormBlocks, 256);
-    int rc = scratch_alloc(&base, partial_bytes + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
+    const size_t partial_bytes = up(sizeof(double) * kNormBlocks, 256), factor_bytes = up(sizeof(Factors) * kMostSegments, 256);
+    int rc = scratch_alloc(&base, partial_bytes + factor_bytes + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
     if (rc) return rc;
     char* at = static_cast<char*>(base);
     double* partial = reinterpret_cast<double*>(at);
     at += partial_bytes;
+    Factors* factors = reinterpret_cast<Factors*>(at);
+    at += factor_bytes;
     auto matrix = [&](long long rows, long long cols, long long ld, size_t bytes, int exp) {
         Matrix x{{reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + bytes)}, rows, cols, ld, exp};
         at += 2 * bytes;
@@ -1186,18 +1212,19 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
     norm_kernel<<<blocks, 256, 0, st>>>(s, partial);
     rc = check_launch("norm_kernel");
     if (!rc) {
-        const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx);
+        const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx, factors, segments);
         rc = e == cudaSuccess ? check_launch("scale_kernel") : cuda_fail(e, "scale_kernel launch");
     }
     const bool small = k <= 128;
     if (!rc && small && std::max(s.r, s.d) <= 128 * kShortChunks) {
-        rc = whole<OUT>(x, tall, steps, segments, res, st);
+        rc = whole<OUT>(x, tall, steps, segments, res, factors, st);
         scratch_free(base, st);
         return rc;
     }
     for (int seg = 0; seg < segments && !rc; ++seg) {
         const int n = steps * (seg + 1) / segments - steps * seg / segments;
-        rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+        const float* gram = &factors[seg].gram;
+        rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st, gram) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st, gram);
         Matrix q = P[0];
         if (!rc && small) {
             if (n > 1) q = Q[0];
@@ -1215,10 +1242,10 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
         }
         if (rc) break;
         if (seg < segments - 1) {
-            rc = apply<kSplit>(tall, q, x, x2, res, st);
+            rc = apply<kSplit>(tall, q, x, x2, res, factors + seg, st);
             std::swap(x, x2);
         } else {
-            rc = apply<OUT>(tall, q, x, x, res, st);
+            rc = apply<OUT>(tall, q, x, x, res, factors + seg, st);
         }
     }
     scratch_free(base, st);
