@@ -451,10 +451,14 @@ int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
  * which brings U's singular values near 1 and keeps its singular vectors.  No
  * reference counterpart.  x is [r][ldx] of TB_F32 or TB_BF16, out [r][ldo] of
  * TB_BF16, any strides; the shorter side ends at 32768.  Products keep 22 bits (two
- * FP16 parts of each operand, FP32 sums): the result is within 5e-4 (2-norm) of the
- * formula's, before it is rounded to BF16, whether |U| is above eps or far below it
- * (down to 2^-70 of it; what is smaller tends to zeros).  A zero matrix gives zeros; a NaN or an
- * infinity makes all of out NaN.
+ * FP16 parts of each operand, FP32 sums): up to five steps the result is within 5e-4
+ * (2-norm) of the formula's, before it is rounded to BF16, whether |U| is above eps or
+ * far below it (down to 2^-70 of it; what is smaller tends to zeros).  Each further
+ * step can make 3.44 times as much of what rounding leaves in directions that U lacks:
+ * with two directions of 3000 in FP32, 1e-3 at six steps, 2e-3 at seven, 1e-1 at ten, and
+ * all of the result from twelve on (FP32 products lose half as much); with BF16 values,
+ * whose own roundings are such directions, 7e-4 at twelve.  A zero matrix gives zeros; a
+ * NaN or an infinity makes all of out NaN.
  * Scratch from the library's per-device pool: 8 bytes per value of x (4 up to three
  * steps) and 24 for each of min(r, d)^2. */
 int tb_orthogonalize(const void* x, int x_dtype, int64_t ldx, int r, int d, void* out, int out_dtype, int64_t ldo,

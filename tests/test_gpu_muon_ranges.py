@@ -51,3 +51,32 @@ def test_step_far_below_eps(cuda, r, d, far):
     tb.check(tb.muon_step(args, stream=stream()))
     status()
     assert_near(W, want, want.abs() * 2.0 ** -22, PROMISED * want.norm().item(), f"{far:g}")
+
+
+def few_directions(r, d, k, seed=7):
+    """k directions and exact zeros beside them but for FP32's rounding (k = 1: all values of one sign)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    make = (lambda *s: 0.5 + torch.rand(*s, device="cuda", generator=g)) if k == 1 else (lambda *s: torch.randn(*s, device="cuda", generator=g))
+    return make(r, k) @ make(k, d) * 1e-3
+
+
+def allowed(steps):
+    """The polynomial's slope is at most a = 3.4445, so much a further step can make of an error; what it adds itself is far smaller."""
+    return PROMISED * 3.4445 ** max(0, steps - 5)
+
+
+@pytest.mark.parametrize("r,d", [(100, 100), (128, 1000), (64, 2049), (130, 260), (1024, 1024), (300, 4000), (3100, 3000)])
+@pytest.mark.parametrize("k", [1, 2, 8, 48])
+def test_few_directions(cuda, r, d, k):
+    x = few_directions(r, d, k)
+    for steps in (1, 2, 3, 4, 5, 6, 7, 8):
+        want = ortho(x, steps)
+        assert_near(run_ortho(x, steps), want, want.abs() * 2.0 ** -8, allowed(steps) * want.norm().item(), f"{steps} steps")
+
+
+@pytest.mark.parametrize("r,d", [(100, 100), (64, 2049), (130, 260), (300, 200), (1500, 2100), (3300, 3300)])
+@pytest.mark.parametrize("kind", ["noise", "falling", "low"])
+def test_as_promised(cuda, r, d, kind):
+    x = gradient(r, d, kind)
+    want = ortho(x)
+    assert_near(run_ortho(x), want, want.abs() * 2.0 ** -8, PROMISED * want.norm().item(), kind)
