@@ -210,6 +210,8 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
     return v;
 }
+// 1 / c within FP32: a logit of zero stays zero under the smallest cap too.
+__device__ __forceinline__ float inverse_cap(float cap) { return fminf(1.0f / cap, 3.4028235e38f); }
 template <int N>
 __device__ __forceinline__ void tanh_of(float* v, float inverse) {
     float most = 0.0f;
@@ -288,7 +290,7 @@ struct Logits {
         const long long row = w.tm * 256ll + row_in + lane;
         const int col = w.tn * 256 + half * 128, cols = p.cols - col;
         if (p.cap > 0.0f) {
-            const float inverse = 1.0f / p.cap;
+            const float inverse = inverse_cap(p.cap);
 #pragma unroll
             for (int c = 0; c < 128; c += 32) tanh_of<32>(acc + c, inverse);
 #pragma unroll
@@ -336,7 +338,7 @@ struct Gradient {
         const int at = r.target - p.col0 - col;
         const bool hit = at >= 0 && at < 128;
         if (p.cap > 0.0f) {
-            const float inverse = 1.0f / p.cap;
+            const float inverse = inverse_cap(p.cap);
 #pragma unroll
             for (int c = 0; c < 128; c += 32) {
                 tanh_of<32>(acc + c, inverse);
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             const long long entry = static_cast<long long>(tile) * p.tile + in;
             const bool inside = in < p.tile && entry < p.vocab;
             if (p.cap > 0.0f) {
-                const float inverse = 1.0f / p.cap;
+                const float inverse = inverse_cap(p.cap);
 #pragma unroll
                 for (int c = 0; c < NT; c += 16) tanh_of<16>(z + c, inverse);
             }

@@ -97,3 +97,26 @@ def test_gradients_of_nearly_certain_tokens(cuda, n, cap, size):
     for got, want, bound, name in ((dh, dh_want, dh_off, "dh"), (dw, dw_want, dw_off, "dw")):
         err = (got.double() - want).abs()
         assert (err <= bound + 2.0 ** -133).all(), f"{name}: worst {float((err / (bound + 2.0 ** -133)).max()):.3g} of its bound"
+
+
+@pytest.mark.parametrize("n", [5, 300])
+@pytest.mark.parametrize("cap", [1e-40, 2.0 ** -126, 3e38])
+def test_smallest_and_largest_caps(cuda, n, cap):
+    """Tokens of zeros: every logit is zero, its slope one.  (1 / 1e-40 is beyond FP32.)"""
+    d, vocab = 64, 500
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(vocab, d, device="cuda", generator=g).to(BF)
+    h = torch.randn(n, d, device="cuda", generator=g).to(BF)
+    h[::2] = 0
+    target = torch.randint(0, vocab, (n,), device="cuda", generator=g)
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    loss, lse = call(h, w, target, cap, torch.ones(n, device="cuda"), dh, dw)
+    want = torch.log(torch.tensor(float(vocab), device="cuda", dtype=torch.float64))
+    for x in (loss[::2], lse[::2]) if cap > 1 else (loss, lse):  # (capped so low all logits are zeros beside one)
+        assert ((x.double() - want).abs() <= want * 2.0 ** -22).all()
+    one = torch.full((len(target[::2]), vocab), 1.0 / vocab, device="cuda", dtype=torch.float64)
+    one[torch.arange(len(one)), target[::2]] -= 1.0
+    rows, size = one @ w.double(), one.abs() @ w.double().abs()
+    # G's rounding, the result's, and 32 steps of the tensor core's sum
+    assert ((dh[::2].double() - rows).abs() <= size * (2.0 ** -8 + 40 * 2.0 ** -23) + rows.abs() * 2.0 ** -8 * 1.01).all()
+    assert torch.isfinite(dw).all() and torch.isfinite(dh).all()
