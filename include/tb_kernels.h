@@ -212,7 +212,9 @@ int tb_gemm_nt_bf16(const void* a, long long lda, const void* b, long long ldb, 
                     int lower_only, void* stream);
 /* TB_ERR_TIMEOUT if a bounded pipeline wait inside a GEMM, or inside a product
  * of the checkpoint, adapter, loss and update entries below, launched since the
- * last call expired (the kernel then skipped its output); synchronises. */
+ * last call expired; synchronises.  Sums that were not finished are then not
+ * written, and where a call has several kernels, its later ones write no results
+ * (a loss, a gradient or a weight keeps what it held, a step's momentum has moved on). */
 int tb_gemm_status(void* stream);
 
 /* ---- stage 3: column-block exact OBS against calibration activations ----- */

@@ -117,7 +117,7 @@ struct Params {
 constexpr int kPartTile = 256 * 256;
 
 __device__ __forceinline__ void give_up(volatile int* abort_flag) {
-    *abort_flag = 1;
+    abort_pair(abort_flag);
     atomicExch(&g_linear_error, 1);
 }
 // Sets bits of a word of both CTAs, before what this warp tells anyone next.
@@ -474,7 +474,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
     uint64_t* empty = ready + kStages;    // stage read by the MMAs
     uint64_t* accfull = empty + kStages;      // [kAcc] accumulator finished
     uint64_t* accempty = accfull + C::kAcc;   // [kAcc] (even CTA) accumulator taken by both CTAs
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + C::kAcc);
+    uint64_t* drained = accempty + C::kAcc;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* odd_flag = tmem_slot + 2;  // a bit for each adapter whose factor had values that are not finite (set in both CTAs, never reset)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -494,6 +495,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
             mbar_init(smem_u32(&accfull[b]), 1);
             mbar_init(smem_u32(&accempty[b]), 2 * kEpiWarps);
         }
+        mbar_init(smem_u32(drained), 1);
         *abort_flag = 0;
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -839,10 +841,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tA, const __grid_constant__ CU
                     }
                     return true;
                 });
-                if (!done) {
-                    give_up(abort_flag);
-                    for (int b = 0; b < C::kAcc; ++b) commit_pair(smem_u32(&accfull[b]));  // releases the waiting epilogues
-                }
+                if (!done) give_up(abort_flag);
+                if (*abort_flag) drain_pair(smem_u32(drained));
             }
             __syncwarp();
         } else if (C::kCodes) {

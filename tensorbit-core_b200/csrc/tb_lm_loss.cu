@@ -70,6 +70,7 @@ struct Scratch {
     long long rows;   // n in whole tiles
     long long ld;     // of h's copy
     int* count;       // kept tokens
+    int* failed;      // 1 once a wait has expired in one of the call's products
     float* unit;
     Tally* tallies;   // [ceil(n / kScan)], or NULL
     long long* token; // [rows] the kept tokens, in order
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *s.count = all.kept;
         *s.unit = unit;
+        *s.failed = 0;
     }
     const long long t = t0 + (ONE ? 0 : warp);
     const int part = ONE ? threadIdx.x : lane;  // of a row's units
@@ -253,6 +255,7 @@ __device__ __forceinline__ void exp_below(float (&v)[N], float from) {
 struct Params {
     const int* count;
     const float* unit;
+    int* failed;
     int tiles_n;
     int cols;          // columns of the product that exist
     int k;             // K of the product (dW: counted on the device)
@@ -411,6 +414,7 @@ struct WeightGrad {
             return;
         }
         const float unit = *p.unit;
+        if (*p.failed) return;
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] *= unit;
         if (p.out_tma) store_tma<true, 1>(&L.o[0][0], buf, acc, col, row0, 0, p.cols, false, lane);
@@ -422,9 +426,9 @@ struct WeightGrad {
 __global__ void __launch_bounds__(256) join_loss_kernel(const Args a, const Scratch s, const int pieces) {
     __shared__ float2 shared[32][9];
     pdl_wait();
-    const int count = *s.count, tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int count = *s.count, failed = *s.failed, tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
     const long long r = static_cast<long long>(blockIdx.x) * 8 + tx;
-    if (blockIdx.x * 8ll >= count) return;
+    if (blockIdx.x * 8ll >= count || failed) return;
     float m = -INFINITY, sum = 0.0f;
     auto add = [&](float2 x) {
         const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(256) join_dh_kernel(const Args a, const Scratc
     const int chunks = (a.d + 1023) / 1024;
     const long long r = blockIdx.x / chunks;
     const int i = static_cast<int>(blockIdx.x % chunks) * 1024 + 4 * threadIdx.x;
-    if (r >= *s.count || i >= a.d) return;
+    if (r >= *s.count || i >= a.d || *s.failed) return;
     const float unit = *s.unit;
     const float* part = s.part + r * s.ldp + i;
     float4 v = *reinterpret_cast<const float4*>(part);
@@ -474,18 +478,19 @@ __global__ void __launch_bounds__(256) join_dh_kernel(const Args a, const Scratc
 }
 
 // A piece's dW from its shares, in order: 1024 columns of a row a block.
-__global__ void __launch_bounds__(256) join_dw_kernel(const float* part, const long long ldp, const int rows, const int d, const int splits, const float* unit, bf16* out,
+__global__ void __launch_bounds__(256) join_dw_kernel(const float* part, const long long ldp, const int rows, const int d, const int splits, const Scratch s, bf16* out,
                                                       const long long ldo) {
     pdl_wait();
     const int chunks = (d + 1023) / 1024, r = blockIdx.x / chunks, i = static_cast<int>(blockIdx.x % chunks) * 1024 + 4 * threadIdx.x;
-    if (i >= d) return;
+    if (i >= d || *s.failed) return;
+    const float unit = *s.unit;
     float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll 4
     for (int q = 0; q < splits; ++q) {
         const float4 x = *reinterpret_cast<const float4*>(part + (static_cast<long long>(q) * rows + r) * ldp + i);
         v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
-    const float f[4] = {v.x * *unit, v.y * *unit, v.z * *unit, v.w * *unit};
+    const float f[4] = {v.x * unit, v.y * unit, v.z * unit, v.w * unit};
     for (int e = 0; e < 4 && i + e < d; ++e) out[r * ldo + i + e] = __float2bfloat16_rn(f[e]);
 }
 
@@ -506,6 +511,7 @@ int make_scratch(const Args& a, size_t more, Scratch* s, void** base, char** res
     auto take = [&](size_t b) { char* q = p; p += up(b, 256); return q; };
     s->count = reinterpret_cast<int*>(take(sizes[0]));
     s->unit = reinterpret_cast<float*>(s->count + 1);
+    s->failed = s->count + 2;
     s->tallies = sizes[1] ? reinterpret_cast<Tally*>(take(sizes[1])) : nullptr;
     s->token = reinterpret_cast<long long*>(take(sizes[2]));
     s->row = reinterpret_cast<Row*>(take(sizes[3]));
@@ -537,6 +543,7 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
 // copy rate 41.  128000 x 4096, 8 tokens: 167, at that rate 162.)
 constexpr int kFewMost = 128;
 constexpr int kFewThreads = 320;  // warps 0-7 results, 8 loads, 9 MMAs
+constexpr int kFewCtas = 148;     // at most
 constexpr int kFewGroup = 1;
 template <int NT>
 struct FewCfg {
@@ -558,6 +565,7 @@ struct FewParams {
     float2* stats;     // [tiles][NT]
     bf16* g;           // [NT][ldg]
     long long ldg;
+    int* failed;       // forward: a word a CTA; backward: the call's
 };
 struct FewMaps {
     CUtensorMap w, h;
@@ -594,7 +602,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
     uint64_t* empty = ready + kStages;
     uint64_t* accfull = empty + kStages;  // [2]
     uint64_t* accempty = accfull + 2;     // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    uint64_t* drained = accempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr uint32_t kColumns = NT <= 16 ? 64 : NT <= 32 ? 128 : NT <= 64 ? 256 : 512;  // two sums of two halves
@@ -612,6 +621,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             mbar_init(smem_u32(&accfull[b]), 1);
             mbar_init(smem_u32(&accempty[b]), 8);
         }
+        mbar_init(smem_u32(drained), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -778,6 +788,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
                         }
                         mma_commit(smem_u32(&empty[at.s]));
                     }
+                    if (!ok) break;
                     mma_commit(smem_u32(&accfull[ac.s]));
                     ac.next();
                 }
@@ -785,20 +796,25 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             if (!ok) {
                 *abort_flag = 1;
                 atomicExch(&g_loss_error, 1);
-                for (int b = 0; b < 2; ++b) mma_commit(smem_u32(&accfull[b]));  // releases the waiting warps
             }
+            if (*abort_flag) drain_one(smem_u32(drained));
         }
         __syncwarp();
     }
     fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) {
+        if (!GRAD) p.failed[blockIdx.x] = *abort_flag;
+        else if (*abort_flag) atomicExch(p.failed, 1);
+    }
+    __syncwarp();
     if (warp == 0) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns));
     }
 }
 // A token a block: its tiles' maxima and sums.
-__global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float* top, const float2* stats, const int tiles, const int pitch) {
+__global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float* top, const float2* stats, const int tiles, const int pitch, const int* failed) {
     __shared__ float2 shared[8];
     pdl_wait();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -806,6 +822,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float
         if (threadIdx.x == 0) a.loss[t] = a.lse[t] = 0.0f;
         return;
     }
+    const int gone = threadIdx.x < min(tiles, kFewCtas) ? failed[threadIdx.x] : 0;
     float m = -INFINITY, sum = 0.0f;
     auto add = [&](float2 x) {
         const float most = fmaxf(m, x.x), base = most == -INFINITY ? 0.0f : most;
@@ -824,8 +841,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(const Args a, const float
         add(make_float2(m1, s1));
     }
     if (lane == 0) shared[warp] = make_float2(m, sum);
-    __syncthreads();
-    if (threadIdx.x) return;
+    if (__syncthreads_or(gone) || threadIdx.x) return;
     m = shared[0].x;
     sum = shared[0].y;
     for (int q = 1; q < 8; ++q) add(shared[q]);
@@ -850,7 +866,7 @@ int launch_few(const FewMaps& maps, const FewParams& p, cudaStream_t st) {
             if (dev < 64) prepared |= 1ull << dev;
         }
     }
-    const cudaError_t e = launch_pdl(few_logits_kernel<NT, GRAD>, dim3(std::min(p.tiles, 148)), dim3(kFewThreads), FewCfg<NT>::kSmem, st, maps, p);
+    const cudaError_t e = launch_pdl(few_logits_kernel<NT, GRAD>, dim3(std::min(p.tiles, kFewCtas)), dim3(kFewThreads), FewCfg<NT>::kSmem, st, maps, p);
     return e == cudaSuccess ? check_launch("few_logits_kernel") : cuda_fail(e, "few_logits_kernel launch");
 }
 // The shares of the vocabulary: as few passes of up to 256 entries as 148 CTAs need, each as even as eights allow.
@@ -872,7 +888,7 @@ int few_logits(const Args& a, const bf16* h, long long ldh, const bf16* w, FewPa
 }
 FewParams few_params(const Args& a, int col0, int cols) {
     FewParams p{};
-    const long long passes = (cols + 148 * 256ll - 1) / (148 * 256ll), share = (cols + 148 * passes - 1) / (148 * passes);
+    const long long passes = (cols + kFewCtas * 256ll - 1) / (kFewCtas * 256ll), share = (cols + kFewCtas * passes - 1) / (kFewCtas * passes);
     p.tile = static_cast<int>((share + 7) / 8 * 8);
     p.tiles = static_cast<int>((cols + static_cast<long long>(p.tile) - 1) / p.tile);
     p.vocab = cols;
@@ -887,14 +903,17 @@ int forward_few(const Args& a, cudaStream_t st) {
     FewParams p = few_params(a, 0, a.vocab);
     const int nt = few_tokens(a.n);
     void* base = nullptr;
-    int rc = scratch_alloc(&base, 512 + sizeof(float2) * nt * static_cast<size_t>(p.tiles), st);
+    constexpr size_t kTop = sizeof(float) * kFewMost, kFailed = sizeof(int) * 160;
+    static_assert(kFailed >= sizeof(int) * kFewCtas && (kTop + kFailed) % 16 == 0, "a word for each CTA");
+    int rc = scratch_alloc(&base, kTop + kFailed + sizeof(float2) * nt * static_cast<size_t>(p.tiles), st);
     if (rc) return rc;
     p.top = static_cast<float*>(base);
-    p.stats = reinterpret_cast<float2*>(static_cast<char*>(base) + 512);
+    p.failed = reinterpret_cast<int*>(static_cast<char*>(base) + kTop);
+    p.stats = reinterpret_cast<float2*>(static_cast<char*>(base) + kTop + kFailed);
     pdl_fence(st);  // the caller may have queued a cross-stream wait
     rc = few_logits<false>(a, a.h, a.ldh, a.w, p, st);
     if (!rc) {
-        const cudaError_t e = launch_pdl(join_few_kernel, dim3(static_cast<unsigned>(a.n)), dim3(256), 0, st, a, p.top, p.stats, p.tiles, nt);
+        const cudaError_t e = launch_pdl(join_few_kernel, dim3(static_cast<unsigned>(a.n)), dim3(256), 0, st, a, p.top, p.stats, p.tiles, nt, p.failed);
         rc = e == cudaSuccess ? check_launch("join_few_kernel") : cuda_fail(e, "join_few_kernel launch");
     }
     scratch_free(base, st);
@@ -916,6 +935,7 @@ int forward(const Args& a, cudaStream_t st) {
     rc = gather<false>(a, s, st);
     pair::Launch<Logits> L{};
     L.p.count = s.count;
+    L.p.failed = s.failed;
     L.p.tiles_n = tiles_n;
     L.p.cols = a.vocab;
     L.p.k = a.d;
@@ -979,12 +999,14 @@ int backward(const Args& a, cudaStream_t st) {
         Params p{};
         p.count = s.count;
         p.unit = s.unit;
+        p.failed = s.failed;
         p.cap = a.cap;
         p.rows = rows;
         p.row = s.row;
         if (few) {
             FewParams q = few_params(a, static_cast<int>(v0), cols);
             q.count = s.count;
+            q.failed = s.failed;
             q.row = s.row;
             q.g = s.g;
             q.ldg = piece;
@@ -1032,7 +1054,7 @@ int backward(const Args& a, cudaStream_t st) {
             else if (!rc && L.p.out_tma) rc = make_out_map(&L.o[0][0], L.p.out, true, a.d, cols, 1, a.lddw, a.lddw * cols);
             if (!rc) rc = launch_product(L, static_cast<long long>(tiles(cols, 256)) * tiles_d * dw_splits, st);
             if (!rc && dw_splits > 1)
-                rc = launch_small("join_dw_kernel", join_dw_kernel, static_cast<long long>(cols) * ((a.d + 1023) / 1024), st, dw_part, ldp, cols, a.d, dw_splits, s.unit, a.dw, a.lddw);
+                rc = launch_small("join_dw_kernel", join_dw_kernel, static_cast<long long>(cols) * ((a.d + 1023) / 1024), st, dw_part, ldp, cols, a.d, dw_splits, s, a.dw, a.lddw);
         }
     }
     if (!rc && a.dh) rc = launch_small("join_dh_kernel", join_dh_kernel, a.n * ((a.d + 1023) / 1024), st, a, s, splits);

@@ -200,9 +200,9 @@ __global__ void __launch_bounds__(256, 4) norm_kernel(const Source s, double* pa
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
-// X's parts, in rows of ld, and the segments' factors.
+// X's parts, in rows of ld, and the segments' factors; `failed` is reset.
 __global__ void __launch_bounds__(256, 4) scale_kernel(const Source s, const double* partial, const int parts, const float eps, uint16_t* hi, uint16_t* lo,
-                                                    const long long ld, Factors* factors, const int segments) {
+                                                    const long long ld, Factors* factors, int* failed, const int segments) {
     __shared__ double shared[8];
     pdl_wait();
     double sum = 0.0;
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(256, 4) scale_kernel(const Source s, const dou
     const double size = sqrt(sum), below = size + static_cast<double>(eps);
     const bool some = size > 0.0 && size < INFINITY;
     const int shift = some ? min(max(-ilogb(size / below) - 1, 0), kMostShift) : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *failed = 0;
     if (blockIdx.x == 0 && threadIdx.x < segments) {
         const int now = max(shift - kGrowth * static_cast<int>(threadIdx.x), 0), then = max(now - kGrowth, 0);
         factors[threadIdx.x] = Factors{ldexpf(1.0f, -2 * now), ldexpf(1.0f, then - now), ldexpf(1.0f, -now)};
@@ -241,6 +242,7 @@ struct Params {
     const uint16_t* c[2]; // P: A's parts
     uint16_t* out[2][2];  // [product][part]
     long long ld;         // of c and out
+    int* failed;          // 1 once a wait has expired in one of the call's kernels: no results then
     // results
     void* result;
     long long ldr;
@@ -515,6 +517,7 @@ struct Apply {
         const int rows = min(32, p.m - row0), cols = p.n - col;
         if (rows <= 0 || cols <= 0) return;
         const float alpha = p.alpha[0] * *p.factor;
+        if (OUT != kSplit && *p.failed) return;
         if constexpr (OUT == kSplit) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -564,10 +567,12 @@ struct Apply {
         return Work{tile / tiles, tile % tiles, 0, (p.k + 63) / 64, 0, -1};
     }
     static constexpr bool kMirror = false;
-    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Apply>& L, int, int) { return make_uint4(__float_as_uint(*L.p.factor), 0, 0, 0); }
+    static __device__ __forceinline__ uint4 fetch_quad(const Launch<Apply>& L, int, int) {
+        return make_uint4(__float_as_uint(*L.p.factor), OUT != kSplit ? static_cast<uint32_t>(*L.p.failed) : 0u, 0, 0);
+    }
     static __device__ __forceinline__ void finish_quad(const Launch<Apply>& L, const Work&, int row, int col, const float4& v, const uint4& c, uint4&) {
         const Params& p = L.p;
-        if (row >= p.m || col >= p.n) return;
+        if (row >= p.m || col >= p.n || c.y) return;
         const float alpha = p.alpha[0] * __uint_as_float(c.x), factor = OUT == kWeights ? alpha * p.step : alpha;
         const float x[4] = {v.x * factor, v.y * factor, v.z * factor, v.w * factor};
         if constexpr (OUT == kSplit) {
@@ -615,6 +620,7 @@ struct ShortParams {
     int steps, segments;
     int core;
     const Factors* factors;  // each segment's
+    int* failed;
     uint16_t* x[2];    // X's parts, written anew between segments; or Q's
     long long ld;
     void* result;
@@ -645,7 +651,8 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
     uint64_t* used = loaded + 2;                                            // [2] and read
     uint64_t* done = used + 2;                                              // [2] an accumulator finished
     uint64_t* taken = done + 2;                                             // [2] and read (products with X)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
+    uint64_t* drained = taken + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
@@ -660,6 +667,7 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
             mbar_init(smem_u32(&done[b]), 1);
             mbar_init(smem_u32(&taken[b]), 16);
         }
+        mbar_init(smem_u32(drained), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -684,9 +692,10 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
     auto tile_desc = [&](uint32_t at, bool mn) {
         return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(mn ? kShortTile >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
     };
-    auto gave_up = [&] {
+    auto gave_up = [&] {  // (what follows goes on, but no result is written)
         *abort_flag = 1;
         atomicExch(&g_muon_error, 1);
+        atomicExch(p.failed, 1);
     };
     // the issuer's counts: loads into each buffer, products with X into each accumulator
     int loads[2] = {0, 0}, products[2] = {0, 0};
@@ -839,6 +848,8 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
                 __syncwarp();
                 cluster_arrive();
                 cluster_wait();
+                // (a CTA that gave up has no sums)
+                if (lane < ctas && lane != rank && load_cluster_int(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(lane))) *abort_flag = 1;
                 const int row0 = 2 * share_at(64, rank, ctas), rows = 2 * share_at(64, rank + 1, ctas) - row0;
                 for (int i = threadIdx.x; i < rows * 32; i += kShortThreads) {
                     const int r = row0 + (i >> 5), c = 4 * (i & 31);
@@ -1004,9 +1015,11 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
         }
         meet(true);
     }
-    if (issuer && *abort_flag)  // loads in flight, within a limit
+    if (issuer && *abort_flag) {  // loads and MMAs in flight, within a limit
         for (int b = 0; b < 2; ++b)
             if (loads[b]) wait(smem_u32(&loaded[b]), (loads[b] - 1) & 1, nullptr);
+        drain_one(smem_u32(drained));
+    }
     meet(false);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
 }
@@ -1035,7 +1048,7 @@ int out_maps(CUtensorMap (&maps)[2], const Matrix& x) {
 // With a second B and out, two products with the same A; with a factor (in device memory), that too.
 template <bool MN>
 int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, const Matrix* c, float beta, float diagonal, const Matrix* b2, const Matrix* out2,
-              cudaStream_t st, const float* factor = nullptr) {
+              int* failed, cudaStream_t st, const float* factor = nullptr) {
     Launch<Symmetric<MN>> L{};
     Params& p = L.p;
     p.m = p.n = static_cast<int>(out.rows);
@@ -1050,6 +1063,7 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
     if (!rc && b2) rc = out_maps(L.o[1], *out2);
     if (rc) return rc;
     p.factor = factor;
+    p.failed = failed;
     p.alpha[0] = scale * power(out.exp - a.exp - b.exp);
     if (b2) p.alpha[1] = scale * power(out2->exp - a.exp - b2->exp);
     for (int q = 0; q < 2; ++q) {
@@ -1066,6 +1080,7 @@ int symmetric(const Matrix& a, const Matrix& b, const Matrix& out, float scale, 
 }
 
 struct Result {
+    int* failed;
     void* out;
     long long ld;
     Mask mask;
@@ -1088,6 +1103,7 @@ int apply(const Matrix& q, const Matrix& x, const Matrix& out, const Result& res
     if (rc) return rc;
     p.factor = OUT == kSplit ? &factors->next : &factors->result;
     p.alpha[0] = power((OUT == kSplit ? out.exp : 0) - q.exp - x.exp);
+    p.failed = res.failed;
     p.result = res.out;
     p.ldr = res.ld;
     p.mask = res.mask;
@@ -1139,7 +1155,7 @@ int launch_short(const ShortMaps& maps, const ShortParams& p, int ctas, cudaStre
     return e == cudaSuccess ? check_launch("short_kernel") : cuda_fail(e, "short_kernel launch");
 }
 // Q of `steps` steps from A, for k up to 128.
-int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
+int core(const Matrix& A, const Matrix& q, int steps, int* failed, cudaStream_t st) {
     ShortMaps maps{};
     const int rc = operand_maps(maps.x, A, false);
     if (rc) return rc;
@@ -1148,6 +1164,7 @@ int core(const Matrix& A, const Matrix& q, int steps, cudaStream_t st) {
     p.steps = steps;
     p.segments = 1;
     p.core = 1;
+    p.failed = failed;
     p.x[0] = q.part[0];
     p.x[1] = q.part[1];
     p.ld = q.ld;
@@ -1168,6 +1185,7 @@ int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res
     p.steps = steps;
     p.segments = segments;
     p.factors = factors;
+    p.failed = res.failed;
     p.x[0] = x.part[0];
     p.x[1] = x.part[1];
     p.ld = x.ld;
@@ -1182,19 +1200,20 @@ int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res
 
 // O(U) to the result.
 template <int OUT>
-int orthogonalize(const Source& s, int steps, float eps, const Result& res, cudaStream_t st) {
+int orthogonalize(const Source& s, int steps, float eps, Result res, cudaStream_t st) {
     const bool tall = s.r > s.d;
     const long long k = std::min(s.r, s.d), ldx = up(s.d, 8), ldk = up(k, 8);
     const size_t x_bytes = up(2ll * s.r * ldx, 256), k_bytes = up(2ll * k * ldk, 256);
     const int segments = (steps + kSegment - 1) / kSegment;
     void* base = nullptr;
-    const size_t partial_bytes = up(sizeof(double) * kNormBlocks, 256), factor_bytes = up(sizeof(Factors) * kMostSegments, 256);
+    const size_t partial_bytes = up(sizeof(double) * kNormBlocks, 256), factor_bytes = up(sizeof(Factors) * kMostSegments + sizeof(int), 256);
     int rc = scratch_alloc(&base, partial_bytes + factor_bytes + (segments > 1 ? 4 : 2) * x_bytes + 12 * k_bytes, st);
     if (rc) return rc;
     char* at = static_cast<char*>(base);
     double* partial = reinterpret_cast<double*>(at);
     at += partial_bytes;
     Factors* factors = reinterpret_cast<Factors*>(at);
+    int* failed = res.failed = reinterpret_cast<int*>(factors + kMostSegments);
     at += factor_bytes;
     auto matrix = [&](long long rows, long long cols, long long ld, size_t bytes, int exp) {
         Matrix x{{reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + bytes)}, rows, cols, ld, exp};
@@ -1212,7 +1231,7 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
     norm_kernel<<<blocks, 256, 0, st>>>(s, partial);
     rc = check_launch("norm_kernel");
     if (!rc) {
-        const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx, factors, segments);
+        const cudaError_t e = launch_pdl(scale_kernel, dim3(blocks), dim3(256), 0, st, s, partial, static_cast<int>(blocks), eps, x.part[0], x.part[1], ldx, factors, failed, segments);
         rc = e == cudaSuccess ? check_launch("scale_kernel") : cuda_fail(e, "scale_kernel launch");
     }
     const bool small = k <= 128;
@@ -1224,20 +1243,20 @@ int orthogonalize(const Source& s, int steps, float eps, const Result& res, cuda
     for (int seg = 0; seg < segments && !rc; ++seg) {
         const int n = steps * (seg + 1) / segments - steps * seg / segments;
         const float* gram = &factors[seg].gram;
-        rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st, gram) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st, gram);
+        rc = tall ? symmetric<true>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, failed, st, gram) : symmetric<false>(x, x, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, failed, st, gram);
         Matrix q = P[0];
         if (!rc && small) {
             if (n > 1) q = Q[0];
-            rc = core(A, q, n, st);
+            rc = core(A, q, n, failed, st);
         }
         for (int i = 0; i < n && !rc && !small; ++i) {
             const Matrix& p = P[i & 1];
-            rc = symmetric<false>(A, A, p, kC, &A, kB, kA, nullptr, nullptr, st);
+            rc = symmetric<false>(A, A, p, kC, &A, kB, kA, nullptr, nullptr, failed, st);
             const Matrix& next = Q[i & 1];
             const bool last = i == n - 1;
-            if (!rc && !last) rc = i ? symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, &q, &next, st) : symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
-            if (!rc && !last) rc = symmetric<false>(p, T, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
-            if (!rc && last && i) rc = symmetric<false>(p, q, next, 1.0f, nullptr, 0, 0, nullptr, nullptr, st);
+            if (!rc && !last) rc = i ? symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, &q, &next, failed, st) : symmetric<false>(p, A, T, 1.0f, nullptr, 0, 0, nullptr, nullptr, failed, st);
+            if (!rc && !last) rc = symmetric<false>(p, T, A, 1.0f, nullptr, 0, 0, nullptr, nullptr, failed, st);
+            if (!rc && last && i) rc = symmetric<false>(p, q, next, 1.0f, nullptr, 0, 0, nullptr, nullptr, failed, st);
             if (i) q = next;
         }
         if (rc) break;

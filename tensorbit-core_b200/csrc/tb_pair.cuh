@@ -45,6 +45,26 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
     return false;
 }
 
+// Tells the roles of both CTAs that one of them has given up.
+__device__ __forceinline__ void abort_pair(volatile int* abort_flag) {
+    *abort_flag = 1;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.u32 [a], %1;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 1;\n\tst.shared::cluster.u32 [a], %1;\n\t}" ::"r"(smem_u32(const_cast<int*>(abort_flag))), "r"(1)
+        : "memory");
+}
+// The issuing thread's way out: its MMAs are done when this returns, so that TMEM and their operands' places may be given
+// back.  `bar` is for this alone: one that results wait for would pass an unfinished sum off as a finished one.
+__device__ __forceinline__ void drain_pair(uint32_t bar) {
+    commit_pair(bar);
+    wait(bar, 0, nullptr);
+}
+__device__ __forceinline__ void drain_one(uint32_t bar) {
+    mma_commit(bar);
+    wait(bar, 0, nullptr);
+}
+
 // (An explicit .release.cluster here cost about 0.4 us per slice: 1235 against
 // 675 us for the 7000 x 4096 x 14336 forward.)
 __device__ __forceinline__ void arrive_even(uint32_t bar) {

@@ -18,8 +18,9 @@
 //   finish(L, w, acc, buf, row, half, lane)
 //   error()        where an expired wait is recorded
 // `acc` is columns 128 half .. of the tile's row `row` + lane; `buf` is 4 KB of
-// shared memory of the warp's own.  Every wait is bounded; on expiry
-// the kernel records an error and leaves.
+// shared memory of the warp's own.  Every wait is bounded; on expiry the kernel
+// records an error, there and in the word p.failed of its call, and leaves: only
+// finished sums reach finish(), and what writes a call's results looks at that word.
 #pragma once
 
 #include <algorithm>
@@ -91,7 +92,8 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
     uint64_t* empty = ready + kStages;                                // slice read by the MMAs
     uint64_t* accfull = empty + kStages;                              // [2] sum finished
     uint64_t* accempty = accfull + 2;                                 // [2] (even CTA) sum taken by both CTAs
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    uint64_t* drained = accempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
@@ -112,6 +114,7 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
             mbar_init(smem_u32(&accfull[b]), 1);
             mbar_init(smem_u32(&accempty[b]), 16);
         }
+        mbar_init(smem_u32(drained), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -125,6 +128,11 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
     const uint32_t tmem = *tmem_slot;
     pdl_wait();  // nothing above touched memory that an earlier kernel writes
     const int items = OP::items(L.p);
+    auto gave_up = [&] {
+        abort_pair(abort_flag);
+        atomicExch(OP::error(), 1);
+        atomicExch(L.p.failed, 1);
+    };
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -149,10 +157,7 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
             if (ok) OP::finish(L, w, acc, buf, rank * 128 + quad * 32, half, lane);
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        if (!ok) {
-            *abort_flag = 1;
-            atomicExch(OP::error(), 1);
-        }
+        if (!ok) gave_up();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == kLoadWarp && lane == 0) {
@@ -187,8 +192,7 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
                 }
             }
             if (!ok) {
-                *abort_flag = 1;
-                atomicExch(OP::error(), 1);
+                gave_up();
                 // Loads in flight, each stage's last phase waited for within a limit (the odd CTA's count on the
                 // even one's barrier).  A stage never used answers at once.
                 for (int i = 0; i < kStages && rank == 0; ++i)
@@ -234,15 +238,13 @@ product_kernel(const __grid_constant__ Launch<OP> L) {
                         }
                         commit_pair(empty0 + 8 * at.s);
                     }
+                    if (!ok) break;
                     commit_pair(smem_u32(&accfull[ac.s]));
                     ac.next();
                 }
             }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(OP::error(), 1);
-                for (int b = 0; b < 2; ++b) commit_pair(smem_u32(&accfull[b]));  // releases the waiting epilogues
-            }
+            if (!ok) gave_up();
+            if (*abort_flag) drain_pair(smem_u32(drained));
         }
         __syncwarp();
     }

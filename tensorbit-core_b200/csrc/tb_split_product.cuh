@@ -50,6 +50,16 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t addr, uint32_t rank) {
         : "memory");
     return v;
 }
+__device__ __forceinline__ int load_cluster_int(uint32_t addr, uint32_t rank) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\t"
+        "ld.shared::cluster.u32 %0, [a];\n\t}"
+        : "=r"(v)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
@@ -63,7 +73,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
     uint64_t* empty = ready + kStages;
     uint64_t* accfull = empty + kStages;  // [2]
     uint64_t* accempty = accfull + 2;     // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    uint64_t* drained = accempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
@@ -84,6 +95,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
             mbar_init(smem_u32(&accfull[b]), 1);
             mbar_init(smem_u32(&accempty[b]), 4);
         }
+        mbar_init(smem_u32(drained), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -100,6 +112,12 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
     w.k0 = first;
     w.slices = share_at(all, rank + 1, ctas) - first;
     pdl_wait();  // nothing above touched memory that an earlier kernel writes
+
+    auto gave_up = [&] {
+        *abort_flag = 1;
+        atomicExch(OP::error(), 1);
+        atomicExch(L.p.failed, 1);
+    };
 
     float* sums = reinterpret_cast<float*>(smem);
     if (warp < 4) {
@@ -131,8 +149,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
 #pragma unroll
             for (int i = 0; i < 128; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         } else {
-            *abort_flag = 1;
-            atomicExch(OP::error(), 1);
+            gave_up();
         }
     } else if (warp == 4) {
         if (lane == 0) {
@@ -164,8 +181,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
                 }
             }
             if (!ok) {
-                *abort_flag = 1;
-                atomicExch(OP::error(), 1);
+                gave_up();
                 for (int i = 0; i < kStages; ++i)  // loads in flight, within a limit
                     if (i < at.s || at.phase) wait(smem_u32(&ready[i]), i < at.s ? at.phase : at.phase ^ 1, nullptr);
             }
@@ -209,14 +225,12 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
                     }
                     mma_commit(empty0 + 8 * at.s);
                 }
+                if (!ok) break;
                 mma_commit(smem_u32(&accfull[ac.s]));
                 ac.next();
             }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(OP::error(), 1);
-                for (int b = 0; b < 2; ++b) mma_commit(smem_u32(&accfull[b]));  // releases the waiting epilogues
-            }
+            if (!ok) gave_up();
+            if (*abort_flag) drain_one(smem_u32(drained));
         }
         __syncwarp();
     }
@@ -230,7 +244,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
         __syncthreads();
     }
     uint32_t* words = reinterpret_cast<uint32_t*>(sums + 128 * kSplitPitch);
-    if (!*abort_flag) {
+    // A CTA that gave up has no sums: a lane has another CTA's word, looked at when that CTA's sums are here too.
+    int gone = *abort_flag;
+    if (lane < ctas && lane != rank) gone = load_cluster_int(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(lane));
+    {
         constexpr int kBatch = 2;  // quads of a thread whose loads are under way together
         for (int i0 = threadIdx.x; i0 < rows * 32; i0 += kBatch * kSplitThreads) {
             float4 v[kBatch][kSplitMost];
@@ -248,6 +265,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
                         if (q < ctas) v[b][q] = load_cluster4(smem_u32(at), static_cast<uint32_t>(q));
                 }
             }
+            if (__any_sync(~0u, gone)) break;
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int i = i0 + b * kSplitThreads;
@@ -263,10 +281,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_product_kernel(const _
             }
         }
     }
+    const bool whole = !__any_sync(~0u, gone);
     if (ctas > 1) cluster_arrive();  // (what the others read here has been read once all have arrived)
     if constexpr (OP::kMirror) {
         __syncthreads();
-        if (!*abort_flag) OP::mirror(L, w, words, kSplitPitch, w.tm * 128 + row, rows, static_cast<int>(threadIdx.x));
+        if (whole) OP::mirror(L, w, words, kSplitPitch, w.tm * 128 + row, rows, static_cast<int>(threadIdx.x));
     }
     if (ctas > 1) cluster_wait();
     __syncthreads();
