@@ -599,7 +599,7 @@ struct Apply {
 };
 
 // ---- short sides up to 128 -----------------------------------------------------------------
-// All of the iteration in one launch, by a cluster of up to 8 CTAs that share the long side out.
+// All of the iteration in one launch, by a cluster of up to 4 CTAs that share the long side out, up to two chunks of 128 each.
 // Each sums its part of A; the cluster's CTAs add up a share of A's rows each, through distributed shared memory,
 // and copy the others'; then each forms Q by itself, and its own part of Q X.
 //
@@ -608,9 +608,10 @@ struct Apply {
 // four tiles of 64 columns x 128 rows (hi, hi, lo, lo) in the places of P and Q, which are not needed then.  The same
 // tile in memory is an operand along its rows and one along its columns.
 // (128 x 128, whole call: 56 us, of which a product of the chain takes 1.65; as eight launches 79.  16 x 512: 61 and 66; 128 x 1024: 80
-// and 81; 128 x 2048: 89 and 83.)  With `core` the kernel forms Q from A alone: longer sides are better shared out over all SMs.
+// and 81; 128 x 2048: 89 and 83.)  With `core` the kernel forms Q from A alone: of longer sides
+// A comes from clusters of 8, and Q X is shared out over all SMs.
 constexpr int kShortThreads = 512, kShortMatrix = 65536, kShortTile = 16384;  // thread 0 also loads and issues MMAs
-constexpr int kShortChunks = 8;  // of 128: the most that the whole iteration is done here with
+constexpr int kShortChunks = 8, kShortCtas = 4;  // the most that the whole iteration is done here with, two chunks a CTA
 constexpr size_t kShortSmem = 3 * kShortMatrix + 1024 + 128;
 struct ShortMaps {
     CUtensorMap x[2];  // X's parts, or A's
@@ -806,13 +807,13 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
                     const int b = i & 1;
                     if (i + 1 < own) load_chunk(i + 1, b ^ 1);
                     if (!chunk_ready(b)) break;
-                    // (two accumulators, so that no sum has more than half of the chunks)
+                    // (an accumulator for each chunk)
                     for (int s = 0; s < (p.tall || 64 < p.d - 128 * (first + i) ? 2 : 1); ++s)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             const uint64_t x = p.tall ? tile_desc(buffer(1 + b), true) + (4 * s + kk) * 128 : tile_desc(buffer(1 + b) + s * kShortTile, false) + 2 * kk;
                             const uint32_t idesc = kIdesc | kN128 | (p.tall ? kAlongM | kAlongN : 0u);
-                            mma_one16<true>(tmem + 128 * b, x + kLoChunk, x, idesc, i >= 2 || s || kk);
+                            mma_one16<true>(tmem + 128 * b, x + kLoChunk, x, idesc, s || kk);
                             mma_one16<true>(tmem + 128 * b, x, x + kLoChunk, idesc, 1);
                             mma_one16<true>(tmem + 128 * b, x, x, idesc, 1);
                         }
@@ -853,12 +854,12 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
                 const int row0 = 2 * share_at(64, rank, ctas), rows = 2 * share_at(64, rank + 1, ctas) - row0;
                 for (int i = threadIdx.x; i < rows * 32; i += kShortThreads) {
                     const int r = row0 + (i >> 5), c = 4 * (i & 31);
-                    float4 v[kSplitMost];
+                    float4 v[kShortCtas];
 #pragma unroll
-                    for (int q = 0; q < kSplitMost; ++q)
+                    for (int q = 0; q < kShortCtas; ++q)
                         if (q < ctas) v[q] = load_cluster4(smem_u32(sums + r * kSplitPitch + c), static_cast<uint32_t>(q));
 #pragma unroll
-                    for (int q = 1; q < kSplitMost; ++q)
+                    for (int q = 1; q < kShortCtas; ++q)
                         if (q < ctas) { v[0].x += v[q].x; v[0].y += v[q].y; v[0].z += v[q].z; v[0].w += v[q].w; }
                     uint2 h, l;
                     split16x2(v[0].x * gram, v[0].y * gram, h.x, l.x);
@@ -968,7 +969,6 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
             const int b = i & 1, at = 128 * (first + i);
             if (issuer && i + 1 < own) {
                 multiply(i + 1);
-                if (i + 2 < own) load_chunk(i + 2, b);
             }
             __syncwarp();
             finished(b);
@@ -1195,7 +1195,7 @@ int whole(const Matrix& x, bool tall, int steps, int segments, const Result& res
     p.w_bf16 = res.w_bf16;
     p.decay = res.decay;
     p.step = res.step;
-    return launch_short<OUT>(maps, p, std::min(kSplitMost, (p.chunks + 1) / 2), st);
+    return launch_short<OUT>(maps, p, (p.chunks + 1) / 2, st);
 }
 
 // O(U) to the result.
