@@ -200,8 +200,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
     }
 }
 
-// tanh of each of v / c, in place: the odd polynomial of degree 9 nearest to it up to 1/2 (1.4e-8 of the value; fitted at
-// Chebyshev points in 64 bits) where all of the lane's neighbours' values lie there, which takes a quarter of tanhf's time.
+// tanh of each of v / c, in place: an odd polynomial of degree 9 up to 1/2 (2.6e-8 of the value, 8.4e-8 as FP32 evaluates it;
+// fitted at Chebyshev points in 64 bits) where all of the warp's values lie there, which takes a quarter of tanhf's time.  Where
+// some do not, looking costs its share.  (Loss of 8000 tokens, 512 features, 32000 entries: small logits 273 us, 373 by tanhf
+// alone; logits of the cap's order 449 and 390.  2048 tokens, 4096 features, behind whose products most of it hides: 363 and 385; 487 and 493.)
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
     uint64_t v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
