@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_logits_kernel(const __grid
             if (p.cap > 0.0f) {
                 const float inverse = inverse_cap(p.cap);
 #pragma unroll
-                for (int c = 0; c < NT; c += 16) tanh_of<16>(z + c, inverse);
+                for (int i = 0; i < NT; ++i) z[i] = tanhf(z[i] * inverse);  // (not as what other tokens hold decides: some may be left out)
             }
             if constexpr (GRAD) {
 #pragma unroll

@@ -120,3 +120,23 @@ def test_smallest_and_largest_caps(cuda, n, cap):
     # G's rounding, the result's, and 32 steps of the tensor core's sum
     assert ((dh[::2].double() - rows).abs() <= size * (2.0 ** -8 + 40 * 2.0 ** -23) + rows.abs() * 2.0 ** -8 * 1.01).all()
     assert torch.isfinite(dw).all() and torch.isfinite(dh).all()
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_left_out_rows_change_no_bit(cuda, n, cap):
+    """Tokens left out hold zeros, then values whose logits are far beyond the cap, then NaN."""
+    d, vocab = 256, 700
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = (torch.randn(vocab, d, device="cuda", generator=g) * 0.1).to(BF)
+    h = torch.randn(n, d, device="cuda", generator=g).to(BF)
+    target = torch.randint(0, vocab, (n,), device="cuda", generator=g)
+    target[::3] = -100
+    got = []
+    for size in (0.0, 300.0, float("nan")):
+        h[::3] = (torch.randn(len(h[::3]), d, device="cuda", generator=g) * size).to(BF)
+        dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+        got.append((*call(h, w, target, cap, torch.ones(n, device="cuda"), dh, dw), dh, dw))
+    for other in got[1:]:
+        for x, y in zip(got[0], other):
+            assert torch.equal(x, y)
