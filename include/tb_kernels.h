@@ -430,7 +430,8 @@ typedef struct tb_lm_loss_args {
  * rounding: 7e-7 of the loss (2-norm) at 4096 features, as with FP32 products.
  * A loss is never below zero: exponentials are of exact differences from the largest logit.
  * Scratch from the library's per-device pool: 2 bytes per value of h, and 16 bytes
- * per token and 256 entries. */
+ * per token and 256 entries; up to 128 tokens at most 144 KB more than 16 bytes for each
+ * of them and 256 entries. */
 int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
 /* Gradients of sum_t dloss_t loss_t + dlse_t lse_t, with lse from the forward on the
  * same h, w and targets:
@@ -440,10 +441,10 @@ int tb_lm_loss(const tb_lm_loss_args* args, void* stream);
  * The vocabulary is gone through in pieces whose g enters both products as BF16
  * (2^-8 of each value).  dh and dw overwrite what is there; each sum has a fixed
  * order.  dh may be h's own memory, with its stride.  n = 0 gives a dw of zeros.
- * Scratch: 2 bytes per value of h, up to 128 MB of g (more beyond 2^18 tokens), 4
- * bytes per value of dh, up to 32 times that where its 256 x 256 tiles leave much of
- * the GPU's last wave idle, and for dw at most 74 such tiles in FP32 where it has
- * fewer than half as many. */
+ * Scratch, tokens rounded up to 256: 2 bytes per value of h, up to 128 MB of g (more
+ * beyond 2^18 tokens), 4 bytes per value of dh, up to 32 times that where its 256 x 256
+ * tiles leave much of the GPU's last wave idle, and for dw at most 74 such tiles in FP32
+ * where it has fewer than half as many. */
 int tb_lm_loss_backward(const tb_lm_loss_args* args, void* stream);
 
 /* ---- orthogonalised updates ------------------------------------------------ */
