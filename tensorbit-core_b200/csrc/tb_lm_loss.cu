@@ -178,8 +178,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, const Scratch
                 if (BACKWARD) {
                     r.lse = a.lse[t];
                     const float dl = a.dloss[t];
-                    r.dloss = dl == unit ? 1.0f : dl * inverse;
-                    r.both = a.dlse ? fmaf(a.dlse[t], inverse, r.dloss) : r.dloss;
+                    auto scaled = [&](float x) { return x == unit ? 1.0f : x * inverse; };
+                    r.dloss = scaled(dl);
+                    r.both = a.dlse ? scaled(dl + a.dlse[t]) : r.dloss;  // (the sum first: it is exact where the two nearly cancel)
                 }
                 s.row[to] = r;
             }

@@ -4,12 +4,13 @@ import pytest
 import torch
 
 import tbabi as tb
+from lm_loss_ref import assert_within, reference
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
 
-def call(h, w, target, cap=0.0, dloss=None, dh=None, dw=None):
+def call(h, w, target, cap=0.0, dloss=None, dh=None, dw=None, dlse=None):
     n, d = h.shape
     loss, lse = torch.full((n,), 7.0, device="cuda"), torch.full((n,), 7.0, device="cuda")
     args = tb.lm_loss_args(n=n, d=d, vocab=w.shape[0], h=h.data_ptr(), ldh=h.stride(0), w=w.data_ptr(), ldw=w.stride(0), target=target.data_ptr(),
@@ -17,6 +18,7 @@ def call(h, w, target, cap=0.0, dloss=None, dh=None, dw=None):
     stream = torch.cuda.current_stream().cuda_stream
     tb.check(tb.lm_loss(args, stream=stream))
     if dloss is not None:
+        args.dlse = None if dlse is None else dlse.data_ptr()
         args.dloss, args.dh, args.lddh, args.dw, args.lddw = dloss.data_ptr(), dh.data_ptr(), dh.stride(0), dw.data_ptr(), dw.stride(0)
         tb.check(tb.lm_loss_backward(args, stream=stream))
     tb.check(tb.call("tb_gemm_status", stream))
@@ -140,3 +142,20 @@ def test_left_out_rows_change_no_bit(cuda, n, cap):
     for other in got[1:]:
         for x, y in zip(got[0], other):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n", [40, 300])
+def test_factors_that_nearly_cancel(cuda, n):
+    """dloss + dlse is a small difference: for all entries but the target it alone counts."""
+    d, vocab = 64, 500
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(vocab, d, device="cuda", generator=g).to(BF)
+    h = (torch.randn(n, d, device="cuda", generator=g) * 0.2).to(BF)
+    target = torch.randint(0, vocab // 2, (n,), device="cuda", generator=g)  # (the other half of dw is of the differences alone)
+    dloss = torch.rand(n, device="cuda", generator=g) + 0.1
+    dlse = -dloss * (1 + 2.0 ** -16 * torch.rand(n, device="cuda", generator=g))
+    dh, dw = torch.empty(n, d, device="cuda", dtype=BF), torch.empty(vocab, d, device="cuda", dtype=BF)
+    call(h, w, target, 0.0, dloss, dh, dw, dlse)
+    ref = reference(h, w, target, 0.0, dloss, dlse)
+    assert_within(dh, ref, "dh")
+    assert_within(dw, ref, "dw")
