@@ -542,7 +542,7 @@ int launch_small(const char* what, void (*kernel)(P...), long long blocks, cudaS
 // vocabulary and all tokens.  Sums of 64 terms in the tensor core, which costs nothing here, added in one order in both
 // directions: p is of the difference of the backward's logits and the forward's lse.  (The backward from the last features on, which
 // L2 still has, is 3 % sooner for 37 tokens, 4096 x 32000, with gradients, but adds in another order: 3e-5 of a logit of 60.)
-// (32000 x 4096, whole calls: 52 us for 1 token, 56 for 37, 68 for 128, by tiles of 256 tokens 70; w at the measured
+// (32000 x 4096, whole calls: 53 us for 1 token, 54 for 37, 64 for 128, by tiles of 256 tokens 70; w at the measured
 // copy rate 41.  128000 x 4096, 8 tokens: 167, at that rate 162.)
 constexpr int kFewMost = 128;
 constexpr int kFewThreads = 320;  // warps 0-7 results, 8 loads, 9 MMAs
